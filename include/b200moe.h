@@ -20,7 +20,7 @@
  * calls that share a workspace must be ordered (same stream, or joined by
  * events); two calls running at once on one workspace race.
  *
- * Dtype codes: 0 = bf16, 1 = f16, 2 = f32.
+ * Dtype codes: 0 = bf16, 1 = f16, 2 = f32, 3 = e4m3.
  *
  * Reference interfaces replaced are cited as path:line inside the
  * sglang-restomod source tree.
@@ -43,6 +43,7 @@ extern "C" {
 #define B200_DTYPE_BF16 0
 #define B200_DTYPE_F16 1
 #define B200_DTYPE_F32 2
+#define B200_DTYPE_E4M3 3 /* key/value caches only */
 
 #define B200_QUANT_FP8_BLOCK 0 /* e4m3 weights, fp32 scales per 128x128 block */
 #define B200_QUANT_NVFP4 1     /* e2m1 weights, e4m3 scales per 16 K, fp32 global */
@@ -63,8 +64,8 @@ int b200_num_sms(void);
 /*
  * Device-side error bits recorded in a workspace (1 = a pipeline wait timed
  * out, 2 = an expert id >= E reached a GEMM, 4 = a route pointed past the
- * activation rows) or an expert-parallel region (8 = a wait on another rank
- * timed out). Synchronizes `stream`; clears the bits when reset != 0.
+ * activation rows, 16 = a page number outside the key/value cache) or an
+ * expert-parallel region (8 = a wait on another rank timed out). Synchronizes `stream`; clears the bits when reset != 0.
  */
 int b200_workspace_status(void* workspace, int32_t* bits, int32_t reset, void* stream);
 
@@ -412,6 +413,16 @@ int b200_w8a8_linear(const void* x, int32_t x_dtype, int64_t m, int64_t k, const
                      const float* w_scales, int64_t n, int32_t gated_mode, void* y,
                      int32_t y_dtype, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* b200_w8a8_linear on activations that are already quantized: q [m, k] e4m3
+ * and scales [k / 128][scales_ld] as b200_fp8_act_quant or b200_add_rms_norm
+ * write them, scales_ld a multiple of 4 and at least m rounded up to 128 (the
+ * entries past row m are copied, not used), q and scales 16-byte aligned.
+ * Workspace: b200_gemm_workspace_bytes(0). */
+int b200_w8a8_linear_quantized(const uint8_t* q, const float* scales, int64_t scales_ld, int64_t m,
+                               int64_t k, const uint8_t* w_e4m3, const float* w_scales, int64_t n,
+                               int32_t gated_mode, void* y, int32_t y_dtype, void* workspace,
+                               int64_t workspace_bytes, void* stream);
+
 /* Grouped expert GEMM with the routing of b200_moe_gemm
  * (moe_wna16_marlin_gemm semantics: slot p of block b multiplies activation
  * row sorted_token_ids[p] / top_k by expert expert_ids[b] and writes output
@@ -427,6 +438,104 @@ int b200_w8a8_moe_gemm(const void* a, int32_t a_dtype, int64_t a_rows, int64_t k
                        int64_t num_routes, const float* topk_weights, int32_t mul_topk_weights,
                        void* c, int32_t c_dtype, int64_t ldc, void* workspace,
                        int64_t workspace_bytes, void* stream);
+
+/* ------------------------------- norm, key/value cache, paged attention */
+
+/*
+ * Residual-add RMS norm (no counterpart among the reference's kernels, which
+ * leave norms to upstream SGLang): per row of `hidden` columns
+ *   h = x + residual                (fp32; residual NULL: h = x)
+ *   residual_out = h                (NULL: not written)
+ *   y = h * rsqrt(mean(h^2) + eps) * (weight + weight_bias)
+ * stored as y (type of x; NULL: not wanted) and / or quantized from the fp32 y
+ * as b200_fp8_act_quant does: q [rows, hidden] e4m3 (contiguous), scales
+ * [hidden / 128][scales_ld] fp32, scale = max(amax / 448, 1e-8) per (row, 128
+ * columns); a group with a NaN has a NaN scale. weight: bf16, f16 or f32;
+ * weight_bias 1 for weights stored as offsets from one. Leading dimensions in
+ * elements, multiples of 8; 0 repeats one row of x or residual. residual_out
+ * and y may be x or residual themselves (same leading dimension), and may not
+ * overlap them otherwise. hidden % 8 == 0 (% 128 with q), hidden <= 32768.
+ */
+int b200_add_rms_norm(const void* x, int32_t dtype, int64_t x_ld, int64_t rows, int64_t hidden,
+                      const void* residual, int64_t residual_ld, const void* weight,
+                      int32_t weight_dtype, float weight_bias, float eps, void* residual_out,
+                      int64_t residual_out_ld, void* y, int64_t y_ld, uint8_t* q, float* scales,
+                      int64_t scales_ld, void* stream);
+
+/*
+ * A paged key/value cache, owned by the caller. Element i of the vector of
+ * (page, offset, head) lies at page * page_stride + offset * token_stride +
+ * head * head_stride + i in k and in v (elements of `dtype`), so pages may be
+ * stored token-major or head-major. dtype B200_DTYPE_E4M3: each vector of
+ * head_dim codes has one power-of-two scale, byte b = 2^(b - 127) (255: NaN),
+ * at the scale strides of k_scale / v_scale; a code stands for code * scale.
+ * Otherwise bf16 or f16 and no scales (NULL). head_dim 64, 128 or 256; every
+ * vector 16-byte aligned; num_pages * page_size < 2^31. Slot s = page s /
+ * page_size, offset s % page_size.
+ */
+typedef struct b200_kv_cache {
+  void* k;
+  void* v;
+  uint8_t* k_scale;
+  uint8_t* v_scale;
+  int64_t num_pages;
+  int32_t page_size;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t dtype;
+  int64_t page_stride, token_stride, head_stride;
+  int64_t scale_page_stride, scale_token_stride, scale_head_stride;
+} b200_kv_cache;
+
+/*
+ * Writes the keys and values of `tokens` tokens (bf16 / f16, [tokens,
+ * kv_heads, head_dim] at the given strides, in elements) into their slots,
+ * quantized when the cache is e4m3: the scale is the smallest power of two 2^e,
+ * e in [-24, 7], with max|x| <= 448 * 2^e (magnitudes above 57344 saturate); a
+ * vector holding an infinity or NaN reads back as NaN. Slots outside the cache
+ * (-1: a padding token) are skipped; of two tokens with one slot either may win.
+ */
+int b200_kv_cache_write(const b200_kv_cache* cache, const void* k, const void* v, int32_t dtype,
+                        int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride,
+                        int64_t v_head_stride, const int64_t* slots, int64_t tokens, void* stream);
+
+/* The reverse: the values of the given slots as bf16 / f16 (zeros for slots
+ * outside the cache), k and v with the same strides. */
+int b200_kv_cache_read(const b200_kv_cache* cache, const int64_t* slots, int64_t tokens, void* k,
+                       void* v, int32_t dtype, int64_t token_stride, int64_t head_stride,
+                       void* stream);
+
+/*
+ * Attention of new tokens over the paged cache. Sequence s has kv_lens[s]
+ * cached tokens (its own new ones, written before, included), whose pages are
+ * page_table[s * page_table_stride ..], page_table_width entries; its
+ * q_starts[s + 1] - q_starts[s] new tokens are rows q_starts[s].. of q
+ * [q_tokens, q_heads, head_dim] and sit at its last positions. q_starts[0 ..
+ * seqs] ascends within [0, q_tokens]. Query head h reads key/value head
+ * h / (q_heads / kv_heads).
+ *   out = softmax(scale * q . k) v over the tokens a row sees,
+ *   lse = ln(sum e^(scale * q . k))  (fp32 [q_tokens, q_heads]; NULL: not wanted)
+ * causal: position p sees positions <= p, and with window > 0 only the last
+ * `window` of them; not causal: all cached tokens. A row that sees nothing
+ * gets zeros and lse = -inf. max_q_len bounds the new tokens of any sequence
+ * (1: decode); further ones would be left unwritten. Page numbers outside the
+ * cache read as zeros and set status bit 16. Cached values past kv_lens are
+ * never read. The cache is e4m3, or of q's type. q and out: vectors 16-byte
+ * aligned, strides in elements. No host synchronization, and no host knowledge
+ * of the lengths: one captured call serves any contents of kv_lens, q_starts
+ * and page_table. Sums and softmax statistics are fp32; P is rounded to 16
+ * bits before it multiplies the values. Workspace: zero-filled before first
+ * use; it may be the one the GEMM calls use.
+ */
+int64_t b200_paged_attention_workspace_bytes(int32_t head_dim, int64_t q_tokens, int32_t seqs);
+int b200_paged_attention(const b200_kv_cache* cache, const void* q, int32_t dtype, int64_t q_tokens,
+                         int32_t q_heads, int64_t q_token_stride, int64_t q_head_stride,
+                         const int32_t* page_table, int64_t page_table_stride,
+                         int32_t page_table_width, const int32_t* kv_lens, const int32_t* q_starts,
+                         int32_t seqs, int32_t max_q_len, float scale, int32_t causal,
+                         int32_t window, void* out, int64_t out_token_stride,
+                         int64_t out_head_stride, float* lse, void* workspace,
+                         int64_t workspace_bytes, void* stream);
 
 /* ---------------------------------------- expert parallelism (peer memory) */
 

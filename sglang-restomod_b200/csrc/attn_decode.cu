@@ -1,0 +1,909 @@
+// Attention of a few new tokens per sequence over the paged cache (decode):
+// one pass over the cached keys and values, split evenly over the whole GPU.
+//
+//   s = scale * q . k,  m = max s,  l = sum e^(s - m),
+//   out = sum e^(s - m) v / l,  lse = m + ln l
+//
+// Rows of a sequence and key/value head: its new tokens x the query heads
+// that share the head, up to 16 (two groups of 8).
+//
+// Bound: HBM, each cached vector is read once. 2 B (e4m3: 1 B + 1/head_dim)
+// per cached element against 2 rows' multiply-adds per element, far below the
+// tensor rate, so the work is to keep enough loads in flight:
+//
+// * The sequences' key ranges, in tiles of 64 tokens, are laid end to end over
+//   (sequence, head, tile) and cut into equal ranges, one per block, so uneven
+//   lengths leave no block idle. A block finds its range from kv_lens itself
+//   (no host knowledge of the lengths, no planning launch). A (sequence, head)
+//   cut by a range border leaves partial (O, m, l) in the scratch; the last
+//   block to arrive at the pair's counter adds them in block order, so the
+//   result does not depend on which block that is.
+// * Each warp streams its own 16 of a tile's 64 tokens through a private ring
+//   of cp.async stages: no block barrier inside a pair, and the ring runs on
+//   into the next pair while the present one is finished. Page numbers travel
+//   through the same ring one ring length ahead, so no load waits on another.
+// * The products are taken transposed (S^T = K Q^T, O^T = V^T P^T): the
+//   m16n8k16 tile then has 16 cached tokens or 16 head columns in M and 8 rows
+//   in N, so 8 query heads per key/value head waste nothing. K is read as the
+//   A operand; V^T is ldmatrix.trans, or for e4m3 a byte interleave of two
+//   tokens that the conversion needs anyway.
+// * e4m3 codes are converted to f16 (exact) for every model type: bf16 queries
+//   are brought to f16 by a power of two per row (exact but for parts 2^-24
+//   below the row's largest), P is rounded to f16. The key's scale multiplies
+//   s in fp32; the value's multiplies P relative to the largest seen.
+// * The maximum is lazy: O and l are rescaled only when some s exceeds m by
+//   more than 2^8, so P stays below 2^8 and most tiles need no cross-lane
+//   reduction at all.
+#include "common.cuh"
+#include "internal.h"
+
+namespace b200 {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kTile = 64;           // tokens per block step
+constexpr int kWarpTokens = kTile / kWarps;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLazy = 8.f;        // log2 of the largest P before a rescale
+constexpr int kMaxCtas = 1024;      // arrival counters in the workspace
+// A block takes at least this many tiles: below it the pair's merge costs more
+// than the extra blocks bring.
+constexpr int kMinTiles = 2;
+
+struct DecodeParams {
+  AttnLaunch a;
+  int groups;          // query heads per key/value head
+  float scale_log2;
+  int page_shift;      // log2 of the page size, -1 where it is no power of two
+};
+
+enum { kBf16 = 0, kF16 = 1, kE4m3 = 2 };
+
+// One ring entry's description, written when its page numbers are requested.
+struct TileInfo {
+  int seq, head;   // seq < 0: past the block's range
+  int token0;      // first token of this warp's 16
+  int end;         // tokens from here on do not exist
+};
+
+template <int D, int KV, int NR>
+struct Shape {
+  static constexpr int kElem = KV == kE4m3 ? 1 : 2;
+  static constexpr int kRowBytes = D * kElem;
+  static constexpr int kStageBytes = 2 * kWarpTokens * kRowBytes;  // K then V of a warp
+  static constexpr int kRows = 8 * NR;
+  // Ring depth: 80 to 96 KB per block and two blocks per SM; head_dim 256, whose
+  // stages are 32 to 64 KB, takes one block per SM with 160 to 192 KB.
+  static constexpr int kBlocks = D == 256 ? 1 : 2;
+  static constexpr int kStages = KV == kE4m3 ? (D == 64 ? 10 : 5) : (D == 64 ? 5 : 3);
+  static constexpr int kAhead = kStages - 1;
+  static constexpr int kRing = 2 * kStages;  // page-number entries
+  static constexpr int kQPitch = D + 8;      // 16-bit elements, conflict-free rows
+  static constexpr int kMergePitch = D + 4;  // fp32
+  struct Smem {
+    uint8_t stage[kWarps][kStages][kStageBytes];
+    uint16_t q[kRows][kQPitch];
+    float merge[kRows][kMergePitch];
+    int pages[kWarps][kRing][kWarpTokens];
+    TileInfo info[kWarps][kRing];
+    float row_scale[kRows];
+    int row_lo[kRows], row_hi[kRows];
+    float wm[kWarps][kRows], wl[kWarps][kRows];
+    int wv[kWarps];
+    long long scan[kWarps];
+    int start_seq;
+    long long start_off;
+    int flag;
+  };
+};
+
+__device__ __forceinline__ void cp_async_16_zfill(void* dst, const void* src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src),
+               "r"(on ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 "
+      "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <int KV>
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                    uint32_t b1) {
+  if (KV == kBf16)
+    mma_bf16(d, a, b0, b1);
+  else
+    mma_16816(d, a, b0, b1);
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// 2^e for e in [-254, 0]; 0 below the normal range.
+__device__ __forceinline__ float pow2(int e) {
+  return e < -126 ? 0.f : __uint_as_float((uint32_t)(127 + e) << 23);
+}
+
+// Bytes of a warp's tile rows, 16-byte chunk `chunk` of token row `row`,
+// placed so that the operand reads below touch all banks evenly.
+template <int D, int KV, bool IS_V>
+__device__ __forceinline__ int chunk_at(int row, int chunk) {
+  constexpr int kChunks = Shape<D, KV, 1>::kRowBytes / 16;
+  int x;
+  if (KV != kE4m3)
+    x = row & 7;  // ldmatrix: 8 rows of one chunk column
+  else if (kChunks == 4)
+    x = (row >> 1) & 3;  // two rows fill the banks
+  else
+    x = IS_V ? (row & 6) : ((row & 1) << 2);
+  return (row * kChunks + (chunk ^ x)) * 16;
+}
+
+// The key range of a sequence: tokens [begin, end) some row may see, as tiles.
+// A sequence with new tokens always has one tile, so that its rows are written
+// even where nothing is cached.
+struct SeqRange {
+  int begin, end, q_len, kv_len, tiles;
+};
+__device__ __forceinline__ SeqRange seq_range(const AttnLaunch& a, int s) {
+  SeqRange r;
+  const int q0 = __ldg(a.q_starts + s), q1 = __ldg(a.q_starts + s + 1);
+  const long long cap = (long long)a.table_width * a.c.page_size;
+  int kv = __ldg(a.kv_lens + s);
+  kv = kv < 0 ? 0 : kv;
+  if (kv > cap) kv = (int)cap;
+  int ql = q1 - q0;
+  if (q0 < 0 || q1 > a.q_tokens) ql = 0;  // outside q: nothing is read or written
+  ql = ql < 0 ? 0 : (ql > a.max_q ? a.max_q : ql);
+  r.q_len = ql;
+  r.kv_len = kv;
+  r.end = kv;
+  r.begin = 0;
+  if (a.window > 0) {
+    const long long b = (long long)kv - ql - a.window + 1;  // first token the first row sees
+    r.begin = b > 0 ? (int)b : 0;
+  }
+  const int n = r.end - r.begin;
+  r.tiles = ql == 0 ? 0 : (n <= 0 ? 1 : (n + kTile - 1) / kTile);
+  return r;
+}
+
+template <int D, int KV, int NR>
+__global__ void __launch_bounds__(kThreads, Shape<D, KV, NR>::kBlocks) attn_decode_kernel(const DecodeParams p) {
+  using S = Shape<D, KV, NR>;
+  using Smem = typename S::Smem;
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
+  const AttnLaunch& a = p.a;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int g = lane >> 2, c = lane & 3;
+  const int heads = a.c.heads;
+  griddep_wait();
+
+  // ---- this block's range of the flattened (sequence, head, tile) space
+  long long total;
+  {
+    const int per = (a.seqs + kThreads - 1) / kThreads;
+    const int s0 = tid * per, s1 = min(s0 + per, a.seqs);
+    long long mine = 0;
+    for (int s = s0; s < s1; ++s) mine += (long long)seq_range(a, s).tiles * heads;
+    long long before = mine;  // inclusive scan, made exclusive below
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long v = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += v;
+    }
+    if (lane == 31) sm.scan[warp] = before;
+    __syncthreads();
+    before -= mine;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += sm.scan[w];
+      total += sm.scan[w];
+    }
+    if (total == 0) return;
+    long long ctas = (total + kMinTiles - 1) / kMinTiles;
+    if (ctas > gridDim.x) ctas = gridDim.x;
+    if (blockIdx.x >= ctas) return;
+    const long long t0 = total * blockIdx.x / ctas;
+    if (t0 >= before && t0 < before + mine) {
+      int s = s0;
+      for (;; ++s) {
+        const long long n = (long long)seq_range(a, s).tiles * heads;
+        if (t0 < before + n) break;
+        before += n;
+      }
+      sm.start_seq = s;
+      sm.start_off = t0 - before;
+    }
+    __syncthreads();
+  }
+  const int ctas = (int)min((long long)gridDim.x, (total + kMinTiles - 1) / kMinTiles);
+  const long long t0 = total * blockIdx.x / ctas;
+  const long long t1 = total * (blockIdx.x + 1) / ctas;
+
+  // ---- the request cursor: page numbers of the warp's next tile
+  int r_seq = sm.start_seq, r_head, r_tile;
+  SeqRange r_range = seq_range(a, r_seq);
+  r_head = (int)(sm.start_off / r_range.tiles);
+  r_tile = (int)(sm.start_off - (long long)r_head * r_range.tiles);
+  long long r_at = t0;
+  int r_slot = 0;
+  auto page_of = [&](int token) {
+    return p.page_shift >= 0 ? token >> p.page_shift : token / a.c.page_size;
+  };
+  // Requests one tile's page numbers into ring entry r_slot. `now`: by plain
+  // loads (the prologue), else asynchronously with the next group.
+  auto request = [&](bool now) {
+    TileInfo ti;
+    ti.seq = -1;
+    ti.head = r_head;
+    ti.token0 = 0;
+    ti.end = 0;
+    if (r_at < t1) {
+      ti.seq = r_seq;
+      ti.token0 = r_range.begin + r_tile * kTile + warp * kWarpTokens;
+      ti.end = r_range.end;
+      if (lane < kWarpTokens && ti.token0 + lane < ti.end) {
+        const int* src = a.table + r_seq * a.table_stride + page_of(ti.token0 + lane);
+        int* dst = &sm.pages[warp][r_slot][lane];
+        if (now)
+          *dst = __ldg(src);
+        else
+          cp_async_4(dst, src);
+      }
+      ++r_at;
+      if (++r_tile == r_range.tiles) {
+        r_tile = 0;
+        if (++r_head == heads) {
+          r_head = 0;
+          if (r_at < t1) {
+            do {
+              r_range = seq_range(a, ++r_seq);
+            } while (r_range.tiles == 0);
+          }
+        }
+      }
+    }
+    if (lane == 0) sm.info[warp][r_slot] = ti;
+    r_slot = r_slot + 1 == S::kRing ? 0 : r_slot + 1;
+  };
+
+  // Issues the copies of ring entry `slot` into stage `stage`.
+  auto issue = [&](int slot, int stage) {
+    const TileInfo ti = sm.info[warp][slot];
+    if (ti.seq >= 0) {
+      constexpr int kChunks = S::kRowBytes / 16;
+      uint8_t* ks = sm.stage[warp][stage];
+      uint8_t* vs = ks + kWarpTokens * S::kRowBytes;
+      const long long head_off = (long long)ti.head * a.c.head_stride;
+      // byte offset of token row lane & 15, or -1
+      long long mine = -1;
+      {
+        const int token = ti.token0 + (lane & 15);
+        if (token < ti.end) {
+          const int page = sm.pages[warp][slot][lane & 15];
+          const int at_page = token - page_of(token) * a.c.page_size;
+          if (page >= 0 && page < a.c.num_pages)
+            mine = (page * a.c.page_stride + at_page * a.c.token_stride + head_off) * S::kElem;
+          else
+            atomicOr(a.status, kDevBadPage);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kWarpTokens * kChunks / 32; ++i) {
+        const int id = i * 32 + lane;
+        const int row = id / kChunks, chunk = id % kChunks;
+        long long off = __shfl_sync(0xffffffffu, mine, row);
+        const bool on = off >= 0;
+        off = on ? off + chunk * 16 : 0;
+        cp_async_16_zfill(ks + chunk_at<D, KV, false>(row, chunk),
+                          static_cast<const uint8_t*>(a.c.k) + off, on);
+        cp_async_16_zfill(vs + chunk_at<D, KV, true>(row, chunk),
+                          static_cast<const uint8_t*>(a.c.v) + off, on);
+      }
+    }
+  };
+  // The scale byte of this lane's token in ring entry `slot`: keys in lanes
+  // 0-15, values in 16-31. 0 (2^-127, and codes of zero) for absent tokens.
+  auto scale_byte = [&](int slot) -> uint32_t {
+    if (KV != kE4m3) return 0;
+    const TileInfo ti = sm.info[warp][slot];
+    const int row = lane & 15, token = ti.token0 + row;
+    if (ti.seq < 0 || token >= ti.end) return 0;
+    const int page = sm.pages[warp][slot][row];
+    if (page < 0 || page >= a.c.num_pages) return 0;
+    const uint8_t* base = lane < 16 ? a.c.k_scale : a.c.v_scale;
+    return __ldg(base + page * a.c.scale_page_stride +
+                 (token - page_of(token) * a.c.page_size) * a.c.scale_token_stride +
+                 ti.head * a.c.scale_head_stride);
+  };
+
+  // ---- prologue
+  for (int i = 0; i < S::kAhead; ++i) request(true);
+  __syncwarp();
+  for (int i = 0; i < S::kAhead; ++i) {
+    issue(i, i);
+    request(false);
+    cp_async_commit();
+  }
+  uint32_t next_byte = scale_byte(0);
+
+  // ---- consume
+  float o[D / 16][NR][4];
+  float m[NR][2], l[NR][2];   // rows 8 nr + 2c, + 1
+  int v_exp = 1;              // e4m3: byte of the largest value scale so far
+  long long at = t0;
+  int slot = 0, stage = 0;
+  while (at < t1) {
+    // -- a (sequence, head) pair begins: its tiles of this block are
+    // [at, pair_end); u0, u1 bound the whole pair
+    cp_async_wait<S::kAhead - 1>();
+    __syncwarp();
+    const TileInfo first = sm.info[warp][slot];
+    const SeqRange range = seq_range(a, first.seq);
+    const int head = first.head;
+    const long long u0 =
+        at - (first.token0 - warp * kWarpTokens - range.begin) / kTile;
+    const long long u1 = u0 + range.tiles;
+    const long long pair_end = u1 < t1 ? u1 : t1;
+    const int q0 = __ldg(a.q_starts + first.seq);
+    const int rows = range.q_len * p.groups;
+
+    // Q rows to shared memory as the B operand's source
+    for (int r = warp; r < S::kRows; r += kWarps) {
+      constexpr int kPer = D / 32;  // consecutive columns per lane
+      float v[kPer];
+      float amax = 0.f;
+      const bool on = r < rows;
+      const uint16_t* src = static_cast<const uint16_t*>(a.q) +
+                            (long long)(q0 + (on ? r / p.groups : 0)) * a.q_token_stride +
+                            (long long)(head * p.groups + (on ? r % p.groups : 0)) * a.q_head_stride +
+                            lane * kPer;
+      uint16_t bits[kPer];
+#pragma unroll
+      for (int i = 0; i < kPer; i += 2) {
+        const uint32_t w = on ? __ldg(reinterpret_cast<const uint32_t*>(src + i)) : 0u;
+        bits[i] = (uint16_t)w;
+        bits[i + 1] = (uint16_t)(w >> 16);
+      }
+      float scale = 1.f;
+      if (KV == kE4m3 && !a.q_f16) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          v[i] = __bfloat162float(__ushort_as_bfloat16(bits[i]));
+          amax = fmaxf(amax, fabsf(v[i]));
+        }
+#pragma unroll
+        for (int s = 16; s > 0; s >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, s));
+        // 2^-x brings the largest magnitude into [1, 2): exact in f16 down to
+        // 2^-24. An infinity stays one through any factor.
+        int x = (int)(__float_as_uint(amax) >> 23) - 127;
+        x = min(max(x, -126), 126);
+        scale = __uint_as_float((uint32_t)(127 + x) << 23);
+        const float inv = __uint_as_float((uint32_t)(127 - x) << 23);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) bits[i] = __half_as_ushort(__float2half_rn(v[i] * inv));
+      }
+#pragma unroll
+      for (int i = 0; i < kPer; i += 2)
+        *reinterpret_cast<uint32_t*>(&sm.q[r][lane * kPer + i]) =
+            bits[i] | (uint32_t)bits[i + 1] << 16;
+      if (lane == 0) {
+        sm.row_scale[r] = scale * p.scale_log2;
+        // tokens row r sees: [row_lo, row_hi)
+        const int pos = range.kv_len - range.q_len + r / p.groups;
+        int hi = a.causal ? min(range.end, pos + 1) : range.end;
+        int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+        if (!on) hi = 0;
+        sm.row_hi[r] = hi;
+        sm.row_lo[r] = lo;
+      }
+    }
+    __syncthreads();
+
+    // Q as B fragments: for k-step ks, register pair [ks][nr]. K's columns are
+    // taken in the order the A operand finds them in memory.
+    constexpr int kSteps = D / 16;
+    constexpr bool kQInRegs = D * NR <= 256;
+    uint32_t qf[kQInRegs ? kSteps : 1][NR][2];
+    auto load_q = [&](int ks, int nr, uint32_t& b0, uint32_t& b1) {
+      const uint16_t* row = sm.q[8 * nr + g];
+      if (KV != kE4m3) {
+        b0 = *reinterpret_cast<const uint32_t*>(row + ks * 16 + 2 * c);
+        b1 = *reinterpret_cast<const uint32_t*>(row + ks * 16 + 2 * c + 8);
+      } else {
+        // step ks = word (ks & 3) of the lane's chunk c + 4 (ks >> 2): columns
+        // 2, 3 of the word are the low k pair, columns 0, 1 the high one
+        const uint2 w = *reinterpret_cast<const uint2*>(row + (c + 4 * (ks >> 2)) * 16 + (ks & 3) * 4);
+        b0 = w.y;
+        b1 = w.x;
+      }
+    };
+    if (kQInRegs) {
+#pragma unroll
+      for (int ks = 0; ks < kSteps; ++ks)
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr) load_q(ks, nr, qf[ks][nr][0], qf[ks][nr][1]);
+    }
+    float row_scale[NR][2];
+    int row_lo[NR][2], row_hi[NR][2];
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        row_scale[nr][j] = sm.row_scale[8 * nr + 2 * c + j];
+        row_lo[nr][j] = sm.row_lo[8 * nr + 2 * c + j];
+        row_hi[nr][j] = sm.row_hi[8 * nr + 2 * c + j];
+        m[nr][j] = -INFINITY;
+        l[nr][j] = 0.f;
+      }
+    v_exp = 1;
+#pragma unroll
+    for (int t = 0; t < D / 16; ++t)
+#pragma unroll
+      for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[t][nr][j] = 0.f;
+
+    for (; at < pair_end; ++at) {
+      cp_async_wait<S::kAhead - 1>();
+      __syncwarp();
+      const int token0 = sm.info[warp][slot].token0;
+      const uint32_t byte = next_byte;
+      // refill: the stage freed last step, from the entry kAhead steps on
+      {
+        const int s2 = slot + S::kAhead < S::kRing ? slot + S::kAhead : slot + S::kAhead - S::kRing;
+        issue(s2, stage + S::kAhead < S::kStages ? stage + S::kAhead : stage + S::kAhead - S::kStages);
+        request(false);
+        cp_async_commit();
+      }
+      const uint8_t* ks_ptr = sm.stage[warp][stage];
+      const uint8_t* vs_ptr = ks_ptr + kWarpTokens * S::kRowBytes;
+
+      // -- S^T = K Q^T
+      float s[NR][4];
+#pragma unroll
+      for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[nr][j] = 0.f;
+      if (KV != kE4m3) {
+        const uint32_t base = smem_u32(ks_ptr);
+        const int row = lane & 15;
+#pragma unroll
+        for (int ks = 0; ks < kSteps; ++ks) {
+          uint32_t af[4];
+          ldsm4(af, base + chunk_at<D, KV, false>(row, 2 * ks + (lane >> 4)));
+#pragma unroll
+          for (int nr = 0; nr < NR; ++nr) {
+            uint32_t b0, b1;
+            if (kQInRegs) {
+              b0 = qf[kQInRegs ? ks : 0][nr][0];
+              b1 = qf[kQInRegs ? ks : 0][nr][1];
+            } else {
+              load_q(ks, nr, b0, b1);
+            }
+            mma<KV>(s[nr], af, b0, b1);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int q4 = 0; q4 < D / 64; ++q4) {
+          const uint4 lo = ld_shared_u128(ks_ptr + chunk_at<D, KV, false>(g, c + 4 * q4));
+          const uint4 hi = ld_shared_u128(ks_ptr + chunk_at<D, KV, false>(g + 8, c + 4 * q4));
+          const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint32_t af[4];
+            // byte pairs (2, 3) and (0, 1) of a word: the k order load_q gives Q
+            af[0] = e4m3x2_to_f16x2((uint16_t)(wl[j] >> 16));
+            af[1] = e4m3x2_to_f16x2((uint16_t)(wh[j] >> 16));
+            af[2] = e4m3x2_to_f16x2((uint16_t)wl[j]);
+            af[3] = e4m3x2_to_f16x2((uint16_t)wh[j]);
+#pragma unroll
+            for (int nr = 0; nr < NR; ++nr) {
+              uint32_t b0, b1;
+              if (kQInRegs) {
+                b0 = qf[kQInRegs ? 4 * q4 + j : 0][nr][0];
+                b1 = qf[kQInRegs ? 4 * q4 + j : 0][nr][1];
+              } else {
+                load_q(4 * q4 + j, nr, b0, b1);
+              }
+              mma<KV>(s[nr], af, b0, b1);
+            }
+          }
+        }
+      }
+
+      // -- scales, masks, lazy maximum
+      float k_scale[2] = {1.f, 1.f};
+      int v_byte[2] = {0, 0};
+      bool raise_v = false;
+      if (KV == kE4m3) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint32_t kb = __shfl_sync(0xffffffffu, byte, g + 8 * j);
+          k_scale[j] = kb == 255u ? __int_as_float(0x7fc00000) : __uint_as_float(kb << 23);
+          v_byte[j] = (int)__shfl_sync(0xffffffffu, byte, 16 + g + 8 * j);
+          raise_v |= v_byte[j] > v_exp && v_byte[j] != 255;
+        }
+        next_byte = scale_byte(slot + 1 == S::kRing ? 0 : slot + 1);
+      }
+      bool raise = false;
+#pragma unroll
+      for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int token = token0 + g + 8 * (j >> 1);
+          const bool seen = token >= row_lo[nr][j & 1] && token < row_hi[nr][j & 1];
+          float x = s[nr][j] * row_scale[nr][j & 1];
+          if (KV == kE4m3) x *= k_scale[j >> 1];
+          x = seen ? x : -INFINITY;
+          s[nr][j] = x;
+          raise |= x > m[nr][j & 1] + kLazy;
+        }
+      if (__any_sync(0xffffffffu, raise || raise_v)) {
+        float o_scale[NR][2];
+        int top = max(v_exp, max(v_byte[0] == 255 ? 0 : v_byte[0], v_byte[1] == 255 ? 0 : v_byte[1]));
+        if (KV == kE4m3) {
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, x));
+        }
+        // 2^(old - new) of the values' reference exponent
+        const float v_ratio = KV == kE4m3 ? pow2(v_exp - top) : 1.f;
+        if (KV == kE4m3) v_exp = top;
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float mx = fmaxf(s[nr][j], s[nr][j + 2]);
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+            // a row that nothing pushed past the threshold keeps its maximum
+            const float mn = mx > m[nr][j] + kLazy ? mx : m[nr][j];
+            const float f = m[nr][j] == mn ? 1.f : exp2_fast(m[nr][j] - mn);
+            l[nr][j] *= f;
+            m[nr][j] = mn;
+            o_scale[nr][j] = f * v_ratio;
+          }
+#pragma unroll
+        for (int t = 0; t < D / 16; ++t)
+#pragma unroll
+          for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[t][nr][j] *= o_scale[nr][j & 1];
+      }
+
+      // -- P^T, as the B operand
+      float v_scale[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        v_scale[j] = KV != kE4m3 ? 1.f
+                     : v_byte[j] == 255 ? __int_as_float(0x7fc00000)
+                                        : pow2(v_byte[j] - v_exp);
+      uint32_t pf[NR][2];
+#pragma unroll
+      for (int nr = 0; nr < NR; ++nr) {
+        float pr[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float base = m[nr][j & 1] == -INFINITY ? 0.f : m[nr][j & 1];
+          pr[j] = exp2_fast(s[nr][j] - base);
+          l[nr][j & 1] += pr[j];
+          // a masked token's P is zero whatever its value's scale says
+          if (KV == kE4m3) pr[j] = pr[j] == 0.f ? 0.f : pr[j] * v_scale[j >> 1];
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t pk;
+          if (KV == kBf16) {
+            const __nv_bfloat162 b = __floats2bfloat162_rn(pr[2 * h], pr[2 * h + 1]);
+            pk = *reinterpret_cast<const uint32_t*>(&b);
+          } else {
+            const __half2 b = __floats2half2_rn(pr[2 * h], pr[2 * h + 1]);
+            pk = *reinterpret_cast<const uint32_t*>(&b);
+          }
+          pf[nr][h] = transpose8x8(pk);
+        }
+      }
+
+      // -- O^T += V^T P^T
+      if (KV != kE4m3) {
+        const uint32_t base = smem_u32(vs_ptr);
+        // matrices: (tokens 0-7, columns 0-7), (0-7, 8-15), (8-15, 0-7), (8-15, 8-15)
+        const int row = (lane & 7) + ((lane >> 4) << 3);
+#pragma unroll
+        for (int t = 0; t < D / 16; ++t) {
+          uint32_t af[4];
+          ldsm4_t(af, base + chunk_at<D, KV, true>(row, 2 * t + ((lane >> 3) & 1)));
+#pragma unroll
+          for (int nr = 0; nr < NR; ++nr) mma<KV>(o[t][nr], af, pf[nr][0], pf[nr][1]);
+        }
+      } else {
+        // lane group g holds 16 (head_dim 64: 8) neighbouring columns of the
+        // tokens 2c, 2c + 1, 2c + 8, 2c + 9; tile t takes columns 2t, 2t + 1
+        constexpr int kHalf = D >= 128 ? D / 128 : 1;
+#pragma unroll
+        for (int hf = 0; hf < kHalf; ++hf) {
+          uint32_t w[4][4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int row = 2 * c + (i & 1) + 8 * (i >> 1);
+            if (D >= 128) {
+              const uint4 x = ld_shared_u128(vs_ptr + chunk_at<D, KV, true>(row, g + 8 * hf));
+              w[i][0] = x.x;
+              w[i][1] = x.y;
+              w[i][2] = x.z;
+              w[i][3] = x.w;
+            } else {
+              const uint2 x = *reinterpret_cast<const uint2*>(
+                  vs_ptr + chunk_at<D, KV, true>(row, g >> 1) + (g & 1) * 8);
+              w[i][0] = x.x;
+              w[i][1] = x.y;
+            }
+          }
+#pragma unroll
+          for (int t = 0; t < (D >= 128 ? 8 : 4); ++t) {
+            const uint32_t x = __byte_perm(w[0][t / 2], w[1][t / 2], t & 1 ? 0x7362 : 0x5140);
+            const uint32_t y = __byte_perm(w[2][t / 2], w[3][t / 2], t & 1 ? 0x7362 : 0x5140);
+            uint32_t af[4];
+            af[0] = e4m3x2_to_f16x2((uint16_t)x);
+            af[1] = e4m3x2_to_f16x2((uint16_t)(x >> 16));
+            af[2] = e4m3x2_to_f16x2((uint16_t)y);
+            af[3] = e4m3x2_to_f16x2((uint16_t)(y >> 16));
+#pragma unroll
+            for (int nr = 0; nr < NR; ++nr) mma<KV>(o[8 * hf + t][nr], af, pf[nr][0], pf[nr][1]);
+          }
+        }
+      }
+      __syncwarp();
+      slot = slot + 1 == S::kRing ? 0 : slot + 1;
+      stage = stage + 1 == S::kStages ? 0 : stage + 1;
+    }
+
+    // -- the four warps' (O, m, l) to one
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1)
+          l[nr][j] += __shfl_xor_sync(0xffffffffu, l[nr][j], x);
+        if (g == 0) {
+          sm.wm[warp][8 * nr + 2 * c + j] = m[nr][j];
+          sm.wl[warp][8 * nr + 2 * c + j] = l[nr][j];
+        }
+      }
+    if (lane == 0) sm.wv[warp] = v_exp;
+    __syncthreads();
+    float f[NR][2];
+    {
+#pragma unroll
+      for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float mx = -INFINITY;
+          for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, sm.wm[w][8 * nr + 2 * c + j]);
+          f[nr][j] = m[nr][j] == -INFINITY ? 0.f : exp2_fast(m[nr][j] - mx);
+          // O is in units of 2^(v_exp - 127)
+          if (KV == kE4m3) f[nr][j] *= __uint_as_float((uint32_t)v_exp << 23);
+        }
+    }
+    for (int w = 0; w < kWarps; ++w) {
+      if (warp == w) {
+#pragma unroll
+        for (int t = 0; t < D / 16; ++t)
+#pragma unroll
+          for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              int d;
+              if (KV != kE4m3)
+                d = 16 * t + g + 8 * (j >> 1);
+              else if (D >= 128)
+                d = 16 * (g + 8 * (t / 8)) + 2 * (t % 8) + (j >> 1);
+              else
+                d = 8 * g + 2 * t + (j >> 1);
+              float* dst = &sm.merge[8 * nr + 2 * c + (j & 1)][d];
+              const float v = f[nr][j & 1] == 0.f ? 0.f : o[t][nr][j] * f[nr][j & 1];
+              *dst = w == 0 ? v : *dst + v;
+            }
+      }
+      __syncthreads();
+    }
+
+    // -- out: the whole pair, or this block's part of it
+    const long long row_floats = D + 2;
+    if (u0 >= t0 && u1 <= t1) {
+      for (int r = warp; r < rows; r += kWarps) {
+        float mx = -INFINITY, sum = 0.f;
+        for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, sm.wm[w][r]);
+        for (int w = 0; w < kWarps; ++w)
+          sum += sm.wm[w][r] == -INFINITY ? sm.wl[w][r] : sm.wl[w][r] * exp2_fast(sm.wm[w][r] - mx);
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const long long tok = q0 + r / p.groups;
+        const int qh = head * p.groups + r % p.groups;
+        uint16_t* dst = static_cast<uint16_t*>(a.out) + tok * a.out_token_stride +
+                        qh * a.out_head_stride;
+        for (int d = lane * 2; d < D; d += 64) {
+          const float x = sm.merge[r][d] * inv, y = sm.merge[r][d + 1] * inv;
+          uint32_t pk;
+          if (a.q_f16) {
+            const __half2 b = __floats2half2_rn(x, y);
+            pk = *reinterpret_cast<const uint32_t*>(&b);
+          } else {
+            const __nv_bfloat162 b = __floats2bfloat162_rn(x, y);
+            pk = *reinterpret_cast<const uint32_t*>(&b);
+          }
+          *reinterpret_cast<uint32_t*>(dst + d) = pk;
+        }
+        if (a.lse != nullptr && lane == 0)
+          a.lse[tok * a.q_heads + qh] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) / kLog2e;
+      }
+    } else {
+      // Blocks of the pair: c_first holds its first tile, c_last its last one.
+      const int c_first = (int)(((u0 + 1) * ctas - 1) / total);
+      const int c_last = (int)((u1 * ctas - 1) / total);
+      const long long slot_floats = (long long)S::kRows * row_floats;
+      float* scratch = reinterpret_cast<float*>(a.scratch);
+      // slot 0: a block that enters the pair from the one before; 1: the first
+      float* part = scratch + (2ll * blockIdx.x + (u0 >= t0 ? 1 : 0)) * slot_floats;
+      for (int r = warp; r < rows; r += kWarps) {
+        float mx = -INFINITY, sum = 0.f;
+        for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, sm.wm[w][r]);
+        for (int w = 0; w < kWarps; ++w)
+          sum += sm.wm[w][r] == -INFINITY ? sm.wl[w][r] : sm.wl[w][r] * exp2_fast(sm.wm[w][r] - mx);
+        float* dst = part + r * row_floats;
+        for (int d = lane * 2; d < D; d += 64)
+          *reinterpret_cast<float2*>(dst + 2 + d) = make_float2(sm.merge[r][d], sm.merge[r][d + 1]);
+        if (lane == 0) *reinterpret_cast<float2*>(dst) = make_float2(mx, sum);
+      }
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) {
+        const int n = atomicAdd(a.counters + c_first, 1) + 1;
+        sm.flag = n == c_last - c_first + 1;
+        if (sm.flag) a.counters[c_first] = 0;
+        __threadfence();
+      }
+      __syncthreads();
+      if (sm.flag) {
+        // A warp per row: the parts' maximum, then their weighted sum.
+        for (int r = warp; r < rows; r += kWarps) {
+          float mx = -INFINITY;
+          for (int b = c_first + lane; b <= c_last; b += 32) {
+            const float* src = scratch + (2ll * b + (b == c_first ? 1 : 0)) * slot_floats + r * row_floats;
+            mx = fmaxf(mx, __ldcg(src));
+          }
+#pragma unroll
+          for (int x = 16; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+          float sum = 0.f, acc[D / 32];
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
+#pragma unroll 4
+          for (int b = c_first; b <= c_last; ++b) {
+            const float* src = scratch + (2ll * b + (b == c_first ? 1 : 0)) * slot_floats + r * row_floats;
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(src));
+            const float w = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : exp2_fast(ml.x - mx);
+            sum += ml.y * w;
+#pragma unroll
+            for (int i = 0; i < D / 64; ++i) {
+              const float2 v = __ldcg(reinterpret_cast<const float2*>(src + 2 + 64 * i + 2 * lane));
+              acc[2 * i] += w == 0.f ? 0.f : v.x * w;
+              acc[2 * i + 1] += w == 0.f ? 0.f : v.y * w;
+            }
+          }
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+          const long long tok = q0 + r / p.groups;
+          const int qh = head * p.groups + r % p.groups;
+          uint16_t* dst = static_cast<uint16_t*>(a.out) + tok * a.out_token_stride +
+                          qh * a.out_head_stride;
+#pragma unroll
+          for (int i = 0; i < D / 64; ++i) {
+            uint32_t pk;
+            if (a.q_f16) {
+              const __half2 b = __floats2half2_rn(acc[2 * i] * inv, acc[2 * i + 1] * inv);
+              pk = *reinterpret_cast<const uint32_t*>(&b);
+            } else {
+              const __nv_bfloat162 b = __floats2bfloat162_rn(acc[2 * i] * inv, acc[2 * i + 1] * inv);
+              pk = *reinterpret_cast<const uint32_t*>(&b);
+            }
+            *reinterpret_cast<uint32_t*>(dst + 64 * i + 2 * lane) = pk;
+          }
+          if (a.lse != nullptr && lane == 0)
+            a.lse[tok * a.q_heads + qh] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) / kLog2e;
+        }
+      }
+    }
+    __syncthreads();
+  }
+  cp_async_wait<0>();
+  griddep_launch_dependents();
+}
+
+template <int D, int KV, int NR>
+cudaError_t launch(const DecodeParams& p, cudaStream_t stream) {
+  using Smem = typename Shape<D, KV, NR>::Smem;
+  static bool configured[64] = {};
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err != cudaSuccess) return err;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (!configured[dev]) {
+    err = cudaFuncSetAttribute(attn_decode_kernel<D, KV, NR>,
+                               cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Smem));
+    if (err != cudaSuccess) return err;
+    configured[dev] = true;
+  }
+  static_assert((sizeof(Smem) + 1024) * Shape<D, KV, NR>::kBlocks <= 228 * 1024, "fits the SM");
+  return launch_pdl(attn_decode_kernel<D, KV, NR>, 
+                    dim3((unsigned)(Shape<D, KV, NR>::kBlocks * device_sm_count())), dim3(kThreads),
+                    sizeof(Smem), stream, p);
+}
+
+template <int D, int KV>
+cudaError_t launch_rows(const DecodeParams& p, int rows, cudaStream_t stream) {
+  return rows <= 8 ? launch<D, KV, 1>(p, stream) : launch<D, KV, 2>(p, stream);
+}
+
+template <int D>
+cudaError_t launch_type(const DecodeParams& p, int rows, cudaStream_t stream) {
+  if (p.a.cache_dtype == 3) return launch_rows<D, kE4m3>(p, rows, stream);
+  return p.a.cache_dtype == 1 ? launch_rows<D, kF16>(p, rows, stream)
+                              : launch_rows<D, kBf16>(p, rows, stream);
+}
+
+}  // namespace
+
+int attn_decode_rows() { return 16; }
+int attn_max_ctas() { return kMaxCtas; }
+
+long long attn_decode_scratch_bytes(int head_dim) {
+  return 2ll * 2 * device_sm_count() * 16 * (head_dim + 2) * 4;
+}
+
+cudaError_t launch_attn_decode(const AttnLaunch& l, cudaStream_t stream) {
+  DecodeParams p{};
+  p.a = l;
+  p.groups = l.q_heads / l.c.heads;
+  p.scale_log2 = l.scale * kLog2e;
+  p.page_shift = (l.c.page_size & (l.c.page_size - 1)) == 0 ? __builtin_ctz(l.c.page_size) : -1;
+  const int rows = l.max_q * p.groups;
+  switch (l.c.head_dim) {
+    case 64: return launch_type<64>(p, rows, stream);
+    case 128: return launch_type<128>(p, rows, stream);
+    default: return launch_type<256>(p, rows, stream);
+  }
+}
+
+}  // namespace b200

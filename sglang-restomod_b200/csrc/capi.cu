@@ -256,6 +256,7 @@ int b200::set_last_error(int code, const char* message) {
 
 int64_t b200::ws_head_bytes() { return kStatusBytes + kCounterBytes; }
 int64_t b200::ws_fixed_bytes() { return stream_ws_bytes(); }
+int64_t b200::ws_counter_offset() { return kStatusBytes; }
 
 extern "C" {
 
@@ -1508,6 +1509,45 @@ int b200_w8a8_linear(const void* x, int32_t x_dtype, int64_t m, int64_t k, const
   L.out_f16 = y_dtype == B200_DTYPE_F16;
   L.status = ws.status;
   return check_cuda(launch_w8a8_gemm(L, st), "W8A8 GEMM launch");
+}
+
+int b200_w8a8_linear_quantized(const uint8_t* q, const float* scales, int64_t scales_ld, int64_t m,
+                               int64_t k, const uint8_t* w_e4m3, const float* w_scales, int64_t n,
+                               int32_t gated_mode, void* y, int32_t y_dtype, void* workspace,
+                               int64_t workspace_bytes, void* stream) {
+  int rc = check_w8_weights(n, k, gated_mode);
+  if (rc) return rc;
+  if (!valid_dtype16(y_dtype)) return fail(B200_ERR_UNSUPPORTED, "the output must be bf16 or f16");
+  if (m < 0 || m >= (1ll << 31)) return fail(B200_ERR_INVALID, "bad M %lld", (long long)m);
+  if (m == 0) return B200_OK;
+  if (q == nullptr || scales == nullptr || w_e4m3 == nullptr || w_scales == nullptr || y == nullptr)
+    return fail(B200_ERR_INVALID, "null pointer argument");
+  if (!aligned16(q) || !aligned16(scales) || !aligned16(w_e4m3))
+    return fail(B200_ERR_INVALID, "q, scales and weights must be 16-byte aligned");
+  // An item copies the scales of 128 rows at once, the last one past row m.
+  if (scales_ld < (m + 127) / 128 * 128 || scales_ld % 4)
+    return fail(B200_ERR_INVALID,
+                "scales_ld %lld must be a multiple of 4 and at least M %lld rounded up to 128",
+                (long long)scales_ld, (long long)m);
+  WsView ws;
+  if (!carve(workspace, workspace_bytes, ws))
+    return fail(B200_ERR_INVALID, "workspace smaller than b200_gemm_workspace_bytes(0)");
+  W8Launch L{};
+  L.w = w_e4m3;
+  L.wscale = w_scales;
+  L.xq = q;
+  L.xscale = scales;
+  L.xs_ld = scales_ld;
+  L.rows = m;
+  L.E = 1;
+  L.N = (int)n;
+  L.K = (int)k;
+  L.gated = gated_mode == B200_GATED_FUSED;
+  L.out = y;
+  L.ldo = gated_mode == B200_GATED_FUSED ? n / 2 : n;
+  L.out_f16 = y_dtype == B200_DTYPE_F16;
+  L.status = ws.status;
+  return check_cuda(launch_w8a8_gemm(L, reinterpret_cast<cudaStream_t>(stream)), "W8A8 GEMM launch");
 }
 
 int b200_w8a8_moe_gemm(const void* a, int32_t a_dtype, int64_t a_rows, int64_t k,

@@ -21,6 +21,7 @@ enum DeviceError : int {
   kDevBadExpert = 2,     // an expert id outside [0, E) reached a GEMM
   kDevBadRoute = 4,      // a route index outside the activation rows
   kDevPeerTimeout = 8,   // an expert-parallel wait on another rank gave up
+  kDevBadPage = 16,      // a page number outside the key/value cache
 };
 
 // A wait that has not completed after this many nanoseconds records

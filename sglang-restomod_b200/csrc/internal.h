@@ -256,6 +256,83 @@ cudaError_t launch_fp8_act_quant(const void* x, int x_f16, long long x_rows, int
                                  long long out_rows, uint8_t* q, float* scales, long long ld,
                                  int* status, cudaStream_t stream);
 
+// Residual-add RMS norm (norm.cu). Strides in elements; nullptr residual /
+// residual_out / y / q: not given or not wanted. hidden % 8 == 0, and % 128
+// with q; scales [hidden / 128][scales_ld].
+struct NormLaunch {
+  const void* x;
+  const void* residual;
+  const void* weight;
+  void* residual_out;
+  void* y;
+  uint8_t* q;
+  float* scales;
+  long long x_ld, residual_ld, residual_out_ld, y_ld, scales_ld, rows, hidden;
+  int f16;
+  int weight_dtype;  // 0 bf16, 1 f16, 2 f32
+  float eps, weight_bias;
+};
+cudaError_t launch_add_rms_norm(const NormLaunch& l, cudaStream_t stream);
+long long norm_max_hidden();
+
+// A paged key/value cache: element (page, offset, head, i) of k and v at
+// page * page_stride + offset * token_stride + head * head_stride + i, in
+// elements of the cache's type (e4m3 where k_scale is given: one scale byte
+// per vector at the scale strides; 16-bit otherwise).
+struct KvCacheView {
+  void* k;
+  void* v;
+  uint8_t* k_scale;
+  uint8_t* v_scale;
+  long long num_pages;
+  long long page_stride, token_stride, head_stride;
+  long long scale_page_stride, scale_token_stride, scale_head_stride;
+  int page_size, heads, head_dim;
+};
+cudaError_t launch_kv_write(const KvCacheView& c, const void* k, const void* v, bool f16,
+                            long long k_token_stride, long long k_head_stride,
+                            long long v_token_stride, long long v_head_stride,
+                            const long long* slots, long long tokens, cudaStream_t stream);
+cudaError_t launch_kv_read(const KvCacheView& c, void* k, void* v, bool f16,
+                           long long token_stride, long long head_stride, const long long* slots,
+                           long long tokens, cudaStream_t stream);
+
+// Attention of the last q_starts[s + 1] - q_starts[s] tokens of each sequence
+// over its kv_lens[s] cached ones (attn_decode.cu, attn_prefill.cu).
+struct AttnLaunch {
+  KvCacheView c;
+  int cache_dtype;  // 0 bf16, 1 f16, 3 e4m3
+  const void* q;
+  int q_f16;
+  long long q_token_stride, q_head_stride, q_tokens;
+  const int* table;  // [seqs][table_stride], table_width entries each
+  long long table_stride;
+  int table_width;
+  const int* kv_lens;
+  const int* q_starts;
+  int seqs, max_q, q_heads;
+  float scale;
+  int causal, window;  // window 0: none
+  void* out;           // type of q
+  long long out_token_stride, out_head_stride;
+  float* lse;          // [q_tokens][q_heads] or nullptr
+  int* status;
+  int* counters;       // the workspace's 1024 arrival counters, zero between calls
+  uint8_t* scratch;
+};
+// The decode kernel takes up to attn_decode_rows() rows (new tokens x query
+// heads per key/value head) of a sequence; the tensor-core kernel any number.
+int attn_decode_rows();
+long long attn_decode_scratch_bytes(int head_dim);
+cudaError_t launch_attn_decode(const AttnLaunch& l, cudaStream_t stream);
+long long attn_prefill_scratch_bytes(int head_dim, long long q_tokens, int seqs);
+cudaError_t launch_attn_prefill(const AttnLaunch& l, cudaStream_t stream);
+inline long long attn_scratch_bytes(int head_dim, long long q_tokens, int seqs) {
+  const long long d = attn_decode_scratch_bytes(head_dim);
+  const long long p = attn_prefill_scratch_bytes(head_dim, q_tokens, seqs);
+  return d > p ? d : p;
+}
+
 // Records `message` as this thread's b200_last_error() and returns `code`.
 int set_last_error(int code, const char* message);
 
@@ -264,5 +341,6 @@ int set_last_error(int code, const char* message);
 // split partial sums) is ws_fixed_bytes() on the current device.
 int64_t ws_head_bytes();
 int64_t ws_fixed_bytes();
+int64_t ws_counter_offset();
 
 }  // namespace b200

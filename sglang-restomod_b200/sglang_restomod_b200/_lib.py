@@ -25,6 +25,7 @@ ERR_CUDA = 3
 DTYPE_BF16 = 0
 DTYPE_F16 = 1
 DTYPE_F32 = 2
+DTYPE_E4M3 = 3
 
 QUANT_FP8_BLOCK = 0
 QUANT_NVFP4 = 1
@@ -148,11 +149,38 @@ SIGNATURES = {
         [c_void_p, c_int32, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int32, c_void_p,
          c_int32, c_void_p, c_int64, c_void_p],
     ),
+    "b200_w8a8_linear_quantized": (
+        c_int32,
+        [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int32,
+         c_void_p, c_int32, c_void_p, c_int64, c_void_p],
+    ),
     "b200_w8a8_moe_gemm": (
         c_int32,
         [c_void_p, c_int32, c_int64, c_int64, c_void_p, c_void_p, c_int32, c_int64, c_int32,
          c_void_p, c_void_p, c_int64, c_void_p, c_int32, c_int32, c_int64, c_void_p, c_int32,
          c_void_p, c_int32, c_int64, c_void_p, c_int64, c_void_p],
+    ),
+    "b200_add_rms_norm": (
+        c_int32,
+        [c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int32,
+         c_float, c_float, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64,
+         c_void_p],
+    ),
+    "b200_kv_cache_write": (
+        c_int32,
+        [c_void_p, c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int64, c_int64, c_void_p,
+         c_int64, c_void_p],
+    ),
+    "b200_kv_cache_read": (
+        c_int32,
+        [c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int32, c_int64, c_int64, c_void_p],
+    ),
+    "b200_paged_attention_workspace_bytes": (c_int64, [c_int32, c_int64, c_int32]),
+    "b200_paged_attention": (
+        c_int32,
+        [c_void_p, c_void_p, c_int32, c_int64, c_int32, c_int64, c_int64, c_void_p, c_int64,
+         c_int32, c_void_p, c_void_p, c_int32, c_int32, c_float, c_int32, c_int32, c_void_p,
+         c_int64, c_int64, c_void_p, c_void_p, c_int64, c_void_p],
     ),
     "b200_ep_region_bytes": (c_int64, [c_int32, c_int64, c_int32, c_int64]),
     "b200_ep_region_layout": (c_int32, [c_int32, c_int64, c_int32, c_int64, ctypes.POINTER(c_int64)]),
@@ -179,6 +207,18 @@ SIGNATURES = {
          c_int32, c_int32, c_void_p, c_int64, c_void_p],
     ),
 }
+
+
+class KVCacheDesc(ctypes.Structure):
+    """``b200_kv_cache``: a paged key/value cache's pointers and strides."""
+
+    _fields_ = [
+        ("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p),
+        ("num_pages", c_int64), ("page_size", c_int32), ("kv_heads", c_int32),
+        ("head_dim", c_int32), ("dtype", c_int32), ("page_stride", c_int64),
+        ("token_stride", c_int64), ("head_stride", c_int64), ("scale_page_stride", c_int64),
+        ("scale_token_stride", c_int64), ("scale_head_stride", c_int64),
+    ]
 
 
 class B200Error(RuntimeError):

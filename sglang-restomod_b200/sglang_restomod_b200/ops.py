@@ -691,3 +691,301 @@ def w8a8_moe_gemm(a: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, *, n
         )
     )
     return c
+
+
+def w8a8_scales_ld(rows: int) -> int:
+    """Leading dimension of activation scales that :func:`w8a8_linear_quantized` takes."""
+    return (rows + 127) // 128 * 128
+
+
+def w8a8_linear_quantized(q: torch.Tensor, scales: torch.Tensor, w: torch.Tensor,
+                          w_scales: torch.Tensor, *, gated_mode: int = _lib.GATED_NONE,
+                          out: torch.Tensor | None = None,
+                          out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """:func:`w8a8_linear` on activations that are already quantized: ``q`` e4m3
+    ``[M, K]`` and ``scales`` fp32 ``[K/128, >= w8a8_scales_ld(M)]``, as
+    :func:`fp8_act_quant` or :func:`add_rms_norm_fp8` return them."""
+    _contig(q, "q")
+    _contig(scales, "scales")
+    _w8_weights(w, w_scales)
+    if q.dtype != torch.float8_e4m3fn or scales.dtype != torch.float32:
+        raise TypeError(f"q must be float8_e4m3fn and scales float32, got {q.dtype}, {scales.dtype}")
+    m, k = (int(d) for d in q.shape)
+    if w.shape[-1] != k or scales.shape[0] != k // 128:
+        raise ValueError(f"K differs: q {k}, weight {w.shape[-1]}, scales {scales.shape[0]} groups")
+    n = int(w.shape[-2])
+    cols = n // 2 if gated_mode == _lib.GATED_FUSED else n
+    if out is None:
+        out = torch.empty(m, cols, dtype=out_dtype, device=q.device)
+    ws = workspace(gemm_workspace_bytes(0), q.device)
+    _lib.check(
+        lib().b200_w8a8_linear_quantized(
+            _vp(q), _vp(scales), scales.shape[1], m, k, _vp(w), _vp(w_scales), n, gated_mode,
+            _vp(out), _code(out, "out"), _vp(ws), ws.numel(), _stream(q.device))
+    )
+    return out
+
+
+# ------------------------------------------- norm, key/value cache, attention
+# Decode calls these several times a layer on microseconds of GPU work, so the
+# wrappers keep their own host time low: plain integers instead of ctypes
+# objects, and the current stream by its raw handle.
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _on_device(what: str, *tensors: torch.Tensor | None) -> int:
+    """The index of the one CUDA device all tensors are on; it must be the
+    current one, whose context the library launches in."""
+    index = -1
+    for t in tensors:
+        if t is None:
+            continue
+        at = t.get_device()
+        if at < 0:
+            raise ValueError(f"{what}: operands must be CUDA tensors")
+        if index < 0:
+            index = at
+        elif at != index:
+            raise ValueError(f"{what}: operands are on different devices")
+    if index != torch.cuda.current_device():
+        raise ValueError(f"{what}: operands are on cuda:{index}, the current device is "
+                         f"cuda:{torch.cuda.current_device()}")
+    return index
+
+
+def _norm(x, weight, eps, residual, weight_bias, residual_out, y, q, scales, scales_ld, like):
+    index = _on_device("add_rms_norm", x, weight, residual, residual_out, y)
+    code = _DTYPE_CODE.get(x.dtype)
+    wcode = _LOGIT_CODE.get(weight.dtype)
+    if code is None or wcode is None:
+        raise TypeError(f"x must be bf16 or f16 and weight bf16, f16 or f32, got {x.dtype}, "
+                        f"{weight.dtype}")
+    hidden = x.shape[-1]
+    if weight.dim() != 1 or weight.shape[0] != hidden or not weight.is_contiguous():
+        raise ValueError(f"weight must be a contiguous [{hidden}], got {tuple(weight.shape)}")
+    rows = x.shape[0]
+    for t in (residual, residual_out, y):
+        if t is None:
+            continue
+        if t.shape != x.shape or t.dtype != x.dtype or t.stride(-1) != 1:
+            raise ValueError(f"{like} must be {tuple(x.shape)} {x.dtype} rows, got "
+                             f"{tuple(t.shape)} {t.dtype}")
+    _lib.check(
+        lib().b200_add_rms_norm(
+            x.data_ptr(), code, x.stride(0), rows, hidden,
+            None if residual is None else residual.data_ptr(),
+            0 if residual is None else residual.stride(0), weight.data_ptr(), wcode,
+            weight_bias, eps, None if residual_out is None else residual_out.data_ptr(),
+            0 if residual_out is None else residual_out.stride(0),
+            None if y is None else y.data_ptr(), 0 if y is None else y.stride(0),
+            None if q is None else q.data_ptr(), None if scales is None else scales.data_ptr(),
+            scales_ld, _raw_stream(index))
+    )
+
+
+def _norm_rows(x: torch.Tensor) -> None:
+    if x.dim() != 2 or x.stride(-1) != 1:
+        raise ValueError("x must be [rows, hidden] with contiguous rows")
+
+
+def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *,
+                 residual: torch.Tensor | None = None, weight_bias: float = 0.0,
+                 out: torch.Tensor | None = None, residual_out: torch.Tensor | None = None):
+    """``(y, h)``: ``h = x + residual`` (``None`` without a residual) and ``y = h *
+    rsqrt(mean(h^2) + eps) * (weight + weight_bias)``, both in ``x``'s type.
+
+    ``x``, ``residual`` and the outputs are ``[rows, hidden]`` with contiguous
+    rows; ``out`` and ``residual_out`` may be ``x`` or ``residual`` (in place)."""
+    _norm_rows(x)
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if residual is not None and residual_out is None:
+        residual_out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    _norm(x, weight, eps, residual, weight_bias, residual_out, out, None, None, 0,
+          "residual, residual_out and out")
+    return out, residual_out
+
+
+def add_rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *,
+                     residual: torch.Tensor | None = None, weight_bias: float = 0.0,
+                     residual_out: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                     scales_ld: int | None = None):
+    """``(q, scales, h)``: :func:`add_rms_norm` with its output quantized as
+    :func:`fp8_act_quant` does (e4m3 ``[rows, hidden]``, fp32 scales ``[hidden /
+    128, scales_ld]``, default ``scales_ld = rows``; pass ``w8a8_scales_ld(rows)``
+    for :func:`w8a8_linear_quantized`). ``out``: also store the 16-bit output."""
+    _norm_rows(x)
+    rows, hidden = x.shape
+    ld = rows if scales_ld is None else int(scales_ld)
+    q = torch.empty(rows, hidden, dtype=torch.float8_e4m3fn, device=x.device)
+    scales = torch.empty(hidden // 128, ld, dtype=torch.float32, device=x.device)
+    if residual is not None and residual_out is None:
+        residual_out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    _norm(x, weight, eps, residual, weight_bias, residual_out, out, q, scales, ld,
+          "residual, residual_out and out")
+    return q, scales, residual_out
+
+
+def _vectors(t: torch.Tensor, cache, what: str) -> None:
+    if t.dim() != 3 or t.shape[1] != cache.kv_heads or t.shape[2] != cache.head_dim \
+            or t.stride(2) != 1:
+        raise ValueError(f"{what} must be [tokens, {cache.kv_heads}, {cache.head_dim}] with "
+                         f"contiguous vectors, got {tuple(t.shape)} strides {t.stride()}")
+
+
+def _slots(slots: torch.Tensor, tokens: int | None = None) -> None:
+    if slots.dtype != torch.int64 or slots.dim() != 1 or not slots.is_contiguous():
+        raise ValueError("slots must be a contiguous int64 [tokens]")
+    if tokens is not None and slots.shape[0] != tokens:
+        raise ValueError(f"{slots.shape[0]} slots for {tokens} tokens")
+
+
+def kv_cache_write(cache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
+    """Writes ``k`` and ``v`` ``[tokens, kv_heads, head_dim]`` (any strides over
+    tokens and heads) into their slots (int64 ``page * page_size + offset``;
+    negative: skipped), quantized when the cache is e4m3."""
+    index = _on_device("kv_cache_write", k, v, slots, cache.k)
+    _vectors(k, cache, "k")
+    _vectors(v, cache, "v")
+    _slots(slots, k.shape[0])
+    code = _DTYPE_CODE.get(k.dtype)
+    if code is None or v.dtype != k.dtype or v.shape[0] != k.shape[0]:
+        raise TypeError(f"k and v must be bf16 or f16 alike, got {k.dtype} {tuple(k.shape)}, "
+                        f"{v.dtype} {tuple(v.shape)}")
+    _lib.check(
+        lib().b200_kv_cache_write(cache.desc, k.data_ptr(), v.data_ptr(), code, k.stride(0),
+                                  k.stride(1), v.stride(0), v.stride(1), slots.data_ptr(),
+                                  k.shape[0], _raw_stream(index))
+    )
+
+
+def kv_cache_read(cache, slots: torch.Tensor, dtype: torch.dtype | None = None):
+    """``(k, v)`` ``[tokens, kv_heads, head_dim]`` of the given slots as values
+    (zeros for slots outside the cache). ``dtype``: bf16 or f16, by default the
+    cache's own, bf16 for an e4m3 cache."""
+    index = _on_device("kv_cache_read", slots, cache.k)
+    _slots(slots)
+    if dtype is None:
+        dtype = torch.bfloat16 if cache.k_scale is not None else cache.k.dtype
+    code = _DTYPE_CODE.get(dtype)
+    if code is None:
+        raise TypeError(f"dtype must be bf16 or f16, got {dtype}")
+    n = slots.shape[0]
+    kv = torch.empty(2, n, cache.kv_heads, cache.head_dim, dtype=dtype, device=slots.device)
+    k, v = kv[0], kv[1]
+    _lib.check(
+        lib().b200_kv_cache_read(cache.desc, slots.data_ptr(), n, k.data_ptr(), v.data_ptr(), code,
+                                 cache.kv_heads * cache.head_dim, cache.head_dim,
+                                 _raw_stream(index))
+    )
+    return k, v
+
+
+# Attention keeps one workspace per (device, stream): calls on two streams may
+# overlap, and its arrival counters and partial sums must not.
+_ATTN_WORKSPACES: dict[tuple[int, int], torch.Tensor] = {}
+_ATTN_BYTES: dict[tuple[int, int, int], int] = {}
+
+
+def paged_attention_workspace_bytes(head_dim: int, q_tokens: int, seqs: int) -> int:
+    n = int(lib().b200_paged_attention_workspace_bytes(head_dim, q_tokens, seqs))
+    if n < 0:
+        raise ValueError(f"no attention kernel for head_dim {head_dim}")
+    return n
+
+
+def _attn_workspace(index: int, stream: int, head_dim: int, q_tokens: int, seqs: int):
+    # Sizes are asked for rounded up, so few distinct ones are kept.
+    key = (head_dim, 1 << max(0, q_tokens - 1).bit_length(), 1 << max(0, seqs - 1).bit_length())
+    nbytes = _ATTN_BYTES.get(key)
+    if nbytes is None:
+        nbytes = _ATTN_BYTES[key] = paged_attention_workspace_bytes(*key)
+    ws = _ATTN_WORKSPACES.get((index, stream))
+    if ws is not None and ws.numel() >= nbytes:
+        return ws
+    if torch.cuda.is_current_stream_capturing():
+        # A capture runs on a stream of its own: this call's workspace comes
+        # from the graph's pool, and each replay clears the part that counts
+        # arrivals. reserve_attention_workspace() on the capturing stream, or
+        # the workspace argument, saves the clearing.
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
+        ws[:8192].zero_()
+        return ws
+    ws = torch.zeros(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
+    with _WS_LOCK:
+        _ATTN_WORKSPACES[(index, stream)] = ws
+    return ws
+
+
+def reserve_attention_workspace(head_dim: int, q_tokens: int, seqs: int,
+                                device: torch.device | None = None) -> torch.Tensor:
+    """The current stream's attention workspace, for calls of up to these sizes."""
+    index = torch.cuda.current_device() if device is None or device.index is None else device.index
+    return _attn_workspace(index, _raw_stream(index), head_dim, q_tokens, seqs)
+
+
+def attention_status(device: torch.device | None = None, reset: bool = True) -> int:
+    """Error bits of the attention calls on a device's streams (0 = none, 16 = a
+    page number outside the cache). Synchronizes the device."""
+    index = torch.cuda.current_device() if device is None or device.index is None else device.index
+    torch.cuda.synchronize(index)
+    bits = 0
+    for (at, stream), ws in list(_ATTN_WORKSPACES.items()):
+        if at == index:
+            word = ctypes.c_int32(0)
+            _lib.check(lib().b200_workspace_status(_vp(ws), ctypes.byref(word), int(reset),
+                                                   ctypes.c_void_p(stream)))
+            bits |= int(word.value)
+    return bits
+
+
+def paged_attention(q: torch.Tensor, cache, page_table: torch.Tensor, kv_lens: torch.Tensor,
+                    q_starts: torch.Tensor, max_q_len: int, *, scale: float | None = None,
+                    causal: bool = True, window: int = 0, out: torch.Tensor | None = None,
+                    return_lse: bool = False, workspace: torch.Tensor | None = None):
+    """Attention of each sequence's new tokens over its cached ones.
+
+    ``q`` ``[tokens, q_heads, head_dim]`` holds the new tokens of all sequences
+    (sequence s: rows ``q_starts[s] : q_starts[s + 1]``, at most ``max_q_len``),
+    which are the last of its ``kv_lens[s]`` tokens in ``cache`` (a
+    :class:`~.kv_cache.PagedKVCache`; write them first), on the pages
+    ``page_table[s]`` (int32 ``[seqs, pages]``). ``causal`` masks by position,
+    ``window`` (causal only; 0: none) keeps the last ``window`` positions. Rows
+    that see nothing give zeros and ``-inf``. ``scale`` defaults to
+    ``head_dim ** -0.5``. Returns ``out``, or ``(out, lse)`` with the fp32
+    ``[tokens, q_heads]`` log-sum-exp. ``max_q_len * q_heads / kv_heads <= 16``
+    (decode) streams the cache; larger calls run on the tensor cores."""
+    index = _on_device("paged_attention", q, cache.k, page_table, kv_lens, q_starts, out)
+    dtype = q.dtype
+    code = _DTYPE_CODE.get(dtype)
+    if code is None:
+        raise TypeError(f"q must be bf16 or f16, got {dtype}")
+    if q.dim() != 3 or q.shape[2] != cache.head_dim or q.stride(2) != 1:
+        raise ValueError(f"q must be [tokens, heads, {cache.head_dim}] with contiguous vectors, "
+                         f"got {tuple(q.shape)} strides {q.stride()}")
+    tokens, heads, dim = q.shape
+    seqs = kv_lens.shape[0]
+    for t, what in ((page_table, "page_table"), (kv_lens, "kv_lens"), (q_starts, "q_starts")):
+        if t.dtype != torch.int32 or t.stride(-1) != 1:
+            raise ValueError(f"{what} must be int32 with contiguous rows, got {t.dtype}")
+    if q_starts.shape[0] != seqs + 1 or page_table.dim() != 2 or page_table.shape[0] != seqs:
+        raise ValueError(f"{seqs} sequences need q_starts [{seqs + 1}] and page_table [{seqs}, "
+                         f"pages], got {tuple(q_starts.shape)}, {tuple(page_table.shape)}")
+    if out is None:
+        out = torch.empty(tokens, heads, dim, dtype=dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != dtype or out.stride(2) != 1:
+        raise ValueError(f"out must be {tuple(q.shape)} {dtype}, got {tuple(out.shape)} {out.dtype}")
+    lse = torch.empty(tokens, heads, dtype=torch.float32, device=q.device) if return_lse else None
+    stream = _raw_stream(index)
+    ws = workspace
+    if ws is None:
+        ws = _attn_workspace(index, stream, dim, tokens, seqs)
+    _lib.check(
+        lib().b200_paged_attention(
+            cache.desc, q.data_ptr(), code, tokens, heads, q.stride(0), q.stride(1),
+            page_table.data_ptr(), page_table.stride(0), page_table.shape[1], kv_lens.data_ptr(),
+            q_starts.data_ptr(), seqs, max_q_len, dim ** -0.5 if scale is None else scale,
+            causal, window, out.data_ptr(), out.stride(0), out.stride(1),
+            None if lse is None else lse.data_ptr(), ws.data_ptr(), ws.numel(), stream)
+    )
+    return (out, lse) if return_lse else out
