@@ -1,96 +1,984 @@
-// Attention of chunks of new tokens over the paged cache: the plain kernel,
-// one warp per (token, query head), fp32 throughout.
+// Attention of chunks of new tokens over the paged cache, on the tcgen05
+// tensor cores: one pass over a tile of rows' keys with the running maximum
+// and sum of the softmax.
 //
-// Bound: instruction issue, several instructions per key element and row.
+//   S = scale * Q K^T,  m = max S,  l = sum e^(S - m),
+//   out = sum e^(S - m) V / l,  lse = m + ln l
+//
+// Rows: the query heads that share a key/value head are rows of one tile
+// (row r = token r / groups, head r % groups), so a tile of 128 rows reads
+// each key once for all of them.
+//
+// Bound: tensor cores, 4 * head_dim operations per (row, key); beside it the
+// exponentials, one per (row, key) at 16 a clock and SM, which at head_dim 128
+// take as long as the two products (2 x 128 x 128 x 128 multiply-adds in 1024
+// clocks, 128 x 128 exponentials in 1024).
+//
+// One block per SM. Warps by role:
+//
+//   softmax   one warpgroup per S buffer, one thread per row: S from tensor
+//             memory, e^(S - m) back over it as 16-bit P
+//   producer  one warpgroup: Q, K and V tiles into shared memory in the
+//             operands' 128-byte-swizzled layout, 16 bytes per copy. Plain
+//             cp.async rather than tensor copies, since a page may be of any
+//             size down to one token and rows past the end have to be zero;
+//             e4m3 codes are converted on the way (times their power of two:
+//             exact in bf16; in f16 exact but for values below its smallest
+//             subnormal step)
+//   mma       one thread: S = Q K^T into one of two S buffers, O += P V
+//             (P from tensor memory, V as the transposed B operand)
+//
+// head_dim 64 and 128: two tiles of 128 rows in turn ("duo"), so that one
+// tile's softmax runs beside the other's products. Calls whose sequences have
+// at most 128 rows, and head_dim 256 (whose O takes half of tensor memory): one
+// tile, the next keys' S beside the present softmax ("solo").
+//
+// Work: the tiles' key ranges laid end to end and cut evenly over the blocks
+// (attn_plan_kernel finds each block's start from q_starts and kv_lens); a tile
+// cut by a border leaves partial (O, m, l) and the last block to arrive adds
+// them in block order.
+//
+// The maximum is lazy: e^(S - m) is taken with the m of earlier keys, and only
+// where some S exceeds it by more than 8 (in log2) is m raised, O rescaled and
+// P computed again.
 #include "common.cuh"
 #include "internal.h"
+#include "tcgen05.cuh"
 
 namespace b200 {
 namespace {
 
+using namespace tcg;
+
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLazy = 8.f;
+constexpr int kMinTiles = 2;  // a block takes at least this many key tiles
+constexpr uint32_t kTmemCols = 512;
+constexpr uint32_t kTmemO = 256;  // O after the two S buffers of up to 128 columns
 
-__device__ __forceinline__ float load16(const void* base, long long i, int f16) {
-  const uint16_t b = static_cast<const uint16_t*>(base)[i];
-  return f16 ? __half2float(__ushort_as_half(b)) : __bfloat162float(__ushort_as_bfloat16(b));
-}
-__device__ __forceinline__ float load_cached(const AttnLaunch& a, const void* base, long long i) {
-  if (a.cache_dtype != 3) return load16(base, i, a.cache_dtype == 1);
-  const uint32_t h = e4m3x2_to_f16x2(static_cast<const uint8_t*>(base)[i]);
-  return __half2float(__ushort_as_half((uint16_t)h));
-}
-__device__ __forceinline__ float scale_of(uint8_t b) {
-  return b == 255 ? __int_as_float(0x7fc00000) : __uint_as_float((uint32_t)b << 23);
-}
+enum { kBf16 = 0, kF16 = 1, kE4m3Bf16 = 2, kE4m3F16 = 3 };
 
-template <int D>
-__global__ void __launch_bounds__(128) attn_prefill_kernel(const AttnLaunch a) {
-  griddep_wait();
-  constexpr int kPer = D / 32;
-  const int lane = threadIdx.x & 31;
-  const long long id = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const long long token = id / a.q_heads;
-  const int qh = (int)(id - token * a.q_heads);
-  if (token >= a.q_tokens) return;
-  int s = -1;
-  for (int i = 0; i < a.seqs; ++i)
-    if (a.q_starts[i] <= token && token < a.q_starts[i + 1]) s = i;
-  if (s < 0) return;
-  const int q0 = a.q_starts[s], q_len = min(a.q_starts[s + 1] - q0, a.max_q);
-  if (token - q0 >= q_len) return;
-  const long long cap = (long long)a.table_width * a.c.page_size;
-  const int kv = (int)min((long long)max(a.kv_lens[s], 0), cap);
-  const int pos = kv - q_len + (int)(token - q0);
-  const int hi = a.causal ? min(kv, pos + 1) : kv;
-  const int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-  const int head = qh / (a.q_heads / a.c.heads);
-  float q[kPer], o[kPer], m = -INFINITY, l = 0.f;
-  for (int i = 0; i < kPer; ++i) {
-    q[i] = load16(a.q, token * a.q_token_stride + qh * a.q_head_stride + i * 32 + lane, a.q_f16);
-    o[i] = 0.f;
-  }
-  for (int t = lo; t < hi; ++t) {
-    const int page = a.table[s * a.table_stride + t / a.c.page_size], off = t % a.c.page_size;
-    if (page < 0 || page >= a.c.num_pages) {
-      if (lane == 0) atomicOr(a.status, kDevBadPage);
-      l = m == -INFINITY ? 1.f : l + exp2f(-m);
-      if (m == -INFINITY) m = 0.f;
-      continue;
+struct PrefillParams {
+  AttnLaunch a;
+  int groups;
+  int tile_tokens;  // new tokens per 128 rows: 128 / groups
+  float scale_log2;
+  // the plan (attn_plan_kernel), in the scratch
+  long long* head;  // [0] tiles in all, [1] blocks
+  int4* start;      // per block: unit, head, tile of its first key tile
+  int* seq_base;    // units before each sequence
+  int4* units;      // sequence, first token in it, first key, key tiles
+  int max_units;
+  float* parts;
+};
+
+template <int D, int MT>
+struct Shape {
+  static constexpr int kBN = D == 256 ? 64 : 128;  // keys per tile
+  static constexpr int kSlices = D / 64;
+  static constexpr int kQSlice = 128 * 128;         // bytes: 128 rows x 64 columns
+  static constexpr int kKvSlice = kBN * 128;
+  static constexpr int kQBytes = MT * kSlices * kQSlice;
+  static constexpr int kTileBytes = kSlices * kKvSlice;
+  static constexpr int kRoom = 227 * 1024 - 2048 - 1024 - 4 * kBN * 16 - kQBytes;
+  static constexpr int kFit = kRoom / kTileBytes;
+  static constexpr int kStages = kFit > 8 ? 8 : kFit;
+  static constexpr int kThreads = (MT + 1) * 128 + 32;
+  static constexpr int kOffRing = kQBytes;
+  static constexpr int kOffTable = kOffRing + kStages * kTileBytes;
+  static constexpr int kOffCtl = kOffTable + 4 * kBN * 16;
+  static constexpr size_t kSmem = kOffCtl + 2048 + 1024;
+};
+
+// What the producer knows about a key row: byte offset of its vector (-1: none)
+// and its scales as 16-bit factors.
+struct __align__(16) RowInfo {
+  long long off;
+  uint32_t k_factor, v_factor;  // e4m3: two copies of the factor
+};
+
+struct Ctl {
+  uint64_t full[8], empty[8];
+  uint64_t q_full, q_empty;
+  uint64_t s_full[2], p_ready[2], pv_done[2];
+  uint64_t drained;
+  uint32_t tmem;
+  int abort;
+  int flag[2];
+};
+
+// Bounded wait. A role that gives up sets the block's abort flag; from then on
+// no wait waits, so every role runs through its loops (and block barriers) and
+// the block ends with the status bit set.
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, Ctl* ctl, int* status) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const unsigned long long t0 = global_timer_ns();
+  for (uint32_t i = 1;; ++i) {
+    if (*reinterpret_cast<volatile int*>(&ctl->abort)) return false;
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 255u) == 0u && global_timer_ns() - t0 > kWaitLimitNs) {
+      atomicOr(status, kDevWaitTimeout);
+      *reinterpret_cast<volatile int*>(&ctl->abort) = 1;
+      return false;
     }
-    const long long at = page * a.c.page_stride + off * a.c.token_stride + head * a.c.head_stride;
-    const long long sat = page * a.c.scale_page_stride + off * a.c.scale_token_stride +
-                          head * a.c.scale_head_stride;
-    float x = 0.f;
-    for (int i = 0; i < kPer; ++i) x += q[i] * load_cached(a, a.c.k, at + i * 32 + lane);
-    for (int d = 16; d > 0; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
-    if (a.cache_dtype == 3) x *= scale_of(a.c.k_scale[sat]);
-    x *= a.scale * kLog2e;
-    const float mn = fmaxf(m, x), f = exp2f(m - mn), p = exp2f(x - mn);
-    l = l * f + p;
-    const float ps = a.cache_dtype == 3 ? p * scale_of(a.c.v_scale[sat]) : p;
-    for (int i = 0; i < kPer; ++i) o[i] = o[i] * f + ps * load_cached(a, a.c.v, at + i * 32 + lane);
-    m = mn;
   }
-  for (int i = 0; i < kPer; ++i) {
-    const float v = l == 0.f ? 0.f : o[i] / l;
-    const long long at = token * a.out_token_stride + qh * a.out_head_stride + i * 32 + lane;
-    static_cast<uint16_t*>(a.out)[at] = a.q_f16 ? __half_as_ushort(__float2half_rn(v))
-                                                : __bfloat16_as_ushort(__float2bfloat16_rn(v));
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+template <bool F16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  uint32_t r;
+  if (F16)
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// Completes the tensor-memory loads into r (the operands tie their uses to the wait).
+__device__ __forceinline__ void tmem_wait32(uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.wait::ld.sync.aligned;"
+      : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]),
+        "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]),
+        "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]),
+        "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]),
+        "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
+}
+
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
+      "%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
+      "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]),
+      "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]),
+      "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+// A K-major or (mn_stride > 0) MN-major operand, 128-byte swizzle: 8 lines of
+// 128 B per atom, atoms 1024 B apart; blocks of 64 MN elements mn_stride apart.
+__device__ __forceinline__ uint64_t smem_desc(uint32_t saddr, uint32_t mn_stride) {
+  uint64_t d = smem_desc_sw128(saddr);
+  if (mn_stride) {
+    d &= ~((uint64_t)0x3fffu << 16);
+    d |= (uint64_t)(mn_stride >> 4) << 16;
   }
-  if (a.lse != nullptr && lane == 0)
-    a.lse[token * a.q_heads + qh] = l == 0.f ? -INFINITY : m / kLog2e + logf(l);
+  return d;
+}
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                       uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      "  .reg .pred p;\n"
+      "  setp.ne.b32 p, %4, 0;\n"
+      "  tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
+      "}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+                                       uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      "  .reg .pred p;\n"
+      "  setp.ne.b32 p, %4, 0;\n"
+      "  tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+      "}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// fp32 accumulator, both operands f16 or bf16, M = 128.
+__device__ __forceinline__ uint32_t instr_desc(bool f16, int n, bool b_mn_major) {
+  const uint32_t type = f16 ? 0u : 1u;
+  return 1u << 4 | type << 7 | type << 10 | (b_mn_major ? 1u << 16 : 0u) |
+         (uint32_t)(n >> 3) << 17 | (128u >> 4) << 24;
+}
+
+__device__ __forceinline__ void fence_async_smem() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+__device__ __forceinline__ void cp_async_16_zfill(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+               "r"(on ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() {
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+__device__ __forceinline__ void st_shared_u128(uint32_t dst, uint4 v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z),
+               "r"(v.w)
+               : "memory");
+}
+
+// Four e4m3 codes times a 16-bit power of two (two copies in `factor`).
+// bf16: a code's bits moved to bf16's exponent and mantissa fields read 2^-120
+// of its value (subnormals included); the factor holds 2^(120 + e).
+template <bool F16>
+__device__ __forceinline__ uint2 convert4(uint32_t w, uint32_t factor) {
+  uint2 r;
+  if (F16) {
+    r.x = hmul2_u32(e4m3x2_to_f16x2((uint16_t)w), factor);
+    r.y = hmul2_u32(e4m3x2_to_f16x2((uint16_t)(w >> 16)), factor);
+  } else {
+    const uint32_t lo = __byte_perm(w, 0, 0x1404), hi = __byte_perm(w, 0, 0x3424);
+    const uint32_t a = (lo & 0x80008000u) | ((lo >> 4) & 0x07f007f0u);
+    const uint32_t b = (hi & 0x80008000u) | ((hi >> 4) & 0x07f007f0u);
+    const __nv_bfloat162 f = *reinterpret_cast<const __nv_bfloat162*>(&factor);
+    const __nv_bfloat162 x = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), f);
+    const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&b), f);
+    r.x = *reinterpret_cast<const uint32_t*>(&x);
+    r.y = *reinterpret_cast<const uint32_t*>(&y);
+  }
+  return r;
+}
+// The factor of a scale byte (127 + e), for convert4.
+template <bool F16>
+__device__ __forceinline__ uint32_t factor_of(uint32_t byte) {
+  uint32_t h;
+  if (F16)
+    h = byte == 255u ? 0x7e00u
+                     : __half_as_ushort(__float2half_rn(__uint_as_float(byte << 23)));
+  else  // bf16 exponent field 127 + 120 + e, at most 254
+    h = byte == 255u ? 0x7fc0u : min(byte + 120u, 254u) << 7;
+  return h | h << 16;
+}
+
+// ------------------------------------------------------------------- plan
+// New tokens and cached tokens of a sequence, within the call's bounds.
+struct SeqLens {
+  int q0, q_len, kv_len;
+};
+__device__ __forceinline__ SeqLens seq_lens(const AttnLaunch& a, int s) {
+  SeqLens r;
+  const int q0 = __ldg(a.q_starts + s), q1 = __ldg(a.q_starts + s + 1);
+  const long long cap = (long long)a.table_width * a.c.page_size;
+  int kv = max(__ldg(a.kv_lens + s), 0);
+  if (kv > cap) kv = (int)cap;
+  int n = q1 - q0;
+  if (q0 < 0 || q1 > a.q_tokens) n = 0;  // outside q: nothing is read or written
+  r.q0 = q0;
+  r.q_len = min(max(n, 0), a.max_q);
+  r.kv_len = kv;
+  return r;
+}
+
+constexpr int kPlanThreads = 1024;
+
+__device__ long long block_scan(long long v, long long* sh, long long& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();
+  if (lane == 31) sh[warp] = x;
+  __syncthreads();
+  if (warp == 0) {
+    long long t = sh[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, t, o);
+      if (lane >= o) t += y;
+    }
+    sh[lane] = t;
+  }
+  __syncthreads();
+  total = sh[31];
+  return x - v + (warp ? sh[warp - 1] : 0);
+}
+
+// One block: the units (sequence, rows of unit_tokens tokens) with their key
+// ranges, and where in the flattened (unit, head, key tile) space each block of
+// the attention kernel starts.
+__global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const PrefillParams p,
+                                                                 int unit_tokens, int bn,
+                                                                 int max_ctas) {
+  __shared__ long long sh[32];
+  griddep_wait();
+  const AttnLaunch& a = p.a;
+  const int tid = threadIdx.x;
+  long long total_units, total;
+  {
+    const int per = (a.seqs + kPlanThreads - 1) / kPlanThreads;
+    const int s0 = min(tid * per, a.seqs), s1 = min(s0 + per, a.seqs);
+    long long n = 0;
+    for (int s = s0; s < s1; ++s) n += (seq_lens(a, s).q_len + unit_tokens - 1) / unit_tokens;
+    long long base = block_scan(n, sh, total_units);
+    for (int s = s0; s < s1; ++s) {
+      p.seq_base[s] = (int)base;
+      base += (seq_lens(a, s).q_len + unit_tokens - 1) / unit_tokens;
+    }
+    if (tid == 0) p.seq_base[a.seqs] = (int)total_units;
+  }
+  __syncthreads();
+  // q_starts that ascend within q_tokens give at most max_units.
+  const int units = (int)min(total_units, (long long)p.max_units);
+  const int per = (units + kPlanThreads - 1) / kPlanThreads;
+  const int u0 = min(tid * per, units), u1 = min(u0 + per, units);
+  long long mine = 0;
+  if (u0 < u1) {
+    int lo = 0, hi = a.seqs - 1;  // last sequence whose base is <= u0
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (p.seq_base[mid] <= u0)
+        lo = mid;
+      else
+        hi = mid - 1;
+    }
+    int s = lo;
+    SeqLens q = seq_lens(a, s);
+    for (int u = u0; u < u1; ++u) {
+      while (s + 1 < a.seqs && p.seq_base[s + 1] <= u) q = seq_lens(a, ++s);
+      const int tok0 = (u - p.seq_base[s]) * unit_tokens;
+      const int last = min(tok0 + unit_tokens, q.q_len) - 1;
+      const int shift = q.kv_len - q.q_len;
+      int end = a.causal ? min(q.kv_len, shift + last + 1) : q.kv_len;
+      int begin = a.window > 0 ? max(0, shift + tok0 - a.window + 1) : 0;
+      const int tiles = end > begin ? (end - begin + bn - 1) / bn : 1;
+      p.units[u] = make_int4(s, tok0, begin, tiles);
+      mine += (long long)tiles * a.c.heads;
+    }
+  }
+  long long at = block_scan(mine, sh, total);
+  long long ctas = (total + kMinTiles - 1) / kMinTiles;
+  if (ctas > max_ctas) ctas = max_ctas;
+  if (tid == 0) {
+    p.head[0] = total;
+    p.head[1] = ctas;
+  }
+  for (int u = u0; u < u1; ++u) {
+    const long long n = (long long)p.units[u].w * a.c.heads;
+    // blocks whose first tile floor(total * c / ctas) lies in [at, at + n)
+    for (long long c = (at * ctas + total - 1) / total; c < ctas; ++c) {
+      const long long t0 = total * c / ctas;
+      if (t0 >= at + n) break;
+      const int h = (int)((t0 - at) / p.units[u].w);
+      p.start[c] = make_int4(u, h, (int)(t0 - at - (long long)h * p.units[u].w), 0);
+    }
+    at += n;
+  }
+  griddep_launch_dependents();
+}
+
+// ---------------------------------------------------------------- attention
+// The segments of a block: runs of key tiles of one (unit, head).
+struct Segment {
+  int unit, head;
+  int seq, tok0, begin;   // from the plan
+  int tile0, tiles;       // this block's key tiles of the pair
+  int unit_tiles;
+  long long at;           // flattened index of tile0
+};
+struct Cursor {
+  const PrefillParams* p;
+  int unit, head, tile;
+  long long at, end;
+  __device__ void start(const PrefillParams& pp, long long t0, long long t1) {
+    p = &pp;
+    const int4 s = __ldcg(pp.start + blockIdx.x);
+    unit = s.x, head = s.y, tile = s.z;
+    at = t0, end = t1;
+  }
+  __device__ bool next(Segment& g) {
+    if (at >= end) return false;
+    const int4 u = __ldcg(p->units + unit);
+    g.unit = unit, g.head = head;
+    g.seq = u.x, g.tok0 = u.y, g.begin = u.z, g.unit_tiles = u.w;
+    g.tile0 = tile;
+    g.at = at;
+    const long long left = end - at;
+    g.tiles = u.w - tile < left ? u.w - tile : (int)left;
+    at += g.tiles;
+    tile = 0;
+    if (++head == p->a.c.heads) {
+      head = 0;
+      ++unit;
+    }
+    return true;
+  }
+};
+
+// One pass over a row's S in tensor memory: P = 2^(s * scale - m) packed, the
+// largest exponent (relative to m) and the sum. P == nullptr-like MAX_ONLY: the
+// largest s * scale only.
+template <int BN, bool F16, bool MASK, bool MAX_ONLY>
+__device__ __forceinline__ void softmax_pass(uint32_t ts, float scale, float m, int col0, int lo,
+                                             int hi, uint32_t* pk, float& top, float& sum) {
+  float mx0 = -INFINITY, mx1 = -INFINITY, sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+  for (int c = 0; c < BN / 32; ++c) {
+    uint32_t s[32];
+    tmem_ld32_nowait(ts + 32 * c, s);
+    tmem_wait32(s);
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+      float x = fmaf(__uint_as_float(s[i]), scale, -m);
+      float y = fmaf(__uint_as_float(s[i + 1]), scale, -m);
+      if (MASK) {
+        const int col = col0 + 32 * c + i;
+        x = col >= lo && col < hi ? x : -INFINITY;
+        y = col + 1 >= lo && col + 1 < hi ? y : -INFINITY;
+      }
+      mx0 = fmaxf(mx0, x);
+      mx1 = fmaxf(mx1, y);
+      if (!MAX_ONLY) {
+        x = ex2(x);
+        y = ex2(y);
+        sum0 += x;
+        sum1 += y;
+        pk[16 * c + i / 2] = pack2<F16>(x, y);
+      }
+    }
+  }
+  top = fmaxf(mx0, mx1);
+  sum = sum0 + sum1;
+}
+
+template <int D, int MT, int KV>
+__global__ void __launch_bounds__(Shape<D, MT>::kThreads, 1)
+    attn_prefill_kernel(const PrefillParams p) {
+  using S = Shape<D, MT>;
+  constexpr int BN = S::kBN;
+  constexpr bool kHalf = KV == kF16 || KV == kE4m3F16;  // operand type f16
+  constexpr bool kQuant = KV >= kE4m3Bf16;
+  constexpr int kProducer = MT * 4, kMma = MT * 4 + 4;  // first warps of the roles
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  uint8_t* smem = smem_raw + ((1024u - (raw & 1023u)) & 1023u);
+  const uint32_t sq = smem_u32(smem), ring = sq + S::kOffRing;
+  RowInfo* table = reinterpret_cast<RowInfo*>(smem + S::kOffTable);
+  Ctl* ctl = reinterpret_cast<Ctl*>(smem + S::kOffCtl);
+  const AttnLaunch& a = p.a;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  if (tid == 0) {
+    for (int i = 0; i < S::kStages; ++i) {
+      mbar_init(&ctl->full[i], 128);
+      mbar_init(&ctl->empty[i], 1);
+    }
+    mbar_init(&ctl->q_full, 128);
+    mbar_init(&ctl->q_empty, 1);
+    mbar_init(&ctl->drained, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&ctl->s_full[i], 1);
+      mbar_init(&ctl->p_ready[i], 128);
+      mbar_init(&ctl->pv_done[i], 1);
+    }
+    ctl->abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == kMma) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(&ctl->tmem)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&ctl->tmem);
+  griddep_wait();
+  const long long total = __ldcg(p.head), ctas = __ldcg(p.head + 1);
+  const bool on = blockIdx.x < ctas;
+  const long long t0 = on ? total * blockIdx.x / ctas : 0;
+  const long long t1 = on ? total * (blockIdx.x + 1) / ctas : 0;
+  Cursor cur;
+  if (on) cur.start(p, t0, t1);
+  Segment g;
+  if (!on) {
+    // nothing: the block only gives its tensor memory back
+  } else if (warp < kProducer) {
+    // ------------------------------------------------------------- softmax
+    const int wg = warp >> 2;                       // S buffer's tile (duo)
+    const int row = (warp & 3) * 32 + lane;         // row of the tile
+    const uint32_t lane_addr = tmem + ((uint32_t)(warp & 3) << 21);
+    const int row_token = row / p.groups, row_head = row % p.groups;
+    uint32_t step = 0;                              // S tiles of this warpgroup so far
+    uint64_t* pv_done = &ctl->pv_done[MT == 2 ? wg : 0];  // one phase per step
+    while (cur.next(g)) {
+      const SeqLens q = seq_lens(a, g.seq);
+      const int tok = g.tok0 + wg * p.tile_tokens + row_token;
+      const bool valid = row < p.tile_tokens * p.groups && tok < q.q_len &&
+                         tok < g.tok0 + MT * p.tile_tokens;
+      const int pos = q.kv_len - q.q_len + tok;
+      const int hi = !valid ? 0 : a.causal ? min(q.kv_len, pos + 1) : q.kv_len;
+      const int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+      // a row that sees nothing needs no maximum: every key is masked
+      float m = hi > lo ? -INFINITY : 0.f, l = 0.f;
+      const uint32_t to = lane_addr + kTmemO + (MT == 2 ? wg * D : 0);
+      for (int k = 0; k < g.tiles; ++k, ++step) {
+        const int buf = MT == 2 ? wg : (int)(step & 1u);
+        const uint32_t phase = MT == 2 ? step & 1u : (step >> 1) & 1u;
+        const uint32_t ts = lane_addr + buf * 128;
+        const int col0 = g.begin + (g.tile0 + k) * BN;
+        wait_bar(&ctl->s_full[buf], phase, ctl, a.status);
+        __syncwarp();
+        tc_fence_after();
+        const bool masked = __any_sync(0xffffffffu, col0 < lo || col0 + BN > hi);
+        uint32_t pk[BN / 2];
+        float top = 0.f, sum = 0.f;
+        bool redo = __any_sync(0xffffffffu, m == -INFINITY);
+        if (!redo) {
+          if (masked)
+            softmax_pass<BN, kHalf, true, false>(ts, p.scale_log2, m, col0, lo, hi, pk, top, sum);
+          else
+            softmax_pass<BN, kHalf, false, false>(ts, p.scale_log2, m, col0, lo, hi, pk, top, sum);
+          redo = __any_sync(0xffffffffu, top > kLazy);
+        }
+        if (redo) {
+          softmax_pass<BN, kHalf, true, true>(ts, p.scale_log2, 0.f, col0, lo, hi, pk, top, sum);
+          const float mn = m == -INFINITY || top > m + kLazy ? top : m;
+          const float f = m == mn || m == -INFINITY ? 1.f : ex2(m - mn);
+          if (k > 0 && __any_sync(0xffffffffu, f != 1.f)) {
+            // the product before this one may still be adding to O
+            wait_bar(pv_done, (step - 1) & 1u, ctl, a.status);
+            __syncwarp();
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t o[32];
+              tmem_ld32_nowait(to + 32 * c, o);
+              tmem_wait32(o);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+              tmem_st32(to + 32 * c, o);
+            }
+            tmem_st_wait();
+          }
+          l *= f;
+          m = mn;
+          const float base = m == -INFINITY ? 0.f : m;
+          softmax_pass<BN, kHalf, true, false>(ts, p.scale_log2, base, col0, lo, hi, pk, top, sum);
+        }
+        l += sum;
+#pragma unroll
+        for (int c = 0; c < BN / 64; ++c) tmem_st32(ts + 32 * c, pk + 32 * c);
+        tmem_st_wait();
+        // Solo: the S that was waited for came before the previous product, so
+        // that product is waited for here; no wait is then ever two phases
+        // behind. (Duo: this S came after it.) It has had the whole softmax.
+        if (MT == 1 && k > 0) wait_bar(pv_done, (step - 1) & 1u, ctl, a.status);
+        tc_fence_before();
+        mbar_arrive(&ctl->p_ready[buf]);
+      }
+      // -- the last product, then O out
+      wait_bar(pv_done, (step - 1) & 1u, ctl, a.status);
+      __syncwarp();
+      tc_fence_after();
+      const long long u0 = g.at - g.tile0, u1 = u0 + g.unit_tiles;
+      const bool whole = u0 >= t0 && u1 <= t1;
+      const long long token = (long long)q.q0 + tok;
+      const int qh = g.head * p.groups + row_head;
+      uint16_t* dst = static_cast<uint16_t*>(a.out) + token * a.out_token_stride +
+                      (long long)qh * a.out_head_stride;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      constexpr long long kPart = (long long)(D + 2) * 128;  // floats of a tile's partial
+      float* part = p.parts + ((2ll * blockIdx.x + (u0 >= t0 ? 1 : 0)) * MT + wg) * kPart + row;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        tmem_ld32_nowait(to + 32 * c, o);
+        tmem_wait32(o);
+        if (whole) {
+          if (valid) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+              uint4 v;
+              uint32_t* w = &v.x;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                // O of a row without keys is the sum of nothing but zeros
+                const float x = __uint_as_float(o[i + 2 * j]) * inv;
+                const float y = __uint_as_float(o[i + 2 * j + 1]) * inv;
+                w[j] = a.q_f16 ? pack2<true>(x, y) : pack2<false>(x, y);
+              }
+              *reinterpret_cast<uint4*>(dst + 32 * c + i) = v;
+            }
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) part[(2 + 32 * c + i) * 128] = __uint_as_float(o[i]);
+        }
+      }
+      if (whole) {
+        if (valid && a.lse != nullptr)
+          a.lse[token * a.q_heads + qh] = l == 0.f ? -INFINITY : (m + log2f(l)) / kLog2e;
+        continue;
+      }
+      part[0] = l == 0.f ? -INFINITY : m;
+      part[128] = l;
+      const int c_first = (int)(((u0 + 1) * ctas - 1) / total);
+      const int c_last = (int)((u1 * ctas - 1) / total);
+      __threadfence();
+      named_bar_sync(2 + wg, 128);
+      if ((tid & 127) == 0) {
+        int* counter = a.counters + 2 * c_first + wg;
+        const bool last = atomicAdd(counter, 1) == c_last - c_first;
+        if (last) *counter = 0;
+        ctl->flag[wg] = last;
+        __threadfence();
+      }
+      named_bar_sync(2 + wg, 128);
+      const bool last = *reinterpret_cast<volatile int*>(&ctl->flag[wg]) != 0;
+      named_bar_sync(2 + wg, 128);  // the flag may be written again
+      if (last && valid) {
+      const float* parts = p.parts + row;
+      auto part_at = [&](int b) {
+        return parts + ((2ll * b + (b == c_first ? 1 : 0)) * MT + wg) * kPart;
+      };
+      float mx = -INFINITY, sum = 0.f;
+      for (int b = c_first; b <= c_last; ++b) mx = fmaxf(mx, __ldcg(part_at(b)));
+      for (int b = c_first; b <= c_last; ++b) {
+        const float mb = __ldcg(part_at(b)), lb = __ldcg(part_at(b) + 128);
+        sum += mb == -INFINITY ? lb : lb * ex2(mb - mx);
+      }
+      const float inv_sum = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        float acc[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) acc[i] = 0.f;
+        for (int b = c_first; b <= c_last; ++b) {
+          const float* src = part_at(b);
+          const float mb = __ldcg(src);
+          const float w = mb == -INFINITY ? 0.f : ex2(mb - mx);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const float v = __ldcg(src + (2 + 32 * c + i) * 128);
+            acc[i] += w == 0.f ? 0.f : v * w;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 32; i += 8) {
+          uint4 v;
+          uint32_t* w = &v.x;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float x = acc[i + 2 * j] * inv_sum, y = acc[i + 2 * j + 1] * inv_sum;
+            w[j] = a.q_f16 ? pack2<true>(x, y) : pack2<false>(x, y);
+          }
+          *reinterpret_cast<uint4*>(dst + 32 * c + i) = v;
+        }
+      }
+      if (a.lse != nullptr)
+        a.lse[token * a.q_heads + qh] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) / kLog2e;
+      }
+      __syncwarp();
+    }
+  } else if (warp < kMma) {
+    // ------------------------------------------------------------ producer
+    const int pt = tid - kProducer * 32;  // 0..127
+    uint32_t stage = 0, fill = 0;         // ring position and pass
+    uint32_t q_count = 0;
+    constexpr int kElem = kQuant ? 1 : 2;
+    constexpr int kRowBytes = D * kElem;
+    constexpr int kChunks = kRowBytes / 16;           // 16-byte reads per key row
+    constexpr int kPer = BN * kChunks / 128;          // of them per thread and tile
+    const int p_row = pt / kChunks, p_chunk = pt % kChunks;
+    constexpr int kRowStep = 128 / kChunks;
+
+    while (cur.next(g)) {
+      const SeqLens q = seq_lens(a, g.seq);
+      const int end = q.kv_len;
+      const int* pages = a.table + g.seq * a.table_stride;
+      // -- row information, two tiles ahead: page number, then offset and scales
+      auto page_of = [&](int t) -> int {  // this thread's row of key tile t
+        const int token = g.begin + (g.tile0 + t) * BN + pt;
+        return t < g.tiles && pt < BN && token < end ? __ldg(pages + token / a.c.page_size) : -1;
+      };
+      auto info_of = [&](int t, int page) {
+        RowInfo r;
+        r.off = -1;
+        r.k_factor = r.v_factor = 0;
+        const int token = g.begin + (g.tile0 + t) * BN + pt;
+        if (t < g.tiles && pt < BN && token < end) {
+          if (page < 0 || page >= a.c.num_pages) {
+            atomicOr(a.status, kDevBadPage);
+          } else {
+            const int at = token % a.c.page_size;
+            r.off = (page * a.c.page_stride + at * a.c.token_stride +
+                     g.head * a.c.head_stride) * kElem;
+            if (kQuant) {
+              const long long so = page * a.c.scale_page_stride + at * a.c.scale_token_stride +
+                                   g.head * a.c.scale_head_stride;
+              r.k_factor = __ldg(a.c.k_scale + so);
+              r.v_factor = __ldg(a.c.v_scale + so);
+            }
+          }
+        }
+        return r;
+      };
+      auto store_info = [&](int t, RowInfo r) {
+        if (pt < BN) {
+          if (kQuant && r.off >= 0) {
+            r.k_factor = factor_of<kHalf>(r.k_factor);
+            r.v_factor = factor_of<kHalf>(r.v_factor);
+          }
+          table[(t & 3) * BN + pt] = r;
+        }
+      };
+      RowInfo info = info_of(0, page_of(0));
+      int page1 = page_of(1);
+      // -- Q
+      wait_bar(&ctl->q_empty, (q_count & 1u) ^ 1u, ctl, a.status);
+      ++q_count;
+      {
+        constexpr int kQChunks = D / 8;
+        const int chunk = pt % kQChunks;
+#pragma unroll 4
+        for (int r = pt / kQChunks; r < MT * 128; r += 128 / kQChunks) {
+          const int tile = r >> 7, rr = r & 127;
+          const int tok = g.tok0 + tile * p.tile_tokens + rr / p.groups;
+          const bool valid = rr < p.tile_tokens * p.groups && tok < q.q_len;
+          const uint16_t* src =
+              static_cast<const uint16_t*>(a.q) +
+              (valid ? (q.q0 + tok) * a.q_token_stride +
+                           (long long)(g.head * p.groups + rr % p.groups) * a.q_head_stride + chunk * 8
+                     : 0);
+          const uint32_t dst = sq + (tile * S::kSlices + chunk / 8) * S::kQSlice + rr * 128 +
+                               (((chunk & 7) ^ (rr & 7)) << 4);
+          cp_async_16_zfill(dst, src, valid);
+        }
+        cp_async_arrive_noinc(&ctl->q_full);
+      }
+      store_info(0, info);
+      named_bar_sync(1, 128);
+      // -- keys and values, in the order the products take them:
+      // duo K0 V0 K1 V1 ..., solo K0 K1 V0 K2 V1 ... V(n-1)
+      uint4 held[kQuant ? kPer : 1];  // e4m3: the loads of the copy in progress
+      auto copy = [&](int t, bool is_v) {
+        wait_bar(&ctl->empty[stage], (fill & 1u) ^ 1u, ctl, a.status);
+        const uint32_t dst0 = ring + stage * S::kTileBytes;
+        const uint8_t* base = static_cast<const uint8_t*>(is_v ? a.c.v : a.c.k) + p_chunk * 16;
+        const RowInfo* rows = table + (t & 3) * BN;
+        if (!kQuant) {
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) {
+            const int r = p_row + i * kRowStep;
+            const long long off = rows[r].off;
+            const uint32_t dst = dst0 + (p_chunk / 8) * S::kKvSlice + r * 128 +
+                                 (((p_chunk & 7) ^ (r & 7)) << 4);
+            cp_async_16_zfill(dst, base + (off < 0 ? 0 : off), off >= 0);
+          }
+          cp_async_arrive_noinc(&ctl->full[stage]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) {
+            const long long off = rows[p_row + i * kRowStep].off;
+            held[i] = off < 0 ? make_uint4(0u, 0u, 0u, 0u)
+                              : __ldg(reinterpret_cast<const uint4*>(base + off));
+          }
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) {
+            const int r = p_row + i * kRowStep;
+            const uint32_t f = is_v ? rows[r].v_factor : rows[r].k_factor;
+            const uint2 x = convert4<kHalf>(held[i].x, f), y = convert4<kHalf>(held[i].y, f);
+            const uint2 z = convert4<kHalf>(held[i].z, f), w = convert4<kHalf>(held[i].w, f);
+            // 16 columns: chunks 2c and 2c + 1 of the 16-bit row
+            const int c2 = 2 * p_chunk;
+            const uint32_t dst = dst0 + (c2 / 8) * S::kKvSlice + r * 128;
+            st_shared_u128(dst + (((c2 & 7) ^ (r & 7)) << 4), make_uint4(x.x, x.y, y.x, y.y));
+            st_shared_u128(dst + ((((c2 & 7) + 1) ^ (r & 7)) << 4), make_uint4(z.x, z.y, w.x, w.y));
+          }
+          mbar_arrive(&ctl->full[stage]);
+        }
+        if (++stage == S::kStages) {
+          stage = 0;
+          ++fill;
+        }
+      };
+      for (int t = 0; t < g.tiles; ++t) {
+        const RowInfo next = info_of(t + 1, page1);
+        page1 = page_of(t + 2);
+        copy(t, false);
+        if (MT == 2)
+          copy(t, true);
+        else if (t > 0)
+          copy(t - 1, true);
+        store_info(t + 1, next);
+        named_bar_sync(1, 128);
+      }
+      if (MT == 1) copy(g.tiles - 1, true);
+      // the table's entries are this segment's: all have read them
+      named_bar_sync(1, 128);
+    }
+    cp_async_wait_all();
+  } else if (warp == kMma && elect_one()) {
+    // ----------------------------------------------------------------- mma
+    const uint32_t id_s = instr_desc(kHalf, BN, false), id_o = instr_desc(kHalf, D, true);
+    uint32_t stage = 0, fill = 0;      // next ring entry to consume
+    uint32_t s_count = 0, p_count = 0; // S tiles issued, P tiles consumed (all segments)
+    uint32_t q_count = 0;
+    bool ok = true;
+    // Waits for the next ring entry. The copies are plain writes to shared
+    // memory, the products read it through the async proxy: the fence orders them.
+    auto take = [&]() -> uint32_t {
+      ok = wait_bar(&ctl->full[stage], fill & 1u, ctl, a.status);
+      fence_async_smem();
+      return stage;
+    };
+    auto advance = [&]() {
+      if (++stage == S::kStages) {
+        stage = 0;
+        ++fill;
+      }
+    };
+    while (ok && cur.next(g)) {
+      ok = wait_bar(&ctl->q_full, q_count & 1u, ctl, a.status);
+      if (!ok) break;
+      fence_async_smem();
+      ++q_count;
+      const int steps = MT * g.tiles;
+      uint32_t k_stage = 0, v_stage = 0;
+      auto issue_s = [&](int i) {
+        if (MT == 1 || (i & 1) == 0) {
+          k_stage = take();
+          advance();
+          if (!ok) return;
+        }
+        tc_fence_after();
+        const int buf = MT == 2 ? i & 1 : (int)(s_count & 1u);
+        const uint32_t qa = sq + (MT == 2 ? (i & 1) * S::kSlices * S::kQSlice : 0);
+        const uint32_t ka = ring + k_stage * S::kTileBytes;
+#pragma unroll
+        for (int sl = 0; sl < S::kSlices; ++sl)
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            mma_ss(tmem + buf * 128, smem_desc(qa + sl * S::kQSlice + kk * 32, 0),
+                   smem_desc(ka + sl * S::kKvSlice + kk * 32, 0), id_s, sl + kk > 0);
+        mma_commit(&ctl->s_full[buf]);
+        if (MT == 1 || (i & 1)) mma_commit(&ctl->empty[k_stage]);
+        if (i == steps - 1) mma_commit(&ctl->q_empty);
+        ++s_count;
+      };
+      issue_s(0);
+      if (ok && steps > 1) issue_s(1);
+      for (int i = 0; i < steps && ok; ++i) {
+        const int buf = MT == 2 ? i & 1 : (int)(p_count & 1u);
+        if (MT == 1 || (i & 1) == 0) {
+          v_stage = take();
+          advance();
+          if (!ok) break;
+        }
+        ok = wait_bar(&ctl->p_ready[buf], (p_count >> 1) & 1u, ctl, a.status);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t va = ring + v_stage * S::kTileBytes;
+        const uint32_t to = tmem + kTmemO + (MT == 2 ? (i & 1) * D : 0);
+#pragma unroll
+        for (int kk = 0; kk < BN / 16; ++kk)
+          mma_ts(to, tmem + buf * 128 + kk * 8, smem_desc(va + kk * 2048, S::kKvSlice), id_o,
+                 i >= MT || kk > 0);
+        mma_commit(&ctl->pv_done[MT == 2 ? i & 1 : 0]);
+        if (MT == 1 || (i & 1)) mma_commit(&ctl->empty[v_stage]);
+        ++p_count;
+        if (i + 2 < steps) issue_s(i + 2);
+      }
+    }
+    // Everything issued has finished, and every commit has arrived, before the
+    // block gives its memories back.
+    mma_commit(&ctl->drained);
+    mbar_wait(&ctl->drained, 0, a.status);
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMma) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                 "r"(kTmemCols)
+                 : "memory");
+  }
+  griddep_launch_dependents();
+}
+
+long long align256(long long v) { return (v + 255) / 256 * 256; }
+
+// Units at the smallest unit of tokens that any call makes: one token.
+long long max_units(long long q_tokens, int seqs, int unit_tokens) {
+  return q_tokens / unit_tokens + seqs;
+}
+
+template <int D, int MT, int KV>
+cudaError_t launch(const PrefillParams& p, cudaStream_t stream) {
+  using S = Shape<D, MT>;
+  static bool configured[64] = {};
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err != cudaSuccess) return err;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (!configured[dev]) {
+    err = cudaFuncSetAttribute(attn_prefill_kernel<D, MT, KV>,
+                               cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem);
+    if (err != cudaSuccess) return err;
+    configured[dev] = true;
+  }
+  static_assert(S::kSmem <= 227 * 1024 && S::kStages >= 4, "shared memory");
+  static_assert(sizeof(Ctl) <= 2048, "control block");
+  const int sms = device_sm_count();
+  err = launch_pdl(attn_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, p,
+                   MT * p.tile_tokens, S::kBN, sms);
+  if (err != cudaSuccess) return err;
+  return launch_pdl(attn_prefill_kernel<D, MT, KV>, dim3((unsigned)sms), dim3(S::kThreads),
+                    S::kSmem, stream, p);
+}
+
+template <int D, int MT>
+cudaError_t launch_type(const PrefillParams& p, cudaStream_t stream) {
+  if (p.a.cache_dtype == 3)
+    return p.a.q_f16 ? launch<D, MT, kE4m3F16>(p, stream) : launch<D, MT, kE4m3Bf16>(p, stream);
+  return p.a.q_f16 ? launch<D, MT, kF16>(p, stream) : launch<D, MT, kBf16>(p, stream);
 }
 
 }  // namespace
 
-long long attn_prefill_scratch_bytes(int, long long, int) { return 0; }
+long long attn_prefill_scratch_bytes(int head_dim, long long q_tokens, int seqs) {
+  const long long sms = device_sm_count();
+  return 256 + align256(sms * 16) + align256(4ll * (seqs + 1)) +
+         align256(16 * max_units(q_tokens, seqs, 1)) +
+         sms * 2 * (head_dim == 256 ? 1 : 2) * (head_dim + 2) * 128 * 4;
+}
 
 cudaError_t launch_attn_prefill(const AttnLaunch& l, cudaStream_t stream) {
-  const dim3 grid((unsigned)((l.q_tokens * l.q_heads + 3) / 4)), block(128);
+  PrefillParams p{};
+  p.a = l;
+  p.groups = l.q_heads / l.c.heads;
+  p.tile_tokens = 128 / p.groups;
+  p.scale_log2 = l.scale * kLog2e;
+  const long long sms = device_sm_count();
+  p.max_units = (int)max_units(l.q_tokens, l.seqs, 1);
+  uint8_t* at = l.scratch;
+  p.head = reinterpret_cast<long long*>(at);
+  at += 256;
+  p.start = reinterpret_cast<int4*>(at);
+  at += align256(sms * 16);
+  p.seq_base = reinterpret_cast<int*>(at);
+  at += align256(4ll * (l.seqs + 1));
+  p.units = reinterpret_cast<int4*>(at);
+  at += align256(16ll * p.max_units);
+  p.parts = reinterpret_cast<float*>(at);
+  // Two tiles in turn pay once a sequence fills more than one.
+  const bool duo = (long long)l.max_q * p.groups > 128;
   switch (l.c.head_dim) {
-    case 64: return launch_pdl(attn_prefill_kernel<64>, grid, block, 0, stream, l);
-    case 128: return launch_pdl(attn_prefill_kernel<128>, grid, block, 0, stream, l);
-    default: return launch_pdl(attn_prefill_kernel<256>, grid, block, 0, stream, l);
+    case 64: return duo ? launch_type<64, 2>(p, stream) : launch_type<64, 1>(p, stream);
+    case 128: return duo ? launch_type<128, 2>(p, stream) : launch_type<128, 1>(p, stream);
+    default: return launch_type<256, 1>(p, stream);
   }
 }
 
