@@ -16,15 +16,17 @@
 //
 // One block per SM. Warps by role:
 //
-//   softmax   one warpgroup per S buffer, one thread per row: S from tensor
-//             memory, e^(S - m) back over it as 16-bit P
-//   producer  one warpgroup: Q, K and V tiles into shared memory in the
+//   softmax   one warpgroup per S buffer, one thread per row: the row's maximum
+//             over S in tensor memory, then e^(S - m) back over it as 16-bit P
+//   producer  two warpgroups: Q, K and V tiles into shared memory in the
 //             operands' 128-byte-swizzled layout, 16 bytes per copy. Plain
 //             cp.async rather than tensor copies, since a page may be of any
 //             size down to one token and rows past the end have to be zero;
 //             e4m3 codes are converted on the way (times their power of two:
 //             exact in bf16; in f16 exact but for values below its smallest
 //             subnormal step)
+//   relay     one thread: passes each tile that has landed on to the tensor
+//             core's reads (a proxy fence, off the mma thread's path)
 //   mma       one thread: S = Q K^T into one of two S buffers, O += P V
 //             (P from tensor memory, V as the transposed B operand)
 //
@@ -33,14 +35,14 @@
 // at most 128 rows, and head_dim 256 (whose O takes half of tensor memory): one
 // tile, the next keys' S beside the present softmax ("solo").
 //
-// Work: the tiles' key ranges laid end to end and cut evenly over the blocks
+// Work: the tiles' key ranges laid end to end, with a constant for what each
+// costs besides its key tiles, and cut evenly over the blocks
 // (attn_plan_kernel finds each block's start from q_starts and kv_lens); a tile
 // cut by a border leaves partial (O, m, l) and the last block to arrive adds
 // them in block order.
 //
-// The maximum is lazy: e^(S - m) is taken with the m of earlier keys, and only
-// where some S exceeds it by more than 8 (in log2) is m raised, O rescaled and
-// P computed again.
+// The maximum is lazy: m is raised, and O rescaled, only where some S exceeds it
+// by more than 8 (in log2), so that most tiles leave O alone.
 #include "common.cuh"
 #include "internal.h"
 #include "tcgen05.cuh"
@@ -52,7 +54,10 @@ using namespace tcg;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 8.f;
-constexpr int kMinTiles = 2;  // a block takes at least this many key tiles
+constexpr int kMinTiles = 4;  // a block takes at least this much work, in key tiles
+// What a run of key tiles of one (rows, head) costs beside them, in key tiles:
+// Q in, O out and the pipeline's filling.
+constexpr int kUnitCost = 2;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kTmemO = 256;  // O after the two S buffers of up to 128 columns
 
@@ -64,13 +69,15 @@ struct PrefillParams {
   int tile_tokens;  // new tokens per 128 rows: 128 / groups
   float scale_log2;
   // the plan (attn_plan_kernel), in the scratch
-  long long* head;  // [0] tiles in all, [1] blocks
-  int4* start;      // per block: unit, head, tile of its first key tile
+  long long* head;  // [0] cost in all, [1] blocks
+  int4* start;      // per block: unit, head, place in the unit's cost
   int* seq_base;    // units before each sequence
   int4* units;      // sequence, first token in it, first key, key tiles
   int max_units;
   float* parts;
 };
+
+constexpr int kProducers = 256;
 
 template <int D, int MT>
 struct Shape {
@@ -80,26 +87,33 @@ struct Shape {
   static constexpr int kKvSlice = kBN * 128;
   static constexpr int kQBytes = MT * kSlices * kQSlice;
   static constexpr int kTileBytes = kSlices * kKvSlice;
-  static constexpr int kRoom = 227 * 1024 - 2048 - 1024 - 4 * kBN * 16 - kQBytes;
-  static constexpr int kFit = kRoom / kTileBytes;
+  static constexpr int kTableBytes = 4 * kBN * (16 + 8);
+  static constexpr int kOutBytes = MT * 4 * 2048;   // 32 rows x 32 columns per warp
+  static constexpr int kFixed = kQBytes + kTableBytes + kOutBytes + 2048 + 1024;
+  static constexpr int kFit = (227 * 1024 - kFixed) / kTileBytes;
   static constexpr int kStages = kFit > 8 ? 8 : kFit;
-  static constexpr int kThreads = (MT + 1) * 128 + 32;
+  static constexpr int kThreads = MT * 128 + kProducers + 64;
   static constexpr int kOffRing = kQBytes;
   static constexpr int kOffTable = kOffRing + kStages * kTileBytes;
-  static constexpr int kOffCtl = kOffTable + 4 * kBN * 16;
-  static constexpr size_t kSmem = kOffCtl + 2048 + 1024;
+  static constexpr int kOffOut = kOffTable + kTableBytes;
+  static constexpr int kOffCtl = kOffOut + kOutBytes;
+  static constexpr size_t kSmem = kFixed + kStages * kTileBytes;
 };
 
-// What the producer knows about a key row: byte offset of its vector (-1: none)
-// and its scales as 16-bit factors.
+// What the producer knows about a key row: its vectors, or zeros for a row that
+// does not exist, and (e4m3) its scales as pairs of 16-bit factors.
 struct __align__(16) RowInfo {
-  long long off;
-  uint32_t k_factor, v_factor;  // e4m3: two copies of the factor
+  const uint8_t* k;
+  const uint8_t* v;
 };
+struct __align__(8) RowFactor {
+  uint32_t k, v;
+};
+__device__ uint4 g_zero_row[32];
 
 struct Ctl {
-  uint64_t full[8], empty[8];
-  uint64_t q_full, q_empty;
+  uint64_t landed[8], full[8], empty[8];
+  uint64_t q_landed, q_full, q_empty;
   uint64_t s_full[2], p_ready[2], pv_done[2];
   uint64_t drained;
   uint32_t tmem;
@@ -151,6 +165,15 @@ __device__ __forceinline__ void tmem_wait32(uint32_t (&r)[32]) {
         "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
 }
 
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
+      "%14,%15,%16};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
+      "r"(v[15])
+      : "memory");
+}
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* v) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
@@ -209,10 +232,8 @@ __device__ __forceinline__ uint32_t instr_desc(bool f16, int n, bool b_mn_major)
 __device__ __forceinline__ void fence_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
-__device__ __forceinline__ void cp_async_16_zfill(uint32_t dst, const void* src, bool on) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
-               "r"(on ? 16 : 0)
-               : "memory");
+__device__ __forceinline__ void cp_async_16_at(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_async_wait_all() {
   asm volatile("cp.async.wait_all;" ::: "memory");
@@ -303,8 +324,9 @@ __device__ long long block_scan(long long v, long long* sh, long long& total) {
 }
 
 // One block: the units (sequence, rows of unit_tokens tokens) with their key
-// ranges, and where in the flattened (unit, head, key tile) space each block of
-// the attention kernel starts.
+// ranges, and where in the flattened (unit, head, cost) space each block of the
+// attention kernel starts. A unit's first kUnitCost places stand for its
+// constant cost, the others for one key tile each.
 __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const PrefillParams p,
                                                                  int unit_tokens, int bn,
                                                                  int max_ctas) {
@@ -351,7 +373,7 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const PrefillPa
       int begin = a.window > 0 ? max(0, shift + tok0 - a.window + 1) : 0;
       const int tiles = end > begin ? (end - begin + bn - 1) / bn : 1;
       p.units[u] = make_int4(s, tok0, begin, tiles);
-      mine += (long long)tiles * a.c.heads;
+      mine += (long long)(tiles + kUnitCost) * a.c.heads;
     }
   }
   long long at = block_scan(mine, sh, total);
@@ -362,13 +384,14 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const PrefillPa
     p.head[1] = ctas;
   }
   for (int u = u0; u < u1; ++u) {
-    const long long n = (long long)p.units[u].w * a.c.heads;
+    const int cost = p.units[u].w + kUnitCost;
+    const long long n = (long long)cost * a.c.heads;
     // blocks whose first tile floor(total * c / ctas) lies in [at, at + n)
     for (long long c = (at * ctas + total - 1) / total; c < ctas; ++c) {
       const long long t0 = total * c / ctas;
       if (t0 >= at + n) break;
-      const int h = (int)((t0 - at) / p.units[u].w);
-      p.start[c] = make_int4(u, h, (int)(t0 - at - (long long)h * p.units[u].w), 0);
+      const int h = (int)((t0 - at) / cost);
+      p.start[c] = make_int4(u, h, (int)(t0 - at - (long long)h * cost), 0);
     }
     at += n;
   }
@@ -378,75 +401,130 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const PrefillPa
 // ---------------------------------------------------------------- attention
 // The segments of a block: runs of key tiles of one (unit, head).
 struct Segment {
-  int unit, head;
+  int head;
   int seq, tok0, begin;   // from the plan
   int tile0, tiles;       // this block's key tiles of the pair
   int unit_tiles;
-  long long at;           // flattened index of tile0
+  long long at;           // place of the pair's first cost
 };
 struct Cursor {
   const PrefillParams* p;
-  int unit, head, tile;
+  int unit, head, x;      // x: place in the pair's cost
   long long at, end;
   __device__ void start(const PrefillParams& pp, long long t0, long long t1) {
     p = &pp;
     const int4 s = __ldcg(pp.start + blockIdx.x);
-    unit = s.x, head = s.y, tile = s.z;
+    unit = s.x, head = s.y, x = s.z;
     at = t0, end = t1;
   }
   __device__ bool next(Segment& g) {
-    if (at >= end) return false;
-    const int4 u = __ldcg(p->units + unit);
-    g.unit = unit, g.head = head;
-    g.seq = u.x, g.tok0 = u.y, g.begin = u.z, g.unit_tiles = u.w;
-    g.tile0 = tile;
-    g.at = at;
-    const long long left = end - at;
-    g.tiles = u.w - tile < left ? u.w - tile : (int)left;
-    at += g.tiles;
-    tile = 0;
-    if (++head == p->a.c.heads) {
-      head = 0;
-      ++unit;
+    while (at < end) {
+      const int4 u = __ldcg(p->units + unit);
+      const int cost = u.w + kUnitCost;
+      const int x1 = cost - x < end - at ? cost : x + (int)(end - at);
+      g.head = head;
+      g.seq = u.x, g.tok0 = u.y, g.begin = u.z, g.unit_tiles = u.w;
+      g.tile0 = max(0, x - kUnitCost);
+      g.tiles = max(0, x1 - kUnitCost) - g.tile0;
+      g.at = at - x;
+      at += x1 - x;
+      x = 0;
+      if (++head == p->a.c.heads) {
+        head = 0;
+        ++unit;
+      }
+      if (g.tiles > 0) return true;
     }
-    return true;
+    return false;
   }
 };
 
-// One pass over a row's S in tensor memory: P = 2^(s * scale - m) packed, the
-// largest exponent (relative to m) and the sum. P == nullptr-like MAX_ONLY: the
-// largest s * scale only.
-template <int BN, bool F16, bool MASK, bool MAX_ONLY>
-__device__ __forceinline__ void softmax_pass(uint32_t ts, float scale, float m, int col0, int lo,
-                                             int hi, uint32_t* pk, float& top, float& sum) {
-  float mx0 = -INFINITY, mx1 = -INFINITY, sum0 = 0.f, sum1 = 0.f;
+__device__ __forceinline__ uint64_t f32x2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 unpack_f32x2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// Bit i: key col + i lies in [lo, hi).
+__device__ __forceinline__ uint32_t seen_bits(int col, int lo, int hi) {
+  const int a = min(max(hi - col, 0), 32), b = min(max(lo - col, 0), 32);
+  const uint32_t below_hi = a == 32 ? 0xffffffffu : (1u << a) - 1u;
+  const uint32_t below_lo = b == 32 ? 0xffffffffu : (1u << b) - 1u;
+  return below_hi & ~below_lo;
+}
+
+// The largest s * sign of a row's visible keys (sign: of the scale).
+template <int BN, bool MASK, bool NEG>
+__device__ __forceinline__ float max_pass(uint32_t ts, int col0, int lo, int hi) {
+  float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
   for (int c = 0; c < BN / 32; ++c) {
     uint32_t s[32];
     tmem_ld32_nowait(ts + 32 * c, s);
     tmem_wait32(s);
+    const uint32_t seen = MASK ? seen_bits(col0 + 32 * c, lo, hi) : 0xffffffffu;
 #pragma unroll
-    for (int i = 0; i < 32; i += 2) {
-      float x = fmaf(__uint_as_float(s[i]), scale, -m);
-      float y = fmaf(__uint_as_float(s[i + 1]), scale, -m);
-      if (MASK) {
-        const int col = col0 + 32 * c + i;
-        x = col >= lo && col < hi ? x : -INFINITY;
-        y = col + 1 >= lo && col + 1 < hi ? y : -INFINITY;
+    for (int i = 0; i < 32; i += 4) {
+      float x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x[j] = NEG ? -__uint_as_float(s[i + j]) : __uint_as_float(s[i + j]);
+        if (MASK) x[j] = seen >> (i + j) & 1u ? x[j] : -INFINITY;
       }
-      mx0 = fmaxf(mx0, x);
-      mx1 = fmaxf(mx1, y);
-      if (!MAX_ONLY) {
-        x = ex2(x);
-        y = ex2(y);
-        sum0 += x;
-        sum1 += y;
-        pk[16 * c + i / 2] = pack2<F16>(x, y);
-      }
+      mx0 = fmaxf(fmaxf(mx0, x[0]), x[1]);
+      mx1 = fmaxf(fmaxf(mx1, x[2]), x[3]);
     }
   }
-  top = fmaxf(mx0, mx1);
-  sum = sum0 + sum1;
+  return fmaxf(mx0, mx1);
+}
+
+// P = 2^(s * scale - m) over S in tensor memory, 16-bit pairs in its first
+// BN / 2 columns (each written after the S columns it covers were read).
+// Returns the sum of the unrounded P.
+template <int BN, bool F16, bool MASK>
+__device__ __forceinline__ float exp_pass(uint32_t ts, float scale, float m, int col0, int lo,
+                                          int hi) {
+  const uint64_t scale2 = f32x2(scale, scale), m2 = f32x2(-m, -m);
+  uint64_t sum0 = 0, sum1 = 0;
+#pragma unroll
+  for (int c = 0; c < BN / 32; ++c) {
+    uint32_t s[32], pk[16];
+    tmem_ld32_nowait(ts + 32 * c, s);
+    tmem_wait32(s);
+    const uint32_t seen = MASK ? seen_bits(col0 + 32 * c, lo, hi) : 0xffffffffu;
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+      float2 x = unpack_f32x2(
+          fma_f32x2(f32x2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), scale2, m2));
+      if (MASK) {
+        x.x = seen >> i & 1u ? x.x : -INFINITY;
+        x.y = seen >> (i + 1) & 1u ? x.y : -INFINITY;
+      }
+      x.x = ex2(x.x);
+      x.y = ex2(x.y);
+      uint64_t& sum = i & 2 ? sum1 : sum0;
+      sum = add_f32x2(sum, f32x2(x.x, x.y));
+      pk[i / 2] = pack2<F16>(x.x, x.y);
+    }
+    tmem_st16(ts + 16 * c, pk);
+  }
+  const float2 t = unpack_f32x2(add_f32x2(sum0, sum1));
+  return t.x + t.y;
 }
 
 template <int D, int MT, int KV>
@@ -456,22 +534,25 @@ __global__ void __launch_bounds__(Shape<D, MT>::kThreads, 1)
   constexpr int BN = S::kBN;
   constexpr bool kHalf = KV == kF16 || KV == kE4m3F16;  // operand type f16
   constexpr bool kQuant = KV >= kE4m3Bf16;
-  constexpr int kProducer = MT * 4, kMma = MT * 4 + 4;  // first warps of the roles
+  constexpr int kProducer = MT * 4, kMma = kProducer + kProducers / 32, kRelay = kMma + 1;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   uint8_t* smem = smem_raw + ((1024u - (raw & 1023u)) & 1023u);
   const uint32_t sq = smem_u32(smem), ring = sq + S::kOffRing;
   RowInfo* table = reinterpret_cast<RowInfo*>(smem + S::kOffTable);
+  RowFactor* factors = reinterpret_cast<RowFactor*>(smem + S::kOffTable + 4 * BN * 16);
   Ctl* ctl = reinterpret_cast<Ctl*>(smem + S::kOffCtl);
   const AttnLaunch& a = p.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (tid == 0) {
     for (int i = 0; i < S::kStages; ++i) {
-      mbar_init(&ctl->full[i], 128);
+      mbar_init(&ctl->landed[i], kProducers);
+      mbar_init(&ctl->full[i], 1);
       mbar_init(&ctl->empty[i], 1);
     }
-    mbar_init(&ctl->q_full, 128);
+    mbar_init(&ctl->q_landed, kProducers);
+    mbar_init(&ctl->q_full, 1);
     mbar_init(&ctl->q_empty, 1);
     mbar_init(&ctl->drained, 1);
     for (int i = 0; i < 2; ++i) {
@@ -531,44 +612,36 @@ __global__ void __launch_bounds__(Shape<D, MT>::kThreads, 1)
         __syncwarp();
         tc_fence_after();
         const bool masked = __any_sync(0xffffffffu, col0 < lo || col0 + BN > hi);
-        uint32_t pk[BN / 2];
-        float top = 0.f, sum = 0.f;
-        bool redo = __any_sync(0xffffffffu, m == -INFINITY);
-        if (!redo) {
-          if (masked)
-            softmax_pass<BN, kHalf, true, false>(ts, p.scale_log2, m, col0, lo, hi, pk, top, sum);
-          else
-            softmax_pass<BN, kHalf, false, false>(ts, p.scale_log2, m, col0, lo, hi, pk, top, sum);
-          redo = __any_sync(0xffffffffu, top > kLazy);
-        }
-        if (redo) {
-          softmax_pass<BN, kHalf, true, true>(ts, p.scale_log2, 0.f, col0, lo, hi, pk, top, sum);
-          const float mn = m == -INFINITY || top > m + kLazy ? top : m;
-          const float f = m == mn || m == -INFINITY ? 1.f : ex2(m - mn);
-          if (k > 0 && __any_sync(0xffffffffu, f != 1.f)) {
-            // the product before this one may still be adding to O
-            wait_bar(pv_done, (step - 1) & 1u, ctl, a.status);
-            __syncwarp();
-            tc_fence_after();
+        float top;
+        if (p.scale_log2 >= 0.f)
+          top = masked ? max_pass<BN, true, false>(ts, col0, lo, hi)
+                       : max_pass<BN, false, false>(ts, col0, lo, hi);
+        else
+          top = max_pass<BN, true, true>(ts, col0, lo, hi);
+        // (a scale of zero makes every visible score zero)
+        top = top == -INFINITY ? top : top * fabsf(p.scale_log2);
+        const float mn = m == -INFINITY || top > m + kLazy ? top : m;
+        const float f = m == mn || m == -INFINITY ? 1.f : ex2(m - mn);
+        if (k > 0 && __any_sync(0xffffffffu, f != 1.f)) {
+          // the product before this one may still be adding to O
+          wait_bar(pv_done, (step - 1) & 1u, ctl, a.status);
+          __syncwarp();
+          tc_fence_after();
 #pragma unroll
-            for (int c = 0; c < D / 32; ++c) {
-              uint32_t o[32];
-              tmem_ld32_nowait(to + 32 * c, o);
-              tmem_wait32(o);
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld32_nowait(to + 32 * c, o);
+            tmem_wait32(o);
 #pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-              tmem_st32(to + 32 * c, o);
-            }
-            tmem_st_wait();
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            tmem_st32(to + 32 * c, o);
           }
-          l *= f;
-          m = mn;
-          const float base = m == -INFINITY ? 0.f : m;
-          softmax_pass<BN, kHalf, true, false>(ts, p.scale_log2, base, col0, lo, hi, pk, top, sum);
         }
-        l += sum;
-#pragma unroll
-        for (int c = 0; c < BN / 64; ++c) tmem_st32(ts + 32 * c, pk + 32 * c);
+        l *= f;
+        m = mn;
+        const float base = m == -INFINITY ? 0.f : m;
+        l += masked ? exp_pass<BN, kHalf, true>(ts, p.scale_log2, base, col0, lo, hi)
+                    : exp_pass<BN, kHalf, false>(ts, p.scale_log2, base, col0, lo, hi);
         tmem_st_wait();
         // Solo: the S that was waited for came before the previous product, so
         // that product is waited for here; no wait is then ever two phases
@@ -581,50 +654,77 @@ __global__ void __launch_bounds__(Shape<D, MT>::kThreads, 1)
       wait_bar(pv_done, (step - 1) & 1u, ctl, a.status);
       __syncwarp();
       tc_fence_after();
-      const long long u0 = g.at - g.tile0, u1 = u0 + g.unit_tiles;
-      const bool whole = u0 >= t0 && u1 <= t1;
+      const bool whole = g.tiles == g.unit_tiles;
       const long long token = (long long)q.q0 + tok;
       const int qh = g.head * p.groups + row_head;
-      uint16_t* dst = static_cast<uint16_t*>(a.out) + token * a.out_token_stride +
-                      (long long)qh * a.out_head_stride;
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      constexpr long long kPart = (long long)(D + 2) * 128;  // floats of a tile's partial
-      float* part = p.parts + ((2ll * blockIdx.x + (u0 >= t0 ? 1 : 0)) * MT + wg) * kPart + row;
+      // 32 columns of the warp's 32 rows, through shared memory so that a store
+      // covers 64 neighbouring bytes of each of 8 rows
+      long long out_at[4];
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t o[32];
-        tmem_ld32_nowait(to + 32 * c, o);
-        tmem_wait32(o);
-        if (whole) {
-          if (valid) {
-#pragma unroll
-            for (int i = 0; i < 32; i += 8) {
-              uint4 v;
-              uint32_t* w = &v.x;
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                // O of a row without keys is the sum of nothing but zeros
-                const float x = __uint_as_float(o[i + 2 * j]) * inv;
-                const float y = __uint_as_float(o[i + 2 * j + 1]) * inv;
-                w[j] = a.q_f16 ? pack2<true>(x, y) : pack2<false>(x, y);
-              }
-              *reinterpret_cast<uint4*>(dst + 32 * c + i) = v;
-            }
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) part[(2 + 32 * c + i) * 128] = __uint_as_float(o[i]);
-        }
+      for (int j = 0; j < 4; ++j) {
+        const int r = (warp & 3) * 32 + 8 * j + (lane >> 2);
+        const int t = g.tok0 + wg * p.tile_tokens + r / p.groups;
+        out_at[j] = r < p.tile_tokens * p.groups && t < q.q_len
+                        ? ((long long)q.q0 + t) * a.out_token_stride +
+                              (long long)(g.head * p.groups + r % p.groups) * a.out_head_stride +
+                              (lane & 3) * 8
+                        : -1;
       }
+      uint8_t* stage_out = smem + S::kOffOut + warp * 2048;
+      auto emit = [&](int c, const float (&v)[32]) {
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t w[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            w[j] = a.q_f16 ? pack2<true>(v[8 * i + 2 * j], v[8 * i + 2 * j + 1])
+                           : pack2<false>(v[8 * i + 2 * j], v[8 * i + 2 * j + 1]);
+          *reinterpret_cast<uint4*>(stage_out + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) =
+              make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int r = 8 * j + (lane >> 2);
+          const uint4 x = *reinterpret_cast<const uint4*>(stage_out + r * 64 +
+                                                          (((lane & 3) ^ ((r >> 1) & 3)) << 4));
+          if (out_at[j] >= 0)
+            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + out_at[j] + 32 * c) = x;
+        }
+      };
       if (whole) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          float v[32];
+          tmem_ld32_nowait(to + 32 * c, o);
+          tmem_wait32(o);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(o[i]) * inv;
+          emit(c, v);
+        }
         if (valid && a.lse != nullptr)
           a.lse[token * a.q_heads + qh] = l == 0.f ? -INFINITY : (m + log2f(l)) / kLog2e;
         continue;
       }
+      constexpr long long kPart = (long long)(D + 2) * 128;  // floats of a tile's partial
+      float* part = p.parts + ((2ll * blockIdx.x + (g.tile0 == 0 ? 1 : 0)) * MT + wg) * kPart + row;
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        tmem_ld32_nowait(to + 32 * c, o);
+        tmem_wait32(o);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) part[(2 + 32 * c + i) * 128] = __uint_as_float(o[i]);
+      }
       part[0] = l == 0.f ? -INFINITY : m;
       part[128] = l;
-      const int c_first = (int)(((u0 + 1) * ctas - 1) / total);
-      const int c_last = (int)((u1 * ctas - 1) / total);
+      // the blocks that hold the pair's first and last key tile
+      const long long first = g.at + kUnitCost, end = first + g.unit_tiles;
+      const int c_first = (int)(((first + 1) * ctas - 1) / total);
+      const int c_last = (int)((end * ctas - 1) / total);
       __threadfence();
       named_bar_sync(2 + wg, 128);
       if ((tid & 127) == 0) {
@@ -637,7 +737,7 @@ __global__ void __launch_bounds__(Shape<D, MT>::kThreads, 1)
       named_bar_sync(2 + wg, 128);
       const bool last = *reinterpret_cast<volatile int*>(&ctl->flag[wg]) != 0;
       named_bar_sync(2 + wg, 128);  // the flag may be written again
-      if (last && valid) {
+      if (!last) continue;
       const float* parts = p.parts + row;
       auto part_at = [&](int b) {
         return parts + ((2ll * b + (b == c_first ? 1 : 0)) * MT + wg) * kPart;
@@ -648,7 +748,7 @@ __global__ void __launch_bounds__(Shape<D, MT>::kThreads, 1)
         const float mb = __ldcg(part_at(b)), lb = __ldcg(part_at(b) + 128);
         sum += mb == -INFINITY ? lb : lb * ex2(mb - mx);
       }
-      const float inv_sum = sum == 0.f ? 0.f : 1.f / sum;
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         float acc[32];
@@ -665,160 +765,225 @@ __global__ void __launch_bounds__(Shape<D, MT>::kThreads, 1)
           }
         }
 #pragma unroll
-        for (int i = 0; i < 32; i += 8) {
-          uint4 v;
-          uint32_t* w = &v.x;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float x = acc[i + 2 * j] * inv_sum, y = acc[i + 2 * j + 1] * inv_sum;
-            w[j] = a.q_f16 ? pack2<true>(x, y) : pack2<false>(x, y);
-          }
-          *reinterpret_cast<uint4*>(dst + 32 * c + i) = v;
-        }
+        for (int i = 0; i < 32; ++i) acc[i] *= inv;
+        emit(c, acc);
       }
-      if (a.lse != nullptr)
+      if (valid && a.lse != nullptr)
         a.lse[token * a.q_heads + qh] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) / kLog2e;
-      }
-      __syncwarp();
     }
   } else if (warp < kMma) {
     // ------------------------------------------------------------ producer
-    const int pt = tid - kProducer * 32;  // 0..127
+    const int pt = tid - kProducer * 32;  // 0 .. kProducers - 1
     uint32_t stage = 0, fill = 0;         // ring position and pass
     uint32_t q_count = 0;
     constexpr int kElem = kQuant ? 1 : 2;
-    constexpr int kRowBytes = D * kElem;
-    constexpr int kChunks = kRowBytes / 16;           // 16-byte reads per key row
-    constexpr int kPer = BN * kChunks / 128;          // of them per thread and tile
+    constexpr int kChunks = D * kElem / 16;           // 16-byte reads per key row
+    constexpr int kPer = BN * kChunks / kProducers;   // of them per thread and tile
+    constexpr int kRowStep = kProducers / kChunks;
+    static_assert(kPer >= 1 && kRowStep % 8 == 0, "a thread's rows share a swizzle");
     const int p_row = pt / kChunks, p_chunk = pt % kChunks;
-    constexpr int kRowStep = 128 / kChunks;
+    const uint8_t* zeros = reinterpret_cast<const uint8_t*>(g_zero_row);
 
-    while (cur.next(g)) {
-      const SeqLens q = seq_lens(a, g.seq);
-      const int end = q.kv_len;
-      const int* pages = a.table + g.seq * a.table_stride;
-      // -- row information, two tiles ahead: page number, then offset and scales
-      auto page_of = [&](int t) -> int {  // this thread's row of key tile t
-        const int token = g.begin + (g.tile0 + t) * BN + pt;
-        return t < g.tiles && pt < BN && token < end ? __ldg(pages + token / a.c.page_size) : -1;
-      };
-      auto info_of = [&](int t, int page) {
-        RowInfo r;
-        r.off = -1;
-        r.k_factor = r.v_factor = 0;
-        const int token = g.begin + (g.tile0 + t) * BN + pt;
-        if (t < g.tiles && pt < BN && token < end) {
-          if (page < 0 || page >= a.c.num_pages) {
-            atomicOr(a.status, kDevBadPage);
-          } else {
-            const int at = token % a.c.page_size;
-            r.off = (page * a.c.page_stride + at * a.c.token_stride +
-                     g.head * a.c.head_stride) * kElem;
-            if (kQuant) {
-              const long long so = page * a.c.scale_page_stride + at * a.c.scale_token_stride +
-                                   g.head * a.c.scale_head_stride;
-              r.k_factor = __ldg(a.c.k_scale + so);
-              r.v_factor = __ldg(a.c.v_scale + so);
-            }
-          }
-        }
-        return r;
-      };
-      auto store_info = [&](int t, RowInfo r) {
-        if (pt < BN) {
-          if (kQuant && r.off >= 0) {
-            r.k_factor = factor_of<kHalf>(r.k_factor);
-            r.v_factor = factor_of<kHalf>(r.v_factor);
-          }
-          table[(t & 3) * BN + pt] = r;
-        }
-      };
-      RowInfo info = info_of(0, page_of(0));
-      int page1 = page_of(1);
-      // -- Q
-      wait_bar(&ctl->q_empty, (q_count & 1u) ^ 1u, ctl, a.status);
-      ++q_count;
-      {
-        constexpr int kQChunks = D / 8;
-        const int chunk = pt % kQChunks;
-#pragma unroll 4
-        for (int r = pt / kQChunks; r < MT * 128; r += 128 / kQChunks) {
-          const int tile = r >> 7, rr = r & 127;
-          const int tok = g.tok0 + tile * p.tile_tokens + rr / p.groups;
-          const bool valid = rr < p.tile_tokens * p.groups && tok < q.q_len;
-          const uint16_t* src =
-              static_cast<const uint16_t*>(a.q) +
-              (valid ? (q.q0 + tok) * a.q_token_stride +
-                           (long long)(g.head * p.groups + rr % p.groups) * a.q_head_stride + chunk * 8
-                     : 0);
-          const uint32_t dst = sq + (tile * S::kSlices + chunk / 8) * S::kQSlice + rr * 128 +
-                               (((chunk & 7) ^ (rr & 7)) << 4);
-          cp_async_16_zfill(dst, src, valid);
-        }
-        cp_async_arrive_noinc(&ctl->q_full);
-      }
-      store_info(0, info);
-      named_bar_sync(1, 128);
-      // -- keys and values, in the order the products take them:
-      // duo K0 V0 K1 V1 ..., solo K0 K1 V0 K2 V1 ... V(n-1)
-      uint4 held[kQuant ? kPer : 1];  // e4m3: the loads of the copy in progress
-      auto copy = [&](int t, bool is_v) {
-        wait_bar(&ctl->empty[stage], (fill & 1u) ^ 1u, ctl, a.status);
-        const uint32_t dst0 = ring + stage * S::kTileBytes;
-        const uint8_t* base = static_cast<const uint8_t*>(is_v ? a.c.v : a.c.k) + p_chunk * 16;
-        const RowInfo* rows = table + (t & 3) * BN;
-        if (!kQuant) {
-#pragma unroll
-          for (int i = 0; i < kPer; ++i) {
-            const int r = p_row + i * kRowStep;
-            const long long off = rows[r].off;
-            const uint32_t dst = dst0 + (p_chunk / 8) * S::kKvSlice + r * 128 +
-                                 (((p_chunk & 7) ^ (r & 7)) << 4);
-            cp_async_16_zfill(dst, base + (off < 0 ? 0 : off), off >= 0);
-          }
-          cp_async_arrive_noinc(&ctl->full[stage]);
+    // Thread pt < BN looks after key row pt of each tile: its page number, then
+    // its offset and scales, each a tile ahead of its use and across segments.
+    struct Info {
+      long long off;  // -1: no such row
+      uint32_t k_byte, v_byte;
+    };
+    auto page_of = [&](const Segment& sg, int kv_len, int t) -> int {
+      const int token = sg.begin + (sg.tile0 + t) * BN + pt;
+      return t < sg.tiles && pt < BN && token < kv_len
+                 ? __ldg(a.table + sg.seq * a.table_stride + token / a.c.page_size)
+                 : -1;
+    };
+    auto info_of = [&](const Segment& sg, int kv_len, int t, int page) {
+      Info r;
+      r.off = -1;
+      r.k_byte = r.v_byte = 0;
+      const int token = sg.begin + (sg.tile0 + t) * BN + pt;
+      if (t < sg.tiles && pt < BN && token < kv_len) {
+        if (page < 0 || page >= a.c.num_pages) {
+          atomicOr(a.status, kDevBadPage);
         } else {
+          const int at = token % a.c.page_size;
+          r.off = (page * a.c.page_stride + at * a.c.token_stride + sg.head * a.c.head_stride) *
+                  kElem;
+          if (kQuant) {
+            const long long so = page * a.c.scale_page_stride + at * a.c.scale_token_stride +
+                                 sg.head * a.c.scale_head_stride;
+            r.k_byte = __ldg(a.c.k_scale + so);
+            r.v_byte = __ldg(a.c.v_scale + so);
+          }
+        }
+      }
+      return r;
+    };
+    auto store_info = [&](int t, const Info& r) {
+      if (pt >= BN) return;
+      RowInfo row;
+      row.k = r.off < 0 ? zeros : static_cast<const uint8_t*>(a.c.k) + r.off;
+      row.v = r.off < 0 ? zeros : static_cast<const uint8_t*>(a.c.v) + r.off;
+      table[(t & 3) * BN + pt] = row;
+      if (kQuant) {
+        RowFactor f;
+        f.k = factor_of<kHalf>(r.k_byte);
+        f.v = factor_of<kHalf>(r.v_byte);
+        factors[(t & 3) * BN + pt] = f;
+      }
+    };
+    bool more = cur.next(g);
+    SeqLens q = seq_lens(a, g.seq);
+    int page2 = page_of(g, q.kv_len, 2);
+    Info info0 = info_of(g, q.kv_len, 0, page_of(g, q.kv_len, 0));
+    Info info1 = info_of(g, q.kv_len, 1, page_of(g, q.kv_len, 1));
+    while (more) {
+      store_info(0, info0);
+      store_info(1, info1);
+      named_bar_sync(1, kProducers);
+      // the next segment's first pages, on their way while this one is copied
+      Segment gn = g;
+      const bool more_n = cur.next(gn);
+      SeqLens qn = q;
+      int page0n = -1, page1n = -1;
+      if (more_n) {
+        qn = seq_lens(a, gn.seq);
+        page0n = page_of(gn, qn.kv_len, 0);
+        page1n = page_of(gn, qn.kv_len, 1);
+      }
+      // Ring entry n of the segment, in the order the products take them: duo
+      // K0 V0 K1 V1 ..., solo K0 K1 V0 K2 V1 ... V(last).
+      const int items = 2 * g.tiles;
+      auto item = [&](int n, int& t, bool& is_v) {
+        if (MT == 2) {
+          t = n >> 1;
+          is_v = n & 1;
+        } else {
+          t = (n + 1) >> 1;
+          is_v = n > 0 && ((n & 1) == 0 || t == g.tiles);
+          if (is_v) t = n == items - 1 ? g.tiles - 1 : (n >> 1) - 1;
+        }
+      };
+      uint4 held[kQuant ? kPer : 1];  // e4m3: the codes of the next entry
+      auto load = [&](int n) {
+        int t;
+        bool is_v;
+        item(n, t, is_v);
+        const RowInfo* rows = table + (t & 3) * BN;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          const RowInfo& r = rows[p_row + i * kRowStep];
+          held[kQuant ? i : 0] =
+              __ldg(reinterpret_cast<const uint4*>((is_v ? r.v : r.k) + p_chunk * 16));
+        }
+      };
+      auto fill_entry = [&](int n) {
+        int t;
+        bool is_v;
+        item(n, t, is_v);
+        if (!kQuant) {
+          wait_bar(&ctl->empty[stage], (fill & 1u) ^ 1u, ctl, a.status);
+          const RowInfo* rows = table + (t & 3) * BN;
+          const uint32_t dst = ring + stage * S::kTileBytes + (p_chunk / 8) * S::kKvSlice +
+                               p_row * 128 + (((p_chunk & 7) ^ (p_row & 7)) << 4);
 #pragma unroll
           for (int i = 0; i < kPer; ++i) {
-            const long long off = rows[p_row + i * kRowStep].off;
-            held[i] = off < 0 ? make_uint4(0u, 0u, 0u, 0u)
-                              : __ldg(reinterpret_cast<const uint4*>(base + off));
+            const RowInfo& r = rows[p_row + i * kRowStep];
+            cp_async_16_at(dst + i * kRowStep * 128, (is_v ? r.v : r.k) + p_chunk * 16);
           }
+          cp_async_arrive_noinc(&ctl->landed[stage]);
+        } else {
+          uint4 codes[kQuant ? kPer : 1];
 #pragma unroll
-          for (int i = 0; i < kPer; ++i) {
-            const int r = p_row + i * kRowStep;
-            const uint32_t f = is_v ? rows[r].v_factor : rows[r].k_factor;
-            const uint2 x = convert4<kHalf>(held[i].x, f), y = convert4<kHalf>(held[i].y, f);
-            const uint2 z = convert4<kHalf>(held[i].z, f), w = convert4<kHalf>(held[i].w, f);
-            // 16 columns: chunks 2c and 2c + 1 of the 16-bit row
-            const int c2 = 2 * p_chunk;
-            const uint32_t dst = dst0 + (c2 / 8) * S::kKvSlice + r * 128;
-            st_shared_u128(dst + (((c2 & 7) ^ (r & 7)) << 4), make_uint4(x.x, x.y, y.x, y.y));
-            st_shared_u128(dst + ((((c2 & 7) + 1) ^ (r & 7)) << 4), make_uint4(z.x, z.y, w.x, w.y));
+          for (int i = 0; i < (kQuant ? kPer : 1); ++i) codes[i] = held[i];
+          if (n + 1 < items) load(n + 1);
+          wait_bar(&ctl->empty[stage], (fill & 1u) ^ 1u, ctl, a.status);
+          const RowFactor* fs = factors + (t & 3) * BN;
+          // 16 columns: chunks 2c and 2c + 1 of the 16-bit row
+          const int c2 = 2 * p_chunk;
+          const uint32_t dst = ring + stage * S::kTileBytes + (c2 / 8) * S::kKvSlice + p_row * 128;
+          const uint32_t x0 = ((c2 & 7) ^ (p_row & 7)) << 4, x1 = (((c2 & 7) + 1) ^ (p_row & 7)) << 4;
+#pragma unroll
+          for (int i = 0; i < (kQuant ? kPer : 1); ++i) {
+            const RowFactor& rf = fs[p_row + i * kRowStep];
+            const uint32_t f = is_v ? rf.v : rf.k;
+            const uint2 x = convert4<kHalf>(codes[i].x, f), y = convert4<kHalf>(codes[i].y, f);
+            const uint2 z = convert4<kHalf>(codes[i].z, f), w = convert4<kHalf>(codes[i].w, f);
+            st_shared_u128(dst + i * kRowStep * 128 + x0, make_uint4(x.x, x.y, y.x, y.y));
+            st_shared_u128(dst + i * kRowStep * 128 + x1, make_uint4(z.x, z.y, w.x, w.y));
           }
-          mbar_arrive(&ctl->full[stage]);
+          mbar_arrive(&ctl->landed[stage]);
         }
         if (++stage == S::kStages) {
           stage = 0;
           ++fill;
         }
       };
+      if (kQuant) load(0);
       for (int t = 0; t < g.tiles; ++t) {
-        const RowInfo next = info_of(t + 1, page1);
-        page1 = page_of(t + 2);
-        copy(t, false);
-        if (MT == 2)
-          copy(t, true);
-        else if (t > 0)
-          copy(t - 1, true);
-        store_info(t + 1, next);
-        named_bar_sync(1, 128);
+        const Info next = info_of(g, q.kv_len, t + 2, page2);
+        page2 = page_of(g, q.kv_len, t + 3);
+        fill_entry(2 * t);
+        if (t == 0) {
+          // Q after the first keys: it waits for the last segment's products
+          wait_bar(&ctl->q_empty, (q_count & 1u) ^ 1u, ctl, a.status);
+          ++q_count;
+          constexpr int kQChunks = D / 8;
+          const int chunk = pt % kQChunks;
+#pragma unroll 4
+          for (int r = pt / kQChunks; r < MT * 128; r += kProducers / kQChunks) {
+            const int tile = r >> 7, rr = r & 127;
+            const int tok = g.tok0 + tile * p.tile_tokens + rr / p.groups;
+            const bool valid = rr < p.tile_tokens * p.groups && tok < q.q_len;
+            const uint8_t* src =
+                valid ? static_cast<const uint8_t*>(a.q) +
+                            ((q.q0 + tok) * a.q_token_stride +
+                             (long long)(g.head * p.groups + rr % p.groups) * a.q_head_stride +
+                             chunk * 8) * 2
+                      : zeros + chunk * 16;
+            cp_async_16_at(sq + (tile * S::kSlices + chunk / 8) * S::kQSlice + rr * 128 +
+                               (((chunk & 7) ^ (rr & 7)) << 4),
+                           src);
+          }
+          cp_async_arrive_noinc(&ctl->q_landed);
+        }
+        fill_entry(2 * t + 1);
+        store_info(t + 2, next);
+        if (t + 1 == g.tiles && more_n) {
+          info0 = info_of(gn, qn.kv_len, 0, page0n);
+          info1 = info_of(gn, qn.kv_len, 1, page1n);
+          page2 = page_of(gn, qn.kv_len, 2);
+        }
+        named_bar_sync(1, kProducers);
       }
-      if (MT == 1) copy(g.tiles - 1, true);
-      // the table's entries are this segment's: all have read them
-      named_bar_sync(1, 128);
+      g = gn;
+      q = qn;
+      more = more_n;
     }
     cp_async_wait_all();
+  } else if (warp == kRelay) {
+    // --------------------------------------------------------------- relay
+    // The copies are writes of the generic proxy, the products read through
+    // the async proxy: a fence between them, in the order of the copies.
+    if (elect_one()) {
+      uint32_t stage = 0, fill = 0, q_count = 0;
+      auto pass = [&]() {
+        wait_bar(&ctl->landed[stage], fill & 1u, ctl, a.status);
+        fence_async_smem();
+        mbar_arrive(&ctl->full[stage]);
+        if (++stage == S::kStages) {
+          stage = 0;
+          ++fill;
+        }
+      };
+      while (cur.next(g)) {
+        pass();
+        wait_bar(&ctl->q_landed, q_count & 1u, ctl, a.status);
+        fence_async_smem();
+        mbar_arrive(&ctl->q_full);
+        ++q_count;
+        for (int t = 1; t < 2 * g.tiles; ++t) pass();
+      }
+    }
   } else if (warp == kMma && elect_one()) {
     // ----------------------------------------------------------------- mma
     const uint32_t id_s = instr_desc(kHalf, BN, false), id_o = instr_desc(kHalf, D, true);
@@ -826,11 +991,8 @@ __global__ void __launch_bounds__(Shape<D, MT>::kThreads, 1)
     uint32_t s_count = 0, p_count = 0; // S tiles issued, P tiles consumed (all segments)
     uint32_t q_count = 0;
     bool ok = true;
-    // Waits for the next ring entry. The copies are plain writes to shared
-    // memory, the products read it through the async proxy: the fence orders them.
-    auto take = [&]() -> uint32_t {
+    auto take = [&]() -> uint32_t {  // waits for the next ring entry
       ok = wait_bar(&ctl->full[stage], fill & 1u, ctl, a.status);
-      fence_async_smem();
       return stage;
     };
     auto advance = [&]() {
@@ -842,7 +1004,6 @@ __global__ void __launch_bounds__(Shape<D, MT>::kThreads, 1)
     while (ok && cur.next(g)) {
       ok = wait_bar(&ctl->q_full, q_count & 1u, ctl, a.status);
       if (!ok) break;
-      fence_async_smem();
       ++q_count;
       const int steps = MT * g.tiles;
       uint32_t k_stage = 0, v_stage = 0;
