@@ -75,11 +75,14 @@ struct PrefillParams {
   int4* units;      // sequence, first token in it, first key, key tiles
   int max_units;
   float* parts;
+  // tensor copies: rows of a page that one copy takes (a power of two that
+  // divides the page size), and whether heads come before tokens in the map
+  int box_rows, heads_first;
 };
 
 constexpr int kProducers = 256;
 
-template <int D, int MT>
+template <int D, int MT, bool TMA>
 struct Shape {
   static constexpr int kBN = D == 256 ? 64 : 128;  // keys per tile
   static constexpr int kSlices = D / 64;
@@ -87,12 +90,13 @@ struct Shape {
   static constexpr int kKvSlice = kBN * 128;
   static constexpr int kQBytes = MT * kSlices * kQSlice;
   static constexpr int kTileBytes = kSlices * kKvSlice;
-  static constexpr int kTableBytes = 4 * kBN * (16 + 8);
+  static constexpr int kTableBytes = TMA ? 0 : 4 * kBN * (16 + 8);
   static constexpr int kOutBytes = MT * 4 * 2048;   // 32 rows x 32 columns per warp
   static constexpr int kFixed = kQBytes + kTableBytes + kOutBytes + 2048 + 1024;
   static constexpr int kFit = (227 * 1024 - kFixed) / kTileBytes;
   static constexpr int kStages = kFit > 8 ? 8 : kFit;
-  static constexpr int kThreads = MT * 128 + kProducers + 64;
+  static constexpr int kLoaders = TMA ? 32 : kProducers;
+  static constexpr int kThreads = MT * 128 + kLoaders + 64;
   static constexpr int kOffRing = kQBytes;
   static constexpr int kOffTable = kOffRing + kStages * kTileBytes;
   static constexpr int kOffOut = kOffTable + kTableBytes;
@@ -121,21 +125,36 @@ struct Ctl {
   int flag[2];
 };
 
+// One try with a suspension hint: the waiting warps of a block are many, and
+// without it their polling takes half of the issue slots.
+__device__ __forceinline__ bool try_wait_long(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n"
+      "  .reg .pred p;\n"
+      "  mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
+      "  selp.u32 %0, 1, 0, p;\n"
+      "}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(100000u)  // ns
+      : "memory");
+  return ok != 0;
+}
+
 // Bounded wait. A role that gives up sets the block's abort flag; from then on
 // no wait waits, so every role runs through its loops (and block barriers) and
 // the block ends with the status bit set.
 __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, Ctl* ctl, int* status) {
-  if (mbar_try_wait(bar, parity)) return true;
+  if (try_wait_long(bar, parity)) return true;
   const unsigned long long t0 = global_timer_ns();
-  for (uint32_t i = 1;; ++i) {
-    if (*reinterpret_cast<volatile int*>(&ctl->abort)) return false;
-    if (mbar_try_wait(bar, parity)) return true;
-    if ((i & 255u) == 0u && global_timer_ns() - t0 > kWaitLimitNs) {
+  while (!*reinterpret_cast<volatile int*>(&ctl->abort)) {
+    if (try_wait_long(bar, parity)) return true;
+    if (global_timer_ns() - t0 > kWaitLimitNs) {
       atomicOr(status, kDevWaitTimeout);
       *reinterpret_cast<volatile int*>(&ctl->abort) = 1;
-      return false;
     }
   }
+  return false;
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -165,6 +184,22 @@ __device__ __forceinline__ void tmem_wait32(uint32_t (&r)[32]) {
         "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
 }
 
+__device__ __forceinline__ void tmem_ld16_nowait(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,"
+      "%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait16(uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.wait::ld.sync.aligned;"
+      : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]),
+        "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]),
+        "+r"(r[14]), "+r"(r[15])::"memory");
+}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
@@ -174,30 +209,21 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16
       "r"(v[15])
       : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* v) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
-      "%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
-      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
-      "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]),
-      "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]),
-      "r"(v[29]), "r"(v[30]), "r"(v[31])
-      : "memory");
-}
 __device__ __forceinline__ void tmem_st_wait() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
-// A K-major or (mn_stride > 0) MN-major operand, 128-byte swizzle: 8 lines of
-// 128 B per atom, atoms 1024 B apart; blocks of 64 MN elements mn_stride apart.
-__device__ __forceinline__ uint64_t smem_desc(uint32_t saddr, uint32_t mn_stride) {
-  uint64_t d = smem_desc_sw128(saddr);
-  if (mn_stride) {
-    d &= ~((uint64_t)0x3fffu << 16);
-    d |= (uint64_t)(mn_stride >> 4) << 16;
-  }
-  return d;
+// Shared-memory operand descriptors, 128-byte swizzle: 8 lines of 128 B per
+// atom, atoms 1024 B apart. The low word holds the address (16-byte units) and
+// for an MN-major operand the distance of its blocks of 64 MN elements; the
+// mma thread, whose instructions all wait on one another, then steps through a
+// tile by adding constants to it.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t mn_stride) {
+  return ((saddr >> 4) & 0x3fffu) | (mn_stride ? mn_stride >> 4 : 1u) << 16;
+}
+__device__ __forceinline__ uint64_t desc_of(uint32_t lo) {
+  constexpr uint64_t kHi = (uint64_t)(1024u >> 4) << 32 | (uint64_t)1u << 46 | (uint64_t)2u << 61;
+  return kHi | lo;
 }
 
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
@@ -330,6 +356,7 @@ __device__ long long block_scan(long long v, long long* sh, long long& total) {
 __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const PrefillParams p,
                                                                  int unit_tokens, int bn,
                                                                  int max_ctas) {
+  // (with tensor copies a unit's first key is moved down to a copy's border)
   __shared__ long long sh[32];
   griddep_wait();
   const AttnLaunch& a = p.a;
@@ -371,6 +398,7 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const PrefillPa
       const int shift = q.kv_len - q.q_len;
       int end = a.causal ? min(q.kv_len, shift + last + 1) : q.kv_len;
       int begin = a.window > 0 ? max(0, shift + tok0 - a.window + 1) : 0;
+      begin -= begin % p.box_rows;
       const int tiles = end > begin ? (end - begin + bn - 1) / bn : 1;
       p.units[u] = make_int4(s, tok0, begin, tiles);
       mine += (long long)(tiles + kUnitCost) * a.c.heads;
@@ -527,14 +555,100 @@ __device__ __forceinline__ float exp_pass(uint32_t ts, float scale, float m, int
   return t.x + t.y;
 }
 
-template <int D, int MT, int KV>
-__global__ void __launch_bounds__(Shape<D, MT>::kThreads, 1)
-    attn_prefill_kernel(const PrefillParams p) {
-  using S = Shape<D, MT>;
+// Ties r's uses to a tcgen05.wait::ld that came before.
+__device__ __forceinline__ void tie32(uint32_t* r) {
+  asm volatile(""
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
+                 "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                 "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]),
+                 "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31]));
+}
+// A row's S into registers.
+template <int BN>
+__device__ __forceinline__ void load_row(uint32_t ts, uint32_t (&s)[BN]) {
+#pragma unroll
+  for (int c = 0; c < BN / 32; ++c)
+    tmem_ld32_nowait(ts + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(s + 32 * c));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int c = 0; c < BN / 32; ++c) tie32(s + 32 * c);
+}
+template <int BN>
+__device__ __forceinline__ void mask_row(uint32_t (&s)[BN], int col0, int lo, int hi, float hidden) {
+#pragma unroll
+  for (int c = 0; c < BN / 32; ++c) {
+    const uint32_t seen = seen_bits(col0 + 32 * c, lo, hi);
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      s[32 * c + i] = seen >> i & 1u ? s[32 * c + i] : __float_as_uint(hidden);
+  }
+}
+template <int BN, bool NEG>
+__device__ __forceinline__ float max_row(const uint32_t (&s)[BN]) {
+  float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int i = 0; i < BN; i += 8)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float x = __uint_as_float(s[i + 2 * j]), y = __uint_as_float(s[i + 2 * j + 1]);
+      mx[j] = NEG ? fmaxf(fmaxf(mx[j], -x), -y) : fmaxf(fmaxf(mx[j], x), y);
+    }
+  return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+}
+// P of a row in registers to tensor memory; see exp_pass.
+template <int BN, bool F16>
+__device__ __forceinline__ float exp_row(uint32_t ts, const uint32_t (&s)[BN], float scale, float m) {
+  const uint64_t scale2 = f32x2(scale, scale), m2 = f32x2(-m, -m);
+  uint64_t sum0 = 0, sum1 = 0;
+#pragma unroll
+  for (int c = 0; c < BN / 32; ++c) {
+    uint32_t pk[16];
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+      float2 x = unpack_f32x2(fma_f32x2(
+          f32x2(__uint_as_float(s[32 * c + i]), __uint_as_float(s[32 * c + i + 1])), scale2, m2));
+      x.x = ex2(x.x);
+      x.y = ex2(x.y);
+      uint64_t& sum = i & 2 ? sum1 : sum0;
+      sum = add_f32x2(sum, f32x2(x.x, x.y));
+      pk[i / 2] = pack2<F16>(x.x, x.y);
+    }
+    tmem_st16(ts + 16 * c, pk);
+  }
+  const float2 t = unpack_f32x2(add_f32x2(sum0, sum1));
+  return t.x + t.y;
+}
+
+// One box of a page: 64 columns x box_rows tokens.
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z,
+                                            int w, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z,
+                                            uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      : "memory");
+}
+
+template <int D, int MT, int KV, bool TMA>
+__global__ void __launch_bounds__(Shape<D, MT, TMA>::kThreads, 1)
+    attn_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap q_map,
+                        const __grid_constant__ CUtensorMap k_map,
+                        const __grid_constant__ CUtensorMap v_map) {
+  using S = Shape<D, MT, TMA>;
   constexpr int BN = S::kBN;
   constexpr bool kHalf = KV == kF16 || KV == kE4m3F16;  // operand type f16
   constexpr bool kQuant = KV >= kE4m3Bf16;
-  constexpr int kProducer = MT * 4, kMma = kProducer + kProducers / 32, kRelay = kMma + 1;
+  constexpr int kProducer = MT * 4, kMma = kProducer + S::kLoaders / 32, kRelay = kMma + 1;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   uint8_t* smem = smem_raw + ((1024u - (raw & 1023u)) & 1023u);
@@ -547,11 +661,11 @@ __global__ void __launch_bounds__(Shape<D, MT>::kThreads, 1)
 
   if (tid == 0) {
     for (int i = 0; i < S::kStages; ++i) {
-      mbar_init(&ctl->landed[i], kProducers);
+      mbar_init(&ctl->landed[i], TMA ? 1 : kProducers);
       mbar_init(&ctl->full[i], 1);
       mbar_init(&ctl->empty[i], 1);
     }
-    mbar_init(&ctl->q_landed, kProducers);
+    mbar_init(&ctl->q_landed, TMA ? 1 : kProducers);
     mbar_init(&ctl->q_full, 1);
     mbar_init(&ctl->q_empty, 1);
     mbar_init(&ctl->drained, 1);
@@ -608,12 +722,17 @@ __global__ void __launch_bounds__(Shape<D, MT>::kThreads, 1)
         const uint32_t phase = MT == 2 ? step & 1u : (step >> 1) & 1u;
         const uint32_t ts = lane_addr + buf * 128;
         const int col0 = g.begin + (g.tile0 + k) * BN;
-        wait_bar(&ctl->s_full[buf], phase, ctl, a.status);
-        __syncwarp();
+        if ((warp & 3) == 0) wait_bar(&ctl->s_full[buf], phase, ctl, a.status);
+        named_bar_sync(2 + wg, 128);
         tc_fence_after();
         const bool masked = __any_sync(0xffffffffu, col0 < lo || col0 + BN > hi);
         float top;
-        if (p.scale_log2 >= 0.f)
+        uint32_t s[TMA ? BN : 32];  // TMA: the row's S, read once
+        if constexpr (TMA) {
+          load_row<BN>(ts, s);
+          if (masked) mask_row<BN>(s, col0, lo, hi, p.scale_log2 >= 0.f ? -INFINITY : INFINITY);
+          top = p.scale_log2 >= 0.f ? max_row<BN, false>(s) : max_row<BN, true>(s);
+        } else if (p.scale_log2 >= 0.f)
           top = masked ? max_pass<BN, true, false>(ts, col0, lo, hi)
                        : max_pass<BN, false, false>(ts, col0, lo, hi);
         else
@@ -627,21 +746,25 @@ __global__ void __launch_bounds__(Shape<D, MT>::kThreads, 1)
           wait_bar(pv_done, (step - 1) & 1u, ctl, a.status);
           __syncwarp();
           tc_fence_after();
+          // (few columns at a time: the row's S stays in registers beside them)
+#pragma unroll 1
+          for (int c = 0; c < D / 16; ++c) {
+            uint32_t o[16];
+            tmem_ld16_nowait(to + 16 * c, o);
+            tmem_wait16(o);
 #pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld32_nowait(to + 32 * c, o);
-            tmem_wait32(o);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-            tmem_st32(to + 32 * c, o);
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            tmem_st16(to + 16 * c, o);
           }
         }
         l *= f;
         m = mn;
         const float base = m == -INFINITY ? 0.f : m;
-        l += masked ? exp_pass<BN, kHalf, true>(ts, p.scale_log2, base, col0, lo, hi)
-                    : exp_pass<BN, kHalf, false>(ts, p.scale_log2, base, col0, lo, hi);
+        if constexpr (TMA)
+          l += exp_row<BN, kHalf>(ts, s, p.scale_log2, base);
+        else
+          l += masked ? exp_pass<BN, kHalf, true>(ts, p.scale_log2, base, col0, lo, hi)
+                      : exp_pass<BN, kHalf, false>(ts, p.scale_log2, base, col0, lo, hi);
         tmem_st_wait();
         // Solo: the S that was waited for came before the previous product, so
         // that product is waited for here; no wait is then ever two phases
@@ -651,8 +774,8 @@ __global__ void __launch_bounds__(Shape<D, MT>::kThreads, 1)
         mbar_arrive(&ctl->p_ready[buf]);
       }
       // -- the last product, then O out
-      wait_bar(pv_done, (step - 1) & 1u, ctl, a.status);
-      __syncwarp();
+      if ((warp & 3) == 0) wait_bar(pv_done, (step - 1) & 1u, ctl, a.status);
+      named_bar_sync(2 + wg, 128);
       tc_fence_after();
       const bool whole = g.tiles == g.unit_tiles;
       const long long token = (long long)q.q0 + tok;
@@ -771,7 +894,84 @@ __global__ void __launch_bounds__(Shape<D, MT>::kThreads, 1)
       if (valid && a.lse != nullptr)
         a.lse[token * a.q_heads + qh] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) / kLog2e;
     }
-  } else if (warp < kMma) {
+  } else if (TMA && warp < kMma) {
+    // -------------------------------------------------------------- loader
+    // One warp, a lane per box of box_rows keys. Boxes past the last key and
+    // boxes of pages outside the cache are copied from past the map's end,
+    // which fills zeros.
+    uint32_t stage = 0, fill = 0, q_count = 0;
+    const int boxes = BN / p.box_rows;
+    auto page_of = [&](const Segment& sg, int kv_len, int t) -> int {
+      const int token = sg.begin + (sg.tile0 + t) * BN + lane * p.box_rows;
+      if (t >= sg.tiles || lane >= boxes || token >= kv_len) return -2;
+      return __ldg(a.table + sg.seq * a.table_stride + token / a.c.page_size);
+    };
+    bool more = cur.next(g);
+    SeqLens q = seq_lens(a, g.seq);
+    int page_n = page_of(g, q.kv_len, 0);
+    while (more) {
+      Segment gn = g;
+      const bool more_n = cur.next(gn);
+      const SeqLens qn = more_n ? seq_lens(a, gn.seq) : q;
+      int page = -2, page_before = -2;  // of tile t and t - 1
+      auto fill_entry = [&](int t, bool is_v, int pg) {
+        if (lane == 0) {
+          wait_bar(&ctl->empty[stage], (fill & 1u) ^ 1u, ctl, a.status);
+          mbar_arrive_expect_tx(&ctl->landed[stage], S::kTileBytes);
+        }
+        __syncwarp();
+        if (lane < boxes) {
+          const int token = g.begin + (g.tile0 + t) * BN + lane * p.box_rows;
+          int at = token % a.c.page_size;
+          if (pg < 0 || pg >= a.c.num_pages) {
+            if (token < q.kv_len) atomicOr(a.status, kDevBadPage);
+            pg = (int)a.c.num_pages;
+            at = 0;
+          }
+          const uint32_t dst = ring + stage * S::kTileBytes + lane * p.box_rows * 128;
+          const CUtensorMap* map = is_v ? &v_map : &k_map;
+#pragma unroll
+          for (int sl = 0; sl < S::kSlices; ++sl)
+            tma_load_4d(dst + sl * S::kKvSlice, map, 64 * sl, p.heads_first ? g.head : at,
+                        p.heads_first ? at : g.head, pg, &ctl->landed[stage]);
+        }
+        if (++stage == S::kStages) {
+          stage = 0;
+          ++fill;
+        }
+      };
+      for (int t = 0; t < g.tiles; ++t) {
+        page_before = page;
+        page = page_n;
+        // the next tile's pages, or the next segment's first
+        page_n = t + 1 < g.tiles ? page_of(g, q.kv_len, t + 1)
+                                 : more_n ? page_of(gn, qn.kv_len, 0) : -2;
+        fill_entry(t, false, page);
+        if (t == 0) {
+          if (lane == 0) {
+            wait_bar(&ctl->q_empty, (q_count & 1u) ^ 1u, ctl, a.status);
+            mbar_arrive_expect_tx(&ctl->q_landed,
+                                  MT * S::kSlices * p.tile_tokens * p.groups * 128);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+              for (int sl = 0; sl < S::kSlices; ++sl)
+                tma_load_3d(sq + (mt * S::kSlices + sl) * S::kQSlice, &q_map, 64 * sl,
+                            g.head * p.groups, q.q0 + g.tok0 + mt * p.tile_tokens, &ctl->q_landed);
+          }
+          ++q_count;
+        }
+        if (MT == 2)
+          fill_entry(t, true, page);
+        else if (t > 0)
+          fill_entry(t - 1, true, page_before);
+      }
+      if (MT == 1) fill_entry(g.tiles - 1, true, page);
+      g = gn;
+      q = qn;
+      more = more_n;
+    }
+  } else if (!TMA && warp < kMma) {
     // ------------------------------------------------------------ producer
     const int pt = tid - kProducer * 32;  // 0 .. kProducers - 1
     uint32_t stage = 0, fill = 0;         // ring position and pass
@@ -876,12 +1076,16 @@ __global__ void __launch_bounds__(Shape<D, MT>::kThreads, 1)
               __ldg(reinterpret_cast<const uint4*>((is_v ? r.v : r.k) + p_chunk * 16));
         }
       };
+      auto acquire = [&]() {  // the ring's next place; also publishes store_info's rows
+        if (pt < 32) wait_bar(&ctl->empty[stage], (fill & 1u) ^ 1u, ctl, a.status);
+        named_bar_sync(1, kProducers);
+      };
       auto fill_entry = [&](int n) {
         int t;
         bool is_v;
         item(n, t, is_v);
         if (!kQuant) {
-          wait_bar(&ctl->empty[stage], (fill & 1u) ^ 1u, ctl, a.status);
+          acquire();
           const RowInfo* rows = table + (t & 3) * BN;
           const uint32_t dst = ring + stage * S::kTileBytes + (p_chunk / 8) * S::kKvSlice +
                                p_row * 128 + (((p_chunk & 7) ^ (p_row & 7)) << 4);
@@ -896,7 +1100,7 @@ __global__ void __launch_bounds__(Shape<D, MT>::kThreads, 1)
 #pragma unroll
           for (int i = 0; i < (kQuant ? kPer : 1); ++i) codes[i] = held[i];
           if (n + 1 < items) load(n + 1);
-          wait_bar(&ctl->empty[stage], (fill & 1u) ^ 1u, ctl, a.status);
+          acquire();
           const RowFactor* fs = factors + (t & 3) * BN;
           // 16 columns: chunks 2c and 2c + 1 of the 16-bit row
           const int c2 = 2 * p_chunk;
@@ -925,7 +1129,8 @@ __global__ void __launch_bounds__(Shape<D, MT>::kThreads, 1)
         fill_entry(2 * t);
         if (t == 0) {
           // Q after the first keys: it waits for the last segment's products
-          wait_bar(&ctl->q_empty, (q_count & 1u) ^ 1u, ctl, a.status);
+          if (pt < 32) wait_bar(&ctl->q_empty, (q_count & 1u) ^ 1u, ctl, a.status);
+          named_bar_sync(1, kProducers);
           ++q_count;
           constexpr int kQChunks = D / 8;
           const int chunk = pt % kQChunks;
@@ -946,15 +1151,15 @@ __global__ void __launch_bounds__(Shape<D, MT>::kThreads, 1)
           }
           cp_async_arrive_noinc(&ctl->q_landed);
         }
-        fill_entry(2 * t + 1);
         store_info(t + 2, next);
+        fill_entry(2 * t + 1);
         if (t + 1 == g.tiles && more_n) {
           info0 = info_of(gn, qn.kv_len, 0, page0n);
           info1 = info_of(gn, qn.kv_len, 1, page1n);
           page2 = page_of(gn, qn.kv_len, 2);
         }
-        named_bar_sync(1, kProducers);
       }
+      named_bar_sync(1, kProducers);  // all have read this segment's rows
       g = gn;
       q = qn;
       more = more_n;
@@ -962,30 +1167,57 @@ __global__ void __launch_bounds__(Shape<D, MT>::kThreads, 1)
     cp_async_wait_all();
   } else if (warp == kRelay) {
     // --------------------------------------------------------------- relay
-    // The copies are writes of the generic proxy, the products read through
-    // the async proxy: a fence between them, in the order of the copies.
-    if (elect_one()) {
-      uint32_t stage = 0, fill = 0, q_count = 0;
-      auto pass = [&]() {
-        wait_bar(&ctl->landed[stage], fill & 1u, ctl, a.status);
+    // Plain copies are writes of the generic proxy, the products read through
+    // the async proxy: a fence between them, in the order of the copies. Tensor
+    // copies need none, but bring whatever a page holds past the last key:
+    // those rows of V are set to zero, since zero times NaN is NaN.
+    uint32_t stage = 0, fill = 0, q_count = 0;
+    auto pass = [&](int first_zero_row) {
+      if (lane == 0) wait_bar(&ctl->landed[stage], fill & 1u, ctl, a.status);
+      __syncwarp();
+      if (TMA && first_zero_row < BN) {
+        for (int i = first_zero_row * 8 + lane; i < BN * 8; i += 32)
+#pragma unroll
+          for (int sl = 0; sl < S::kSlices; ++sl)
+            st_shared_u128(ring + stage * S::kTileBytes + sl * S::kKvSlice + i * 16,
+                           make_uint4(0u, 0u, 0u, 0u));
         fence_async_smem();
+        __syncwarp();
+      }
+      if (lane == 0) {
+        if (!TMA) fence_async_smem();
         mbar_arrive(&ctl->full[stage]);
-        if (++stage == S::kStages) {
-          stage = 0;
-          ++fill;
+      }
+      if (++stage == S::kStages) {
+        stage = 0;
+        ++fill;
+      }
+    };
+    while (cur.next(g)) {
+      const int kv_len = TMA ? seq_lens(a, g.seq).kv_len : 0;
+      for (int n = 0; n < 2 * g.tiles; ++n) {
+        int zero_row = BN;
+        if (TMA) {
+          // a V entry's rows past the last key
+          const bool is_v = MT == 2 ? n & 1 : n > 0 && ((n & 1) == 0 || n == 2 * g.tiles - 1);
+          const int t = MT == 2 ? n >> 1 : n == 2 * g.tiles - 1 ? g.tiles - 1 : (n >> 1) - 1;
+          if (is_v) zero_row = max(0, min(BN, kv_len - (g.begin + (g.tile0 + t) * BN)));
         }
-      };
-      while (cur.next(g)) {
-        pass();
-        wait_bar(&ctl->q_landed, q_count & 1u, ctl, a.status);
-        fence_async_smem();
-        mbar_arrive(&ctl->q_full);
-        ++q_count;
-        for (int t = 1; t < 2 * g.tiles; ++t) pass();
+        pass(zero_row);
+        if (n == 0) {
+          if (lane == 0) {
+            wait_bar(&ctl->q_landed, q_count & 1u, ctl, a.status);
+            if (!TMA) fence_async_smem();
+            mbar_arrive(&ctl->q_full);
+          }
+          ++q_count;
+        }
       }
     }
   } else if (warp == kMma && elect_one()) {
     // ----------------------------------------------------------------- mma
+    const uint32_t q_desc = desc_lo(sq, 0), k_desc = desc_lo(ring, 0);
+    const uint32_t v_desc = desc_lo(ring, S::kKvSlice);
     const uint32_t id_s = instr_desc(kHalf, BN, false), id_o = instr_desc(kHalf, D, true);
     uint32_t stage = 0, fill = 0;      // next ring entry to consume
     uint32_t s_count = 0, p_count = 0; // S tiles issued, P tiles consumed (all segments)
@@ -1015,14 +1247,14 @@ __global__ void __launch_bounds__(Shape<D, MT>::kThreads, 1)
         }
         tc_fence_after();
         const int buf = MT == 2 ? i & 1 : (int)(s_count & 1u);
-        const uint32_t qa = sq + (MT == 2 ? (i & 1) * S::kSlices * S::kQSlice : 0);
-        const uint32_t ka = ring + k_stage * S::kTileBytes;
+        const uint32_t qa = q_desc + (MT == 2 ? (i & 1) * (S::kSlices * S::kQSlice >> 4) : 0);
+        const uint32_t ka = k_desc + k_stage * (S::kTileBytes >> 4);
 #pragma unroll
         for (int sl = 0; sl < S::kSlices; ++sl)
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
-            mma_ss(tmem + buf * 128, smem_desc(qa + sl * S::kQSlice + kk * 32, 0),
-                   smem_desc(ka + sl * S::kKvSlice + kk * 32, 0), id_s, sl + kk > 0);
+            mma_ss(tmem + buf * 128, desc_of(qa + (sl * S::kQSlice >> 4) + 2 * kk),
+                   desc_of(ka + (sl * S::kKvSlice >> 4) + 2 * kk), id_s, sl + kk > 0);
         mma_commit(&ctl->s_full[buf]);
         if (MT == 1 || (i & 1)) mma_commit(&ctl->empty[k_stage]);
         if (i == steps - 1) mma_commit(&ctl->q_empty);
@@ -1040,11 +1272,11 @@ __global__ void __launch_bounds__(Shape<D, MT>::kThreads, 1)
         ok = wait_bar(&ctl->p_ready[buf], (p_count >> 1) & 1u, ctl, a.status);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t va = ring + v_stage * S::kTileBytes;
+        const uint32_t va = v_desc + v_stage * (S::kTileBytes >> 4);
         const uint32_t to = tmem + kTmemO + (MT == 2 ? (i & 1) * D : 0);
 #pragma unroll
         for (int kk = 0; kk < BN / 16; ++kk)
-          mma_ts(to, tmem + buf * 128 + kk * 8, smem_desc(va + kk * 2048, S::kKvSlice), id_o,
+          mma_ts(to, tmem + buf * 128 + kk * 8, desc_of(va + kk * (2048 >> 4)), id_o,
                  i >= MT || kk > 0);
         mma_commit(&ctl->pv_done[MT == 2 ? i & 1 : 0]);
         if (MT == 1 || (i & 1)) mma_commit(&ctl->empty[v_stage]);
@@ -1076,16 +1308,16 @@ long long max_units(long long q_tokens, int seqs, int unit_tokens) {
   return q_tokens / unit_tokens + seqs;
 }
 
-template <int D, int MT, int KV>
-cudaError_t launch(const PrefillParams& p, cudaStream_t stream) {
-  using S = Shape<D, MT>;
+template <int D, int MT, int KV, bool TMA>
+cudaError_t launch(const PrefillParams& p, const CUtensorMap (&maps)[3], cudaStream_t stream) {
+  using S = Shape<D, MT, TMA>;
   static bool configured[64] = {};
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return err;
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   if (!configured[dev]) {
-    err = cudaFuncSetAttribute(attn_prefill_kernel<D, MT, KV>,
+    err = cudaFuncSetAttribute(attn_prefill_kernel<D, MT, KV, TMA>,
                                cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem);
     if (err != cudaSuccess) return err;
     configured[dev] = true;
@@ -1096,15 +1328,75 @@ cudaError_t launch(const PrefillParams& p, cudaStream_t stream) {
   err = launch_pdl(attn_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, p,
                    MT * p.tile_tokens, S::kBN, sms);
   if (err != cudaSuccess) return err;
-  return launch_pdl(attn_prefill_kernel<D, MT, KV>, dim3((unsigned)sms), dim3(S::kThreads),
-                    S::kSmem, stream, p);
+  return launch_pdl(attn_prefill_kernel<D, MT, KV, TMA>, dim3((unsigned)sms), dim3(S::kThreads),
+                    S::kSmem, stream, p, maps[0], maps[1], maps[2]);
+}
+
+// Tensor maps of q [tokens][heads][D] and of the cache [page][head][token][D]
+// (the two middle ones in the order of their strides). False where a map cannot
+// describe the call: pages that are no multiple of 8 tokens (a swizzle atom),
+// strides of zero, layouts the encoder declines.
+bool make_maps(PrefillParams& p, int bn, CUtensorMap (&maps)[3]) {
+  const AttnLaunch& a = p.a;
+  int rows = 8;
+  if (a.c.page_size % 8) return false;
+  while (rows < bn && a.c.page_size % (2 * rows) == 0) rows *= 2;
+  tcg_host::EncodeTiledFn fn = tcg_host::encode_tiled();
+  if (fn == nullptr) return false;
+  const CUtensorMapDataType type = a.q_f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                           : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const cuuint32_t ones[4] = {1, 1, 1, 1};
+  const cuuint64_t d = (cuuint64_t)a.c.head_dim;
+  // a dimension of one element has no stride of its own
+  auto bytes = [&](long long stride, long long size, cuuint64_t other) {
+    return size == 1 ? other : (cuuint64_t)stride * 2;
+  };
+  {
+    const cuuint64_t hs = bytes(a.q_head_stride, a.q_heads, d * 2);
+    const cuuint64_t ts = bytes(a.q_token_stride, a.q_tokens, hs * (cuuint64_t)a.q_heads);
+    if (hs == 0 || ts == 0) return false;
+    const cuuint64_t dims[3] = {d, (cuuint64_t)a.q_heads, (cuuint64_t)a.q_tokens};
+    const cuuint64_t strides[2] = {hs, ts};
+    const cuuint32_t box[3] = {64, (cuuint32_t)p.groups, (cuuint32_t)p.tile_tokens};
+    if (fn(&maps[0], type, 3, const_cast<void*>(a.q), dims, strides, box, ones,
+           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+           CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return false;
+  }
+  const cuuint64_t ts = bytes(a.c.token_stride, a.c.page_size, d * 2);
+  const cuuint64_t hs = bytes(a.c.head_stride, a.c.heads, ts * (cuuint64_t)a.c.page_size);
+  const cuuint64_t ps =
+      bytes(a.c.page_stride, a.c.num_pages,
+            (ts > hs ? ts * (cuuint64_t)a.c.page_size : hs * (cuuint64_t)a.c.heads));
+  if (ts == 0 || hs == 0 || ps == 0) return false;
+  p.heads_first = hs < ts;
+  p.box_rows = rows;
+  const cuuint64_t np = (cuuint64_t)a.c.num_pages, nt = (cuuint64_t)a.c.page_size;
+  const cuuint64_t nh = (cuuint64_t)a.c.heads;
+  const cuuint64_t dims[4] = {d, p.heads_first ? nh : nt, p.heads_first ? nt : nh, np};
+  const cuuint64_t strides[3] = {p.heads_first ? hs : ts, p.heads_first ? ts : hs, ps};
+  const cuuint32_t r = (cuuint32_t)rows;
+  const cuuint32_t box[4] = {64, p.heads_first ? 1u : r, p.heads_first ? r : 1u, 1};
+  for (int i = 0; i < 2; ++i)
+    if (fn(&maps[1 + i], type, 4, i ? a.c.v : a.c.k, dims, strides, box, ones,
+           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return false;
+  return true;
 }
 
 template <int D, int MT>
-cudaError_t launch_type(const PrefillParams& p, cudaStream_t stream) {
+cudaError_t launch_type(PrefillParams& p, cudaStream_t stream) {
+  CUtensorMap maps[3] = {};
   if (p.a.cache_dtype == 3)
-    return p.a.q_f16 ? launch<D, MT, kE4m3F16>(p, stream) : launch<D, MT, kE4m3Bf16>(p, stream);
-  return p.a.q_f16 ? launch<D, MT, kF16>(p, stream) : launch<D, MT, kBf16>(p, stream);
+    return p.a.q_f16 ? launch<D, MT, kE4m3F16, false>(p, maps, stream)
+                     : launch<D, MT, kE4m3Bf16, false>(p, maps, stream);
+  if (make_maps(p, Shape<D, MT, true>::kBN, maps))
+    return p.a.q_f16 ? launch<D, MT, kF16, true>(p, maps, stream)
+                     : launch<D, MT, kBf16, true>(p, maps, stream);
+  p.box_rows = 1;
+  return p.a.q_f16 ? launch<D, MT, kF16, false>(p, maps, stream)
+                   : launch<D, MT, kBf16, false>(p, maps, stream);
 }
 
 }  // namespace
@@ -1122,6 +1414,7 @@ cudaError_t launch_attn_prefill(const AttnLaunch& l, cudaStream_t stream) {
   p.groups = l.q_heads / l.c.heads;
   p.tile_tokens = 128 / p.groups;
   p.scale_log2 = l.scale * kLog2e;
+  p.box_rows = 1;
   const long long sms = device_sm_count();
   p.max_units = (int)max_units(l.q_tokens, l.seqs, 1);
   uint8_t* at = l.scratch;
