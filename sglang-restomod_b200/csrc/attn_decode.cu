@@ -11,14 +11,14 @@
 // per cached element against 2 rows' multiply-adds per element, far below the
 // tensor rate, so the work is to keep enough loads in flight:
 //
-// * The sequences' key ranges, in tiles of 64 tokens, are laid end to end over
+// * The sequences' key ranges, in tiles of 64 or 128 tokens, are laid end to end over
 //   (sequence, head, tile) and cut into equal ranges, one per block, so uneven
 //   lengths leave no block idle. A block finds its range from kv_lens itself
 //   (no host knowledge of the lengths, no planning launch). A (sequence, head)
 //   cut by a range border leaves partial (O, m, l) in the scratch; the last
 //   block to arrive at the pair's counter adds them in block order, so the
 //   result does not depend on which block that is.
-// * Each warp streams its own 16 of a tile's 64 tokens through a private ring
+// * Each warp streams its own quarter of a tile's tokens through a private ring
 //   of cp.async stages: no block barrier inside a pair, and the ring runs on
 //   into the next pair while the present one is finished. Page numbers travel
 //   through the same ring one ring length ahead, so no load waits on another.
@@ -42,14 +42,12 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kTile = 64;           // tokens per block step
-constexpr int kWarpTokens = kTile / kWarps;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 8.f;        // log2 of the largest P before a rescale
 constexpr int kMaxCtas = 1024;      // arrival counters in the workspace
 // A block takes at least this many tiles: below it the pair's merge costs more
 // than the extra blocks bring.
-constexpr int kMinTiles = 2;
+constexpr int kMinTiles = 4;
 
 struct DecodeParams {
   AttnLaunch a;
@@ -63,7 +61,7 @@ enum { kBf16 = 0, kF16 = 1, kE4m3 = 2 };
 // One ring entry's description, written when its page numbers are requested.
 struct TileInfo {
   int seq, head;   // seq < 0: past the block's range
-  int token0;      // first token of this warp's 16
+  int token0;      // first of this warp's tokens
   int end;         // tokens from here on do not exist
 };
 
@@ -71,12 +69,18 @@ template <int D, int KV, int NR>
 struct Shape {
   static constexpr int kElem = KV == kE4m3 ? 1 : 2;
   static constexpr int kRowBytes = D * kElem;
-  static constexpr int kStageBytes = 2 * kWarpTokens * kRowBytes;  // K then V of a warp
+  // Tokens of a warp's step: 32 where the stages stay small, so that what a
+  // step costs besides its products (copies' addresses, ring, masks) is spread
+  // over two m16 tiles whose chains of instructions also fill each other's gaps.
+  static constexpr int kTokens = kRowBytes <= 128 ? 32 : 16;
+  static constexpr int kTiles16 = kTokens / 16;
+  static constexpr int kTile = kTokens * kWarps;               // tokens per block step
+  static constexpr int kStageBytes = 2 * kTokens * kRowBytes;  // K then V of a warp
   static constexpr int kRows = 8 * NR;
-  // Ring depth: 80 to 96 KB per block and two blocks per SM; head_dim 256, whose
+  // Ring depth: 64 to 96 KB per block and two blocks per SM; head_dim 256, whose
   // stages are 32 to 64 KB, takes one block per SM with 160 to 192 KB.
   static constexpr int kBlocks = D == 256 ? 1 : 2;
-  static constexpr int kStages = KV == kE4m3 ? (D == 64 ? 10 : 5) : (D == 64 ? 5 : 3);
+  static constexpr int kStages = KV == kE4m3 ? (D == 64 ? 5 : D == 128 ? 3 : 5) : 3;
   static constexpr int kAhead = kStages - 1;
   static constexpr int kRing = 2 * kStages;  // page-number entries
   static constexpr int kQPitch = D + 8;      // 16-bit elements, conflict-free rows
@@ -85,11 +89,11 @@ struct Shape {
     uint8_t stage[kWarps][kStages][kStageBytes];
     uint16_t q[kRows][kQPitch];
     float merge[kRows][kMergePitch];
-    int pages[kWarps][kRing][kWarpTokens];
+    int pages[kWarps][kRing][kTokens];
     TileInfo info[kWarps][kRing];
     float row_scale[kRows];
     int row_lo[kRows], row_hi[kRows];
-    float wm[kWarps][kRows], wl[kWarps][kRows];
+    float wm[kWarps][kRows], wl[kWarps][kRows], mx[kRows];
     int wv[kWarps];
     long long scan[kWarps];
     int start_seq;
@@ -174,6 +178,7 @@ __device__ __forceinline__ int chunk_at(int row, int chunk) {
 struct SeqRange {
   int begin, end, q_len, kv_len, tiles;
 };
+template <int kTile>
 __device__ __forceinline__ SeqRange seq_range(const AttnLaunch& a, int s) {
   SeqRange r;
   const int q0 = __ldg(a.q_starts + s), q1 = __ldg(a.q_starts + s + 1);
@@ -215,7 +220,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV, NR>::kBlocks) attn_deco
     const int per = (a.seqs + kThreads - 1) / kThreads;
     const int s0 = tid * per, s1 = min(s0 + per, a.seqs);
     long long mine = 0;
-    for (int s = s0; s < s1; ++s) mine += (long long)seq_range(a, s).tiles * heads;
+    for (int s = s0; s < s1; ++s) mine += (long long)seq_range<S::kTile>(a, s).tiles * heads;
     long long before = mine;  // inclusive scan, made exclusive below
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -239,7 +244,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV, NR>::kBlocks) attn_deco
     if (t0 >= before && t0 < before + mine) {
       int s = s0;
       for (;; ++s) {
-        const long long n = (long long)seq_range(a, s).tiles * heads;
+        const long long n = (long long)seq_range<S::kTile>(a, s).tiles * heads;
         if (t0 < before + n) break;
         before += n;
       }
@@ -254,7 +259,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV, NR>::kBlocks) attn_deco
 
   // ---- the request cursor: page numbers of the warp's next tile
   int r_seq = sm.start_seq, r_head, r_tile;
-  SeqRange r_range = seq_range(a, r_seq);
+  SeqRange r_range = seq_range<S::kTile>(a, r_seq);
   r_head = (int)(sm.start_off / r_range.tiles);
   r_tile = (int)(sm.start_off - (long long)r_head * r_range.tiles);
   long long r_at = t0;
@@ -272,9 +277,9 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV, NR>::kBlocks) attn_deco
     ti.end = 0;
     if (r_at < t1) {
       ti.seq = r_seq;
-      ti.token0 = r_range.begin + r_tile * kTile + warp * kWarpTokens;
+      ti.token0 = r_range.begin + r_tile * S::kTile + warp * S::kTokens;
       ti.end = r_range.end;
-      if (lane < kWarpTokens && ti.token0 + lane < ti.end) {
+      if (lane < S::kTokens && ti.token0 + lane < ti.end) {
         const int* src = a.table + r_seq * a.table_stride + page_of(ti.token0 + lane);
         int* dst = &sm.pages[warp][r_slot][lane];
         if (now)
@@ -289,7 +294,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV, NR>::kBlocks) attn_deco
           r_head = 0;
           if (r_at < t1) {
             do {
-              r_range = seq_range(a, ++r_seq);
+              r_range = seq_range<S::kTile>(a, ++r_seq);
             } while (r_range.tiles == 0);
           }
         }
@@ -305,14 +310,14 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV, NR>::kBlocks) attn_deco
     if (ti.seq >= 0) {
       constexpr int kChunks = S::kRowBytes / 16;
       uint8_t* ks = sm.stage[warp][stage];
-      uint8_t* vs = ks + kWarpTokens * S::kRowBytes;
+      uint8_t* vs = ks + S::kTokens * S::kRowBytes;
       const long long head_off = (long long)ti.head * a.c.head_stride;
-      // byte offset of token row lane & 15, or -1
+      // byte offset of token row lane % kTokens, or -1
       long long mine = -1;
       {
-        const int token = ti.token0 + (lane & 15);
+        const int token = ti.token0 + lane % S::kTokens;
         if (token < ti.end) {
-          const int page = sm.pages[warp][slot][lane & 15];
+          const int page = sm.pages[warp][slot][lane % S::kTokens];
           const int at_page = token - page_of(token) * a.c.page_size;
           if (page >= 0 && page < a.c.num_pages)
             mine = (page * a.c.page_stride + at_page * a.c.token_stride + head_off) * S::kElem;
@@ -321,7 +326,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV, NR>::kBlocks) attn_deco
         }
       }
 #pragma unroll
-      for (int i = 0; i < kWarpTokens * kChunks / 32; ++i) {
+      for (int i = 0; i < S::kTokens * kChunks / 32; ++i) {
         const int id = i * 32 + lane;
         const int row = id / kChunks, chunk = id % kChunks;
         long long off = __shfl_sync(0xffffffffu, mine, row);
@@ -334,19 +339,19 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV, NR>::kBlocks) attn_deco
       }
     }
   };
-  // The scale byte of this lane's token in ring entry `slot`: keys in lanes
-  // 0-15, values in 16-31. 0 (2^-127, and codes of zero) for absent tokens.
-  auto scale_byte = [&](int slot) -> uint32_t {
+  // The scale bytes of token lane % kTokens in ring entry `slot`: the key's,
+  // the value's << 8. 0 (2^-127, and codes of zero) for absent tokens.
+  auto scale_bytes = [&](int slot) -> uint32_t {
     if (KV != kE4m3) return 0;
     const TileInfo ti = sm.info[warp][slot];
-    const int row = lane & 15, token = ti.token0 + row;
+    const int row = lane % S::kTokens, token = ti.token0 + row;
     if (ti.seq < 0 || token >= ti.end) return 0;
     const int page = sm.pages[warp][slot][row];
     if (page < 0 || page >= a.c.num_pages) return 0;
-    const uint8_t* base = lane < 16 ? a.c.k_scale : a.c.v_scale;
-    return __ldg(base + page * a.c.scale_page_stride +
-                 (token - page_of(token) * a.c.page_size) * a.c.scale_token_stride +
-                 ti.head * a.c.scale_head_stride);
+    const long long at = page * a.c.scale_page_stride +
+                         (token - page_of(token) * a.c.page_size) * a.c.scale_token_stride +
+                         ti.head * a.c.scale_head_stride;
+    return __ldg(a.c.k_scale + at) | (uint32_t)__ldg(a.c.v_scale + at) << 8;
   };
 
   // ---- prologue
@@ -357,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV, NR>::kBlocks) attn_deco
     request(false);
     cp_async_commit();
   }
-  uint32_t next_byte = scale_byte(0);
+  uint32_t next_bytes = scale_bytes(0);
 
   // ---- consume
   float o[D / 16][NR][4];
@@ -371,10 +376,10 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV, NR>::kBlocks) attn_deco
     cp_async_wait<S::kAhead - 1>();
     __syncwarp();
     const TileInfo first = sm.info[warp][slot];
-    const SeqRange range = seq_range(a, first.seq);
+    const SeqRange range = seq_range<S::kTile>(a, first.seq);
     const int head = first.head;
     const long long u0 =
-        at - (first.token0 - warp * kWarpTokens - range.begin) / kTile;
+        at - (first.token0 - warp * S::kTokens - range.begin) / S::kTile;
     const long long u1 = u0 + range.tiles;
     const long long pair_end = u1 < t1 ? u1 : t1;
     const int q0 = __ldg(a.q_starts + first.seq);
@@ -456,8 +461,9 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV, NR>::kBlocks) attn_deco
 #pragma unroll
         for (int nr = 0; nr < NR; ++nr) load_q(ks, nr, qf[ks][nr][0], qf[ks][nr][1]);
     }
-    float row_scale[NR][2];
+    float row_scale[NR][2], raise_at[NR][2];
     int row_lo[NR][2], row_hi[NR][2];
+    int all_lo = 0, all_hi = 0x7fffffff;  // tokens that every row sees
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
@@ -466,8 +472,18 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV, NR>::kBlocks) attn_deco
         row_lo[nr][j] = sm.row_lo[8 * nr + 2 * c + j];
         row_hi[nr][j] = sm.row_hi[8 * nr + 2 * c + j];
         m[nr][j] = -INFINITY;
+        raise_at[nr][j] = -INFINITY;
         l[nr][j] = 0.f;
+        if (8 * nr + 2 * c + j < rows) {
+          all_lo = max(all_lo, row_lo[nr][j]);
+          all_hi = min(all_hi, row_hi[nr][j]);
+        }
       }
+#pragma unroll
+    for (int x = 1; x < 4; x <<= 1) {
+      all_lo = max(all_lo, __shfl_xor_sync(0xffffffffu, all_lo, x));
+      all_hi = min(all_hi, __shfl_xor_sync(0xffffffffu, all_hi, x));
+    }
     v_exp = 1;
 #pragma unroll
     for (int t = 0; t < D / 16; ++t)
@@ -480,7 +496,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV, NR>::kBlocks) attn_deco
       cp_async_wait<S::kAhead - 1>();
       __syncwarp();
       const int token0 = sm.info[warp][slot].token0;
-      const uint32_t byte = next_byte;
+      const uint32_t bytes = next_bytes;
       // refill: the stage freed last step, from the entry kAhead steps on
       {
         const int s2 = slot + S::kAhead < S::kRing ? slot + S::kAhead : slot + S::kAhead - S::kRing;
@@ -489,93 +505,132 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV, NR>::kBlocks) attn_deco
         cp_async_commit();
       }
       const uint8_t* ks_ptr = sm.stage[warp][stage];
-      const uint8_t* vs_ptr = ks_ptr + kWarpTokens * S::kRowBytes;
+      const uint8_t* vs_ptr = ks_ptr + S::kTokens * S::kRowBytes;
+      constexpr int kG = S::kTiles16;
 
       // -- S^T = K Q^T
-      float s[NR][4];
+      float s[kG][NR][4];
 #pragma unroll
-      for (int nr = 0; nr < NR; ++nr)
+      for (int t16 = 0; t16 < kG; ++t16)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[nr][j] = 0.f;
+        for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[t16][nr][j] = 0.f;
       if (KV != kE4m3) {
         const uint32_t base = smem_u32(ks_ptr);
-        const int row = lane & 15;
 #pragma unroll
         for (int ks = 0; ks < kSteps; ++ks) {
-          uint32_t af[4];
-          ldsm4(af, base + chunk_at<D, KV, false>(row, 2 * ks + (lane >> 4)));
+          uint32_t b[NR][2];
 #pragma unroll
           for (int nr = 0; nr < NR; ++nr) {
-            uint32_t b0, b1;
             if (kQInRegs) {
-              b0 = qf[kQInRegs ? ks : 0][nr][0];
-              b1 = qf[kQInRegs ? ks : 0][nr][1];
+              b[nr][0] = qf[kQInRegs ? ks : 0][nr][0];
+              b[nr][1] = qf[kQInRegs ? ks : 0][nr][1];
             } else {
-              load_q(ks, nr, b0, b1);
+              load_q(ks, nr, b[nr][0], b[nr][1]);
             }
-            mma<KV>(s[nr], af, b0, b1);
+          }
+#pragma unroll
+          for (int t16 = 0; t16 < kG; ++t16) {
+            uint32_t af[4];
+            ldsm4(af, base + chunk_at<D, KV, false>(16 * t16 + (lane & 15), 2 * ks + (lane >> 4)));
+#pragma unroll
+            for (int nr = 0; nr < NR; ++nr) mma<KV>(s[t16][nr], af, b[nr][0], b[nr][1]);
           }
         }
       } else {
 #pragma unroll
         for (int q4 = 0; q4 < D / 64; ++q4) {
-          const uint4 lo = ld_shared_u128(ks_ptr + chunk_at<D, KV, false>(g, c + 4 * q4));
-          const uint4 hi = ld_shared_u128(ks_ptr + chunk_at<D, KV, false>(g + 8, c + 4 * q4));
-          const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
+          uint32_t wl[kG][4], wh[kG][4];
+#pragma unroll
+          for (int t16 = 0; t16 < kG; ++t16) {
+            const uint4 x = ld_shared_u128(ks_ptr + chunk_at<D, KV, false>(16 * t16 + g, c + 4 * q4));
+            const uint4 y =
+                ld_shared_u128(ks_ptr + chunk_at<D, KV, false>(16 * t16 + g + 8, c + 4 * q4));
+            wl[t16][0] = x.x, wl[t16][1] = x.y, wl[t16][2] = x.z, wl[t16][3] = x.w;
+            wh[t16][0] = y.x, wh[t16][1] = y.y, wh[t16][2] = y.z, wh[t16][3] = y.w;
+          }
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            uint32_t af[4];
-            // byte pairs (2, 3) and (0, 1) of a word: the k order load_q gives Q
-            af[0] = e4m3x2_to_f16x2((uint16_t)(wl[j] >> 16));
-            af[1] = e4m3x2_to_f16x2((uint16_t)(wh[j] >> 16));
-            af[2] = e4m3x2_to_f16x2((uint16_t)wl[j]);
-            af[3] = e4m3x2_to_f16x2((uint16_t)wh[j]);
+            uint32_t b[NR][2];
 #pragma unroll
             for (int nr = 0; nr < NR; ++nr) {
-              uint32_t b0, b1;
               if (kQInRegs) {
-                b0 = qf[kQInRegs ? 4 * q4 + j : 0][nr][0];
-                b1 = qf[kQInRegs ? 4 * q4 + j : 0][nr][1];
+                b[nr][0] = qf[kQInRegs ? 4 * q4 + j : 0][nr][0];
+                b[nr][1] = qf[kQInRegs ? 4 * q4 + j : 0][nr][1];
               } else {
-                load_q(4 * q4 + j, nr, b0, b1);
+                load_q(4 * q4 + j, nr, b[nr][0], b[nr][1]);
               }
-              mma<KV>(s[nr], af, b0, b1);
+            }
+#pragma unroll
+            for (int t16 = 0; t16 < kG; ++t16) {
+              uint32_t af[4];
+              // byte pairs (2, 3) and (0, 1) of a word: the k order load_q gives Q
+              af[0] = e4m3x2_to_f16x2((uint16_t)(wl[t16][j] >> 16));
+              af[1] = e4m3x2_to_f16x2((uint16_t)(wh[t16][j] >> 16));
+              af[2] = e4m3x2_to_f16x2((uint16_t)wl[t16][j]);
+              af[3] = e4m3x2_to_f16x2((uint16_t)wh[t16][j]);
+#pragma unroll
+              for (int nr = 0; nr < NR; ++nr) mma<KV>(s[t16][nr], af, b[nr][0], b[nr][1]);
             }
           }
         }
       }
 
       // -- scales, masks, lazy maximum
-      float k_scale[2] = {1.f, 1.f};
-      int v_byte[2] = {0, 0};
+      int v_byte[kG][2] = {};
       bool raise_v = false;
       if (KV == kE4m3) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const uint32_t kb = __shfl_sync(0xffffffffu, byte, g + 8 * j);
-          k_scale[j] = kb == 255u ? __int_as_float(0x7fc00000) : __uint_as_float(kb << 23);
-          v_byte[j] = (int)__shfl_sync(0xffffffffu, byte, 16 + g + 8 * j);
-          raise_v |= v_byte[j] > v_exp && v_byte[j] != 255;
-        }
-        next_byte = scale_byte(slot + 1 == S::kRing ? 0 : slot + 1);
+        for (int t16 = 0; t16 < kG; ++t16)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint32_t both = __shfl_sync(0xffffffffu, bytes, 16 * t16 + g + 8 * j);
+            const uint32_t kb = both & 0xffu;
+            const float k_scale = kb == 255u ? __int_as_float(0x7fc00000) : __uint_as_float(kb << 23);
+            v_byte[t16][j] = (int)(both >> 8);
+            raise_v |= v_byte[t16][j] > v_exp && v_byte[t16][j] != 255;
+#pragma unroll
+            for (int nr = 0; nr < NR; ++nr) {
+              s[t16][nr][2 * j] *= k_scale;
+              s[t16][nr][2 * j + 1] *= k_scale;
+            }
+          }
+        next_bytes = scale_bytes(slot + 1 == S::kRing ? 0 : slot + 1);
       }
       bool raise = false;
 #pragma unroll
-      for (int nr = 0; nr < NR; ++nr)
+      for (int t16 = 0; t16 < kG; ++t16)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int token = token0 + g + 8 * (j >> 1);
-          const bool seen = token >= row_lo[nr][j & 1] && token < row_hi[nr][j & 1];
-          float x = s[nr][j] * row_scale[nr][j & 1];
-          if (KV == kE4m3) x *= k_scale[j >> 1];
-          x = seen ? x : -INFINITY;
-          s[nr][j] = x;
-          raise |= x > m[nr][j & 1] + kLazy;
-        }
+        for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[t16][nr][j] *= row_scale[nr][j & 1];
+      if (token0 < all_lo || token0 + S::kTokens > all_hi) {
+#pragma unroll
+        for (int t16 = 0; t16 < kG; ++t16)
+#pragma unroll
+          for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int token = token0 + 16 * t16 + g + 8 * (j >> 1);
+              const bool seen = token >= row_lo[nr][j & 1] && token < row_hi[nr][j & 1];
+              s[t16][nr][j] = seen ? s[t16][nr][j] : -INFINITY;
+            }
+      }
+#pragma unroll
+      for (int t16 = 0; t16 < kG; ++t16)
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) raise |= s[t16][nr][j] > raise_at[nr][j & 1];
       if (__any_sync(0xffffffffu, raise || raise_v)) {
         float o_scale[NR][2];
-        int top = max(v_exp, max(v_byte[0] == 255 ? 0 : v_byte[0], v_byte[1] == 255 ? 0 : v_byte[1]));
+        int top = v_exp;
         if (KV == kE4m3) {
+#pragma unroll
+          for (int t16 = 0; t16 < kG; ++t16)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) top = max(top, v_byte[t16][j] == 255 ? 0 : v_byte[t16][j]);
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, x));
         }
@@ -586,14 +641,18 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV, NR>::kBlocks) attn_deco
         for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            float mx = fmaxf(s[nr][j], s[nr][j + 2]);
+            float mx = fmaxf(s[0][nr][j], s[0][nr][j + 2]);
+#pragma unroll
+            for (int t16 = 1; t16 < kG; ++t16)
+              mx = fmaxf(mx, fmaxf(s[t16][nr][j], s[t16][nr][j + 2]));
 #pragma unroll
             for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
             // a row that nothing pushed past the threshold keeps its maximum
-            const float mn = mx > m[nr][j] + kLazy ? mx : m[nr][j];
+            const float mn = mx > raise_at[nr][j] ? mx : m[nr][j];
             const float f = m[nr][j] == mn ? 1.f : exp2_fast(m[nr][j] - mn);
             l[nr][j] *= f;
             m[nr][j] = mn;
+            raise_at[nr][j] = mn + kLazy;
             o_scale[nr][j] = f * v_ratio;
           }
 #pragma unroll
@@ -605,84 +664,91 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV, NR>::kBlocks) attn_deco
       }
 
       // -- P^T, as the B operand
-      float v_scale[2];
+      uint32_t pf[kG][NR][2];
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-        v_scale[j] = KV != kE4m3 ? 1.f
-                     : v_byte[j] == 255 ? __int_as_float(0x7fc00000)
-                                        : pow2(v_byte[j] - v_exp);
-      uint32_t pf[NR][2];
+      for (int t16 = 0; t16 < kG; ++t16) {
+        float v_scale[2];
 #pragma unroll
-      for (int nr = 0; nr < NR; ++nr) {
-        float pr[4];
+        for (int j = 0; j < 2; ++j)
+          v_scale[j] = KV != kE4m3 ? 1.f
+                       : v_byte[t16][j] == 255 ? __int_as_float(0x7fc00000)
+                                               : pow2(v_byte[t16][j] - v_exp);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float base = m[nr][j & 1] == -INFINITY ? 0.f : m[nr][j & 1];
-          pr[j] = exp2_fast(s[nr][j] - base);
-          l[nr][j & 1] += pr[j];
-          // a masked token's P is zero whatever its value's scale says
-          if (KV == kE4m3) pr[j] = pr[j] == 0.f ? 0.f : pr[j] * v_scale[j >> 1];
-        }
+        for (int nr = 0; nr < NR; ++nr) {
+          float pr[4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t pk;
-          if (KV == kBf16) {
-            const __nv_bfloat162 b = __floats2bfloat162_rn(pr[2 * h], pr[2 * h + 1]);
-            pk = *reinterpret_cast<const uint32_t*>(&b);
-          } else {
-            const __half2 b = __floats2half2_rn(pr[2 * h], pr[2 * h + 1]);
-            pk = *reinterpret_cast<const uint32_t*>(&b);
+          for (int j = 0; j < 4; ++j) {
+            const float base = m[nr][j & 1] == -INFINITY ? 0.f : m[nr][j & 1];
+            pr[j] = exp2_fast(s[t16][nr][j] - base);
+            l[nr][j & 1] += pr[j];
+            // a masked token's P is zero whatever its value's scale says
+            if (KV == kE4m3) pr[j] = pr[j] == 0.f ? 0.f : pr[j] * v_scale[j >> 1];
           }
-          pf[nr][h] = transpose8x8(pk);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t pk;
+            if (KV == kBf16) {
+              const __nv_bfloat162 b = __floats2bfloat162_rn(pr[2 * h], pr[2 * h + 1]);
+              pk = *reinterpret_cast<const uint32_t*>(&b);
+            } else {
+              const __half2 b = __floats2half2_rn(pr[2 * h], pr[2 * h + 1]);
+              pk = *reinterpret_cast<const uint32_t*>(&b);
+            }
+            pf[t16][nr][h] = transpose8x8(pk);
+          }
         }
       }
 
       // -- O^T += V^T P^T
-      if (KV != kE4m3) {
-        const uint32_t base = smem_u32(vs_ptr);
-        // matrices: (tokens 0-7, columns 0-7), (0-7, 8-15), (8-15, 0-7), (8-15, 8-15)
-        const int row = (lane & 7) + ((lane >> 4) << 3);
 #pragma unroll
-        for (int t = 0; t < D / 16; ++t) {
-          uint32_t af[4];
-          ldsm4_t(af, base + chunk_at<D, KV, true>(row, 2 * t + ((lane >> 3) & 1)));
+      for (int t16 = 0; t16 < kG; ++t16) {
+        if (KV != kE4m3) {
+          const uint32_t base = smem_u32(vs_ptr);
+          // matrices: (tokens 0-7, columns 0-7), (0-7, 8-15), (8-15, 0-7), (8-15, 8-15)
+          const int row = 16 * t16 + (lane & 7) + ((lane >> 4) << 3);
 #pragma unroll
-          for (int nr = 0; nr < NR; ++nr) mma<KV>(o[t][nr], af, pf[nr][0], pf[nr][1]);
-        }
-      } else {
-        // lane group g holds 16 (head_dim 64: 8) neighbouring columns of the
-        // tokens 2c, 2c + 1, 2c + 8, 2c + 9; tile t takes columns 2t, 2t + 1
-        constexpr int kHalf = D >= 128 ? D / 128 : 1;
-#pragma unroll
-        for (int hf = 0; hf < kHalf; ++hf) {
-          uint32_t w[4][4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int row = 2 * c + (i & 1) + 8 * (i >> 1);
-            if (D >= 128) {
-              const uint4 x = ld_shared_u128(vs_ptr + chunk_at<D, KV, true>(row, g + 8 * hf));
-              w[i][0] = x.x;
-              w[i][1] = x.y;
-              w[i][2] = x.z;
-              w[i][3] = x.w;
-            } else {
-              const uint2 x = *reinterpret_cast<const uint2*>(
-                  vs_ptr + chunk_at<D, KV, true>(row, g >> 1) + (g & 1) * 8);
-              w[i][0] = x.x;
-              w[i][1] = x.y;
-            }
-          }
-#pragma unroll
-          for (int t = 0; t < (D >= 128 ? 8 : 4); ++t) {
-            const uint32_t x = __byte_perm(w[0][t / 2], w[1][t / 2], t & 1 ? 0x7362 : 0x5140);
-            const uint32_t y = __byte_perm(w[2][t / 2], w[3][t / 2], t & 1 ? 0x7362 : 0x5140);
+          for (int t = 0; t < D / 16; ++t) {
             uint32_t af[4];
-            af[0] = e4m3x2_to_f16x2((uint16_t)x);
-            af[1] = e4m3x2_to_f16x2((uint16_t)(x >> 16));
-            af[2] = e4m3x2_to_f16x2((uint16_t)y);
-            af[3] = e4m3x2_to_f16x2((uint16_t)(y >> 16));
+            ldsm4_t(af, base + chunk_at<D, KV, true>(row, 2 * t + ((lane >> 3) & 1)));
 #pragma unroll
-            for (int nr = 0; nr < NR; ++nr) mma<KV>(o[8 * hf + t][nr], af, pf[nr][0], pf[nr][1]);
+            for (int nr = 0; nr < NR; ++nr) mma<KV>(o[t][nr], af, pf[t16][nr][0], pf[t16][nr][1]);
+          }
+        } else {
+          // lane group g holds 16 (head_dim 64: 8) neighbouring columns of the
+          // tokens 2c, 2c + 1, 2c + 8, 2c + 9; tile t takes columns 2t, 2t + 1
+          constexpr int kHalf = D >= 128 ? D / 128 : 1;
+#pragma unroll
+          for (int hf = 0; hf < kHalf; ++hf) {
+            uint32_t w[4][4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int row = 16 * t16 + 2 * c + (i & 1) + 8 * (i >> 1);
+              if (D >= 128) {
+                const uint4 x = ld_shared_u128(vs_ptr + chunk_at<D, KV, true>(row, g + 8 * hf));
+                w[i][0] = x.x;
+                w[i][1] = x.y;
+                w[i][2] = x.z;
+                w[i][3] = x.w;
+              } else {
+                const uint2 x = *reinterpret_cast<const uint2*>(
+                    vs_ptr + chunk_at<D, KV, true>(row, g >> 1) + (g & 1) * 8);
+                w[i][0] = x.x;
+                w[i][1] = x.y;
+              }
+            }
+#pragma unroll
+            for (int t = 0; t < (D >= 128 ? 8 : 4); ++t) {
+              const uint32_t x = __byte_perm(w[0][t / 2], w[1][t / 2], t & 1 ? 0x7362 : 0x5140);
+              const uint32_t y = __byte_perm(w[2][t / 2], w[3][t / 2], t & 1 ? 0x7362 : 0x5140);
+              uint32_t af[4];
+              af[0] = e4m3x2_to_f16x2((uint16_t)x);
+              af[1] = e4m3x2_to_f16x2((uint16_t)(x >> 16));
+              af[2] = e4m3x2_to_f16x2((uint16_t)y);
+              af[3] = e4m3x2_to_f16x2((uint16_t)(y >> 16));
+#pragma unroll
+              for (int nr = 0; nr < NR; ++nr)
+                mma<KV>(o[8 * hf + t][nr], af, pf[t16][nr][0], pf[t16][nr][1]);
+            }
           }
         }
       }
@@ -798,49 +864,56 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV, NR>::kBlocks) attn_deco
       }
       __syncthreads();
       if (sm.flag) {
-        // A warp per row: the parts' maximum, then their weighted sum.
+        // The parts' maximum, a warp per row; then their weighted sum, a thread
+        // per two columns and row at a time, eight parts in flight.
+        auto part_at = [&](int b) {
+          return scratch + (2ll * b + (b == c_first ? 1 : 0)) * slot_floats;
+        };
         for (int r = warp; r < rows; r += kWarps) {
           float mx = -INFINITY;
-          for (int b = c_first + lane; b <= c_last; b += 32) {
-            const float* src = scratch + (2ll * b + (b == c_first ? 1 : 0)) * slot_floats + r * row_floats;
-            mx = fmaxf(mx, __ldcg(src));
-          }
+          for (int b = c_first + lane; b <= c_last; b += 32)
+            mx = fmaxf(mx, __ldcg(part_at(b) + r * row_floats));
 #pragma unroll
           for (int x = 16; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-          float sum = 0.f, acc[D / 32];
+          if (lane == 0) sm.mx[r] = mx;
+        }
+        __syncthreads();
+        for (int i = tid; i < rows * (D / 2); i += kThreads) {
+          const int r = i / (D / 2), d = 2 * (i % (D / 2));
+          const float mx = sm.mx[r];
+          float sum = 0.f, x = 0.f, y = 0.f;
+          for (int b0 = c_first; b0 <= c_last; b0 += 8) {
+            float2 ml[8], v[8];
 #pragma unroll
-          for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
-#pragma unroll 4
-          for (int b = c_first; b <= c_last; ++b) {
-            const float* src = scratch + (2ll * b + (b == c_first ? 1 : 0)) * slot_floats + r * row_floats;
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(src));
-            const float w = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : exp2_fast(ml.x - mx);
-            sum += ml.y * w;
+            for (int j = 0; j < 8; ++j) {
+              const float* src = part_at(min(b0 + j, c_last)) + r * row_floats;
+              ml[j] = __ldcg(reinterpret_cast<const float2*>(src));
+              v[j] = __ldcg(reinterpret_cast<const float2*>(src + 2 + d));
+            }
 #pragma unroll
-            for (int i = 0; i < D / 64; ++i) {
-              const float2 v = __ldcg(reinterpret_cast<const float2*>(src + 2 + 64 * i + 2 * lane));
-              acc[2 * i] += w == 0.f ? 0.f : v.x * w;
-              acc[2 * i + 1] += w == 0.f ? 0.f : v.y * w;
+            for (int j = 0; j < 8; ++j) {
+              // (a part without a visible key has m = -inf and l = 0, or NaN)
+              float w = ml[j].x == -INFINITY ? (ml[j].y == 0.f ? 0.f : 1.f) : exp2_fast(ml[j].x - mx);
+              if (b0 + j > c_last) w = 0.f;
+              sum += w == 0.f ? 0.f : ml[j].y * w;
+              x += w == 0.f ? 0.f : v[j].x * w;
+              y += w == 0.f ? 0.f : v[j].y * w;
             }
           }
           const float inv = sum == 0.f ? 0.f : 1.f / sum;
           const long long tok = q0 + r / p.groups;
           const int qh = head * p.groups + r % p.groups;
-          uint16_t* dst = static_cast<uint16_t*>(a.out) + tok * a.out_token_stride +
-                          qh * a.out_head_stride;
-#pragma unroll
-          for (int i = 0; i < D / 64; ++i) {
-            uint32_t pk;
-            if (a.q_f16) {
-              const __half2 b = __floats2half2_rn(acc[2 * i] * inv, acc[2 * i + 1] * inv);
-              pk = *reinterpret_cast<const uint32_t*>(&b);
-            } else {
-              const __nv_bfloat162 b = __floats2bfloat162_rn(acc[2 * i] * inv, acc[2 * i + 1] * inv);
-              pk = *reinterpret_cast<const uint32_t*>(&b);
-            }
-            *reinterpret_cast<uint32_t*>(dst + 64 * i + 2 * lane) = pk;
+          uint32_t pk;
+          if (a.q_f16) {
+            const __half2 b = __floats2half2_rn(x * inv, y * inv);
+            pk = *reinterpret_cast<const uint32_t*>(&b);
+          } else {
+            const __nv_bfloat162 b = __floats2bfloat162_rn(x * inv, y * inv);
+            pk = *reinterpret_cast<const uint32_t*>(&b);
           }
-          if (a.lse != nullptr && lane == 0)
+          *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + tok * a.out_token_stride +
+                                       qh * a.out_head_stride + d) = pk;
+          if (a.lse != nullptr && d == 0)
             a.lse[tok * a.q_heads + qh] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) / kLog2e;
         }
       }

@@ -70,13 +70,12 @@ __device__ __forceinline__ int scale_exponent(float top) {
 }
 
 // LPV lanes per vector, 8 values each. Each thread carries the same lane of
-// kUnroll vectors (key and value of kUnroll / 2 heads or tokens), so four
-// loads are in flight.
+// kUnroll vectors, key and value, so 2 * kUnroll loads are in flight.
 constexpr int kCopyThreads = 256;
-constexpr int kUnroll = 2;
+constexpr int kUnroll = 4;
 
 template <bool F16, bool QUANT, int LPV>
-__global__ void __launch_bounds__(kCopyThreads) kv_write_kernel(CopyParams p) {
+__global__ void __launch_bounds__(kCopyThreads, 4) kv_write_kernel(CopyParams p) {
   griddep_wait();
   const int lane = threadIdx.x % LPV;
   const long long stride = (long long)gridDim.x * (kCopyThreads / LPV);
@@ -157,7 +156,7 @@ __device__ __forceinline__ uint4 decode8(uint2 codes, uint8_t byte) {
 }
 
 template <bool F16, bool QUANT, int LPV>
-__global__ void __launch_bounds__(kCopyThreads) kv_read_kernel(CopyParams p) {
+__global__ void __launch_bounds__(kCopyThreads, 4) kv_read_kernel(CopyParams p) {
   griddep_wait();
   const int lane = threadIdx.x % LPV;
   const long long stride = (long long)gridDim.x * (kCopyThreads / LPV);

@@ -11,9 +11,12 @@
 //
 // Bound: HBM. Per element 2 B of x, 2 + 2 B of residual read and written,
 // 1 B of q (or 2 B of y). A row stays in its threads' registers between the
-// sum of squares and the scaling, so each byte moves once; the weights stay in
-// registers across a thread's rows. A group of 128 columns is 16 lanes x 8
-// columns, so its maximum is four shuffles.
+// sum of squares and the scaling, so each byte moves once; the weights come from
+// L1. Rows wider than 1024 columns take a block each and come by bulk copies
+// into a ring of stages, so that the next rows are on their way while one is
+// summed, scaled and stored; narrower ones (the per-head norms of queries and
+// keys) take a warp each, 8 in flight per block and no block barrier. A group
+// of 128 columns is 16 lanes x 8 columns, so its maximum is four shuffles.
 #include "common.cuh"
 #include "internal.h"
 
@@ -99,109 +102,174 @@ __device__ __forceinline__ uint4 load_row(const uint4* src) {
   return v;
 }
 
-// A row belongs to one warp (WARP) or to the whole block, V vectors of 8
-// columns to a thread. Up to V = 2 the next row's values are loaded while the
-// present ones are reduced; with V = 4 the registers do not hold both.
-//
-// Rows of up to 1024 columns (the per-head norms of queries and keys, small
-// hidden sizes) take a warp each: no block barrier, 8 rows in flight per block.
-template <bool F16, int V, bool WARP>
-__global__ void __launch_bounds__(WARP ? 256 : 1024) add_rms_norm_kernel(NormParams p) {
-  constexpr bool kPrefetch = V <= 2;
-  __shared__ float sums[2][32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int threads = WARP ? 32 : blockDim.x;
-  const int me = WARP ? lane : threadIdx.x;
-  const long long step = WARP ? (long long)gridDim.x * (blockDim.x >> 5) : gridDim.x;
-  long long row = WARP ? (long long)blockIdx.x * (blockDim.x >> 5) + warp : blockIdx.x;
-  griddep_wait();
+// The 8 columns y[vec] of a scaled row: 16-bit output, and the group's scale
+// and codes. Called by all lanes of a warp (h8 is a multiple of 16 with q, so
+// a group's 16 lanes are on together).
+template <bool F16>
+__device__ __forceinline__ void store_vec(const NormParams& p, long long row, int vec,
+                                          const float (&h)[8], float rstd) {
+  const bool on = vec < p.h8;
+  float y[8], w[8];
+  if (on) load_weight(p, vec, w);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = on ? h[i] * rstd * w[i] : 0.f;
+  if (p.y != nullptr && on) *vec_at(p.y, row, p.y_ld, vec) = pack8<F16>(y);
+  if (p.q == nullptr) return;
+  float amax = 0.f;
+  bool nan = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    amax = fmaxf(amax, fabsf(y[i]));
+    nan |= y[i] != y[i];
+  }
+  if (nan) amax = __int_as_float(0x7fc00000);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) {
+    const float other = __shfl_xor_sync(0xffffffffu, amax, o);
+    amax = amax != amax || other != other ? __int_as_float(0x7fc00000) : fmaxf(amax, other);
+  }
+  // A NaN in the group makes its scale NaN (fmaxf alone would drop it).
+  const float scale = amax != amax ? amax : fmaxf(amax / 448.f, 1e-8f);
+  if (!on) return;
+  uint16_t b[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;"
+        : "=h"(b[i])
+        : "f"(y[2 * i + 1] / scale), "f"(y[2 * i] / scale));
+  *reinterpret_cast<uint2*>(p.q + (row * p.h8 + vec) * 8) =
+      make_uint2(b[0] | (uint32_t)b[1] << 16, b[2] | (uint32_t)b[3] << 16);
+  if ((vec & 15) == 0) p.scales[(long long)(vec >> 4) * p.scales_ld + row] = scale;
+}
 
+// h = x (+ r) and the sum of its squares.
+template <bool F16>
+__device__ __forceinline__ float add_vec(const NormParams& p, uint4 x, uint4 r, float (&h)[8]) {
+  float rv[8], sum = 0.f;
+  unpack8<F16>(x, h);
+  unpack8<F16>(r, rv);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (p.residual != nullptr) h[i] += rv[i];
+    sum += h[i] * h[i];
+  }
+  return sum;
+}
+
+// A warp per row, V vectors of 8 columns per lane; the next row's values are
+// loaded while the present ones are reduced (V = 4: the registers do not hold both).
+template <bool F16, int V>
+__global__ void __launch_bounds__(256) add_rms_norm_warp_kernel(NormParams p) {
+  constexpr bool kPrefetch = V <= 2;
+  const int lane = threadIdx.x & 31;
+  const long long step = (long long)gridDim.x * (blockDim.x >> 5);
+  griddep_wait();
   uint4 xin[V], rin[V];
   auto fetch = [&](long long r) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const int vec = me + j * threads;
+      const int vec = lane + j * 32;
       const bool on = vec < p.h8 && r < p.rows;
       xin[j] = rin[j] = make_uint4(0u, 0u, 0u, 0u);
       if (on) xin[j] = load_row(vec_at(p.x, r, p.x_ld, vec));
       if (on && p.residual != nullptr) rin[j] = load_row(vec_at(p.residual, r, p.residual_ld, vec));
     }
   };
+  long long row = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   if (kPrefetch) fetch(row);
-  for (int parity = 0; row < p.rows; row += step, parity ^= 1) {
+  for (; row < p.rows; row += step) {
     if (!kPrefetch) fetch(row);
-    float h[V][8];
-    float sum = 0.f;
+    float h[V][8], sum = 0.f;
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      float r[8];
-      unpack8<F16>(xin[j], h[j]);
-      unpack8<F16>(rin[j], r);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (p.residual != nullptr) h[j][i] += r[i];
-        sum += h[j][i] * h[j][i];
-      }
-    }
-    // In-place outputs: row + step belongs to this thread group alone, so
-    // loading it before this row's stores is safe.
+    for (int j = 0; j < V; ++j) sum += add_vec<F16>(p, xin[j], rin[j], h[j]);
+    // In-place outputs: row + step is this warp's alone, so loading it before
+    // this row's stores is safe.
     if (kPrefetch) fetch(row + step);
-    if (p.residual_out != nullptr) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const int vec = me + j * threads;
-        if (vec < p.h8) *vec_at(p.residual_out, row, p.residual_out_ld, vec) = pack8<F16>(h[j]);
-      }
-    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (!WARP) {
-      // Two buffers in turn: a warp may write the next row's partial while
-      // another still reads this row's.
-      if (lane == 0) sums[parity][warp] = sum;
-      __syncthreads();
-      sum = lane < (blockDim.x >> 5) ? sums[parity][lane] : 0.f;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    }
     const float rstd = rsqrtf(sum * p.inv_hidden + p.eps);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const int vec = me + j * threads;
-      float y[8], w[8];
-      if (vec < p.h8) load_weight(p, vec, w);
+      const int vec = lane + j * 32;
+      if (p.residual_out != nullptr && vec < p.h8)
+        *vec_at(p.residual_out, row, p.residual_out_ld, vec) = pack8<F16>(h[j]);
+      store_vec<F16>(p, row, vec, h[j], rstd);
+    }
+  }
+  griddep_launch_dependents();
+}
+
+constexpr int kMaxStages = 4;
+
+// A block per row. Thread 0 keeps `stages` rows (x, then residual) in flight by
+// bulk copies; V vectors of 8 columns per thread.
+template <bool F16, int V>
+__global__ void __launch_bounds__(1024) add_rms_norm_kernel(NormParams p, int stages) {
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ uint64_t full[kMaxStages];
+  __shared__ float sums[2][32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t row_bytes = (uint32_t)p.h8 * 16;
+  const uint32_t stage_bytes = p.residual != nullptr ? 2 * row_bytes : row_bytes;
+  if (tid == 0) {
+    for (int i = 0; i < stages; ++i) mbar_init(&full[i], 1);
+    fence_mbar_init();
+  }
+  __syncthreads();
+  griddep_wait();
+  const uint64_t policy = l2_policy_evict_first();
+  auto issue = [&](long long r, int stage) {  // thread 0
+    if (r >= p.rows) return;
+    uint8_t* dst = ring + stage * stage_bytes;
+    mbar_arrive_expect_tx(&full[stage], stage_bytes);
+    bulk_g2s(dst, vec_at(p.x, r, p.x_ld, 0), row_bytes, &full[stage], policy);
+    if (p.residual != nullptr)
+      bulk_g2s(dst + row_bytes, vec_at(p.residual, r, p.residual_ld, 0), row_bytes, &full[stage],
+               policy);
+  };
+  const long long step = gridDim.x;
+  if (tid == 0)
+    for (int i = 0; i < stages; ++i) issue(blockIdx.x + i * step, i);
+  int stage = 0, phase = 0, parity = 0;
+  for (long long row = blockIdx.x; row < p.rows; row += step, parity ^= 1) {
+    // Bounded: a copy that never lands leaves its row's outputs wrong, not the
+    // kernel hanging.
+    mbar_wait(&full[stage], (uint32_t)phase, nullptr);
+    const uint4* xs = reinterpret_cast<const uint4*>(ring + stage * stage_bytes);
+    float h[V][8], sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = vec < p.h8 ? h[j][i] * rstd * w[i] : 0.f;
-      if (p.y != nullptr && vec < p.h8) *vec_at(p.y, row, p.y_ld, vec) = pack8<F16>(y);
-      if (p.q != nullptr) {
-        // h8 is a multiple of 16 here, so a group's 16 lanes are on together.
-        float amax = 0.f;
-        bool nan = false;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          amax = fmaxf(amax, fabsf(y[i]));
-          nan |= y[i] != y[i];
-        }
-        if (nan) amax = __int_as_float(0x7fc00000);
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) {
-          const float other = __shfl_xor_sync(0xffffffffu, amax, o);
-          amax = amax != amax || other != other ? __int_as_float(0x7fc00000) : fmaxf(amax, other);
-        }
-        // A NaN in the group makes its scale NaN (fmaxf alone would drop it).
-        const float scale = amax != amax ? amax : fmaxf(amax / 448.f, 1e-8f);
-        if (vec < p.h8) {
-          uint16_t b[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;"
-                : "=h"(b[i])
-                : "f"(y[2 * i + 1] / scale), "f"(y[2 * i] / scale));
-          *reinterpret_cast<uint2*>(p.q + (row * p.h8 + vec) * 8) =
-              make_uint2(b[0] | (uint32_t)b[1] << 16, b[2] | (uint32_t)b[3] << 16);
-          if ((vec & 15) == 0) p.scales[(long long)(vec >> 4) * p.scales_ld + row] = scale;
-        }
+    for (int j = 0; j < V; ++j) {
+      const int vec = tid + j * blockDim.x;
+      uint4 x = make_uint4(0u, 0u, 0u, 0u), r = x;
+      if (vec < p.h8) {
+        x = xs[vec];
+        if (p.residual != nullptr) r = xs[p.h8 + vec];
       }
+      sum += add_vec<F16>(p, x, r, h[j]);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    // Two buffers in turn: a warp may write the next row's partial while
+    // another still reads this row's.
+    if (lane == 0) sums[parity][warp] = sum;
+    __syncthreads();
+    // Every thread has taken its values: the stage may be filled again. (In
+    // place: later rows of this block are its own alone.)
+    if (tid == 0) issue(row + stages * step, stage);
+    if (++stage == stages) {
+      stage = 0;
+      phase ^= 1;
+    }
+    sum = lane < (int)(blockDim.x >> 5) ? sums[parity][lane] : 0.f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const float rstd = rsqrtf(sum * p.inv_hidden + p.eps);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int vec = tid + j * blockDim.x;
+      if (p.residual_out != nullptr && vec < p.h8)
+        *vec_at(p.residual_out, row, p.residual_out_ld, vec) = pack8<F16>(h[j]);
+      store_vec<F16>(p, row, vec, h[j], rstd);
     }
   }
   griddep_launch_dependents();
@@ -215,19 +283,37 @@ cudaError_t launch(const NormParams& p, cudaStream_t stream) {
     long long blocks = (p.rows + kWarps - 1) / kWarps;
     if (blocks > 8ll * sms) blocks = 8ll * sms;
     const dim3 grid((unsigned)blocks), block(kWarps * 32);
-    if (p.h8 <= 32) return launch_pdl(add_rms_norm_kernel<F16, 1, true>, grid, block, 0, stream, p);
-    if (p.h8 <= 64) return launch_pdl(add_rms_norm_kernel<F16, 2, true>, grid, block, 0, stream, p);
-    return launch_pdl(add_rms_norm_kernel<F16, 4, true>, grid, block, 0, stream, p);
+    if (p.h8 <= 32) return launch_pdl(add_rms_norm_warp_kernel<F16, 1>, grid, block, 0, stream, p);
+    if (p.h8 <= 64) return launch_pdl(add_rms_norm_warp_kernel<F16, 2>, grid, block, 0, stream, p);
+    return launch_pdl(add_rms_norm_warp_kernel<F16, 4>, grid, block, 0, stream, p);
   }
+  // Two vectors per thread up to 16384 columns, four beyond. Blocks per SM by
+  // threads and by two stages each of 200 KB of shared memory, then as many
+  // stages as fit (one at least: the widest rows with a residual take 128 KB).
   const int v = p.h8 <= 2048 ? 2 : 4;
   const int threads = ((p.h8 + v - 1) / v + 31) / 32 * 32;
-  long long per_sm = 2048 / threads;
+  const int stage_bytes = p.h8 * 16 * (p.residual != nullptr ? 2 : 1);
+  constexpr int kRoom = 200 * 1024;
+  int per_sm = 1024 / threads;
   if (per_sm > 4) per_sm = 4;
-  long long blocks = per_sm * sms;
+  while (per_sm > 1 && per_sm * 2 * stage_bytes > kRoom) --per_sm;
+  int stages = kRoom / per_sm / stage_bytes;
+  if (stages > kMaxStages) stages = kMaxStages;
+  long long blocks = (long long)per_sm * sms;
   if (blocks > p.rows) blocks = p.rows;
-  const dim3 grid((unsigned)blocks), block((unsigned)threads);
-  if (v == 2) return launch_pdl(add_rms_norm_kernel<F16, 2, false>, grid, block, 0, stream, p);
-  return launch_pdl(add_rms_norm_kernel<F16, 4, false>, grid, block, 0, stream, p);
+  auto* kernel = v == 2 ? add_rms_norm_kernel<F16, 2> : add_rms_norm_kernel<F16, 4>;
+  static bool configured[2][64] = {};
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err != cudaSuccess) return err;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (!configured[v == 4][dev]) {
+    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRoom);
+    if (err != cudaSuccess) return err;
+    configured[v == 4][dev] = true;
+  }
+  return launch_pdl(kernel, dim3((unsigned)blocks), dim3((unsigned)threads),
+                    (size_t)stages * stage_bytes, stream, p, stages);
 }
 
 }  // namespace

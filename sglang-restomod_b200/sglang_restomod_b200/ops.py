@@ -53,7 +53,7 @@ def _contig(t: torch.Tensor, what: str) -> None:
 
 
 def lib():
-    return _lib.load()
+    return _lib._LIB or _lib.load()
 
 
 def num_sms() -> int:
@@ -729,58 +729,52 @@ def w8a8_linear_quantized(q: torch.Tensor, scales: torch.Tensor, w: torch.Tensor
 # ------------------------------------------- norm, key/value cache, attention
 # Decode calls these several times a layer on microseconds of GPU work, so the
 # wrappers keep their own host time low: plain integers instead of ctypes
-# objects, and the current stream by its raw handle.
+# objects, and the current stream and device by their raw handles.
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 
 
 def _on_device(what: str, *tensors: torch.Tensor | None) -> int:
     """The index of the one CUDA device all tensors are on; it must be the
     current one, whose context the library launches in."""
-    index = -1
+    index = _current_device()
     for t in tensors:
-        if t is None:
-            continue
-        at = t.get_device()
-        if at < 0:
-            raise ValueError(f"{what}: operands must be CUDA tensors")
-        if index < 0:
-            index = at
-        elif at != index:
-            raise ValueError(f"{what}: operands are on different devices")
-    if index != torch.cuda.current_device():
-        raise ValueError(f"{what}: operands are on cuda:{index}, the current device is "
-                         f"cuda:{torch.cuda.current_device()}")
+        if t is not None and t.get_device() != index:
+            if not t.is_cuda:
+                raise ValueError(f"{what}: operands must be CUDA tensors")
+            raise ValueError(f"{what}: an operand is on {t.device}, the current device is "
+                             f"cuda:{index}")
     return index
 
 
 def _norm(x, weight, eps, residual, weight_bias, residual_out, y, q, scales, scales_ld, like):
     index = _on_device("add_rms_norm", x, weight, residual, residual_out, y)
-    code = _DTYPE_CODE.get(x.dtype)
+    dtype, shape = x.dtype, x.shape
+    code = _DTYPE_CODE.get(dtype)
     wcode = _LOGIT_CODE.get(weight.dtype)
     if code is None or wcode is None:
-        raise TypeError(f"x must be bf16 or f16 and weight bf16, f16 or f32, got {x.dtype}, "
+        raise TypeError(f"x must be bf16 or f16 and weight bf16, f16 or f32, got {dtype}, "
                         f"{weight.dtype}")
-    hidden = x.shape[-1]
-    if weight.dim() != 1 or weight.shape[0] != hidden or not weight.is_contiguous():
+    rows, hidden = shape
+    if weight.shape != (hidden,) or not weight.is_contiguous():
         raise ValueError(f"weight must be a contiguous [{hidden}], got {tuple(weight.shape)}")
-    rows = x.shape[0]
+    ptrs = []  # residual, residual_out, y: address and leading dimension
     for t in (residual, residual_out, y):
         if t is None:
+            ptrs += (None, 0)
             continue
-        if t.shape != x.shape or t.dtype != x.dtype or t.stride(-1) != 1:
-            raise ValueError(f"{like} must be {tuple(x.shape)} {x.dtype} rows, got "
+        ld, one = t.stride()
+        if t.shape != shape or t.dtype != dtype or one != 1:
+            raise ValueError(f"{like} must be {tuple(shape)} {dtype} rows, got "
                              f"{tuple(t.shape)} {t.dtype}")
-    _lib.check(
-        lib().b200_add_rms_norm(
-            x.data_ptr(), code, x.stride(0), rows, hidden,
-            None if residual is None else residual.data_ptr(),
-            0 if residual is None else residual.stride(0), weight.data_ptr(), wcode,
-            weight_bias, eps, None if residual_out is None else residual_out.data_ptr(),
-            0 if residual_out is None else residual_out.stride(0),
-            None if y is None else y.data_ptr(), 0 if y is None else y.stride(0),
-            None if q is None else q.data_ptr(), None if scales is None else scales.data_ptr(),
-            scales_ld, _raw_stream(index))
-    )
+        ptrs += (t.data_ptr(), ld)
+    status = lib().b200_add_rms_norm(
+        x.data_ptr(), code, x.stride(0), rows, hidden, ptrs[0], ptrs[1], weight.data_ptr(), wcode,
+        weight_bias, eps, ptrs[2], ptrs[3], ptrs[4], ptrs[5],
+        None if q is None else q.data_ptr(), None if scales is None else scales.data_ptr(),
+        scales_ld, _raw_stream(index))
+    if status:
+        _lib.check(status)
 
 
 def _norm_rows(x: torch.Tensor) -> None:
@@ -798,9 +792,9 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *,
     rows; ``out`` and ``residual_out`` may be ``x`` or ``residual`` (in place)."""
     _norm_rows(x)
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
     if residual is not None and residual_out is None:
-        residual_out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        residual_out = torch.empty_like(x, memory_format=torch.contiguous_format)
     _norm(x, weight, eps, residual, weight_bias, residual_out, out, None, None, 0,
           "residual, residual_out and out")
     return out, residual_out
@@ -817,10 +811,10 @@ def add_rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *
     _norm_rows(x)
     rows, hidden = x.shape
     ld = rows if scales_ld is None else int(scales_ld)
-    q = torch.empty(rows, hidden, dtype=torch.float8_e4m3fn, device=x.device)
-    scales = torch.empty(hidden // 128, ld, dtype=torch.float32, device=x.device)
+    q = torch.empty_like(x, dtype=torch.float8_e4m3fn, memory_format=torch.contiguous_format)
+    scales = x.new_empty((hidden // 128, ld), dtype=torch.float32)
     if residual is not None and residual_out is None:
-        residual_out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        residual_out = torch.empty_like(x, memory_format=torch.contiguous_format)
     _norm(x, weight, eps, residual, weight_bias, residual_out, out, q, scales, ld,
           "residual, residual_out and out")
     return q, scales, residual_out
