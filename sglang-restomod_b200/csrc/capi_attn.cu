@@ -86,7 +86,9 @@ int check_copy(const b200_kv_cache* c, int32_t dtype, const int64_t* slots, int6
   if (!valid_dtype16(dtype)) return fail(B200_ERR_UNSUPPORTED, "keys and values must be bf16 or f16");
   if (c->dtype != B200_DTYPE_E4M3 && c->dtype != dtype)
     return fail(B200_ERR_INVALID, "a 16-bit cache holds keys and values of its own type");
-  if (tokens < 0 || tokens > 0x7fffffffll) return fail(B200_ERR_INVALID, "bad token count %lld", (long long)tokens);
+  if (tokens < 0) return fail(B200_ERR_INVALID, "bad token count %lld", (long long)tokens);
+  if (tokens > 0x7fffffffll / c->kv_heads)
+    return fail(B200_ERR_UNSUPPORTED, "more than 2^31 - 1 vectors in one call");
   if (tokens > 0 && (slots == nullptr || !aligned(slots, 8)))
     return fail(B200_ERR_INVALID, "slots must be an 8-byte aligned array");
   return B200_OK;

@@ -29,18 +29,21 @@ struct CopyParams {
   uint8_t* out[2];       // read: k, v
   long long token_bytes[2], head_bytes[2];  // strides of in / out
   const long long* slots;
-  long long tokens;
-  long long vectors;  // tokens * heads, each for k and v
+  uint32_t items;    // tokens * groups
+  uint32_t groups;   // groups of U heads a token has
+  int page_shift;    // log2 of the page size, -1 where it is no power of two
 };
 
-// Offsets of a slot's vector in the cache, or -1 outside it.
-__device__ __forceinline__ bool slot_offsets(const KvCacheView& c, long long slot, int head,
-                                             long long& elem, long long& scale) {
+// Offsets of a slot's first head in the cache; false outside it.
+__device__ __forceinline__ bool slot_offsets(const CopyParams& p, long long slot, long long& elem,
+                                             long long& scale) {
+  const KvCacheView& c = p.c;
   if (slot < 0 || slot >= c.num_pages * c.page_size) return false;
-  const uint32_t page = (uint32_t)slot / (uint32_t)c.page_size;
-  const uint32_t off = (uint32_t)slot - page * (uint32_t)c.page_size;
-  elem = page * c.page_stride + off * c.token_stride + head * c.head_stride;
-  scale = page * c.scale_page_stride + off * c.scale_token_stride + head * c.scale_head_stride;
+  const uint32_t s = (uint32_t)slot;
+  const uint32_t page = p.page_shift >= 0 ? s >> p.page_shift : s / (uint32_t)c.page_size;
+  const uint32_t off = s - page * (uint32_t)c.page_size;
+  elem = page * c.page_stride + off * c.token_stride;
+  scale = page * c.scale_page_stride + off * c.scale_token_stride;
   return true;
 }
 
@@ -69,43 +72,47 @@ __device__ __forceinline__ int scale_exponent(float top) {
   return min(max(e, -24), 7);
 }
 
-// LPV lanes per vector, 8 values each. Each thread carries the same lane of
-// kUnroll vectors, key and value, so 2 * kUnroll loads are in flight.
+// LPV lanes per vector, 8 values each; a thread carries the same lane of U
+// neighbouring heads' keys and values of one token, so the slot's arithmetic is
+// spread over 2 U vectors (per vector it took longer to issue than the bytes to
+// move) and 2 U loads are in flight.
 constexpr int kCopyThreads = 256;
-constexpr int kUnroll = 4;
 
-template <bool F16, bool QUANT, int LPV>
+template <bool F16, bool QUANT, int LPV, int U>
 __global__ void __launch_bounds__(kCopyThreads, 4) kv_write_kernel(CopyParams p) {
   griddep_wait();
   const int lane = threadIdx.x % LPV;
-  const long long stride = (long long)gridDim.x * (kCopyThreads / LPV);
-  const long long first = (long long)blockIdx.x * (kCopyThreads / LPV) + threadIdx.x / LPV;
+  const uint32_t stride = gridDim.x * (kCopyThreads / LPV);
+  const uint32_t first = blockIdx.x * (kCopyThreads / LPV);
   // The trip count is the block's, so that every lane takes part in the shuffles.
-  for (long long base = first - threadIdx.x / LPV; base < p.vectors; base += stride * kUnroll) {
-    uint4 raw[kUnroll][2];
-    long long elem[kUnroll], scale[kUnroll];
-    bool on[kUnroll];
+  for (uint32_t base = first; base < p.items; base += stride) {
+    const uint32_t item = base + threadIdx.x / LPV;
+    bool on = item < p.items;
+    const uint32_t t = on ? item / p.groups : 0;
+    const int h0 = on ? (int)(item - t * p.groups) * U : 0;
+    long long elem = 0, scale = 0;
+    on = on && slot_offsets(p, __ldg(p.slots + t), elem, scale);
+    elem += h0 * p.c.head_stride;
+    scale += h0 * p.c.scale_head_stride;
+    uint4 raw[U][2];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const long long vec = base + threadIdx.x / LPV + u * stride;
-      on[u] = vec < p.vectors;
-      const uint32_t t = on[u] ? (uint32_t)(vec / p.c.heads) : 0;
-      const int h = on[u] ? (int)(vec - (long long)t * p.c.heads) : 0;
-      on[u] = on[u] && slot_offsets(p.c, __ldg(p.slots + t), h, elem[u], scale[u]);
+    for (int s = 0; s < 2; ++s) {
+      const uint8_t* src = p.in[s] + t * p.token_bytes[s] + h0 * p.head_bytes[s] + lane * 16;
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
-        raw[u][s] = on[u] ? *reinterpret_cast<const uint4*>(p.in[s] + t * p.token_bytes[s] +
-                                                            h * p.head_bytes[s] + lane * 16)
-                          : make_uint4(0u, 0u, 0u, 0u);
+      for (int u = 0; u < U; ++u)
+        raw[u][s] = on && h0 + u < p.c.heads
+                        ? *reinterpret_cast<const uint4*>(src + u * p.head_bytes[s])
+                        : make_uint4(0u, 0u, 0u, 0u);
     }
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
+    for (int u = 0; u < U; ++u) {
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         uint8_t* cache = static_cast<uint8_t*>(s ? p.c.v : p.c.k);
+        const bool store = on && h0 + u < p.c.heads;
+        const long long at = elem + u * p.c.head_stride;
         if (!QUANT) {
-          if (on[u])
-            *reinterpret_cast<uint4*>(cache + elem[u] * 2 + lane * 16) = raw[u][s];
+          if (store) *reinterpret_cast<uint4*>(cache + at * 2 + lane * 16) = raw[u][s];
           continue;
         }
         uint32_t top = top_bits(raw[u][s]);
@@ -117,15 +124,18 @@ __global__ void __launch_bounds__(kCopyThreads, 4) kv_write_kernel(CopyParams p)
         const uint32_t w[4] = {raw[u][s].x, raw[u][s].y, raw[u][s].z, raw[u][s].w};
         uint16_t b[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;"
-              : "=h"(b[i])
-              : "f"(half_bits<F16>(w[i] >> 16) * inv), "f"(half_bits<F16>(w[i] & 0xffffu) * inv));
-        if (on[u]) {
-          *reinterpret_cast<uint2*>(cache + elem[u] + lane * 8) =
+        for (int i = 0; i < 4; ++i) {
+          const float lo = F16 ? half_bits<F16>(w[i] & 0xffffu) : __uint_as_float(w[i] << 16);
+          const float hi = F16 ? half_bits<F16>(w[i] >> 16) : __uint_as_float(w[i] & 0xffff0000u);
+          asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(b[i]) : "f"(hi * inv), "f"(lo * inv));
+        }
+        if (store) {
+          *reinterpret_cast<uint2*>(cache + at + lane * 8) =
               bad ? make_uint2(0u, 0u)
                   : make_uint2(b[0] | (uint32_t)b[1] << 16, b[2] | (uint32_t)b[3] << 16);
-          if (lane == 0) (s ? p.c.v_scale : p.c.k_scale)[scale[u]] = bad ? 255 : (uint8_t)(127 + e);
+          if (lane == 0)
+            (s ? p.c.v_scale : p.c.k_scale)[scale + u * p.c.scale_head_stride] =
+                bad ? 255 : (uint8_t)(127 + e);
         }
       }
     }
@@ -144,90 +154,100 @@ __device__ __forceinline__ uint4 decode8(uint2 codes, uint8_t byte) {
   for (int i = 0; i < 4; ++i) {
     const uint32_t h = e4m3x2_to_f16x2((uint16_t)(w[i / 2] >> (16 * (i & 1))));
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-    if (F16) {
-      const __half2 r = __floats2half2_rn(f.x * scale, f.y * scale);
-      o[i] = *reinterpret_cast<const uint32_t*>(&r);
-    } else {
-      const __nv_bfloat162 r = __floats2bfloat162_rn(f.x * scale, f.y * scale);
-      o[i] = *reinterpret_cast<const uint32_t*>(&r);
-    }
+    if (F16)
+      asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(o[i]) : "f"(f.y * scale), "f"(f.x * scale));
+    else
+      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(o[i]) : "f"(f.y * scale), "f"(f.x * scale));
   }
   return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
-template <bool F16, bool QUANT, int LPV>
+template <bool F16, bool QUANT, int LPV, int U>
 __global__ void __launch_bounds__(kCopyThreads, 4) kv_read_kernel(CopyParams p) {
   griddep_wait();
   const int lane = threadIdx.x % LPV;
-  const long long stride = (long long)gridDim.x * (kCopyThreads / LPV);
-  for (long long base = (long long)blockIdx.x * (kCopyThreads / LPV) + threadIdx.x / LPV;
-       base < p.vectors; base += stride * kUnroll) {
-    uint4 raw[kUnroll][2];
-    uint8_t byte[kUnroll][2];
+  const uint32_t stride = gridDim.x * (kCopyThreads / LPV);
+  for (uint32_t item = blockIdx.x * (kCopyThreads / LPV) + threadIdx.x / LPV; item < p.items;
+       item += stride) {
+    const uint32_t t = item / p.groups;
+    const int h0 = (int)(item - t * p.groups) * U;
+    long long elem = 0, scale = 0;
+    const bool on = slot_offsets(p, __ldg(p.slots + t), elem, scale);
+    elem += h0 * p.c.head_stride;
+    scale += h0 * p.c.scale_head_stride;
+    uint4 raw[U][2];
+    uint8_t byte[U][2];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const long long vec = base + u * stride;
-      const uint32_t t = vec < p.vectors ? (uint32_t)(vec / p.c.heads) : 0;
-      const int h = vec < p.vectors ? (int)(vec - (long long)t * p.c.heads) : 0;
-      long long elem = 0, scale = 0;
-      const bool on = vec < p.vectors && slot_offsets(p.c, __ldg(p.slots + t), h, elem, scale);
+    for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         const uint8_t* cache = static_cast<const uint8_t*>(s ? p.c.v : p.c.k);
+        const long long at = elem + u * p.c.head_stride;
         raw[u][s] = make_uint4(0u, 0u, 0u, 0u);
         byte[u][s] = 0;
-        if (!on) continue;
+        if (!on || h0 + u >= p.c.heads) continue;
         if (QUANT) {
-          const uint2 c = *reinterpret_cast<const uint2*>(cache + elem + lane * 8);
+          const uint2 c = *reinterpret_cast<const uint2*>(cache + at + lane * 8);
           raw[u][s].x = c.x;
           raw[u][s].y = c.y;
-          byte[u][s] = (s ? p.c.v_scale : p.c.k_scale)[scale];
+          byte[u][s] = (s ? p.c.v_scale : p.c.k_scale)[scale + u * p.c.scale_head_stride];
         } else {
-          raw[u][s] = *reinterpret_cast<const uint4*>(cache + elem * 2 + lane * 16);
+          raw[u][s] = *reinterpret_cast<const uint4*>(cache + at * 2 + lane * 16);
         }
       }
-    }
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const long long vec = base + u * stride;
-      if (vec >= p.vectors) continue;
-      const uint32_t t = (uint32_t)(vec / p.c.heads);
-      const int h = (int)(vec - (long long)t * p.c.heads);
+    for (int s = 0; s < 2; ++s) {
+      uint8_t* dst = p.out[s] + t * p.token_bytes[s] + h0 * p.head_bytes[s] + lane * 16;
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
-        *reinterpret_cast<uint4*>(p.out[s] + t * p.token_bytes[s] + h * p.head_bytes[s] +
-                                  lane * 16) =
-            QUANT ? decode8<F16>(make_uint2(raw[u][s].x, raw[u][s].y), byte[u][s]) : raw[u][s];
+      for (int u = 0; u < U; ++u)
+        if (h0 + u < p.c.heads)
+          *reinterpret_cast<uint4*>(dst + u * p.head_bytes[s]) =
+              QUANT ? decode8<F16>(make_uint2(raw[u][s].x, raw[u][s].y), byte[u][s]) : raw[u][s];
     }
   }
   griddep_launch_dependents();
 }
 
-template <bool F16, bool QUANT, int LPV>
-cudaError_t launch(const CopyParams& p, bool write, cudaStream_t stream) {
-  constexpr int kPerBlock = kCopyThreads / LPV;
-  long long blocks = (p.vectors + kPerBlock - 1) / kPerBlock;
-  const long long cap = (long long)device_sm_count() * 8;
+template <bool F16, bool QUANT, int LPV, int U>
+cudaError_t launch(CopyParams& p, long long tokens, bool write, cudaStream_t stream) {
+  p.groups = (uint32_t)(p.c.heads + U - 1) / U;
+  p.items = (uint32_t)tokens * p.groups;
+  constexpr uint32_t kPerBlock = kCopyThreads / LPV;
+  uint32_t blocks = (p.items + kPerBlock - 1) / kPerBlock;
+  const uint32_t cap = (uint32_t)device_sm_count() * 8;
   if (blocks > cap) blocks = cap;
-  return launch_pdl(write ? kv_write_kernel<F16, QUANT, LPV> : kv_read_kernel<F16, QUANT, LPV>,
-                    dim3((unsigned)blocks), dim3(kCopyThreads), 0, stream, p);
+  return launch_pdl(write ? kv_write_kernel<F16, QUANT, LPV, U> : kv_read_kernel<F16, QUANT, LPV, U>,
+                    dim3(blocks), dim3(kCopyThreads), 0, stream, p);
+}
+
+// Four heads a thread fill the SMs' load queues; a small batch (a decode step)
+// spreads over more threads instead.
+template <bool F16, bool QUANT, int LPV>
+cudaError_t launch_heads(CopyParams& p, long long tokens, bool write, cudaStream_t stream) {
+  const long long threads = tokens * p.c.heads * LPV;
+  if (p.c.heads >= 3 && threads > 2048ll * 4 * device_sm_count())
+    return launch<F16, QUANT, LPV, 4>(p, tokens, write, stream);
+  return launch<F16, QUANT, LPV, 1>(p, tokens, write, stream);
 }
 
 template <bool F16, bool QUANT>
-cudaError_t launch_dim(const CopyParams& p, bool write, cudaStream_t stream) {
+cudaError_t launch_dim(CopyParams& p, long long tokens, bool write, cudaStream_t stream) {
   switch (p.c.head_dim) {
-    case 64: return launch<F16, QUANT, 8>(p, write, stream);
-    case 128: return launch<F16, QUANT, 16>(p, write, stream);
-    default: return launch<F16, QUANT, 32>(p, write, stream);
+    case 64: return launch_heads<F16, QUANT, 8>(p, tokens, write, stream);
+    case 128: return launch_heads<F16, QUANT, 16>(p, tokens, write, stream);
+    default: return launch_heads<F16, QUANT, 32>(p, tokens, write, stream);
   }
 }
 
-cudaError_t launch_copy(const CopyParams& p, bool f16, bool write, cudaStream_t stream) {
-  if (p.vectors <= 0) return cudaSuccess;
+cudaError_t launch_copy(CopyParams& p, long long tokens, bool f16, bool write, cudaStream_t stream) {
+  if (tokens <= 0) return cudaSuccess;
+  p.page_shift =
+      (p.c.page_size & (p.c.page_size - 1)) == 0 ? __builtin_ctz((unsigned)p.c.page_size) : -1;
   if (p.c.k_scale != nullptr)
-    return f16 ? launch_dim<true, true>(p, write, stream) : launch_dim<false, true>(p, write, stream);
+    return f16 ? launch_dim<true, true>(p, tokens, write, stream)
+               : launch_dim<false, true>(p, tokens, write, stream);
   // 16-bit caches are copied as bits: one instantiation serves both types.
-  return launch_dim<false, false>(p, write, stream);
+  return launch_dim<false, false>(p, tokens, write, stream);
 }
 
 }  // namespace
@@ -245,9 +265,7 @@ cudaError_t launch_kv_write(const KvCacheView& c, const void* k, const void* v, 
   p.token_bytes[1] = v_token_stride * 2;
   p.head_bytes[1] = v_head_stride * 2;
   p.slots = slots;
-  p.tokens = tokens;
-  p.vectors = tokens * c.heads;
-  return launch_copy(p, f16, true, stream);
+  return launch_copy(p, tokens, f16, true, stream);
 }
 
 cudaError_t launch_kv_read(const KvCacheView& c, void* k, void* v, bool f16,
@@ -260,9 +278,7 @@ cudaError_t launch_kv_read(const KvCacheView& c, void* k, void* v, bool f16,
   p.token_bytes[0] = p.token_bytes[1] = token_stride * 2;
   p.head_bytes[0] = p.head_bytes[1] = head_stride * 2;
   p.slots = slots;
-  p.tokens = tokens;
-  p.vectors = tokens * c.heads;
-  return launch_copy(p, f16, false, stream);
+  return launch_copy(p, tokens, f16, false, stream);
 }
 
 }  // namespace b200

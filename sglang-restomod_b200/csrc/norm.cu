@@ -42,8 +42,12 @@ __device__ __forceinline__ void unpack8(uint4 raw, float (&v)[8]) {
   const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float2 f = F16 ? __half22float2(*reinterpret_cast<const __half2*>(&w[i]))
-                         : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]));
+    if (!F16) {  // a bf16 is the upper half of its fp32
+      v[2 * i] = __uint_as_float(w[i] << 16);
+      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      continue;
+    }
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
     v[2 * i] = f.x;
     v[2 * i + 1] = f.y;
   }
@@ -87,8 +91,10 @@ __device__ __forceinline__ void load_weight(const NormParams& p, int vec, float 
     else
       unpack8<false>(raw, w);
   }
+  if (p.weight_bias != 0.f) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) w[i] += p.weight_bias;
+    for (int i = 0; i < 8; ++i) w[i] += p.weight_bias;
+  }
 }
 
 // Row data is read once: past L1, which keeps the weights. (Not the read-only
@@ -102,58 +108,115 @@ __device__ __forceinline__ uint4 load_row(const uint4* src) {
   return v;
 }
 
+// Two fp32 operations per instruction: with the conversions, a row's arithmetic
+// would otherwise take longer to issue than its bytes to arrive.
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+// The larger, NaN if either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // The 8 columns y[vec] of a scaled row: 16-bit output, and the group's scale
 // and codes. Called by all lanes of a warp (h8 is a multiple of 16 with q, so
 // a group's 16 lanes are on together).
 template <bool F16>
 __device__ __forceinline__ void store_vec(const NormParams& p, long long row, int vec,
-                                          const float (&h)[8], float rstd) {
+                                          const uint64_t (&h)[4], float rstd) {
   const bool on = vec < p.h8;
-  float y[8], w[8];
-  if (on) load_weight(p, vec, w);
+  float y[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = on ? h[i] * rstd * w[i] : 0.f;
+  for (int i = 0; i < 8; ++i) y[i] = 0.f;
+  if (on) {
+    float w[8];
+    load_weight(p, vec, w);
+    const uint64_t r2 = pair(rstd, rstd);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 v = unpair(mul2(mul2(h[i], r2), pair(w[2 * i], w[2 * i + 1])));
+      y[2 * i] = v.x;
+      y[2 * i + 1] = v.y;
+    }
+  }
   if (p.y != nullptr && on) *vec_at(p.y, row, p.y_ld, vec) = pack8<F16>(y);
   if (p.q == nullptr) return;
-  float amax = 0.f;
-  bool nan = false;
+  // A NaN in the group makes its scale NaN.
+  float amax = fabsf(y[0]);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    amax = fmaxf(amax, fabsf(y[i]));
-    nan |= y[i] != y[i];
-  }
-  if (nan) amax = __int_as_float(0x7fc00000);
+  for (int i = 1; i < 8; ++i) amax = max_nan(amax, fabsf(y[i]));
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) {
-    const float other = __shfl_xor_sync(0xffffffffu, amax, o);
-    amax = amax != amax || other != other ? __int_as_float(0x7fc00000) : fmaxf(amax, other);
-  }
-  // A NaN in the group makes its scale NaN (fmaxf alone would drop it).
-  const float scale = amax != amax ? amax : fmaxf(amax / 448.f, 1e-8f);
+  for (int o = 8; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
   if (!on) return;
+  const float scale = max_nan(amax / 448.f, 1e-8f);
+  // One reciprocal for the eight quotients: at most one rounding of fp32 from
+  // them, so a code differs only for a y that lies that close to a border.
+  const float inv = __frcp_rn(scale);
+  const uint64_t inv2 = pair(inv, inv);
   uint16_t b[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;"
-        : "=h"(b[i])
-        : "f"(y[2 * i + 1] / scale), "f"(y[2 * i] / scale));
+  for (int i = 0; i < 4; ++i) {
+    const float2 v = unpair(mul2(pair(y[2 * i], y[2 * i + 1]), inv2));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(b[i]) : "f"(v.y), "f"(v.x));
+  }
   *reinterpret_cast<uint2*>(p.q + (row * p.h8 + vec) * 8) =
       make_uint2(b[0] | (uint32_t)b[1] << 16, b[2] | (uint32_t)b[3] << 16);
   if ((vec & 15) == 0) p.scales[(long long)(vec >> 4) * p.scales_ld + row] = scale;
 }
 
-// h = x (+ r) and the sum of its squares.
+// h = x (+ r), and the sum of its squares.
 template <bool F16>
-__device__ __forceinline__ float add_vec(const NormParams& p, uint4 x, uint4 r, float (&h)[8]) {
-  float rv[8], sum = 0.f;
-  unpack8<F16>(x, h);
-  unpack8<F16>(r, rv);
+__device__ __forceinline__ float add_vec(const NormParams& p, uint4 x, uint4 r, uint64_t (&h)[4]) {
+  float v[8];
+  unpack8<F16>(x, v);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if (p.residual != nullptr) h[i] += rv[i];
-    sum += h[i] * h[i];
+  for (int i = 0; i < 4; ++i) h[i] = pair(v[2 * i], v[2 * i + 1]);
+  if (p.residual != nullptr) {
+    unpack8<F16>(r, v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = add2(h[i], pair(v[2 * i], v[2 * i + 1]));
   }
-  return sum;
+  uint64_t s = mul2(h[0], h[0]);
+#pragma unroll
+  for (int i = 1; i < 4; ++i) s = fma2(h[i], h[i], s);
+  const float2 t = unpair(s);
+  return t.x + t.y;
+}
+
+template <bool F16>
+__device__ __forceinline__ uint4 pack8(const uint64_t (&h)[4]) {
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 t = unpair(h[i]);
+    v[2 * i] = t.x;
+    v[2 * i + 1] = t.y;
+  }
+  return pack8<F16>(v);
 }
 
 // A warp per row, V vectors of 8 columns per lane; the next row's values are
@@ -179,7 +242,8 @@ __global__ void __launch_bounds__(256) add_rms_norm_warp_kernel(NormParams p) {
   if (kPrefetch) fetch(row);
   for (; row < p.rows; row += step) {
     if (!kPrefetch) fetch(row);
-    float h[V][8], sum = 0.f;
+    uint64_t h[V][4];
+    float sum = 0.f;
 #pragma unroll
     for (int j = 0; j < V; ++j) sum += add_vec<F16>(p, xin[j], rin[j], h[j]);
     // In-place outputs: row + step is this warp's alone, so loading it before
@@ -236,7 +300,8 @@ __global__ void __launch_bounds__(1024) add_rms_norm_kernel(NormParams p, int st
     // kernel hanging.
     mbar_wait(&full[stage], (uint32_t)phase, nullptr);
     const uint4* xs = reinterpret_cast<const uint4*>(ring + stage * stage_bytes);
-    float h[V][8], sum = 0.f;
+    uint64_t h[V][4];
+    float sum = 0.f;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const int vec = tid + j * blockDim.x;
