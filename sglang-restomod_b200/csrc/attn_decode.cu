@@ -18,10 +18,12 @@
 //   cut by a range border leaves partial (O, m, l) in the scratch; the last
 //   block to arrive at the pair's counter adds them in block order, so the
 //   result does not depend on which block that is.
-// * Each warp streams its own quarter of a tile's tokens through a private ring
-//   of cp.async stages: no block barrier inside a pair, and the ring runs on
-//   into the next pair while the present one is finished. Page numbers travel
-//   through the same ring one ring length ahead, so no load waits on another.
+// * Each warp streams its own 16 of a tile's tokens through a private ring of
+//   stages: no block barrier inside a pair, and the ring runs on into the next
+//   pair while the present one is finished. Pages of a multiple of 8 tokens
+//   come by tensor copies, one or two boxes each of K and V a step, issued by
+//   one lane; other pages (single-token ones, say) by 16-byte cp.async, whose
+//   addresses take longer to compute than a step's products.
 // * The products are taken transposed (S^T = K Q^T, O^T = V^T P^T): the
 //   m16n8k16 tile then has 16 cached tokens or 16 head columns in M and 8 rows
 //   in N, so 8 query heads per key/value head waste nothing. K is read as the
@@ -34,14 +36,13 @@
 // * The maximum is lazy: O and l are rescaled only when some s exceeds m by
 //   more than 2^8, so P stays below 2^8 and most tiles need no cross-lane
 //   reduction at all.
+#include "attn_maps.cuh"
 #include "common.cuh"
 #include "internal.h"
 
 namespace b200 {
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kThreads = kWarps * 32;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 8.f;        // log2 of the largest P before a rescale
 constexpr int kMaxCtas = 1024;      // arrival counters in the workspace
@@ -54,6 +55,9 @@ struct DecodeParams {
   int groups;          // query heads per key/value head
   float scale_log2;
   int page_shift;      // log2 of the page size, -1 where it is no power of two
+  // tensor copies: token rows of a box (16 or 8), and whether heads come before
+  // tokens in the maps
+  int box_rows, heads_first;
 };
 
 enum { kBf16 = 0, kF16 = 1, kE4m3 = 2 };
@@ -63,38 +67,39 @@ struct TileInfo {
   int seq, head;   // seq < 0: past the block's range
   int token0;      // first of this warp's tokens
   int end;         // tokens from here on do not exist
+  int page[2];     // tensor copies: pages of tokens 0-7 and 8-15
 };
 
-template <int D, int KV, int NR>
+template <int D, int KV, int NR, bool TMA>
 struct Shape {
   static constexpr int kElem = KV == kE4m3 ? 1 : 2;
   static constexpr int kRowBytes = D * kElem;
-  // Tokens of a warp's step: 32 where the stages stay small, so that what a
-  // step costs besides its products (copies' addresses, ring, masks) is spread
-  // over two m16 tiles whose chains of instructions also fill each other's gaps.
-  static constexpr int kTokens = kRowBytes <= 128 ? 32 : 16;
-  static constexpr int kTiles16 = kTokens / 16;
+  // A warp takes 16 tokens a step. Its instructions wait on one another (loads,
+  // products, softmax, products), so as many warps share an SM as registers (128
+  // a thread at 16 warps) and the ring's stages allow: 16 for e4m3 and head_dim
+  // 64, 8 for head_dim 128 in 16 bits and 256 in e4m3, 4 for 256 in 16 bits.
+  static constexpr int kTokens = 16;
+  static constexpr int kWarps = KV == kE4m3 || D == 64 ? 8 : 4;
+  static constexpr int kThreads = kWarps * 32;
   static constexpr int kTile = kTokens * kWarps;               // tokens per block step
   static constexpr int kStageBytes = 2 * kTokens * kRowBytes;  // K then V of a warp
   static constexpr int kRows = 8 * NR;
-  // Ring depth: 64 to 96 KB per block and two blocks per SM; head_dim 256, whose
-  // stages are 32 to 64 KB, takes one block per SM with 160 to 192 KB.
+  // Ring depth: 80 to 96 KB per block and two blocks per SM; head_dim 256, whose
+  // stages are 64 KB a block, takes one block per SM with 192 KB.
   static constexpr int kBlocks = D == 256 ? 1 : 2;
-  static constexpr int kStages = KV == kE4m3 ? (D == 64 ? 5 : D == 128 ? 3 : 5) : 3;
+  static constexpr int kStages = KV == kE4m3 && D == 64 ? 5 : 3;
   static constexpr int kAhead = kStages - 1;
-  static constexpr int kRing = 2 * kStages;  // page-number entries
+  static constexpr int kRing = 2 * kStages;  // tile descriptions
   static constexpr int kQPitch = D + 8;      // 16-bit elements, conflict-free rows
-  static constexpr int kMergePitch = D + 4;  // fp32
   struct Smem {
-    uint8_t stage[kWarps][kStages][kStageBytes];
+    alignas(1024) uint8_t stage[kWarps][kStages][kStageBytes];
     uint16_t q[kRows][kQPitch];
-    float merge[kRows][kMergePitch];
-    int pages[kWarps][kRing][kTokens];
+    uint64_t full[kWarps][kStages];
+    int pages[TMA ? 1 : kWarps][kRing][kTokens];
     TileInfo info[kWarps][kRing];
     float row_scale[kRows];
     int row_lo[kRows], row_hi[kRows];
-    float wm[kWarps][kRows], wl[kWarps][kRows], mx[kRows];
-    int wv[kWarps];
+    float wm[kWarps][kRows], wl[kWarps][kRows], mx[kRows], sum[kRows];
     long long scan[kWarps];
     int start_seq;
     long long start_off;
@@ -157,19 +162,28 @@ __device__ __forceinline__ float pow2(int e) {
   return e < -126 ? 0.f : __uint_as_float((uint32_t)(127 + e) << 23);
 }
 
-// Bytes of a warp's tile rows, 16-byte chunk `chunk` of token row `row`,
-// placed so that the operand reads below touch all banks evenly.
-template <int D, int KV, bool IS_V>
+// Byte of 16-byte chunk `chunk` of token row `row` in a warp's K or V tile,
+// placed so that the operand reads below touch the banks evenly. Tensor copies
+// leave slices of 128 B with chunks XORed by the row's low bits (64 B rows: by
+// the row pair's).
+template <int D, int KV, bool IS_V, bool TMA>
 __device__ __forceinline__ int chunk_at(int row, int chunk) {
-  constexpr int kChunks = Shape<D, KV, 1>::kRowBytes / 16;
+  constexpr int kChunks = D * (KV == kE4m3 ? 1 : 2) / 16;
+  if (kChunks == 4) return (row * 4 + (chunk ^ ((row >> 1) & 3))) * 16;
+  if (TMA) return (chunk >> 3) * 2048 + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
   int x;
   if (KV != kE4m3)
     x = row & 7;  // ldmatrix: 8 rows of one chunk column
-  else if (kChunks == 4)
-    x = (row >> 1) & 3;  // two rows fill the banks
   else
     x = IS_V ? (row & 6) : ((row & 1) << 2);
   return (row * kChunks + (chunk ^ x)) * 16;
+}
+
+// Where column d of a row of O lies in a warp's free stage, so that the lanes
+// that write the accumulators touch different banks (c: the lane's row pair).
+template <int KV>
+__device__ __forceinline__ int merge_col(int d, int c) {
+  return KV != kE4m3 ? d ^ (c << 3) : d ^ (((d >> 5) & 3) | (c << 2));
 }
 
 // The key range of a sequence: tokens [begin, end) some row may see, as tiles.
@@ -179,7 +193,7 @@ struct SeqRange {
   int begin, end, q_len, kv_len, tiles;
 };
 template <int kTile>
-__device__ __forceinline__ SeqRange seq_range(const AttnLaunch& a, int s) {
+__device__ __forceinline__ SeqRange seq_range(const AttnLaunch& a, int s, int align) {
   SeqRange r;
   const int q0 = __ldg(a.q_starts + s), q1 = __ldg(a.q_starts + s + 1);
   const long long cap = (long long)a.table_width * a.c.page_size;
@@ -196,22 +210,34 @@ __device__ __forceinline__ SeqRange seq_range(const AttnLaunch& a, int s) {
   if (a.window > 0) {
     const long long b = (long long)kv - ql - a.window + 1;  // first token the first row sees
     r.begin = b > 0 ? (int)b : 0;
+    r.begin -= r.begin % align;  // a copy's border
   }
   const int n = r.end - r.begin;
   r.tiles = ql == 0 ? 0 : (n <= 0 ? 1 : (n + kTile - 1) / kTile);
   return r;
 }
 
-template <int D, int KV, int NR>
-__global__ void __launch_bounds__(kThreads, Shape<D, KV, NR>::kBlocks) attn_decode_kernel(const DecodeParams p) {
-  using S = Shape<D, KV, NR>;
+template <int D, int KV, int NR, bool TMA>
+__global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, NR, TMA>::kBlocks)
+    attn_decode_kernel(const DecodeParams p, const __grid_constant__ CUtensorMap k_map,
+                       const __grid_constant__ CUtensorMap v_map) {
+  using S = Shape<D, KV, NR, TMA>;
+  constexpr int kAlign = TMA ? 16 : 1;
   using Smem = typename S::Smem;
-  extern __shared__ __align__(128) uint8_t smem_raw[];
-  Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
+  constexpr int kWarps = S::kWarps, kThreads = S::kThreads;
+  extern __shared__ uint8_t smem_raw[];
+  Smem& sm = *reinterpret_cast<Smem*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
   const AttnLaunch& a = p.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, c = lane & 3;
   const int heads = a.c.heads;
+  if (TMA) {
+    if (lane == 0) {
+      for (int i = 0; i < S::kStages; ++i) mbar_init(&sm.full[warp][i], 1);
+      fence_mbar_init();
+    }
+    __syncwarp();
+  }
   griddep_wait();
 
   // ---- this block's range of the flattened (sequence, head, tile) space
@@ -220,7 +246,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV, NR>::kBlocks) attn_deco
     const int per = (a.seqs + kThreads - 1) / kThreads;
     const int s0 = tid * per, s1 = min(s0 + per, a.seqs);
     long long mine = 0;
-    for (int s = s0; s < s1; ++s) mine += (long long)seq_range<S::kTile>(a, s).tiles * heads;
+    for (int s = s0; s < s1; ++s) mine += (long long)seq_range<S::kTile>(a, s, kAlign).tiles * heads;
     long long before = mine;  // inclusive scan, made exclusive below
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -244,7 +270,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV, NR>::kBlocks) attn_deco
     if (t0 >= before && t0 < before + mine) {
       int s = s0;
       for (;; ++s) {
-        const long long n = (long long)seq_range<S::kTile>(a, s).tiles * heads;
+        const long long n = (long long)seq_range<S::kTile>(a, s, kAlign).tiles * heads;
         if (t0 < before + n) break;
         before += n;
       }
@@ -257,9 +283,9 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV, NR>::kBlocks) attn_deco
   const long long t0 = total * blockIdx.x / ctas;
   const long long t1 = total * (blockIdx.x + 1) / ctas;
 
-  // ---- the request cursor: page numbers of the warp's next tile
+  // ---- the request cursor: the warp's next tile
   int r_seq = sm.start_seq, r_head, r_tile;
-  SeqRange r_range = seq_range<S::kTile>(a, r_seq);
+  SeqRange r_range = seq_range<S::kTile>(a, r_seq, kAlign);
   r_head = (int)(sm.start_off / r_range.tiles);
   r_tile = (int)(sm.start_off - (long long)r_head * r_range.tiles);
   long long r_at = t0;
@@ -267,26 +293,16 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV, NR>::kBlocks) attn_deco
   auto page_of = [&](int token) {
     return p.page_shift >= 0 ? token >> p.page_shift : token / a.c.page_size;
   };
-  // Requests one tile's page numbers into ring entry r_slot. `now`: by plain
-  // loads (the prologue), else asynchronously with the next group.
-  auto request = [&](bool now) {
+  auto next_tile = [&]() {
     TileInfo ti;
     ti.seq = -1;
     ti.head = r_head;
-    ti.token0 = 0;
-    ti.end = 0;
+    ti.token0 = ti.end = 0;
+    ti.page[0] = ti.page[1] = -1;
     if (r_at < t1) {
       ti.seq = r_seq;
       ti.token0 = r_range.begin + r_tile * S::kTile + warp * S::kTokens;
       ti.end = r_range.end;
-      if (lane < S::kTokens && ti.token0 + lane < ti.end) {
-        const int* src = a.table + r_seq * a.table_stride + page_of(ti.token0 + lane);
-        int* dst = &sm.pages[warp][r_slot][lane];
-        if (now)
-          *dst = __ldg(src);
-        else
-          cp_async_4(dst, src);
-      }
       ++r_at;
       if (++r_tile == r_range.tiles) {
         r_tile = 0;
@@ -294,17 +310,31 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV, NR>::kBlocks) attn_deco
           r_head = 0;
           if (r_at < t1) {
             do {
-              r_range = seq_range<S::kTile>(a, ++r_seq);
+              r_range = seq_range<S::kTile>(a, ++r_seq, kAlign);
             } while (r_range.tiles == 0);
           }
         }
       }
     }
+    return ti;
+  };
+
+  // -- cp.async: page numbers go into ring entry r_slot, by plain loads (`now`,
+  // the prologue) or asynchronously with the next group of copies, kAhead steps
+  // before the copies that need them.
+  auto request = [&](bool now) {
+    const TileInfo ti = next_tile();
+    if (ti.seq >= 0 && lane < S::kTokens && ti.token0 + lane < ti.end) {
+      const int* src = a.table + ti.seq * a.table_stride + page_of(ti.token0 + lane);
+      int* dst = &sm.pages[TMA ? 0 : warp][r_slot][lane];
+      if (now)
+        *dst = __ldg(src);
+      else
+        cp_async_4(dst, src);
+    }
     if (lane == 0) sm.info[warp][r_slot] = ti;
     r_slot = r_slot + 1 == S::kRing ? 0 : r_slot + 1;
   };
-
-  // Issues the copies of ring entry `slot` into stage `stage`.
   auto issue = [&](int slot, int stage) {
     const TileInfo ti = sm.info[warp][slot];
     if (ti.seq >= 0) {
@@ -317,7 +347,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV, NR>::kBlocks) attn_deco
       {
         const int token = ti.token0 + lane % S::kTokens;
         if (token < ti.end) {
-          const int page = sm.pages[warp][slot][lane % S::kTokens];
+          const int page = sm.pages[TMA ? 0 : warp][slot][lane % S::kTokens];
           const int at_page = token - page_of(token) * a.c.page_size;
           if (page >= 0 && page < a.c.num_pages)
             mine = (page * a.c.page_stride + at_page * a.c.token_stride + head_off) * S::kElem;
@@ -332,37 +362,104 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV, NR>::kBlocks) attn_deco
         long long off = __shfl_sync(0xffffffffu, mine, row);
         const bool on = off >= 0;
         off = on ? off + chunk * 16 : 0;
-        cp_async_16_zfill(ks + chunk_at<D, KV, false>(row, chunk),
+        cp_async_16_zfill(ks + chunk_at<D, KV, false, TMA>(row, chunk),
                           static_cast<const uint8_t*>(a.c.k) + off, on);
-        cp_async_16_zfill(vs + chunk_at<D, KV, true>(row, chunk),
+        cp_async_16_zfill(vs + chunk_at<D, KV, true, TMA>(row, chunk),
                           static_cast<const uint8_t*>(a.c.v) + off, on);
       }
     }
   };
-  // The scale bytes of token lane % kTokens in ring entry `slot`: the key's,
-  // the value's << 8. 0 (2^-127, and codes of zero) for absent tokens.
-  auto scale_bytes = [&](int slot) -> uint32_t {
-    if (KV != kE4m3) return 0;
+
+  // -- tensor copies: lanes 0 and 1 look up the pages of tokens 0-7 and 8-15
+  // one step before the copy. Boxes past the last key and of pages outside the
+  // cache come from past the maps' end, which gives zeros.
+  auto look = [&](const TileInfo& ti) -> int {
+    const int token = ti.token0 + 8 * lane;
+    return ti.seq >= 0 && lane < 2 && token < ti.end
+               ? __ldg(a.table + ti.seq * a.table_stride + page_of(token))
+               : -2;
+  };
+  auto issue_tma = [&](TileInfo ti, int page, int stage) {
+    if (ti.seq >= 0) {
+      const int token = ti.token0 + 8 * lane;
+      int at = 0;
+      if (lane < 2) {
+        if (page < 0 || page >= a.c.num_pages) {
+          if (token < ti.end) atomicOr(a.status, kDevBadPage);
+          page = -1;
+        } else {
+          at = token - page_of(token) * a.c.page_size;
+        }
+      }
+      ti.page[0] = __shfl_sync(0xffffffffu, page, 0);
+      ti.page[1] = __shfl_sync(0xffffffffu, page, 1);
+      if (lane == 0) mbar_arrive_expect_tx(&sm.full[warp][stage], S::kStageBytes);
+      __syncwarp();
+      if (lane < (p.box_rows == 8 ? 2 : 1)) {
+        const uint32_t dst = smem_u32(sm.stage[warp][stage]) +
+                             lane * 8 * (S::kRowBytes < 128 ? S::kRowBytes : 128);
+        const int pg = page < 0 ? (int)a.c.num_pages : page;
+        const int y = p.heads_first ? ti.head : at, z = p.heads_first ? at : ti.head;
+        constexpr int kSlices = S::kRowBytes <= 128 ? 1 : S::kRowBytes / 128;
+        constexpr int kCols = (S::kRowBytes < 128 ? S::kRowBytes : 128) / S::kElem;
+#pragma unroll
+        for (int sl = 0; sl < kSlices; ++sl) {
+          tma_load_4d(dst + sl * 2048, &k_map, sl * kCols, y, z, pg, &sm.full[warp][stage]);
+          tma_load_4d(dst + S::kTokens * S::kRowBytes + sl * 2048, &v_map, sl * kCols, y, z, pg,
+                      &sm.full[warp][stage]);
+        }
+      }
+    }
+    if (lane == 0) sm.info[warp][r_slot] = ti;
+    r_slot = r_slot + 1 == S::kRing ? 0 : r_slot + 1;
+  };
+
+  // The scale bytes of token lane % 16 in ring entry `slot`: 0 (2^-127, and
+  // codes of zero) for absent tokens. (Two registers: joining them would wait
+  // for the loads here, a step before they are needed.)
+  auto scale_bytes = [&](int slot, uint32_t& kb, uint32_t& vb) {
+    kb = vb = 0;
+    if (KV != kE4m3) return;
     const TileInfo ti = sm.info[warp][slot];
     const int row = lane % S::kTokens, token = ti.token0 + row;
-    if (ti.seq < 0 || token >= ti.end) return 0;
-    const int page = sm.pages[warp][slot][row];
-    if (page < 0 || page >= a.c.num_pages) return 0;
+    if (ti.seq < 0 || token >= ti.end) return;
+    const int page = TMA ? ti.page[p.box_rows == 8 ? row >> 3 : 0]
+                         : sm.pages[TMA ? 0 : warp][slot][row];
+    if (page < 0 || page >= a.c.num_pages) return;
     const long long at = page * a.c.scale_page_stride +
                          (token - page_of(token) * a.c.page_size) * a.c.scale_token_stride +
                          ti.head * a.c.scale_head_stride;
-    return __ldg(a.c.k_scale + at) | (uint32_t)__ldg(a.c.v_scale + at) << 8;
+    kb = __ldg(a.c.k_scale + at);
+    vb = __ldg(a.c.v_scale + at);
   };
 
   // ---- prologue
-  for (int i = 0; i < S::kAhead; ++i) request(true);
-  __syncwarp();
-  for (int i = 0; i < S::kAhead; ++i) {
-    issue(i, i);
-    request(false);
-    cp_async_commit();
+  TileInfo ahead;        // tensor copies: the tile to be issued next,
+  int ahead_page = -2;   // and its pages
+  if (TMA) {
+    TileInfo ti[S::kAhead];
+    int pg[S::kAhead];
+#pragma unroll
+    for (int i = 0; i < S::kAhead; ++i) {
+      ti[i] = next_tile();
+      pg[i] = look(ti[i]);
+    }
+    ahead = next_tile();
+    ahead_page = look(ahead);
+#pragma unroll
+    for (int i = 0; i < S::kAhead; ++i) issue_tma(ti[i], pg[i], i);
+  } else {
+    for (int i = 0; i < S::kAhead; ++i) request(true);
+    __syncwarp();
+    for (int i = 0; i < S::kAhead; ++i) {
+      issue(i, i);
+      request(false);
+      cp_async_commit();
+    }
   }
-  uint32_t next_bytes = scale_bytes(0);
+  __syncwarp();
+  uint32_t next_kb, next_vb;
+  scale_bytes(0, next_kb, next_vb);
 
   // ---- consume
   float o[D / 16][NR][4];
@@ -370,13 +467,14 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV, NR>::kBlocks) attn_deco
   int v_exp = 1;              // e4m3: byte of the largest value scale so far
   long long at = t0;
   int slot = 0, stage = 0;
+  uint32_t phase = 0;
   while (at < t1) {
     // -- a (sequence, head) pair begins: its tiles of this block are
     // [at, pair_end); u0, u1 bound the whole pair
-    cp_async_wait<S::kAhead - 1>();
+    if (!TMA) cp_async_wait<S::kAhead - 1>();
     __syncwarp();
     const TileInfo first = sm.info[warp][slot];
-    const SeqRange range = seq_range<S::kTile>(a, first.seq);
+    const SeqRange range = seq_range<S::kTile>(a, first.seq, kAlign);
     const int head = first.head;
     const long long u0 =
         at - (first.token0 - warp * S::kTokens - range.begin) / S::kTile;
@@ -493,20 +591,38 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV, NR>::kBlocks) attn_deco
         for (int j = 0; j < 4; ++j) o[t][nr][j] = 0.f;
 
     for (; at < pair_end; ++at) {
-      cp_async_wait<S::kAhead - 1>();
-      __syncwarp();
-      const int token0 = sm.info[warp][slot].token0;
-      const uint32_t bytes = next_bytes;
-      // refill: the stage freed last step, from the entry kAhead steps on
-      {
+      const TileInfo ti = sm.info[warp][slot];
+      const int token0 = ti.token0;
+      const uint32_t kb_lane = next_kb, vb_lane = next_vb;
+      // refill: the stage freed last step, with the tile kAhead steps on
+      const int refill = stage == 0 ? S::kStages - 1 : stage - 1;
+      if (TMA) {
+        issue_tma(ahead, ahead_page, refill);
+        ahead = next_tile();
+        ahead_page = look(ahead);
+        mbar_wait(&sm.full[warp][stage], phase, a.status);
+        if (token0 + S::kTokens > ti.end) {
+          // what a page holds past the last key may be NaN, and P zero times it
+          // NaN again: those rows of V become zeros
+          uint8_t* v = sm.stage[warp][stage] + S::kTokens * S::kRowBytes;
+          constexpr int kChunks = S::kRowBytes / 16;
+          for (int i = max(ti.end - token0, 0) * kChunks + lane; i < S::kTokens * kChunks; i += 32)
+            *reinterpret_cast<uint4*>(v + chunk_at<D, KV, true, TMA>(i / kChunks, i % kChunks)) =
+                make_uint4(0u, 0u, 0u, 0u);
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the next copy here
+          __syncwarp();
+        }
+      } else {
+        cp_async_wait<S::kAhead - 1>();
+        __syncwarp();
         const int s2 = slot + S::kAhead < S::kRing ? slot + S::kAhead : slot + S::kAhead - S::kRing;
-        issue(s2, stage + S::kAhead < S::kStages ? stage + S::kAhead : stage + S::kAhead - S::kStages);
+        issue(s2, refill);
         request(false);
         cp_async_commit();
       }
       const uint8_t* ks_ptr = sm.stage[warp][stage];
       const uint8_t* vs_ptr = ks_ptr + S::kTokens * S::kRowBytes;
-      constexpr int kG = S::kTiles16;
+      constexpr int kG = S::kTokens / 16;
 
       // -- S^T = K Q^T
       float s[kG][NR][4];
@@ -533,7 +649,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV, NR>::kBlocks) attn_deco
 #pragma unroll
           for (int t16 = 0; t16 < kG; ++t16) {
             uint32_t af[4];
-            ldsm4(af, base + chunk_at<D, KV, false>(16 * t16 + (lane & 15), 2 * ks + (lane >> 4)));
+            ldsm4(af, base + chunk_at<D, KV, false, TMA>(16 * t16 + (lane & 15), 2 * ks + (lane >> 4)));
 #pragma unroll
             for (int nr = 0; nr < NR; ++nr) mma<KV>(s[t16][nr], af, b[nr][0], b[nr][1]);
           }
@@ -544,9 +660,9 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV, NR>::kBlocks) attn_deco
           uint32_t wl[kG][4], wh[kG][4];
 #pragma unroll
           for (int t16 = 0; t16 < kG; ++t16) {
-            const uint4 x = ld_shared_u128(ks_ptr + chunk_at<D, KV, false>(16 * t16 + g, c + 4 * q4));
+            const uint4 x = ld_shared_u128(ks_ptr + chunk_at<D, KV, false, TMA>(16 * t16 + g, c + 4 * q4));
             const uint4 y =
-                ld_shared_u128(ks_ptr + chunk_at<D, KV, false>(16 * t16 + g + 8, c + 4 * q4));
+                ld_shared_u128(ks_ptr + chunk_at<D, KV, false, TMA>(16 * t16 + g + 8, c + 4 * q4));
             wl[t16][0] = x.x, wl[t16][1] = x.y, wl[t16][2] = x.z, wl[t16][3] = x.w;
             wh[t16][0] = y.x, wh[t16][1] = y.y, wh[t16][2] = y.z, wh[t16][3] = y.w;
           }
@@ -585,10 +701,9 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV, NR>::kBlocks) attn_deco
         for (int t16 = 0; t16 < kG; ++t16)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const uint32_t both = __shfl_sync(0xffffffffu, bytes, 16 * t16 + g + 8 * j);
-            const uint32_t kb = both & 0xffu;
+            const uint32_t kb = __shfl_sync(0xffffffffu, kb_lane, 16 * t16 + g + 8 * j);
             const float k_scale = kb == 255u ? __int_as_float(0x7fc00000) : __uint_as_float(kb << 23);
-            v_byte[t16][j] = (int)(both >> 8);
+            v_byte[t16][j] = (int)__shfl_sync(0xffffffffu, vb_lane, 16 * t16 + g + 8 * j);
             raise_v |= v_byte[t16][j] > v_exp && v_byte[t16][j] != 255;
 #pragma unroll
             for (int nr = 0; nr < NR; ++nr) {
@@ -596,7 +711,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV, NR>::kBlocks) attn_deco
               s[t16][nr][2 * j + 1] *= k_scale;
             }
           }
-        next_bytes = scale_bytes(slot + 1 == S::kRing ? 0 : slot + 1);
+        scale_bytes(slot + 1 == S::kRing ? 0 : slot + 1, next_kb, next_vb);
       }
       bool raise = false;
 #pragma unroll
@@ -709,7 +824,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV, NR>::kBlocks) attn_deco
 #pragma unroll
           for (int t = 0; t < D / 16; ++t) {
             uint32_t af[4];
-            ldsm4_t(af, base + chunk_at<D, KV, true>(row, 2 * t + ((lane >> 3) & 1)));
+            ldsm4_t(af, base + chunk_at<D, KV, true, TMA>(row, 2 * t + ((lane >> 3) & 1)));
 #pragma unroll
             for (int nr = 0; nr < NR; ++nr) mma<KV>(o[t][nr], af, pf[t16][nr][0], pf[t16][nr][1]);
           }
@@ -724,14 +839,14 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV, NR>::kBlocks) attn_deco
             for (int i = 0; i < 4; ++i) {
               const int row = 16 * t16 + 2 * c + (i & 1) + 8 * (i >> 1);
               if (D >= 128) {
-                const uint4 x = ld_shared_u128(vs_ptr + chunk_at<D, KV, true>(row, g + 8 * hf));
+                const uint4 x = ld_shared_u128(vs_ptr + chunk_at<D, KV, true, TMA>(row, g + 8 * hf));
                 w[i][0] = x.x;
                 w[i][1] = x.y;
                 w[i][2] = x.z;
                 w[i][3] = x.w;
               } else {
                 const uint2 x = *reinterpret_cast<const uint2*>(
-                    vs_ptr + chunk_at<D, KV, true>(row, g >> 1) + (g & 1) * 8);
+                    vs_ptr + chunk_at<D, KV, true, TMA>(row, g >> 1) + (g & 1) * 8);
                 w[i][0] = x.x;
                 w[i][1] = x.y;
               }
@@ -754,10 +869,15 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV, NR>::kBlocks) attn_deco
       }
       __syncwarp();
       slot = slot + 1 == S::kRing ? 0 : slot + 1;
-      stage = stage + 1 == S::kStages ? 0 : stage + 1;
+      if (++stage == S::kStages) {
+        stage = 0;
+        phase ^= 1;
+      }
     }
 
-    // -- the four warps' (O, m, l) to one
+    // -- the warps' (O, m, l) to one: each warp leaves its O in the stage that it
+    // has just read (the next copy into it is issued after the barriers), eight
+    // rows at a time, and all threads add the warps' values
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
@@ -770,90 +890,84 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV, NR>::kBlocks) attn_deco
           sm.wl[warp][8 * nr + 2 * c + j] = l[nr][j];
         }
       }
-    if (lane == 0) sm.wv[warp] = v_exp;
     __syncthreads();
-    float f[NR][2];
-    {
-#pragma unroll
-      for (int nr = 0; nr < NR; ++nr)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          float mx = -INFINITY;
-          for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, sm.wm[w][8 * nr + 2 * c + j]);
-          f[nr][j] = m[nr][j] == -INFINITY ? 0.f : exp2_fast(m[nr][j] - mx);
-          // O is in units of 2^(v_exp - 127)
-          if (KV == kE4m3) f[nr][j] *= __uint_as_float((uint32_t)v_exp << 23);
-        }
+    if (tid < S::kRows) {
+      float mx = -INFINITY, sum = 0.f;
+      for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, sm.wm[w][tid]);
+      for (int w = 0; w < kWarps; ++w)
+        sum += sm.wm[w][tid] == -INFINITY ? sm.wl[w][tid] : sm.wl[w][tid] * exp2_fast(sm.wm[w][tid] - mx);
+      sm.mx[tid] = mx;
+      sm.sum[tid] = sum;
     }
-    for (int w = 0; w < kWarps; ++w) {
-      if (warp == w) {
+    const bool whole = u0 >= t0 && u1 <= t1;
+    const long long row_floats = D + 2;
+    const long long slot_floats = (long long)S::kRows * row_floats;
+    float* scratch = reinterpret_cast<float*>(a.scratch);
+    // slot 0: a block that enters the pair from the one before; 1: the first
+    float* part = scratch + (2ll * blockIdx.x + (u0 >= t0 ? 1 : 0)) * slot_floats;
+    const int free_stage = stage == 0 ? S::kStages - 1 : stage - 1;
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr) {
+      if (nr > 0) __syncthreads();  // the rows before have been read
+      float* mine = reinterpret_cast<float*>(sm.stage[warp][free_stage]);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int r = 8 * nr + 2 * c + j;
+        float mx = -INFINITY;
+        for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, sm.wm[w][r]);
+        float f = m[nr][j] == -INFINITY ? 0.f : exp2_fast(m[nr][j] - mx);
+        // O is in units of 2^(v_exp - 127)
+        if (KV == kE4m3) f *= __uint_as_float((uint32_t)v_exp << 23);
 #pragma unroll
         for (int t = 0; t < D / 16; ++t)
 #pragma unroll
-          for (int nr = 0; nr < NR; ++nr)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              int d;
-              if (KV != kE4m3)
-                d = 16 * t + g + 8 * (j >> 1);
-              else if (D >= 128)
-                d = 16 * (g + 8 * (t / 8)) + 2 * (t % 8) + (j >> 1);
-              else
-                d = 8 * g + 2 * t + (j >> 1);
-              float* dst = &sm.merge[8 * nr + 2 * c + (j & 1)][d];
-              const float v = f[nr][j & 1] == 0.f ? 0.f : o[t][nr][j] * f[nr][j & 1];
-              *dst = w == 0 ? v : *dst + v;
-            }
+          for (int h = 0; h < 2; ++h) {
+            int d;
+            if (KV != kE4m3)
+              d = 16 * t + g + 8 * h;
+            else if (D >= 128)
+              d = 16 * (g + 8 * (t / 8)) + 2 * (t % 8) + h;
+            else
+              d = 8 * g + 2 * t + h;
+            mine[(2 * c + j) * D + merge_col<KV>(d, c)] = f == 0.f ? 0.f : o[t][nr][2 * h + j] * f;
+          }
       }
       __syncthreads();
-    }
-
-    // -- out: the whole pair, or this block's part of it
-    const long long row_floats = D + 2;
-    if (u0 >= t0 && u1 <= t1) {
-      for (int r = warp; r < rows; r += kWarps) {
-        float mx = -INFINITY, sum = 0.f;
-        for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, sm.wm[w][r]);
+      for (int i = tid; i < 8 * D; i += kThreads) {
+        const int r = 8 * nr + i / D, d = i % D;
+        if (r >= rows) break;
+        const int at_col = (i / D) * D + merge_col<KV>(d, (i / D) >> 1);
+        float v = 0.f;
+#pragma unroll
         for (int w = 0; w < kWarps; ++w)
-          sum += sm.wm[w][r] == -INFINITY ? sm.wl[w][r] : sm.wl[w][r] * exp2_fast(sm.wm[w][r] - mx);
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        const long long tok = q0 + r / p.groups;
-        const int qh = head * p.groups + r % p.groups;
-        uint16_t* dst = static_cast<uint16_t*>(a.out) + tok * a.out_token_stride +
-                        qh * a.out_head_stride;
-        for (int d = lane * 2; d < D; d += 64) {
-          const float x = sm.merge[r][d] * inv, y = sm.merge[r][d + 1] * inv;
-          uint32_t pk;
-          if (a.q_f16) {
-            const __half2 b = __floats2half2_rn(x, y);
-            pk = *reinterpret_cast<const uint32_t*>(&b);
-          } else {
-            const __nv_bfloat162 b = __floats2bfloat162_rn(x, y);
-            pk = *reinterpret_cast<const uint32_t*>(&b);
-          }
-          *reinterpret_cast<uint32_t*>(dst + d) = pk;
+          v += reinterpret_cast<const float*>(sm.stage[w][free_stage])[at_col];
+        if (whole) {
+          const float sum = sm.sum[r];
+          const float x = sum == 0.f ? 0.f : v / sum;
+          static_cast<uint16_t*>(a.out)[(long long)(q0 + r / p.groups) * a.out_token_stride +
+                                        (long long)(head * p.groups + r % p.groups) * a.out_head_stride +
+                                        d] =
+              a.q_f16 ? __half_as_ushort(__float2half_rn(x)) : __bfloat16_as_ushort(__float2bfloat16_rn(x));
+        } else {
+          part[r * row_floats + 2 + d] = v;
         }
-        if (a.lse != nullptr && lane == 0)
-          a.lse[tok * a.q_heads + qh] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) / kLog2e;
       }
-    } else {
+    }
+    if (tid < rows) {
+      const float mx = sm.mx[tid], sum = sm.sum[tid];
+      if (!whole)
+        *reinterpret_cast<float2*>(part + tid * row_floats) = make_float2(mx, sum);
+      else if (a.lse != nullptr)
+        a.lse[(long long)(q0 + tid / p.groups) * a.q_heads + head * p.groups + tid % p.groups] =
+            sum == 0.f ? -INFINITY : (mx + log2f(sum)) / kLog2e;
+    }
+    // the copies that overwrite the stages come after these plain accesses
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+
+    if (!whole) {
       // Blocks of the pair: c_first holds its first tile, c_last its last one.
       const int c_first = (int)(((u0 + 1) * ctas - 1) / total);
       const int c_last = (int)((u1 * ctas - 1) / total);
-      const long long slot_floats = (long long)S::kRows * row_floats;
-      float* scratch = reinterpret_cast<float*>(a.scratch);
-      // slot 0: a block that enters the pair from the one before; 1: the first
-      float* part = scratch + (2ll * blockIdx.x + (u0 >= t0 ? 1 : 0)) * slot_floats;
-      for (int r = warp; r < rows; r += kWarps) {
-        float mx = -INFINITY, sum = 0.f;
-        for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, sm.wm[w][r]);
-        for (int w = 0; w < kWarps; ++w)
-          sum += sm.wm[w][r] == -INFINITY ? sm.wl[w][r] : sm.wl[w][r] * exp2_fast(sm.wm[w][r] - mx);
-        float* dst = part + r * row_floats;
-        for (int d = lane * 2; d < D; d += 64)
-          *reinterpret_cast<float2*>(dst + 2 + d) = make_float2(sm.merge[r][d], sm.merge[r][d + 1]);
-        if (lane == 0) *reinterpret_cast<float2*>(dst) = make_float2(mx, sum);
-      }
       __threadfence();
       __syncthreads();
       if (tid == 0) {
@@ -924,33 +1038,47 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV, NR>::kBlocks) attn_deco
   griddep_launch_dependents();
 }
 
-template <int D, int KV, int NR>
-cudaError_t launch(const DecodeParams& p, cudaStream_t stream) {
-  using Smem = typename Shape<D, KV, NR>::Smem;
+template <int D, int KV, int NR, bool TMA>
+cudaError_t launch(const DecodeParams& p, const CUtensorMap (&maps)[2], cudaStream_t stream) {
+  using S = Shape<D, KV, NR, TMA>;
   static bool configured[64] = {};
+  constexpr size_t kSmem = sizeof(typename S::Smem) + 1024;  // (to align the stages)
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return err;
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   if (!configured[dev]) {
-    err = cudaFuncSetAttribute(attn_decode_kernel<D, KV, NR>,
-                               cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Smem));
+    err = cudaFuncSetAttribute(attn_decode_kernel<D, KV, NR, TMA>,
+                               cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
     if (err != cudaSuccess) return err;
     configured[dev] = true;
   }
-  static_assert((sizeof(Smem) + 1024) * Shape<D, KV, NR>::kBlocks <= 228 * 1024, "fits the SM");
-  return launch_pdl(attn_decode_kernel<D, KV, NR>, 
-                    dim3((unsigned)(Shape<D, KV, NR>::kBlocks * device_sm_count())), dim3(kThreads),
-                    sizeof(Smem), stream, p);
+  static_assert((kSmem + 1024) * S::kBlocks <= 228 * 1024, "fits the SM");
+  static_assert(8 * D * 4 <= S::kStageBytes, "eight rows of O fit a stage");
+  return launch_pdl(attn_decode_kernel<D, KV, NR, TMA>,
+                    dim3((unsigned)(S::kBlocks * device_sm_count())), dim3(S::kThreads), kSmem,
+                    stream, p, maps[0], maps[1]);
 }
 
 template <int D, int KV>
-cudaError_t launch_rows(const DecodeParams& p, int rows, cudaStream_t stream) {
-  return rows <= 8 ? launch<D, KV, 1>(p, stream) : launch<D, KV, 2>(p, stream);
+cudaError_t launch_rows(DecodeParams& p, int rows, cudaStream_t stream) {
+  constexpr int kElem = KV == kE4m3 ? 1 : 2, kRowBytes = D * kElem;
+  const CUtensorMapDataType type = KV == kE4m3  ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                   : KV == kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  CUtensorMap maps[2] = {};
+  p.box_rows = cache_box_rows(p.a.c, 16);
+  if (make_cache_maps(p.a.c, type, kElem, (kRowBytes < 128 ? kRowBytes : 128) / kElem, p.box_rows,
+                      kRowBytes < 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                      &maps[0], &maps[1], &p.heads_first))
+    return rows <= 8 ? launch<D, KV, 1, true>(p, maps, stream)
+                     : launch<D, KV, 2, true>(p, maps, stream);
+  return rows <= 8 ? launch<D, KV, 1, false>(p, maps, stream)
+                   : launch<D, KV, 2, false>(p, maps, stream);
 }
 
 template <int D>
-cudaError_t launch_type(const DecodeParams& p, int rows, cudaStream_t stream) {
+cudaError_t launch_type(DecodeParams& p, int rows, cudaStream_t stream) {
   if (p.a.cache_dtype == 3) return launch_rows<D, kE4m3>(p, rows, stream);
   return p.a.cache_dtype == 1 ? launch_rows<D, kF16>(p, rows, stream)
                               : launch_rows<D, kBf16>(p, rows, stream);

@@ -43,6 +43,7 @@
 //
 // The maximum is lazy: m is raised, and O rescaled, only where some S exceeds it
 // by more than 8 (in log2), so that most tiles leave O alone.
+#include "attn_maps.cuh"
 #include "common.cuh"
 #include "internal.h"
 #include "tcgen05.cuh"
@@ -621,15 +622,6 @@ __device__ __forceinline__ float exp_row(uint32_t ts, const uint32_t (&s)[BN], f
   return t.x + t.y;
 }
 
-// One box of a page: 64 columns x box_rows tokens.
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z,
-                                            int w, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
-      "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
-      : "memory");
-}
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z,
                                             uint64_t* bar) {
   asm volatile(
@@ -1332,57 +1324,29 @@ cudaError_t launch(const PrefillParams& p, const CUtensorMap (&maps)[3], cudaStr
                     S::kSmem, stream, p, maps[0], maps[1], maps[2]);
 }
 
-// Tensor maps of q [tokens][heads][D] and of the cache [page][head][token][D]
-// (the two middle ones in the order of their strides). False where a map cannot
-// describe the call: pages that are no multiple of 8 tokens (a swizzle atom),
-// strides of zero, layouts the encoder declines.
+// Tensor maps of q [tokens][heads][D] and of the cache. False where maps cannot
+// describe the call (see make_cache_maps).
 bool make_maps(PrefillParams& p, int bn, CUtensorMap (&maps)[3]) {
   const AttnLaunch& a = p.a;
-  int rows = 8;
-  if (a.c.page_size % 8) return false;
-  while (rows < bn && a.c.page_size % (2 * rows) == 0) rows *= 2;
-  tcg_host::EncodeTiledFn fn = tcg_host::encode_tiled();
-  if (fn == nullptr) return false;
   const CUtensorMapDataType type = a.q_f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                            : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  const cuuint32_t ones[4] = {1, 1, 1, 1};
+  p.box_rows = cache_box_rows(a.c, bn);
+  if (!make_cache_maps(a.c, type, 2, 64, p.box_rows, CU_TENSOR_MAP_SWIZZLE_128B, &maps[1], &maps[2],
+                       &p.heads_first))
+    return false;
   const cuuint64_t d = (cuuint64_t)a.c.head_dim;
-  // a dimension of one element has no stride of its own
-  auto bytes = [&](long long stride, long long size, cuuint64_t other) {
-    return size == 1 ? other : (cuuint64_t)stride * 2;
-  };
-  {
-    const cuuint64_t hs = bytes(a.q_head_stride, a.q_heads, d * 2);
-    const cuuint64_t ts = bytes(a.q_token_stride, a.q_tokens, hs * (cuuint64_t)a.q_heads);
-    if (hs == 0 || ts == 0) return false;
-    const cuuint64_t dims[3] = {d, (cuuint64_t)a.q_heads, (cuuint64_t)a.q_tokens};
-    const cuuint64_t strides[2] = {hs, ts};
-    const cuuint32_t box[3] = {64, (cuuint32_t)p.groups, (cuuint32_t)p.tile_tokens};
-    if (fn(&maps[0], type, 3, const_cast<void*>(a.q), dims, strides, box, ones,
-           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-           CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-      return false;
-  }
-  const cuuint64_t ts = bytes(a.c.token_stride, a.c.page_size, d * 2);
-  const cuuint64_t hs = bytes(a.c.head_stride, a.c.heads, ts * (cuuint64_t)a.c.page_size);
-  const cuuint64_t ps =
-      bytes(a.c.page_stride, a.c.num_pages,
-            (ts > hs ? ts * (cuuint64_t)a.c.page_size : hs * (cuuint64_t)a.c.heads));
-  if (ts == 0 || hs == 0 || ps == 0) return false;
-  p.heads_first = hs < ts;
-  p.box_rows = rows;
-  const cuuint64_t np = (cuuint64_t)a.c.num_pages, nt = (cuuint64_t)a.c.page_size;
-  const cuuint64_t nh = (cuuint64_t)a.c.heads;
-  const cuuint64_t dims[4] = {d, p.heads_first ? nh : nt, p.heads_first ? nt : nh, np};
-  const cuuint64_t strides[3] = {p.heads_first ? hs : ts, p.heads_first ? ts : hs, ps};
-  const cuuint32_t r = (cuuint32_t)rows;
-  const cuuint32_t box[4] = {64, p.heads_first ? 1u : r, p.heads_first ? r : 1u, 1};
-  for (int i = 0; i < 2; ++i)
-    if (fn(&maps[1 + i], type, 4, i ? a.c.v : a.c.k, dims, strides, box, ones,
-           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-      return false;
-  return true;
+  const cuuint64_t hs = a.q_heads == 1 ? d * 2 : (cuuint64_t)a.q_head_stride * 2;
+  const cuuint64_t ts =
+      a.q_tokens == 1 ? hs * (cuuint64_t)a.q_heads : (cuuint64_t)a.q_token_stride * 2;
+  if (hs == 0 || ts == 0) return false;
+  const cuuint64_t dims[3] = {d, (cuuint64_t)a.q_heads, (cuuint64_t)a.q_tokens};
+  const cuuint64_t strides[2] = {hs, ts};
+  const cuuint32_t box[3] = {64, (cuuint32_t)p.groups, (cuuint32_t)p.tile_tokens};
+  const cuuint32_t ones[3] = {1, 1, 1};
+  return tcg_host::encode_tiled()(&maps[0], type, 3, const_cast<void*>(a.q), dims, strides, box,
+                                  ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                  CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <int D, int MT>
