@@ -18,12 +18,12 @@
 //   cut by a range border leaves partial (O, m, l) in the scratch; the last
 //   block to arrive at the pair's counter adds them in block order, so the
 //   result does not depend on which block that is.
-// * Each warp streams its own 16 of a tile's tokens through a private ring of
-//   stages: no block barrier inside a pair, and the ring runs on into the next
-//   pair while the present one is finished. Pages of a multiple of 8 tokens
-//   come by tensor copies, one or two boxes each of K and V a step, issued by
-//   one lane; other pages (single-token ones, say) by 16-byte cp.async, whose
-//   addresses take longer to compute than a step's products.
+// * One warp fills a ring of stages, a tile of 16 tokens per consumer warp each,
+//   and runs on into the next pair while the present one is finished. Pages of
+//   a multiple of 8 tokens come by tensor copies; other pages (single-token
+//   ones, say) by 16-byte cp.async. (When every warp issued the copies of its
+//   own tokens, issuing them took a third of its step: 75 to 150 clocks each.)
+//   Consumers meet only where a pair ends.
 // * The products are taken transposed (S^T = K Q^T, O^T = V^T P^T): the
 //   m16n8k16 tile then has 16 cached tokens or 16 head columns in M and 8 rows
 //   in N, so 8 query heads per key/value head waste nothing. K is read as the
@@ -62,45 +62,45 @@ struct DecodeParams {
 
 enum { kBf16 = 0, kF16 = 1, kE4m3 = 2 };
 
-// One ring entry's description, written when its page numbers are requested.
+// A tile's description, written by the producer a tile ahead of its copies.
 struct TileInfo {
   int seq, head;   // seq < 0: past the block's range
-  int token0;      // first of this warp's tokens
+  int token0;      // first token
   int end;         // tokens from here on do not exist
-  int page[2];     // tensor copies: pages of tokens 0-7 and 8-15
 };
 
 template <int D, int KV, int NR, bool TMA>
 struct Shape {
   static constexpr int kElem = KV == kE4m3 ? 1 : 2;
   static constexpr int kRowBytes = D * kElem;
-  // A warp takes 16 tokens a step. Its instructions wait on one another (loads,
-  // products, softmax, products), so as many warps share an SM as registers (128
-  // a thread at 16 warps) and the ring's stages allow: 16 for e4m3 and head_dim
-  // 64, 8 for head_dim 128 in 16 bits and 256 in e4m3, 4 for 256 in 16 bits.
+  // A consumer warp takes 16 tokens of a tile. Its instructions wait on one
+  // another (products, softmax, products), so as many warps share an SM as
+  // registers allow where a step is mostly conversions: 16 with the producers
+  // for e4m3 and head_dim 64 (128 registers a thread). 16-bit vectors of 128
+  // and 256 need no conversion and keep up with 7 and 4.
   static constexpr int kTokens = 16;
-  static constexpr int kWarps = KV == kE4m3 || D == 64 ? 8 : 4;
-  static constexpr int kThreads = kWarps * 32;
-  static constexpr int kTile = kTokens * kWarps;               // tokens per block step
-  static constexpr int kStageBytes = 2 * kTokens * kRowBytes;  // K then V of a warp
+  static constexpr int kWarps = D == 256 ? (KV == kE4m3 ? 7 : 4) : 7;
+  static constexpr int kConsumers = kWarps * 32;
+  static constexpr int kThreads = kConsumers + 32;
+  static constexpr int kTile = kTokens * kWarps;            // tokens per step
+  static constexpr int kHalfBytes = kTile * kRowBytes;      // K, or V, of a stage
+  static constexpr int kStageBytes = 2 * kHalfBytes;
   static constexpr int kRows = 8 * NR;
-  // Ring depth: 80 to 96 KB per block and two blocks per SM; head_dim 256, whose
-  // stages are 64 KB a block, takes one block per SM with 192 KB.
-  static constexpr int kBlocks = D == 256 ? 1 : 2;
+  // Ring: 70 to 84 KB per block and two blocks per SM, or 112 to 192 KB and one.
+  static constexpr int kBlocks = D == 64 || (D == 128 && KV == kE4m3) ? 2 : 1;
   static constexpr int kStages = KV == kE4m3 && D == 64 ? 5 : 3;
-  static constexpr int kAhead = kStages - 1;
-  static constexpr int kRing = 2 * kStages;  // tile descriptions
+  static constexpr int kRing = kStages + 2;  // tile descriptions
   static constexpr int kQPitch = D + 8;      // 16-bit elements, conflict-free rows
   struct Smem {
-    alignas(1024) uint8_t stage[kWarps][kStages][kStageBytes];
+    alignas(1024) uint8_t stage[kStages][kStageBytes];
     uint16_t q[kRows][kQPitch];
-    uint64_t full[kWarps][kStages];
-    int pages[TMA ? 1 : kWarps][kRing][kTokens];
-    TileInfo info[kWarps][kRing];
+    uint64_t full[kStages], empty[kStages];
+    int pages[kRing][TMA ? kTile / 8 : kTile];  // of 8 tokens, or of each
+    TileInfo info[kRing];
     float row_scale[kRows];
     int row_lo[kRows], row_hi[kRows];
     float wm[kWarps][kRows], wl[kWarps][kRows], mx[kRows], sum[kRows];
-    long long scan[kWarps];
+    long long scan[kWarps + 1];
     int start_seq;
     long long start_off;
     int flag;
@@ -111,13 +111,6 @@ __device__ __forceinline__ void cp_async_16_zfill(void* dst, const void* src, bo
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src),
                "r"(on ? 16 : 0)
                : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() {
-  asm volatile("cp.async.commit_group;" ::: "memory");
-}
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
@@ -162,15 +155,15 @@ __device__ __forceinline__ float pow2(int e) {
   return e < -126 ? 0.f : __uint_as_float((uint32_t)(127 + e) << 23);
 }
 
-// Byte of 16-byte chunk `chunk` of token row `row` in a warp's K or V tile,
+// Byte of 16-byte chunk `chunk` of token row `row` in a stage's K or V tile,
 // placed so that the operand reads below touch the banks evenly. Tensor copies
 // leave slices of 128 B with chunks XORed by the row's low bits (64 B rows: by
 // the row pair's).
-template <int D, int KV, bool IS_V, bool TMA>
+template <int D, int KV, bool IS_V, bool TMA, int TILE>
 __device__ __forceinline__ int chunk_at(int row, int chunk) {
   constexpr int kChunks = D * (KV == kE4m3 ? 1 : 2) / 16;
   if (kChunks == 4) return (row * 4 + (chunk ^ ((row >> 1) & 3))) * 16;
-  if (TMA) return (chunk >> 3) * 2048 + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
+  if (TMA) return (chunk >> 3) * (TILE * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
   int x;
   if (KV != kE4m3)
     x = row & 7;  // ldmatrix: 8 rows of one chunk column
@@ -179,7 +172,7 @@ __device__ __forceinline__ int chunk_at(int row, int chunk) {
   return (row * kChunks + (chunk ^ x)) * 16;
 }
 
-// Where column d of a row of O lies in a warp's free stage, so that the lanes
+// Where column d of a row of O lies in the warp's part of a stage, so that the lanes
 // that write the accumulators touch different banks (c: the lane's row pair).
 template <int KV>
 __device__ __forceinline__ int merge_col(int d, int c) {
@@ -224,19 +217,19 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
   using S = Shape<D, KV, NR, TMA>;
   constexpr int kAlign = TMA ? 16 : 1;
   using Smem = typename S::Smem;
-  constexpr int kWarps = S::kWarps, kThreads = S::kThreads;
+  constexpr int kWarps = S::kWarps, kThreads = S::kThreads, kConsumers = S::kConsumers;
   extern __shared__ uint8_t smem_raw[];
   Smem& sm = *reinterpret_cast<Smem*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
   const AttnLaunch& a = p.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, c = lane & 3;
   const int heads = a.c.heads;
-  if (TMA) {
-    if (lane == 0) {
-      for (int i = 0; i < S::kStages; ++i) mbar_init(&sm.full[warp][i], 1);
-      fence_mbar_init();
+  if (tid == 0) {
+    for (int i = 0; i < S::kStages; ++i) {
+      mbar_init(&sm.full[i], TMA ? 1 : 33);  // (lane 0's own arrival, and the copies')
+      mbar_init(&sm.empty[i], kWarps);
     }
-    __syncwarp();
+    fence_mbar_init();
   }
   griddep_wait();
 
@@ -258,7 +251,7 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
     before -= mine;
     total = 0;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w <= kWarps; ++w) {
       if (w < warp) before += sm.scan[w];
       total += sm.scan[w];
     }
@@ -283,148 +276,167 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
   const long long t0 = total * blockIdx.x / ctas;
   const long long t1 = total * (blockIdx.x + 1) / ctas;
 
-  // ---- the request cursor: the warp's next tile
-  int r_seq = sm.start_seq, r_head, r_tile;
-  SeqRange r_range = seq_range<S::kTile>(a, r_seq, kAlign);
-  r_head = (int)(sm.start_off / r_range.tiles);
-  r_tile = (int)(sm.start_off - (long long)r_head * r_range.tiles);
-  long long r_at = t0;
-  int r_slot = 0;
   auto page_of = [&](int token) {
     return p.page_shift >= 0 ? token >> p.page_shift : token / a.c.page_size;
   };
-  auto next_tile = [&]() {
-    TileInfo ti;
-    ti.seq = -1;
-    ti.head = r_head;
-    ti.token0 = ti.end = 0;
-    ti.page[0] = ti.page[1] = -1;
-    if (r_at < t1) {
-      ti.seq = r_seq;
-      ti.token0 = r_range.begin + r_tile * S::kTile + warp * S::kTokens;
-      ti.end = r_range.end;
-      ++r_at;
-      if (++r_tile == r_range.tiles) {
-        r_tile = 0;
-        if (++r_head == heads) {
-          r_head = 0;
-          if (r_at < t1) {
-            do {
-              r_range = seq_range<S::kTile>(a, ++r_seq, kAlign);
-            } while (r_range.tiles == 0);
+
+  if (warp == kWarps) {
+    // ------------------------------------------------------------ producer
+    int seq = sm.start_seq;
+    SeqRange range = seq_range<S::kTile>(a, seq, kAlign);
+    int head = (int)(sm.start_off / range.tiles);
+    int tile = (int)(sm.start_off - (long long)head * range.tiles);
+    long long at = t0;
+    auto next_tile = [&]() {
+      TileInfo ti;
+      ti.seq = -1;
+      ti.head = head;
+      ti.token0 = ti.end = 0;
+      if (at < t1) {
+        ti.seq = seq;
+        ti.token0 = range.begin + tile * S::kTile;
+        ti.end = range.end;
+        ++at;
+        if (++tile == range.tiles) {
+          tile = 0;
+          if (++head == heads) {
+            head = 0;
+            if (at < t1) {
+              do {
+                range = seq_range<S::kTile>(a, ++seq, kAlign);
+              } while (range.tiles == 0);
+            }
           }
         }
       }
-    }
-    return ti;
-  };
-
-  // -- cp.async: page numbers go into ring entry r_slot, by plain loads (`now`,
-  // the prologue) or asynchronously with the next group of copies, kAhead steps
-  // before the copies that need them.
-  auto request = [&](bool now) {
-    const TileInfo ti = next_tile();
-    if (ti.seq >= 0 && lane < S::kTokens && ti.token0 + lane < ti.end) {
-      const int* src = a.table + ti.seq * a.table_stride + page_of(ti.token0 + lane);
-      int* dst = &sm.pages[TMA ? 0 : warp][r_slot][lane];
-      if (now)
-        *dst = __ldg(src);
-      else
-        cp_async_4(dst, src);
-    }
-    if (lane == 0) sm.info[warp][r_slot] = ti;
-    r_slot = r_slot + 1 == S::kRing ? 0 : r_slot + 1;
-  };
-  auto issue = [&](int slot, int stage) {
-    const TileInfo ti = sm.info[warp][slot];
-    if (ti.seq >= 0) {
-      constexpr int kChunks = S::kRowBytes / 16;
-      uint8_t* ks = sm.stage[warp][stage];
-      uint8_t* vs = ks + S::kTokens * S::kRowBytes;
-      const long long head_off = (long long)ti.head * a.c.head_stride;
-      // byte offset of token row lane % kTokens, or -1
-      long long mine = -1;
-      {
-        const int token = ti.token0 + lane % S::kTokens;
-        if (token < ti.end) {
-          const int page = sm.pages[TMA ? 0 : warp][slot][lane % S::kTokens];
-          const int at_page = token - page_of(token) * a.c.page_size;
-          if (page >= 0 && page < a.c.num_pages)
-            mine = (page * a.c.page_stride + at_page * a.c.token_stride + head_off) * S::kElem;
-          else
-            atomicOr(a.status, kDevBadPage);
-        }
-      }
+      return ti;
+    };
+    // Page numbers: of the lane's box (tensor copies), or of token rows lane,
+    // lane + 32, ...; on their way while the tile before is copied.
+    constexpr int kLook = TMA ? 1 : (S::kTile + 31) / 32;
+    struct Pages {
+      int p[kLook];
+    };
+    const int box_rows = TMA ? p.box_rows : 1, boxes = S::kTile / box_rows;
+    auto look = [&](const TileInfo& ti) {
+      Pages pg;
 #pragma unroll
-      for (int i = 0; i < S::kTokens * kChunks / 32; ++i) {
-        const int id = i * 32 + lane;
-        const int row = id / kChunks, chunk = id % kChunks;
-        long long off = __shfl_sync(0xffffffffu, mine, row);
-        const bool on = off >= 0;
-        off = on ? off + chunk * 16 : 0;
-        cp_async_16_zfill(ks + chunk_at<D, KV, false, TMA>(row, chunk),
-                          static_cast<const uint8_t*>(a.c.k) + off, on);
-        cp_async_16_zfill(vs + chunk_at<D, KV, true, TMA>(row, chunk),
-                          static_cast<const uint8_t*>(a.c.v) + off, on);
+      for (int i = 0; i < kLook; ++i) {
+        const int row = (lane + 32 * i) * box_rows, token = ti.token0 + row;
+        pg.p[i] = ti.seq >= 0 && row < S::kTile && token < ti.end
+                      ? __ldg(a.table + ti.seq * a.table_stride + page_of(token))
+                      : -2;
       }
-    }
-  };
-
-  // -- tensor copies: lanes 0 and 1 look up the pages of tokens 0-7 and 8-15
-  // one step before the copy. Boxes past the last key and of pages outside the
-  // cache come from past the maps' end, which gives zeros.
-  auto look = [&](const TileInfo& ti) -> int {
-    const int token = ti.token0 + 8 * lane;
-    return ti.seq >= 0 && lane < 2 && token < ti.end
-               ? __ldg(a.table + ti.seq * a.table_stride + page_of(token))
-               : -2;
-  };
-  auto issue_tma = [&](TileInfo ti, int page, int stage) {
-    if (ti.seq >= 0) {
-      const int token = ti.token0 + 8 * lane;
-      int at = 0;
-      if (lane < 2) {
-        if (page < 0 || page >= a.c.num_pages) {
-          if (token < ti.end) atomicOr(a.status, kDevBadPage);
-          page = -1;
-        } else {
-          at = token - page_of(token) * a.c.page_size;
-        }
+      return pg;
+    };
+    auto publish = [&](int slot, const TileInfo& ti, const Pages& pg) {
+      if (lane == 0) sm.info[slot] = ti;
+      if (TMA) {
+        if (lane < boxes)
+          for (int i = 0; i < box_rows / 8; ++i) sm.pages[slot][lane * (box_rows / 8) + i] = pg.p[0];
+      } else {
+#pragma unroll
+        for (int i = 0; i < kLook; ++i)
+          if (lane + 32 * i < S::kTile) sm.pages[slot][lane + 32 * i] = pg.p[i];
       }
-      ti.page[0] = __shfl_sync(0xffffffffu, page, 0);
-      ti.page[1] = __shfl_sync(0xffffffffu, page, 1);
-      if (lane == 0) mbar_arrive_expect_tx(&sm.full[warp][stage], S::kStageBytes);
       __syncwarp();
-      if (lane < (p.box_rows == 8 ? 2 : 1)) {
-        const uint32_t dst = smem_u32(sm.stage[warp][stage]) +
-                             lane * 8 * (S::kRowBytes < 128 ? S::kRowBytes : 128);
-        const int pg = page < 0 ? (int)a.c.num_pages : page;
-        const int y = p.heads_first ? ti.head : at, z = p.heads_first ? at : ti.head;
-        constexpr int kSlices = S::kRowBytes <= 128 ? 1 : S::kRowBytes / 128;
-        constexpr int kCols = (S::kRowBytes < 128 ? S::kRowBytes : 128) / S::kElem;
+    };
+    TileInfo ti = next_tile(), ahead = next_tile();
+    Pages pg = look(ti), pg_ahead = look(ahead);
+    publish(0, ti, pg);
+    int slot = 0, stage = 0;
+    uint32_t phase = 1;  // a fresh stage is free
+    while (ti.seq >= 0) {
+      // the next tile's description is there before this one's copies land
+      slot = slot + 1 == S::kRing ? 0 : slot + 1;
+      publish(slot, ahead, pg_ahead);
+      mbar_wait(&sm.empty[stage], phase, a.status);
+      uint8_t* ks = sm.stage[stage];
+      if (TMA) {
+        if (lane == 0) mbar_arrive_expect_tx(&sm.full[stage], S::kStageBytes);
+        __syncwarp();
+        if (lane < boxes) {
+          const int token = ti.token0 + lane * box_rows;
+          int page = pg.p[0], row = 0;
+          if (page >= 0 && page < a.c.num_pages) {
+            row = token - page_of(token) * a.c.page_size;
+          } else {
+            // past the last key, or no page of the cache: from past the maps'
+            // end, which gives zeros
+            if (token < ti.end) atomicOr(a.status, kDevBadPage);
+            page = (int)a.c.num_pages;
+          }
+          const int y = p.heads_first ? ti.head : row, z = p.heads_first ? row : ti.head;
+          constexpr int kSliceBytes = S::kRowBytes < 128 ? S::kRowBytes : 128;
+          const uint32_t dst = smem_u32(ks) + lane * box_rows * kSliceBytes;
 #pragma unroll
-        for (int sl = 0; sl < kSlices; ++sl) {
-          tma_load_4d(dst + sl * 2048, &k_map, sl * kCols, y, z, pg, &sm.full[warp][stage]);
-          tma_load_4d(dst + S::kTokens * S::kRowBytes + sl * 2048, &v_map, sl * kCols, y, z, pg,
-                      &sm.full[warp][stage]);
+          for (int sl = 0; sl < S::kRowBytes / kSliceBytes; ++sl) {
+            const int x = sl * (kSliceBytes / S::kElem);
+            tma_load_4d(dst + sl * S::kTile * 128, &k_map, x, y, z, page, &sm.full[stage]);
+            tma_load_4d(dst + S::kHalfBytes + sl * S::kTile * 128, &v_map, x, y, z, page,
+                        &sm.full[stage]);
+          }
         }
+      } else {
+        constexpr int kChunks = S::kRowBytes / 16;
+        long long off[kLook];  // byte offsets of rows lane + 32 i, or -1
+#pragma unroll
+        for (int i = 0; i < kLook; ++i) {
+          const int row = lane + 32 * i, token = ti.token0 + row;
+          off[i] = -1;
+          if (row < S::kTile && token < ti.end) {
+            if (pg.p[i] >= 0 && pg.p[i] < a.c.num_pages)
+              off[i] = (pg.p[i] * a.c.page_stride +
+                        (token - page_of(token) * a.c.page_size) * a.c.token_stride +
+                        ti.head * a.c.head_stride) * S::kElem;
+            else
+              atomicOr(a.status, kDevBadPage);
+          }
+        }
+        constexpr int kPerPass = 32 / kChunks;  // rows per instruction
+#pragma unroll
+        for (int i = 0; i < kLook; ++i)
+#pragma unroll 4
+          for (int j = 0; j < (kChunks < 32 ? kChunks : 32); ++j) {
+            const int r32 = j * kPerPass + lane / kChunks, row = 32 * i + r32;
+            long long o = __shfl_sync(0xffffffffu, off[i], r32);
+            const bool on = o >= 0;
+            const int chunk = lane % kChunks;
+            o = on ? o + chunk * 16 : 0;
+            if (row < S::kTile) {
+              cp_async_16_zfill(ks + chunk_at<D, KV, false, TMA, S::kTile>(row, chunk),
+                                static_cast<const uint8_t*>(a.c.k) + o, on);
+              cp_async_16_zfill(ks + S::kHalfBytes + chunk_at<D, KV, true, TMA, S::kTile>(row, chunk),
+                                static_cast<const uint8_t*>(a.c.v) + o, on);
+            }
+          }
+        cp_async_arrive_noinc(&sm.full[stage]);
+        if (lane == 0) mbar_arrive(&sm.full[stage]);
+      }
+      ti = ahead;
+      pg = pg_ahead;
+      ahead = next_tile();
+      pg_ahead = look(ahead);
+      if (++stage == S::kStages) {
+        stage = 0;
+        phase ^= 1;
       }
     }
-    if (lane == 0) sm.info[warp][r_slot] = ti;
-    r_slot = r_slot + 1 == S::kRing ? 0 : r_slot + 1;
-  };
+    if (!TMA) asm volatile("cp.async.wait_all;" ::: "memory");
+    griddep_launch_dependents();
+    return;
+  }
 
-  // The scale bytes of token lane % 16 in ring entry `slot`: 0 (2^-127, and
-  // codes of zero) for absent tokens. (Two registers: joining them would wait
-  // for the loads here, a step before they are needed.)
+  // The scale bytes of token lane % 16 of this warp's part of tile `slot`: 0
+  // (2^-127, and codes of zero) for absent tokens. (Two registers: joining them
+  // would wait for the loads here, a step before they are needed.)
   auto scale_bytes = [&](int slot, uint32_t& kb, uint32_t& vb) {
     kb = vb = 0;
     if (KV != kE4m3) return;
-    const TileInfo ti = sm.info[warp][slot];
-    const int row = lane % S::kTokens, token = ti.token0 + row;
+    const TileInfo ti = sm.info[slot];
+    const int row = warp * S::kTokens + lane % S::kTokens, token = ti.token0 + row;
     if (ti.seq < 0 || token >= ti.end) return;
-    const int page = TMA ? ti.page[p.box_rows == 8 ? row >> 3 : 0]
-                         : sm.pages[TMA ? 0 : warp][slot][row];
+    const int page = sm.pages[slot][TMA ? row >> 3 : row];
     if (page < 0 || page >= a.c.num_pages) return;
     const long long at = page * a.c.scale_page_stride +
                          (token - page_of(token) * a.c.page_size) * a.c.scale_token_stride +
@@ -432,34 +444,7 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
     kb = __ldg(a.c.k_scale + at);
     vb = __ldg(a.c.v_scale + at);
   };
-
-  // ---- prologue
-  TileInfo ahead;        // tensor copies: the tile to be issued next,
-  int ahead_page = -2;   // and its pages
-  if (TMA) {
-    TileInfo ti[S::kAhead];
-    int pg[S::kAhead];
-#pragma unroll
-    for (int i = 0; i < S::kAhead; ++i) {
-      ti[i] = next_tile();
-      pg[i] = look(ti[i]);
-    }
-    ahead = next_tile();
-    ahead_page = look(ahead);
-#pragma unroll
-    for (int i = 0; i < S::kAhead; ++i) issue_tma(ti[i], pg[i], i);
-  } else {
-    for (int i = 0; i < S::kAhead; ++i) request(true);
-    __syncwarp();
-    for (int i = 0; i < S::kAhead; ++i) {
-      issue(i, i);
-      request(false);
-      cp_async_commit();
-    }
-  }
-  __syncwarp();
-  uint32_t next_kb, next_vb;
-  scale_bytes(0, next_kb, next_vb);
+  auto sync_consumers = [&]() { named_bar_sync(1, kConsumers); };
 
   // ---- consume
   float o[D / 16][NR][4];
@@ -467,17 +452,17 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
   int v_exp = 1;              // e4m3: byte of the largest value scale so far
   long long at = t0;
   int slot = 0, stage = 0;
-  uint32_t phase = 0;
+  uint32_t phase = 0, next_kb = 0, next_vb = 0;
   while (at < t1) {
     // -- a (sequence, head) pair begins: its tiles of this block are
     // [at, pair_end); u0, u1 bound the whole pair
-    if (!TMA) cp_async_wait<S::kAhead - 1>();
-    __syncwarp();
-    const TileInfo first = sm.info[warp][slot];
+    mbar_wait(&sm.full[stage], phase, a.status);
+    const TileInfo first = sm.info[slot];
+    if (at == t0) scale_bytes(slot, next_kb, next_vb);
     const SeqRange range = seq_range<S::kTile>(a, first.seq, kAlign);
     const int head = first.head;
     const long long u0 =
-        at - (first.token0 - warp * S::kTokens - range.begin) / S::kTile;
+        at - (first.token0 - range.begin) / S::kTile;
     const long long u1 = u0 + range.tiles;
     const long long pair_end = u1 < t1 ? u1 : t1;
     const int q0 = __ldg(a.q_starts + first.seq);
@@ -533,7 +518,7 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
         sm.row_lo[r] = lo;
       }
     }
-    __syncthreads();
+    sync_consumers();
 
     // Q as B fragments: for k-step ks, register pair [ks][nr]. K's columns are
     // taken in the order the A operand finds them in memory.
@@ -591,37 +576,24 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
         for (int j = 0; j < 4; ++j) o[t][nr][j] = 0.f;
 
     for (; at < pair_end; ++at) {
-      const TileInfo ti = sm.info[warp][slot];
-      const int token0 = ti.token0;
+      mbar_wait(&sm.full[stage], phase, a.status);
+      const int token0 = sm.info[slot].token0 + warp * S::kTokens;
       const uint32_t kb_lane = next_kb, vb_lane = next_vb;
-      // refill: the stage freed last step, with the tile kAhead steps on
-      const int refill = stage == 0 ? S::kStages - 1 : stage - 1;
-      if (TMA) {
-        issue_tma(ahead, ahead_page, refill);
-        ahead = next_tile();
-        ahead_page = look(ahead);
-        mbar_wait(&sm.full[warp][stage], phase, a.status);
-        if (token0 + S::kTokens > ti.end) {
-          // what a page holds past the last key may be NaN, and P zero times it
-          // NaN again: those rows of V become zeros
-          uint8_t* v = sm.stage[warp][stage] + S::kTokens * S::kRowBytes;
-          constexpr int kChunks = S::kRowBytes / 16;
-          for (int i = max(ti.end - token0, 0) * kChunks + lane; i < S::kTokens * kChunks; i += 32)
-            *reinterpret_cast<uint4*>(v + chunk_at<D, KV, true, TMA>(i / kChunks, i % kChunks)) =
-                make_uint4(0u, 0u, 0u, 0u);
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the next copy here
-          __syncwarp();
-        }
-      } else {
-        cp_async_wait<S::kAhead - 1>();
+      const int first_row = warp * S::kTokens;
+      if (TMA && token0 + S::kTokens > range.end) {
+        // what a page holds past the last key may be NaN, and P zero times it
+        // NaN again: those rows of V become zeros
+        uint8_t* v = sm.stage[stage] + S::kHalfBytes;
+        constexpr int kChunks = S::kRowBytes / 16;
+        for (int i = max(range.end - token0, 0) * kChunks + lane; i < S::kTokens * kChunks; i += 32)
+          *reinterpret_cast<uint4*>(v + chunk_at<D, KV, true, TMA, S::kTile>(first_row + i / kChunks,
+                                                                             i % kChunks)) =
+              make_uint4(0u, 0u, 0u, 0u);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the next copy here
         __syncwarp();
-        const int s2 = slot + S::kAhead < S::kRing ? slot + S::kAhead : slot + S::kAhead - S::kRing;
-        issue(s2, refill);
-        request(false);
-        cp_async_commit();
       }
-      const uint8_t* ks_ptr = sm.stage[warp][stage];
-      const uint8_t* vs_ptr = ks_ptr + S::kTokens * S::kRowBytes;
+      const uint8_t* ks_ptr = sm.stage[stage];
+      const uint8_t* vs_ptr = ks_ptr + S::kHalfBytes;
       constexpr int kG = S::kTokens / 16;
 
       // -- S^T = K Q^T
@@ -649,7 +621,7 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
 #pragma unroll
           for (int t16 = 0; t16 < kG; ++t16) {
             uint32_t af[4];
-            ldsm4(af, base + chunk_at<D, KV, false, TMA>(16 * t16 + (lane & 15), 2 * ks + (lane >> 4)));
+            ldsm4(af, base + chunk_at<D, KV, false, TMA, S::kTile>(first_row + 16 * t16 + (lane & 15), 2 * ks + (lane >> 4)));
 #pragma unroll
             for (int nr = 0; nr < NR; ++nr) mma<KV>(s[t16][nr], af, b[nr][0], b[nr][1]);
           }
@@ -660,9 +632,9 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
           uint32_t wl[kG][4], wh[kG][4];
 #pragma unroll
           for (int t16 = 0; t16 < kG; ++t16) {
-            const uint4 x = ld_shared_u128(ks_ptr + chunk_at<D, KV, false, TMA>(16 * t16 + g, c + 4 * q4));
+            const uint4 x = ld_shared_u128(ks_ptr + chunk_at<D, KV, false, TMA, S::kTile>(first_row + 16 * t16 + g, c + 4 * q4));
             const uint4 y =
-                ld_shared_u128(ks_ptr + chunk_at<D, KV, false, TMA>(16 * t16 + g + 8, c + 4 * q4));
+                ld_shared_u128(ks_ptr + chunk_at<D, KV, false, TMA, S::kTile>(first_row + 16 * t16 + g + 8, c + 4 * q4));
             wl[t16][0] = x.x, wl[t16][1] = x.y, wl[t16][2] = x.z, wl[t16][3] = x.w;
             wh[t16][0] = y.x, wh[t16][1] = y.y, wh[t16][2] = y.z, wh[t16][3] = y.w;
           }
@@ -820,11 +792,11 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
         if (KV != kE4m3) {
           const uint32_t base = smem_u32(vs_ptr);
           // matrices: (tokens 0-7, columns 0-7), (0-7, 8-15), (8-15, 0-7), (8-15, 8-15)
-          const int row = 16 * t16 + (lane & 7) + ((lane >> 4) << 3);
+          const int row = first_row + 16 * t16 + (lane & 7) + ((lane >> 4) << 3);
 #pragma unroll
           for (int t = 0; t < D / 16; ++t) {
             uint32_t af[4];
-            ldsm4_t(af, base + chunk_at<D, KV, true, TMA>(row, 2 * t + ((lane >> 3) & 1)));
+            ldsm4_t(af, base + chunk_at<D, KV, true, TMA, S::kTile>(row, 2 * t + ((lane >> 3) & 1)));
 #pragma unroll
             for (int nr = 0; nr < NR; ++nr) mma<KV>(o[t][nr], af, pf[t16][nr][0], pf[t16][nr][1]);
           }
@@ -837,16 +809,16 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
             uint32_t w[4][4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const int row = 16 * t16 + 2 * c + (i & 1) + 8 * (i >> 1);
+              const int row = first_row + 16 * t16 + 2 * c + (i & 1) + 8 * (i >> 1);
               if (D >= 128) {
-                const uint4 x = ld_shared_u128(vs_ptr + chunk_at<D, KV, true, TMA>(row, g + 8 * hf));
+                const uint4 x = ld_shared_u128(vs_ptr + chunk_at<D, KV, true, TMA, S::kTile>(row, g + 8 * hf));
                 w[i][0] = x.x;
                 w[i][1] = x.y;
                 w[i][2] = x.z;
                 w[i][3] = x.w;
               } else {
                 const uint2 x = *reinterpret_cast<const uint2*>(
-                    vs_ptr + chunk_at<D, KV, true, TMA>(row, g >> 1) + (g & 1) * 8);
+                    vs_ptr + chunk_at<D, KV, true, TMA, S::kTile>(row, g >> 1) + (g & 1) * 8);
                 w[i][0] = x.x;
                 w[i][1] = x.y;
               }
@@ -867,7 +839,9 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
           }
         }
       }
+      // The pair's last stage is kept: the warps' results meet in it.
       __syncwarp();
+      if (lane == 0 && at + 1 < pair_end) mbar_arrive(&sm.empty[stage]);
       slot = slot + 1 == S::kRing ? 0 : slot + 1;
       if (++stage == S::kStages) {
         stage = 0;
@@ -875,9 +849,8 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
       }
     }
 
-    // -- the warps' (O, m, l) to one: each warp leaves its O in the stage that it
-    // has just read (the next copy into it is issued after the barriers), eight
-    // rows at a time, and all threads add the warps' values
+    // -- the warps' (O, m, l) to one: each warp leaves its O in the pair's last
+    // stage, eight rows at a time, and all threads add the warps' values
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
@@ -890,7 +863,7 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
           sm.wl[warp][8 * nr + 2 * c + j] = l[nr][j];
         }
       }
-    __syncthreads();
+    sync_consumers();
     if (tid < S::kRows) {
       float mx = -INFINITY, sum = 0.f;
       for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, sm.wm[w][tid]);
@@ -905,11 +878,11 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
     float* scratch = reinterpret_cast<float*>(a.scratch);
     // slot 0: a block that enters the pair from the one before; 1: the first
     float* part = scratch + (2ll * blockIdx.x + (u0 >= t0 ? 1 : 0)) * slot_floats;
-    const int free_stage = stage == 0 ? S::kStages - 1 : stage - 1;
+    const int last_stage = stage == 0 ? S::kStages - 1 : stage - 1;
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr) {
-      if (nr > 0) __syncthreads();  // the rows before have been read
-      float* mine = reinterpret_cast<float*>(sm.stage[warp][free_stage]);
+      if (nr > 0) sync_consumers();  // the rows before have been read
+      float* mine = reinterpret_cast<float*>(sm.stage[last_stage]) + warp * 8 * D;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int r = 8 * nr + 2 * c + j;
@@ -932,15 +905,15 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
             mine[(2 * c + j) * D + merge_col<KV>(d, c)] = f == 0.f ? 0.f : o[t][nr][2 * h + j] * f;
           }
       }
-      __syncthreads();
-      for (int i = tid; i < 8 * D; i += kThreads) {
+      sync_consumers();
+      for (int i = tid; i < 8 * D; i += kConsumers) {
         const int r = 8 * nr + i / D, d = i % D;
         if (r >= rows) break;
         const int at_col = (i / D) * D + merge_col<KV>(d, (i / D) >> 1);
         float v = 0.f;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w)
-          v += reinterpret_cast<const float*>(sm.stage[w][free_stage])[at_col];
+          v += reinterpret_cast<const float*>(sm.stage[last_stage])[w * 8 * D + at_col];
         if (whole) {
           const float sum = sm.sum[r];
           const float x = sum == 0.f ? 0.f : v / sum;
@@ -969,14 +942,14 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
       const int c_first = (int)(((u0 + 1) * ctas - 1) / total);
       const int c_last = (int)((u1 * ctas - 1) / total);
       __threadfence();
-      __syncthreads();
+      sync_consumers();
       if (tid == 0) {
         const int n = atomicAdd(a.counters + c_first, 1) + 1;
         sm.flag = n == c_last - c_first + 1;
         if (sm.flag) a.counters[c_first] = 0;
         __threadfence();
       }
-      __syncthreads();
+      sync_consumers();
       if (sm.flag) {
         // The parts' maximum, a warp per row; then their weighted sum, a thread
         // per two columns and row at a time, eight parts in flight.
@@ -991,8 +964,8 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
           for (int x = 16; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
           if (lane == 0) sm.mx[r] = mx;
         }
-        __syncthreads();
-        for (int i = tid; i < rows * (D / 2); i += kThreads) {
+        sync_consumers();
+        for (int i = tid; i < rows * (D / 2); i += kConsumers) {
           const int r = i / (D / 2), d = 2 * (i % (D / 2));
           const float mx = sm.mx[r];
           float sum = 0.f, x = 0.f, y = 0.f;
@@ -1032,9 +1005,9 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
         }
       }
     }
-    __syncthreads();
+    sync_consumers();
+    if (lane == 0) mbar_arrive(&sm.empty[last_stage]);
   }
-  cp_async_wait<0>();
   griddep_launch_dependents();
 }
 
@@ -1054,7 +1027,7 @@ cudaError_t launch(const DecodeParams& p, const CUtensorMap (&maps)[2], cudaStre
     configured[dev] = true;
   }
   static_assert((kSmem + 1024) * S::kBlocks <= 228 * 1024, "fits the SM");
-  static_assert(8 * D * 4 <= S::kStageBytes, "eight rows of O fit a stage");
+  static_assert(S::kWarps * 8 * D * 4 <= S::kStageBytes, "eight rows of O a warp fit a stage");
   return launch_pdl(attn_decode_kernel<D, KV, NR, TMA>,
                     dim3((unsigned)(S::kBlocks * device_sm_count())), dim3(S::kThreads), kSmem,
                     stream, p, maps[0], maps[1]);
@@ -1067,7 +1040,7 @@ cudaError_t launch_rows(DecodeParams& p, int rows, cudaStream_t stream) {
                                    : KV == kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   CUtensorMap maps[2] = {};
-  p.box_rows = cache_box_rows(p.a.c, 16);
+  p.box_rows = cache_box_rows(p.a.c, 16);  // a warp's tokens
   if (make_cache_maps(p.a.c, type, kElem, (kRowBytes < 128 ? kRowBytes : 128) / kElem, p.box_rows,
                       kRowBytes < 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
                       &maps[0], &maps[1], &p.heads_first))
