@@ -46,9 +46,16 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 8.f;        // log2 of the largest P before a rescale
 constexpr int kMaxCtas = 1024;      // arrival counters in the workspace
-// A block takes at least this many tiles: below it the pair's merge costs more
-// than the extra blocks bring.
+// A block takes at least this much work, in tiles: below it the pair's merge
+// costs more than the extra blocks bring. And a pair is cut into at most
+// kMaxParts, whose sum one block takes.
 constexpr int kMinTiles = 4;
+constexpr int kMaxParts = 64;
+// What a (sequence, head) pair costs besides its tiles, in tiles of about 100
+// tokens (1 us): its start and the warps' meeting. Cutting by tiles alone left
+// the block with the most short sequences at 177 us where the median took 100
+// (64 sequences of 1 to 8192 tokens, 8 heads, e4m3).
+constexpr int kPairCost = 3;
 
 struct DecodeParams {
   AttnLaunch a;
@@ -63,10 +70,15 @@ struct DecodeParams {
 enum { kBf16 = 0, kF16 = 1, kE4m3 = 2 };
 
 // A tile's description, written by the producer a tile ahead of its copies.
-struct TileInfo {
-  int seq, head;   // seq < 0: past the block's range
-  int token0;      // first token
-  int end;         // tokens from here on do not exist
+struct __align__(16) TileInfo {
+  int seq, head;      // seq < 0: past the block's range
+  int token0;         // first token
+  int end;            // tokens from here on do not exist
+  int q0, q_len;      // the sequence's new tokens
+  int tile, tiles;    // of the pair
+  int left;           // this block's tiles of the pair from here on
+  int pair;           // pairs of this block before it
+  long long pair_at;  // place of the pair in the flattened cost
 };
 
 template <int D, int KV, int NR, bool TMA>
@@ -93,14 +105,13 @@ struct Shape {
   static constexpr int kQPitch = D + 8;      // 16-bit elements, conflict-free rows
   struct Smem {
     alignas(1024) uint8_t stage[kStages][kStageBytes];
-    uint16_t q[kRows][kQPitch];
-    uint64_t full[kStages], empty[kStages];
+    uint16_t q[2][kRows][kQPitch];  // of a pair, and of the next one
+    uint64_t full[kStages], empty[kStages], q_full[2], q_empty[2];
     int pages[kRing][TMA ? kTile / 8 : kTile];  // of 8 tokens, or of each
     TileInfo info[kRing];
     float row_scale[kRows];
-    int row_lo[kRows], row_hi[kRows];
     float wm[kWarps][kRows], wl[kWarps][kRows], mx[kRows], sum[kRows];
-    long long scan[kWarps + 1];
+    long long scan[kWarps + 1], scan_pairs[kWarps + 1];
     int start_seq;
     long long start_off;
     int flag;
@@ -183,7 +194,7 @@ __device__ __forceinline__ int merge_col(int d, int c) {
 // A sequence with new tokens always has one tile, so that its rows are written
 // even where nothing is cached.
 struct SeqRange {
-  int begin, end, q_len, kv_len, tiles;
+  int begin, end, q0, q_len, kv_len, tiles;
 };
 template <int kTile>
 __device__ __forceinline__ SeqRange seq_range(const AttnLaunch& a, int s, int align) {
@@ -196,6 +207,7 @@ __device__ __forceinline__ SeqRange seq_range(const AttnLaunch& a, int s, int al
   int ql = q1 - q0;
   if (q0 < 0 || q1 > a.q_tokens) ql = 0;  // outside q: nothing is read or written
   ql = ql < 0 ? 0 : (ql > a.max_q ? a.max_q : ql);
+  r.q0 = q0;
   r.q_len = ql;
   r.kv_len = kv;
   r.end = kv;
@@ -229,50 +241,67 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
       mbar_init(&sm.full[i], TMA ? 1 : 33);  // (lane 0's own arrival, and the copies')
       mbar_init(&sm.empty[i], kWarps);
     }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sm.q_full[i], 32);
+      mbar_init(&sm.q_empty[i], kWarps);
+    }
     fence_mbar_init();
   }
   griddep_wait();
 
-  // ---- this block's range of the flattened (sequence, head, tile) space
+  // ---- this block's range of the flattened (sequence, head, cost) space: a
+  // pair's first kPairCost places stand for its constant cost, the others for a
+  // tile each
   long long total;
+  int ctas;
+  auto cost_of = [&](const SeqRange& r) { return r.tiles ? r.tiles + kPairCost : 0; };
   {
     const int per = (a.seqs + kThreads - 1) / kThreads;
-    const int s0 = tid * per, s1 = min(s0 + per, a.seqs);
-    long long mine = 0;
-    for (int s = s0; s < s1; ++s) mine += (long long)seq_range<S::kTile>(a, s, kAlign).tiles * heads;
+    const int s0 = min(tid * per, a.seqs), s1 = min(s0 + per, a.seqs);
+    long long mine = 0, pairs = 0;
+    for (int s = s0; s < s1; ++s) {
+      const int n = cost_of(seq_range<S::kTile>(a, s, kAlign));
+      mine += (long long)n * heads;
+      pairs += n ? heads : 0;
+    }
     long long before = mine;  // inclusive scan, made exclusive below
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const long long v = __shfl_up_sync(0xffffffffu, before, o);
       if (lane >= o) before += v;
+      pairs += __shfl_xor_sync(0xffffffffu, pairs, o);
     }
-    if (lane == 31) sm.scan[warp] = before;
+    if (lane == 31) {
+      sm.scan[warp] = before;
+      sm.scan_pairs[warp] = pairs;
+    }
     __syncthreads();
     before -= mine;
-    total = 0;
+    total = pairs = 0;
 #pragma unroll
     for (int w = 0; w <= kWarps; ++w) {
       if (w < warp) before += sm.scan[w];
       total += sm.scan[w];
+      pairs += sm.scan_pairs[w];
     }
     if (total == 0) return;
-    long long ctas = (total + kMinTiles - 1) / kMinTiles;
-    if (ctas > gridDim.x) ctas = gridDim.x;
+    long long n = (total + kMinTiles - 1) / kMinTiles;
+    n = min(n, min(pairs * kMaxParts, (long long)gridDim.x));
+    ctas = (int)n;
     if (blockIdx.x >= ctas) return;
     const long long t0 = total * blockIdx.x / ctas;
     if (t0 >= before && t0 < before + mine) {
       int s = s0;
       for (;; ++s) {
-        const long long n = (long long)seq_range<S::kTile>(a, s, kAlign).tiles * heads;
-        if (t0 < before + n) break;
-        before += n;
+        const long long n1 = (long long)cost_of(seq_range<S::kTile>(a, s, kAlign)) * heads;
+        if (t0 < before + n1) break;
+        before += n1;
       }
       sm.start_seq = s;
       sm.start_off = t0 - before;
     }
     __syncthreads();
   }
-  const int ctas = (int)min((long long)gridDim.x, (total + kMinTiles - 1) / kMinTiles);
   const long long t0 = total * blockIdx.x / ctas;
   const long long t1 = total * (blockIdx.x + 1) / ctas;
 
@@ -284,28 +313,42 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
     // ------------------------------------------------------------ producer
     int seq = sm.start_seq;
     SeqRange range = seq_range<S::kTile>(a, seq, kAlign);
-    int head = (int)(sm.start_off / range.tiles);
-    int tile = (int)(sm.start_off - (long long)head * range.tiles);
+    int head = (int)(sm.start_off / cost_of(range));
+    int x = (int)(sm.start_off - (long long)head * cost_of(range));  // place in the pair
     long long at = t0;
+    int pair = -1;
     auto next_tile = [&]() {
       TileInfo ti;
       ti.seq = -1;
-      ti.head = head;
       ti.token0 = ti.end = 0;
-      if (at < t1) {
-        ti.seq = seq;
-        ti.token0 = range.begin + tile * S::kTile;
-        ti.end = range.end;
-        ++at;
-        if (++tile == range.tiles) {
-          tile = 0;
-          if (++head == heads) {
-            head = 0;
-            if (at < t1) {
-              do {
-                range = seq_range<S::kTile>(a, ++seq, kAlign);
-              } while (range.tiles == 0);
-            }
+      if (at < t1 && x < kPairCost) {
+        const int skip = (int)min((long long)(kPairCost - x), t1 - at);
+        x += skip;
+        at += skip;
+        if (at == t1) return ti;
+      }
+      if (at == t1) return ti;
+      ti.seq = seq;
+      ti.head = head;
+      ti.tile = x - kPairCost;
+      ti.tiles = range.tiles;
+      ti.token0 = range.begin + ti.tile * S::kTile;
+      ti.end = range.end;
+      ti.q0 = range.q0;
+      ti.q_len = range.q_len;
+      ti.left = (int)min((long long)(range.tiles - ti.tile), t1 - at);
+      ti.pair_at = at - x;
+      if (ti.tile == 0 || pair < 0) ++pair;
+      ti.pair = pair;
+      ++at;
+      if (++x == kPairCost + range.tiles) {
+        x = 0;
+        if (++head == heads) {
+          head = 0;
+          if (at < t1) {
+            do {
+              range = seq_range<S::kTile>(a, ++seq, kAlign);
+            } while (range.tiles == 0);
           }
         }
       }
@@ -344,13 +387,33 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
     TileInfo ti = next_tile(), ahead = next_tile();
     Pages pg = look(ti), pg_ahead = look(ahead);
     publish(0, ti, pg);
+    __syncthreads();  // the consumers see whether there is a tile at all
     int slot = 0, stage = 0;
     uint32_t phase = 1;  // a fresh stage is free
+    int pair_done = -1;  // last pair whose Q is on its way
     while (ti.seq >= 0) {
       // the next tile's description is there before this one's copies land
       slot = slot + 1 == S::kRing ? 0 : slot + 1;
       publish(slot, ahead, pg_ahead);
       mbar_wait(&sm.empty[stage], phase, a.status);
+      if (ti.pair != pair_done) {
+        // a pair's Q rows, two pairs in turn
+        pair_done = ti.pair;
+        const int buf = ti.pair & 1;
+        mbar_wait(&sm.q_empty[buf], (uint32_t)((ti.pair >> 1) & 1) ^ 1u, a.status);
+        const int rows = ti.q_len * p.groups;
+        for (int i = lane; i < S::kRows * (D / 8); i += 32) {
+          const int r = i / (D / 8), chunk = i % (D / 8);
+          const bool on = r < rows;
+          const uint16_t* src =
+              static_cast<const uint16_t*>(a.q) +
+              (on ? (long long)(ti.q0 + r / p.groups) * a.q_token_stride +
+                        (long long)(ti.head * p.groups + r % p.groups) * a.q_head_stride + chunk * 8
+                  : 0);
+          cp_async_16_zfill(&sm.q[buf][r][chunk * 8], src, on);
+        }
+        cp_async_arrive_noinc(&sm.q_full[buf]);
+      }
       uint8_t* ks = sm.stage[stage];
       if (TMA) {
         if (lane == 0) mbar_arrive_expect_tx(&sm.full[stage], S::kStageBytes);
@@ -422,7 +485,7 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
         phase ^= 1;
       }
     }
-    if (!TMA) asm volatile("cp.async.wait_all;" ::: "memory");
+    asm volatile("cp.async.wait_all;" ::: "memory");
     griddep_launch_dependents();
     return;
   }
@@ -450,75 +513,44 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
   float o[D / 16][NR][4];
   float m[NR][2], l[NR][2];   // rows 8 nr + 2c, + 1
   int v_exp = 1;              // e4m3: byte of the largest value scale so far
-  long long at = t0;
+  __syncthreads();  // the producer's first description
   int slot = 0, stage = 0;
   uint32_t phase = 0, next_kb = 0, next_vb = 0;
-  while (at < t1) {
-    // -- a (sequence, head) pair begins: its tiles of this block are
-    // [at, pair_end); u0, u1 bound the whole pair
-    mbar_wait(&sm.full[stage], phase, a.status);
+  if (sm.info[0].seq >= 0) scale_bytes(0, next_kb, next_vb);
+  while (sm.info[slot].seq >= 0) {
+    // -- a (sequence, head) pair begins
     const TileInfo first = sm.info[slot];
-    if (at == t0) scale_bytes(slot, next_kb, next_vb);
-    const SeqRange range = seq_range<S::kTile>(a, first.seq, kAlign);
-    const int head = first.head;
-    const long long u0 =
-        at - (first.token0 - range.begin) / S::kTile;
-    const long long u1 = u0 + range.tiles;
-    const long long pair_end = u1 < t1 ? u1 : t1;
-    const int q0 = __ldg(a.q_starts + first.seq);
-    const int rows = range.q_len * p.groups;
-
-    // Q rows to shared memory as the B operand's source
-    for (int r = warp; r < S::kRows; r += kWarps) {
-      constexpr int kPer = D / 32;  // consecutive columns per lane
-      float v[kPer];
-      float amax = 0.f;
-      const bool on = r < rows;
-      const uint16_t* src = static_cast<const uint16_t*>(a.q) +
-                            (long long)(q0 + (on ? r / p.groups : 0)) * a.q_token_stride +
-                            (long long)(head * p.groups + (on ? r % p.groups : 0)) * a.q_head_stride +
-                            lane * kPer;
-      uint16_t bits[kPer];
-#pragma unroll
-      for (int i = 0; i < kPer; i += 2) {
-        const uint32_t w = on ? __ldg(reinterpret_cast<const uint32_t*>(src + i)) : 0u;
-        bits[i] = (uint16_t)w;
-        bits[i + 1] = (uint16_t)(w >> 16);
-      }
-      float scale = 1.f;
-      if (KV == kE4m3 && !a.q_f16) {
+    const int head = first.head, q0 = first.q0;
+    const int rows = first.q_len * p.groups;
+    const int buf = first.pair & 1;
+    mbar_wait(&sm.q_full[buf], (uint32_t)(first.pair >> 1) & 1u, a.status);
+    if (KV == kE4m3 && !a.q_f16) {
+      // bf16 rows to f16, in place
+      for (int r = warp; r < S::kRows; r += kWarps) {
+        constexpr int kPer = D / 64;  // words of two columns per lane
+        uint32_t w[kPer], top = 0;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-          v[i] = __bfloat162float(__ushort_as_bfloat16(bits[i]));
-          amax = fmaxf(amax, fabsf(v[i]));
+          w[i] = *reinterpret_cast<const uint32_t*>(&sm.q[buf][r][2 * (lane + 32 * i)]);
+          top = __vmaxu2(top, w[i] & 0x7fff7fffu);
         }
+        top = max(top & 0xffffu, top >> 16);
 #pragma unroll
-        for (int s = 16; s > 0; s >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, s));
+        for (int s = 16; s > 0; s >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, s));
         // 2^-x brings the largest magnitude into [1, 2): exact in f16 down to
-        // 2^-24. An infinity stays one through any factor.
-        int x = (int)(__float_as_uint(amax) >> 23) - 127;
-        x = min(max(x, -126), 126);
-        scale = __uint_as_float((uint32_t)(127 + x) << 23);
+        // 2^-24. An infinity or NaN stays one through any factor.
+        const int x = min(max((int)(top >> 7) - 127, -126), 126);
         const float inv = __uint_as_float((uint32_t)(127 - x) << 23);
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) bits[i] = __half_as_ushort(__float2half_rn(v[i] * inv));
+        for (int i = 0; i < kPer; ++i) {
+          const __half2 h = __floats2half2_rn(__uint_as_float(w[i] << 16) * inv,
+                                              __uint_as_float(w[i] & 0xffff0000u) * inv);
+          *reinterpret_cast<__half2*>(&sm.q[buf][r][2 * (lane + 32 * i)]) = h;
+        }
+        if (lane == 0) sm.row_scale[r] = __uint_as_float((uint32_t)(127 + x) << 23);
       }
-#pragma unroll
-      for (int i = 0; i < kPer; i += 2)
-        *reinterpret_cast<uint32_t*>(&sm.q[r][lane * kPer + i]) =
-            bits[i] | (uint32_t)bits[i + 1] << 16;
-      if (lane == 0) {
-        sm.row_scale[r] = scale * p.scale_log2;
-        // tokens row r sees: [row_lo, row_hi)
-        const int pos = range.kv_len - range.q_len + r / p.groups;
-        int hi = a.causal ? min(range.end, pos + 1) : range.end;
-        int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-        if (!on) hi = 0;
-        sm.row_hi[r] = hi;
-        sm.row_lo[r] = lo;
-      }
+      sync_consumers();
     }
-    sync_consumers();
 
     // Q as B fragments: for k-step ks, register pair [ks][nr]. K's columns are
     // taken in the order the A operand finds them in memory.
@@ -526,7 +558,7 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
     constexpr bool kQInRegs = D * NR <= 256;
     uint32_t qf[kQInRegs ? kSteps : 1][NR][2];
     auto load_q = [&](int ks, int nr, uint32_t& b0, uint32_t& b1) {
-      const uint16_t* row = sm.q[8 * nr + g];
+      const uint16_t* row = sm.q[buf][8 * nr + g];
       if (KV != kE4m3) {
         b0 = *reinterpret_cast<const uint32_t*>(row + ks * 16 + 2 * c);
         b1 = *reinterpret_cast<const uint32_t*>(row + ks * 16 + 2 * c + 8);
@@ -551,9 +583,12 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
     for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        row_scale[nr][j] = sm.row_scale[8 * nr + 2 * c + j];
-        row_lo[nr][j] = sm.row_lo[8 * nr + 2 * c + j];
-        row_hi[nr][j] = sm.row_hi[8 * nr + 2 * c + j];
+        const int r = 8 * nr + 2 * c + j;
+        row_scale[nr][j] = p.scale_log2 * (KV == kE4m3 && !a.q_f16 ? sm.row_scale[r] : 1.f);
+        // tokens row r sees: [row_lo, row_hi)
+        const int pos = first.end - first.q_len + r / p.groups;
+        row_hi[nr][j] = r >= rows ? 0 : a.causal ? min(first.end, pos + 1) : first.end;
+        row_lo[nr][j] = a.window > 0 ? max(0, pos - a.window + 1) : 0;
         m[nr][j] = -INFINITY;
         raise_at[nr][j] = -INFINITY;
         l[nr][j] = 0.f;
@@ -575,17 +610,17 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[t][nr][j] = 0.f;
 
-    for (; at < pair_end; ++at) {
+    for (int left = first.left; left > 0; --left) {
       mbar_wait(&sm.full[stage], phase, a.status);
       const int token0 = sm.info[slot].token0 + warp * S::kTokens;
       const uint32_t kb_lane = next_kb, vb_lane = next_vb;
       const int first_row = warp * S::kTokens;
-      if (TMA && token0 + S::kTokens > range.end) {
+      if (TMA && token0 + S::kTokens > first.end) {
         // what a page holds past the last key may be NaN, and P zero times it
         // NaN again: those rows of V become zeros
         uint8_t* v = sm.stage[stage] + S::kHalfBytes;
         constexpr int kChunks = S::kRowBytes / 16;
-        for (int i = max(range.end - token0, 0) * kChunks + lane; i < S::kTokens * kChunks; i += 32)
+        for (int i = max(first.end - token0, 0) * kChunks + lane; i < S::kTokens * kChunks; i += 32)
           *reinterpret_cast<uint4*>(v + chunk_at<D, KV, true, TMA, S::kTile>(first_row + i / kChunks,
                                                                              i % kChunks)) =
               make_uint4(0u, 0u, 0u, 0u);
@@ -841,7 +876,7 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
       }
       // The pair's last stage is kept: the warps' results meet in it.
       __syncwarp();
-      if (lane == 0 && at + 1 < pair_end) mbar_arrive(&sm.empty[stage]);
+      if (lane == 0 && left > 1) mbar_arrive(&sm.empty[stage]);
       slot = slot + 1 == S::kRing ? 0 : slot + 1;
       if (++stage == S::kStages) {
         stage = 0;
@@ -872,12 +907,12 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
       sm.mx[tid] = mx;
       sm.sum[tid] = sum;
     }
-    const bool whole = u0 >= t0 && u1 <= t1;
-    const long long row_floats = D + 2;
+    const bool whole = first.left == first.tiles;
+    constexpr int row_floats = D + 4;  // m, l, -, -, O
     const long long slot_floats = (long long)S::kRows * row_floats;
     float* scratch = reinterpret_cast<float*>(a.scratch);
     // slot 0: a block that enters the pair from the one before; 1: the first
-    float* part = scratch + (2ll * blockIdx.x + (u0 >= t0 ? 1 : 0)) * slot_floats;
+    float* part = scratch + (2ll * blockIdx.x + (first.tile == 0 ? 1 : 0)) * slot_floats;
     const int last_stage = stage == 0 ? S::kStages - 1 : stage - 1;
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr) {
@@ -922,7 +957,7 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
                                         d] =
               a.q_f16 ? __half_as_ushort(__float2half_rn(x)) : __bfloat16_as_ushort(__float2bfloat16_rn(x));
         } else {
-          part[r * row_floats + 2 + d] = v;
+          part[r * row_floats + 4 + d] = v;
         }
       }
     }
@@ -938,7 +973,8 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 
     if (!whole) {
-      // Blocks of the pair: c_first holds its first tile, c_last its last one.
+      // The blocks that hold the pair's first and last tile.
+      const long long u0 = first.pair_at + kPairCost, u1 = u0 + first.tiles;
       const int c_first = (int)(((u0 + 1) * ctas - 1) / total);
       const int c_last = (int)((u1 * ctas - 1) / total);
       __threadfence();
@@ -951,8 +987,9 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
       }
       sync_consumers();
       if (sm.flag) {
-        // The parts' maximum, a warp per row; then their weighted sum, a thread
-        // per two columns and row at a time, eight parts in flight.
+        // The parts' maximum, a warp per row; then each warp its share of the
+        // parts, a row's columns over the lanes and four rows in flight; then
+        // the warps' sums, through the stage again.
         auto part_at = [&](int b) {
           return scratch + (2ll * b + (b == c_first ? 1 : 0)) * slot_floats;
         };
@@ -965,48 +1002,79 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
           if (lane == 0) sm.mx[r] = mx;
         }
         sync_consumers();
-        for (int i = tid; i < rows * (D / 2); i += kConsumers) {
-          const int r = i / (D / 2), d = 2 * (i % (D / 2));
-          const float mx = sm.mx[r];
-          float sum = 0.f, x = 0.f, y = 0.f;
-          for (int b0 = c_first; b0 <= c_last; b0 += 8) {
-            float2 ml[8], v[8];
+        constexpr int kCols = D / 32;  // columns per lane: two, four or eight
+        float* sums = reinterpret_cast<float*>(sm.stage[last_stage]) + warp * 8 * D;
+        for (int r0 = 0; r0 < rows; r0 += 4) {
+          float acc[4][kCols], l_sum[4];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const float* src = part_at(min(b0 + j, c_last)) + r * row_floats;
-              ml[j] = __ldcg(reinterpret_cast<const float2*>(src));
-              v[j] = __ldcg(reinterpret_cast<const float2*>(src + 2 + d));
+          for (int i = 0; i < 4; ++i) {
+            l_sum[i] = 0.f;
+#pragma unroll
+            for (int k = 0; k < kCols; ++k) acc[i][k] = 0.f;
+          }
+          for (int b = c_first + warp; b <= c_last; b += kWarps) {
+            const float* src = part_at(b);
+            float2 ml[4];
+            float v[4][kCols];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float* row = src + min(r0 + i, rows - 1) * row_floats;
+              ml[i] = __ldcg(reinterpret_cast<const float2*>(row));
+#pragma unroll
+              for (int k = 0; k < kCols; k += 2) {
+                const float2 t = __ldcg(reinterpret_cast<const float2*>(row + 4 + 32 * k + 2 * lane));
+                v[i][k] = t.x;
+                v[i][k + 1] = t.y;
+              }
             }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
+            for (int i = 0; i < 4; ++i) {
               // (a part without a visible key has m = -inf and l = 0, or NaN)
-              float w = ml[j].x == -INFINITY ? (ml[j].y == 0.f ? 0.f : 1.f) : exp2_fast(ml[j].x - mx);
-              if (b0 + j > c_last) w = 0.f;
-              sum += w == 0.f ? 0.f : ml[j].y * w;
-              x += w == 0.f ? 0.f : v[j].x * w;
-              y += w == 0.f ? 0.f : v[j].y * w;
+              const float mx = sm.mx[min(r0 + i, rows - 1)];
+              const float w = ml[i].x == -INFINITY ? (ml[i].y == 0.f ? 0.f : 1.f)
+                                                   : exp2_fast(ml[i].x - mx);
+              l_sum[i] += w == 0.f ? 0.f : ml[i].y * w;
+#pragma unroll
+              for (int k = 0; k < kCols; ++k) acc[i][k] += w == 0.f ? 0.f : v[i][k] * w;
             }
           }
-          const float inv = sum == 0.f ? 0.f : 1.f / sum;
-          const long long tok = q0 + r / p.groups;
-          const int qh = head * p.groups + r % p.groups;
-          uint32_t pk;
-          if (a.q_f16) {
-            const __half2 b = __floats2half2_rn(x * inv, y * inv);
-            pk = *reinterpret_cast<const uint32_t*>(&b);
-          } else {
-            const __nv_bfloat162 b = __floats2bfloat162_rn(x * inv, y * inv);
-            pk = *reinterpret_cast<const uint32_t*>(&b);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (lane == 0) sm.wl[warp][min(r0 + i, S::kRows - 1)] = l_sum[i];
+#pragma unroll
+            for (int k = 0; k < kCols; k += 2)
+              *reinterpret_cast<float2*>(sums + i * D + 32 * k + 2 * lane) =
+                  make_float2(acc[i][k], acc[i][k + 1]);
           }
-          *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + tok * a.out_token_stride +
-                                       qh * a.out_head_stride + d) = pk;
-          if (a.lse != nullptr && d == 0)
-            a.lse[tok * a.q_heads + qh] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) / kLog2e;
+          sync_consumers();
+          for (int i = tid; i < 4 * D; i += kConsumers) {
+            const int r = r0 + i / D, d = i % D;
+            if (r >= rows) break;
+            float v = 0.f, sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+              v += reinterpret_cast<const float*>(sm.stage[last_stage])[w * 8 * D + (i / D) * D + d];
+              sum += sm.wl[w][r];
+            }
+            const float x = sum == 0.f ? 0.f : v / sum;
+            const long long tok = q0 + r / p.groups;
+            const int qh = head * p.groups + r % p.groups;
+            static_cast<uint16_t*>(a.out)[tok * a.out_token_stride + qh * a.out_head_stride + d] =
+                a.q_f16 ? __half_as_ushort(__float2half_rn(x)) : __bfloat16_as_ushort(__float2bfloat16_rn(x));
+            if (a.lse != nullptr && d == 0)
+              a.lse[tok * a.q_heads + qh] =
+                  sum == 0.f ? -INFINITY : (sm.mx[r] + log2f(sum)) / kLog2e;
+          }
+          sync_consumers();
         }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
     }
     sync_consumers();
-    if (lane == 0) mbar_arrive(&sm.empty[last_stage]);
+    if (lane == 0) {
+      mbar_arrive(&sm.empty[last_stage]);
+      mbar_arrive(&sm.q_empty[buf]);
+    }
   }
   griddep_launch_dependents();
 }
@@ -1063,7 +1131,7 @@ int attn_decode_rows() { return 16; }
 int attn_max_ctas() { return kMaxCtas; }
 
 long long attn_decode_scratch_bytes(int head_dim) {
-  return 2ll * 2 * device_sm_count() * 16 * (head_dim + 2) * 4;
+  return 2ll * 2 * device_sm_count() * 16 * (head_dim + 4) * 4;
 }
 
 cudaError_t launch_attn_decode(const AttnLaunch& l, cudaStream_t stream) {
