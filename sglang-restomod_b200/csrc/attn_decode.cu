@@ -49,7 +49,7 @@ constexpr int kMaxCtas = 1024;      // arrival counters in the workspace
 // A block takes at least this much work, in tiles: below it the pair's merge
 // costs more than the extra blocks bring. And a pair is cut into at most
 // kMaxParts, whose sum one block takes.
-constexpr int kMinTiles = 4;
+constexpr int kMinTiles = 2;
 constexpr int kMaxParts = 64;
 // What a (sequence, head) pair costs besides its tiles, in tiles of about 100
 // tokens (1 us): its start and the warps' meeting. Cutting by tiles alone left
@@ -87,20 +87,21 @@ struct Shape {
   static constexpr int kRowBytes = D * kElem;
   // A consumer warp takes 16 tokens of a tile. Its instructions wait on one
   // another (products, softmax, products), so as many warps share an SM as
-  // registers allow where a step is mostly conversions: 16 with the producers
-  // for e4m3 and head_dim 64 (128 registers a thread). 16-bit vectors of 128
-  // and 256 need no conversion and keep up with 7 and 4.
+  // registers and stages allow: 16 with the producers for e4m3 and head_dim 64
+  // (128 registers a thread), 8 and 7 for 16-bit vectors of 128 and 256, whose
+  // stages are large (16 sequences of up to 32768 tokens, head_dim 256, bf16:
+  // 144, 120, 108, 98 us with 2, 3, 4, 6 consumer warps).
   static constexpr int kTokens = 16;
-  static constexpr int kWarps = D == 256 ? (KV == kE4m3 ? 7 : 4) : 7;
+  static constexpr int kWarps = D == 256 && KV != kE4m3 ? 6 : 7;
   static constexpr int kConsumers = kWarps * 32;
   static constexpr int kThreads = kConsumers + 32;
   static constexpr int kTile = kTokens * kWarps;            // tokens per step
   static constexpr int kHalfBytes = kTile * kRowBytes;      // K, or V, of a stage
   static constexpr int kStageBytes = 2 * kHalfBytes;
   static constexpr int kRows = 8 * NR;
-  // Ring: 70 to 84 KB per block and two blocks per SM, or 112 to 192 KB and one.
+  // Ring: 70 to 84 KB per block and two blocks per SM, or 168 to 192 KB and one.
   static constexpr int kBlocks = D == 64 || (D == 128 && KV == kE4m3) ? 2 : 1;
-  static constexpr int kStages = KV == kE4m3 && D == 64 ? 5 : 3;
+  static constexpr int kStages = D == 256 && KV != kE4m3 ? 2 : KV == kE4m3 && D == 64 ? 5 : 3;
   static constexpr int kRing = kStages + 2;  // tile descriptions
   static constexpr int kQPitch = D + 8;      // 16-bit elements, conflict-free rows
   struct Smem {

@@ -79,6 +79,11 @@ struct PrefillParams {
   // tensor copies: rows of a page that one copy takes (a power of two that
   // divides the page size), and whether heads come before tokens in the map
   int box_rows, heads_first;
+  int page_shift;  // log2 of the page size, -1 where it is no power of two
+
+  __device__ int page_of(int token) const {
+    return page_shift >= 0 ? token >> page_shift : token / a.c.page_size;
+  }
 };
 
 constexpr int kProducers = 256;
@@ -896,7 +901,7 @@ __global__ void __launch_bounds__(Shape<D, MT, TMA>::kThreads, 1)
     auto page_of = [&](const Segment& sg, int kv_len, int t) -> int {
       const int token = sg.begin + (sg.tile0 + t) * BN + lane * p.box_rows;
       if (t >= sg.tiles || lane >= boxes || token >= kv_len) return -2;
-      return __ldg(a.table + sg.seq * a.table_stride + token / a.c.page_size);
+      return __ldg(a.table + sg.seq * a.table_stride + p.page_of(token));
     };
     bool more = cur.next(g);
     SeqLens q = seq_lens(a, g.seq);
@@ -914,7 +919,7 @@ __global__ void __launch_bounds__(Shape<D, MT, TMA>::kThreads, 1)
         __syncwarp();
         if (lane < boxes) {
           const int token = g.begin + (g.tile0 + t) * BN + lane * p.box_rows;
-          int at = token % a.c.page_size;
+          int at = token - p.page_of(token) * a.c.page_size;
           if (pg < 0 || pg >= a.c.num_pages) {
             if (token < q.kv_len) atomicOr(a.status, kDevBadPage);
             pg = (int)a.c.num_pages;
@@ -985,7 +990,7 @@ __global__ void __launch_bounds__(Shape<D, MT, TMA>::kThreads, 1)
     auto page_of = [&](const Segment& sg, int kv_len, int t) -> int {
       const int token = sg.begin + (sg.tile0 + t) * BN + pt;
       return t < sg.tiles && pt < BN && token < kv_len
-                 ? __ldg(a.table + sg.seq * a.table_stride + token / a.c.page_size)
+                 ? __ldg(a.table + sg.seq * a.table_stride + p.page_of(token))
                  : -1;
     };
     auto info_of = [&](const Segment& sg, int kv_len, int t, int page) {
@@ -997,7 +1002,7 @@ __global__ void __launch_bounds__(Shape<D, MT, TMA>::kThreads, 1)
         if (page < 0 || page >= a.c.num_pages) {
           atomicOr(a.status, kDevBadPage);
         } else {
-          const int at = token % a.c.page_size;
+          const int at = token - p.page_of(token) * a.c.page_size;
           r.off = (page * a.c.page_stride + at * a.c.token_stride + sg.head * a.c.head_stride) *
                   kElem;
           if (kQuant) {
@@ -1379,6 +1384,7 @@ cudaError_t launch_attn_prefill(const AttnLaunch& l, cudaStream_t stream) {
   p.tile_tokens = 128 / p.groups;
   p.scale_log2 = l.scale * kLog2e;
   p.box_rows = 1;
+  p.page_shift = (l.c.page_size & (l.c.page_size - 1)) == 0 ? __builtin_ctz(l.c.page_size) : -1;
   const long long sms = device_sm_count();
   p.max_units = (int)max_units(l.q_tokens, l.seqs, 1);
   uint8_t* at = l.scratch;
