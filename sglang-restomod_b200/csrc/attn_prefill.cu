@@ -329,6 +329,7 @@ __device__ __forceinline__ SeqLens seq_lens(const AttnLaunch& a, int s) {
 }
 
 constexpr int kPlanThreads = 1024;
+constexpr int kPlanSeqs = 4095;  // sequences whose unit counts fit shared memory
 
 __device__ long long block_scan(long long v, long long* sh, long long& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -364,6 +365,9 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const PrefillPa
                                                                  int max_ctas) {
   // (with tensor copies a unit's first key is moved down to a copy's border)
   __shared__ long long sh[32];
+  __shared__ int base_sh[kPlanSeqs + 1];
+  // (each step of the search below reads it: from global memory 1 us a step)
+  int* seq_base = p.a.seqs <= kPlanSeqs ? base_sh : p.seq_base;
   griddep_wait();
   const AttnLaunch& a = p.a;
   const int tid = threadIdx.x;
@@ -375,10 +379,10 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const PrefillPa
     for (int s = s0; s < s1; ++s) n += (seq_lens(a, s).q_len + unit_tokens - 1) / unit_tokens;
     long long base = block_scan(n, sh, total_units);
     for (int s = s0; s < s1; ++s) {
-      p.seq_base[s] = (int)base;
+      seq_base[s] = (int)base;
       base += (seq_lens(a, s).q_len + unit_tokens - 1) / unit_tokens;
     }
-    if (tid == 0) p.seq_base[a.seqs] = (int)total_units;
+    if (tid == 0) seq_base[a.seqs] = (int)total_units;
   }
   __syncthreads();
   // q_starts that ascend within q_tokens give at most max_units.
@@ -386,11 +390,12 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const PrefillPa
   const int per = (units + kPlanThreads - 1) / kPlanThreads;
   const int u0 = min(tid * per, units), u1 = min(u0 + per, units);
   long long mine = 0;
+  int first_tiles = 0;  // of unit u0: most threads have one unit at most
   if (u0 < u1) {
     int lo = 0, hi = a.seqs - 1;  // last sequence whose base is <= u0
     while (lo < hi) {
       const int mid = (lo + hi + 1) / 2;
-      if (p.seq_base[mid] <= u0)
+      if (seq_base[mid] <= u0)
         lo = mid;
       else
         hi = mid - 1;
@@ -398,8 +403,8 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const PrefillPa
     int s = lo;
     SeqLens q = seq_lens(a, s);
     for (int u = u0; u < u1; ++u) {
-      while (s + 1 < a.seqs && p.seq_base[s + 1] <= u) q = seq_lens(a, ++s);
-      const int tok0 = (u - p.seq_base[s]) * unit_tokens;
+      while (s + 1 < a.seqs && seq_base[s + 1] <= u) q = seq_lens(a, ++s);
+      const int tok0 = (u - seq_base[s]) * unit_tokens;
       const int last = min(tok0 + unit_tokens, q.q_len) - 1;
       const int shift = q.kv_len - q.q_len;
       int end = a.causal ? min(q.kv_len, shift + last + 1) : q.kv_len;
@@ -407,6 +412,7 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const PrefillPa
       begin -= begin % p.box_rows;
       const int tiles = end > begin ? (end - begin + bn - 1) / bn : 1;
       p.units[u] = make_int4(s, tok0, begin, tiles);
+      if (u == u0) first_tiles = tiles;
       mine += (long long)(tiles + kUnitCost) * a.c.heads;
     }
   }
@@ -418,7 +424,7 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const PrefillPa
     p.head[1] = ctas;
   }
   for (int u = u0; u < u1; ++u) {
-    const int cost = p.units[u].w + kUnitCost;
+    const int cost = (u == u0 ? first_tiles : p.units[u].w) + kUnitCost;
     const long long n = (long long)cost * a.c.heads;
     // blocks whose first tile floor(total * c / ctas) lies in [at, at + n)
     for (long long c = (at * ctas + total - 1) / total; c < ctas; ++c) {
