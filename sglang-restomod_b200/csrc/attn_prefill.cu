@@ -22,9 +22,11 @@
 //             operands' 128-byte-swizzled layout, 16 bytes per copy. Plain
 //             cp.async rather than tensor copies, since a page may be of any
 //             size down to one token and rows past the end have to be zero;
-//             e4m3 codes are converted on the way (times their power of two:
-//             exact in bf16; in f16 exact but for values below its smallest
-//             subnormal step)
+//             e4m3 codes are converted on the way, to f16 for every model type
+//             (two instructions a pair where bf16 took five): a code times its
+//             power of two is exact in f16 but for what lies below its smallest
+//             subnormal step, 2^-9 of a vector's largest value at worst; bf16
+//             queries are brought to f16 by a power of two per row
 //   relay     one thread: passes each tile that has landed on to the tensor
 //             core's reads (a proxy fence, off the mma thread's path)
 //   mma       one thread: S = Q K^T into one of two S buffers, O += P V
@@ -62,7 +64,7 @@ constexpr int kUnitCost = 2;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kTmemO = 256;  // O after the two S buffers of up to 128 columns
 
-enum { kBf16 = 0, kF16 = 1, kE4m3Bf16 = 2, kE4m3F16 = 3 };
+enum { kBf16 = 0, kF16 = 1, kE4m3 = 2 };
 
 struct PrefillParams {
   AttnLaunch a;
@@ -98,7 +100,7 @@ struct Shape {
   static constexpr int kTileBytes = kSlices * kKvSlice;
   static constexpr int kTableBytes = TMA ? 0 : 4 * kBN * (16 + 8);
   static constexpr int kOutBytes = MT * 4 * 2048;   // 32 rows x 32 columns per warp
-  static constexpr int kFixed = kQBytes + kTableBytes + kOutBytes + 2048 + 1024;
+  static constexpr int kFixed = kQBytes + kTableBytes + kOutBytes + 4096 + 1024;
   static constexpr int kFit = (227 * 1024 - kFixed) / kTileBytes;
   static constexpr int kStages = kFit > 8 ? 8 : kFit;
   static constexpr int kLoaders = TMA ? 32 : kProducers;
@@ -126,9 +128,11 @@ struct Ctl {
   uint64_t q_landed, q_full, q_empty;
   uint64_t s_full[2], p_ready[2], pv_done[2];
   uint64_t drained;
+  uint64_t q_scaled[2];  // e4m3: q_scale of even and odd segments is written
   uint32_t tmem;
   int abort;
   int flag[2];
+  float q_scale[2][2][128];  // e4m3: of Q's rows; segment parity, tile, row
 };
 
 // One try with a suspension hint: the waiting warps of a block are many, and
@@ -276,36 +280,15 @@ __device__ __forceinline__ void st_shared_u128(uint32_t dst, uint4 v) {
                : "memory");
 }
 
-// Four e4m3 codes times a 16-bit power of two (two copies in `factor`).
-// bf16: a code's bits moved to bf16's exponent and mantissa fields read 2^-120
-// of its value (subnormals included); the factor holds 2^(120 + e).
-template <bool F16>
+// Four e4m3 codes times an f16 power of two (two copies in `factor`).
 __device__ __forceinline__ uint2 convert4(uint32_t w, uint32_t factor) {
-  uint2 r;
-  if (F16) {
-    r.x = hmul2_u32(e4m3x2_to_f16x2((uint16_t)w), factor);
-    r.y = hmul2_u32(e4m3x2_to_f16x2((uint16_t)(w >> 16)), factor);
-  } else {
-    const uint32_t lo = __byte_perm(w, 0, 0x1404), hi = __byte_perm(w, 0, 0x3424);
-    const uint32_t a = (lo & 0x80008000u) | ((lo >> 4) & 0x07f007f0u);
-    const uint32_t b = (hi & 0x80008000u) | ((hi >> 4) & 0x07f007f0u);
-    const __nv_bfloat162 f = *reinterpret_cast<const __nv_bfloat162*>(&factor);
-    const __nv_bfloat162 x = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), f);
-    const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&b), f);
-    r.x = *reinterpret_cast<const uint32_t*>(&x);
-    r.y = *reinterpret_cast<const uint32_t*>(&y);
-  }
-  return r;
+  return make_uint2(hmul2_u32(e4m3x2_to_f16x2((uint16_t)w), factor),
+                    hmul2_u32(e4m3x2_to_f16x2((uint16_t)(w >> 16)), factor));
 }
 // The factor of a scale byte (127 + e), for convert4.
-template <bool F16>
 __device__ __forceinline__ uint32_t factor_of(uint32_t byte) {
-  uint32_t h;
-  if (F16)
-    h = byte == 255u ? 0x7e00u
-                     : __half_as_ushort(__float2half_rn(__uint_as_float(byte << 23)));
-  else  // bf16 exponent field 127 + 120 + e, at most 254
-    h = byte == 255u ? 0x7fc0u : min(byte + 120u, 254u) << 7;
+  const uint32_t h =
+      byte == 255u ? 0x7e00u : __half_as_ushort(__float2half_rn(__uint_as_float(byte << 23)));
   return h | h << 16;
 }
 
@@ -649,8 +632,8 @@ __global__ void __launch_bounds__(Shape<D, MT, TMA>::kThreads, 1)
                         const __grid_constant__ CUtensorMap v_map) {
   using S = Shape<D, MT, TMA>;
   constexpr int BN = S::kBN;
-  constexpr bool kHalf = KV == kF16 || KV == kE4m3F16;  // operand type f16
-  constexpr bool kQuant = KV >= kE4m3Bf16;
+  constexpr bool kHalf = KV != kBf16;  // operand type f16
+  constexpr bool kQuant = KV == kE4m3;
   constexpr int kProducer = MT * 4, kMma = kProducer + S::kLoaders / 32, kRelay = kMma + 1;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
@@ -672,6 +655,7 @@ __global__ void __launch_bounds__(Shape<D, MT, TMA>::kThreads, 1)
     mbar_init(&ctl->q_full, 1);
     mbar_init(&ctl->q_empty, 1);
     mbar_init(&ctl->drained, 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&ctl->q_scaled[i], kProducers);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&ctl->s_full[i], 1);
       mbar_init(&ctl->p_ready[i], 128);
@@ -708,6 +692,7 @@ __global__ void __launch_bounds__(Shape<D, MT, TMA>::kThreads, 1)
     const uint32_t lane_addr = tmem + ((uint32_t)(warp & 3) << 21);
     const int row_token = row / p.groups, row_head = row % p.groups;
     uint32_t step = 0;                              // S tiles of this warpgroup so far
+    uint32_t segment = 0;                           // segments so far
     uint64_t* pv_done = &ctl->pv_done[MT == 2 ? wg : 0];  // one phase per step
     while (cur.next(g)) {
       const SeqLens q = seq_lens(a, g.seq);
@@ -719,6 +704,16 @@ __global__ void __launch_bounds__(Shape<D, MT, TMA>::kThreads, 1)
       const int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
       // a row that sees nothing needs no maximum: every key is masked
       float m = hi > lo ? -INFINITY : 0.f, l = 0.f;
+      float scale = p.scale_log2;
+      if (kQuant && !a.q_f16) {
+        // (Q of the segment after next waits for this one's products, so the
+        // barrier is never two phases on)
+        if ((warp & 3) == 0)
+          wait_bar(&ctl->q_scaled[segment & 1u], segment >> 1 & 1u, ctl, a.status);
+        named_bar_sync(2 + wg, 128);
+        scale *= ctl->q_scale[segment & 1u][wg][row];
+      }
+      ++segment;
       const uint32_t to = lane_addr + kTmemO + (MT == 2 ? wg * D : 0);
       for (int k = 0; k < g.tiles; ++k, ++step) {
         const int buf = MT == 2 ? wg : (int)(step & 1u);
@@ -733,15 +728,15 @@ __global__ void __launch_bounds__(Shape<D, MT, TMA>::kThreads, 1)
         uint32_t s[TMA ? BN : 32];  // TMA: the row's S, read once
         if constexpr (TMA) {
           load_row<BN>(ts, s);
-          if (masked) mask_row<BN>(s, col0, lo, hi, p.scale_log2 >= 0.f ? -INFINITY : INFINITY);
-          top = p.scale_log2 >= 0.f ? max_row<BN, false>(s) : max_row<BN, true>(s);
-        } else if (p.scale_log2 >= 0.f)
+          if (masked) mask_row<BN>(s, col0, lo, hi, scale >= 0.f ? -INFINITY : INFINITY);
+          top = scale >= 0.f ? max_row<BN, false>(s) : max_row<BN, true>(s);
+        } else if (scale >= 0.f)
           top = masked ? max_pass<BN, true, false>(ts, col0, lo, hi)
                        : max_pass<BN, false, false>(ts, col0, lo, hi);
         else
           top = max_pass<BN, true, true>(ts, col0, lo, hi);
         // (a scale of zero makes every visible score zero)
-        top = top == -INFINITY ? top : top * fabsf(p.scale_log2);
+        top = top == -INFINITY ? top : top * fabsf(scale);
         const float mn = m == -INFINITY || top > m + kLazy ? top : m;
         const float f = m == mn || m == -INFINITY ? 1.f : ex2(m - mn);
         if (k > 0 && __any_sync(0xffffffffu, f != 1.f)) {
@@ -764,10 +759,10 @@ __global__ void __launch_bounds__(Shape<D, MT, TMA>::kThreads, 1)
         m = mn;
         const float base = m == -INFINITY ? 0.f : m;
         if constexpr (TMA)
-          l += exp_row<BN, kHalf>(ts, s, p.scale_log2, base);
+          l += exp_row<BN, kHalf>(ts, s, scale, base);
         else
-          l += masked ? exp_pass<BN, kHalf, true>(ts, p.scale_log2, base, col0, lo, hi)
-                      : exp_pass<BN, kHalf, false>(ts, p.scale_log2, base, col0, lo, hi);
+          l += masked ? exp_pass<BN, kHalf, true>(ts, scale, base, col0, lo, hi)
+                      : exp_pass<BN, kHalf, false>(ts, scale, base, col0, lo, hi);
         tmem_st_wait();
         // Solo: the S that was waited for came before the previous product, so
         // that product is waited for here; no wait is then ever two phases
@@ -1029,8 +1024,8 @@ __global__ void __launch_bounds__(Shape<D, MT, TMA>::kThreads, 1)
       table[(t & 3) * BN + pt] = row;
       if (kQuant) {
         RowFactor f;
-        f.k = factor_of<kHalf>(r.k_byte);
-        f.v = factor_of<kHalf>(r.v_byte);
+        f.k = factor_of(r.k_byte);
+        f.v = factor_of(r.v_byte);
         factors[(t & 3) * BN + pt] = f;
       }
     };
@@ -1113,8 +1108,8 @@ __global__ void __launch_bounds__(Shape<D, MT, TMA>::kThreads, 1)
           for (int i = 0; i < (kQuant ? kPer : 1); ++i) {
             const RowFactor& rf = fs[p_row + i * kRowStep];
             const uint32_t f = is_v ? rf.v : rf.k;
-            const uint2 x = convert4<kHalf>(codes[i].x, f), y = convert4<kHalf>(codes[i].y, f);
-            const uint2 z = convert4<kHalf>(codes[i].z, f), w = convert4<kHalf>(codes[i].w, f);
+            const uint2 x = convert4(codes[i].x, f), y = convert4(codes[i].y, f);
+            const uint2 z = convert4(codes[i].z, f), w = convert4(codes[i].w, f);
             st_shared_u128(dst + i * kRowStep * 128 + x0, make_uint4(x.x, x.y, y.x, y.y));
             st_shared_u128(dst + i * kRowStep * 128 + x1, make_uint4(z.x, z.y, w.x, w.y));
           }
@@ -1137,6 +1132,7 @@ __global__ void __launch_bounds__(Shape<D, MT, TMA>::kThreads, 1)
           ++q_count;
           constexpr int kQChunks = D / 8;
           const int chunk = pt % kQChunks;
+          const bool to_f16 = kQuant && !a.q_f16;
 #pragma unroll 4
           for (int r = pt / kQChunks; r < MT * 128; r += kProducers / kQChunks) {
             const int tile = r >> 7, rr = r & 127;
@@ -1148,11 +1144,38 @@ __global__ void __launch_bounds__(Shape<D, MT, TMA>::kThreads, 1)
                              (long long)(g.head * p.groups + rr % p.groups) * a.q_head_stride +
                              chunk * 8) * 2
                       : zeros + chunk * 16;
-            cp_async_16_at(sq + (tile * S::kSlices + chunk / 8) * S::kQSlice + rr * 128 +
-                               (((chunk & 7) ^ (rr & 7)) << 4),
-                           src);
+            const uint32_t dst = sq + (tile * S::kSlices + chunk / 8) * S::kQSlice + rr * 128 +
+                                 (((chunk & 7) ^ (rr & 7)) << 4);
+            if (!to_f16) {
+              cp_async_16_at(dst, src);
+              continue;
+            }
+            // bf16 to f16: 2^-x brings the row's largest magnitude into [1, 2),
+            // exact in f16 down to 2^-24; infinities and NaN stay
+            const uint4 raw = __ldg(reinterpret_cast<const uint4*>(src));
+            const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+            uint32_t top = 0, o[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = __vmaxu2(top, w[i] & 0x7fff7fffu);
+            top = max(top & 0xffffu, top >> 16);
+#pragma unroll
+            for (int x = kQChunks / 2; x > 0; x >>= 1)
+              top = max(top, __shfl_xor_sync(0xffffffffu, top, x));
+            const int x = min(max((int)(top >> 7) - 127, -126), 126);
+            const float inv = __uint_as_float((uint32_t)(127 - x) << 23);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              o[i] = pack2<true>(__uint_as_float(w[i] << 16) * inv,
+                                 __uint_as_float(w[i] & 0xffff0000u) * inv);
+            st_shared_u128(dst, make_uint4(o[0], o[1], o[2], o[3]));
+            if (chunk == 0)
+              ctl->q_scale[(q_count ^ 1u) & 1u][tile][rr] = __uint_as_float((uint32_t)(127 + x) << 23);
           }
-          cp_async_arrive_noinc(&ctl->q_landed);
+          if (to_f16) {
+            mbar_arrive(&ctl->q_scaled[(q_count ^ 1u) & 1u]);
+            mbar_arrive(&ctl->q_landed);
+          } else
+            cp_async_arrive_noinc(&ctl->q_landed);
         }
         store_info(t + 2, next);
         fill_entry(2 * t + 1);
@@ -1326,7 +1349,7 @@ cudaError_t launch(const PrefillParams& p, const CUtensorMap (&maps)[3], cudaStr
     configured[dev] = true;
   }
   static_assert(S::kSmem <= 227 * 1024 && S::kStages >= 4, "shared memory");
-  static_assert(sizeof(Ctl) <= 2048, "control block");
+  static_assert(sizeof(Ctl) <= 4096, "control block");
   const int sms = device_sm_count();
   err = launch_pdl(attn_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, p,
                    MT * p.tile_tokens, S::kBN, sms);
@@ -1364,8 +1387,7 @@ template <int D, int MT>
 cudaError_t launch_type(PrefillParams& p, cudaStream_t stream) {
   CUtensorMap maps[3] = {};
   if (p.a.cache_dtype == 3)
-    return p.a.q_f16 ? launch<D, MT, kE4m3F16, false>(p, maps, stream)
-                     : launch<D, MT, kE4m3Bf16, false>(p, maps, stream);
+    return launch<D, MT, kE4m3, false>(p, maps, stream);
   if (make_maps(p, Shape<D, MT, true>::kBN, maps))
     return p.a.q_f16 ? launch<D, MT, kF16, true>(p, maps, stream)
                      : launch<D, MT, kBf16, true>(p, maps, stream);
