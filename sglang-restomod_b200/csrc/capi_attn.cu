@@ -30,6 +30,16 @@ int check_cuda(cudaError_t err, const char* what) {
 bool aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 bool valid_dtype16(int32_t d) { return d == B200_DTYPE_BF16 || d == B200_DTYPE_F16; }
 
+// Vectors that are written must not share memory: with both strides at least a
+// vector, either order of tokens and heads, and only extents above one count.
+bool apart(int64_t token_stride, int64_t tokens, int64_t head_stride, int64_t heads, int64_t dim) {
+  if (tokens <= 1) return heads <= 1 || head_stride >= dim;
+  if (heads <= 1) return token_stride >= dim;
+  return head_stride <= token_stride
+             ? head_stride >= dim && token_stride >= (heads - 1) * head_stride + dim
+             : token_stride >= dim && head_stride >= (tokens - 1) * token_stride + dim;
+}
+
 // The cache's description, checked and in the kernels' form.
 int cache_view(const b200_kv_cache* c, KvCacheView& v) {
   if (c == nullptr || c->k == nullptr || c->v == nullptr)
@@ -178,6 +188,8 @@ int b200_kv_cache_read(const b200_kv_cache* cache, const int64_t* slots, int64_t
   if (rc || tokens == 0) return rc;
   if ((rc = check_rows("k", k, token_stride, head_stride))) return rc;
   if ((rc = check_rows("v", v, token_stride, head_stride))) return rc;
+  if (!apart(token_stride, tokens, head_stride, c.heads, c.head_dim))
+    return fail(B200_ERR_INVALID, "the output's vectors overlap");
   return check_cuda(launch_kv_read(c, k, v, dtype == B200_DTYPE_F16, token_stride, head_stride,
                                    reinterpret_cast<const long long*>(slots), tokens,
                                    reinterpret_cast<cudaStream_t>(stream)),
@@ -218,6 +230,8 @@ int b200_paged_attention(const b200_kv_cache* cache, const void* q, int32_t dtyp
   if (seqs == 0 || q_tokens == 0 || max_q_len == 0) return B200_OK;
   if ((rc = check_rows("q", q, q_token_stride, q_head_stride))) return rc;
   if ((rc = check_rows("out", out, out_token_stride, out_head_stride))) return rc;
+  if (!apart(out_token_stride, q_tokens, out_head_stride, q_heads, l.c.head_dim))
+    return fail(B200_ERR_INVALID, "the output's vectors overlap");
   if (kv_lens == nullptr || q_starts == nullptr || (page_table_width > 0 && page_table == nullptr))
     return fail(B200_ERR_INVALID, "null pointer argument");
   if (!aligned(page_table, 4) || !aligned(kv_lens, 4) || !aligned(q_starts, 4) || !aligned(lse, 4))

@@ -717,6 +717,9 @@ def w8a8_linear_quantized(q: torch.Tensor, scales: torch.Tensor, w: torch.Tensor
     cols = n // 2 if gated_mode == _lib.GATED_FUSED else n
     if out is None:
         out = torch.empty(m, cols, dtype=out_dtype, device=q.device)
+    elif out.shape != (m, cols) or not out.is_contiguous() or out.device != q.device:
+        raise ValueError(f"out must be a contiguous [{m}, {cols}] on {q.device}, got "
+                         f"{tuple(out.shape)} on {out.device}")
     ws = workspace(gemm_workspace_bytes(0), q.device)
     _lib.check(
         lib().b200_w8a8_linear_quantized(
@@ -865,8 +868,8 @@ def kv_cache_read(cache, slots: torch.Tensor, dtype: torch.dtype | None = None):
     if code is None:
         raise TypeError(f"dtype must be bf16 or f16, got {dtype}")
     n = slots.shape[0]
-    kv = torch.empty(2, n, cache.kv_heads, cache.head_dim, dtype=dtype, device=slots.device)
-    k, v = kv[0], kv[1]
+    k = torch.empty(n, cache.kv_heads, cache.head_dim, dtype=dtype, device=slots.device)
+    v = torch.empty_like(k)
     _lib.check(
         lib().b200_kv_cache_read(cache.desc, slots.data_ptr(), n, k.data_ptr(), v.data_ptr(), code,
                                  cache.kv_heads * cache.head_dim, cache.head_dim,
@@ -879,6 +882,9 @@ def kv_cache_read(cache, slots: torch.Tensor, dtype: torch.dtype | None = None):
 # overlap, and its arrival counters and partial sums must not.
 _ATTN_WORKSPACES: dict[tuple[int, int], torch.Tensor] = {}
 _ATTN_BYTES: dict[tuple[int, int, int], int] = {}
+# Workspaces that a larger one has replaced: a captured graph may still use
+# them. Sizes grow by powers of two, so together they are below the present one.
+_ATTN_OUTGROWN: list[torch.Tensor] = []
 
 
 def paged_attention_workspace_bytes(head_dim: int, q_tokens: int, seqs: int) -> int:
@@ -907,6 +913,9 @@ def _attn_workspace(index: int, stream: int, head_dim: int, q_tokens: int, seqs:
         return ws
     ws = torch.zeros(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
     with _WS_LOCK:
+        old = _ATTN_WORKSPACES.get((index, stream))
+        if old is not None:
+            _ATTN_OUTGROWN.append(old)
         _ATTN_WORKSPACES[(index, stream)] = ws
     return ws
 
@@ -949,7 +958,8 @@ def paged_attention(q: torch.Tensor, cache, page_table: torch.Tensor, kv_lens: t
     ``head_dim ** -0.5``. Returns ``out``, or ``(out, lse)`` with the fp32
     ``[tokens, q_heads]`` log-sum-exp. ``max_q_len * q_heads / kv_heads <= 16``
     (decode) streams the cache; larger calls run on the tensor cores."""
-    index = _on_device("paged_attention", q, cache.k, page_table, kv_lens, q_starts, out)
+    index = _on_device("paged_attention", q, cache.k, page_table, kv_lens, q_starts, out,
+                       workspace)
     dtype = q.dtype
     code = _DTYPE_CODE.get(dtype)
     if code is None:
@@ -972,7 +982,10 @@ def paged_attention(q: torch.Tensor, cache, page_table: torch.Tensor, kv_lens: t
     lse = torch.empty(tokens, heads, dtype=torch.float32, device=q.device) if return_lse else None
     stream = _raw_stream(index)
     ws = workspace
-    if ws is None:
+    if ws is not None:
+        if ws.dtype != torch.uint8 or not ws.is_contiguous():
+            raise TypeError(f"the workspace must be contiguous uint8, got {ws.dtype}")
+    else:
         ws = _attn_workspace(index, stream, dim, tokens, seqs)
     _lib.check(
         lib().b200_paged_attention(
