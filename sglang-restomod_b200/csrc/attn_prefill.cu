@@ -88,9 +88,7 @@ struct PrefillParams {
   }
 };
 
-constexpr int kProducers = 256;
-
-template <int D, int MT, bool TMA>
+template <int D, int MT, int KV, bool TMA>
 struct Shape {
   static constexpr int kBN = D == 256 ? 64 : 128;  // keys per tile
   static constexpr int kSlices = D / 64;
@@ -103,8 +101,18 @@ struct Shape {
   static constexpr int kFixed = kQBytes + kTableBytes + kOutBytes + 4096 + 1024;
   static constexpr int kFit = (227 * 1024 - kFixed) / kTileBytes;
   static constexpr int kStages = kFit > 8 ? 8 : kFit;
+  // Duo with threads that copy 16-bit keys: registers are dealt out anew by
+  // warpgroup, so that a softmax thread can hold its row of S and reads tensor
+  // memory once: of 512 threads launched with 128 each, 256 get 184, the 128
+  // that copy 80, and relay, mma and two idle warps 64 (a chunk of 512 tokens on
+  // 16384, single-token pages, 183 -> 143 us; tensor copies take 136). For e4m3
+  // the copying threads convert as well, 256 of them with their 112 registers:
+  // 181 us on the same chunk against 190 with 128 threads and 80.
+  static constexpr bool kDeal = MT == 2 && !TMA && KV != kE4m3;
+  static constexpr bool kRowInRegs = TMA || kDeal;
+  static constexpr int kProducers = kDeal ? 128 : 256;  // threads that copy
   static constexpr int kLoaders = TMA ? 32 : kProducers;
-  static constexpr int kThreads = MT * 128 + kLoaders + 64;
+  static constexpr int kThreads = MT * 128 + kLoaders + (kDeal ? 128 : 64);
   static constexpr int kOffRing = kQBytes;
   static constexpr int kOffTable = kOffRing + kStages * kTileBytes;
   static constexpr int kOffOut = kOffTable + kTableBytes;
@@ -626,14 +634,15 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
 }
 
 template <int D, int MT, int KV, bool TMA>
-__global__ void __launch_bounds__(Shape<D, MT, TMA>::kThreads, 1)
+__global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
     attn_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap q_map,
                         const __grid_constant__ CUtensorMap k_map,
                         const __grid_constant__ CUtensorMap v_map) {
-  using S = Shape<D, MT, TMA>;
+  using S = Shape<D, MT, KV, TMA>;
   constexpr int BN = S::kBN;
   constexpr bool kHalf = KV != kBf16;  // operand type f16
   constexpr bool kQuant = KV == kE4m3;
+  constexpr int kProducers = S::kProducers;
   constexpr int kProducer = MT * 4, kMma = kProducer + S::kLoaders / 32, kRelay = kMma + 1;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
@@ -686,6 +695,7 @@ __global__ void __launch_bounds__(Shape<D, MT, TMA>::kThreads, 1)
   if (!on) {
     // nothing: the block only gives its tensor memory back
   } else if (warp < kProducer) {
+    if constexpr (S::kDeal) asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
     // ------------------------------------------------------------- softmax
     const int wg = warp >> 2;                       // S buffer's tile (duo)
     const int row = (warp & 3) * 32 + lane;         // row of the tile
@@ -725,8 +735,8 @@ __global__ void __launch_bounds__(Shape<D, MT, TMA>::kThreads, 1)
         tc_fence_after();
         const bool masked = __any_sync(0xffffffffu, col0 < lo || col0 + BN > hi);
         float top;
-        uint32_t s[TMA ? BN : 32];  // TMA: the row's S, read once
-        if constexpr (TMA) {
+        uint32_t s[S::kRowInRegs ? BN : 32];  // the row's S, read once
+        if constexpr (S::kRowInRegs) {
           load_row<BN>(ts, s);
           if (masked) mask_row<BN>(s, col0, lo, hi, scale >= 0.f ? -INFINITY : INFINITY);
           top = scale >= 0.f ? max_row<BN, false>(s) : max_row<BN, true>(s);
@@ -758,7 +768,7 @@ __global__ void __launch_bounds__(Shape<D, MT, TMA>::kThreads, 1)
         l *= f;
         m = mn;
         const float base = m == -INFINITY ? 0.f : m;
-        if constexpr (TMA)
+        if constexpr (S::kRowInRegs)
           l += exp_row<BN, kHalf>(ts, s, scale, base);
         else
           l += masked ? exp_pass<BN, kHalf, true>(ts, scale, base, col0, lo, hi)
@@ -970,6 +980,7 @@ __global__ void __launch_bounds__(Shape<D, MT, TMA>::kThreads, 1)
       more = more_n;
     }
   } else if (!TMA && warp < kMma) {
+    if constexpr (S::kDeal) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     // ------------------------------------------------------------ producer
     const int pt = tid - kProducer * 32;  // 0 .. kProducers - 1
     uint32_t stage = 0, fill = 0;         // ring position and pass
@@ -1191,129 +1202,132 @@ __global__ void __launch_bounds__(Shape<D, MT, TMA>::kThreads, 1)
       more = more_n;
     }
     cp_async_wait_all();
-  } else if (warp == kRelay) {
-    // --------------------------------------------------------------- relay
-    // Plain copies are writes of the generic proxy, the products read through
-    // the async proxy: a fence between them, in the order of the copies. Tensor
-    // copies need none, but bring whatever a page holds past the last key:
-    // those rows of V are set to zero, since zero times NaN is NaN.
-    uint32_t stage = 0, fill = 0, q_count = 0;
-    auto pass = [&](int first_zero_row) {
-      if (lane == 0) wait_bar(&ctl->landed[stage], fill & 1u, ctl, a.status);
-      __syncwarp();
-      if (TMA && first_zero_row < BN) {
-        for (int i = first_zero_row * 8 + lane; i < BN * 8; i += 32)
+  } else {
+    if constexpr (S::kDeal) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if (warp == kRelay) {
+      // --------------------------------------------------------------- relay
+      // Plain copies are writes of the generic proxy, the products read through
+      // the async proxy: a fence between them, in the order of the copies. Tensor
+      // copies need none, but bring whatever a page holds past the last key:
+      // those rows of V are set to zero, since zero times NaN is NaN.
+      uint32_t stage = 0, fill = 0, q_count = 0;
+      auto pass = [&](int first_zero_row) {
+        if (lane == 0) wait_bar(&ctl->landed[stage], fill & 1u, ctl, a.status);
+        __syncwarp();
+        if (TMA && first_zero_row < BN) {
+          for (int i = first_zero_row * 8 + lane; i < BN * 8; i += 32)
+#pragma unroll
+            for (int sl = 0; sl < S::kSlices; ++sl)
+              st_shared_u128(ring + stage * S::kTileBytes + sl * S::kKvSlice + i * 16,
+                             make_uint4(0u, 0u, 0u, 0u));
+          fence_async_smem();
+          __syncwarp();
+        }
+        if (lane == 0) {
+          if (!TMA) fence_async_smem();
+          mbar_arrive(&ctl->full[stage]);
+        }
+        if (++stage == S::kStages) {
+          stage = 0;
+          ++fill;
+        }
+      };
+      while (cur.next(g)) {
+        const int kv_len = TMA ? seq_lens(a, g.seq).kv_len : 0;
+        for (int n = 0; n < 2 * g.tiles; ++n) {
+          int zero_row = BN;
+          if (TMA) {
+            // a V entry's rows past the last key, and before any row's window
+            const bool is_v = MT == 2 ? n & 1 : n > 0 && ((n & 1) == 0 || n == 2 * g.tiles - 1);
+            const int t = MT == 2 ? n >> 1 : n == 2 * g.tiles - 1 ? g.tiles - 1 : (n >> 1) - 1;
+            if (is_v) zero_row = max(0, min(BN, kv_len - (g.begin + (g.tile0 + t) * BN)));
+          }
+          pass(zero_row);
+          if (n == 0) {
+            if (lane == 0) {
+              wait_bar(&ctl->q_landed, q_count & 1u, ctl, a.status);
+              if (!TMA) fence_async_smem();
+              mbar_arrive(&ctl->q_full);
+            }
+            ++q_count;
+          }
+        }
+      }
+    } else if (warp == kMma && elect_one()) {
+      // ----------------------------------------------------------------- mma
+      const uint32_t q_desc = desc_lo(sq, 0), k_desc = desc_lo(ring, 0);
+      const uint32_t v_desc = desc_lo(ring, S::kKvSlice);
+      const uint32_t id_s = instr_desc(kHalf, BN, false), id_o = instr_desc(kHalf, D, true);
+      uint32_t stage = 0, fill = 0;      // next ring entry to consume
+      uint32_t s_count = 0, p_count = 0; // S tiles issued, P tiles consumed (all segments)
+      uint32_t q_count = 0;
+      bool ok = true;
+      auto take = [&]() -> uint32_t {  // waits for the next ring entry
+        ok = wait_bar(&ctl->full[stage], fill & 1u, ctl, a.status);
+        return stage;
+      };
+      auto advance = [&]() {
+        if (++stage == S::kStages) {
+          stage = 0;
+          ++fill;
+        }
+      };
+      while (ok && cur.next(g)) {
+        ok = wait_bar(&ctl->q_full, q_count & 1u, ctl, a.status);
+        if (!ok) break;
+        ++q_count;
+        const int steps = MT * g.tiles;
+        uint32_t k_stage = 0, v_stage = 0;
+        auto issue_s = [&](int i) {
+          if (MT == 1 || (i & 1) == 0) {
+            k_stage = take();
+            advance();
+            if (!ok) return;
+          }
+          tc_fence_after();
+          const int buf = MT == 2 ? i & 1 : (int)(s_count & 1u);
+          const uint32_t qa = q_desc + (MT == 2 ? (i & 1) * (S::kSlices * S::kQSlice >> 4) : 0);
+          const uint32_t ka = k_desc + k_stage * (S::kTileBytes >> 4);
 #pragma unroll
           for (int sl = 0; sl < S::kSlices; ++sl)
-            st_shared_u128(ring + stage * S::kTileBytes + sl * S::kKvSlice + i * 16,
-                           make_uint4(0u, 0u, 0u, 0u));
-        fence_async_smem();
-        __syncwarp();
-      }
-      if (lane == 0) {
-        if (!TMA) fence_async_smem();
-        mbar_arrive(&ctl->full[stage]);
-      }
-      if (++stage == S::kStages) {
-        stage = 0;
-        ++fill;
-      }
-    };
-    while (cur.next(g)) {
-      const int kv_len = TMA ? seq_lens(a, g.seq).kv_len : 0;
-      for (int n = 0; n < 2 * g.tiles; ++n) {
-        int zero_row = BN;
-        if (TMA) {
-          // a V entry's rows past the last key
-          const bool is_v = MT == 2 ? n & 1 : n > 0 && ((n & 1) == 0 || n == 2 * g.tiles - 1);
-          const int t = MT == 2 ? n >> 1 : n == 2 * g.tiles - 1 ? g.tiles - 1 : (n >> 1) - 1;
-          if (is_v) zero_row = max(0, min(BN, kv_len - (g.begin + (g.tile0 + t) * BN)));
-        }
-        pass(zero_row);
-        if (n == 0) {
-          if (lane == 0) {
-            wait_bar(&ctl->q_landed, q_count & 1u, ctl, a.status);
-            if (!TMA) fence_async_smem();
-            mbar_arrive(&ctl->q_full);
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              mma_ss(tmem + buf * 128, desc_of(qa + (sl * S::kQSlice >> 4) + 2 * kk),
+                     desc_of(ka + (sl * S::kKvSlice >> 4) + 2 * kk), id_s, sl + kk > 0);
+          mma_commit(&ctl->s_full[buf]);
+          if (MT == 1 || (i & 1)) mma_commit(&ctl->empty[k_stage]);
+          if (i == steps - 1) mma_commit(&ctl->q_empty);
+          ++s_count;
+        };
+        issue_s(0);
+        if (ok && steps > 1) issue_s(1);
+        for (int i = 0; i < steps && ok; ++i) {
+          const int buf = MT == 2 ? i & 1 : (int)(p_count & 1u);
+          if (MT == 1 || (i & 1) == 0) {
+            v_stage = take();
+            advance();
+            if (!ok) break;
           }
-          ++q_count;
-        }
-      }
-    }
-  } else if (warp == kMma && elect_one()) {
-    // ----------------------------------------------------------------- mma
-    const uint32_t q_desc = desc_lo(sq, 0), k_desc = desc_lo(ring, 0);
-    const uint32_t v_desc = desc_lo(ring, S::kKvSlice);
-    const uint32_t id_s = instr_desc(kHalf, BN, false), id_o = instr_desc(kHalf, D, true);
-    uint32_t stage = 0, fill = 0;      // next ring entry to consume
-    uint32_t s_count = 0, p_count = 0; // S tiles issued, P tiles consumed (all segments)
-    uint32_t q_count = 0;
-    bool ok = true;
-    auto take = [&]() -> uint32_t {  // waits for the next ring entry
-      ok = wait_bar(&ctl->full[stage], fill & 1u, ctl, a.status);
-      return stage;
-    };
-    auto advance = [&]() {
-      if (++stage == S::kStages) {
-        stage = 0;
-        ++fill;
-      }
-    };
-    while (ok && cur.next(g)) {
-      ok = wait_bar(&ctl->q_full, q_count & 1u, ctl, a.status);
-      if (!ok) break;
-      ++q_count;
-      const int steps = MT * g.tiles;
-      uint32_t k_stage = 0, v_stage = 0;
-      auto issue_s = [&](int i) {
-        if (MT == 1 || (i & 1) == 0) {
-          k_stage = take();
-          advance();
-          if (!ok) return;
-        }
-        tc_fence_after();
-        const int buf = MT == 2 ? i & 1 : (int)(s_count & 1u);
-        const uint32_t qa = q_desc + (MT == 2 ? (i & 1) * (S::kSlices * S::kQSlice >> 4) : 0);
-        const uint32_t ka = k_desc + k_stage * (S::kTileBytes >> 4);
-#pragma unroll
-        for (int sl = 0; sl < S::kSlices; ++sl)
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            mma_ss(tmem + buf * 128, desc_of(qa + (sl * S::kQSlice >> 4) + 2 * kk),
-                   desc_of(ka + (sl * S::kKvSlice >> 4) + 2 * kk), id_s, sl + kk > 0);
-        mma_commit(&ctl->s_full[buf]);
-        if (MT == 1 || (i & 1)) mma_commit(&ctl->empty[k_stage]);
-        if (i == steps - 1) mma_commit(&ctl->q_empty);
-        ++s_count;
-      };
-      issue_s(0);
-      if (ok && steps > 1) issue_s(1);
-      for (int i = 0; i < steps && ok; ++i) {
-        const int buf = MT == 2 ? i & 1 : (int)(p_count & 1u);
-        if (MT == 1 || (i & 1) == 0) {
-          v_stage = take();
-          advance();
+          ok = wait_bar(&ctl->p_ready[buf], (p_count >> 1) & 1u, ctl, a.status);
           if (!ok) break;
-        }
-        ok = wait_bar(&ctl->p_ready[buf], (p_count >> 1) & 1u, ctl, a.status);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t va = v_desc + v_stage * (S::kTileBytes >> 4);
-        const uint32_t to = tmem + kTmemO + (MT == 2 ? (i & 1) * D : 0);
+          tc_fence_after();
+          const uint32_t va = v_desc + v_stage * (S::kTileBytes >> 4);
+          const uint32_t to = tmem + kTmemO + (MT == 2 ? (i & 1) * D : 0);
 #pragma unroll
-        for (int kk = 0; kk < BN / 16; ++kk)
-          mma_ts(to, tmem + buf * 128 + kk * 8, desc_of(va + kk * (2048 >> 4)), id_o,
-                 i >= MT || kk > 0);
-        mma_commit(&ctl->pv_done[MT == 2 ? i & 1 : 0]);
-        if (MT == 1 || (i & 1)) mma_commit(&ctl->empty[v_stage]);
-        ++p_count;
-        if (i + 2 < steps) issue_s(i + 2);
+          for (int kk = 0; kk < BN / 16; ++kk)
+            mma_ts(to, tmem + buf * 128 + kk * 8, desc_of(va + kk * (2048 >> 4)), id_o,
+                   i >= MT || kk > 0);
+          mma_commit(&ctl->pv_done[MT == 2 ? i & 1 : 0]);
+          if (MT == 1 || (i & 1)) mma_commit(&ctl->empty[v_stage]);
+          ++p_count;
+          if (i + 2 < steps) issue_s(i + 2);
+        }
       }
+      // Everything issued has finished, and every commit has arrived, before the
+      // block gives its memories back.
+      mma_commit(&ctl->drained);
+      mbar_wait(&ctl->drained, 0, a.status);
     }
-    // Everything issued has finished, and every commit has arrived, before the
-    // block gives its memories back.
-    mma_commit(&ctl->drained);
-    mbar_wait(&ctl->drained, 0, a.status);
   }
 
   tc_fence_before();
@@ -1336,7 +1350,7 @@ long long max_units(long long q_tokens, int seqs, int unit_tokens) {
 
 template <int D, int MT, int KV, bool TMA>
 cudaError_t launch(const PrefillParams& p, const CUtensorMap (&maps)[3], cudaStream_t stream) {
-  using S = Shape<D, MT, TMA>;
+  using S = Shape<D, MT, KV, TMA>;
   static bool configured[64] = {};
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
@@ -1388,7 +1402,7 @@ cudaError_t launch_type(PrefillParams& p, cudaStream_t stream) {
   CUtensorMap maps[3] = {};
   if (p.a.cache_dtype == 3)
     return launch<D, MT, kE4m3, false>(p, maps, stream);
-  if (make_maps(p, Shape<D, MT, true>::kBN, maps))
+  if (make_maps(p, Shape<D, MT, kBf16, true>::kBN, maps))
     return p.a.q_f16 ? launch<D, MT, kF16, true>(p, maps, stream)
                      : launch<D, MT, kBf16, true>(p, maps, stream);
   p.box_rows = 1;
