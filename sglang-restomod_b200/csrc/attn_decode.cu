@@ -603,6 +603,8 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
       all_lo = max(all_lo, __shfl_xor_sync(0xffffffffu, all_lo, x));
       all_hi = min(all_hi, __shfl_xor_sync(0xffffffffu, all_hi, x));
     }
+    // the first token that any row sees
+    const int lowest = a.window > 0 ? first.end - first.q_len - a.window + 1 : 0;
     v_exp = 1;
 #pragma unroll
     for (int t = 0; t < D / 16; ++t)
@@ -616,15 +618,18 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
       const int token0 = sm.info[slot].token0 + warp * S::kTokens;
       const uint32_t kb_lane = next_kb, vb_lane = next_vb;
       const int first_row = warp * S::kTokens;
-      if (TMA && token0 + S::kTokens > first.end) {
-        // what a page holds past the last key may be NaN, and P zero times it
-        // NaN again: those rows of V become zeros
+      if (TMA && (token0 + S::kTokens > first.end || token0 < lowest)) {
+        // what a page holds past the last key or before the window may be NaN,
+        // and P zero times it NaN again: those rows of V become zeros
         uint8_t* v = sm.stage[stage] + S::kHalfBytes;
         constexpr int kChunks = S::kRowBytes / 16;
-        for (int i = max(first.end - token0, 0) * kChunks + lane; i < S::kTokens * kChunks; i += 32)
+        for (int i = lane; i < S::kTokens * kChunks; i += 32) {
+          const int token = token0 + i / kChunks;
+          if (token >= lowest && token < first.end) continue;
           *reinterpret_cast<uint4*>(v + chunk_at<D, KV, true, TMA, S::kTile>(first_row + i / kChunks,
                                                                              i % kChunks)) =
               make_uint4(0u, 0u, 0u, 0u);
+        }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the next copy here
         __syncwarp();
       }

@@ -1208,18 +1208,21 @@ __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
       // --------------------------------------------------------------- relay
       // Plain copies are writes of the generic proxy, the products read through
       // the async proxy: a fence between them, in the order of the copies. Tensor
-      // copies need none, but bring whatever a page holds past the last key:
-      // those rows of V are set to zero, since zero times NaN is NaN.
+      // copies need none, but bring whatever a page holds past the last key and
+      // before the window: those rows of V are set to zero, since zero times
+      // NaN is NaN.
       uint32_t stage = 0, fill = 0, q_count = 0;
-      auto pass = [&](int first_zero_row) {
+      auto pass = [&](int seen_from, int seen_to) {  // rows of V outside become zeros
         if (lane == 0) wait_bar(&ctl->landed[stage], fill & 1u, ctl, a.status);
         __syncwarp();
-        if (TMA && first_zero_row < BN) {
-          for (int i = first_zero_row * 8 + lane; i < BN * 8; i += 32)
+        if (TMA && (seen_from > 0 || seen_to < BN)) {
+          for (int i = lane; i < BN * 8; i += 32) {
+            if (i >= seen_from * 8 && i < seen_to * 8) continue;
 #pragma unroll
             for (int sl = 0; sl < S::kSlices; ++sl)
               st_shared_u128(ring + stage * S::kTileBytes + sl * S::kKvSlice + i * 16,
                              make_uint4(0u, 0u, 0u, 0u));
+          }
           fence_async_smem();
           __syncwarp();
         }
@@ -1233,16 +1236,22 @@ __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
         }
       };
       while (cur.next(g)) {
-        const int kv_len = TMA ? seq_lens(a, g.seq).kv_len : 0;
+        const SeqLens q = seq_lens(a, g.seq);
+        // the first key that any row of the unit sees
+        const int lowest = a.window > 0 ? q.kv_len - q.q_len + g.tok0 - a.window + 1 : 0;
         for (int n = 0; n < 2 * g.tiles; ++n) {
-          int zero_row = BN;
+          int seen_from = 0, seen_to = BN;
           if (TMA) {
             // a V entry's rows past the last key, and before any row's window
             const bool is_v = MT == 2 ? n & 1 : n > 0 && ((n & 1) == 0 || n == 2 * g.tiles - 1);
             const int t = MT == 2 ? n >> 1 : n == 2 * g.tiles - 1 ? g.tiles - 1 : (n >> 1) - 1;
-            if (is_v) zero_row = max(0, min(BN, kv_len - (g.begin + (g.tile0 + t) * BN)));
+            if (is_v) {
+              const int col0 = g.begin + (g.tile0 + t) * BN;
+              seen_from = lowest - col0;
+              seen_to = min(BN, q.kv_len - col0);
+            }
           }
-          pass(zero_row);
+          pass(seen_from, seen_to);
           if (n == 0) {
             if (lane == 0) {
               wait_bar(&ctl->q_landed, q_count & 1u, ctl, a.status);

@@ -1,0 +1,34 @@
+"""Values outside a call's window or past its lengths may be anything, an
+infinity or NaN too: no row that does not see them shows it."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from tests.test_gpu_attention import BF16, E4M3, F16, build, check
+
+pytestmark = pytest.mark.gpu
+
+
+def poison(case, s, tokens, page):
+    """Infinities and NaN at some cached tokens of sequence s (their float64
+    values stay what they were: no row sees them)."""
+    cache, table = case[0], case[2]
+    for i, t in enumerate(tokens):
+        at = (table[s, t // page].item(), t % page)
+        if cache.k_scale is None:
+            cache.k[at] = cache.v[at] = float("nan") if i % 2 else float("inf")
+        else:
+            cache.k_scale[at] = cache.v_scale[at] = 255
+
+
+@pytest.mark.parametrize("store,q_dtype", [(BF16, BF16), (F16, F16), (E4M3, BF16)])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("page", [1, 16, 24, 64])
+@pytest.mark.parametrize("q_len", [1, 4, 45, 150])
+def test_not_finite_before_the_window(cuda_device, store, q_dtype, dim, page, q_len):
+    window, kv = 37, 301
+    case = build(dim + page + q_len, [q_len, 1], [kv, 20], 2, 3, dim, page, q_dtype, store)
+    poison(case, 0, range(kv - q_len - window + 1), page)
+    check(case, window=window)
