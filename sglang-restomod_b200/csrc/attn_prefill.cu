@@ -357,6 +357,7 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const PrefillPa
   // (with tensor copies a unit's first key is moved down to a copy's border)
   __shared__ long long sh[32];
   __shared__ int base_sh[kPlanSeqs + 1];
+  __shared__ long long at_sh[kPlanThreads];
   // (each step of the search below reads it: from global memory 1 us a step)
   int* seq_base = p.a.seqs <= kPlanSeqs ? base_sh : p.seq_base;
   griddep_wait();
@@ -381,7 +382,6 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const PrefillPa
   const int per = (units + kPlanThreads - 1) / kPlanThreads;
   const int u0 = min(tid * per, units), u1 = min(u0 + per, units);
   long long mine = 0;
-  int first_tiles = 0;  // of unit u0: most threads have one unit at most
   if (u0 < u1) {
     int lo = 0, hi = a.seqs - 1;  // last sequence whose base is <= u0
     while (lo < hi) {
@@ -403,28 +403,40 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const PrefillPa
       begin -= begin % p.box_rows;
       const int tiles = end > begin ? (end - begin + bn - 1) / bn : 1;
       p.units[u] = make_int4(s, tok0, begin, tiles);
-      if (u == u0) first_tiles = tiles;
       mine += (long long)(tiles + kUnitCost) * a.c.heads;
     }
   }
-  long long at = block_scan(mine, sh, total);
+  const long long at = block_scan(mine, sh, total);
+  at_sh[tid] = at;  // of unit u0; `total` where the thread has none
   long long ctas = (total + kMinTiles - 1) / kMinTiles;
   if (ctas > max_ctas) ctas = max_ctas;
   if (tid == 0) {
     p.head[0] = total;
     p.head[1] = ctas;
   }
-  for (int u = u0; u < u1; ++u) {
-    const int cost = (u == u0 ? first_tiles : p.units[u].w) + kUnitCost;
-    const long long n = (long long)cost * a.c.heads;
-    // blocks whose first tile floor(total * c / ctas) lies in [at, at + n)
-    for (long long c = (at * ctas + total - 1) / total; c < ctas; ++c) {
-      const long long t0 = total * c / ctas;
-      if (t0 >= at + n) break;
-      const int h = (int)((t0 - at) / cost);
-      p.start[c] = make_int4(u, h, (int)(t0 - at - (long long)h * cost), 0);
+  __syncthreads();
+  // A thread per block finds the unit of the block's first place. (A thread per
+  // unit that stepped through the blocks starting in it took 37 us where one
+  // unit fed all 148; the search takes the kernel to 4.)
+  for (long long c = tid; c < ctas; c += kPlanThreads) {
+    const long long t0 = total * c / ctas;
+    int lo = 0, hi = kPlanThreads - 1;  // last thread with at_sh <= t0
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (at_sh[mid] <= t0)
+        lo = mid;
+      else
+        hi = mid - 1;
     }
-    at += n;
+    long long x = t0 - at_sh[lo];
+    int u = lo * per;
+    int cost = p.units[u].w + kUnitCost;
+    while (x >= (long long)cost * a.c.heads) {
+      x -= (long long)cost * a.c.heads;
+      cost = p.units[++u].w + kUnitCost;
+    }
+    const int h = (int)(x / cost);
+    p.start[c] = make_int4(u, h, (int)(x - (long long)h * cost), 0);
   }
   griddep_launch_dependents();
 }
