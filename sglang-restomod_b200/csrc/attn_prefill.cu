@@ -40,8 +40,8 @@
 // Work: the tiles' key ranges laid end to end, with a constant for what each
 // costs besides its key tiles, and cut evenly over the blocks
 // (attn_plan_kernel finds each block's start from q_starts and kv_lens); a tile
-// cut by a border leaves partial (O, m, l) and the last block to arrive adds
-// them in block order.
+// cut by a border leaves partial (O, m, l), which attn_combine_kernel adds in
+// block order.
 //
 // The maximum is lazy: m is raised, and O rescaled, only where some S exceeds it
 // by more than 8 (in log2), so that most tiles leave O alone.
@@ -101,18 +101,19 @@ struct Shape {
   static constexpr int kFixed = kQBytes + kTableBytes + kOutBytes + 4096 + 1024;
   static constexpr int kFit = (227 * 1024 - kFixed) / kTileBytes;
   static constexpr int kStages = kFit > 8 ? 8 : kFit;
-  // Duo with threads that copy 16-bit keys: registers are dealt out anew by
-  // warpgroup, so that a softmax thread can hold its row of S and reads tensor
-  // memory once: of 512 threads launched with 128 each, 256 get 184, the 128
-  // that copy 80, and relay, mma and two idle warps 64 (a chunk of 512 tokens on
-  // 16384, single-token pages, 183 -> 143 us; tensor copies take 136). For e4m3
-  // the copying threads convert as well, 256 of them with their 112 registers:
-  // 181 us on the same chunk against 190 with 128 threads and 80.
-  static constexpr bool kDeal = MT == 2 && !TMA && KV != kE4m3;
+  // Duo deals registers out anew by warpgroup, so that a softmax thread can
+  // hold its row of S and reads tensor memory once. With threads that copy: of
+  // 512 launched with 128 each, 256 get 184, the 128 that copy 80, and relay,
+  // mma and two idle warps 64 (a chunk of 512 tokens on 16384, single-token
+  // pages, 183 -> 143 us; tensor copies take 136). With tensor copies: of 384
+  // launched with 168, 256 get 200 and loader, relay, mma and an idle warp 104.
+  // For e4m3 the copying threads convert as well, 256 of them with their 112
+  // registers: 181 us on the same chunk against 190 with 128 threads and 80.
+  static constexpr bool kDeal = MT == 2 && KV != kE4m3;
   static constexpr bool kRowInRegs = TMA || kDeal;
-  static constexpr int kProducers = kDeal ? 128 : 256;  // threads that copy
+  static constexpr int kProducers = kDeal && !TMA ? 128 : 256;  // threads that copy
   static constexpr int kLoaders = TMA ? 32 : kProducers;
-  static constexpr int kThreads = MT * 128 + kLoaders + (kDeal ? 128 : 64);
+  static constexpr int kThreads = MT * 128 + kLoaders + (!kDeal ? 64 : TMA ? 96 : 128);
   static constexpr int kOffRing = kQBytes;
   static constexpr int kOffTable = kOffRing + kStages * kTileBytes;
   static constexpr int kOffOut = kOffTable + kTableBytes;
@@ -139,7 +140,6 @@ struct Ctl {
   uint64_t q_scaled[2];  // e4m3: q_scale of even and odd segments is written
   uint32_t tmem;
   int abort;
-  int flag[2];
   float q_scale[2][2][128];  // e4m3: of Q's rows; segment parity, tile, row
 };
 
@@ -503,6 +503,12 @@ __device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
   return r;
 }
 
+// Where a block's partial (m, l, O) of a tile of 128 rows lies, in floats: the
+// block's first run of keys continues a pair, its last one may begin another.
+__device__ __forceinline__ long long part_at(long long block, bool begins, int mt, int tile, int d) {
+  return ((2 * block + (begins ? 1 : 0)) * mt + tile) * (long long)(d + 2) * 128;
+}
+
 // Bit i: key col + i lies in [lo, hi).
 __device__ __forceinline__ uint32_t seen_bits(int col, int lo, int hi) {
   const int a = min(max(hi - col, 0), 32), b = min(max(lo - col, 0), 32);
@@ -645,6 +651,81 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
+// Adds the parts of the (unit, head) pairs that were cut, in block order: grid
+// (attention blocks, tiles x D / 16), a thread per row with 16 columns. Block x
+// takes the pair that ends in attention block x's first run, if there is one.
+// (When the last attention block to arrive added a pair's parts, its four warps
+// had 16 KB under way at a time: 1.2 us a part. As a launch of its own it took a
+// chunk of 100 tokens on 16384 e4m3 ones, one key/value head, from 181 to 45 us;
+// 40 tokens on 8192, 8 heads, 59 to 32; 512 on 16384, e4m3, 176 to 166; where
+// little is cut it costs 1 to 2 us of 55.)
+constexpr int kCombineCols = 16;
+__global__ void __launch_bounds__(128) attn_combine_kernel(const PrefillParams p, int d, int mt) {
+  griddep_wait();
+  const AttnLaunch& a = p.a;
+  const long long total = __ldcg(p.head), ctas = __ldcg(p.head + 1), c = blockIdx.x;
+  if (c >= ctas) return;
+  const int4 s = __ldcg(p.start + c);
+  if (s.z <= kUnitCost) return;  // all of the pair's key tiles are this block's
+  const int4 u = __ldcg(p.units + s.x);
+  const long long t0 = total * c / ctas, t1 = total * (c + 1) / ctas;
+  const int cost = u.w + kUnitCost;
+  if (t1 - t0 < cost - s.z) return;  // the pair goes on
+  const int groups = d / kCombineCols, tile = blockIdx.y / groups;
+  const int col = blockIdx.y % groups * kCombineCols, row = threadIdx.x;
+  const SeqLens q = seq_lens(a, u.x);
+  const int tok = u.y + tile * p.tile_tokens + row / p.groups;
+  if (row >= p.tile_tokens * p.groups || tok >= q.q_len) return;
+  // the block that holds the pair's first key tile
+  const long long first = ((t0 - s.z + kUnitCost + 1) * ctas - 1) / total;
+  float m = -INFINITY, l = 0.f, acc[kCombineCols];
+#pragma unroll
+  for (int i = 0; i < kCombineCols; ++i) acc[i] = 0.f;
+  constexpr int kBatch = 4;  // parts on their way together
+  for (long long b0 = first; b0 <= c; b0 += kBatch) {
+    float mb[kBatch], lb[kBatch], v[kBatch][kCombineCols];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const bool on = b0 + j <= c;
+      const float* part =
+          p.parts + part_at(on ? b0 + j : c, on && b0 + j == first, mt, tile, d) + row;
+      mb[j] = on ? __ldcg(part) : -INFINITY;
+      lb[j] = on ? __ldcg(part + 128) : 0.f;
+#pragma unroll
+      for (int i = 0; i < kCombineCols; ++i) v[j][i] = __ldcg(part + (2 + col + i) * 128);
+    }
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      // (a part without a visible key has m = -inf, l = 0 and O = 0; one with a
+      // NaN has l = NaN whatever its m)
+      const float mn = fmaxf(m, mb[j]);
+      const float f = m == mn ? 1.f : ex2(m - mn), w = mb[j] == mn ? 1.f : ex2(mb[j] - mn);
+      m = mn;
+      if (mb[j] == -INFINITY && lb[j] == 0.f) continue;
+      l = l * f + lb[j] * w;
+#pragma unroll
+      for (int i = 0; i < kCombineCols; ++i) acc[i] = acc[i] * f + v[j][i] * w;
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const long long token = (long long)q.q0 + tok;
+  const int qh = s.y * p.groups + row % p.groups;
+  uint16_t* out = static_cast<uint16_t*>(a.out) + token * a.out_token_stride +
+                  (long long)qh * a.out_head_stride + col;
+#pragma unroll
+  for (int i = 0; i < kCombineCols; i += 8) {
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float x = acc[i + 2 * j] * inv, y = acc[i + 2 * j + 1] * inv;
+      w[j] = a.q_f16 ? pack2<true>(x, y) : pack2<false>(x, y);
+    }
+    *reinterpret_cast<uint4*>(out + i) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  if (col == 0 && a.lse != nullptr)
+    a.lse[token * a.q_heads + qh] = l == 0.f ? -INFINITY : (m + log2f(l)) / kLog2e;
+}
+
 template <int D, int MT, int KV, bool TMA>
 __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
     attn_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap q_map,
@@ -707,7 +788,8 @@ __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
   if (!on) {
     // nothing: the block only gives its tensor memory back
   } else if (warp < kProducer) {
-    if constexpr (S::kDeal) asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    if constexpr (S::kDeal && TMA) asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    if constexpr (S::kDeal && !TMA) asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
     // ------------------------------------------------------------- softmax
     const int wg = warp >> 2;                       // S buffer's tile (duo)
     const int row = (warp & 3) * 32 + lane;         // row of the tile
@@ -852,8 +934,8 @@ __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
           a.lse[token * a.q_heads + qh] = l == 0.f ? -INFINITY : (m + log2f(l)) / kLog2e;
         continue;
       }
-      constexpr long long kPart = (long long)(D + 2) * 128;  // floats of a tile's partial
-      float* part = p.parts + ((2ll * blockIdx.x + (g.tile0 == 0 ? 1 : 0)) * MT + wg) * kPart + row;
+      // partial (O, m, l) for attn_combine_kernel, rows adjacent
+      float* part = p.parts + part_at(blockIdx.x, g.tile0 == 0, MT, wg, D) + row;
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];
@@ -864,57 +946,10 @@ __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
       }
       part[0] = l == 0.f ? -INFINITY : m;
       part[128] = l;
-      // the blocks that hold the pair's first and last key tile
-      const long long first = g.at + kUnitCost, end = first + g.unit_tiles;
-      const int c_first = (int)(((first + 1) * ctas - 1) / total);
-      const int c_last = (int)((end * ctas - 1) / total);
-      __threadfence();
-      named_bar_sync(2 + wg, 128);
-      if ((tid & 127) == 0) {
-        int* counter = a.counters + 2 * c_first + wg;
-        const bool last = atomicAdd(counter, 1) == c_last - c_first;
-        if (last) *counter = 0;
-        ctl->flag[wg] = last;
-        __threadfence();
-      }
-      named_bar_sync(2 + wg, 128);
-      const bool last = *reinterpret_cast<volatile int*>(&ctl->flag[wg]) != 0;
-      named_bar_sync(2 + wg, 128);  // the flag may be written again
-      if (!last) continue;
-      const float* parts = p.parts + row;
-      auto part_at = [&](int b) {
-        return parts + ((2ll * b + (b == c_first ? 1 : 0)) * MT + wg) * kPart;
-      };
-      float mx = -INFINITY, sum = 0.f;
-      for (int b = c_first; b <= c_last; ++b) mx = fmaxf(mx, __ldcg(part_at(b)));
-      for (int b = c_first; b <= c_last; ++b) {
-        const float mb = __ldcg(part_at(b)), lb = __ldcg(part_at(b) + 128);
-        sum += mb == -INFINITY ? lb : lb * ex2(mb - mx);
-      }
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
-        float acc[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) acc[i] = 0.f;
-        for (int b = c_first; b <= c_last; ++b) {
-          const float* src = part_at(b);
-          const float mb = __ldcg(src);
-          const float w = mb == -INFINITY ? 0.f : ex2(mb - mx);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float v = __ldcg(src + (2 + 32 * c + i) * 128);
-            acc[i] += w == 0.f ? 0.f : v * w;
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < 32; ++i) acc[i] *= inv;
-        emit(c, acc);
-      }
-      if (valid && a.lse != nullptr)
-        a.lse[token * a.q_heads + qh] = sum == 0.f ? -INFINITY : (mx + log2f(sum)) / kLog2e;
     }
-  } else if (TMA && warp < kMma) {
+  } else {
+  if constexpr (S::kDeal && TMA) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+  if (TMA && warp < kMma) {
     // -------------------------------------------------------------- loader
     // One warp, a lane per box of box_rows keys. Boxes past the last key and
     // boxes of pages outside the cache are copied from past the map's end,
@@ -992,7 +1027,7 @@ __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
       more = more_n;
     }
   } else if (!TMA && warp < kMma) {
-    if constexpr (S::kDeal) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    if constexpr (S::kDeal && !TMA) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
     // ------------------------------------------------------------ producer
     const int pt = tid - kProducer * 32;  // 0 .. kProducers - 1
     uint32_t stage = 0, fill = 0;         // ring position and pass
@@ -1215,7 +1250,7 @@ __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
     }
     cp_async_wait_all();
   } else {
-    if constexpr (S::kDeal) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if constexpr (S::kDeal && !TMA) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     if (warp == kRelay) {
       // --------------------------------------------------------------- relay
       // Plain copies are writes of the generic proxy, the products read through
@@ -1350,6 +1385,7 @@ __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
       mbar_wait(&ctl->drained, 0, a.status);
     }
   }
+  }
 
   tc_fence_before();
   __syncthreads();
@@ -1389,8 +1425,11 @@ cudaError_t launch(const PrefillParams& p, const CUtensorMap (&maps)[3], cudaStr
   err = launch_pdl(attn_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, p,
                    MT * p.tile_tokens, S::kBN, sms);
   if (err != cudaSuccess) return err;
-  return launch_pdl(attn_prefill_kernel<D, MT, KV, TMA>, dim3((unsigned)sms), dim3(S::kThreads),
-                    S::kSmem, stream, p, maps[0], maps[1], maps[2]);
+  err = launch_pdl(attn_prefill_kernel<D, MT, KV, TMA>, dim3((unsigned)sms), dim3(S::kThreads),
+                   S::kSmem, stream, p, maps[0], maps[1], maps[2]);
+  if (err != cudaSuccess) return err;
+  return launch_pdl(attn_combine_kernel, dim3((unsigned)sms, MT * (D / kCombineCols)), dim3(128), 0,
+                    stream, p, D, MT);
 }
 
 // Tensor maps of q [tokens][heads][D] and of the cache. False where maps cannot
