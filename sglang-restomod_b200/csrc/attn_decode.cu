@@ -45,7 +45,6 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 8.f;        // log2 of the largest P before a rescale
-constexpr int kMaxCtas = 1024;      // arrival counters in the workspace
 // A block takes at least this much work, in tiles: below it the pair's merge
 // costs more than the extra blocks bring. And a pair is cut into at most
 // kMaxParts, whose sum one block takes.
@@ -1114,12 +1113,17 @@ cudaError_t launch_rows(DecodeParams& p, int rows, cudaStream_t stream) {
                                    : KV == kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   CUtensorMap maps[2] = {};
+  // Tensor copies against cp.async, 64 sequences of up to 8192 tokens, 8 heads
+  // of 128: e4m3, pages of 64 and 16, 110 / 215 and 116 / 215 us; bf16, pages of
+  // 64 and 8, 205 / 427 and 344 / 442.
   p.box_rows = cache_box_rows(p.a.c, 16);  // a warp's tokens
   if (make_cache_maps(p.a.c, type, kElem, (kRowBytes < 128 ? kRowBytes : 128) / kElem, p.box_rows,
                       kRowBytes < 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
-                      &maps[0], &maps[1], &p.heads_first))
-    return rows <= 8 ? launch<D, KV, 1, true>(p, maps, stream)
-                     : launch<D, KV, 2, true>(p, maps, stream);
+                      &maps[0], &maps[1], &p.heads_first)) {
+    if constexpr (KV == kE4m3 || D == 64)
+      if (rows > 8) return launch<D, KV, 2, true>(p, maps, stream);
+    return launch<D, KV, 1, true>(p, maps, stream);
+  }
   return rows <= 8 ? launch<D, KV, 1, false>(p, maps, stream)
                    : launch<D, KV, 2, false>(p, maps, stream);
 }
@@ -1133,8 +1137,16 @@ cudaError_t launch_type(DecodeParams& p, int rows, cudaStream_t stream) {
 
 }  // namespace
 
-int attn_decode_rows() { return 16; }
-int attn_max_ctas() { return kMaxCtas; }
+// 16 rows fill two groups of 8; the tensor cores' kernel (attn_prefill.cu) takes
+// the second one's place where its tiles come by tensor copies unconverted and
+// are wide enough. This kernel against that one in us, 16 rows, bf16, 4 heads:
+// head_dim 128, 1 x 4000 keys 25 / 22, 1 x 60000 54 / 46, 64 x 4000 76 / 69;
+// head_dim 256 36 / 26, 79 / 68, 121 / 119; but head_dim 64 21 / 19, 46 / 41,
+// 43 / 64, and 64 x 8192 e4m3 keys, 8 heads, 258 / 476. With 8 rows this kernel
+// is ahead in all but the last by 2 to 8 us (64 x 4000, head_dim 128: 69 / 69).
+int attn_decode_rows(const AttnLaunch& l) {
+  return l.cache_dtype != 3 && l.c.head_dim >= 128 && l.c.page_size % 8 == 0 ? 8 : 16;
+}
 
 long long attn_decode_scratch_bytes(int head_dim) {
   return 2ll * 2 * device_sm_count() * 16 * (head_dim + 4) * 4;

@@ -16,26 +16,29 @@
 //
 // One block per SM. Warps by role:
 //
-//   softmax   one warpgroup per S buffer, one thread per row: the row's maximum
-//             over S in tensor memory, then e^(S - m) back over it as 16-bit P
-//   producer  two warpgroups: Q, K and V tiles into shared memory in the
-//             operands' 128-byte-swizzled layout, 16 bytes per copy. Plain
-//             cp.async rather than tensor copies, since a page may be of any
-//             size down to one token and rows past the end have to be zero;
-//             e4m3 codes are converted on the way, to f16 for every model type
-//             (two instructions a pair where bf16 took five): a code times its
-//             power of two is exact in f16 but for what lies below its smallest
-//             subnormal step, 2^-9 of a vector's largest value at worst; bf16
-//             queries are brought to f16 by a power of two per row
-//   relay     one thread: passes each tile that has landed on to the tensor
-//             core's reads (a proxy fence, off the mma thread's path)
+//   softmax   one warpgroup per tile of rows, one thread per row: the row's
+//             maximum over S in tensor memory, then e^(S - m) back over it as
+//             16-bit P
+//   loader    one warp: Q, K and V tiles by tensor copies, a lane per box of a
+//             page's tokens (16-bit caches with pages of a multiple of 8 tokens)
+//   producer  or four or eight warps: the same tiles by 16-byte copies, since a
+//             page may be of any size down to one token (a prompt of 8192 bf16
+//             tokens: 622 us, by tensor copies 522), or, e4m3, loads that are
+//             converted on the way, to f16 for every model type (two instructions
+//             a pair where bf16 took five): a code times its power of two is
+//             exact in f16 but for what lies below its smallest subnormal step,
+//             2^-9 of a vector's largest value at worst; bf16 queries are brought
+//             to f16 by a power of two per row
+//   relay     one warp: passes each tile that has landed on to the tensor core's
+//             reads (a proxy fence, off the mma thread's path) and zeroes what a
+//             tensor copy brought of no use
 //   mma       one thread: S = Q K^T into one of two S buffers, O += P V
 //             (P from tensor memory, V as the transposed B operand)
 //
 // head_dim 64 and 128: two tiles of 128 rows in turn ("duo"), so that one
 // tile's softmax runs beside the other's products. Calls whose sequences have
-// at most 128 rows, and head_dim 256 (whose O takes half of tensor memory): one
-// tile, the next keys' S beside the present softmax ("solo").
+// few rows, and head_dim 256 (whose O takes half of tensor memory): one tile,
+// the next keys' S beside the present softmax ("solo").
 //
 // Work: the tiles' key ranges laid end to end, with a constant for what each
 // costs besides its key tiles, and cut evenly over the blocks
@@ -44,7 +47,17 @@
 // block order.
 //
 // The maximum is lazy: m is raised, and O rescaled, only where some S exceeds it
-// by more than 8 (in log2), so that most tiles leave O alone.
+// by more than 8 (in log2), so that most tiles leave O alone. P is at most 2^8
+// then, and its rounding to 16 bits relative whatever m is; l sums the unrounded
+// fp32 P.
+//
+// Measured (one B200): a prompt of 8192 bf16 tokens, 32 heads of 128 over 8,
+// 506 to 528 us, 1040 to 1085 TFLOP/s, 63 to 66 % of the measured bf16 product
+// rate; a tile of 256 rows and 128 keys takes 2.3 us and its exponentials 1.1,
+// so the chain S -> maximum -> P -> product, two tiles deep, sets the time.
+// (Tried without gain: half rows by four warpgroups, keys by 64 with four S
+// buffers, polynomials for an eighth to a half of the exponentials, P handed
+// over in halves.) 512 tokens on 16384 e4m3 ones: 166 us, 813 TFLOP/s; bf16 136.
 #include "attn_maps.cuh"
 #include "common.cuh"
 #include "internal.h"
@@ -57,9 +70,13 @@ using namespace tcg;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 8.f;
-constexpr int kMinTiles = 4;  // a block takes at least this much work, in key tiles
+// A block takes at least this much work, in key tiles (2 instead: 100 tokens on
+// 16384, one head, 46 us against 45; 16 mixed chunks 62 against 56).
+constexpr int kMinTiles = 4;
 // What a run of key tiles of one (rows, head) costs beside them, in key tiles:
-// Q in, O out and the pipeline's filling.
+// Q in, O out and the pipeline's filling (3.7 us, a tile 2.2). With 1, 2, 3 a
+// prompt of 8192 tokens takes 570, 515, 527 us, 16 mixed chunks 61, 56, 66, 512
+// tokens on 16384 e4m3 ones 169, 166, 164.
 constexpr int kUnitCost = 2;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kTmemO = 256;  // O after the two S buffers of up to 128 columns
@@ -1499,8 +1516,14 @@ cudaError_t launch_attn_prefill(const AttnLaunch& l, cudaStream_t stream) {
   p.units = reinterpret_cast<int4*>(at);
   at += align256(16ll * p.max_units);
   p.parts = reinterpret_cast<float*>(at);
-  // Two tiles in turn pay once a sequence fills more than one.
-  const bool duo = (long long)l.max_q * p.groups > 128;
+  // Two tiles in turn pay where sequences fill several. Solo against duo in us,
+  // head_dim 128, rows a sequence: bf16 by tensor copies 55 / 62 (256, 16 x
+  // 4096 keys), 35 / 38 (512, 4 x 4096), 87 / 78 (1024, 16384), 613 / 506
+  // (32768, a prompt of 8192); where threads copy, and hold no row of S in
+  // registers when solo, 82 / 89 (128 e4m3), 106 / 116 and 80 / 75 (256, head_dim
+  // 128 and 64), 59 / 56 (512), 150 / 104 (1024), 272 / 165 (2048).
+  const bool tensor_copies = l.cache_dtype != 3 && l.c.page_size % 8 == 0;
+  const bool duo = (long long)l.max_q * p.groups > (tensor_copies ? 512 : 128);
   switch (l.c.head_dim) {
     case 64: return duo ? launch_type<64, 2>(p, stream) : launch_type<64, 1>(p, stream);
     case 128: return duo ? launch_type<128, 2>(p, stream) : launch_type<128, 1>(p, stream);

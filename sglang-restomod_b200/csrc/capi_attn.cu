@@ -269,10 +269,9 @@ int b200_paged_attention(const b200_kv_cache* cache, const void* q, int32_t dtyp
   l.counters = reinterpret_cast<int*>(base + ws_counter_offset());
   l.scratch = base + fixed;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  // Both kernels take any number of rows in principle; up to 16 rows a
-  // sequence and key/value head the streaming kernel wastes nothing.
+  // Rows of a sequence and key/value head: the streaming kernel takes few.
   const int64_t rows = (int64_t)max_q_len * (q_heads / cache->kv_heads);
-  if (rows <= attn_decode_rows())
+  if (rows <= attn_decode_rows(l))
     return check_cuda(launch_attn_decode(l, st), "attention (decode) launch");
   return check_cuda(launch_attn_prefill(l, st), "attention (prefill) launch");
 }

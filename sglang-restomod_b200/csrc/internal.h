@@ -322,7 +322,7 @@ struct AttnLaunch {
 };
 // The decode kernel takes up to attn_decode_rows() rows (new tokens x query
 // heads per key/value head) of a sequence; the tensor-core kernel any number.
-int attn_decode_rows();
+int attn_decode_rows(const AttnLaunch& l);
 long long attn_decode_scratch_bytes(int head_dim);
 cudaError_t launch_attn_decode(const AttnLaunch& l, cudaStream_t stream);
 long long attn_prefill_scratch_bytes(int head_dim, long long q_tokens, int seqs);

@@ -12,10 +12,10 @@
 // Bound: HBM. Per element 2 B of x, 2 + 2 B of residual read and written,
 // 1 B of q (or 2 B of y). A row stays in its threads' registers between the
 // sum of squares and the scaling, so each byte moves once; the weights come from
-// L1. Rows wider than 1024 columns take a block each and come by bulk copies
-// into a ring of stages, so that the next rows are on their way while one is
-// summed, scaled and stored; narrower ones (the per-head norms of queries and
-// keys) take a warp each, 8 in flight per block and no block barrier. A group
+// L1. Wide rows take a block each and come by bulk copies into a ring of
+// stages, so that the next rows are on their way while one is summed, scaled and
+// stored; narrow ones (the per-head norms of queries and keys) take a warp each,
+// 8 in flight per block and no block barrier. A group
 // of 128 columns is 16 lanes x 8 columns, so its maximum is four shuffles.
 #include "common.cuh"
 #include "internal.h"
@@ -343,7 +343,12 @@ __global__ void __launch_bounds__(1024) add_rms_norm_kernel(NormParams p, int st
 template <bool F16>
 cudaError_t launch(const NormParams& p, cudaStream_t stream) {
   const int sms = device_sm_count();
-  if (p.h8 <= 128) {
+  // A warp per row up to 512 columns, and up to 1024 once there are more rows
+  // than the block kernel keeps at a time: 16384 rows to e4m3 take 13 / 27 us by
+  // warps and 45 / 49 by blocks (512 / 1024 columns), 64 rows 2.5 / 3.9 and 2.8 /
+  // 2.9. At 2048 columns a warp's registers no longer hold the row: 70 us by
+  // warps, 57 by blocks.
+  if (p.h8 <= 64 || (p.h8 <= 128 && p.rows > 4ll * sms)) {
     constexpr int kWarps = 8;
     long long blocks = (p.rows + kWarps - 1) / kWarps;
     if (blocks > 8ll * sms) blocks = 8ll * sms;

@@ -956,8 +956,9 @@ def paged_attention(q: torch.Tensor, cache, page_table: torch.Tensor, kv_lens: t
     ``window`` (causal only; 0: none) keeps the last ``window`` positions. Rows
     that see nothing give zeros and ``-inf``. ``scale`` defaults to
     ``head_dim ** -0.5``. Returns ``out``, or ``(out, lse)`` with the fp32
-    ``[tokens, q_heads]`` log-sum-exp. ``max_q_len * q_heads / kv_heads <= 16``
-    (decode) streams the cache; larger calls run on the tensor cores."""
+    ``[tokens, q_heads]`` log-sum-exp. A few new tokens (``max_q_len * q_heads /
+    kv_heads`` up to 8 or 16, by type and head size) stream the cache; larger calls
+    run on the tensor cores' kernel."""
     index = _on_device("paged_attention", q, cache.k, page_table, kv_lens, q_starts, out,
                        workspace)
     dtype = q.dtype

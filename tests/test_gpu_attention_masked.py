@@ -1,5 +1,6 @@
 """Values outside a call's window or past its lengths may be anything, an
-infinity or NaN too: no row that does not see them shows it."""
+infinity or NaN too: no row that does not see them shows it. And calls at the
+borders of the kernels' rules."""
 
 from __future__ import annotations
 
@@ -32,3 +33,21 @@ def test_not_finite_before_the_window(cuda_device, store, q_dtype, dim, page, q_
     case = build(dim + page + q_len, [q_len, 1], [kv, 20], 2, 3, dim, page, q_dtype, store)
     poison(case, 0, range(kv - q_len - window + 1), page)
     check(case, window=window)
+
+
+def test_more_sequences_than_the_plan_keeps_on_chip(cuda_device):
+    seqs = 4200
+    check(build(3, [3] * seqs, [3 + s % 7 for s in range(seqs)], 1, 6, 64, 8, BF16, BF16))
+
+
+@pytest.mark.parametrize("store,q_dtype", [(BF16, BF16), (F16, F16), (E4M3, BF16)])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("page", [8, 12])
+@pytest.mark.parametrize("q_len,groups", [(1, 8), (2, 8), (1, 9), (2, 16), (33, 4), (129, 4), (171, 3)])
+def test_rows_around_the_rules(cuda_device, store, q_dtype, dim, page, q_len, groups):
+    check(build(dim + q_len, [q_len, 1, 0], [q_len + 150, 70, 3], 1, groups, dim, page, q_dtype, store))
+
+
+def test_one_unit_over_all_blocks(cuda_device):
+    check(build(5, [20], [20011], 1, 1, 128, 64, BF16, E4M3))
+    check(build(6, [20, 2], [20011, 9000], 1, 1, 256, 16, F16, F16), window=15000)
