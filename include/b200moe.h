@@ -518,7 +518,7 @@ int b200_kv_cache_read(const b200_kv_cache* cache, const int64_t* slots, int64_t
  * causal: position p sees positions <= p, and with window > 0 only the last
  * `window` of them; not causal: all cached tokens. A row that sees nothing
  * gets zeros and lse = -inf. max_q_len bounds the new tokens of any sequence
- * (1: decode); further ones would be left unwritten. Page numbers outside the
+ * (1: decode); further ones, and rows of no sequence, are left unwritten. Page numbers outside the
  * cache read as zeros and set status bit 16. Cached values past kv_lens are
  * never read. The cache is e4m3, or of q's type. q and out: vectors 16-byte
  * aligned, strides in elements. No host synchronization, and no host knowledge

@@ -26,9 +26,10 @@
 //             tokens: 622 us, by tensor copies 522), or, e4m3, loads that are
 //             converted on the way, to f16 for every model type (two instructions
 //             a pair where bf16 took five): a code times its power of two is
-//             exact in f16 but for what lies below its smallest subnormal step,
-//             2^-9 of a vector's largest value at worst; bf16 queries are brought
-//             to f16 by a power of two per row
+//             exact in f16 down to its smallest step, 2^-24, an absolute error of
+//             2^-25 in values below it (it shows in bf16 results where all of V
+//             is below 2^-17); bf16 queries are brought to f16 by a power of two
+//             per row
 //   relay     one warp: passes each tile that has landed on to the tensor core's
 //             reads (a proxy fence, off the mma thread's path) and zeroes what a
 //             tensor copy brought of no use

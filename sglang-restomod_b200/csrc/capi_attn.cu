@@ -222,7 +222,7 @@ int b200_paged_attention(const b200_kv_cache* cache, const void* q, int32_t dtyp
   if (q_heads / cache->kv_heads > 128)
     return fail(B200_ERR_UNSUPPORTED, "at most 128 query heads per key/value head, got %d",
                 q_heads / cache->kv_heads);
-  if (seqs < 0 || q_tokens < 0 || q_tokens > 0x7fffffffll || max_q_len < 0 || page_table_width < 0)
+  if (seqs < 0 || q_tokens < 0 || q_tokens + seqs > 0x7fffffffll || max_q_len < 0 || page_table_width < 0)
     return fail(B200_ERR_INVALID, "negative or too large count");
   if (window < 0 || (window > 0 && !causal))
     return fail(B200_ERR_INVALID, "a window needs causal attention and at least one token");

@@ -17,6 +17,10 @@
 // stored; narrow ones (the per-head norms of queries and keys) take a warp each,
 // 8 in flight per block and no block barrier. A group
 // of 128 columns is 16 lanes x 8 columns, so its maximum is four shuffles.
+//
+// Measured (one B200, graph replay): 16384 rows of 7168 bf16 with residual to
+// e4m3 142 us, 5.8 TB/s (89 % of the measured copy rate); 1021 rows of 2048 f16
+// 3.7 us; one row of 7168 to e4m3 3.2 us, nearly all of it the launch.
 #include "common.cuh"
 #include "internal.h"
 

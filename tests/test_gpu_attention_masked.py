@@ -4,6 +4,8 @@ borders of the kernels' rules."""
 
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -51,3 +53,27 @@ def test_rows_around_the_rules(cuda_device, store, q_dtype, dim, page, q_len, gr
 def test_one_unit_over_all_blocks(cuda_device):
     check(build(5, [20], [20011], 1, 1, 128, 64, BF16, E4M3))
     check(build(6, [20, 2], [20011, 9000], 1, 1, 256, 16, F16, F16), window=15000)
+
+
+@pytest.mark.parametrize("store,q_dtype", [(BF16, BF16), (F16, F16), (E4M3, BF16), (E4M3, F16)])
+@pytest.mark.parametrize("page", [1, 16])
+@pytest.mark.parametrize("scale", [0.0, -0.11, 1e-30])
+@pytest.mark.parametrize("q_len,groups", [(1, 8), (40, 4), (150, 4)])
+def test_scales_of_any_sign(cuda_device, store, q_dtype, page, scale, q_len, groups):
+    check(build(q_len, [q_len, 2], [q_len + 190, 2], 1, groups, 128, page, q_dtype, store), scale=scale)
+
+
+@pytest.mark.parametrize("page", [1, 16])
+@pytest.mark.parametrize("q_len", [1, 40, 150])
+@pytest.mark.parametrize("size", [2.0 ** -12, 2.0 ** 13])
+def test_e4m3_of_small_and_large_values(cuda_device, page, q_len, size):
+    """Values of V about `size`; K's are the usual ones."""
+    cache, q, table, kv_lens, starts, kc, vc = build(q_len, [q_len], [q_len + 190], 1, 4, 128, page,
+                                                     BF16, E4M3)
+    shift = round(math.log2(size))
+    scaled = cache.v_scale.cpu().int() + shift
+    written = cache.v_scale.cpu() != 255
+    # the bytes' powers of two moved alike: codes and float64 values follow
+    cache.v_scale.copy_(torch.where(written, scaled.clamp(103, 134), 255).to(torch.uint8))
+    assert (scaled[written] >= 103).all() and (scaled[written] <= 134).all()
+    check((cache, q, table, kv_lens, starts, kc, vc * size))
