@@ -1502,7 +1502,9 @@ cudaError_t launch_attn_prefill(const AttnLaunch& l, cudaStream_t stream) {
   p.a = l;
   p.groups = l.q_heads / l.c.heads;
   p.tile_tokens = 128 / p.groups;
-  p.scale_log2 = l.scale * kLog2e;
+  // A masked score is an infinity that the scale multiplies, so a scale of zero
+  // becomes the smallest normal number: finite scores still come to e^0.
+  p.scale_log2 = l.scale == 0.f ? 1.1754944e-38f : l.scale * kLog2e;
   p.box_rows = 1;
   p.page_shift = (l.c.page_size & (l.c.page_size - 1)) == 0 ? __builtin_ctz(l.c.page_size) : -1;
   const long long sms = device_sm_count();

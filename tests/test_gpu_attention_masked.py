@@ -9,7 +9,9 @@ import math
 import pytest
 import torch
 
-from tests.test_gpu_attention import BF16, E4M3, F16, build, check
+from oracle import attention as ref
+from sglang_restomod_b200 import ops
+from tests.test_gpu_attention import BF16, E4M3, F16, bounds, build, check
 
 pytestmark = pytest.mark.gpu
 
@@ -60,7 +62,15 @@ def test_one_unit_over_all_blocks(cuda_device):
 @pytest.mark.parametrize("scale", [0.0, -0.11, 1e-30])
 @pytest.mark.parametrize("q_len,groups", [(1, 8), (40, 4), (150, 4)])
 def test_scales_of_any_sign(cuda_device, store, q_dtype, page, scale, q_len, groups):
-    check(build(q_len, [q_len, 2], [q_len + 190, 2], 1, groups, 128, page, q_dtype, store), scale=scale)
+    case = build(q_len, [q_len, 2], [q_len + 190, 2], 1, groups, 128, page, q_dtype, store)
+    cache, q, table, kv_lens, starts, kc, vc = case
+    out, lse = ops.paged_attention(q.cuda(), cache, table.cuda(), kv_lens.cuda(), starts.cuda(),
+                                   max(q_len, 2), scale=scale, return_lse=True)
+    want, want_lse = ref.paged_attention_ref(q, kc, vc, table, kv_lens, starts, scale)
+    # (the bound grows with the scores' magnitude, whatever their sign)
+    tol, lse_tol = bounds(q, kc, vc, abs(scale), q_dtype, q_dtype)
+    assert (out.cpu().double() - want).abs().max().item() <= tol
+    assert (lse.cpu().double() - want_lse).abs().max().item() <= lse_tol
 
 
 @pytest.mark.parametrize("page", [1, 16])
