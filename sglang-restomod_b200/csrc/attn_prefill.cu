@@ -119,19 +119,31 @@ struct Shape {
   static constexpr int kFixed = kQBytes + kTableBytes + kOutBytes + 4096 + 1024;
   static constexpr int kFit = (227 * 1024 - kFixed) / kTileBytes;
   static constexpr int kStages = kFit > 8 ? 8 : kFit;
-  // Duo deals registers out anew by warpgroup, so that a softmax thread can
-  // hold its row of S and reads tensor memory once. With threads that copy: of
-  // 512 launched with 128 each, 256 get 184, the 128 that copy 80, and relay,
-  // mma and two idle warps 64 (a chunk of 512 tokens on 16384, single-token
-  // pages, 183 -> 143 us; tensor copies take 136). With tensor copies: of 384
-  // launched with 168, 256 get 200 and loader, relay, mma and an idle warp 104.
-  // For e4m3 the copying threads convert as well, 256 of them with their 112
-  // registers: 181 us on the same chunk against 190 with 128 threads and 80.
-  static constexpr bool kDeal = MT == 2 && KV != kE4m3;
+  // Registers are dealt out anew by warpgroup where a softmax thread can then
+  // hold its row of S and read tensor memory once (us without and with, head_dim
+  // 128 unless said; d64: head_dim 64):
+  //   solo, threads copy   e4m3 16 x 32 tokens on 4096, 82 / 66, d64 61 / 47;
+  //                        single-token pages of bf16, 72 / 57
+  //   duo, threads copy    16-bit, 512 tokens on 16384, single-token pages, 183 /
+  //                        143; e4m3, 8 x 512 on 2048, d64 108 / 89; not e4m3 at
+  //                        head_dim 128, whose converting threads need more than
+  //                        is left (512 on 16384 167 / 171)
+  //   duo, tensor copies   spills go, 551 / 517 for a prompt of 8192
+  // Solo with tensor copies has registers enough as it is launched. The sum is
+  // what the block is launched with: threads x registers of softmax, copying
+  // threads, and the rest (relay, mma, idle warps; the loader).
+  static constexpr bool kDeal = MT == 2 ? KV != kE4m3 || D == 64 : !TMA;
   static constexpr bool kRowInRegs = TMA || kDeal;
-  static constexpr int kProducers = kDeal && !TMA ? 128 : 256;  // threads that copy
+  static constexpr int kProducers = MT == 2 && KV != kE4m3 && !TMA ? 128 : 256;  // threads that copy
   static constexpr int kLoaders = TMA ? 32 : kProducers;
-  static constexpr int kThreads = MT * 128 + kLoaders + (!kDeal ? 64 : TMA ? 96 : 128);
+  static constexpr int kRest = !kDeal ? 64 : TMA ? 96 : 128;
+  static constexpr int kThreads = MT * 128 + kLoaders + kRest;
+  static constexpr int kSoftmaxRegs = MT == 1 ? 216 : TMA ? 200 : KV == kE4m3 ? 160 : 184;
+  static constexpr int kRestRegs = MT == 1 ? 88 : TMA ? 104 : KV == kE4m3 ? 48 : 64;
+  static constexpr int kCopyRegs = MT == 1 ? 104 : TMA ? kRestRegs : KV == kE4m3 ? 56 : 80;
+  static constexpr int kDealtRegs =
+      MT * 128 * kSoftmaxRegs + kLoaders * kCopyRegs + kRest * kRestRegs;
+  static_assert(!kDeal || kDealtRegs <= kThreads * (65536 / kThreads / 8 * 8), "more than there is");
   static constexpr int kOffRing = kQBytes;
   static constexpr int kOffTable = kOffRing + kStages * kTileBytes;
   static constexpr int kOffOut = kOffTable + kTableBytes;
@@ -191,6 +203,16 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, Ctl* ct
     }
   }
   return false;
+}
+
+// Registers of a warpgroup's threads, from what the block was launched with.
+template <int N>
+__device__ __forceinline__ void regs_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -806,8 +828,7 @@ __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
   if (!on) {
     // nothing: the block only gives its tensor memory back
   } else if (warp < kProducer) {
-    if constexpr (S::kDeal && TMA) asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
-    if constexpr (S::kDeal && !TMA) asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    if constexpr (S::kDeal) regs_up<S::kSoftmaxRegs>();
     // ------------------------------------------------------------- softmax
     const int wg = warp >> 2;                       // S buffer's tile (duo)
     const int row = (warp & 3) * 32 + lane;         // row of the tile
@@ -966,7 +987,7 @@ __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
       part[128] = l;
     }
   } else {
-  if constexpr (S::kDeal && TMA) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+  if constexpr (S::kDeal && TMA) regs_down<S::kRestRegs>();
   if (TMA && warp < kMma) {
     // -------------------------------------------------------------- loader
     // One warp, a lane per box of box_rows keys. Boxes past the last key and
@@ -1045,7 +1066,7 @@ __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
       more = more_n;
     }
   } else if (!TMA && warp < kMma) {
-    if constexpr (S::kDeal && !TMA) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    if constexpr (S::kDeal) regs_down<S::kCopyRegs>();
     // ------------------------------------------------------------ producer
     const int pt = tid - kProducer * 32;  // 0 .. kProducers - 1
     uint32_t stage = 0, fill = 0;         // ring position and pass
@@ -1170,11 +1191,12 @@ __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
           }
           cp_async_arrive_noinc(&ctl->landed[stage]);
         } else {
-          uint4 codes[kQuant ? kPer : 1];
-#pragma unroll
-          for (int i = 0; i < (kQuant ? kPer : 1); ++i) codes[i] = held[i];
-          if (n + 1 < items) load(n + 1);
           acquire();
+          // each register of codes is filled for the next entry once converted
+          int tn = 0;
+          bool v_next = false;
+          if (n + 1 < items) item(n + 1, tn, v_next);
+          const RowInfo* next_rows = table + (tn & 3) * BN;
           const RowFactor* fs = factors + (t & 3) * BN;
           // 16 columns: chunks 2c and 2c + 1 of the 16-bit row
           const int c2 = 2 * p_chunk;
@@ -1184,8 +1206,13 @@ __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
           for (int i = 0; i < (kQuant ? kPer : 1); ++i) {
             const RowFactor& rf = fs[p_row + i * kRowStep];
             const uint32_t f = is_v ? rf.v : rf.k;
-            const uint2 x = convert4(codes[i].x, f), y = convert4(codes[i].y, f);
-            const uint2 z = convert4(codes[i].z, f), w = convert4(codes[i].w, f);
+            const uint4 codes = held[i];
+            if (n + 1 < items) {
+              const RowInfo& r = next_rows[p_row + i * kRowStep];
+              held[i] = __ldg(reinterpret_cast<const uint4*>((v_next ? r.v : r.k) + p_chunk * 16));
+            }
+            const uint2 x = convert4(codes.x, f), y = convert4(codes.y, f);
+            const uint2 z = convert4(codes.z, f), w = convert4(codes.w, f);
             st_shared_u128(dst + i * kRowStep * 128 + x0, make_uint4(x.x, x.y, y.x, y.y));
             st_shared_u128(dst + i * kRowStep * 128 + x1, make_uint4(z.x, z.y, w.x, w.y));
           }
@@ -1268,7 +1295,7 @@ __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
     }
     cp_async_wait_all();
   } else {
-    if constexpr (S::kDeal && !TMA) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if constexpr (S::kDeal && !TMA) regs_down<S::kRestRegs>();
     if (warp == kRelay) {
       // --------------------------------------------------------------- relay
       // Plain copies are writes of the generic proxy, the products read through
@@ -1435,6 +1462,12 @@ cudaError_t launch(const PrefillParams& p, const CUtensorMap (&maps)[3], cudaStr
     err = cudaFuncSetAttribute(attn_prefill_kernel<D, MT, KV, TMA>,
                                cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem);
     if (err != cudaSuccess) return err;
+    if (S::kDeal) {  // the kernel must not ask for more registers than it gets
+      cudaFuncAttributes fa;
+      err = cudaFuncGetAttributes(&fa, attn_prefill_kernel<D, MT, KV, TMA>);
+      if (err != cudaSuccess) return err;
+      if (fa.numRegs * S::kThreads < S::kDealtRegs) return cudaErrorLaunchOutOfResources;
+    }
     configured[dev] = true;
   }
   static_assert(S::kSmem <= 227 * 1024 && S::kStages >= 4, "shared memory");
@@ -1520,13 +1553,11 @@ cudaError_t launch_attn_prefill(const AttnLaunch& l, cudaStream_t stream) {
   at += align256(16ll * p.max_units);
   p.parts = reinterpret_cast<float*>(at);
   // Two tiles in turn pay where sequences fill several. Solo against duo in us,
-  // head_dim 128, rows a sequence: bf16 by tensor copies 55 / 62 (256, 16 x
-  // 4096 keys), 35 / 38 (512, 4 x 4096), 87 / 78 (1024, 16384), 613 / 506
-  // (32768, a prompt of 8192); where threads copy, and hold no row of S in
-  // registers when solo, 82 / 89 (128 e4m3), 106 / 116 and 80 / 75 (256, head_dim
-  // 128 and 64), 59 / 56 (512), 150 / 104 (1024), 272 / 165 (2048).
-  const bool tensor_copies = l.cache_dtype != 3 && l.c.page_size % 8 == 0;
-  const bool duo = (long long)l.max_q * p.groups > (tensor_copies ? 512 : 128);
+  // head_dim 128, by rows of a sequence: 256 (16 x 4096 keys) bf16 55 / 62, e4m3
+  // 93 / 115, single-token pages 71 / 73; 512 (4 x 4096) 35 / 38, 45 / 55, 42 /
+  // 46; 1024 (16384) 87 / 78, 124 / 104, 95 / 85; 2048 (16384) e4m3 221 / 165;
+  // 32768 (a prompt of 8192) bf16 613 / 506.
+  const bool duo = (long long)l.max_q * p.groups > 512;
   switch (l.c.head_dim) {
     case 64: return duo ? launch_type<64, 2>(p, stream) : launch_type<64, 1>(p, stream);
     case 128: return duo ? launch_type<128, 2>(p, stream) : launch_type<128, 1>(p, stream);
