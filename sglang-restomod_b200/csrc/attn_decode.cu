@@ -18,10 +18,10 @@
 //   cut by a range border leaves partial (O, m, l) in the scratch; the last
 //   block to arrive at the pair's counter adds them in block order, so the
 //   result does not depend on which block that is.
-// * One warp fills a ring of stages, a tile of 16 tokens per consumer warp each,
+// * A producer fills a ring of stages, a tile of 16 tokens per consumer warp each,
 //   and runs on into the next pair while the present one is finished. Pages of
-//   a multiple of 8 tokens come by tensor copies; other pages (single-token
-//   ones, say) by 16-byte cp.async. (When every warp issued the copies of its
+//   a multiple of 8 tokens come by tensor copies of one warp; other pages
+//   (single-token ones, say) by 16-byte cp.async of two or four. (When every warp issued the copies of its
 //   own tokens, issuing them took a third of its step: 75 to 150 clocks each.)
 //   Consumers meet only where a pair ends.
 // * The products are taken transposed (S^T = K Q^T, O^T = V^T P^T): the
@@ -97,15 +97,23 @@ struct Shape {
   // stages are large (16 sequences of up to 32768 tokens, head_dim 256, bf16:
   // 144, 120, 108, 98 us with 2, 3, 4, 6 consumer warps).
   static constexpr int kTokens = 16;
-  static constexpr int kWarps = D == 256 && KV != kE4m3 ? 6 : 7;
+  // Without tensor copies one warp cannot issue the copies fast enough: four do
+  // where a block has the SM to itself, two in place of a consumer warp where two
+  // blocks share it (64 sequences of up to 4000 tokens, 4 heads, single-token
+  // pages, 8 rows, us with one and with this: bf16 head_dim 64 71 / 59, 128 141 /
+  // 102, 256 180 / 117; e4m3 head_dim 64 48 / 50, 128 79 / 65, 256 184 / 112).
+  static constexpr int kBlocks = D == 64 || (D == 128 && KV == kE4m3) ? 2 : 1;
+  static constexpr int kWarps =
+      (D == 256 && KV != kE4m3) || (!TMA && kBlocks == 2) ? 6 : 7;
   static constexpr int kConsumers = kWarps * 32;
-  static constexpr int kThreads = kConsumers + 32;
   static constexpr int kTile = kTokens * kWarps;            // tokens per step
   static constexpr int kHalfBytes = kTile * kRowBytes;      // K, or V, of a stage
   static constexpr int kStageBytes = 2 * kHalfBytes;
   static constexpr int kRows = 8 * NR;
   // Ring: 70 to 84 KB per block and two blocks per SM, or 168 to 192 KB and one.
-  static constexpr int kBlocks = D == 64 || (D == 128 && KV == kE4m3) ? 2 : 1;
+  static constexpr int kProducers = TMA ? 1 : kBlocks == 2 ? 2 : 4;
+  static constexpr int kAllWarps = kWarps + kProducers;
+  static constexpr int kThreads = kAllWarps * 32;
   static constexpr int kStages = D == 256 && KV != kE4m3 ? 2 : KV == kE4m3 && D == 64 ? 5 : 3;
   static constexpr int kRing = kStages + 2;  // tile descriptions
   static constexpr int kQPitch = D + 8;      // 16-bit elements, conflict-free rows
@@ -117,7 +125,7 @@ struct Shape {
     TileInfo info[kRing];
     float row_scale[kRows];
     float wm[kWarps][kRows], wl[kWarps][kRows], mx[kRows], sum[kRows];
-    long long scan[kWarps + 1], scan_pairs[kWarps + 1];
+    long long scan[kAllWarps], scan_pairs[kAllWarps];
     int start_seq;
     long long start_off;
     int flag;
@@ -244,7 +252,7 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
   const int heads = a.c.heads;
   if (tid == 0) {
     for (int i = 0; i < S::kStages; ++i) {
-      mbar_init(&sm.full[i], TMA ? 1 : 33);  // (lane 0's own arrival, and the copies')
+      mbar_init(&sm.full[i], TMA ? 1 : 32 * S::kProducers + 1);  // (lane 0's own, the copies')
       mbar_init(&sm.empty[i], kWarps);
     }
     for (int i = 0; i < 2; ++i) {
@@ -285,7 +293,7 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
     before -= mine;
     total = pairs = 0;
 #pragma unroll
-    for (int w = 0; w <= kWarps; ++w) {
+    for (int w = 0; w < S::kAllWarps; ++w) {
       if (w < warp) before += sm.scan[w];
       total += sm.scan[w];
       pairs += sm.scan_pairs[w];
@@ -315,8 +323,9 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
     return p.page_shift >= 0 ? token >> p.page_shift : token / a.c.page_size;
   };
 
-  if (warp == kWarps) {
+  if (warp >= kWarps) {
     // ------------------------------------------------------------ producer
+    const int part = warp - kWarps;  // which of the copying warps; the first also describes
     int seq = sm.start_seq;
     SeqRange range = seq_range<S::kTile>(a, seq, kAlign);
     int head = (int)(sm.start_off / cost_of(range));
@@ -379,6 +388,7 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
       return pg;
     };
     auto publish = [&](int slot, const TileInfo& ti, const Pages& pg) {
+      if (part > 0) return;
       if (lane == 0) sm.info[slot] = ti;
       if (TMA) {
         if (lane < boxes)
@@ -408,7 +418,7 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
         const int buf = ti.pair & 1;
         mbar_wait(&sm.q_empty[buf], (uint32_t)((ti.pair >> 1) & 1) ^ 1u, a.status);
         const int rows = ti.q_len * p.groups;
-        for (int i = lane; i < S::kRows * (D / 8); i += 32) {
+        for (int i = lane; i < (part > 0 ? 0 : S::kRows * (D / 8)); i += 32) {
           const int r = i / (D / 8), chunk = i % (D / 8);
           const bool on = r < rows;
           const uint16_t* src =
@@ -418,7 +428,7 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
                   : 0);
           cp_async_16_zfill(&sm.q[buf][r][chunk * 8], src, on);
         }
-        cp_async_arrive_noinc(&sm.q_full[buf]);
+        if (part == 0) cp_async_arrive_noinc(&sm.q_full[buf]);
       }
       uint8_t* ks = sm.stage[stage];
       if (TMA) {
@@ -466,7 +476,7 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
 #pragma unroll
         for (int i = 0; i < kLook; ++i)
 #pragma unroll 4
-          for (int j = 0; j < (kChunks < 32 ? kChunks : 32); ++j) {
+          for (int j = part; j < (kChunks < 32 ? kChunks : 32); j += S::kProducers) {
             const int r32 = j * kPerPass + lane / kChunks, row = 32 * i + r32;
             long long o = __shfl_sync(0xffffffffu, off[i], r32);
             const bool on = o >= 0;
@@ -480,7 +490,7 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
             }
           }
         cp_async_arrive_noinc(&sm.full[stage]);
-        if (lane == 0) mbar_arrive(&sm.full[stage]);
+        if (lane == 0 && part == 0) mbar_arrive(&sm.full[stage]);
       }
       ti = ahead;
       pg = pg_ahead;
@@ -1120,10 +1130,15 @@ cudaError_t launch_rows(DecodeParams& p, int rows, cudaStream_t stream) {
                                                 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   CUtensorMap maps[2] = {};
   // Tensor copies against cp.async, 64 sequences of up to 8192 tokens, 8 heads
-  // of 128: e4m3, pages of 64 and 16, 110 / 215 and 116 / 215 us; bf16, pages of
-  // 64 and 8, 205 / 427 and 344 / 442.
+  // of 128: e4m3, pages of 64 and 16, 110 / 164 and 115 / 169 us; bf16, pages of
+  // 64 and 8, 205 / 294 and 342 / 306. Of pages that only boxes of 8 rows divide
+  // (8 and 24 tokens), 64 of up to 4000, 4 heads: bf16 head_dim 64 46 / 56 and 48 /
+  // 63, 128 106 / 97 and 108 / 117, e4m3 128 55 / 62 and 56 / 70, 256 114 / 108 and
+  // 116 / 128, but bf16 head_dim 256, four copies a box, 178 / 116 and 179 / 121:
+  // these take cp.async.
   p.box_rows = cache_box_rows(p.a.c, 16);  // a warp's tokens
-  if (make_cache_maps(p.a.c, type, kElem, (kRowBytes < 128 ? kRowBytes : 128) / kElem, p.box_rows,
+  if (!(kRowBytes == 512 && p.box_rows < 16) &&
+      make_cache_maps(p.a.c, type, kElem, (kRowBytes < 128 ? kRowBytes : 128) / kElem, p.box_rows,
                       kRowBytes < 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
                       &maps[0], &maps[1], &p.heads_first)) {
     if constexpr (KV == kE4m3 || D == 64)
