@@ -1159,8 +1159,8 @@ cudaError_t launch_type(DecodeParams& p, int rows, cudaStream_t stream) {
 }  // namespace
 
 // 16 rows fill two groups of 8; the tensor cores' kernel (attn_prefill.cu) takes
-// the second one's place where its tiles come by tensor copies unconverted and
-// are wide enough. This kernel against that one in us, 16 rows, bf16, 4 heads:
+// the second one's place where its tiles are copied unconverted from pages of a
+// multiple of 8 tokens and are wide enough. This kernel against that one in us, 16 rows, bf16, 4 heads:
 // head_dim 128, 1 x 4000 keys 25 / 22, 1 x 60000 54 / 46, 64 x 4000 76 / 69;
 // head_dim 256 36 / 26, 79 / 68, 121 / 119; but head_dim 64 21 / 19, 46 / 41,
 // 43 / 64, and 64 x 8192 e4m3 keys, 8 heads, 258 / 476. With 8 rows this kernel

@@ -20,10 +20,11 @@
 //             maximum over S in tensor memory, then e^(S - m) back over it as
 //             16-bit P
 //   loader    one warp: Q, K and V tiles by tensor copies, a lane per box of a
-//             page's tokens (16-bit caches with pages of a multiple of 8 tokens)
+//             page's tokens (16-bit caches with pages of a multiple of 16
+//             tokens, 32 at head_dim 256)
 //   producer  or four or eight warps: the same tiles by 16-byte copies, since a
-//             page may be of any size down to one token (a prompt of 8192 bf16
-//             tokens: 622 us, by tensor copies 522), or, e4m3, loads that are
+//             page may be of any size down to one token (512 tokens on 16384,
+//             bf16: 143 us, by tensor copies 136), or, e4m3, loads that are
 //             converted on the way, to f16 for every model type (two instructions
 //             a pair where bf16 took five): a code times its power of two is
 //             exact in f16 down to its smallest step, 2^-24, an absolute error of
@@ -1490,6 +1491,12 @@ bool make_maps(PrefillParams& p, int bn, CUtensorMap (&maps)[3]) {
   const CUtensorMapDataType type = a.q_f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                            : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   p.box_rows = cache_box_rows(a.c, bn);
+  // Small boxes come at some 50 ns each whatever they hold. Tensor copies against
+  // threads, 512 tokens on 16384 and 64 x 4 tokens on up to 4000, by the rows of a
+  // box: head_dim 64, 8 rows, 119 / 118 and 83 / 83 us, 134 / 121 where pages of
+  // 24 lie across tiles; 128, 8 rows 181 / 138 and 200 / 154, 16 rows 132 / 140 and
+  // 136 / 153; 256, 16 rows 402 / 326 and 244 / 222, 32 rows 318 / 328 and 217 / 219.
+  if (p.box_rows < (a.c.head_dim == 256 ? 32 : 16)) return false;
   if (!make_cache_maps(a.c, type, 2, 64, p.box_rows, CU_TENSOR_MAP_SWIZZLE_128B, &maps[1], &maps[2],
                        &p.heads_first))
     return false;
