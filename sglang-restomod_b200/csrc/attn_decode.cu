@@ -1160,11 +1160,12 @@ cudaError_t launch_type(DecodeParams& p, int rows, cudaStream_t stream) {
 
 // 16 rows fill two groups of 8; the tensor cores' kernel (attn_prefill.cu) takes
 // the second one's place where its tiles are copied unconverted from pages of a
-// multiple of 8 tokens and are wide enough. This kernel against that one in us, 16 rows, bf16, 4 heads:
-// head_dim 128, 1 x 4000 keys 25 / 22, 1 x 60000 54 / 46, 64 x 4000 76 / 69;
-// head_dim 256 36 / 26, 79 / 68, 121 / 119; but head_dim 64 21 / 19, 46 / 41,
-// 43 / 64, and 64 x 8192 e4m3 keys, 8 heads, 258 / 476. With 8 rows this kernel
-// is ahead in all but the last by 2 to 8 us (64 x 4000, head_dim 128: 69 / 69).
+// multiple of 8 tokens and are wide enough. This kernel against that one in us,
+// 16 rows, bf16, 4 heads: head_dim 128, 1 x 4000 keys 25 / 22, 1 x 60000 54 / 46,
+// 64 x 4000 76 / 69; head_dim 256 36 / 26, 79 / 68, 121 / 119; but head_dim 64 21 /
+// 19, 46 / 41, 43 / 64, single-token pages at 128 26 / 26 and, 16 x 1000, 25 / 30,
+// and 64 x 8192 e4m3 keys, 8 heads, 258 / 476. With 8 rows this kernel is ahead in
+// all but 64 x 4000 keys (head_dim 128: 69 / 69), by 2 to 8 us.
 int attn_decode_rows(const AttnLaunch& l) {
   return l.cache_dtype != 3 && l.c.head_dim >= 128 && l.c.page_size % 8 == 0 ? 8 : 16;
 }
