@@ -103,8 +103,12 @@ using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t
                                    CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
 // cuTensorMapEncodeTiled through the runtime's driver entry point (no link
-// dependency on libcuda).
+// dependency on libcuda). The driver wants a current context, which a thread
+// that has made no runtime call of its own yet does not have: cudaSetDevice to
+// the device it is on makes the primary one current.
 inline EncodeTiledFn encode_tiled() {
+  int dev = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess) (void)cudaSetDevice(dev);
   static EncodeTiledFn fn = nullptr;
   if (fn == nullptr) {
     void* ptr = nullptr;
