@@ -17,8 +17,8 @@
  * at least the size the matching *_workspace_bytes() function returns, zero
  * filled before its first use. The kernels return every counter and partial
  * sum they touch to zero, so one workspace serves any number of calls - but
- * calls that share a workspace must be ordered (same stream, or joined by
- * events); two calls running at once on one workspace race.
+ * calls that share a workspace must be ordered (same stream, from any threads,
+ * or joined by events); two calls running at once on one workspace race.
  *
  * Dtype codes: 0 = bf16, 1 = f16, 2 = f32, 3 = e4m3.
  *

@@ -71,6 +71,7 @@ int64_t stream_ws_bytes() {
 }
 
 struct WsView {
+  std::unique_lock<std::mutex> together;  // held until the call has launched
   int* status;
   int* counters;
   void* plan;
@@ -82,6 +83,7 @@ struct WsView {
 bool carve(void* ws, int64_t bytes, WsView& v) {
   const int64_t fixed = stream_ws_bytes();
   if (ws == nullptr || bytes < fixed || (reinterpret_cast<uintptr_t>(ws) % kAlign) != 0) return false;
+  v.together = std::unique_lock<std::mutex>(launch_mutex());
   uint8_t* base = reinterpret_cast<uint8_t*>(ws);
   v.status = reinterpret_cast<int*>(base);
   v.counters = reinterpret_cast<int*>(base + kStatusBytes);
@@ -252,6 +254,13 @@ bool use_tc_moe(int32_t quant, int32_t block_size, int64_t groups) {
 int b200::set_last_error(int code, const char* message) {
   g_last_error = message;
   return code;
+}
+
+std::mutex& b200::launch_mutex() {
+  static std::mutex mu[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
+  return mu[dev];
 }
 
 int64_t b200::ws_head_bytes() { return kStatusBytes + kCounterBytes; }

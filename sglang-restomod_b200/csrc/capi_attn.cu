@@ -271,6 +271,7 @@ int b200_paged_attention(const b200_kv_cache* cache, const void* q, int32_t dtyp
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   // Rows of a sequence and key/value head: the streaming kernel takes few.
   const int64_t rows = (int64_t)max_q_len * (q_heads / cache->kv_heads);
+  const std::lock_guard<std::mutex> together(launch_mutex());
   if (rows <= attn_decode_rows(l))
     return check_cuda(launch_attn_decode(l, st), "attention (decode) launch");
   return check_cuda(launch_attn_prefill(l, st), "attention (prefill) launch");

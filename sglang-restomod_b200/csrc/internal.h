@@ -7,6 +7,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <mutex>
+
 namespace b200 {
 
 // Weight-streaming GEMM: Y[rows, N] = X[rows, K] * dequant(W[N, K])^T, with
@@ -332,6 +334,12 @@ inline long long attn_scratch_bytes(int head_dim, long long q_tokens, int seqs) 
   const long long p = attn_prefill_scratch_bytes(head_dim, q_tokens, seqs);
   return d > p ? d : p;
 }
+
+// Held, one per device, while a call that uses a workspace puts its launches on a
+// stream: kernels of one call hand on through the workspace (a plan, converted
+// operands, partial sums), and when two threads call on one stream no other
+// call's kernel, a single one either, may come between them.
+std::mutex& launch_mutex();
 
 // Records `message` as this thread's b200_last_error() and returns `code`.
 int set_last_error(int code, const char* message);
