@@ -241,7 +241,8 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
     attn_decode_kernel(const DecodeParams p, const __grid_constant__ CUtensorMap k_map,
                        const __grid_constant__ CUtensorMap v_map) {
   using S = Shape<D, KV, NR, TMA>;
-  constexpr int kAlign = TMA ? 16 : 1;
+  // a window's first box starts within the page of its first token
+  const int align = TMA ? p.box_rows : 1;
   using Smem = typename S::Smem;
   constexpr int kWarps = S::kWarps, kThreads = S::kThreads, kConsumers = S::kConsumers;
   extern __shared__ uint8_t smem_raw[];
@@ -274,7 +275,7 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
     const int s0 = min(tid * per, a.seqs), s1 = min(s0 + per, a.seqs);
     long long mine = 0, pairs = 0;
     for (int s = s0; s < s1; ++s) {
-      const int n = cost_of(seq_range<S::kTile>(a, s, kAlign));
+      const int n = cost_of(seq_range<S::kTile>(a, s, align));
       mine += (long long)n * heads;
       pairs += n ? heads : 0;
     }
@@ -307,7 +308,7 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
     if (t0 >= before && t0 < before + mine) {
       int s = s0;
       for (;; ++s) {
-        const long long n1 = (long long)cost_of(seq_range<S::kTile>(a, s, kAlign)) * heads;
+        const long long n1 = (long long)cost_of(seq_range<S::kTile>(a, s, align)) * heads;
         if (t0 < before + n1) break;
         before += n1;
       }
@@ -327,7 +328,7 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
     // ------------------------------------------------------------ producer
     const int part = warp - kWarps;  // which of the copying warps; the first also describes
     int seq = sm.start_seq;
-    SeqRange range = seq_range<S::kTile>(a, seq, kAlign);
+    SeqRange range = seq_range<S::kTile>(a, seq, align);
     int head = (int)(sm.start_off / cost_of(range));
     int x = (int)(sm.start_off - (long long)head * cost_of(range));  // place in the pair
     long long at = t0;
@@ -362,7 +363,7 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
           head = 0;
           if (at < t1) {
             do {
-              range = seq_range<S::kTile>(a, ++seq, kAlign);
+              range = seq_range<S::kTile>(a, ++seq, align);
             } while (range.tiles == 0);
           }
         }
