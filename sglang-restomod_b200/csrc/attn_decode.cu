@@ -32,9 +32,12 @@
 // * e4m3 codes are converted to f16 (exact) for every model type: bf16 queries
 //   are brought to f16 by a power of two per row (exact but for parts 2^-24
 //   below the row's largest), P is rounded to f16. The key's scale multiplies
-//   s in fp32; the value's multiplies P relative to the largest seen.
+//   s in fp32; the value's 2^e goes into P's exponent, O(row) = sum 2^(s + e - mv)
+//   code with a lazy maximum mv of s + e over the tokens that the row sees, so that
+//   P keeps f16's bits for the tokens that make up the result, however far apart
+//   scales lie (one reference scale for a tile's tokens lost what lay 2^14 below it).
 // * The maximum is lazy: O and l are rescaled only when some s exceeds m by
-//   more than 2^8, so P stays below 2^8 and most tiles need no cross-lane
+//   more than 8 (in log2), so P stays below 2^8 and most tiles need no cross-lane
 //   reduction at all.
 //
 // Measured (one B200, graph replay): 64 sequences of up to 8192 tokens, 8 heads
@@ -173,11 +176,6 @@ __device__ __forceinline__ float exp2_fast(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
-}
-
-// 2^e for e in [-254, 0]; 0 below the normal range.
-__device__ __forceinline__ float pow2(int e) {
-  return e < -126 ? 0.f : __uint_as_float((uint32_t)(127 + e) << 23);
 }
 
 // Byte of 16-byte chunk `chunk` of token row `row` in a stage's K or V tile,
@@ -529,7 +527,7 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
   // ---- consume
   float o[D / 16][NR][4];
   float m[NR][2], l[NR][2];   // rows 8 nr + 2c, + 1
-  int v_exp = 1;              // e4m3: byte of the largest value scale so far
+  float mv[NR][2];            // e4m3: O is in units of 2^mv, as l in units of 2^m
   __syncthreads();  // the producer's first description
   int slot = 0, stage = 0;
   uint32_t phase = 0, next_kb = 0, next_vb = 0;
@@ -607,6 +605,7 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
         row_hi[nr][j] = r >= rows ? 0 : a.causal ? min(first.end, pos + 1) : first.end;
         row_lo[nr][j] = a.window > 0 ? max(0, pos - a.window + 1) : 0;
         m[nr][j] = -INFINITY;
+        mv[nr][j] = -INFINITY;
         raise_at[nr][j] = -INFINITY;
         l[nr][j] = 0.f;
         if (8 * nr + 2 * c + j < rows) {
@@ -621,7 +620,6 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
     }
     // the first token that any row sees
     const int lowest = a.window > 0 ? first.end - first.q_len - a.window + 1 : 0;
-    v_exp = 1;
 #pragma unroll
     for (int t = 0; t < D / 16; ++t)
 #pragma unroll
@@ -723,8 +721,7 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
       }
 
       // -- scales, masks, lazy maximum
-      int v_byte[kG][2] = {};
-      bool raise_v = false;
+      float v_log2[kG][2] = {};  // of the value's scale, NaN for byte 255
       if (KV == kE4m3) {
 #pragma unroll
         for (int t16 = 0; t16 < kG; ++t16)
@@ -732,8 +729,8 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
           for (int j = 0; j < 2; ++j) {
             const uint32_t kb = __shfl_sync(0xffffffffu, kb_lane, 16 * t16 + g + 8 * j);
             const float k_scale = kb == 255u ? __int_as_float(0x7fc00000) : __uint_as_float(kb << 23);
-            v_byte[t16][j] = (int)__shfl_sync(0xffffffffu, vb_lane, 16 * t16 + g + 8 * j);
-            raise_v |= v_byte[t16][j] > v_exp && v_byte[t16][j] != 255;
+            const uint32_t vb = __shfl_sync(0xffffffffu, vb_lane, 16 * t16 + g + 8 * j);
+            v_log2[t16][j] = vb == 255u ? __int_as_float(0x7fc00000) : (float)((int)vb - 127);
 #pragma unroll
             for (int nr = 0; nr < NR; ++nr) {
               s[t16][nr][2 * j] *= k_scale;
@@ -766,21 +763,13 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
 #pragma unroll
         for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) raise |= s[t16][nr][j] > raise_at[nr][j & 1];
-      if (__any_sync(0xffffffffu, raise || raise_v)) {
+          for (int j = 0; j < 4; ++j) {
+            raise |= s[t16][nr][j] > raise_at[nr][j & 1];
+            // (a masked token's -inf raises nothing, whatever its scale)
+            if (KV == kE4m3) raise |= s[t16][nr][j] + v_log2[t16][j >> 1] > mv[nr][j & 1] + kLazy;
+          }
+      if (__any_sync(0xffffffffu, raise)) {
         float o_scale[NR][2];
-        int top = v_exp;
-        if (KV == kE4m3) {
-#pragma unroll
-          for (int t16 = 0; t16 < kG; ++t16)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) top = max(top, v_byte[t16][j] == 255 ? 0 : v_byte[t16][j]);
-#pragma unroll
-          for (int x = 4; x < 32; x <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, x));
-        }
-        // 2^(old - new) of the values' reference exponent
-        const float v_ratio = KV == kE4m3 ? pow2(v_exp - top) : 1.f;
-        if (KV == kE4m3) v_exp = top;
 #pragma unroll
         for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
@@ -797,7 +786,18 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
             l[nr][j] *= f;
             m[nr][j] = mn;
             raise_at[nr][j] = mn + kLazy;
-            o_scale[nr][j] = f * v_ratio;
+            o_scale[nr][j] = f;
+            if (KV == kE4m3) {
+              float top = -INFINITY;
+#pragma unroll
+              for (int t16 = 0; t16 < kG; ++t16)
+                top = fmaxf(top, fmaxf(s[t16][nr][j] + v_log2[t16][0], s[t16][nr][j + 2] + v_log2[t16][1]));
+#pragma unroll
+              for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+              if (!(top > mv[nr][j] + kLazy)) top = mv[nr][j];
+              o_scale[nr][j] = mv[nr][j] == top ? 1.f : exp2_fast(mv[nr][j] - top);
+              mv[nr][j] = top;
+            }
           }
 #pragma unroll
         for (int t = 0; t < D / 16; ++t)
@@ -811,22 +811,19 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
       uint32_t pf[kG][NR][2];
 #pragma unroll
       for (int t16 = 0; t16 < kG; ++t16) {
-        float v_scale[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-          v_scale[j] = KV != kE4m3 ? 1.f
-                       : v_byte[t16][j] == 255 ? __int_as_float(0x7fc00000)
-                                               : pow2(v_byte[t16][j] - v_exp);
 #pragma unroll
         for (int nr = 0; nr < NR; ++nr) {
           float pr[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const float base = m[nr][j & 1] == -INFINITY ? 0.f : m[nr][j & 1];
-            pr[j] = exp2_fast(s[t16][nr][j] - base);
+            const float x = s[t16][nr][j];
+            pr[j] = exp2_fast(x - (m[nr][j & 1] == -INFINITY ? 0.f : m[nr][j & 1]));
             l[nr][j & 1] += pr[j];
-            // a masked token's P is zero whatever its value's scale says
-            if (KV == kE4m3) pr[j] = pr[j] == 0.f ? 0.f : pr[j] * v_scale[j >> 1];
+            // times the value's scale; a masked token's stays zero whatever that holds
+            if (KV == kE4m3) {
+              const float base = mv[nr][j & 1] == -INFINITY ? 0.f : mv[nr][j & 1];
+              pr[j] = x == -INFINITY ? 0.f : exp2_fast(x + v_log2[t16][j >> 1] - base);
+            }
           }
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -945,9 +942,8 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
         const int r = 8 * nr + 2 * c + j;
         float mx = -INFINITY;
         for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, sm.wm[w][r]);
-        float f = m[nr][j] == -INFINITY ? 0.f : exp2_fast(m[nr][j] - mx);
-        // O is in units of 2^(v_exp - 127)
-        if (KV == kE4m3) f *= __uint_as_float((uint32_t)v_exp << 23);
+        const float unit = KV != kE4m3 ? m[nr][j] : mv[nr][j] == -INFINITY ? 0.f : mv[nr][j];
+        const float f = m[nr][j] == -INFINITY ? 0.f : exp2_fast(unit - mx);
 #pragma unroll
         for (int t = 0; t < D / 16; ++t)
 #pragma unroll

@@ -1,12 +1,23 @@
-"""What a row sees and what it does not."""
+"""What a row sees and what it does not: pages freed before a window, and values of
+very different sizes.
+
+Tolerances: P and the output are rounded once each, so an output element is off
+by at most (u_p + u_out + 2 s_err) sum p|v| (u, s_err as in
+test_gpu_attention.py), with the sum of its own column. Below f16's normal range
+P's step is absolute, 2^-24, so each token may add half of that: of an e4m3 cache
+relative to the row's largest P * 2^e, which the kernel keeps at 1 to 2^8, times a
+code of at most 448, where the largest code of a vector is above 224: together
+below 2^-24 of sum p max|v| a token; of an f16 cache 2^-25 max|v|.
+"""
 
 from __future__ import annotations
 
 import pytest
 import torch
 
+from oracle import attention as ref
 from sglang_restomod_b200 import ops
-from tests.test_gpu_attention import BF16, E4M3, F16, build
+from tests.test_gpu_attention import BF16, E4M3, F16, U, build
 
 pytestmark = pytest.mark.gpu
 
@@ -15,6 +26,30 @@ def run(case, max_q, **kw):
     cache, q, table, kv_lens, starts = case[:5]
     return ops.paged_attention(q.cuda(), cache, table.cuda(), kv_lens.cuda(), starts.cuda(), max_q,
                                return_lse=True, **kw)
+
+
+def check_columns(case, max_q, *, window=0, scale=None, products):
+    """The bound of the file's docstring, element by element."""
+    cache, q, table, kv_lens, starts, kc, vc = case
+    scale = q.shape[-1] ** -0.5 if scale is None else scale
+    out, lse = run(case, max_q, window=window, scale=scale)
+    assert ops.attention_status() == 0
+    want, want_lse = ref.paged_attention_ref(q, kc, vc, table, kv_lens, starts, scale, True, window)
+    mag, _ = ref.paged_attention_ref(q, kc, vc.abs(), table, kv_lens, starts, scale, True, window)
+    a = abs(scale) * float(q.double().norm(dim=-1).max()) * \
+        float(torch.nan_to_num(kc).norm(dim=-1).max())
+    s_err = q.shape[-1] * 2.0 ** -22 * a + 2.0 ** -20
+    tol = (U[products] + U[q.dtype] + 2 * s_err) * mag
+    if cache.k_scale is None and products == F16:
+        tol = tol + 2.0 ** -25 * int(kv_lens.max()) * float(torch.nan_to_num(vc).abs().max())
+    elif products == F16:
+        peak = ref.paged_attention_ref(q, kc, vc.abs().amax(-1, keepdim=True).expand_as(vc), table,
+                                       kv_lens, starts, scale, True, window)[0]
+        tol = tol + 2.0 ** -24 * peak * int(kv_lens.max())
+    assert ((out.cpu().double() - want).abs() <= tol).all()
+    seen = torch.isfinite(want_lse)
+    assert torch.equal(torch.isfinite(lse.cpu()), seen)
+    assert ((lse.cpu().double() - want_lse)[seen].abs() <= s_err + 2.0 ** -20 * a).all()
 
 
 @pytest.mark.parametrize("store,q_dtype", [(BF16, BF16), (F16, F16), (E4M3, BF16)])
@@ -32,3 +67,54 @@ def test_pages_before_the_window_may_be_gone(cuda_device, store, q_dtype, dim, p
     got, lse = run(case, q_len, window=window)
     assert ops.attention_status() == 0
     assert torch.equal(got, want) and torch.equal(lse, want_lse)
+
+
+def rewrite(case, s, tokens, k=None, v=None):
+    """Other keys and values for some tokens of sequence s; the float64 values follow."""
+    cache, q, table, kv_lens, starts, kc, vc = case
+    page = cache.page_size
+    t = torch.as_tensor(tokens)
+    slots = (table[s].long()[t // page] * page + t % page).cuda()
+    old_k, old_v = ops.kv_cache_read(cache, slots, q.dtype)
+    ops.kv_cache_write(cache, old_k if k is None else k.cuda(), old_v if v is None else v.cuda(), slots)
+    if cache.k_scale is not None:
+        kc = ref.kv_values_ref(cache.k.cpu(), cache.k_scale.cpu())
+        vc = ref.kv_values_ref(cache.v.cpu(), cache.v_scale.cpu())
+    else:
+        kc, vc = cache.k.cpu().double(), cache.v.cpu().double()
+    return cache, q, table, kv_lens, starts, kc, vc
+
+
+@pytest.mark.parametrize("q_dtype", [BF16, F16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("page", [1, 8, 16, 64])
+@pytest.mark.parametrize("byte", [134, 254])
+@pytest.mark.parametrize("q_len,groups", [(1, 8), (3, 4)])
+def test_stale_scales_before_the_window(cuda_device, q_dtype, dim, page, byte, q_len, groups):
+    """A token that no row sees does not touch what the others contribute,
+    whatever its scale bytes hold."""
+    window, kv = 53, 331
+    case = build(dim + page, [q_len, 1], [kv, 20], 2, groups, dim, page, q_dtype, E4M3)
+    cache, table = case[0], case[2]
+    for t in range(kv - q_len - window + 1):
+        at = (table[0, t // page].item(), t % page)
+        cache.k_scale[at] = cache.v_scale[at] = byte
+    check_columns(case, q_len, window=window, products=F16)
+
+
+@pytest.mark.parametrize("q_dtype,store", [(BF16, E4M3), (F16, E4M3), (BF16, BF16)])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("page", [1, 16])
+@pytest.mark.parametrize("q_len,groups,kv", [(1, 8, 200), (2, 8, 200), (1, 1, 9001)])
+def test_large_value_of_no_weight(cuda_device, q_dtype, store, dim, page, q_len, groups, kv):
+    """One value 2^25 times the others whose weight is e^-60 or so: the others
+    keep their bits."""
+    case = build(dim + page, [q_len], [kv], 1, groups, dim, page, q_dtype, store)
+    cache, q = case[0], case[1]
+    g = torch.Generator().manual_seed(5)
+    q[:] = q.abs()  # so that one key is far from all queries
+    case = rewrite(case, 0, range(kv), v=torch.randn(kv, 1, dim, generator=g).to(q_dtype) * 2.0 ** -14)
+    far = torch.full((1, 1, dim), -80.0 / dim ** 0.5, dtype=q_dtype)
+    # |q| has a mean of 0.8, so q . far * scale is about -0.8 dim 80 / dim = -64
+    case = rewrite(case, 0, [5], k=far, v=torch.full((1, 1, dim), 2.0 ** 11, dtype=q_dtype))
+    check_columns(case, q_len, products=F16 if store == E4M3 else q_dtype)
