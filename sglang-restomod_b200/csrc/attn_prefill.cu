@@ -80,6 +80,9 @@ constexpr int kMinTiles = 4;
 // prompt of 8192 tokens takes 570, 515, 527 us, 16 mixed chunks 61, 56, 66, 512
 // tokens on 16384 e4m3 ones 169, 166, 164.
 constexpr int kUnitCost = 2;
+// A masked score is an infinity that the scale multiplies, so a scale of zero
+// becomes the smallest normal number: finite scores still come to e^0.
+constexpr float kMinScale = 1.1754944e-38f;
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kTmemO = 256;  // O after the two S buffers of up to 128 columns
 
@@ -838,6 +841,8 @@ __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
     uint32_t step = 0;                              // S tiles of this warpgroup so far
     uint32_t segment = 0;                           // segments so far
     uint64_t* pv_done = &ctl->pv_done[MT == 2 ? wg : 0];  // one phase per step
+    // of all rows' scales: the passes over S are taken by whole warps
+    const bool negative = p.scale_log2 < 0.f;
     while (cur.next(g)) {
       const SeqLens q = seq_lens(a, g.seq);
       const int tok = g.tok0 + wg * p.tile_tokens + row_token;
@@ -856,6 +861,8 @@ __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
           wait_bar(&ctl->q_scaled[segment & 1u], segment >> 1 & 1u, ctl, a.status);
         named_bar_sync(2 + wg, 128);
         scale *= ctl->q_scale[segment & 1u][wg][row];
+        // (a row of zeros has 2^-126, and the product may come to zero)
+        scale = negative ? fminf(scale, -kMinScale) : fmaxf(scale, kMinScale);
       }
       ++segment;
       const uint32_t to = lane_addr + kTmemO + (MT == 2 ? wg * D : 0);
@@ -872,9 +879,9 @@ __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
         uint32_t s[S::kRowInRegs ? BN : 32];  // the row's S, read once
         if constexpr (S::kRowInRegs) {
           load_row<BN>(ts, s);
-          if (masked) mask_row<BN>(s, col0, lo, hi, scale >= 0.f ? -INFINITY : INFINITY);
-          top = scale >= 0.f ? max_row<BN, false>(s) : max_row<BN, true>(s);
-        } else if (scale >= 0.f)
+          if (masked) mask_row<BN>(s, col0, lo, hi, negative ? INFINITY : -INFINITY);
+          top = negative ? max_row<BN, true>(s) : max_row<BN, false>(s);
+        } else if (!negative)
           top = masked ? max_pass<BN, true, false>(ts, col0, lo, hi)
                        : max_pass<BN, false, false>(ts, col0, lo, hi);
         else
@@ -1542,9 +1549,7 @@ cudaError_t launch_attn_prefill(const AttnLaunch& l, cudaStream_t stream) {
   p.a = l;
   p.groups = l.q_heads / l.c.heads;
   p.tile_tokens = 128 / p.groups;
-  // A masked score is an infinity that the scale multiplies, so a scale of zero
-  // becomes the smallest normal number: finite scores still come to e^0.
-  p.scale_log2 = l.scale == 0.f ? 1.1754944e-38f : l.scale * kLog2e;
+  p.scale_log2 = l.scale == 0.f ? kMinScale : l.scale * kLog2e;
   p.box_rows = 1;
   p.page_shift = (l.c.page_size & (l.c.page_size - 1)) == 0 ? __builtin_ctz(l.c.page_size) : -1;
   const long long sms = device_sm_count();

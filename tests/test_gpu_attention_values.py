@@ -118,3 +118,16 @@ def test_large_value_of_no_weight(cuda_device, q_dtype, store, dim, page, q_len,
     # |q| has a mean of 0.8, so q . far * scale is about -0.8 dim 80 / dim = -64
     case = rewrite(case, 0, [5], k=far, v=torch.full((1, 1, dim), 2.0 ** 11, dtype=q_dtype))
     check_columns(case, q_len, products=F16 if store == E4M3 else q_dtype)
+
+
+@pytest.mark.parametrize("q_dtype", [BF16, F16])
+@pytest.mark.parametrize("page", [1, 16])
+@pytest.mark.parametrize("q_len,groups", [(1, 8), (40, 4), (150, 4)])
+@pytest.mark.parametrize("scale", [0.0, 1e-30, -1e-30, 0.09])
+@pytest.mark.parametrize("size", [0.0, 2.0 ** -120])
+def test_queries_of_no_size(cuda_device, q_dtype, page, q_len, groups, scale, size):
+    """Rows of zeros and of tiny values, over an e4m3 cache: every score is about
+    zero, so that each row is the mean of what it sees."""
+    case = build(q_len, [q_len, 2], [q_len + 190, 2], 1, groups, 128, page, q_dtype, E4M3)
+    case[1][::2] *= size
+    check_columns(case, max(q_len, 2), scale=scale, products=F16)
