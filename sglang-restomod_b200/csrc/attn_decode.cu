@@ -82,7 +82,8 @@ struct __align__(16) TileInfo {
   int seq, head;      // seq < 0: past the block's range
   int token0;         // first token
   int end;            // tokens from here on do not exist
-  int q0, q_len;      // the sequence's new tokens
+  int q0, q_len;      // the sequence's new tokens that the call takes
+  int pos0;           // position of the first of them
   int tile, tiles;    // of the pair
   int left;           // this block's tiles of the pair from here on
   int pair;           // pairs of this block before it
@@ -206,7 +207,7 @@ __device__ __forceinline__ int merge_col(int d, int c) {
 // A sequence with new tokens always has one tile, so that its rows are written
 // even where nothing is cached.
 struct SeqRange {
-  int begin, end, q0, q_len, kv_len, tiles;
+  int begin, end, q0, q_len, pos0, tiles;
 };
 template <int kTile>
 __device__ __forceinline__ SeqRange seq_range(const AttnLaunch& a, int s, int align) {
@@ -216,21 +217,22 @@ __device__ __forceinline__ SeqRange seq_range(const AttnLaunch& a, int s, int al
   int kv = __ldg(a.kv_lens + s);
   kv = kv < 0 ? 0 : kv;
   if (kv > cap) kv = (int)cap;
-  int ql = q1 - q0;
-  if (q0 < 0 || q1 > a.q_tokens) ql = 0;  // outside q: nothing is read or written
-  ql = ql < 0 ? 0 : (ql > a.max_q ? a.max_q : ql);
+  int n = q1 - q0;
+  if (q0 < 0 || q1 > a.q_tokens) n = 0;  // outside q: nothing is read or written
+  n = n < 0 ? 0 : n;
+  const int ql = n > a.max_q ? a.max_q : n;
   r.q0 = q0;
   r.q_len = ql;
-  r.kv_len = kv;
-  r.end = kv;
+  r.pos0 = kv - n;  // new tokens past max_q keep their places, unread and unwritten
+  r.end = a.causal && n > ql ? max(r.pos0 + ql, 0) : kv;
   r.begin = 0;
   if (a.window > 0) {
-    const long long b = (long long)kv - ql - a.window + 1;  // first token the first row sees
+    const long long b = (long long)r.pos0 - a.window + 1;  // first token the first row sees
     r.begin = b > 0 ? (int)b : 0;
     r.begin -= r.begin % align;  // a copy's border
   }
-  const int n = r.end - r.begin;
-  r.tiles = ql == 0 ? 0 : (n <= 0 ? 1 : (n + kTile - 1) / kTile);
+  const int keys = r.end - r.begin;
+  r.tiles = ql == 0 ? 0 : (keys <= 0 ? 1 : (keys + kTile - 1) / kTile);
   return r;
 }
 
@@ -350,6 +352,7 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
       ti.end = range.end;
       ti.q0 = range.q0;
       ti.q_len = range.q_len;
+      ti.pos0 = range.pos0;
       ti.left = (int)min((long long)(range.tiles - ti.tile), t1 - at);
       ti.pair_at = at - x;
       if (ti.tile == 0 || pair < 0) ++pair;
@@ -601,7 +604,7 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
         const int r = 8 * nr + 2 * c + j;
         row_scale[nr][j] = p.scale_log2 * (KV == kE4m3 && !a.q_f16 ? sm.row_scale[r] : 1.f);
         // tokens row r sees: [row_lo, row_hi)
-        const int pos = first.end - first.q_len + r / p.groups;
+        const int pos = first.pos0 + r / p.groups;
         row_hi[nr][j] = r >= rows ? 0 : a.causal ? min(first.end, pos + 1) : first.end;
         row_lo[nr][j] = a.window > 0 ? max(0, pos - a.window + 1) : 0;
         m[nr][j] = -INFINITY;
@@ -619,7 +622,7 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
       all_hi = min(all_hi, __shfl_xor_sync(0xffffffffu, all_hi, x));
     }
     // the first token that any row sees
-    const int lowest = a.window > 0 ? first.end - first.q_len - a.window + 1 : 0;
+    const int lowest = a.window > 0 ? first.pos0 - a.window + 1 : 0;
 #pragma unroll
     for (int t = 0; t < D / 16; ++t)
 #pragma unroll

@@ -345,9 +345,11 @@ __device__ __forceinline__ uint32_t factor_of(uint32_t byte) {
 }
 
 // ------------------------------------------------------------------- plan
-// New tokens and cached tokens of a sequence, within the call's bounds.
+// New tokens and cached tokens of a sequence, within the call's bounds: new ones
+// past max_q keep their places, unread and unwritten.
 struct SeqLens {
   int q0, q_len, kv_len;
+  int pos0;  // position of the first new token
 };
 __device__ __forceinline__ SeqLens seq_lens(const AttnLaunch& a, int s) {
   SeqLens r;
@@ -358,8 +360,10 @@ __device__ __forceinline__ SeqLens seq_lens(const AttnLaunch& a, int s) {
   int n = q1 - q0;
   if (q0 < 0 || q1 > a.q_tokens) n = 0;  // outside q: nothing is read or written
   r.q0 = q0;
-  r.q_len = min(max(n, 0), a.max_q);
+  n = max(n, 0);
+  r.q_len = min(n, a.max_q);
   r.kv_len = kv;
+  r.pos0 = kv - n;
   return r;
 }
 
@@ -441,9 +445,8 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const PrefillPa
       while (s + 1 < a.seqs && seq_base[s + 1] <= u) q = seq_lens(a, ++s);
       const int tok0 = (u - seq_base[s]) * unit_tokens;
       const int last = min(tok0 + unit_tokens, q.q_len) - 1;
-      const int shift = q.kv_len - q.q_len;
-      int end = a.causal ? min(q.kv_len, shift + last + 1) : q.kv_len;
-      int begin = a.window > 0 ? max(0, shift + tok0 - a.window + 1) : 0;
+      int end = a.causal ? min(q.kv_len, q.pos0 + last + 1) : q.kv_len;
+      int begin = a.window > 0 ? max(0, q.pos0 + tok0 - a.window + 1) : 0;
       begin -= begin % p.box_rows;
       const int tiles = end > begin ? (end - begin + bn - 1) / bn : 1;
       p.units[u] = make_int4(s, tok0, begin, tiles);
@@ -848,7 +851,7 @@ __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
       const int tok = g.tok0 + wg * p.tile_tokens + row_token;
       const bool valid = row < p.tile_tokens * p.groups && tok < q.q_len &&
                          tok < g.tok0 + MT * p.tile_tokens;
-      const int pos = q.kv_len - q.q_len + tok;
+      const int pos = q.pos0 + tok;
       const int hi = !valid ? 0 : a.causal ? min(q.kv_len, pos + 1) : q.kv_len;
       const int lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
       // a row that sees nothing needs no maximum: every key is masked
@@ -1338,7 +1341,7 @@ __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
       while (cur.next(g)) {
         const SeqLens q = seq_lens(a, g.seq);
         // the first key that any row of the unit sees
-        const int lowest = a.window > 0 ? q.kv_len - q.q_len + g.tok0 - a.window + 1 : 0;
+        const int lowest = a.window > 0 ? q.pos0 + g.tok0 - a.window + 1 : 0;
         for (int n = 0; n < 2 * g.tiles; ++n) {
           int seen_from = 0, seen_to = BN;
           if (TMA) {

@@ -17,7 +17,7 @@ import torch
 
 from oracle import attention as ref
 from sglang_restomod_b200 import ops
-from tests.test_gpu_attention import BF16, E4M3, F16, U, build
+from tests.test_gpu_attention import BF16, E4M3, F16, U, bounds, build
 
 pytestmark = pytest.mark.gpu
 
@@ -131,3 +131,26 @@ def test_queries_of_no_size(cuda_device, q_dtype, page, q_len, groups, scale, si
     case = build(q_len, [q_len, 2], [q_len + 190, 2], 1, groups, 128, page, q_dtype, E4M3)
     case[1][::2] *= size
     check_columns(case, max(q_len, 2), scale=scale, products=F16)
+
+
+@pytest.mark.parametrize("q_dtype,store", [(BF16, BF16), (F16, F16), (BF16, E4M3)])
+@pytest.mark.parametrize("page", [1, 16])
+@pytest.mark.parametrize("window", [0, 21])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("q_len,max_q,groups", [(4, 2, 4), (9, 1, 8), (90, 50, 4), (700, 300, 2)])
+def test_more_new_tokens_than_the_call_takes(cuda_device, q_dtype, store, page, window, causal, q_len,
+                                             max_q, groups):
+    """The first max_q_len new tokens of a sequence see what they see in a call
+    that takes all of them; the others are left as they were."""
+    if window and not causal:
+        return
+    case = build(q_len, [q_len, 1, 3], [q_len + 100, 40, 3], 1, groups, 128, page, q_dtype, store)
+    cache, q, table, kv_lens, starts, kc, vc = case
+    out = torch.full(q.shape, 7.0, dtype=q_dtype, device="cuda")
+    run(case, max_q, window=window, causal=causal, out=out)
+    want, _ = ref.paged_attention_ref(q, kc, vc, table, kv_lens, starts, 128 ** -0.5, causal, window)
+    tol, _ = bounds(q, kc, vc, 128 ** -0.5, q_dtype, q_dtype)
+    for a, n in zip(starts.tolist(), (q_len, 1, 3)):
+        took = min(n, max_q)
+        assert (out[a:a + took].cpu().double() - want[a:a + took]).abs().max().item() <= tol
+        assert (out[a + took:a + n] == 7.0).all()
