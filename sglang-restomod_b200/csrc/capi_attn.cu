@@ -259,7 +259,9 @@ int b200_paged_attention(const b200_kv_cache* cache, const void* q, int32_t dtyp
   l.q_heads = q_heads;
   l.scale = scale;
   l.causal = causal != 0;
-  l.window = window;
+  // A window as wide as the table is none; the kernels' positions then stay above
+  // -2^31 (new tokens may outnumber the cached ones, and the first lie below zero).
+  l.window = window < (int64_t)page_table_width * cache->page_size ? window : 0;
   l.out = out;
   l.out_token_stride = out_token_stride;
   l.out_head_stride = out_head_stride;

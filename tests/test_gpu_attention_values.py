@@ -154,3 +154,18 @@ def test_more_new_tokens_than_the_call_takes(cuda_device, q_dtype, store, page, 
         took = min(n, max_q)
         assert (out[a:a + took].cpu().double() - want[a:a + took]).abs().max().item() <= tol
         assert (out[a + took:a + n] == 7.0).all()
+
+
+@pytest.mark.parametrize("store", [BF16, E4M3])
+@pytest.mark.parametrize("page", [1, 16])
+@pytest.mark.parametrize("q_len,groups", [(4, 2), (40, 4), (300, 2)])
+@pytest.mark.parametrize("window", [(1 << 31) - 1, 1 << 30, 160, 320])
+def test_windows_beyond_the_table(cuda_device, store, page, q_len, groups, window):
+    """A window wider than anything cached is no window, also where new tokens
+    outnumber the cached ones and the first of them see nothing."""
+    case = build(q_len, [q_len, 2], [q_len - 3, 9], 1, groups, 128, page, BF16, store)
+    want, want_lse = run(case, q_len)
+    got, lse = run(case, q_len, window=window)
+    if window > q_len:
+        assert torch.equal(got, want) and torch.equal(lse, want_lse)
+    check_columns(case, q_len, window=window, products=F16 if store == E4M3 else BF16)
