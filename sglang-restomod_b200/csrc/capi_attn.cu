@@ -226,7 +226,9 @@ int b200_paged_attention(const b200_kv_cache* cache, const void* q, int32_t dtyp
     return fail(B200_ERR_INVALID, "negative or too large count");
   if (window < 0 || (window > 0 && !causal))
     return fail(B200_ERR_INVALID, "a window needs causal attention and at least one token");
-  if (!std::isfinite(scale)) return fail(B200_ERR_INVALID, "the scale must be finite");
+  // (in units of log2, as the kernels use it)
+  if (!std::isfinite(scale * 1.4426950408889634f))
+    return fail(B200_ERR_INVALID, "the scale must be finite");
   if (seqs == 0 || q_tokens == 0 || max_q_len == 0) return B200_OK;
   if ((rc = check_rows("q", q, q_token_stride, q_head_stride))) return rc;
   if ((rc = check_rows("out", out, out_token_stride, out_head_stride))) return rc;

@@ -169,3 +169,14 @@ def test_windows_beyond_the_table(cuda_device, store, page, q_len, groups, windo
     if window > q_len:
         assert torch.equal(got, want) and torch.equal(lse, want_lse)
     check_columns(case, q_len, window=window, products=F16 if store == E4M3 else BF16)
+
+
+@pytest.mark.parametrize("q_len", [1, 150])
+@pytest.mark.parametrize("store", [BF16, E4M3])
+def test_scales_beyond_fp32(cuda_device, store, q_len):
+    """The kernels take the scale in units of log2, where it must be finite too."""
+    case = build(3, [q_len], [q_len + 5], 1, 4, 64, 16, BF16, store)
+    with pytest.raises(RuntimeError, match="finite"):
+        run(case, q_len, scale=3e38)
+    case[1].zero_()
+    check_columns(case, q_len, scale=2e38, products=F16 if store == E4M3 else BF16)
