@@ -65,9 +65,18 @@ int b200_num_sms(void);
  * Device-side error bits recorded in a workspace (1 = a pipeline wait timed
  * out, 2 = an expert id >= E reached a GEMM, 4 = a route pointed past the
  * activation rows, 16 = a page number outside the key/value cache) or an
- * expert-parallel region (8 = a wait on another rank timed out). Synchronizes `stream`; clears the bits when reset != 0.
+ * expert-parallel region (8 = a wait on another rank timed out). Synchronizes
+ * `stream`; clears the bits when reset != 0.
  */
 int b200_workspace_status(void* workspace, int32_t* bits, int32_t reset, void* stream);
+
+/*
+ * The same bits of all norm and attention calls on the current device since they
+ * were last cleared: those without a workspace, and those whose workspace is
+ * gone or lies in a captured graph. Attention records its bits in its call's
+ * workspace too. Synchronizes `stream`; order it after the calls.
+ */
+int b200_device_status(int32_t* bits, int32_t reset, void* stream);
 
 /* ---------------------------------------------------------------- routing */
 

@@ -444,7 +444,7 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
           } else {
             // past the last key, or no page of the cache: from past the maps'
             // end, which gives zeros
-            if (token < ti.end) atomicOr(a.status, kDevBadPage);
+            if (token < ti.end) report(a.status, kDevBadPage);
             page = (int)a.c.num_pages;
           }
           const int y = p.heads_first ? ti.head : row, z = p.heads_first ? row : ti.head;
@@ -471,7 +471,7 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
                         (token - page_of(token) * a.c.page_size) * a.c.token_stride +
                         ti.head * a.c.head_stride) * S::kElem;
             else
-              atomicOr(a.status, kDevBadPage);
+              report(a.status, kDevBadPage);
           }
         }
         constexpr int kPerPass = 32 / kChunks;  // rows per instruction

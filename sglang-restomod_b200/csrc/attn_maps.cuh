@@ -1,11 +1,22 @@
-// Tensor maps of a paged key/value cache for the attention kernels' tensor
-// copies, and the copies.
+// What the attention kernels share: tensor maps of a paged key/value cache and
+// the copies, and how errors are recorded.
 #pragma once
 
+#include "common.cuh"
 #include "internal.h"
 #include "tcgen05.cuh"
 
 namespace b200 {
+
+__device__ __forceinline__ void report(const StatusWords& s, int bits) {
+  atomicOr(s.call, bits);
+  atomicOr(s.device, bits);
+}
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, const StatusWords& s) {
+  if (mbar_wait(bar, parity, static_cast<int*>(nullptr))) return true;
+  report(s, kDevWaitTimeout);
+  return false;
+}
 
 // One box of a 4-D map at (x, y, z, w); completion as transaction bytes.
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z,

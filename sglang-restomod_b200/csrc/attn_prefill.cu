@@ -196,13 +196,14 @@ __device__ __forceinline__ bool try_wait_long(uint64_t* bar, uint32_t parity) {
 // Bounded wait. A role that gives up sets the block's abort flag; from then on
 // no wait waits, so every role runs through its loops (and block barriers) and
 // the block ends with the status bit set.
-__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, Ctl* ctl, int* status) {
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, Ctl* ctl,
+                                         const StatusWords& status) {
   if (try_wait_long(bar, parity)) return true;
   const unsigned long long t0 = global_timer_ns();
   while (!*reinterpret_cast<volatile int*>(&ctl->abort)) {
     if (try_wait_long(bar, parity)) return true;
     if (global_timer_ns() - t0 > kWaitLimitNs) {
-      atomicOr(status, kDevWaitTimeout);
+      report(status, kDevWaitTimeout);
       *reinterpret_cast<volatile int*>(&ctl->abort) = 1;
     }
   }
@@ -1029,7 +1030,7 @@ __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
           const int token = g.begin + (g.tile0 + t) * BN + lane * p.box_rows;
           int at = token - p.page_of(token) * a.c.page_size;
           if (pg < 0 || pg >= a.c.num_pages) {
-            if (token < q.kv_len) atomicOr(a.status, kDevBadPage);
+            if (token < q.kv_len) report(a.status, kDevBadPage);
             pg = (int)a.c.num_pages;
             at = 0;
           }
@@ -1109,7 +1110,7 @@ __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
       const int token = sg.begin + (sg.tile0 + t) * BN + pt;
       if (t < sg.tiles && pt < BN && token < kv_len) {
         if (page < 0 || page >= a.c.num_pages) {
-          atomicOr(a.status, kDevBadPage);
+          report(a.status, kDevBadPage);
         } else {
           const int at = token - p.page_of(token) * a.c.page_size;
           r.off = (page * a.c.page_stride + at * a.c.token_stride + sg.head * a.c.head_stride) *

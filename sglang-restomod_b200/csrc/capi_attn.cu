@@ -27,6 +27,25 @@ int check_cuda(cudaError_t err, const char* what) {
   return fail(B200_ERR_CUDA, "%s: %s", what, cudaGetErrorString(err));
 }
 
+// The current device's status word (its address is looked up once per device).
+__device__ int g_status;
+int status_word(int** out) {
+  static std::mutex mu;
+  static int* words[64] = {};
+  int dev = 0;
+  int rc = check_cuda(cudaGetDevice(&dev), "current device");
+  if (rc) return rc;
+  if (dev < 0 || dev >= 64) return fail(B200_ERR_CUDA, "device %d", dev);
+  const std::lock_guard<std::mutex> lock(mu);
+  if (words[dev] == nullptr) {
+    void* p = nullptr;
+    if ((rc = check_cuda(cudaGetSymbolAddress(&p, g_status), "status word"))) return rc;
+    words[dev] = static_cast<int*>(p);
+  }
+  *out = words[dev];
+  return B200_OK;
+}
+
 bool aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 bool valid_dtype16(int32_t d) { return d == B200_DTYPE_BF16 || d == B200_DTYPE_F16; }
 
@@ -107,6 +126,13 @@ int check_copy(const b200_kv_cache* c, int32_t dtype, const int64_t* slots, int6
 }  // namespace
 
 extern "C" {
+
+int b200_device_status(int32_t* bits, int32_t reset, void* stream) {
+  if (bits == nullptr) return fail(B200_ERR_INVALID, "null pointer argument");
+  int* word = nullptr;
+  const int rc = status_word(&word);
+  return rc ? rc : b200_workspace_status(word, bits, reset, stream);
+}
 
 int b200_add_rms_norm(const void* x, int32_t dtype, int64_t x_ld, int64_t rows, int64_t hidden,
                       const void* residual, int64_t residual_ld, const void* weight,
@@ -269,7 +295,8 @@ int b200_paged_attention(const b200_kv_cache* cache, const void* q, int32_t dtyp
   l.out_head_stride = out_head_stride;
   l.lse = lse;
   uint8_t* base = static_cast<uint8_t*>(workspace);
-  l.status = reinterpret_cast<int*>(base);
+  l.status.call = reinterpret_cast<int*>(base);
+  if ((rc = status_word(&l.status.device))) return rc;
   l.counters = reinterpret_cast<int*>(base + ws_counter_offset());
   l.scratch = base + fixed;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);

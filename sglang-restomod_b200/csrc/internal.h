@@ -299,6 +299,14 @@ cudaError_t launch_kv_read(const KvCacheView& c, void* k, void* v, bool f16,
                            long long token_stride, long long head_stride, const long long* slots,
                            long long tokens, cudaStream_t stream);
 
+// Where a kernel records its error bits: in the call's workspace, and in a word
+// that the library keeps per device, which outlives workspaces and serves calls
+// that have none and calls replayed from a graph.
+struct StatusWords {
+  int* call;
+  int* device;
+};
+
 // Attention of the last q_starts[s + 1] - q_starts[s] tokens of each sequence
 // over its kv_lens[s] cached ones (attn_decode.cu, attn_prefill.cu).
 struct AttnLaunch {
@@ -318,7 +326,7 @@ struct AttnLaunch {
   void* out;           // type of q
   long long out_token_stride, out_head_stride;
   float* lse;          // [q_tokens][q_heads] or nullptr
-  int* status;
+  StatusWords status;
   int* counters;       // the workspace's 1024 arrival counters, zero between calls
   uint8_t* scratch;
 };

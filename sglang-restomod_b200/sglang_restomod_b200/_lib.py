@@ -54,6 +54,7 @@ SIGNATURES = {
     "b200_last_error": (ctypes.c_char_p, []),
     "b200_num_sms": (c_int32, []),
     "b200_workspace_status": (c_int32, [c_void_p, ctypes.POINTER(c_int32), c_int32, c_void_p]),
+    "b200_device_status": (c_int32, [ctypes.POINTER(c_int32), c_int32, c_void_p]),
     "b200_moe_align_block_size": (
         c_int32,
         [c_void_p, c_int64, c_int32, c_int32, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p],

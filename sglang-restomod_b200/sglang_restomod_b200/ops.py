@@ -928,18 +928,15 @@ def reserve_attention_workspace(head_dim: int, q_tokens: int, seqs: int,
 
 
 def attention_status(device: torch.device | None = None, reset: bool = True) -> int:
-    """Error bits of the attention calls on a device's streams (0 = none, 16 = a
-    page number outside the cache). Synchronizes the device."""
+    """Error bits of a device's norm and attention calls, those replayed from graphs
+    included (0 = none, 1 = a wait gave up, 16 = a page number outside the cache).
+    Synchronizes the device."""
     index = torch.cuda.current_device() if device is None or device.index is None else device.index
     torch.cuda.synchronize(index)
-    bits = 0
-    for (at, stream), ws in list(_ATTN_WORKSPACES.items()):
-        if at == index:
-            word = ctypes.c_int32(0)
-            _lib.check(lib().b200_workspace_status(_vp(ws), ctypes.byref(word), int(reset),
-                                                   ctypes.c_void_p(stream)))
-            bits |= int(word.value)
-    return bits
+    bits = ctypes.c_int32(0)
+    with torch.cuda.device(index):
+        _lib.check(lib().b200_device_status(ctypes.byref(bits), int(reset), _raw_stream(index)))
+    return int(bits.value)
 
 
 def paged_attention(q: torch.Tensor, cache, page_table: torch.Tensor, kv_lens: torch.Tensor,

@@ -3,7 +3,11 @@ bits, workspaces."""
 
 from __future__ import annotations
 
+import os
+import subprocess
+import sys
 import threading
+from pathlib import Path
 
 import pytest
 import torch
@@ -68,3 +72,70 @@ def test_threads_on_one_stream(cuda_device):
         t.join(60)
     assert len(wrong) == 60 * len(calls) and not any(wrong)
     assert ops.attention_status() == 0
+
+
+@pytest.mark.parametrize("store", [BF16, E4M3])
+@pytest.mark.parametrize("q_len", [1, 40])
+@pytest.mark.parametrize("reserved", [False, True])
+def test_errors_of_replayed_graphs_are_seen(cuda_device, store, q_len, reserved):
+    cache, q, table, kv_lens, starts = build(45, [q_len, 1], [90, 33], 1, 4, 64, 16, BF16, store)[:5]
+    args = (q.cuda(), cache, table.cuda(), kv_lens.cuda(), starts.cuda(), q_len)
+    ops.paged_attention(*args)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    if reserved:
+        with torch.cuda.stream(side):
+            ops.reserve_attention_workspace(64, q.shape[0], 2)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        out = ops.paged_attention(*args)
+    graph.replay()
+    assert ops.attention_status() == 0
+    want = out.clone()
+    args[2][1, 0] = cache.num_pages + 7
+    graph.replay()
+    assert ops.attention_status(reset=False) == 16
+    assert ops.attention_status() == 16
+    assert ops.attention_status() == 0
+    args[2][1, 0] = table[1, 0].item()
+    graph.replay()
+    assert ops.attention_status() == 0 and torch.equal(out, want)
+
+
+def test_errors_outlive_their_workspace(cuda_device):
+    cache, q, table, kv_lens, starts = build(46, [1, 1], [90, 33], 1, 4, 64, 16, BF16, BF16)[:5]
+    ws = torch.zeros(ops.paged_attention_workspace_bytes(64, 2, 2), dtype=torch.uint8, device="cuda")
+    bad = table.cuda()
+    bad[0, 2] = -1
+    ops.paged_attention(q.cuda(), cache, bad, kv_lens.cuda(), starts.cuda(), 1, workspace=ws)
+    assert int(ws[:4].view(torch.int32)) == 16  # the call's own word has it too
+    del ws
+    assert ops.attention_status() == 16 and ops.attention_status() == 0
+
+
+FIRST_CALL_IN_A_CAPTURE = """
+import torch
+from sglang_restomod_b200 import kv_cache, ops
+x = torch.ones(3, 7168, dtype=torch.bfloat16, device="cuda")
+w = torch.ones(7168, dtype=torch.bfloat16, device="cuda")
+cache = kv_cache.PagedKVCache.empty(4, 16, 1, 64, "cuda", torch.bfloat16)
+cache.k.zero_(), cache.v.zero_()
+i32 = dict(dtype=torch.int32, device="cuda")
+q = torch.ones(3, 4, 64, dtype=torch.bfloat16, device="cuda")
+args = torch.zeros(3, 1, **i32), torch.ones(3, **i32), torch.arange(4, **i32), 1
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y, _ = ops.add_rms_norm(x, w)
+    o = ops.paged_attention(q, cache, *args)
+graph.replay()
+torch.cuda.synchronize()
+assert (y == 1).all() and (o == 0).all() and ops.attention_status() == 0
+"""
+
+
+def test_first_call_of_a_process_in_a_capture(cuda_device):
+    env = {**os.environ, "PYTHONPATH": str(Path(ops.__file__).resolve().parents[1])}
+    done = subprocess.run([sys.executable, "-c", FIRST_CALL_IN_A_CAPTURE], env=env,
+                          capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr
