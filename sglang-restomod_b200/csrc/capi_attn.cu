@@ -188,6 +188,8 @@ int b200_add_rms_norm(const void* x, int32_t dtype, int64_t x_ld, int64_t rows, 
   l.weight_dtype = weight_dtype;
   l.eps = eps;
   l.weight_bias = weight_bias;
+  const int rc = status_word(&l.status);
+  if (rc) return rc;
   return check_cuda(launch_add_rms_norm(l, reinterpret_cast<cudaStream_t>(stream)), "RMS norm launch");
 }
 

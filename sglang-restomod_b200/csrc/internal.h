@@ -273,6 +273,7 @@ struct NormLaunch {
   int f16;
   int weight_dtype;  // 0 bf16, 1 f16, 2 f32
   float eps, weight_bias;
+  int* status;       // the device's status word
 };
 cudaError_t launch_add_rms_norm(const NormLaunch& l, cudaStream_t stream);
 long long norm_max_hidden();

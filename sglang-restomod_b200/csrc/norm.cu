@@ -39,6 +39,7 @@ struct NormParams {
   int h8;                // 16-byte vectors per row
   int weight_dtype;      // 0 bf16, 1 f16, 2 f32
   float eps, weight_bias, inv_hidden;
+  int* status;           // the device's status word
 };
 
 template <bool F16>
@@ -300,9 +301,7 @@ __global__ void __launch_bounds__(1024) add_rms_norm_kernel(NormParams p, int st
     for (int i = 0; i < stages; ++i) issue(blockIdx.x + i * step, i);
   int stage = 0, phase = 0, parity = 0;
   for (long long row = blockIdx.x; row < p.rows; row += step, parity ^= 1) {
-    // Bounded: a copy that never lands leaves its row's outputs wrong, not the
-    // kernel hanging.
-    mbar_wait(&full[stage], (uint32_t)phase, nullptr);
+    mbar_wait(&full[stage], (uint32_t)phase, tid == 0 ? p.status : nullptr);
     const uint4* xs = reinterpret_cast<const uint4*>(ring + stage * stage_bytes);
     uint64_t h[V][4];
     float sum = 0.f;
@@ -415,6 +414,7 @@ cudaError_t launch_add_rms_norm(const NormLaunch& l, cudaStream_t stream) {
   p.eps = l.eps;
   p.weight_bias = l.weight_bias;
   p.inv_hidden = 1.f / (float)l.hidden;
+  p.status = l.status;
   return l.f16 ? launch<true>(p, stream) : launch<false>(p, stream);
 }
 
