@@ -882,9 +882,12 @@ def kv_cache_read(cache, slots: torch.Tensor, dtype: torch.dtype | None = None):
 # overlap, and its arrival counters and partial sums must not.
 _ATTN_WORKSPACES: dict[tuple[int, int], torch.Tensor] = {}
 _ATTN_BYTES: dict[tuple[int, int, int], int] = {}
-# Workspaces that a larger one has replaced: a captured graph may still use
-# them. Sizes grow by powers of two, so together they are below the present one.
+# Workspaces that a larger one has replaced, kept because a captured graph may still
+# use them. Each is at most half of the one after it, so a stream's together are
+# below its present one. (Nearly all of a workspace is its partial results, a
+# constant: 20 to 40 MB by head_dim, and 16 bytes a token.)
 _ATTN_OUTGROWN: list[torch.Tensor] = []
+_ATTN_MIN_TOKENS, _ATTN_MIN_SEQS = 16384, 4096
 
 
 def paged_attention_workspace_bytes(head_dim: int, q_tokens: int, seqs: int) -> int:
@@ -895,8 +898,10 @@ def paged_attention_workspace_bytes(head_dim: int, q_tokens: int, seqs: int) -> 
 
 
 def _attn_workspace(index: int, stream: int, head_dim: int, q_tokens: int, seqs: int):
-    # Sizes are asked for rounded up, so few distinct ones are kept.
-    key = (head_dim, 1 << max(0, q_tokens - 1).bit_length(), 1 << max(0, seqs - 1).bit_length())
+    # Sizes are asked for rounded up: few distinct ones, and no growth up to the
+    # minimum, which costs a hundredth.
+    key = (head_dim, max(_ATTN_MIN_TOKENS, 1 << max(0, q_tokens - 1).bit_length()),
+           max(_ATTN_MIN_SEQS, 1 << max(0, seqs - 1).bit_length()))
     nbytes = _ATTN_BYTES.get(key)
     if nbytes is None:
         nbytes = _ATTN_BYTES[key] = paged_attention_workspace_bytes(*key)
@@ -911,9 +916,13 @@ def _attn_workspace(index: int, stream: int, head_dim: int, q_tokens: int, seqs:
         ws = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
         ws[:8192].zero_()
         return ws
-    ws = torch.zeros(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
     with _WS_LOCK:
         old = _ATTN_WORKSPACES.get((index, stream))
+        if old is not None and old.numel() >= nbytes:
+            return old  # another thread's, meanwhile
+        if old is not None:
+            nbytes = max(nbytes, 2 * old.numel())
+        ws = torch.zeros(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
         if old is not None:
             _ATTN_OUTGROWN.append(old)
         _ATTN_WORKSPACES[(index, stream)] = ws

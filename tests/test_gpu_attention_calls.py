@@ -139,3 +139,38 @@ def test_first_call_of_a_process_in_a_capture(cuda_device):
     done = subprocess.run([sys.executable, "-c", FIRST_CALL_IN_A_CAPTURE], env=env,
                           capture_output=True, text=True, timeout=300)
     assert done.returncode == 0, done.stderr
+
+
+def test_workspaces_of_growing_batches(cuda_device):
+    """What larger workspaces have replaced stays below the present one."""
+    def kept():
+        return sum(t.numel() for t in ops._ATTN_OUTGROWN)
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        before = kept()
+        sizes = {ops.reserve_attention_workspace(dim, 1 << n, 1 << max(0, n - 4)).numel()
+                 for dim in (64, 256, 128) for n in range(19)}
+        assert len(sizes) <= 3
+        present = ops.reserve_attention_workspace(128, 1, 1)
+        assert kept() - before < present.numel()
+        assert present.numel() < 2 * ops.paged_attention_workspace_bytes(128, 1 << 18, 1 << 14)
+    # a graph that holds an outgrown workspace still answers
+    case = build(47, [60, 2], [200, 40], 1, 4, 128, 16, BF16, BF16)
+    call = on_gpu(case, 60)
+    want = call()
+    torch.cuda.synchronize()
+    other = torch.cuda.Stream()
+    with torch.cuda.stream(other):
+        ops.reserve_attention_workspace(128, 62, 2)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=other):
+        out = call()
+    with torch.cuda.stream(other):
+        first = ops.reserve_attention_workspace(128, 62, 2)
+        assert ops.reserve_attention_workspace(128, 1 << 18, 2).numel() >= 2 * first.numel()
+        junk = torch.full((first.numel(),), 255, dtype=torch.uint8, device="cuda")
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and ops.attention_status() == 0 and junk.numel()
