@@ -180,9 +180,12 @@ def main(prompt: int = 4096, chunk: int = 2048, seqs: int = 8, steps: int = 32,
     x = synth.activations(seqs, shape.hidden, dev, seed=1)
     residual = torch.zeros_like(x)
     layer.forward(x, residual, cache, batch)  # sizes the workspaces
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        ops.reserve_attention_workspace(128, seqs, seqs)
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph):
+    with torch.cuda.graph(graph, stream=side):
         layer.forward(x, residual, cache, batch)
     total = 0.0
     for i in range(steps):

@@ -931,7 +931,12 @@ def _attn_workspace(index: int, stream: int, head_dim: int, q_tokens: int, seqs:
 
 def reserve_attention_workspace(head_dim: int, q_tokens: int, seqs: int,
                                 device: torch.device | None = None) -> torch.Tensor:
-    """The current stream's attention workspace, for calls of up to these sizes."""
+    """The current stream's attention workspace, for calls of up to these sizes.
+
+    Calls captured on this stream then use it instead of clearing one of their own
+    in each replay. They share its counters and partial results with every other
+    call on it: graphs captured so, and calls on this stream, must not run at the
+    same time (replay them on one stream, or join the streams by events)."""
     index = torch.cuda.current_device() if device is None or device.index is None else device.index
     return _attn_workspace(index, _raw_stream(index), head_dim, q_tokens, seqs)
 
