@@ -194,8 +194,9 @@ __device__ __forceinline__ bool try_wait_long(uint64_t* bar, uint32_t parity) {
 }
 
 // Bounded wait. A role that gives up sets the block's abort flag; from then on
-// no wait waits, so every role runs through its loops (and block barriers) and
-// the block ends with the status bit set.
+// no wait waits, so every role runs through its loops (and block barriers), the
+// loader issues no more copies and waits for those on their way (with a limit
+// again), and the block ends with the status bit set.
 __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, Ctl* ctl,
                                          const StatusWords& status) {
   if (try_wait_long(bar, parity)) return true;
@@ -830,6 +831,7 @@ __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
   const bool on = blockIdx.x < ctas;
   const long long t0 = on ? total * blockIdx.x / ctas : 0;
   const long long t1 = on ? total * (blockIdx.x + 1) / ctas : 0;
+  uint32_t copied = 0, q_copied = 0;  // loader: tiles and Q's whose copies it issued
   Cursor cur;
   if (on) cur.start(p, t0, t1);
   Segment g;
@@ -1012,7 +1014,7 @@ __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
       if (t >= sg.tiles || lane >= boxes || token >= kv_len) return -2;
       return __ldg(a.table + sg.seq * a.table_stride + p.page_of(token));
     };
-    bool more = cur.next(g);
+    bool more = cur.next(g), run = true;  // run: no wait has given up
     SeqLens q = seq_lens(a, g.seq);
     int page_n = page_of(g, q.kv_len, 0);
     while (more) {
@@ -1022,11 +1024,12 @@ __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
       int page = -2, page_before = -2;  // of tile t and t - 1
       auto fill_entry = [&](int t, bool is_v, int pg) {
         if (lane == 0) {
-          wait_bar(&ctl->empty[stage], (fill & 1u) ^ 1u, ctl, a.status);
-          mbar_arrive_expect_tx(&ctl->landed[stage], S::kTileBytes);
+          run = run && wait_bar(&ctl->empty[stage], (fill & 1u) ^ 1u, ctl, a.status);
+          if (run) mbar_arrive_expect_tx(&ctl->landed[stage], S::kTileBytes);
         }
-        __syncwarp();
-        if (lane < boxes) {
+        run = __shfl_sync(0xffffffffu, run, 0);
+        copied += run;
+        if (run && lane < boxes) {
           const int token = g.begin + (g.tile0 + t) * BN + lane * p.box_rows;
           int at = token - p.page_of(token) * a.c.page_size;
           if (pg < 0 || pg >= a.c.num_pages) {
@@ -1054,8 +1057,10 @@ __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
                                  : more_n ? page_of(gn, qn.kv_len, 0) : -2;
         fill_entry(t, false, page);
         if (t == 0) {
-          if (lane == 0) {
-            wait_bar(&ctl->q_empty, (q_count & 1u) ^ 1u, ctl, a.status);
+          if (lane == 0)
+            run = run && wait_bar(&ctl->q_empty, (q_count & 1u) ^ 1u, ctl, a.status);
+          if (lane == 0 && run) {
+            ++q_copied;
             mbar_arrive_expect_tx(&ctl->q_landed,
                                   MT * S::kSlices * p.tile_tokens * p.groups * 128);
 #pragma unroll
@@ -1446,6 +1451,12 @@ __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
 
   tc_fence_before();
   __syncthreads();
+  if (TMA && tid == kProducer * 32 && ctl->abort) {
+    // each barrier's last phase is the one its last copies complete
+    for (uint32_t e = copied - min(copied, (uint32_t)S::kStages); e < copied; ++e)
+      mbar_wait(&ctl->landed[e % S::kStages], e / S::kStages & 1u, a.status);
+    if (q_copied) mbar_wait(&ctl->q_landed, q_copied - 1u & 1u, a.status);
+  }
   if (warp == kMma) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
