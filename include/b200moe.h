@@ -64,9 +64,10 @@ int b200_num_sms(void);
 /*
  * Device-side error bits recorded in a workspace (1 = a pipeline wait timed
  * out, 2 = an expert id >= E reached a GEMM, 4 = a route pointed past the
- * activation rows, 16 = a page number outside the key/value cache) or an
- * expert-parallel region (8 = a wait on another rank timed out). Synchronizes
- * `stream`; clears the bits when reset != 0.
+ * activation rows, 16 = a page number outside the key/value cache, 32 = a scale
+ * byte of the cache outside its range) or an expert-parallel region (8 = a wait
+ * on another rank timed out). Synchronizes `stream`; clears the bits when
+ * reset != 0.
  */
 int b200_workspace_status(void* workspace, int32_t* bits, int32_t reset, void* stream);
 
@@ -476,9 +477,11 @@ int b200_add_rms_norm(const void* x, int32_t dtype, int64_t x_ld, int64_t rows, 
  * (page, offset, head) lies at page * page_stride + offset * token_stride +
  * head * head_stride + i in k and in v (elements of `dtype`), so pages may be
  * stored token-major or head-major. dtype B200_DTYPE_E4M3: each vector of
- * head_dim codes has one power-of-two scale, byte b = 2^(b - 127) (255: NaN),
- * at the scale strides of k_scale / v_scale; a code stands for code * scale.
- * Otherwise bf16 or f16 and no scales (NULL). head_dim 64, 128 or 256; every
+ * head_dim codes has one power-of-two scale, byte b = 2^(b - 127), at the scale
+ * strides of k_scale / v_scale; a code stands for code * scale. b is 103 .. 134
+ * (2^-24 .. 2^7, all that b200_kv_cache_write writes), 255 (NaN), or 0 where
+ * nothing was written: attention of chunks holds code * scale in f16, and sets
+ * status bit 32 for any other byte that its rows may see. Otherwise bf16 or f16 and no scales (NULL). head_dim 64, 128 or 256; every
  * vector 16-byte aligned; num_pages * page_size < 2^31. Slot s = page s /
  * page_size, offset s % page_size.
  */

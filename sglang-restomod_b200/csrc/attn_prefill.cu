@@ -339,10 +339,12 @@ __device__ __forceinline__ uint2 convert4(uint32_t w, uint32_t factor) {
   return make_uint2(hmul2_u32(e4m3x2_to_f16x2((uint16_t)w), factor),
                     hmul2_u32(e4m3x2_to_f16x2((uint16_t)(w >> 16)), factor));
 }
-// The factor of a scale byte (127 + e), for convert4.
+// The factor of a scale byte (127 + e), for convert4: e in [-24, 7]; below, f16 has
+// none but zero, above, code times factor would not be finite.
 __device__ __forceinline__ uint32_t factor_of(uint32_t byte) {
   const uint32_t h =
-      byte == 255u ? 0x7e00u : __half_as_ushort(__float2half_rn(__uint_as_float(byte << 23)));
+      byte == 255u ? 0x7e00u
+                   : __half_as_ushort(__float2half_rn(__uint_as_float(min(byte, 134u) << 23)));
   return h | h << 16;
 }
 
@@ -1130,6 +1132,7 @@ __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
       }
       return r;
     };
+    int bad_scale = 0;
     auto store_info = [&](int t, const Info& r) {
       if (pt >= BN) return;
       RowInfo row;
@@ -1141,6 +1144,9 @@ __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
         f.k = factor_of(r.k_byte);
         f.v = factor_of(r.v_byte);
         factors[(t & 3) * BN + pt] = f;
+        // (byte 0, of slots that nothing has written, is zero in any type)
+        auto outside = [](uint32_t b) { return b - 1u < 254u && b - 103u > 31u; };
+        bad_scale |= outside(r.k_byte) | outside(r.v_byte);
       }
     };
     bool more = cur.next(g);
@@ -1311,6 +1317,7 @@ __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
       more = more_n;
     }
     cp_async_wait_all();
+    if (kQuant && bad_scale) report(a.status, kDevBadScale);
   } else {
     if constexpr (S::kDeal && !TMA) regs_down<S::kRestRegs>();
     if (warp == kRelay) {

@@ -22,6 +22,7 @@ enum DeviceError : int {
   kDevBadRoute = 4,      // a route index outside the activation rows
   kDevPeerTimeout = 8,   // an expert-parallel wait on another rank gave up
   kDevBadPage = 16,      // a page number outside the key/value cache
+  kDevBadScale = 32,     // a key/value scale that the kernel's operands cannot hold
 };
 
 // A wait that has not completed after this many nanoseconds records

@@ -3,8 +3,8 @@
 ``k`` and ``v`` are ``[pages, page_size, kv_heads, head_dim]`` views with
 contiguous vectors and equal strides, so pages may be stored token-major or
 head-major. An e4m3 cache has one scale byte per vector, ``[pages, page_size,
-kv_heads]`` uint8: byte b stands for ``2 ** (b - 127)`` (255: NaN), and a code
-for ``code * 2 ** (b - 127)``.
+kv_heads]`` uint8: byte b stands for ``2 ** (b - 127)`` and a code for ``code * 2
+** (b - 127)``; b lies in 103 .. 134, or is 255 (NaN) or 0 (an unwritten slot).
 
 Slot s of the cache is page ``s // page_size``, offset ``s % page_size``.
 :func:`ops.kv_cache_write` fills slots, :func:`ops.kv_cache_read` reads them

@@ -943,8 +943,8 @@ def reserve_attention_workspace(head_dim: int, q_tokens: int, seqs: int,
 
 def attention_status(device: torch.device | None = None, reset: bool = True) -> int:
     """Error bits of a device's norm and attention calls, those replayed from graphs
-    included (0 = none, 1 = a wait gave up, 16 = a page number outside the cache).
-    Synchronizes the device."""
+    included (0 = none, 1 = a wait gave up, 16 = a page number outside the cache,
+    32 = a chunk met a scale byte outside 103 .. 134). Synchronizes the device."""
     index = torch.cuda.current_device() if device is None or device.index is None else device.index
     torch.cuda.synchronize(index)
     bits = ctypes.c_int32(0)

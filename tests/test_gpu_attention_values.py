@@ -180,3 +180,28 @@ def test_scales_beyond_fp32(cuda_device, store, q_len):
         run(case, q_len, scale=3e38)
     case[1].zero_()
     check_columns(case, q_len, scale=2e38, products=F16 if store == E4M3 else BF16)
+
+
+@pytest.mark.parametrize("page", [1, 16])
+@pytest.mark.parametrize("q_len,groups", [(1, 4), (40, 4), (300, 2)])
+@pytest.mark.parametrize("byte,known", [(103, True), (134, True), (0, True), (102, False), (1, False),
+                                        (135, False), (254, False)])
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_scale_bytes_and_their_range(cuda_device, page, q_len, groups, byte, known, which):
+    """Bytes that no write makes: decode takes them as they are, a chunk reports them
+    and stays finite."""
+    case = build(q_len, [q_len], [q_len + 90], 1, groups, 64, page, BF16, E4M3)
+    cache, table = case[0], case[2]
+    at = (table[0, 30 // page].item(), 30 % page)
+    (cache.k_scale if which == "k" else cache.v_scale)[at] = byte
+    case = (*case[:5], ref.kv_values_ref(cache.k.cpu(), cache.k_scale.cpu()),
+            ref.kv_values_ref(cache.v.cpu(), cache.v_scale.cpu()))
+    out, lse = run(case, q_len)
+    status = ops.attention_status()
+    if q_len == 1 and (which == "v" or byte < 200):  # (k at 2^127: scores beyond fp32)
+        assert status == 0
+    elif q_len > 1:
+        assert status == (0 if known else 32)
+        assert torch.isfinite(out).all() and torch.isfinite(lse).all()
+    if known and (which == "v" or byte < 130):
+        check_columns(case, q_len, products=F16)
