@@ -19,8 +19,8 @@
 // of 128 columns is 16 lanes x 8 columns, so its maximum is four shuffles.
 //
 // Measured (one B200, graph replay): 16384 rows of 7168 bf16 with residual to
-// e4m3 142 us, 5.8 TB/s (89 % of the measured copy rate); 1021 rows of 2048 f16
-// 3.7 us; one row of 7168 to e4m3 3.2 us, nearly all of it the launch.
+// e4m3 151 us, 5.5 TB/s (84 % of the measured copy rate); 1021 rows of 2048 f16
+// 3.9 us; one row of 7168 to e4m3 3.3 us, nearly all of it the launch.
 #include "common.cuh"
 #include "internal.h"
 
@@ -147,6 +147,12 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
+__device__ __forceinline__ uint16_t e4m3x2(float2 v) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(v.y), "f"(v.x));
+  return r;
+}
+
 // The 8 columns y[vec] of a scaled row: 16-bit output, and the group's scale
 // and codes. Called by all lanes of a warp (h8 is a multiple of 16 with q, so
 // a group's 16 lanes are on together).
@@ -178,15 +184,28 @@ __device__ __forceinline__ void store_vec(const NormParams& p, long long row, in
   for (int o = 8; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
   if (!on) return;
   const float scale = max_nan(amax / 448.f, 1e-8f);
-  // One reciprocal for the eight quotients: at most one rounding of fp32 from
-  // them, so a code differs only for a y that lies that close to a border.
+  // The codes of the quotients y / scale, as fp8_act_quant_kernel divides them. A
+  // product with the rounded reciprocal lies within 3 roundings (2^-24) of the
+  // rounded quotient, so where products with the reciprocal moved down and up by
+  // 2^-21 round to one code, that is the quotient's; elsewhere (one vector in some
+  // thousands) divide. (16384 x 7168: 151 us, dividing always 171, one product alone
+  // 142, one product and its bits looked at for a border 167.)
   const float inv = __frcp_rn(scale);
-  const uint64_t inv2 = pair(inv, inv);
+  const float less = inv * (1.f - 0x1p-21f), more = inv * (1.f + 0x1p-21f);
+  const uint64_t less2 = pair(less, less), more2 = pair(more, more);
   uint16_t b[4];
+  uint32_t differ = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float2 v = unpair(mul2(pair(y[2 * i], y[2 * i + 1]), inv2));
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(b[i]) : "f"(v.y), "f"(v.x));
+    const uint64_t y2 = pair(y[2 * i], y[2 * i + 1]);
+    const uint16_t lo = e4m3x2(unpair(mul2(y2, less2)));
+    b[i] = e4m3x2(unpair(mul2(y2, more2)));
+    differ |= lo ^ b[i];
+  }
+  if (differ) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      b[i] = e4m3x2(make_float2(y[2 * i] / scale, y[2 * i + 1] / scale));
   }
   *reinterpret_cast<uint2*>(p.q + (row * p.h8 + vec) * 8) =
       make_uint2(b[0] | (uint32_t)b[1] << 16, b[2] | (uint32_t)b[3] << 16);
