@@ -28,28 +28,36 @@ def run(case, max_q, **kw):
                                return_lse=True, **kw)
 
 
-def check_columns(case, max_q, *, window=0, scale=None, products):
-    """The bound of the file's docstring, element by element."""
-    cache, q, table, kv_lens, starts, kc, vc = case
-    scale = q.shape[-1] ** -0.5 if scale is None else scale
-    out, lse = run(case, max_q, window=window, scale=scale)
-    assert ops.attention_status() == 0
-    want, want_lse = ref.paged_attention_ref(q, kc, vc, table, kv_lens, starts, scale, True, window)
-    mag, _ = ref.paged_attention_ref(q, kc, vc.abs(), table, kv_lens, starts, scale, True, window)
+def column_bound(q, kc, vc, table, kv_lens, starts, scale, window, products, quantized, causal=True):
+    """(bound of each output element, bound of lse) by the file's docstring."""
+    def mean(values):
+        return ref.paged_attention_ref(q, kc, values, table, kv_lens, starts, scale, causal, window)[0]
+
     a = abs(scale) * float(q.double().norm(dim=-1).max()) * \
         float(torch.nan_to_num(kc).norm(dim=-1).max())
     s_err = q.shape[-1] * 2.0 ** -22 * a + 2.0 ** -20
-    tol = (U[products] + U[q.dtype] + 2 * s_err) * mag
-    if cache.k_scale is None and products == F16:
-        tol = tol + 2.0 ** -25 * int(kv_lens.max()) * float(torch.nan_to_num(vc).abs().max())
-    elif products == F16:
-        peak = ref.paged_attention_ref(q, kc, vc.abs().amax(-1, keepdim=True).expand_as(vc), table,
-                                       kv_lens, starts, scale, True, window)[0]
+    tol = (U[products] + U[q.dtype] + 2 * s_err) * mean(vc.abs())
+    if quantized and products == F16:
+        peak = mean(vc.abs().amax(-1, keepdim=True).expand_as(vc))
         tol = tol + 2.0 ** -24 * peak * int(kv_lens.max())
+    elif products == F16:
+        tol = tol + 2.0 ** -25 * int(kv_lens.max()) * float(torch.nan_to_num(vc).abs().max())
+    return tol, s_err + 2.0 ** -20 * a
+
+
+def check_columns(case, max_q, *, window=0, scale=None, products, causal=True):
+    """The bound of the file's docstring, element by element."""
+    cache, q, table, kv_lens, starts, kc, vc = case
+    scale = q.shape[-1] ** -0.5 if scale is None else scale
+    out, lse = run(case, max_q, window=window, scale=scale, causal=causal)
+    assert ops.attention_status() == 0
+    want, want_lse = ref.paged_attention_ref(q, kc, vc, table, kv_lens, starts, scale, causal, window)
+    tol, lse_tol = column_bound(q, kc, vc, table, kv_lens, starts, scale, window, products,
+                                cache.k_scale is not None, causal)
     assert ((out.cpu().double() - want).abs() <= tol).all()
     seen = torch.isfinite(want_lse)
     assert torch.equal(torch.isfinite(lse.cpu()), seen)
-    assert ((lse.cpu().double() - want_lse)[seen].abs() <= s_err + 2.0 ** -20 * a).all()
+    assert ((lse.cpu().double() - want_lse)[seen].abs() <= lse_tol).all()
 
 
 @pytest.mark.parametrize("store,q_dtype", [(BF16, BF16), (F16, F16), (E4M3, BF16)])
@@ -205,3 +213,30 @@ def test_scale_bytes_and_their_range(cuda_device, page, q_len, groups, byte, kno
         assert torch.isfinite(out).all() and torch.isfinite(lse).all()
     if known and (which == "v" or byte < 130):
         check_columns(case, q_len, products=F16)
+
+
+@pytest.mark.parametrize("q_dtype,store", [(BF16, BF16), (F16, F16), (BF16, E4M3), (F16, E4M3)])
+@pytest.mark.parametrize("dim,groups,page", [(64, 8, 16), (128, 8, 64), (256, 4, 16), (128, 3, 1),
+                                             (128, 16, 24)])
+@pytest.mark.parametrize("q_len,kv,window", [(1, 20011, 0), (1, 20011, 15000), (2, 9001, 0),
+                                             (40, 9001, 0), (40, 9001, 5000), (150, 12007, 0)])
+def test_every_part_of_a_long_context(cuda_device, q_dtype, store, dim, groups, page, q_len, kv,
+                                      window):
+    """Column d holds a one for the tokens of the d-th of head_dim equal pieces of the
+    context, so the output tells the weight of each piece: one that a part, a tile or
+    a merge drops is missing whole."""
+    case = build(dim + kv, [q_len], [kv], 1, groups, dim, page, q_dtype, store)
+    v = torch.zeros(kv, 1, dim, dtype=q_dtype)
+    t = torch.arange(kv)
+    v[t, 0, t * dim // kv] = 1.0
+    case = rewrite(case, 0, range(kv), v=v)
+    # (e4m3 chunks and decode multiply in f16, the others in q's type)
+    check_columns(case, q_len, window=window, products=F16 if store == E4M3 else q_dtype)
+
+
+@pytest.mark.parametrize("store", [BF16, E4M3])
+@pytest.mark.parametrize("q_len", [1, 40])
+def test_every_part_of_many_sequences(cuda_device, store, q_len):
+    lens = [q_len + (37 * i) % 900 for i in range(60)]
+    case = build(61, [q_len] * 60, lens, 2, 4, 64, 16, BF16, store)
+    check_columns(case, q_len, products=F16 if store == E4M3 else BF16)
