@@ -710,10 +710,18 @@ def w8a8_linear_quantized(q: torch.Tensor, scales: torch.Tensor, w: torch.Tensor
     _w8_weights(w, w_scales)
     if q.dtype != torch.float8_e4m3fn or scales.dtype != torch.float32:
         raise TypeError(f"q must be float8_e4m3fn and scales float32, got {q.dtype}, {scales.dtype}")
+    if q.dim() != 2 or scales.dim() != 2:
+        raise ValueError(f"q must be [M, K] and scales [K/128, ld], got {tuple(q.shape)}, "
+                         f"{tuple(scales.shape)}")
     m, k = (int(d) for d in q.shape)
     if w.shape[-1] != k or scales.shape[0] != k // 128:
         raise ValueError(f"K differs: q {k}, weight {w.shape[-1]}, scales {scales.shape[0]} groups")
     n = int(w.shape[-2])
+    if w.numel() != n * k or w_scales.numel() != n // 128 * (k // 128):
+        raise ValueError(f"weight must be [N, K] with scales [N/128, K/128], got {tuple(w.shape)}, "
+                         f"{tuple(w_scales.shape)}")
+    if any(t.device != q.device for t in (scales, w, w_scales)):
+        raise ValueError("w8a8_linear_quantized: the operands are on different devices")
     cols = n // 2 if gated_mode == _lib.GATED_FUSED else n
     if out is None:
         out = torch.empty(m, cols, dtype=out_dtype, device=q.device)

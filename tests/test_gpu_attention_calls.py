@@ -174,3 +174,21 @@ def test_workspaces_of_growing_batches(cuda_device):
         graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, want) and ops.attention_status() == 0 and junk.numel()
+
+
+def test_quantized_linear_refuses_operands_that_do_not_fit(cuda_device):
+    def zeros(*shape, dtype=torch.float32):
+        return torch.zeros(*shape, device="cuda").to(dtype)
+
+    q, s = zeros(4, 256, dtype=E4M3), zeros(2, 128)
+    w, ws = zeros(384, 256, dtype=E4M3), zeros(3, 2)
+    assert ops.w8a8_linear_quantized(q, s, w, ws).shape == (4, 384)
+    for bad in (zeros(2, 2), zeros(3, 1), zeros(6)[:5]):
+        with pytest.raises(ValueError, match="scales"):
+            ops.w8a8_linear_quantized(q, s, w, bad)
+    with pytest.raises(ValueError, match="weight must be"):
+        ops.w8a8_linear_quantized(q, s, zeros(2, 384, 256, dtype=E4M3), ws)
+    with pytest.raises(ValueError, match="scales"):
+        ops.w8a8_linear_quantized(q, zeros(256), w, ws)
+    with pytest.raises(ValueError, match="K differs"):
+        ops.w8a8_linear_quantized(q, zeros(3, 128), w, ws)
