@@ -884,8 +884,9 @@ __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
         uint32_t s[S::kRowInRegs ? BN : 32];  // the row's S, read once
         if constexpr (S::kRowInRegs) {
           load_row<BN>(ts, s);
-          if (masked) mask_row<BN>(s, col0, lo, hi, negative ? INFINITY : -INFINITY);
-          top = negative ? max_row<BN, true>(s) : max_row<BN, false>(s);
+          // (registers alone: by the thread's own scale, selects instead of branches)
+          if (masked) mask_row<BN>(s, col0, lo, hi, scale >= 0.f ? -INFINITY : INFINITY);
+          top = scale >= 0.f ? max_row<BN, false>(s) : max_row<BN, true>(s);
         } else if (!negative)
           top = masked ? max_pass<BN, true, false>(ts, col0, lo, hi)
                        : max_pass<BN, false, false>(ts, col0, lo, hi);
