@@ -19,8 +19,8 @@
 // of 128 columns is 16 lanes x 8 columns, so its maximum is four shuffles.
 //
 // Measured (one B200, graph replay): 16384 rows of 7168 bf16 with residual to
-// e4m3 151 us, 5.5 TB/s (84 % of the measured copy rate); 1021 rows of 2048 f16
-// 3.9 us; one row of 7168 to e4m3 3.3 us, nearly all of it the launch.
+// e4m3 150 us, 5.5 TB/s (84 % of the measured copy rate); 1021 rows of 2048 f16
+// 3.9 us; one row of 7168 to e4m3 3.4 us, nearly all of it the launch.
 #include "common.cuh"
 #include "internal.h"
 
@@ -153,6 +153,14 @@ __device__ __forceinline__ uint16_t e4m3x2(float2 v) {
   return r;
 }
 
+// (Not inlined: rarely taken, and its divisions would take registers in the loop.)
+__device__ __noinline__ uint2 quotient_codes(float4 a, float4 b, float scale) {
+  return make_uint2(e4m3x2(make_float2(a.x / scale, a.y / scale)) |
+                        (uint32_t)e4m3x2(make_float2(a.z / scale, a.w / scale)) << 16,
+                    e4m3x2(make_float2(b.x / scale, b.y / scale)) |
+                        (uint32_t)e4m3x2(make_float2(b.z / scale, b.w / scale)) << 16);
+}
+
 // The 8 columns y[vec] of a scaled row: 16-bit output, and the group's scale
 // and codes. Called by all lanes of a warp (h8 is a multiple of 16 with q, so
 // a group's 16 lanes are on together).
@@ -188,7 +196,7 @@ __device__ __forceinline__ void store_vec(const NormParams& p, long long row, in
   // product with the rounded reciprocal lies within 3 roundings (2^-24) of the
   // rounded quotient, so where products with the reciprocal moved down and up by
   // 2^-21 round to one code, that is the quotient's; elsewhere (one vector in some
-  // thousands) divide. (16384 x 7168: 151 us, dividing always 171, one product alone
+  // thousands) divide. (16384 x 7168: 150 us, dividing always 171, one product alone
   // 142, one product and its bits looked at for a border 167.)
   const float inv = __frcp_rn(scale);
   const float less = inv * (1.f - 0x1p-21f), more = inv * (1.f + 0x1p-21f);
@@ -202,13 +210,11 @@ __device__ __forceinline__ void store_vec(const NormParams& p, long long row, in
     b[i] = e4m3x2(unpair(mul2(y2, more2)));
     differ |= lo ^ b[i];
   }
-  if (differ) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      b[i] = e4m3x2(make_float2(y[2 * i] / scale, y[2 * i + 1] / scale));
-  }
-  *reinterpret_cast<uint2*>(p.q + (row * p.h8 + vec) * 8) =
-      make_uint2(b[0] | (uint32_t)b[1] << 16, b[2] | (uint32_t)b[3] << 16);
+  uint2 codes = make_uint2(b[0] | (uint32_t)b[1] << 16, b[2] | (uint32_t)b[3] << 16);
+  if (differ)
+    codes = quotient_codes(make_float4(y[0], y[1], y[2], y[3]), make_float4(y[4], y[5], y[6], y[7]),
+                           scale);
+  *reinterpret_cast<uint2*>(p.q + (row * p.h8 + vec) * 8) = codes;
   if ((vec & 15) == 0) p.scales[(long long)(vec >> 4) * p.scales_ld + row] = scale;
 }
 
