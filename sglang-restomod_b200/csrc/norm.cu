@@ -19,8 +19,8 @@
 // of 128 columns is 16 lanes x 8 columns, so its maximum is four shuffles.
 //
 // Measured (one B200, graph replay): 16384 rows of 7168 bf16 with residual to
-// e4m3 150 us, 5.5 TB/s (84 % of the measured copy rate); 1021 rows of 2048 f16
-// 3.9 us; one row of 7168 to e4m3 3.4 us, nearly all of it the launch.
+// e4m3 145 us, 5.7 TB/s (87 % of the measured copy rate); 1021 rows of 2048 f16
+// 3.9 us; one row of 7168 to e4m3 3.3 us, nearly all of it the launch.
 #include "common.cuh"
 #include "internal.h"
 
@@ -153,28 +153,21 @@ __device__ __forceinline__ uint16_t e4m3x2(float2 v) {
   return r;
 }
 
-// (Not inlined: rarely taken, and its divisions would take registers in the loop.)
-__device__ __noinline__ uint2 quotient_codes(float4 a, float4 b, float scale) {
-  return make_uint2(e4m3x2(make_float2(a.x / scale, a.y / scale)) |
-                        (uint32_t)e4m3x2(make_float2(a.z / scale, a.w / scale)) << 16,
-                    e4m3x2(make_float2(b.x / scale, b.y / scale)) |
-                        (uint32_t)e4m3x2(make_float2(b.z / scale, b.w / scale)) << 16);
-}
-
 // The 8 columns y[vec] of a scaled row: 16-bit output, and the group's scale
 // and codes. Called by all lanes of a warp (h8 is a multiple of 16 with q, so
 // a group's 16 lanes are on together).
 template <bool F16>
 __device__ __forceinline__ void store_vec(const NormParams& p, long long row, int vec,
                                           const uint64_t (&h)[4], float rstd) {
-  const bool on = vec < p.h8;
-  float y[8];
+  const bool on = vec < p.h8, quantize = p.q != nullptr;
+  float y[8];  // negated where codes are wanted
 #pragma unroll
   for (int i = 0; i < 8; ++i) y[i] = 0.f;
   if (on) {
     float w[8];
     load_weight(p, vec, w);
-    const uint64_t r2 = pair(rstd, rstd);
+    const float r = quantize ? -rstd : rstd;
+    const uint64_t r2 = pair(r, r);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float2 v = unpair(mul2(mul2(h[i], r2), pair(w[2 * i], w[2 * i + 1])));
@@ -182,8 +175,16 @@ __device__ __forceinline__ void store_vec(const NormParams& p, long long row, in
       y[2 * i + 1] = v.y;
     }
   }
-  if (p.y != nullptr && on) *vec_at(p.y, row, p.y_ld, vec) = pack8<F16>(y);
-  if (p.q == nullptr) return;
+  if (!quantize) {
+    if (on) *vec_at(p.y, row, p.y_ld, vec) = pack8<F16>(y);
+    return;
+  }
+  if (p.y != nullptr && on) {
+    float out[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) out[i] = -y[i];
+    *vec_at(p.y, row, p.y_ld, vec) = pack8<F16>(out);
+  }
   // A NaN in the group makes its scale NaN.
   float amax = fabsf(y[0]);
 #pragma unroll
@@ -192,28 +193,24 @@ __device__ __forceinline__ void store_vec(const NormParams& p, long long row, in
   for (int o = 8; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
   if (!on) return;
   const float scale = max_nan(amax / 448.f, 1e-8f);
-  // The codes of the quotients y / scale, as fp8_act_quant_kernel divides them. A
-  // product with the rounded reciprocal lies within 3 roundings (2^-24) of the
-  // rounded quotient, so where products with the reciprocal moved down and up by
-  // 2^-21 round to one code, that is the quotient's; elsewhere (one vector in some
-  // thousands) divide. (16384 x 7168: 150 us, dividing always 171, one product alone
-  // 142, one product and its bits looked at for a border 167.)
-  const float inv = __frcp_rn(scale);
-  const float less = inv * (1.f - 0x1p-21f), more = inv * (1.f + 0x1p-21f);
-  const uint64_t less2 = pair(less, less), more2 = pair(more, more);
+  // The codes of the quotients y / scale, as fp8_act_quant_kernel divides them. The
+  // quotient is a product with the rounded reciprocal, corrected once by its exact
+  // remainder (P. Markstein, IBM J. Res. Dev. 34, 1990): r = q s - y, q - r / s. Its
+  // code is the division's for every mantissa of a scale and every y next to a border
+  // between codes (all were tried), where the product alone may have the other one;
+  // from -y, so that a zero keeps its sign. (16384 x 7168: 145 us, dividing 171, the
+  // product alone 142, dividing where products on both sides of the quotient differ
+  // in their codes 150.) An infinite scale has no remainder: its quotients are 0 or
+  // NaN already.
+  const float minus_inv = -__frcp_rn(scale), s = scale < INFINITY ? scale : 0.f;
+  const uint64_t inv2 = pair(minus_inv, minus_inv), s2 = pair(s, s);
   uint16_t b[4];
-  uint32_t differ = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint64_t y2 = pair(y[2 * i], y[2 * i + 1]);
-    const uint16_t lo = e4m3x2(unpair(mul2(y2, less2)));
-    b[i] = e4m3x2(unpair(mul2(y2, more2)));
-    differ |= lo ^ b[i];
+    const uint64_t y2 = pair(y[2 * i], y[2 * i + 1]), q2 = mul2(y2, inv2);
+    b[i] = e4m3x2(unpair(fma2(fma2(q2, s2, y2), inv2, q2)));
   }
-  uint2 codes = make_uint2(b[0] | (uint32_t)b[1] << 16, b[2] | (uint32_t)b[3] << 16);
-  if (differ)
-    codes = quotient_codes(make_float4(y[0], y[1], y[2], y[3]), make_float4(y[4], y[5], y[6], y[7]),
-                           scale);
+  const uint2 codes = make_uint2(b[0] | (uint32_t)b[1] << 16, b[2] | (uint32_t)b[3] << 16);
   *reinterpret_cast<uint2*>(p.q + (row * p.h8 + vec) * 8) = codes;
   if ((vec & 15) == 0) p.scales[(long long)(vec >> 4) * p.scales_ld + row] = scale;
 }

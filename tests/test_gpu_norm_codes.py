@@ -64,3 +64,37 @@ def test_codes_agree_with_the_activation_quantizer(cuda_device):
     q2, s2 = ops.fp8_act_quant(w.expand(5, 4096).contiguous().cuda())
     assert torch.equal(q.view(torch.uint8), q2.view(torch.uint8))
     assert torch.equal(s[:, :5], s2[:, :5])
+
+
+@pytest.mark.parametrize("rows,hidden", [(1, 128), (700, 512), (3, 7168)])
+def test_codes_of_infinities_nan_and_zeros(cuda_device, rows, hidden):
+    """A group with an infinity has an infinite scale, zeros and NaN; one with a NaN is
+    NaN; zeros keep their signs. (Rows of ones: y is the weight.)"""
+    w = torch.randn(hidden, generator=torch.Generator().manual_seed(5))
+    w[3], w[5], w[7] = float("inf"), 0.0, -0.0
+    if hidden > 128:
+        w[130], w[261], w[262] = float("nan"), 0.0, -0.0
+    x = torch.ones(rows, hidden, dtype=BF16, device="cuda")
+    q, s, _ = ops.add_rms_norm_fp8(x, w.cuda(), 0.0)
+    groups = w.view(-1, 128)
+    scale = torch.maximum(groups.abs().amax(-1) / 448.0, torch.tensor(1e-8))
+    codes = (groups / scale[:, None]).clamp(-448.0, 448.0).to(E4M3).view(-1)
+    assert torch.equal(torch.nan_to_num(s.cpu(), nan=-1.0), torch.nan_to_num(
+        scale, nan=-1.0)[:, None].expand(-1, rows))
+    for row in (q[0].cpu(), q[-1].cpu()):
+        nan = torch.isnan(codes.float())
+        assert torch.equal(torch.isnan(row.float()), nan)
+        assert torch.equal(row.view(torch.uint8)[~nan], codes.view(torch.uint8)[~nan])
+
+
+@pytest.mark.parametrize("hidden", [128, 1024, 4096])
+def test_both_outputs_are_one_norm(cuda_device, hidden):
+    g = torch.Generator().manual_seed(hidden)
+    x, r = (torch.randn(37, hidden, generator=g).to(BF16).cuda() for _ in "xr")
+    w = torch.randn(hidden, generator=g).cuda()
+    y, h = ops.add_rms_norm(x, w, residual=r)
+    both = torch.empty_like(x)
+    q, s, h2 = ops.add_rms_norm_fp8(x, w, residual=r, out=both)
+    q3, s3, _ = ops.add_rms_norm_fp8(x, w, residual=r)
+    assert torch.equal(both, y) and torch.equal(h, h2)
+    assert torch.equal(q.view(torch.uint8), q3.view(torch.uint8)) and torch.equal(s, s3)
