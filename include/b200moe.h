@@ -530,14 +530,18 @@ int b200_kv_cache_read(const b200_kv_cache* cache, const int64_t* slots, int64_t
  * causal: position p sees positions <= p, and with window > 0 only the last
  * `window` of them; not causal: all cached tokens. A row that sees nothing
  * gets zeros and lse = -inf. max_q_len bounds the new tokens of any sequence
- * (1: decode); further ones, and rows of no sequence, are left unwritten. Page numbers outside the
- * cache read as zeros and set status bit 16. Cached values past kv_lens are
- * never read. The cache is e4m3, or of q's type. q and out: vectors 16-byte
- * aligned, strides in elements. No host synchronization, and no host knowledge
- * of the lengths: one captured call serves any contents of kv_lens, q_starts
- * and page_table. Sums and softmax statistics are fp32; P is rounded to 16
- * bits before it multiplies the values. Workspace: zero-filled before first
- * use; it may be the one the GEMM calls use.
+ * (1: decode); further ones keep their positions, and like rows of no sequence
+ * they are left unwritten. Page numbers outside the cache read as zeros and set
+ * status bit 16. Cached values past kv_lens or before every row's window never
+ * show, though a page's may be read with its others; a value that is infinite or
+ * NaN shows in every row that sees it and may show in rows of the same call's
+ * sequence that mask it. The cache is e4m3, or of q's type. q and out: vectors
+ * 16-byte aligned, strides in elements. |scale| * log2(e) must be finite. No
+ * host synchronization, and no host knowledge of the lengths: one captured call
+ * serves any contents of kv_lens, q_starts and page_table. Sums and softmax
+ * statistics are fp32; P is rounded to 16 bits before it multiplies the values,
+ * and chunks hold e4m3 values as f16 (absolute 2^-25). Workspace: zero-filled
+ * before first use; it may be the one the GEMM calls use.
  */
 int64_t b200_paged_attention_workspace_bytes(int32_t head_dim, int64_t q_tokens, int32_t seqs);
 int b200_paged_attention(const b200_kv_cache* cache, const void* q, int32_t dtype, int64_t q_tokens,

@@ -11,9 +11,9 @@
 // per cached element against 2 rows' multiply-adds per element, far below the
 // tensor rate, so the work is to keep enough loads in flight:
 //
-// * The sequences' key ranges, in tiles of 64 or 128 tokens, are laid end to end over
-//   (sequence, head, tile) and cut into equal ranges, one per block, so uneven
-//   lengths leave no block idle. A block finds its range from kv_lens itself
+// * The sequences' key ranges, in tiles of 96 or 112 tokens (16 a consumer warp), are
+//   laid end to end over (sequence, head, tile) and cut into equal ranges, one per
+//   block, so uneven lengths leave no block idle. A block finds its range from kv_lens itself
 //   (no host knowledge of the lengths, no planning launch). A (sequence, head)
 //   cut by a range border leaves partial (O, m, l) in the scratch; the last
 //   block to arrive at the pair's counter adds them in block order, so the
@@ -21,9 +21,9 @@
 // * A producer fills a ring of stages, a tile of 16 tokens per consumer warp each,
 //   and runs on into the next pair while the present one is finished. Pages of
 //   a multiple of 8 tokens come by tensor copies of one warp; other pages
-//   (single-token ones, say) by 16-byte cp.async of two or four. (When every warp issued the copies of its
-//   own tokens, issuing them took a third of its step: 75 to 150 clocks each.)
-//   Consumers meet only where a pair ends.
+//   (single-token ones, say) by 16-byte cp.async of two or four. (When every warp
+//   issued the copies of its own tokens, issuing them took a third of its step: 75
+//   to 150 clocks each.) Consumers meet only where a pair ends.
 // * The products are taken transposed (S^T = K Q^T, O^T = V^T P^T): the
 //   m16n8k16 tile then has 16 cached tokens or 16 head columns in M and 8 rows
 //   in N, so 8 query heads per key/value head waste nothing. K is read as the
@@ -36,6 +36,10 @@
 //   code with a lazy maximum mv of s + e over the tokens that the row sees, so that
 //   P keeps f16's bits for the tokens that make up the result, however far apart
 //   scales lie (one reference scale for a tile's tokens lost what lay 2^14 below it).
+// * P is rounded to 16 bits, the products' operand type (bf16, or f16 for f16 and
+//   e4m3 caches); l sums it unrounded. Relative 2^-8 a token in bf16, whose errors
+//   partly cancel: 2.1e-3 of the output's norm where fp32 products would leave the
+//   output's own rounding, 1.6e-3 (one of 4099 keys); 2.7e-4 and 2.1e-4 in f16.
 // * The maximum is lazy: O and l are rescaled only when some s exceeds m by
 //   more than 8 (in log2), so P stays below 2^8 and most tiles need no cross-lane
 //   reduction at all.
@@ -43,7 +47,7 @@
 // Measured (one B200, graph replay): 64 sequences of up to 8192 tokens, 8 heads
 // of 128 with 8 query heads each, e4m3 110 us, 4.8 TB/s (73 % of the measured
 // copy rate: the conversions' and products' instructions take the rest), bf16
-// 205 us; 16 of up to 32768, 2 heads of 256, bf16 98 us, 5.2 TB/s (79 %); one of
+// 206 us; with 16 rows, e4m3, 243 us; 16 of up to 32768, 2 heads of 256, bf16 98 us, 5.2 TB/s (79 %); one of
 // 4099, 8 heads of 128, 14 us, the chain launch, first copies, products, parts.
 #include "attn_maps.cuh"
 #include "common.cuh"
@@ -55,8 +59,9 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazy = 8.f;        // log2 of the largest P before a rescale
 // A block takes at least this much work, in tiles: below it the pair's merge
-// costs more than the extra blocks bring. And a pair is cut into at most
-// kMaxParts, whose sum one block takes.
+// costs more than the extra blocks bring. And there are at most kMaxParts blocks a
+// pair on average, since one block adds a pair's parts (a long sequence among short
+// ones may still have more).
 constexpr int kMinTiles = 2;
 constexpr int kMaxParts = 64;
 // What a (sequence, head) pair costs besides its tiles, in tiles of about 100
@@ -1164,7 +1169,7 @@ cudaError_t launch_type(DecodeParams& p, int rows, cudaStream_t stream) {
 // 16 rows, bf16, 4 heads: head_dim 128, 1 x 4000 keys 25 / 22, 1 x 60000 54 / 46,
 // 64 x 4000 76 / 69; head_dim 256 36 / 26, 79 / 68, 121 / 119; but head_dim 64 21 /
 // 19, 46 / 41, 43 / 64, single-token pages at 128 26 / 26 and, 16 x 1000, 25 / 30,
-// and 64 x 8192 e4m3 keys, 8 heads, 258 / 476. With 8 rows this kernel is ahead in
+// and 64 x 8192 e4m3 keys, 8 heads, 272 / 476. With 8 rows this kernel is ahead in
 // all but 64 x 4000 keys (head_dim 128: 69 / 69), by 2 to 8 us.
 int attn_decode_rows(const AttnLaunch& l) {
   return l.cache_dtype != 3 && l.c.head_dim >= 128 && l.c.page_size % 8 == 0 ? 8 : 16;

@@ -50,16 +50,19 @@
 //
 // The maximum is lazy: m is raised, and O rescaled, only where some S exceeds it
 // by more than 8 (in log2), so that most tiles leave O alone. P is at most 2^8
-// then, and its rounding to 16 bits relative whatever m is; l sums the unrounded
-// fp32 P.
+// then, and its rounding to 16 bits, the products' operand type, relative whatever m
+// is (in f16 down to 2^-14, absolute 2^-25 below); l sums the unrounded fp32 P.
+// Against 64 bits a prompt's output is off by 2.1e-3 of its norm in bf16 and mixed
+// chunks' by 2.7e-4 in f16, where fp32 products would leave the output's own
+// rounding, 1.6e-3 and 2.1e-4.
 //
 // Measured (one B200): a prompt of 8192 bf16 tokens, 32 heads of 128 over 8,
-// 506 to 528 us, 1040 to 1085 TFLOP/s, 63 to 66 % of the measured bf16 product
-// rate; a tile of 256 rows and 128 keys takes 2.3 us and its exponentials 1.1,
+// 480 to 530 us replayed and 548 in a long loop under the power cap, 1000 to 1145
+// TFLOP/s, 61 to 69 % of the measured bf16 product rate; a tile of 256 rows and 128 keys takes 2.3 us and its exponentials 1.1,
 // so the chain S -> maximum -> P -> product, two tiles deep, sets the time.
 // (Tried without gain: half rows by four warpgroups, keys by 64 with four S
 // buffers, polynomials for an eighth to a half of the exponentials, P handed
-// over in halves.) 512 tokens on 16384 e4m3 ones: 166 us, 813 TFLOP/s; bf16 136.
+// over in halves.) 512 tokens on 16384 e4m3 ones: 163 us, 830 TFLOP/s; bf16 130.
 #include "attn_maps.cuh"
 #include "common.cuh"
 #include "internal.h"
@@ -132,7 +135,8 @@ struct Shape {
   //                        143; e4m3, 8 x 512 on 2048, d64 108 / 89; not e4m3 at
   //                        head_dim 128, whose converting threads need more than
   //                        is left (512 on 16384 167 / 171)
-  //   duo, tensor copies   spills go, 551 / 517 for a prompt of 8192
+  //   duo, tensor copies   fewer spills (100 B of stores stay), 551 / 517 for a
+  //                        prompt of 8192
   // Solo with tensor copies has registers enough as it is launched. The sum is
   // what the block is launched with: threads x registers of softmax, copying
   // threads, and the rest (relay, mma, idle warps; the loader).
