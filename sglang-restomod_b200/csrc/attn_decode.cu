@@ -47,8 +47,9 @@
 // Measured (one B200, graph replay): 64 sequences of up to 8192 tokens, 8 heads
 // of 128 with 8 query heads each, e4m3 110 us, 4.8 TB/s (73 % of the measured
 // copy rate: the conversions' and products' instructions take the rest), bf16
-// 206 us; with 16 rows, e4m3, 243 us; 16 of up to 32768, 2 heads of 256, bf16 98 us, 5.2 TB/s (79 %); one of
-// 4099, 8 heads of 128, 14 us, the chain launch, first copies, products, parts.
+// 206 us; with 16 rows, e4m3, 243 us; 16 of up to 32768, 2 heads of 256, bf16 98
+// us, 5.2 TB/s (79 %); one of 4099, 8 heads of 128, 14 us, the chain launch, first
+// copies, products, parts.
 #include "attn_maps.cuh"
 #include "common.cuh"
 #include "internal.h"
@@ -178,12 +179,6 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
   else
     mma_16816(d, a, b0, b1);
 }
-__device__ __forceinline__ float exp2_fast(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-
 // Byte of 16-byte chunk `chunk` of token row `row` in a stage's K or V tile,
 // placed so that the operand reads below touch the banks evenly. Tensor copies
 // leave slices of 128 B with chunks XORed by the row's low bits (64 B rows: by
@@ -790,7 +785,7 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
             for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
             // a row that nothing pushed past the threshold keeps its maximum
             const float mn = mx > raise_at[nr][j] ? mx : m[nr][j];
-            const float f = m[nr][j] == mn ? 1.f : exp2_fast(m[nr][j] - mn);
+            const float f = m[nr][j] == mn ? 1.f : ex2(m[nr][j] - mn);
             l[nr][j] *= f;
             m[nr][j] = mn;
             raise_at[nr][j] = mn + kLazy;
@@ -803,7 +798,7 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
 #pragma unroll
               for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
               if (!(top > mv[nr][j] + kLazy)) top = mv[nr][j];
-              o_scale[nr][j] = mv[nr][j] == top ? 1.f : exp2_fast(mv[nr][j] - top);
+              o_scale[nr][j] = mv[nr][j] == top ? 1.f : ex2(mv[nr][j] - top);
               mv[nr][j] = top;
             }
           }
@@ -825,12 +820,12 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const float x = s[t16][nr][j];
-            pr[j] = exp2_fast(x - (m[nr][j & 1] == -INFINITY ? 0.f : m[nr][j & 1]));
+            pr[j] = ex2(x - (m[nr][j & 1] == -INFINITY ? 0.f : m[nr][j & 1]));
             l[nr][j & 1] += pr[j];
             // times the value's scale; a masked token's stays zero whatever that holds
             if (KV == kE4m3) {
               const float base = mv[nr][j & 1] == -INFINITY ? 0.f : mv[nr][j & 1];
-              pr[j] = x == -INFINITY ? 0.f : exp2_fast(x + v_log2[t16][j >> 1] - base);
+              pr[j] = x == -INFINITY ? 0.f : ex2(x + v_log2[t16][j >> 1] - base);
             }
           }
 #pragma unroll
@@ -930,7 +925,7 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
       float mx = -INFINITY, sum = 0.f;
       for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, sm.wm[w][tid]);
       for (int w = 0; w < kWarps; ++w)
-        sum += sm.wm[w][tid] == -INFINITY ? sm.wl[w][tid] : sm.wl[w][tid] * exp2_fast(sm.wm[w][tid] - mx);
+        sum += sm.wm[w][tid] == -INFINITY ? sm.wl[w][tid] : sm.wl[w][tid] * ex2(sm.wm[w][tid] - mx);
       sm.mx[tid] = mx;
       sm.sum[tid] = sum;
     }
@@ -951,7 +946,7 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
         float mx = -INFINITY;
         for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, sm.wm[w][r]);
         const float unit = KV != kE4m3 ? m[nr][j] : mv[nr][j] == -INFINITY ? 0.f : mv[nr][j];
-        const float f = m[nr][j] == -INFINITY ? 0.f : exp2_fast(unit - mx);
+        const float f = m[nr][j] == -INFINITY ? 0.f : ex2(unit - mx);
 #pragma unroll
         for (int t = 0; t < D / 16; ++t)
 #pragma unroll
@@ -1058,7 +1053,7 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
               // (a part without a visible key has m = -inf and l = 0, or NaN)
               const float mx = sm.mx[min(r0 + i, rows - 1)];
               const float w = ml[i].x == -INFINITY ? (ml[i].y == 0.f ? 0.f : 1.f)
-                                                   : exp2_fast(ml[i].x - mx);
+                                                   : ex2(ml[i].x - mx);
               l_sum[i] += w == 0.f ? 0.f : ml[i].y * w;
 #pragma unroll
               for (int k = 0; k < kCols; ++k) acc[i][k] += w == 0.f ? 0.f : v[i][k] * w;

@@ -222,12 +222,6 @@ __device__ __forceinline__ void regs_down() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-
 template <bool F16>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   uint32_t r;
@@ -533,27 +527,6 @@ struct Cursor {
     return false;
   }
 };
-
-__device__ __forceinline__ uint64_t f32x2(float lo, float hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ float2 unpack_f32x2(uint64_t v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 
 // Where a block's partial (m, l, O) of a tile of 128 rows lies, in floats: the
 // block's first run of keys continues a pair, its last one may begin another.
@@ -1480,10 +1453,8 @@ __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
 
 long long align256(long long v) { return (v + 255) / 256 * 256; }
 
-// Units at the smallest unit of tokens that any call makes: one token.
-long long max_units(long long q_tokens, int seqs, int unit_tokens) {
-  return q_tokens / unit_tokens + seqs;
-}
+// The most units a call can have, of one token each.
+long long max_units(long long q_tokens, int seqs) { return q_tokens + seqs; }
 
 template <int D, int MT, int KV, bool TMA>
 cudaError_t launch(const PrefillParams& p, const CUtensorMap (&maps)[3], cudaStream_t stream) {
@@ -1567,7 +1538,7 @@ cudaError_t launch_type(PrefillParams& p, cudaStream_t stream) {
 long long attn_prefill_scratch_bytes(int head_dim, long long q_tokens, int seqs) {
   const long long sms = device_sm_count();
   return 256 + align256(sms * 16) + align256(4ll * (seqs + 1)) +
-         align256(16 * max_units(q_tokens, seqs, 1)) +
+         align256(16 * max_units(q_tokens, seqs)) +
          sms * 2 * (head_dim == 256 ? 1 : 2) * (head_dim + 2) * 128 * 4;
 }
 
@@ -1580,7 +1551,7 @@ cudaError_t launch_attn_prefill(const AttnLaunch& l, cudaStream_t stream) {
   p.box_rows = 1;
   p.page_shift = (l.c.page_size & (l.c.page_size - 1)) == 0 ? __builtin_ctz(l.c.page_size) : -1;
   const long long sms = device_sm_count();
-  p.max_units = (int)max_units(l.q_tokens, l.seqs, 1);
+  p.max_units = (int)max_units(l.q_tokens, l.seqs);
   uint8_t* at = l.scratch;
   p.head = reinterpret_cast<long long*>(at);
   at += 256;

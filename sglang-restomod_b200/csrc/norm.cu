@@ -113,33 +113,6 @@ __device__ __forceinline__ uint4 load_row(const uint4* src) {
   return v;
 }
 
-// Two fp32 operations per instruction: with the conversions, a row's arithmetic
-// would otherwise take longer to issue than its bytes to arrive.
-__device__ __forceinline__ uint64_t pair(float lo, float hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ float2 unpair(uint64_t v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
 // The larger, NaN if either is.
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
@@ -167,10 +140,10 @@ __device__ __forceinline__ void store_vec(const NormParams& p, long long row, in
     float w[8];
     load_weight(p, vec, w);
     const float r = quantize ? -rstd : rstd;
-    const uint64_t r2 = pair(r, r);
+    const uint64_t r2 = f32x2(r, r);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float2 v = unpair(mul2(mul2(h[i], r2), pair(w[2 * i], w[2 * i + 1])));
+      const float2 v = unpack_f32x2(mul_f32x2(mul_f32x2(h[i], r2), f32x2(w[2 * i], w[2 * i + 1])));
       y[2 * i] = v.x;
       y[2 * i + 1] = v.y;
     }
@@ -203,34 +176,36 @@ __device__ __forceinline__ void store_vec(const NormParams& p, long long row, in
   // in their codes 150.) An infinite scale has no remainder: its quotients are 0 or
   // NaN already.
   const float minus_inv = -__frcp_rn(scale), s = scale < INFINITY ? scale : 0.f;
-  const uint64_t inv2 = pair(minus_inv, minus_inv), s2 = pair(s, s);
+  const uint64_t inv2 = f32x2(minus_inv, minus_inv), s2 = f32x2(s, s);
   uint16_t b[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint64_t y2 = pair(y[2 * i], y[2 * i + 1]), q2 = mul2(y2, inv2);
-    b[i] = e4m3x2(unpair(fma2(fma2(q2, s2, y2), inv2, q2)));
+    const uint64_t y2 = f32x2(y[2 * i], y[2 * i + 1]), q2 = mul_f32x2(y2, inv2);
+    b[i] = e4m3x2(unpack_f32x2(fma_f32x2(fma_f32x2(q2, s2, y2), inv2, q2)));
   }
   const uint2 codes = make_uint2(b[0] | (uint32_t)b[1] << 16, b[2] | (uint32_t)b[3] << 16);
   *reinterpret_cast<uint2*>(p.q + (row * p.h8 + vec) * 8) = codes;
   if ((vec & 15) == 0) p.scales[(long long)(vec >> 4) * p.scales_ld + row] = scale;
 }
 
-// h = x (+ r), and the sum of its squares.
+// h = x (+ r), and the sum of its squares: two operations an instruction, here and in
+// store_vec, since with the conversions a row's arithmetic would otherwise take longer
+// to issue than its bytes to arrive.
 template <bool F16>
 __device__ __forceinline__ float add_vec(const NormParams& p, uint4 x, uint4 r, uint64_t (&h)[4]) {
   float v[8];
   unpack8<F16>(x, v);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) h[i] = pair(v[2 * i], v[2 * i + 1]);
+  for (int i = 0; i < 4; ++i) h[i] = f32x2(v[2 * i], v[2 * i + 1]);
   if (p.residual != nullptr) {
     unpack8<F16>(r, v);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = add2(h[i], pair(v[2 * i], v[2 * i + 1]));
+    for (int i = 0; i < 4; ++i) h[i] = add_f32x2(h[i], f32x2(v[2 * i], v[2 * i + 1]));
   }
-  uint64_t s = mul2(h[0], h[0]);
+  uint64_t s = mul_f32x2(h[0], h[0]);
 #pragma unroll
-  for (int i = 1; i < 4; ++i) s = fma2(h[i], h[i], s);
-  const float2 t = unpair(s);
+  for (int i = 1; i < 4; ++i) s = fma_f32x2(h[i], h[i], s);
+  const float2 t = unpack_f32x2(s);
   return t.x + t.y;
 }
 
@@ -239,7 +214,7 @@ __device__ __forceinline__ uint4 pack8(const uint64_t (&h)[4]) {
   float v[8];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float2 t = unpair(h[i]);
+    const float2 t = unpack_f32x2(h[i]);
     v[2 * i] = t.x;
     v[2 * i + 1] = t.y;
   }
