@@ -449,6 +449,29 @@ int b200_w8a8_moe_gemm(const void* a, int32_t a_dtype, int64_t a_rows, int64_t k
                        void* c, int32_t c_dtype, int64_t ldc, void* workspace,
                        int64_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------- 8-bit integer linear */
+
+/*
+ * Linear with 8-bit integer weights and activations (no counterpart in the
+ * reference; upstream SGLang's w8a8_int8 arithmetic): x [m, k] is quantized per
+ * token,
+ *   s[t] = max_k |x[t, k]| / 127,  q[t, k] = rint(x[t, k] / s[t])  (0 where s is 0),
+ *   y[t, n] = (sum_k q[t, k] * w[n, k]) * s[t] * w_scales[n],
+ * the sum exact in int32, the rest fp32. A token with an infinity or NaN has a
+ * NaN scale, codes of zero, and NaN outputs. w int8 [n, k] row-major, any values
+ * (-128 included), w_scales fp32 [n]; k a multiple of 16 up to 131072, any m and
+ * n. No workspace; b200_int8_linear takes q [m, k] and scales [m] to leave the
+ * quantized activations in.
+ */
+int b200_int8_act_quant(const void* x, int32_t x_dtype, int64_t rows, int64_t k, int8_t* q,
+                        float* scales, void* stream);
+int b200_int8_linear_quantized(const int8_t* q, const float* scales, int64_t m, int64_t k,
+                               const int8_t* w, const float* w_scales, int64_t n, void* y,
+                               int32_t y_dtype, void* stream);
+int b200_int8_linear(const void* x, int32_t x_dtype, int64_t m, int64_t k, const int8_t* w,
+                     const float* w_scales, int64_t n, int8_t* q, float* scales, void* y,
+                     int32_t y_dtype, void* stream);
+
 /* ------------------------------- norm, key/value cache, paged attention */
 
 /*

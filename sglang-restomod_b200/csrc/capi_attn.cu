@@ -3,110 +3,15 @@
 // activations that are already quantized. Host-side validation and launches;
 // declared in include/b200moe.h.
 #include <cmath>
-#include <cstdarg>
-#include <cstdio>
 
-#include "../../include/b200moe.h"
-#include "internal.h"
-
-namespace {
+#include "capi_checks.h"
 
 using namespace b200;
 
-int fail(int code, const char* fmt, ...) {
-  char buf[512];
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(buf, sizeof(buf), fmt, ap);
-  va_end(ap);
-  return set_last_error(code, buf);
-}
-
-int check_cuda(cudaError_t err, const char* what) {
-  if (err == cudaSuccess) return B200_OK;
-  return fail(B200_ERR_CUDA, "%s: %s", what, cudaGetErrorString(err));
-}
+namespace {
 
 // The current device's status word (its address is looked up once per device).
 __device__ int g_status;
-int status_word(int** out) {
-  static std::mutex mu;
-  static int* words[64] = {};
-  int dev = 0;
-  int rc = check_cuda(cudaGetDevice(&dev), "current device");
-  if (rc) return rc;
-  if (dev < 0 || dev >= 64) return fail(B200_ERR_CUDA, "device %d", dev);
-  const std::lock_guard<std::mutex> lock(mu);
-  if (words[dev] == nullptr) {
-    void* p = nullptr;
-    if ((rc = check_cuda(cudaGetSymbolAddress(&p, g_status), "status word"))) return rc;
-    words[dev] = static_cast<int*>(p);
-  }
-  *out = words[dev];
-  return B200_OK;
-}
-
-bool aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
-bool valid_dtype16(int32_t d) { return d == B200_DTYPE_BF16 || d == B200_DTYPE_F16; }
-
-// Vectors that are written must not share memory: with both strides at least a
-// vector, either order of tokens and heads, and only extents above one count.
-bool apart(int64_t token_stride, int64_t tokens, int64_t head_stride, int64_t heads, int64_t dim) {
-  if (tokens <= 1) return heads <= 1 || head_stride >= dim;
-  if (heads <= 1) return token_stride >= dim;
-  return head_stride <= token_stride
-             ? head_stride >= dim && token_stride >= (heads - 1) * head_stride + dim
-             : token_stride >= dim && head_stride >= (tokens - 1) * token_stride + dim;
-}
-
-// The cache's description, checked and in the kernels' form.
-int cache_view(const b200_kv_cache* c, KvCacheView& v) {
-  if (c == nullptr || c->k == nullptr || c->v == nullptr)
-    return fail(B200_ERR_INVALID, "null pointer argument");
-  if (c->dtype != B200_DTYPE_BF16 && c->dtype != B200_DTYPE_F16 && c->dtype != B200_DTYPE_E4M3)
-    return fail(B200_ERR_UNSUPPORTED, "the cache must hold bf16, f16 or e4m3, got dtype %d", c->dtype);
-  if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
-    return fail(B200_ERR_UNSUPPORTED, "head_dim must be 64, 128 or 256, got %d", c->head_dim);
-  if (c->num_pages <= 0 || c->page_size <= 0 || c->kv_heads <= 0)
-    return fail(B200_ERR_INVALID, "needs positive pages, page size and heads, got %lld, %d, %d",
-                (long long)c->num_pages, c->page_size, c->kv_heads);
-  if (c->num_pages > 0x7fffffffll / c->page_size)
-    return fail(B200_ERR_UNSUPPORTED, "the cache holds more than 2^31 - 1 tokens");
-  const bool quantized = c->dtype == B200_DTYPE_E4M3;
-  if (quantized != (c->k_scale != nullptr) || quantized != (c->v_scale != nullptr))
-    return fail(B200_ERR_INVALID, "scales belong to an e4m3 cache, and an e4m3 cache needs both");
-  const int64_t unit = quantized ? 16 : 8;  // elements of 16 bytes
-  if (!aligned(c->k, 16) || !aligned(c->v, 16) || c->page_stride % unit || c->token_stride % unit ||
-      c->head_stride % unit)
-    return fail(B200_ERR_INVALID, "the cache's vectors must be 16-byte aligned");
-  if (c->page_stride < 0 || c->token_stride < 0 || c->head_stride < 0 || c->scale_page_stride < 0 ||
-      c->scale_token_stride < 0 || c->scale_head_stride < 0)
-    return fail(B200_ERR_INVALID, "negative strides");
-  v.k = c->k;
-  v.v = c->v;
-  v.k_scale = c->k_scale;
-  v.v_scale = c->v_scale;
-  v.num_pages = c->num_pages;
-  v.page_stride = c->page_stride;
-  v.token_stride = c->token_stride;
-  v.head_stride = c->head_stride;
-  v.scale_page_stride = c->scale_page_stride;
-  v.scale_token_stride = c->scale_token_stride;
-  v.scale_head_stride = c->scale_head_stride;
-  v.page_size = c->page_size;
-  v.heads = c->kv_heads;
-  v.head_dim = c->head_dim;
-  return B200_OK;
-}
-
-// Token and head strides of a [tokens][heads][head_dim] operand, in elements.
-int check_rows(const char* what, const void* base, int64_t token_stride, int64_t head_stride) {
-  if (base == nullptr) return fail(B200_ERR_INVALID, "null pointer argument");
-  if (!aligned(base, 16) || token_stride % 8 || head_stride % 8)
-    return fail(B200_ERR_INVALID, "%s: every vector must be 16-byte aligned", what);
-  if (token_stride < 0 || head_stride < 0) return fail(B200_ERR_INVALID, "negative strides");
-  return B200_OK;
-}
 
 int check_copy(const b200_kv_cache* c, int32_t dtype, const int64_t* slots, int64_t tokens,
                KvCacheView& v) {
@@ -125,12 +30,29 @@ int check_copy(const b200_kv_cache* c, int32_t dtype, const int64_t* slots, int6
 
 }  // namespace
 
+int b200::device_status_word(int** out) {
+  static std::mutex mu;
+  static int* words[64] = {};
+  int dev = 0;
+  int rc = check_cuda(cudaGetDevice(&dev), "current device");
+  if (rc) return rc;
+  if (dev < 0 || dev >= 64) return fail(B200_ERR_CUDA, "device %d", dev);
+  const std::lock_guard<std::mutex> lock(mu);
+  if (words[dev] == nullptr) {
+    void* p = nullptr;
+    if ((rc = check_cuda(cudaGetSymbolAddress(&p, g_status), "status word"))) return rc;
+    words[dev] = static_cast<int*>(p);
+  }
+  *out = words[dev];
+  return B200_OK;
+}
+
 extern "C" {
 
 int b200_device_status(int32_t* bits, int32_t reset, void* stream) {
   if (bits == nullptr) return fail(B200_ERR_INVALID, "null pointer argument");
   int* word = nullptr;
-  const int rc = status_word(&word);
+  const int rc = device_status_word(&word);
   return rc ? rc : b200_workspace_status(word, bits, reset, stream);
 }
 
@@ -188,7 +110,7 @@ int b200_add_rms_norm(const void* x, int32_t dtype, int64_t x_ld, int64_t rows, 
   l.weight_dtype = weight_dtype;
   l.eps = eps;
   l.weight_bias = weight_bias;
-  const int rc = status_word(&l.status);
+  const int rc = device_status_word(&l.status);
   if (rc) return rc;
   return check_cuda(launch_add_rms_norm(l, reinterpret_cast<cudaStream_t>(stream)), "RMS norm launch");
 }
@@ -298,7 +220,7 @@ int b200_paged_attention(const b200_kv_cache* cache, const void* q, int32_t dtyp
   l.lse = lse;
   uint8_t* base = static_cast<uint8_t*>(workspace);
   l.status.call = reinterpret_cast<int*>(base);
-  if ((rc = status_word(&l.status.device))) return rc;
+  if ((rc = device_status_word(&l.status.device))) return rc;
   l.counters = reinterpret_cast<int*>(base + ws_counter_offset());
   l.scratch = base + fixed;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);

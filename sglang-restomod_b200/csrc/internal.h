@@ -258,6 +258,25 @@ cudaError_t launch_fp8_act_quant(const void* x, int x_f16, long long x_rows, int
                                  long long out_rows, uint8_t* q, float* scales, long long ld,
                                  int* status, cudaStream_t stream);
 
+// 8-bit integer linear (int8_linear.cu). q [rows][k] codes of x [rows][k] with
+// one scale a row; y [m][n] = (q . w^T) * x_scales[m] * w_scales[n]. k a multiple
+// of 16; early: the launch before on the stream wrote nothing but q and x_scales.
+cudaError_t launch_int8_quant(const void* x, bool f16, long long rows, int k, int8_t* q,
+                              float* scales, cudaStream_t stream);
+struct Int8Launch {
+  const int8_t* q;
+  const float* x_scales;
+  const int8_t* w;       // [n][k]
+  const float* w_scales; // [n]
+  long long m, n;
+  int k;
+  bool early;
+  void* out;
+  int out_f16;
+  int* status;
+};
+cudaError_t launch_int8_gemm(const Int8Launch& l, cudaStream_t stream);
+
 // Residual-add RMS norm (norm.cu). Strides in elements; nullptr residual /
 // residual_out / y / q: not given or not wanted. hidden % 8 == 0, and % 128
 // with q; scales [hidden / 128][scales_ld].
@@ -349,6 +368,9 @@ inline long long attn_scratch_bytes(int head_dim, long long q_tokens, int seqs) 
 // operands, partial sums), and when two threads call on one stream no other
 // call's kernel, a single one either, may come between them.
 std::mutex& launch_mutex();
+
+// The current device's status word (capi_attn.cu), or an error code.
+int device_status_word(int** out);
 
 // Records `message` as this thread's b200_last_error() and returns `code`.
 int set_last_error(int code, const char* message);

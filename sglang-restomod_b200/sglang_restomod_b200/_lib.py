@@ -161,6 +161,19 @@ SIGNATURES = {
          c_void_p, c_void_p, c_int64, c_void_p, c_int32, c_int32, c_int64, c_void_p, c_int32,
          c_void_p, c_int32, c_int64, c_void_p, c_int64, c_void_p],
     ),
+    "b200_int8_act_quant": (
+        c_int32, [c_void_p, c_int32, c_int64, c_int64, c_void_p, c_void_p, c_void_p]
+    ),
+    "b200_int8_linear_quantized": (
+        c_int32,
+        [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int32,
+         c_void_p],
+    ),
+    "b200_int8_linear": (
+        c_int32,
+        [c_void_p, c_int32, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p,
+         c_void_p, c_int32, c_void_p],
+    ),
     "b200_add_rms_norm": (
         c_int32,
         [c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int32,

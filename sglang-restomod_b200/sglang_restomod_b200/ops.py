@@ -737,6 +737,90 @@ def w8a8_linear_quantized(q: torch.Tensor, scales: torch.Tensor, w: torch.Tensor
     return out
 
 
+# --------------------------------------------------- 8-bit integer linear
+def _int8_weights(w: torch.Tensor, w_scales: torch.Tensor, k: int) -> int:
+    if w.dtype != torch.int8 or w_scales.dtype != torch.float32:
+        raise TypeError(f"the weight must be int8 and its scales float32, got {w.dtype}, "
+                        f"{w_scales.dtype}")
+    if w.dim() != 2 or w.shape[1] != k or w_scales.shape != w.shape[:1]:
+        raise ValueError(f"the weight must be [N, {k}] with scales [N], got {tuple(w.shape)}, "
+                         f"{tuple(w_scales.shape)}")
+    if not w.is_contiguous() or not w_scales.is_contiguous():
+        raise ValueError("the weight and its scales must be contiguous")
+    return int(w.shape[0])
+
+
+def _int8_rows(t: torch.Tensor, what: str) -> None:
+    if t.dim() != 2 or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous [M, K], got {tuple(t.shape)} strides {t.stride()}")
+
+
+def _int8_out(out, m, n, dtype, device):
+    if out is None:
+        return torch.empty(m, n, dtype=dtype, device=device)
+    if out.shape != (m, n) or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous [{m}, {n}], got {tuple(out.shape)} "
+                         f"strides {out.stride()}")
+    return out
+
+
+def int8_act_quant(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Per-token quantization of ``x`` ``[M, K]`` (bf16 or f16): ``scale = max|x| /
+    127``, int8 codes ``rint(x / scale)``. A token with an infinity or NaN has a NaN
+    scale. Returns (codes ``[M, K]``, fp32 scales ``[M]``)."""
+    index = _on_device("int8_act_quant", x)
+    _int8_rows(x, "x")
+    m, k = x.shape
+    code = _code(x, "x")
+    q = torch.empty(m, k, dtype=torch.int8, device=x.device)
+    scales = torch.empty(m, dtype=torch.float32, device=x.device)
+    _lib.check(lib().b200_int8_act_quant(x.data_ptr(), code, m, k, q.data_ptr(), scales.data_ptr(),
+                                         _raw_stream(index)))
+    return q, scales
+
+
+def int8_linear(x: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, *,
+                out: torch.Tensor | None = None,
+                out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """``y = x W^T`` with 8-bit integer products: ``x`` ``[..., K]`` (bf16 or f16) is
+    quantized per token as :func:`int8_act_quant` does, ``w`` int8 ``[N, K]`` has an
+    fp32 scale per output channel ``[N]``. K a multiple of 16; any N. ``out``
+    ``[M, N]`` and ``out_dtype``: bf16 or f16, by default ``x``'s type."""
+    index = _on_device("int8_linear", x, w, w_scales, out)
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    _int8_rows(x2, "x")
+    m, k = x2.shape
+    n = _int8_weights(w, w_scales, k)
+    code = _code(x2, "x")
+    out = _int8_out(out, m, n, out_dtype or x.dtype, x.device)
+    # the codes and their scales, in one allocation
+    buf = torch.empty(m * k + 4 * m, dtype=torch.int8, device=x.device)
+    _lib.check(lib().b200_int8_linear(
+        x2.data_ptr(), code, m, k, w.data_ptr(), w_scales.data_ptr(), n, buf.data_ptr(),
+        buf.data_ptr() + m * k, out.data_ptr(), _code(out, "out"), _raw_stream(index)))
+    return out if x.dim() == 2 else out.view(*x.shape[:-1], n)
+
+
+def int8_linear_quantized(q: torch.Tensor, scales: torch.Tensor, w: torch.Tensor,
+                          w_scales: torch.Tensor, *, out: torch.Tensor | None = None,
+                          out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """:func:`int8_linear` on activations that are already quantized: ``q`` int8
+    ``[M, K]`` and fp32 ``scales`` ``[M]``, as :func:`int8_act_quant` returns them."""
+    index = _on_device("int8_linear_quantized", q, scales, w, w_scales, out)
+    _int8_rows(q, "q")
+    m, k = q.shape
+    if q.dtype != torch.int8 or scales.dtype != torch.float32:
+        raise TypeError(f"q must be int8 and scales float32, got {q.dtype}, {scales.dtype}")
+    if scales.shape != (m,) or not scales.is_contiguous():
+        raise ValueError(f"scales must be a contiguous [{m}], got {tuple(scales.shape)}")
+    n = _int8_weights(w, w_scales, k)
+    out = _int8_out(out, m, n, out_dtype, q.device)
+    _lib.check(lib().b200_int8_linear_quantized(
+        q.data_ptr(), scales.data_ptr(), m, k, w.data_ptr(), w_scales.data_ptr(), n, out.data_ptr(),
+        _code(out, "out"), _raw_stream(index)))
+    return out
+
+
 # ------------------------------------------- norm, key/value cache, attention
 # Decode calls these several times a layer on microseconds of GPU work, so the
 # wrappers keep their own host time low: plain integers instead of ctypes
