@@ -576,6 +576,31 @@ int b200_paged_attention(const b200_kv_cache* cache, const void* q, int32_t dtyp
                          int64_t out_head_stride, float* lse, void* workspace,
                          int64_t workspace_bytes, void* stream);
 
+/*
+ * b200_paged_attention of a batch whose sequences share long prefixes, each
+ * prefix read once for all of its sequences. Group g is the sequences
+ * group_starts[g] .. group_starts[g + 1] (group_starts[0 .. groups] ascends from 0
+ * to seqs); its prefix is the first prefix_lens[g] tokens (0: none) of the pages
+ * prefix_table[g * prefix_table_stride ..], prefix_table_width entries. Sequence
+ * s has kv_lens[s] cached tokens of its own, which come after its group's prefix:
+ * the tables of both may name any pages, and a prefix may end within a page. Every
+ * new token sees its group's whole prefix, and of its sequence's own tokens those at
+ * its position and before. lse is over both. The rest as in
+ * b200_paged_attention. Both passes' results are held in fp32 in the workspace
+ * (8 bytes a query element), and rounded once, when they are added.
+ */
+int64_t b200_shared_prefix_attention_workspace_bytes(int32_t head_dim, int64_t q_tokens,
+                                                     int32_t q_heads, int32_t seqs, int32_t groups);
+int b200_shared_prefix_attention(
+    const b200_kv_cache* cache, const void* q, int32_t dtype, int64_t q_tokens, int32_t q_heads,
+    int64_t q_token_stride, int64_t q_head_stride, const int32_t* prefix_table,
+    int64_t prefix_table_stride, int32_t prefix_table_width, const int32_t* prefix_lens,
+    const int32_t* group_starts, int32_t groups, const int32_t* page_table,
+    int64_t page_table_stride, int32_t page_table_width, const int32_t* kv_lens,
+    const int32_t* q_starts, int32_t seqs, int32_t max_q_len, float scale, void* out,
+    int64_t out_token_stride, int64_t out_head_stride, float* lse, void* workspace,
+    int64_t workspace_bytes, void* stream);
+
 /* ---------------------------------------- expert parallelism (peer memory) */
 
 /*

@@ -75,3 +75,33 @@ def paged_attention_ref(q, k_cache, v_cache, table, kv_lens, q_starts, scale, ca
             # a masked token weighs nothing, whatever its value holds
             out[a:b, h] = p @ torch.where(seen.any(0)[:, None], v[:, h // groups], 0.0)
     return out, lse
+
+
+def _cached(cache, table, n):
+    """The first n tokens of a page table's row: [n, heads, dim]."""
+    at = torch.arange(n)
+    return cache[table.long()[at // cache.shape[1]], at % cache.shape[1]].double()
+
+
+def shared_prefix_attention_ref(q, k_cache, v_cache, prefix_table, prefix_lens, group_starts, table,
+                                kv_lens, q_starts, scale):
+    """(out, lse) in float64: each sequence's new tokens over its group's prefix, whole,
+    and its own tokens, causally."""
+    groups = q.shape[1] // k_cache.shape[2]
+    out = torch.zeros(q.shape, dtype=torch.float64)
+    lse = torch.full(q.shape[:2], -math.inf, dtype=torch.float64)
+    for g, far in enumerate(prefix_lens.tolist()):
+        for s in range(int(group_starts[g]), int(group_starts[g + 1])):
+            a, b, kv = int(q_starts[s]), int(q_starts[s + 1]), int(kv_lens[s])
+            k, v = (torch.cat([_cached(c, prefix_table[g], far), _cached(c, table[s], kv)])
+                    for c in (k_cache, v_cache))
+            if a == b or not len(k):
+                continue
+            at = torch.cat([torch.full((far,), -1 << 31), torch.arange(kv)])
+            seen = at[None, :] <= kv - (b - a) + torch.arange(b - a)[:, None]
+            for h in range(q.shape[1]):
+                x = (q[a:b, h].double() @ k[:, h // groups].T * scale).masked_fill(~seen, -math.inf)
+                lse[a:b, h] = torch.logsumexp(x, -1)
+                p = torch.exp(x - torch.where(lse[a:b, h] > -math.inf, lse[a:b, h], 0.0)[:, None])
+                out[a:b, h] = p @ torch.where(seen.any(0)[:, None], v[:, h // groups], 0.0)
+    return out, lse

@@ -236,6 +236,15 @@ __device__ __forceinline__ SeqRange seq_range(const AttnLaunch& a, int s, int al
   return r;
 }
 
+template <int D>
+__device__ __forceinline__ void store_out(const AttnLaunch& a, long long token, int qh, int d, float x) {
+  if (a.out32 != nullptr)
+    a.out32[(token * a.q_heads + qh) * D + d] = x;
+  else
+    static_cast<uint16_t*>(a.out)[token * a.out_token_stride + qh * a.out_head_stride + d] =
+        a.q_f16 ? __half_as_ushort(__float2half_rn(x)) : __bfloat16_as_ushort(__float2bfloat16_rn(x));
+}
+
 template <int D, int KV, int NR, bool TMA>
 __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, NR, TMA>::kBlocks)
     attn_decode_kernel(const DecodeParams p, const __grid_constant__ CUtensorMap k_map,
@@ -973,10 +982,7 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
         if (whole) {
           const float sum = sm.sum[r];
           const float x = sum == 0.f ? 0.f : v / sum;
-          static_cast<uint16_t*>(a.out)[(long long)(q0 + r / p.groups) * a.out_token_stride +
-                                        (long long)(head * p.groups + r % p.groups) * a.out_head_stride +
-                                        d] =
-              a.q_f16 ? __half_as_ushort(__float2half_rn(x)) : __bfloat16_as_ushort(__float2bfloat16_rn(x));
+          store_out<D>(a, q0 + r / p.groups, head * p.groups + r % p.groups, d, x);
         } else {
           part[r * row_floats + 4 + d] = v;
         }
@@ -1080,8 +1086,7 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
             const float x = sum == 0.f ? 0.f : v / sum;
             const long long tok = q0 + r / p.groups;
             const int qh = head * p.groups + r % p.groups;
-            static_cast<uint16_t*>(a.out)[tok * a.out_token_stride + qh * a.out_head_stride + d] =
-                a.q_f16 ? __half_as_ushort(__float2half_rn(x)) : __bfloat16_as_ushort(__float2bfloat16_rn(x));
+            store_out<D>(a, tok, qh, d, x);
             if (a.lse != nullptr && d == 0)
               a.lse[tok * a.q_heads + qh] =
                   sum == 0.f ? -INFINITY : (sm.mx[r] + log2f(sum)) / kLog2e;

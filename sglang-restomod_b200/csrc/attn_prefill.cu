@@ -63,6 +63,8 @@
 // (Tried without gain: half rows by four warpgroups, keys by 64 with four S
 // buffers, polynomials for an eighth to a half of the exponentials, P handed
 // over in halves.) 512 tokens on 16384 e4m3 ones: 163 us, 830 TFLOP/s; bf16 130.
+#include <algorithm>
+
 #include "attn_maps.cuh"
 #include "common.cuh"
 #include "internal.h"
@@ -97,10 +99,11 @@ struct PrefillParams {
   int tile_tokens;  // new tokens per 128 rows: 128 / groups
   float scale_log2;
   // the plan (attn_plan_kernel), in the scratch
-  long long* head;  // [0] cost in all, [1] blocks
+  long long* head;  // [0] cost in all, [1] blocks, [2] units
   int4* start;      // per block: unit, head, place in the unit's cost
   int* seq_base;    // units before each sequence
   int4* units;      // sequence, first token in it, first key, key tiles
+  long long* unit_at;  // place of each unit's first cost (nullptr: not wanted)
   int max_units;
   float* parts;
   // tensor copies: rows of a page that one copy takes (a power of two that
@@ -352,7 +355,7 @@ struct SeqLens {
 };
 __device__ __forceinline__ SeqLens seq_lens(const AttnLaunch& a, int s) {
   SeqLens r;
-  const int q0 = __ldg(a.q_starts + s), q1 = __ldg(a.q_starts + s + 1);
+  const int q0 = a.q_start(s), q1 = a.q_start(s + 1);
   const long long cap = (long long)a.table_width * a.c.page_size;
   int kv = max(__ldg(a.kv_lens + s), 0);
   if (kv > cap) kv = (int)cap;
@@ -449,16 +452,20 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const PrefillPa
       begin -= begin % p.box_rows;
       const int tiles = end > begin ? (end - begin + bn - 1) / bn : 1;
       p.units[u] = make_int4(s, tok0, begin, tiles);
+      if (p.unit_at != nullptr) p.unit_at[u] = mine;  // (from unit u0; see below)
       mine += (long long)(tiles + kUnitCost) * a.c.heads;
     }
   }
   const long long at = block_scan(mine, sh, total);
   at_sh[tid] = at;  // of unit u0; `total` where the thread has none
+  if (p.unit_at != nullptr)
+    for (int u = u0; u < u1; ++u) p.unit_at[u] += at;
   long long ctas = (total + kMinTiles - 1) / kMinTiles;
   if (ctas > max_ctas) ctas = max_ctas;
   if (tid == 0) {
     p.head[0] = total;
     p.head[1] = ctas;
+    p.head[2] = units;
   }
   __syncthreads();
   // A thread per block finds the unit of the block's first place. (A thread per
@@ -735,20 +742,121 @@ __global__ void __launch_bounds__(128) attn_combine_kernel(const PrefillParams p
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const long long token = (long long)q.q0 + tok;
   const int qh = s.y * p.groups + row % p.groups;
-  uint16_t* out = static_cast<uint16_t*>(a.out) + token * a.out_token_stride +
-                  (long long)qh * a.out_head_stride + col;
+  if (a.out32 != nullptr) {
+    float* out = a.out32 + (token * a.q_heads + qh) * d + col;
 #pragma unroll
-  for (int i = 0; i < kCombineCols; i += 8) {
-    uint32_t w[4];
+    for (int i = 0; i < kCombineCols; i += 4)
+      *reinterpret_cast<float4*>(out + i) =
+          make_float4(acc[i] * inv, acc[i + 1] * inv, acc[i + 2] * inv, acc[i + 3] * inv);
+  } else {
+    uint16_t* out = static_cast<uint16_t*>(a.out) + token * a.out_token_stride +
+                    (long long)qh * a.out_head_stride + col;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float x = acc[i + 2 * j] * inv, y = acc[i + 2 * j + 1] * inv;
-      w[j] = a.q_f16 ? pack2<true>(x, y) : pack2<false>(x, y);
+    for (int i = 0; i < kCombineCols; i += 8) {
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float x = acc[i + 2 * j] * inv, y = acc[i + 2 * j + 1] * inv;
+        w[j] = a.q_f16 ? pack2<true>(x, y) : pack2<false>(x, y);
+      }
+      *reinterpret_cast<uint4*>(out + i) = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    *reinterpret_cast<uint4*>(out + i) = make_uint4(w[0], w[1], w[2], w[3]);
   }
   if (col == 0 && a.lse != nullptr)
     a.lse[token * a.q_heads + qh] = l == 0.f ? -INFINITY : (m + log2f(l)) / kLog2e;
+}
+
+// Where sequences share prefixes: for each row the parts of the pass over its
+// group's prefix (or the row that one block finished) and the row of the pass over
+// its sequence's own tokens, added as attn_combine_kernel adds parts. A finished row
+// is a part with m = lse and l = 1. Rows that the own pass left alone (past max_q, or
+// of no sequence) keep their mark and are left alone here. Threads as there; a block
+// goes through the (unit, head) pairs.
+struct PrefixEnds {
+  const float* own_out;  // fp32 [q_tokens][q_heads][d]
+  const float* own_lse;
+  void* out;
+  float* lse;
+};
+__global__ void __launch_bounds__(128) attn_prefix_finish_kernel(const PrefillParams p,
+                                                                 const PrefixEnds e, int d, int mt) {
+  griddep_wait();
+  const AttnLaunch& a = p.a;
+  const long long total = __ldcg(p.head), ctas = __ldcg(p.head + 1), units = __ldcg(p.head + 2);
+  const int groups = d / kCombineCols, tile = blockIdx.y / groups;
+  const int col = blockIdx.y % groups * kCombineCols, row = threadIdx.x;
+  for (long long pair = blockIdx.x; pair < units * a.c.heads; pair += gridDim.x) {
+    const int unit = (int)(pair / a.c.heads), head = (int)(pair % a.c.heads);
+    const int4 u = __ldcg(p.units + unit);
+    const SeqLens q = seq_lens(a, u.x);
+    const int tok = u.y + tile * p.tile_tokens + row / p.groups;
+    if (row >= p.tile_tokens * p.groups || tok >= q.q_len) continue;
+    const long long token = (long long)q.q0 + tok;
+    const int qh = head * p.groups + row % p.groups;
+    const long long at_row = token * a.q_heads + qh;
+    const float own = __ldcg(e.own_lse + at_row);
+    if (__float_as_uint(own) == kNoRow) continue;
+    float m = -INFINITY, l = 0.f, acc[kCombineCols];
+#pragma unroll
+    for (int i = 0; i < kCombineCols; ++i) acc[i] = 0.f;
+    auto add = [&](float mb, float lb, const float (&v)[kCombineCols]) {
+      if (mb == -INFINITY && lb == 0.f) return;
+      const float mn = fmaxf(m, mb);
+      const float f = m == mn ? 1.f : ex2(m - mn), w = mb == mn ? 1.f : ex2(mb - mn);
+      m = mn;
+      l = l * f + lb * w;
+#pragma unroll
+      for (int i = 0; i < kCombineCols; ++i) acc[i] = acc[i] * f + v[i] * w;
+    };
+    auto add_row = [&](const float* rows, float lse) {
+      float v[kCombineCols];
+#pragma unroll
+      for (int i = 0; i < kCombineCols; i += 4) {
+        const float4 x = __ldcg(reinterpret_cast<const float4*>(rows + at_row * d + col + i));
+        v[i] = x.x, v[i + 1] = x.y, v[i + 2] = x.z, v[i + 3] = x.w;
+      }
+      add(lse * kLog2e, lse == -INFINITY ? 0.f : 1.f, v);
+    };
+    const int cost = u.w + kUnitCost;
+    const long long t = __ldcg(p.unit_at + unit) + (long long)head * cost;
+    const long long first = ((t + kUnitCost + 1) * ctas - 1) / total;
+    const long long last = ((t + cost) * ctas - 1) / total;
+    if (first == last) {
+      add_row(a.out32, __ldcg(a.lse + at_row));
+    } else {
+      constexpr int kBatch = 4;  // parts on their way together
+      for (long long b0 = first; b0 <= last; b0 += kBatch) {
+        float mb[kBatch], lb[kBatch], v[kBatch][kCombineCols];
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          const bool on = b0 + j <= last;
+          const float* part =
+              p.parts + part_at(on ? b0 + j : last, on && b0 + j == first, mt, tile, d) + row;
+          mb[j] = on ? __ldcg(part) : -INFINITY;
+          lb[j] = on ? __ldcg(part + 128) : 0.f;
+#pragma unroll
+          for (int i = 0; i < kCombineCols; ++i) v[j][i] = __ldcg(part + (2 + col + i) * 128);
+        }
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) add(mb[j], lb[j], v[j]);
+      }
+    }
+    add_row(e.own_out, own);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    uint16_t* out = static_cast<uint16_t*>(e.out) + token * a.out_token_stride +
+                    (long long)qh * a.out_head_stride + col;
+#pragma unroll
+    for (int i = 0; i < kCombineCols; i += 8) {
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float x = acc[i + 2 * j] * inv, y = acc[i + 2 * j + 1] * inv;
+        w[j] = a.q_f16 ? pack2<true>(x, y) : pack2<false>(x, y);
+      }
+      *reinterpret_cast<uint4*>(out + i) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    if (col == 0 && e.lse != nullptr) e.lse[at_row] = l == 0.f ? -INFINITY : (m + log2f(l)) / kLog2e;
+  }
 }
 
 template <int D, int MT, int KV, bool TMA>
@@ -912,53 +1020,66 @@ __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
       const bool whole = g.tiles == g.unit_tiles;
       const long long token = (long long)q.q0 + tok;
       const int qh = g.head * p.groups + row_head;
-      // 32 columns of the warp's 32 rows, through shared memory so that a store
-      // covers 64 neighbouring bytes of each of 8 rows
+      if (a.mark != nullptr && valid)
+        a.mark[token * a.q_heads + qh] = __uint_as_float(kNoRow);
+      // 64 bytes of the warp's 32 rows (32 columns, or 16 in fp32), through shared
+      // memory so that a store covers 64 neighbouring bytes of each of 8 rows
+      const bool wide = a.out32 != nullptr;
       long long out_at[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int r = (warp & 3) * 32 + 8 * j + (lane >> 2);
         const int t = g.tok0 + wg * p.tile_tokens + r / p.groups;
+        const long long to_token = (long long)q.q0 + t;
+        const int to_head = g.head * p.groups + r % p.groups;
         out_at[j] = r < p.tile_tokens * p.groups && t < q.q_len
-                        ? ((long long)q.q0 + t) * a.out_token_stride +
-                              (long long)(g.head * p.groups + r % p.groups) * a.out_head_stride +
-                              (lane & 3) * 8
+                        ? (wide ? (to_token * a.q_heads + to_head) * (D * 4)
+                                : (to_token * a.out_token_stride + to_head * a.out_head_stride) * 2) +
+                              (lane & 3) * 16
                         : -1;
       }
+      uint8_t* out_base = wide ? reinterpret_cast<uint8_t*>(a.out32) : static_cast<uint8_t*>(a.out);
       uint8_t* stage_out = smem + S::kOffOut + warp * 2048;
-      auto emit = [&](int c, const float (&v)[32]) {
+      auto emit = [&](int c, const uint32_t (&w)[16]) {
         __syncwarp();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t w[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            w[j] = a.q_f16 ? pack2<true>(v[8 * i + 2 * j], v[8 * i + 2 * j + 1])
-                           : pack2<false>(v[8 * i + 2 * j], v[8 * i + 2 * j + 1]);
+        for (int i = 0; i < 4; ++i)
           *reinterpret_cast<uint4*>(stage_out + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) =
-              make_uint4(w[0], w[1], w[2], w[3]);
-        }
+              make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
         __syncwarp();
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int r = 8 * j + (lane >> 2);
           const uint4 x = *reinterpret_cast<const uint4*>(stage_out + r * 64 +
                                                           (((lane & 3) ^ ((r >> 1) & 3)) << 4));
-          if (out_at[j] >= 0)
-            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + out_at[j] + 32 * c) = x;
+          if (out_at[j] >= 0) *reinterpret_cast<uint4*>(out_base + out_at[j] + 64 * c) = x;
         }
       };
       if (whole) {
         const float inv = l == 0.f ? 0.f : 1.f / l;
+        if (wide) {
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t o[32];
-          float v[32];
-          tmem_ld32_nowait(to + 32 * c, o);
-          tmem_wait32(o);
+          for (int c = 0; c < D / 16; ++c) {
+            uint32_t o[16];
+            tmem_ld16_nowait(to + 16 * c, o);
+            tmem_wait16(o);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(o[i]) * inv;
-          emit(c, v);
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * inv);
+            emit(c, o);
+          }
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32], w[16];
+            tmem_ld32_nowait(to + 32 * c, o);
+            tmem_wait32(o);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float x = __uint_as_float(o[2 * i]) * inv, y = __uint_as_float(o[2 * i + 1]) * inv;
+              w[i] = a.q_f16 ? pack2<true>(x, y) : pack2<false>(x, y);
+            }
+            emit(c, w);
+          }
         }
         if (valid && a.lse != nullptr)
           a.lse[token * a.q_heads + qh] = l == 0.f ? -INFINITY : (m + log2f(l)) / kLog2e;
@@ -1484,7 +1605,7 @@ cudaError_t launch(const PrefillParams& p, const CUtensorMap (&maps)[3], cudaStr
   if (err != cudaSuccess) return err;
   err = launch_pdl(attn_prefill_kernel<D, MT, KV, TMA>, dim3((unsigned)sms), dim3(S::kThreads),
                    S::kSmem, stream, p, maps[0], maps[1], maps[2]);
-  if (err != cudaSuccess) return err;
+  if (err != cudaSuccess || p.unit_at != nullptr) return err;  // (its parts are added later)
   return launch_pdl(attn_combine_kernel, dim3((unsigned)sms, MT * (D / kCombineCols)), dim3(128), 0,
                     stream, p, D, MT);
 }
@@ -1542,7 +1663,19 @@ long long attn_prefill_scratch_bytes(int head_dim, long long q_tokens, int seqs)
          sms * 2 * (head_dim == 256 ? 1 : 2) * (head_dim + 2) * 128 * 4;
 }
 
-cudaError_t launch_attn_prefill(const AttnLaunch& l, cudaStream_t stream) {
+namespace {
+
+// Two tiles in turn pay where sequences fill several. Solo against duo in us,
+// head_dim 128, by rows of a sequence: 256 (16 x 4096 keys) bf16 55 / 62, e4m3
+// 93 / 115, single-token pages 71 / 73; 512 (4 x 4096) 35 / 38, 45 / 55, 42 /
+// 46; 1024 (16384) 87 / 78, 124 / 104, 95 / 85; 2048 (16384) e4m3 221 / 165;
+// 32768 (a prompt of 8192) bf16 613 / 506.
+bool two_tiles(const PrefillParams& p) {
+  const long long rows = p.a.unit_rows ? p.a.unit_rows : (long long)p.a.max_q * p.groups;
+  return p.a.c.head_dim != 256 && rows > 512;
+}
+
+PrefillParams prefill_params(const AttnLaunch& l) {
   PrefillParams p{};
   p.a = l;
   p.groups = l.q_heads / l.c.heads;
@@ -1562,17 +1695,65 @@ cudaError_t launch_attn_prefill(const AttnLaunch& l, cudaStream_t stream) {
   p.units = reinterpret_cast<int4*>(at);
   at += align256(16ll * p.max_units);
   p.parts = reinterpret_cast<float*>(at);
-  // Two tiles in turn pay where sequences fill several. Solo against duo in us,
-  // head_dim 128, by rows of a sequence: 256 (16 x 4096 keys) bf16 55 / 62, e4m3
-  // 93 / 115, single-token pages 71 / 73; 512 (4 x 4096) 35 / 38, 45 / 55, 42 /
-  // 46; 1024 (16384) 87 / 78, 124 / 104, 95 / 85; 2048 (16384) e4m3 221 / 165;
-  // 32768 (a prompt of 8192) bf16 613 / 506.
-  const bool duo = (long long)l.max_q * p.groups > 512;
-  switch (l.c.head_dim) {
+  return p;
+}
+
+cudaError_t launch_prefill(PrefillParams& p, cudaStream_t stream) {
+  const bool duo = two_tiles(p);
+  switch (p.a.c.head_dim) {
     case 64: return duo ? launch_type<64, 2>(p, stream) : launch_type<64, 1>(p, stream);
     case 128: return duo ? launch_type<128, 2>(p, stream) : launch_type<128, 1>(p, stream);
     default: return launch_type<256, 1>(p, stream);
   }
+}
+
+}  // namespace
+
+cudaError_t launch_attn_prefill(const AttnLaunch& l, cudaStream_t stream) {
+  PrefillParams p = prefill_params(l);
+  return launch_prefill(p, stream);
+}
+
+long long attn_prefix_scratch_bytes(int head_dim, long long q_tokens, int q_heads, int seqs,
+                                    int groups) {
+  const long long rows = q_tokens * q_heads;
+  return attn_prefill_scratch_bytes(head_dim, q_tokens, groups) +
+         align256(8 * max_units(q_tokens, groups)) +
+         align256(attn_scratch_bytes(head_dim, q_tokens, seqs)) + 2 * align256(4 * rows * head_dim) +
+         2 * align256(4 * rows);
+}
+
+cudaError_t launch_attn_prefix(AttnLaunch prefix, AttnLaunch own, cudaStream_t stream) {
+  const int d = own.c.head_dim;
+  const long long rows = own.q_tokens * own.q_heads;
+  uint8_t* at = prefix.scratch;
+  auto take = [&](long long bytes) {
+    uint8_t* here = at;
+    at += align256(bytes);
+    return here;
+  };
+  take(attn_prefill_scratch_bytes(d, prefix.q_tokens, prefix.seqs));
+  long long* unit_at = reinterpret_cast<long long*>(take(8 * max_units(prefix.q_tokens, prefix.seqs)));
+  own.scratch = take(attn_scratch_bytes(d, own.q_tokens, own.seqs));
+  const PrefixEnds ends{reinterpret_cast<float*>(take(4 * rows * d)),
+                        reinterpret_cast<float*>(take(4 * rows)), own.out, own.lse};
+  prefix.out32 = reinterpret_cast<float*>(take(4 * rows * d));
+  prefix.lse = reinterpret_cast<float*>(take(4 * rows));
+  prefix.mark = const_cast<float*>(ends.own_lse);
+  own.out32 = const_cast<float*>(ends.own_out);
+  own.lse = const_cast<float*>(ends.own_lse);
+  PrefillParams p = prefill_params(prefix);
+  p.unit_at = unit_at;
+  cudaError_t err = launch_prefill(p, stream);
+  if (err != cudaSuccess) return err;
+  const bool few = (long long)own.max_q * p.groups <= attn_decode_rows(own);
+  err = few ? launch_attn_decode(own, stream) : launch_attn_prefill(own, stream);
+  if (err != cudaSuccess) return err;
+  const int mt = two_tiles(p) ? 2 : 1;
+  const long long pairs = (long long)p.max_units * own.c.heads;
+  const long long blocks = std::min<long long>(pairs, 2ll * device_sm_count());
+  return launch_pdl(attn_prefix_finish_kernel, dim3((unsigned)blocks, mt * (d / kCombineCols)),
+                    dim3(128), 0, stream, p, ends, d, mt);
 }
 
 }  // namespace b200

@@ -28,6 +28,86 @@ int check_copy(const b200_kv_cache* c, int32_t dtype, const int64_t* slots, int6
   return B200_OK;
 }
 
+// What both attention calls take, checked and in the kernels' form; `none`: there is
+// nothing to do.
+int attention_args(const b200_kv_cache* cache, const void* q, int32_t dtype, int64_t q_tokens,
+                   int32_t q_heads, int64_t q_token_stride, int64_t q_head_stride,
+                   const int32_t* page_table, int64_t page_table_stride, int32_t page_table_width,
+                   const int32_t* kv_lens, const int32_t* q_starts, int32_t seqs,
+                   int32_t max_q_len, float scale, int32_t causal, int32_t window, void* out,
+                   int64_t out_token_stride, int64_t out_head_stride, float* lse, AttnLaunch& l,
+                   bool& none) {
+  none = false;
+  int rc = cache_view(cache, l.c);
+  if (rc) return rc;
+  if (!valid_dtype16(dtype)) return fail(B200_ERR_UNSUPPORTED, "q must be bf16 or f16");
+  if (cache->dtype != B200_DTYPE_E4M3 && cache->dtype != dtype)
+    return fail(B200_ERR_INVALID, "a 16-bit cache takes queries of its own type");
+  if (q_heads <= 0 || q_heads % cache->kv_heads)
+    return fail(B200_ERR_INVALID, "%d query heads cannot share %d key/value heads", q_heads,
+                cache->kv_heads);
+  if (q_heads / cache->kv_heads > 128)
+    return fail(B200_ERR_UNSUPPORTED, "at most 128 query heads per key/value head, got %d",
+                q_heads / cache->kv_heads);
+  if (seqs < 0 || q_tokens < 0 || q_tokens + seqs > 0x7fffffffll || max_q_len < 0 || page_table_width < 0)
+    return fail(B200_ERR_INVALID, "negative or too large count");
+  if (window < 0 || (window > 0 && !causal))
+    return fail(B200_ERR_INVALID, "a window needs causal attention and at least one token");
+  // (in units of log2, as the kernels use it)
+  if (!std::isfinite(scale * 1.4426950408889634f))
+    return fail(B200_ERR_INVALID, "the scale must be finite");
+  if (seqs == 0 || q_tokens == 0 || max_q_len == 0) {
+    none = true;
+    return B200_OK;
+  }
+  if ((rc = check_rows("q", q, q_token_stride, q_head_stride))) return rc;
+  if ((rc = check_rows("out", out, out_token_stride, out_head_stride))) return rc;
+  if (!apart(out_token_stride, q_tokens, out_head_stride, q_heads, l.c.head_dim))
+    return fail(B200_ERR_INVALID, "the output's vectors overlap");
+  if (kv_lens == nullptr || q_starts == nullptr || (page_table_width > 0 && page_table == nullptr))
+    return fail(B200_ERR_INVALID, "null pointer argument");
+  if (!aligned(page_table, 4) || !aligned(kv_lens, 4) || !aligned(q_starts, 4) || !aligned(lse, 4))
+    return fail(B200_ERR_INVALID, "page_table, kv_lens, q_starts and lse must be 4-byte aligned");
+  if (page_table_stride < 0) return fail(B200_ERR_INVALID, "negative strides");
+  l.cache_dtype = cache->dtype;
+  l.q = q;
+  l.q_f16 = dtype == B200_DTYPE_F16;
+  l.q_token_stride = q_token_stride;
+  l.q_head_stride = q_head_stride;
+  l.q_tokens = q_tokens;
+  l.table = page_table;
+  l.table_stride = page_table_stride;
+  l.table_width = page_table_width;
+  l.kv_lens = kv_lens;
+  l.q_starts = q_starts;
+  l.seqs = seqs;
+  l.max_q = max_q_len;
+  l.q_heads = q_heads;
+  l.scale = scale;
+  l.causal = causal != 0;
+  // A window as wide as the table is none; the kernels' positions then stay above
+  // -2^31 (new tokens may outnumber the cached ones, and the first lie below zero).
+  l.window = window < (int64_t)page_table_width * cache->page_size ? window : 0;
+  l.out = out;
+  l.out_token_stride = out_token_stride;
+  l.out_head_stride = out_head_stride;
+  l.lse = lse;
+  return B200_OK;
+}
+
+// The workspace's status word, counters and scratch.
+int attention_workspace(AttnLaunch& l, void* workspace, int64_t workspace_bytes, int64_t need,
+                        const char* what) {
+  if (workspace == nullptr || !aligned(workspace, 256) || workspace_bytes < need)
+    return fail(B200_ERR_INVALID, "workspace smaller than %s (%lld) or not 256-byte aligned", what,
+                (long long)need);
+  uint8_t* base = static_cast<uint8_t*>(workspace);
+  l.status.call = reinterpret_cast<int*>(base);
+  l.counters = reinterpret_cast<int*>(base + ws_counter_offset());
+  l.scratch = base + ws_fixed_bytes();
+  return device_status_word(&l.status.device);
+}
+
 }  // namespace
 
 int b200::device_status_word(int** out) {
@@ -161,68 +241,16 @@ int b200_paged_attention(const b200_kv_cache* cache, const void* q, int32_t dtyp
                          int64_t out_head_stride, float* lse, void* workspace,
                          int64_t workspace_bytes, void* stream) {
   AttnLaunch l{};
-  int rc = cache_view(cache, l.c);
-  if (rc) return rc;
-  if (!valid_dtype16(dtype)) return fail(B200_ERR_UNSUPPORTED, "q must be bf16 or f16");
-  if (cache->dtype != B200_DTYPE_E4M3 && cache->dtype != dtype)
-    return fail(B200_ERR_INVALID, "a 16-bit cache takes queries of its own type");
-  if (q_heads <= 0 || q_heads % cache->kv_heads)
-    return fail(B200_ERR_INVALID, "%d query heads cannot share %d key/value heads", q_heads,
-                cache->kv_heads);
-  if (q_heads / cache->kv_heads > 128)
-    return fail(B200_ERR_UNSUPPORTED, "at most 128 query heads per key/value head, got %d",
-                q_heads / cache->kv_heads);
-  if (seqs < 0 || q_tokens < 0 || q_tokens + seqs > 0x7fffffffll || max_q_len < 0 || page_table_width < 0)
-    return fail(B200_ERR_INVALID, "negative or too large count");
-  if (window < 0 || (window > 0 && !causal))
-    return fail(B200_ERR_INVALID, "a window needs causal attention and at least one token");
-  // (in units of log2, as the kernels use it)
-  if (!std::isfinite(scale * 1.4426950408889634f))
-    return fail(B200_ERR_INVALID, "the scale must be finite");
-  if (seqs == 0 || q_tokens == 0 || max_q_len == 0) return B200_OK;
-  if ((rc = check_rows("q", q, q_token_stride, q_head_stride))) return rc;
-  if ((rc = check_rows("out", out, out_token_stride, out_head_stride))) return rc;
-  if (!apart(out_token_stride, q_tokens, out_head_stride, q_heads, l.c.head_dim))
-    return fail(B200_ERR_INVALID, "the output's vectors overlap");
-  if (kv_lens == nullptr || q_starts == nullptr || (page_table_width > 0 && page_table == nullptr))
-    return fail(B200_ERR_INVALID, "null pointer argument");
-  if (!aligned(page_table, 4) || !aligned(kv_lens, 4) || !aligned(q_starts, 4) || !aligned(lse, 4))
-    return fail(B200_ERR_INVALID, "page_table, kv_lens, q_starts and lse must be 4-byte aligned");
-  if (page_table_stride < 0) return fail(B200_ERR_INVALID, "negative strides");
-  const int64_t fixed = ws_fixed_bytes();
-  const int64_t need = fixed + attn_scratch_bytes(l.c.head_dim, q_tokens, seqs);
-  if (workspace == nullptr || !aligned(workspace, 256) || workspace_bytes < need)
-    return fail(B200_ERR_INVALID,
-                "workspace smaller than b200_paged_attention_workspace_bytes (%lld) or not 256-byte aligned",
-                (long long)need);
-  l.cache_dtype = cache->dtype;
-  l.q = q;
-  l.q_f16 = dtype == B200_DTYPE_F16;
-  l.q_token_stride = q_token_stride;
-  l.q_head_stride = q_head_stride;
-  l.q_tokens = q_tokens;
-  l.table = page_table;
-  l.table_stride = page_table_stride;
-  l.table_width = page_table_width;
-  l.kv_lens = kv_lens;
-  l.q_starts = q_starts;
-  l.seqs = seqs;
-  l.max_q = max_q_len;
-  l.q_heads = q_heads;
-  l.scale = scale;
-  l.causal = causal != 0;
-  // A window as wide as the table is none; the kernels' positions then stay above
-  // -2^31 (new tokens may outnumber the cached ones, and the first lie below zero).
-  l.window = window < (int64_t)page_table_width * cache->page_size ? window : 0;
-  l.out = out;
-  l.out_token_stride = out_token_stride;
-  l.out_head_stride = out_head_stride;
-  l.lse = lse;
-  uint8_t* base = static_cast<uint8_t*>(workspace);
-  l.status.call = reinterpret_cast<int*>(base);
-  if ((rc = device_status_word(&l.status.device))) return rc;
-  l.counters = reinterpret_cast<int*>(base + ws_counter_offset());
-  l.scratch = base + fixed;
+  bool none;
+  int rc = attention_args(cache, q, dtype, q_tokens, q_heads, q_token_stride, q_head_stride,
+                          page_table, page_table_stride, page_table_width, kv_lens, q_starts, seqs,
+                          max_q_len, scale, causal, window, out, out_token_stride, out_head_stride,
+                          lse, l, none);
+  if (rc || none) return rc;
+  const int64_t need = ws_fixed_bytes() + attn_scratch_bytes(l.c.head_dim, q_tokens, seqs);
+  if ((rc = attention_workspace(l, workspace, workspace_bytes, need,
+                                "b200_paged_attention_workspace_bytes")))
+    return rc;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   // Rows of a sequence and key/value head: the streaming kernel takes few.
   const int64_t rows = (int64_t)max_q_len * (q_heads / cache->kv_heads);
@@ -230,6 +258,61 @@ int b200_paged_attention(const b200_kv_cache* cache, const void* q, int32_t dtyp
   if (rows <= attn_decode_rows(l))
     return check_cuda(launch_attn_decode(l, st), "attention (decode) launch");
   return check_cuda(launch_attn_prefill(l, st), "attention (prefill) launch");
+}
+
+int64_t b200_shared_prefix_attention_workspace_bytes(int32_t head_dim, int64_t q_tokens,
+                                                     int32_t q_heads, int32_t seqs, int32_t groups) {
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256) return -1;
+  if (q_tokens < 0 || q_heads <= 0 || seqs < 0 || groups < 0) return -1;
+  return ws_fixed_bytes() + attn_prefix_scratch_bytes(head_dim, q_tokens, q_heads, seqs, groups);
+}
+
+int b200_shared_prefix_attention(
+    const b200_kv_cache* cache, const void* q, int32_t dtype, int64_t q_tokens, int32_t q_heads,
+    int64_t q_token_stride, int64_t q_head_stride, const int32_t* prefix_table,
+    int64_t prefix_table_stride, int32_t prefix_table_width, const int32_t* prefix_lens,
+    const int32_t* group_starts, int32_t groups, const int32_t* page_table,
+    int64_t page_table_stride, int32_t page_table_width, const int32_t* kv_lens,
+    const int32_t* q_starts, int32_t seqs, int32_t max_q_len, float scale, void* out,
+    int64_t out_token_stride, int64_t out_head_stride, float* lse, void* workspace,
+    int64_t workspace_bytes, void* stream) {
+  AttnLaunch own{};
+  bool none;
+  int rc = attention_args(cache, q, dtype, q_tokens, q_heads, q_token_stride, q_head_stride,
+                          page_table, page_table_stride, page_table_width, kv_lens, q_starts, seqs,
+                          max_q_len, scale, 1, 0, out, out_token_stride, out_head_stride, lse, own,
+                          none);
+  if (rc) return rc;
+  if (groups < 0 || prefix_table_width < 0 || q_tokens + groups > 0x7fffffffll)
+    return fail(B200_ERR_INVALID, "negative or too large count");
+  if (none || groups == 0) return B200_OK;
+  if (prefix_lens == nullptr || group_starts == nullptr ||
+      (prefix_table_width > 0 && prefix_table == nullptr))
+    return fail(B200_ERR_INVALID, "null pointer argument");
+  if (!aligned(prefix_table, 4) || !aligned(prefix_lens, 4) || !aligned(group_starts, 4))
+    return fail(B200_ERR_INVALID, "prefix_table, prefix_lens and group_starts must be 4-byte aligned");
+  if (prefix_table_stride < 0) return fail(B200_ERR_INVALID, "negative strides");
+  const int64_t need = b200_shared_prefix_attention_workspace_bytes(own.c.head_dim, q_tokens, q_heads,
+                                                                    seqs, groups);
+  if ((rc = attention_workspace(own, workspace, workspace_bytes, need,
+                                "b200_shared_prefix_attention_workspace_bytes")))
+    return rc;
+  // A group's rows over its prefix: all of its sequences' new tokens, none masked.
+  AttnLaunch prefix = own;
+  prefix.table = prefix_table;
+  prefix.table_stride = prefix_table_stride;
+  prefix.table_width = prefix_table_width;
+  prefix.kv_lens = prefix_lens;
+  prefix.group_starts = group_starts;
+  prefix.group_seqs = seqs;
+  prefix.seqs = groups;
+  prefix.max_q = (int)q_tokens;
+  prefix.causal = 0;
+  prefix.unit_rows = q_tokens / groups * (q_heads / cache->kv_heads);
+  if (prefix.unit_rows == 0) prefix.unit_rows = 1;
+  const std::lock_guard<std::mutex> together(launch_mutex());
+  return check_cuda(launch_attn_prefix(prefix, own, reinterpret_cast<cudaStream_t>(stream)),
+                    "shared-prefix attention launch");
 }
 
 }  // extern "C"

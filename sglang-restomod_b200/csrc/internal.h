@@ -349,7 +349,21 @@ struct AttnLaunch {
   StatusWords status;
   int* counters;       // the workspace's 1024 arrival counters, zero between calls
   uint8_t* scratch;
+  // Passes of a call whose sequences share prefixes (launch_attn_prefix):
+  float* out32;            // the outputs, fp32 [q_tokens][q_heads][head_dim], instead of `out`
+  const int* group_starts; // "sequence" g is sequences group_starts[g] ... g + 1 of q_starts
+  int group_seqs;          // how many sequences q_starts has then
+  long long unit_rows;     // rows of a typical sequence (0: max_q's)
+  float* mark;             // [q_tokens][q_heads]: kNoRow at every row of the pass, or nullptr
+
+  __device__ int q_start(int s) const {
+    if (group_starts == nullptr) return __ldg(q_starts + s);
+    const int g = __ldg(group_starts + s);
+    return __ldg(q_starts + (g < 0 ? 0 : g > group_seqs ? group_seqs : g));
+  }
 };
+// What no log-sum-exp is: a NaN of a bit pattern that arithmetic does not make.
+constexpr unsigned kNoRow = 0x7f800001u;
 // The decode kernel takes up to attn_decode_rows() rows (new tokens x query
 // heads per key/value head) of a sequence; the tensor-core kernel any number.
 int attn_decode_rows(const AttnLaunch& l);
@@ -357,6 +371,12 @@ long long attn_decode_scratch_bytes(int head_dim);
 cudaError_t launch_attn_decode(const AttnLaunch& l, cudaStream_t stream);
 long long attn_prefill_scratch_bytes(int head_dim, long long q_tokens, int seqs);
 cudaError_t launch_attn_prefill(const AttnLaunch& l, cudaStream_t stream);
+// Attention of each group of sequences over a prefix that they share (`prefix`: its
+// kv_lens and table by group, group_starts) and over their own tokens (`own`); both
+// with q, out and lse of the call. Scratch: prefix.scratch.
+long long attn_prefix_scratch_bytes(int head_dim, long long q_tokens, int q_heads, int seqs,
+                                    int groups);
+cudaError_t launch_attn_prefix(AttnLaunch prefix, AttnLaunch own, cudaStream_t stream);
 inline long long attn_scratch_bytes(int head_dim, long long q_tokens, int seqs) {
   const long long d = attn_decode_scratch_bytes(head_dim);
   const long long p = attn_prefill_scratch_bytes(head_dim, q_tokens, seqs);

@@ -974,6 +974,7 @@ def kv_cache_read(cache, slots: torch.Tensor, dtype: torch.dtype | None = None):
 # overlap, and its arrival counters and partial sums must not.
 _ATTN_WORKSPACES: dict[tuple[int, int], torch.Tensor] = {}
 _ATTN_BYTES: dict[tuple[int, int, int], int] = {}
+_PREFIX_BYTES: dict[tuple[int, int, int, int, int], int] = {}
 # Workspaces that a larger one has replaced, kept because a captured graph may still
 # use them. Each is at most half of the one after it, so a stream's together are
 # below its present one. (Nearly all of a workspace is its partial results, a
@@ -989,14 +990,22 @@ def paged_attention_workspace_bytes(head_dim: int, q_tokens: int, seqs: int) -> 
     return n
 
 
-def _attn_workspace(index: int, stream: int, head_dim: int, q_tokens: int, seqs: int):
+def _rounded(q_tokens: int, seqs: int) -> tuple[int, int]:
     # Sizes are asked for rounded up: few distinct ones, and no growth up to the
     # minimum, which costs a hundredth.
-    key = (head_dim, max(_ATTN_MIN_TOKENS, 1 << max(0, q_tokens - 1).bit_length()),
-           max(_ATTN_MIN_SEQS, 1 << max(0, seqs - 1).bit_length()))
+    return (max(_ATTN_MIN_TOKENS, 1 << max(0, q_tokens - 1).bit_length()),
+            max(_ATTN_MIN_SEQS, 1 << max(0, seqs - 1).bit_length()))
+
+
+def _attn_workspace(index: int, stream: int, head_dim: int, q_tokens: int, seqs: int):
+    key = (head_dim, *_rounded(q_tokens, seqs))
     nbytes = _ATTN_BYTES.get(key)
     if nbytes is None:
         nbytes = _ATTN_BYTES[key] = paged_attention_workspace_bytes(*key)
+    return _attn_workspace_of(index, stream, nbytes)
+
+
+def _attn_workspace_of(index: int, stream: int, nbytes: int):
     ws = _ATTN_WORKSPACES.get((index, stream))
     if ws is not None and ws.numel() >= nbytes:
         return ws
@@ -1045,6 +1054,40 @@ def attention_status(device: torch.device | None = None, reset: bool = True) -> 
     return int(bits.value)
 
 
+def _attention_args(q, cache, page_table, kv_lens, q_starts, out):
+    """(dtype code, tokens, heads, head_dim, sequences, out) of an attention call."""
+    dtype = q.dtype
+    code = _DTYPE_CODE.get(dtype)
+    if code is None:
+        raise TypeError(f"q must be bf16 or f16, got {dtype}")
+    if q.dim() != 3 or q.shape[2] != cache.head_dim or q.stride(2) != 1:
+        raise ValueError(f"q must be [tokens, heads, {cache.head_dim}] with contiguous vectors, "
+                         f"got {tuple(q.shape)} strides {q.stride()}")
+    tokens, heads, dim = q.shape
+    seqs = kv_lens.shape[0]
+    _tables((page_table, "page_table"), (kv_lens, "kv_lens"), (q_starts, "q_starts"))
+    if q_starts.shape[0] != seqs + 1 or page_table.dim() != 2 or page_table.shape[0] != seqs:
+        raise ValueError(f"{seqs} sequences need q_starts [{seqs + 1}] and page_table [{seqs}, "
+                         f"pages], got {tuple(q_starts.shape)}, {tuple(page_table.shape)}")
+    if out is None:
+        out = torch.empty(tokens, heads, dim, dtype=dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != dtype or out.stride(2) != 1:
+        raise ValueError(f"out must be {tuple(q.shape)} {dtype}, got {tuple(out.shape)} {out.dtype}")
+    return code, tokens, heads, dim, seqs, out
+
+
+def _tables(*named) -> None:
+    for t, what in named:
+        if t.dtype != torch.int32 or t.stride(-1) != 1:
+            raise ValueError(f"{what} must be int32 with contiguous rows, got {t.dtype}")
+
+
+def _own_workspace(ws: torch.Tensor) -> torch.Tensor:
+    if ws.dtype != torch.uint8 or not ws.is_contiguous():
+        raise TypeError(f"the workspace must be contiguous uint8, got {ws.dtype}")
+    return ws
+
+
 def paged_attention(q: torch.Tensor, cache, page_table: torch.Tensor, kv_lens: torch.Tensor,
                     q_starts: torch.Tensor, max_q_len: int, *, scale: float | None = None,
                     causal: bool = True, window: int = 0, out: torch.Tensor | None = None,
@@ -1064,33 +1107,12 @@ def paged_attention(q: torch.Tensor, cache, page_table: torch.Tensor, kv_lens: t
     run on the tensor cores' kernel."""
     index = _on_device("paged_attention", q, cache.k, page_table, kv_lens, q_starts, out,
                        workspace)
-    dtype = q.dtype
-    code = _DTYPE_CODE.get(dtype)
-    if code is None:
-        raise TypeError(f"q must be bf16 or f16, got {dtype}")
-    if q.dim() != 3 or q.shape[2] != cache.head_dim or q.stride(2) != 1:
-        raise ValueError(f"q must be [tokens, heads, {cache.head_dim}] with contiguous vectors, "
-                         f"got {tuple(q.shape)} strides {q.stride()}")
-    tokens, heads, dim = q.shape
-    seqs = kv_lens.shape[0]
-    for t, what in ((page_table, "page_table"), (kv_lens, "kv_lens"), (q_starts, "q_starts")):
-        if t.dtype != torch.int32 or t.stride(-1) != 1:
-            raise ValueError(f"{what} must be int32 with contiguous rows, got {t.dtype}")
-    if q_starts.shape[0] != seqs + 1 or page_table.dim() != 2 or page_table.shape[0] != seqs:
-        raise ValueError(f"{seqs} sequences need q_starts [{seqs + 1}] and page_table [{seqs}, "
-                         f"pages], got {tuple(q_starts.shape)}, {tuple(page_table.shape)}")
-    if out is None:
-        out = torch.empty(tokens, heads, dim, dtype=dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != dtype or out.stride(2) != 1:
-        raise ValueError(f"out must be {tuple(q.shape)} {dtype}, got {tuple(out.shape)} {out.dtype}")
+    code, tokens, heads, dim, seqs, out = _attention_args(q, cache, page_table, kv_lens, q_starts,
+                                                          out)
     lse = torch.empty(tokens, heads, dtype=torch.float32, device=q.device) if return_lse else None
     stream = _raw_stream(index)
-    ws = workspace
-    if ws is not None:
-        if ws.dtype != torch.uint8 or not ws.is_contiguous():
-            raise TypeError(f"the workspace must be contiguous uint8, got {ws.dtype}")
-    else:
-        ws = _attn_workspace(index, stream, dim, tokens, seqs)
+    ws = _own_workspace(workspace) if workspace is not None \
+        else _attn_workspace(index, stream, dim, tokens, seqs)
     _lib.check(
         lib().b200_paged_attention(
             cache.desc, q.data_ptr(), code, tokens, heads, q.stride(0), q.stride(1),
@@ -1098,5 +1120,77 @@ def paged_attention(q: torch.Tensor, cache, page_table: torch.Tensor, kv_lens: t
             q_starts.data_ptr(), seqs, max_q_len, dim ** -0.5 if scale is None else scale,
             causal, window, out.data_ptr(), out.stride(0), out.stride(1),
             None if lse is None else lse.data_ptr(), ws.data_ptr(), ws.numel(), stream)
+    )
+    return (out, lse) if return_lse else out
+
+
+def shared_prefix_attention_workspace_bytes(head_dim: int, q_tokens: int, q_heads: int, seqs: int,
+                                            groups: int) -> int:
+    n = int(lib().b200_shared_prefix_attention_workspace_bytes(head_dim, q_tokens, q_heads, seqs,
+                                                               groups))
+    if n < 0:
+        raise ValueError(f"no attention kernel for head_dim {head_dim}, {q_heads} heads")
+    return n
+
+
+def _prefix_workspace(index: int, stream: int, head_dim: int, q_tokens: int, q_heads: int,
+                      seqs: int, groups: int):
+    # (the rows in fp32 are most of it: they are not rounded up far)
+    key = (head_dim, -(-q_tokens // 256) * 256, q_heads, _rounded(0, seqs)[1],
+           _rounded(0, groups)[1])
+    nbytes = _PREFIX_BYTES.get(key)
+    if nbytes is None:
+        nbytes = _PREFIX_BYTES[key] = shared_prefix_attention_workspace_bytes(*key)
+    return _attn_workspace_of(index, stream, nbytes)
+
+
+def reserve_shared_prefix_workspace(head_dim: int, q_tokens: int, q_heads: int, seqs: int,
+                                    groups: int, device: torch.device | None = None) -> torch.Tensor:
+    """:func:`reserve_attention_workspace` for :func:`shared_prefix_attention` calls of
+    up to these sizes; the same workspace serves both."""
+    index = torch.cuda.current_device() if device is None or device.index is None else device.index
+    return _prefix_workspace(index, _raw_stream(index), head_dim, q_tokens, q_heads, seqs, groups)
+
+
+def shared_prefix_attention(q: torch.Tensor, cache, prefix_table: torch.Tensor,
+                            prefix_lens: torch.Tensor, group_starts: torch.Tensor,
+                            page_table: torch.Tensor, kv_lens: torch.Tensor,
+                            q_starts: torch.Tensor, max_q_len: int, *, scale: float | None = None,
+                            out: torch.Tensor | None = None, return_lse: bool = False,
+                            workspace: torch.Tensor | None = None):
+    """:func:`paged_attention` of a batch whose sequences share long prefixes, each
+    prefix read once for all of its sequences.
+
+    Group g is the sequences ``group_starts[g] : group_starts[g + 1]`` (int32 ``[groups
+    + 1]``, from 0 to the number of sequences); its prefix is the first
+    ``prefix_lens[g]`` tokens (0: none) of the pages ``prefix_table[g]`` (int32
+    ``[groups, pages]``). ``page_table``, ``kv_lens``, ``q_starts`` and ``max_q_len``
+    describe each sequence's own tokens, which come after the prefix and begin on a
+    page of their own; its new tokens are the last of them. Every new token sees its
+    group's whole prefix and its own tokens causally; the log-sum-exp is over both."""
+    index = _on_device("shared_prefix_attention", q, cache.k, prefix_table, prefix_lens,
+                       group_starts, page_table, kv_lens, q_starts, out, workspace)
+    code, tokens, heads, dim, seqs, out = _attention_args(q, cache, page_table, kv_lens, q_starts,
+                                                          out)
+    _tables((prefix_table, "prefix_table"), (prefix_lens, "prefix_lens"),
+            (group_starts, "group_starts"))
+    groups = prefix_lens.shape[0]
+    if group_starts.shape != (groups + 1,) or prefix_table.dim() != 2 \
+            or prefix_table.shape[0] != groups:
+        raise ValueError(f"{groups} groups need group_starts [{groups + 1}] and prefix_table "
+                         f"[{groups}, pages], got {tuple(group_starts.shape)}, "
+                         f"{tuple(prefix_table.shape)}")
+    lse = torch.empty(tokens, heads, dtype=torch.float32, device=q.device) if return_lse else None
+    stream = _raw_stream(index)
+    ws = _own_workspace(workspace) if workspace is not None \
+        else _prefix_workspace(index, stream, dim, tokens, heads, seqs, groups)
+    _lib.check(
+        lib().b200_shared_prefix_attention(
+            cache.desc, q.data_ptr(), code, tokens, heads, q.stride(0), q.stride(1),
+            prefix_table.data_ptr(), prefix_table.stride(0), prefix_table.shape[1],
+            prefix_lens.data_ptr(), group_starts.data_ptr(), groups, page_table.data_ptr(),
+            page_table.stride(0), page_table.shape[1], kv_lens.data_ptr(), q_starts.data_ptr(), seqs,
+            max_q_len, dim ** -0.5 if scale is None else scale, out.data_ptr(), out.stride(0),
+            out.stride(1), None if lse is None else lse.data_ptr(), ws.data_ptr(), ws.numel(), stream)
     )
     return (out, lse) if return_lse else out
