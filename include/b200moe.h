@@ -601,6 +601,33 @@ int b200_shared_prefix_attention(
     int64_t out_token_stride, int64_t out_head_stride, float* lse, void* workspace,
     int64_t workspace_bytes, void* stream);
 
+/*
+ * Eviction of cached tokens by their scores (b200_kv_cache_scores): per sequence and
+ * key/value head, of kv_lens[s] > budget cached tokens stay the first `first`, the
+ * last `recent`, and of those between the budget - first - recent with the largest
+ * scores (ties: the lowest index; NaN counts as the lowest score, -0 as 0). Heads
+ * choose by themselves. The kept tokens stay in order and become tokens 0 .. budget
+ * - 1 of the sequence; keys, values, scales and scores move, bit for bit. Scores:
+ * fp32 of (page, offset, head) at the score strides.
+ * kept [seqs][kv_heads][budget]: their indices before, -1 past the sequence's
+ * end; lens [seqs] = min(kv_lens, budget).
+ * out_table NULL (or page_table): in place, in the sequence's first pages; the
+ * slots after token lens[s] - 1 keep what they hold. No two sequences of the call
+ * may have a page in common then. Otherwise the kept tokens, of sequences within the budget
+ * too, are copied to the pages out_table[s * out_table_stride ..]
+ * (out_table_width entries, enough for the budget), which hold no token of the
+ * call's sequences; the source stays as it is. Page numbers outside the
+ * cache set status bit 16 (b200_device_status): such a token has the lowest score and is not
+ * moved, nor is one whose new page is outside. Capturable; no workspace.
+ */
+int b200_kv_cache_evict(const b200_kv_cache* cache, float* scores, int64_t score_page_stride,
+                        int64_t score_token_stride, int64_t score_head_stride,
+                        const int32_t* page_table, int64_t page_table_stride,
+                        int32_t page_table_width, const int32_t* kv_lens, int32_t seqs,
+                        int32_t budget, int32_t recent, int32_t first, const int32_t* out_table,
+                        int64_t out_table_stride, int32_t out_table_width, int32_t* kept,
+                        int32_t* lens, void* stream);
+
 /* ---------------------------------------- expert parallelism (peer memory) */
 
 /*

@@ -1,4 +1,5 @@
-// C ABI of the 8-bit integer linear. Host-side validation and launches; declared in
+// C ABI of the 8-bit integer linear and of the eviction of cached tokens by their
+// accumulated weights. Host-side validation and launches; declared in
 // include/b200moe.h.
 #include "capi_checks.h"
 
@@ -13,6 +14,16 @@ int check_int8(int64_t m, int64_t k, int64_t n) {
                 (long long)k);
   if (m < 0 || m >= (1ll << 31)) return fail(B200_ERR_INVALID, "bad M %lld", (long long)m);
   if (n <= 0 || n >= (1ll << 31)) return fail(B200_ERR_INVALID, "bad N %lld", (long long)n);
+  return B200_OK;
+}
+
+// The scores of a cache's tokens: an array beside it, and its strides.
+int check_scores(const float* scores, int64_t page_stride, int64_t token_stride,
+                 int64_t head_stride) {
+  if (scores == nullptr) return fail(B200_ERR_INVALID, "null pointer argument");
+  if (!aligned(scores, 4)) return fail(B200_ERR_INVALID, "scores must be 4-byte aligned");
+  if (page_stride < 0 || token_stride < 0 || head_stride < 0)
+    return fail(B200_ERR_INVALID, "negative strides");
   return B200_OK;
 }
 
@@ -95,6 +106,65 @@ int b200_int8_linear(const void* x, int32_t x_dtype, int64_t m, int64_t k, const
   rc = check_cuda(launch_int8_quant(x, x_dtype == B200_DTYPE_F16, m, (int)k, q, scales, st),
                   "int8 quantization launch");
   return rc ? rc : check_cuda(launch_int8_gemm(l, st), "int8 GEMM launch");
+}
+
+int b200_kv_cache_evict(const b200_kv_cache* cache, float* scores, int64_t score_page_stride,
+                        int64_t score_token_stride, int64_t score_head_stride,
+                        const int32_t* page_table, int64_t page_table_stride,
+                        int32_t page_table_width, const int32_t* kv_lens, int32_t seqs,
+                        int32_t budget, int32_t recent, int32_t first, const int32_t* out_table,
+                        int64_t out_table_stride, int32_t out_table_width, int32_t* kept,
+                        int32_t* lens, void* stream) {
+  EvictLaunch l{};
+  int rc = cache_view(cache, l.c);
+  if (rc) return rc;
+  if (seqs < 0 || page_table_width < 0 || out_table_width < 0)
+    return fail(B200_ERR_INVALID, "negative count");
+  if (budget <= 0 || recent < 0 || first < 0 || recent > budget - first)
+    return fail(B200_ERR_INVALID, "the budget %d must be positive and hold the first %d and last %d tokens",
+                budget, first, recent);
+  if ((int64_t)seqs * cache->kv_heads * 8 > 0x7fffffffll)
+    return fail(B200_ERR_UNSUPPORTED, "more than 2^28 rows in one call");
+  // (the grid's second dimension counts the kept tokens)
+  if (budget > 65535 * 64)
+    return fail(B200_ERR_UNSUPPORTED, "the budget is at most %d tokens, got %d", 65535 * 64, budget);
+  if (seqs == 0) return B200_OK;
+  if ((rc = check_scores(scores, score_page_stride, score_token_stride, score_head_stride))) return rc;
+  if (kv_lens == nullptr || kept == nullptr || lens == nullptr ||
+      (page_table_width > 0 && page_table == nullptr))
+    return fail(B200_ERR_INVALID, "null pointer argument");
+  if (!aligned(page_table, 4) || !aligned(kv_lens, 4) || !aligned(out_table, 4) ||
+      !aligned(kept, 4) || !aligned(lens, 4))
+    return fail(B200_ERR_INVALID, "the tables, kv_lens, kept and lens must be 4-byte aligned");
+  if (page_table_stride < 0 || out_table_stride < 0)
+    return fail(B200_ERR_INVALID, "negative strides");
+  const int64_t most = (int64_t)page_table_width * cache->page_size;
+  if (most > 0x7fffffffll) return fail(B200_ERR_UNSUPPORTED, "a table of more than 2^31 - 1 tokens");
+  if (out_table == page_table && out_table_stride == page_table_stride) out_table = nullptr;
+  if (out_table != nullptr &&
+      (int64_t)out_table_width * cache->page_size < (budget < most ? budget : most))
+    return fail(B200_ERR_INVALID, "out_table's %d pages of %d do not hold the budget of %d tokens",
+                out_table_width, cache->page_size, budget);
+  l.scores = scores;
+  l.score_page_stride = score_page_stride;
+  l.score_token_stride = score_token_stride;
+  l.score_head_stride = score_head_stride;
+  l.table = page_table;
+  l.table_stride = page_table_stride;
+  l.table_width = page_table_width;
+  l.kv_lens = kv_lens;
+  l.seqs = seqs;
+  l.budget = budget;
+  l.recent = recent;
+  l.first = first;
+  l.out_table = out_table;
+  l.out_stride = out_table_stride;
+  l.kept = kept;
+  l.lens = lens;
+  if ((rc = device_status_word(&l.status))) return rc;
+  // the move reads what the choice leaves in kept
+  const std::lock_guard<std::mutex> together(launch_mutex());
+  return check_cuda(launch_kv_evict(l, reinterpret_cast<cudaStream_t>(stream)), "eviction launch");
 }
 
 }  // extern "C"

@@ -319,6 +319,25 @@ cudaError_t launch_kv_read(const KvCacheView& c, void* k, void* v, bool f16,
                            long long token_stride, long long head_stride, const long long* slots,
                            long long tokens, cudaStream_t stream);
 
+// Eviction of cached tokens by score (kv_evict.cu). Scores: one fp32 per (page,
+// offset, head) at the score strides.
+struct EvictLaunch {
+  KvCacheView c;
+  float* scores;
+  long long score_page_stride, score_token_stride, score_head_stride;
+  const int* table;      // [seqs][table_stride], table_width entries each
+  long long table_stride;
+  int table_width;
+  const int* kv_lens;
+  int seqs, budget, recent, first;
+  const int* out_table;  // nullptr: in place
+  long long out_stride;
+  int* kept;             // [seqs][heads][budget]
+  int* lens;             // [seqs]
+  int* status;
+};
+cudaError_t launch_kv_evict(const EvictLaunch& l, cudaStream_t stream);
+
 // Where a kernel records its error bits: in the call's workspace, and in a word
 // that the library keeps per device, which outlives workspaces and serves calls
 // that have none and calls replayed from a graph.

@@ -206,6 +206,12 @@ SIGNATURES = {
          c_int32, c_int32, c_float, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64,
          c_void_p],
     ),
+    "b200_kv_cache_evict": (
+        c_int32,
+        [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int32, c_void_p,
+         c_int32, c_int32, c_int32, c_int32, c_void_p, c_int64, c_int32, c_void_p, c_void_p,
+         c_void_p],
+    ),
     "b200_ep_region_bytes": (c_int64, [c_int32, c_int64, c_int32, c_int64]),
     "b200_ep_region_layout": (c_int32, [c_int32, c_int64, c_int32, c_int64, ctypes.POINTER(c_int64)]),
     "b200_ipc_get_handle": (c_int32, [c_void_p, c_void_p, ctypes.POINTER(c_int64)]),

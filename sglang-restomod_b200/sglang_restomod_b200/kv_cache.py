@@ -76,3 +76,11 @@ class PagedKVCache:
         scales = [torch.zeros(num_pages, kv_heads, page_size, dtype=torch.uint8, device=device)
                   .transpose(1, 2) if dtype == torch.float8_e4m3fn else None for _ in range(2)]
         return cls(*kv, *scales)
+
+    def empty_scores(self) -> torch.Tensor:
+        """Scores for :func:`ops.kv_cache_scores` and :func:`ops.kv_cache_evict`: one fp32
+        per token and head, ``[pages, page_size, kv_heads]``, head-major as
+        :meth:`empty`'s pages are. (New tokens' entries are written, not added to: no
+        need to clear them.)"""
+        return torch.empty(self.num_pages, self.kv_heads, self.page_size, dtype=torch.float32,
+                           device=self.k.device).transpose(1, 2)

@@ -1194,3 +1194,51 @@ def shared_prefix_attention(q: torch.Tensor, cache, prefix_table: torch.Tensor,
             out.stride(1), None if lse is None else lse.data_ptr(), ws.data_ptr(), ws.numel(), stream)
     )
     return (out, lse) if return_lse else out
+
+
+# ------------------------------------------------ weights of cached tokens
+def _scores_of(scores: torch.Tensor, cache, what: str = "scores") -> None:
+    if scores.dtype != torch.float32:
+        raise TypeError(f"{what} must be float32, got {scores.dtype}")
+    if scores.shape != cache.k.shape[:3]:
+        raise ValueError(f"{what} must be {tuple(cache.k.shape[:3])} (pages, page size, heads), got "
+                         f"{tuple(scores.shape)}")
+
+
+def kv_cache_evict(cache, scores: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor,
+                   budget: int, *, recent: int = 0, first: int = 0,
+                   out_table: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Keeps ``budget`` tokens of each sequence and key/value head: the first ``first``,
+    the last ``recent``, and of those between the ones with the largest ``scores``
+    (fp32 ``[pages, page_size, kv_heads]``, see :func:`kv_cache_scores`; ties: the
+    lowest index). Heads choose by themselves; the kept tokens stay in order.
+
+    Without ``out_table`` they move to the front of the sequence's own pages, keys,
+    values, scales and scores, in place; no two sequences may have a page in common.
+    With it (int32 ``[seqs, pages]``, pages that hold none of the sequences' tokens)
+    they are copied there, and the source stays.
+
+    Returns (kept int32 ``[seqs, kv_heads, budget]``: the tokens' indices before, -1
+    past the end; lens int32 ``[seqs]``: ``min(kv_lens, budget)``)."""
+    index = _on_device("kv_cache_evict", cache.k, scores, page_table, kv_lens, out_table)
+    _scores_of(scores, cache)
+    _tables((page_table, "page_table"), (kv_lens, "kv_lens"))
+    seqs = kv_lens.shape[0]
+    if kv_lens.dim() != 1 or page_table.dim() != 2 or page_table.shape[0] != seqs:
+        raise ValueError(f"kv_lens must be [seqs] and page_table [seqs, pages], got "
+                         f"{tuple(kv_lens.shape)}, {tuple(page_table.shape)}")
+    to = (None, 0, 0)
+    if out_table is not None:
+        _tables((out_table, "out_table"))
+        if out_table.dim() != 2 or out_table.shape[0] != seqs:
+            raise ValueError(f"out_table must be [{seqs}, pages], got {tuple(out_table.shape)}")
+        to = (out_table.data_ptr(), out_table.stride(0), out_table.shape[1])
+    if not 0 < budget < 1 << 31:
+        raise ValueError(f"the budget must be a positive int32, got {budget}")
+    kept = torch.empty(seqs, cache.kv_heads, budget, dtype=torch.int32, device=scores.device)
+    lens = torch.empty(seqs, dtype=torch.int32, device=scores.device)
+    _lib.check(lib().b200_kv_cache_evict(
+        cache.desc, scores.data_ptr(), *scores.stride(), page_table.data_ptr(),
+        page_table.stride(0), page_table.shape[1], kv_lens.data_ptr(), seqs, budget, recent, first,
+        *to, kept.data_ptr(), lens.data_ptr(), _raw_stream(index)))
+    return kept, lens
