@@ -602,6 +602,37 @@ int b200_shared_prefix_attention(
     int64_t workspace_bytes, void* stream);
 
 /*
+ * The attention weight that cached tokens have gathered: for each of a sequence's
+ * kv_lens[s] tokens t and each key/value head,
+ *   scores_out = (t is one of the new tokens ? 0 : scores)
+ *                + sum over the new tokens and the query heads that share the head,
+ *                  of those that see t, of e^(scale * q . k_t - lse)
+ * (not causal: the queries' tokens are not among the cached ones, none starts from 0)
+ * with lse [q_tokens, q_heads] from the attention call (a row of -inf adds nothing),
+ * and everything else as in b200_paged_attention, whose masks these are; of new
+ * tokens past max_q_len none adds to the sums. lse may also be that of
+ * b200_shared_prefix_attention. Scores are fp32 of (page, offset, head), at strides of
+ * their own; scores_out may be scores. Each score has one writer, in a fixed order: two
+ * calls give the same bits. No two sequences of a call may have a page in common. At
+ * most 64 query heads per key/value head; q's vectors apart in memory. Products are
+ * exact to fp32's sums (e4m3 keys: queries to 2^-22 of their largest element);
+ * a key scale byte may be any. Infinite or NaN queries or keys give NaN scores where
+ * they are seen. Page numbers outside the cache set status bit 16. Workspace as
+ * for b200_paged_attention, and it may be the same one.
+ */
+int64_t b200_kv_cache_scores_workspace_bytes(int32_t head_dim, int64_t q_tokens, int32_t q_heads);
+int b200_kv_cache_scores(const b200_kv_cache* cache, const void* q, int32_t dtype, int64_t q_tokens,
+                         int32_t q_heads, int64_t q_token_stride, int64_t q_head_stride,
+                         const int32_t* page_table, int64_t page_table_stride,
+                         int32_t page_table_width, const int32_t* kv_lens, const int32_t* q_starts,
+                         int32_t seqs, int32_t max_q_len, float scale, int32_t causal,
+                         int32_t window, const float* lse, const float* scores,
+                         int64_t score_page_stride, int64_t score_token_stride,
+                         int64_t score_head_stride, float* scores_out, int64_t out_page_stride,
+                         int64_t out_token_stride, int64_t out_head_stride, void* workspace,
+                         int64_t workspace_bytes, void* stream);
+
+/*
  * Eviction of cached tokens by their scores (b200_kv_cache_scores): per sequence and
  * key/value head, of kv_lens[s] > budget cached tokens stay the first `first`, the
  * last `recent`, and of those between the budget - first - recent with the largest

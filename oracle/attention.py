@@ -105,3 +105,37 @@ def shared_prefix_attention_ref(q, k_cache, v_cache, prefix_table, prefix_lens, 
                 p = torch.exp(x - torch.where(lse[a:b, h] > -math.inf, lse[a:b, h], 0.0)[:, None])
                 out[a:b, h] = p @ torch.where(seen.any(0)[:, None], v[:, h // groups], 0.0)
     return out, lse
+
+
+def kv_cache_scores_ref(q, k_cache, table, kv_lens, q_starts, lse, scores, scale, causal=True,
+                        window=0, max_q=1 << 30):
+    """float64 scores [pages, page_size, heads] after adding each cached token's weights;
+    ``scores`` (same shape) is what they were. Also each token's added sum alone."""
+    groups, page = q.shape[1] // k_cache.shape[2], k_cache.shape[1]
+    out, added = scores.double().clone(), torch.zeros(scores.shape, dtype=torch.float64)
+    for s, kv in enumerate(kv_lens.tolist()):
+        a, b = int(q_starts[s]), int(q_starts[s + 1])
+        if kv == 0:
+            continue
+        at = torch.arange(kv)
+        pages = table[s].long()[at // page]
+        k = k_cache[pages, at % page].double()
+        pos = (kv - (b - a) + torch.arange(b - a)[:, None])[:max_q]
+        n = len(pos)
+        seen = torch.ones(n, kv, dtype=torch.bool)
+        if causal:
+            seen = at[None, :] <= pos
+            if window:
+                seen &= at[None, :] > pos - window
+        old = scores[pages, at % page].double()
+        if causal:
+            old[max(0, kv - (b - a)):] = 0.0
+        total = torch.zeros(kv, k_cache.shape[2], dtype=torch.float64)
+        for h in range(q.shape[1]):
+            z = lse[a:a + n, h].double()[:, None]
+            x = (q[a:a + n, h].double() @ k[:, h // groups].T * scale).masked_fill(~seen, -math.inf)
+            p = torch.where((z == -math.inf) | ~seen, 0.0, torch.exp(x - z))
+            total[:, h // groups] += p.sum(0)
+        out[pages, at % page] = old + total
+        added[pages, at % page] = total
+    return out, added

@@ -315,4 +315,63 @@ int b200_shared_prefix_attention(
                     "shared-prefix attention launch");
 }
 
+int64_t b200_kv_cache_scores_workspace_bytes(int32_t head_dim, int64_t q_tokens, int32_t q_heads) {
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256) return -1;
+  if (q_tokens < 0 || q_heads <= 0) return -1;
+  return ws_fixed_bytes() + kv_scores_scratch_bytes(head_dim, q_tokens, q_heads);
+}
+
+int b200_kv_cache_scores(const b200_kv_cache* cache, const void* q, int32_t dtype, int64_t q_tokens,
+                         int32_t q_heads, int64_t q_token_stride, int64_t q_head_stride,
+                         const int32_t* page_table, int64_t page_table_stride,
+                         int32_t page_table_width, const int32_t* kv_lens, const int32_t* q_starts,
+                         int32_t seqs, int32_t max_q_len, float scale, int32_t causal,
+                         int32_t window, const float* lse, const float* scores,
+                         int64_t score_page_stride, int64_t score_token_stride,
+                         int64_t score_head_stride, float* scores_out, int64_t out_page_stride,
+                         int64_t out_token_stride, int64_t out_head_stride, void* workspace,
+                         int64_t workspace_bytes, void* stream) {
+  ScoresLaunch s{};
+  bool none;
+  // (q stands where attention has its output: as aligned, and apart if it is used)
+  int rc = attention_args(cache, q, dtype, q_tokens, q_heads, q_token_stride, q_head_stride,
+                          page_table, page_table_stride, page_table_width, kv_lens, q_starts, seqs,
+                          max_q_len, scale, causal, window, const_cast<void*>(q), q_token_stride,
+                          q_head_stride, const_cast<float*>(lse), s.a, none);
+  if (rc) return rc;
+  if (q_heads / cache->kv_heads > 64)
+    return fail(B200_ERR_UNSUPPORTED, "at most 64 query heads per key/value head, got %d",
+                q_heads / cache->kv_heads);
+  // (no new tokens change nothing in place; elsewhere they would be a plain copy)
+  if (seqs == 0 || (none && scores == scores_out)) return B200_OK;
+  if (none)
+    return fail(B200_ERR_INVALID, "scores to another place need new tokens: got %lld, at most %d a sequence",
+                (long long)q_tokens, max_q_len);
+  if (lse == nullptr || scores == nullptr || scores_out == nullptr)
+    return fail(B200_ERR_INVALID, "null pointer argument");
+  if (!aligned(scores, 4) || !aligned(scores_out, 4))
+    return fail(B200_ERR_INVALID, "scores must be 4-byte aligned");
+  if (score_page_stride < 0 || score_token_stride < 0 || score_head_stride < 0 ||
+      out_page_stride < 0 || out_token_stride < 0 || out_head_stride < 0)
+    return fail(B200_ERR_INVALID, "negative strides");
+  if (scores == scores_out && (score_page_stride != out_page_stride ||
+                               score_token_stride != out_token_stride ||
+                               score_head_stride != out_head_stride))
+    return fail(B200_ERR_INVALID, "scores in place need the same strides");
+  const int64_t need = b200_kv_cache_scores_workspace_bytes(s.a.c.head_dim, q_tokens, q_heads);
+  if ((rc = attention_workspace(s.a, workspace, workspace_bytes, need,
+                                "b200_kv_cache_scores_workspace_bytes")))
+    return rc;
+  s.scores_in = scores;
+  s.scores_out = scores_out;
+  s.in_page = score_page_stride;
+  s.in_token = score_token_stride;
+  s.in_head = score_head_stride;
+  s.out_page = out_page_stride;
+  s.out_token = out_token_stride;
+  s.out_head = out_head_stride;
+  const std::lock_guard<std::mutex> together(launch_mutex());
+  return check_cuda(launch_kv_scores(s, reinterpret_cast<cudaStream_t>(stream)), "scores launch");
+}
+
 }  // extern "C"

@@ -402,6 +402,17 @@ inline long long attn_scratch_bytes(int head_dim, long long q_tokens, int seqs) 
   return d > p ? d : p;
 }
 
+// Accumulated attention weight of cached tokens (kv_scores.cu): `a` as for attention,
+// without an output; a.lse is read. Strides of both score arrays in elements.
+struct ScoresLaunch {
+  AttnLaunch a;
+  const float* scores_in;
+  float* scores_out;
+  long long in_page, in_token, in_head, out_page, out_token, out_head;
+};
+long long kv_scores_scratch_bytes(int head_dim, long long q_tokens, int q_heads);
+cudaError_t launch_kv_scores(const ScoresLaunch& l, cudaStream_t stream);
+
 // Held, one per device, while a call that uses a workspace puts its launches on a
 // stream: kernels of one call hand on through the workspace (a plan, converted
 // operands, partial sums), and when two threads call on one stream no other

@@ -206,6 +206,14 @@ SIGNATURES = {
          c_int32, c_int32, c_float, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64,
          c_void_p],
     ),
+    "b200_kv_cache_scores_workspace_bytes": (c_int64, [c_int32, c_int64, c_int32]),
+    "b200_kv_cache_scores": (
+        c_int32,
+        [c_void_p, c_void_p, c_int32, c_int64, c_int32, c_int64, c_int64, c_void_p, c_int64,
+         c_int32, c_void_p, c_void_p, c_int32, c_int32, c_float, c_int32, c_int32, c_void_p,
+         c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int64, c_void_p,
+         c_int64, c_void_p],
+    ),
     "b200_kv_cache_evict": (
         c_int32,
         [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int32, c_void_p,

@@ -975,6 +975,7 @@ def kv_cache_read(cache, slots: torch.Tensor, dtype: torch.dtype | None = None):
 _ATTN_WORKSPACES: dict[tuple[int, int], torch.Tensor] = {}
 _ATTN_BYTES: dict[tuple[int, int, int], int] = {}
 _PREFIX_BYTES: dict[tuple[int, int, int, int, int], int] = {}
+_SCORES_BYTES: dict[tuple[int, int, int], int] = {}
 # Workspaces that a larger one has replaced, kept because a captured graph may still
 # use them. Each is at most half of the one after it, so a stream's together are
 # below its present one. (Nearly all of a workspace is its partial results, a
@@ -1203,6 +1204,59 @@ def _scores_of(scores: torch.Tensor, cache, what: str = "scores") -> None:
     if scores.shape != cache.k.shape[:3]:
         raise ValueError(f"{what} must be {tuple(cache.k.shape[:3])} (pages, page size, heads), got "
                          f"{tuple(scores.shape)}")
+
+
+def kv_cache_scores_workspace_bytes(head_dim: int, q_tokens: int, q_heads: int) -> int:
+    n = int(lib().b200_kv_cache_scores_workspace_bytes(head_dim, q_tokens, q_heads))
+    if n < 0:
+        raise ValueError(f"no attention kernel for head_dim {head_dim}, {q_heads} heads")
+    return n
+
+
+def kv_cache_scores(q: torch.Tensor, cache, page_table: torch.Tensor, kv_lens: torch.Tensor,
+                    q_starts: torch.Tensor, max_q_len: int, lse: torch.Tensor,
+                    scores: torch.Tensor, *, scale: float | None = None, causal: bool = True,
+                    window: int = 0, out: torch.Tensor | None = None,
+                    workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Adds to each cached token's score the attention weight it has from the sequences'
+    new tokens, summed over them and the query heads of each key/value head; the new
+    tokens' own scores start from zero (``causal=False``: the queries' tokens are not
+    among the cached ones, and all scores are added to).
+
+    Call it after the attention call, with its arguments and its log-sum-exp ``lse``.
+    ``scores`` fp32 ``[pages, page_size, kv_heads]``, any strides
+    (:meth:`~.kv_cache.PagedKVCache.empty_scores`); ``out``, by default ``scores``
+    itself, takes the new values. No two sequences may have a page in common. The
+    result does not depend on timing. Returns ``out``."""
+    index = _on_device("kv_cache_scores", q, cache.k, page_table, kv_lens, q_starts, lse, scores,
+                       out, workspace)
+    code, tokens, heads, dim, seqs, _ = _attention_args(q, cache, page_table, kv_lens, q_starts, q)
+    if lse.dtype != torch.float32 or lse.shape != (tokens, heads) or not lse.is_contiguous():
+        raise ValueError(f"lse must be a contiguous float32 [{tokens}, {heads}], got {lse.dtype} "
+                         f"{tuple(lse.shape)}")
+    _scores_of(scores, cache)
+    if out is None:
+        out = scores
+    else:
+        _scores_of(out, cache, "out")
+    if 0 in q.stride()[:2]:  # one vector for several rows: not for tensor copies
+        q = q.contiguous()
+    stream = _raw_stream(index)
+    if workspace is not None:
+        ws = _own_workspace(workspace)
+    else:
+        key = (dim, -(-tokens // 256) * 256, heads)
+        nbytes = _SCORES_BYTES.get(key)
+        if nbytes is None:
+            nbytes = _SCORES_BYTES[key] = kv_cache_scores_workspace_bytes(*key)
+        ws = _attn_workspace_of(index, stream, nbytes)
+    _lib.check(lib().b200_kv_cache_scores(
+        cache.desc, q.data_ptr(), code, tokens, heads, q.stride(0), q.stride(1),
+        page_table.data_ptr(), page_table.stride(0), page_table.shape[1], kv_lens.data_ptr(),
+        q_starts.data_ptr(), seqs, max_q_len, dim ** -0.5 if scale is None else scale, causal,
+        window, lse.data_ptr(), scores.data_ptr(), *scores.stride(), out.data_ptr(), *out.stride(),
+        ws.data_ptr(), ws.numel(), stream))
+    return out
 
 
 def kv_cache_evict(cache, scores: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor,
