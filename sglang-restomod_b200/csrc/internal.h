@@ -412,6 +412,8 @@ struct ScoresLaunch {
 };
 long long kv_scores_scratch_bytes(int head_dim, long long q_tokens, int q_heads);
 cudaError_t launch_kv_scores(const ScoresLaunch& l, cudaStream_t stream);
+// up to 16 rows (new tokens x query heads of a key/value head) a sequence
+cudaError_t launch_kv_scores_stream(const ScoresLaunch& l, cudaStream_t stream);
 
 // Held, one per device, while a call that uses a workspace puts its launches on a
 // stream: kernels of one call hand on through the workspace (a plan, converted
