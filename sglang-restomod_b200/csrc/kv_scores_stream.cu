@@ -10,18 +10,21 @@
 //
 // Bound: HBM, each key once; 2 * rows operations an element are far below the
 // tensor rate. A warp takes 16 tokens in M of m16n8k16 and 8 rows in N. The order of
-// a dot product's terms is free, so lane (g, c) reads the 16-byte pieces c, c + 4,
-// ... of tokens g and g + 8 and of row g, and has its part of both operands: no shared
-// memory, no barriers, pages of any size and strides. 16 warps an SM hold 32 registers
-// of keys that they work on and 32 on their way each, 128 KB an SM.
+// a dot product's terms is free, so lane (g, c) takes the 16-byte pieces c, c + 4,
+// ... of tokens g and g + 8 and of row g, and has its part of both operands. Keys
+// come by 16-byte asynchronous copies into shared memory that only the copying lane
+// reads: no barriers, pages of any size and strides, and every warp goes its own way.
+// 16 warps an SM with two stages of 4 KB on their way each hold 128 KB under way.
+// (With the keys on their way in registers, 64 a thread, e4m3 came to 84 us for
+// 64 sequences of up to 8192 tokens, 8 heads of 128: too little was under way.)
 //
 // e4m3 codes become f16 (exact); bf16 queries are brought to f16 by a power of two
 // per row, exact but for what lies 2^-24 below the row's largest element. The
 // key's scale multiplies the products' sum in fp32. A token's weights are added over
 // its lane quarter in a fixed order, by the one warp that has the token.
 //
-// The tiles of all (sequence, head) pairs are laid end to end and cut evenly over all
-// warps of the GPU.
+// The tiles of all (sequence, head) pairs are laid end to end, each pair with a
+// constant for its start, and cut evenly over all warps of the GPU.
 #include <algorithm>
 
 #include "common.cuh"
@@ -34,6 +37,8 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kMinTiles = 2;  // of a warp, where there are few
+// What a pair costs besides its tiles, in tiles: queries in, the first keys' latency.
+constexpr int kPairCost = 3;
 
 enum { kBf16 = 0, kF16 = 1, kE4m3 = 2 };
 
@@ -52,7 +57,10 @@ struct Shape {
   // of 16 tokens, a tile: a lane of a quarter has one token of a tile as its own
   static constexpr int kSets = kRegs >= 32 ? 1 : 2;
   static constexpr int kTile = 16 * kSets;
-  static constexpr int kBlocks = kRegs > 32 ? 1 : kRegs == 8 ? 3 : 2;
+  static constexpr int kStage = kSets * 2 * kPieces * 512;  // bytes of a warp's tile
+  static constexpr int kBlocks = kStage > 4096 ? 1 : 2;
+  static constexpr int kStages = kStage < 4096 ? 6 : 3;
+  static constexpr size_t kSmem = (size_t)kWarps * kStages * (kStage + 128);  // (page numbers)
 };
 
 __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
@@ -92,17 +100,22 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV>::kBlocks)
   __shared__ long long base_sh[kThreads], scan_sh[kWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, c = lane & 3;
+  extern __shared__ __align__(16) uint8_t smem[];
+  constexpr int kStages = S::kStages;
+  uint8_t* stages = smem + warp * kStages * S::kStage + lane * 16;
+  int* pages = reinterpret_cast<int*>(smem + kWarps * kStages * S::kStage) + warp * kStages * 32 + lane;
   griddep_wait();
   griddep_launch_dependents();
 
   // ---- this warp's tiles
   auto tiles_of = [&](const SeqLens& q) { return (q.kv_len + S::kTile - 1) / S::kTile; };
+  auto cost_of = [&](const SeqLens& q) { return q.kv_len ? tiles_of(q) + kPairCost : 0; };
   const int per = (a.seqs + kThreads - 1) / kThreads;
   long long before, total = 0;
   {
     const int s0 = min(tid * per, a.seqs), s1 = min(s0 + per, a.seqs);
     long long mine = 0;
-    for (int s = s0; s < s1; ++s) mine += (long long)tiles_of(seq_lens(a, s)) * a.c.heads;
+    for (int s = s0; s < s1; ++s) mine += (long long)cost_of(seq_lens(a, s)) * a.c.heads;
     before = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -126,7 +139,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV>::kBlocks)
   if (me >= warps) return;
   long long at = total * me / warps;
   const long long end = total * (me + 1) / warps;
-  int seq, head, tile;
+  int seq, head, cost;  // cost: place in the pair's
   {
     int lo = 0, hi = kThreads - 1;  // last thread with a base <= at
     while (lo < hi) {
@@ -138,18 +151,18 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV>::kBlocks)
     }
     long long x = at - base_sh[lo];
     seq = lo * per;
-    int n = tiles_of(seq_lens(a, seq));
+    int n = cost_of(seq_lens(a, seq));
     while (x >= (long long)n * a.c.heads) {
       x -= (long long)n * a.c.heads;
-      n = tiles_of(seq_lens(a, ++seq));
+      n = cost_of(seq_lens(a, ++seq));
     }
     head = (int)(x / n);
-    tile = (int)(x - (long long)head * n);
+    cost = (int)(x - (long long)head * n);
   }
 
-  // Keys of a tile, and of the lane's own token (see own_of) the rest.
-  struct Keys {
-    uint4 k[kSets][2][kPieces];
+  // What belongs to the lane's own token of a tile (see own_of).
+  struct Own {
+    int page;
     uint32_t scale;
     float old;
   };
@@ -158,7 +171,20 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV>::kBlocks)
     // ---- a (sequence, head) pair: tiles [tile, tile1) of it are this warp's
     const SeqLens q = seq_lens(a, seq);
     const int n = tiles_of(q);
-    const int tile1 = (int)min((long long)n, tile + (end - at));
+    const int cost1 = (int)min((long long)(n + kPairCost), cost + (end - at));
+    const int tile = max(0, cost - kPairCost), tile1 = max(0, cost1 - kPairCost);
+    at += cost1 - cost;
+    cost = 0;
+    const int this_seq = seq, this_head = head;
+    if (cost1 == n + kPairCost && ++head == a.c.heads) {
+      head = 0;
+      if (at < end) {
+        do {
+          ++seq;
+        } while (cost_of(seq_lens(a, seq)) == 0);
+      }
+    }
+    if (tile == tile1) continue;
     const int rows = q.q_len * p.groups;
     const int lowest = a.window > 0 ? q.pos0 - a.window + 1 : 0;  // that any row sees
 
@@ -172,7 +198,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV>::kBlocks)
       const int r = 8 * nr + g;
       const uint16_t* src = static_cast<const uint16_t*>(a.q) +
                             (long long)(q.q0 + r / p.groups) * a.q_token_stride +
-                            (long long)(head * p.groups + r % p.groups) * a.q_head_stride;
+                            (long long)(this_head * p.groups + r % p.groups) * a.q_head_stride;
       float unit = 1.f;
       if (KV != kE4m3) {
 #pragma unroll
@@ -222,7 +248,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV>::kBlocks)
         factor[nr][j] = p.scale_log2 * (KV == kE4m3 ? __shfl_sync(0xffffffffu, unit, (2 * c + j) * 4) : 1.f);
         float l = -INFINITY;
         if (row < rows)
-          l = __ldg(a.lse + (long long)(q.q0 + token) * a.q_heads + head * p.groups + row % p.groups);
+          l = __ldg(a.lse + (long long)(q.q0 + token) * a.q_heads + this_head * p.groups + row % p.groups);
         nl[nr][j] = l == -INFINITY ? l : -l * kLog2e;
         row_token[nr][j] = row < rows ? token : -1;
         const int pos = q.pos0 + token;
@@ -238,46 +264,56 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV>::kBlocks)
     const bool copies = p.l.scores_in != p.l.scores_out;
 
     // Bases of this head; a token's place is page * page_stride + offset * token_stride.
-    const uint8_t* keys = static_cast<const uint8_t*>(a.c.k) + head * a.c.head_stride * S::kElem + c * 16;
-    const uint8_t* scales = KV == kE4m3 ? a.c.k_scale + head * a.c.scale_head_stride : nullptr;
-    const float* in = p.l.scores_in + head * p.l.in_head;
-    float* out = p.l.scores_out + head * p.l.out_head;
+    const uint8_t* keys = static_cast<const uint8_t*>(a.c.k) + this_head * a.c.head_stride * S::kElem + c * 16;
+    const uint8_t* scales = KV == kE4m3 ? a.c.k_scale + this_head * a.c.scale_head_stride : nullptr;
+    const float* in = p.l.scores_in + this_head * p.l.in_head;
+    float* out = p.l.scores_out + this_head * p.l.out_head;
     // The lane's own token of a tile: set c / 2, its token g or g + 8.
     const int own_of = (kSets > 1 ? c >> 1 : 0) * 16 + g + 8 * (c & 1);
     // The own token's page: -2 past the last token, -1 outside the cache.
     auto look = [&](int t) {
       const int token = t * S::kTile + own_of;
       return t < tile1 && token < q.kv_len
-                 ? __ldg(a.table + seq * a.table_stride + p.by_page.of(token))
+                 ? __ldg(a.table + this_seq * a.table_stride + p.by_page.of(token))
                  : -2;
     };
-    auto load = [&](Keys& k, int page, int t) {
-      const bool seen = rows > 0 && (t + 1) * S::kTile > lowest;
+    // A tile's keys on their way to a stage, with its page numbers.
+    auto copy = [&](int stage, int page, int t) {
+      pages[stage * 32] = page;
       const int token = t * S::kTile + own_of;
       const int offset = token - p.by_page.of(token) * a.c.page_size;
       const bool there = page >= 0 && page < a.c.num_pages;
       bad |= !there && page != -2;
-      const long long place = there && seen ? (page * a.c.page_stride + offset * a.c.token_stride) * S::kElem
-                                            : -1;
+      const long long place = there && rows > 0 && (t + 1) * S::kTile > lowest
+                                  ? (page * a.c.page_stride + offset * a.c.token_stride) * S::kElem
+                                  : -1;
 #pragma unroll
       for (int i = 0; i < kSets; ++i)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const long long from = __shfl_sync(0xffffffffu, place, 4 * g + 2 * i + h);
+          // (what is not copied is masked, or belongs to a token that is not written)
+          if (from >= 0) {
 #pragma unroll
-          for (int x = 0; x < kPieces; ++x) {
-            k.k[i][h][x] = make_uint4(0u, 0u, 0u, 0u);
-            if (from >= 0) k.k[i][h][x] = __ldcs(reinterpret_cast<const uint4*>(keys + from + x * 64));
+            for (int x = 0; x < kPieces; ++x)
+              cp_async_16(stages + stage * S::kStage + ((i * 2 + h) * kPieces + x) * 512,
+                          keys + from + x * 64);
           }
         }
-      k.scale = 0;
-      if (KV == kE4m3 && there && seen)
-        k.scale = __ldg(scales + page * a.c.scale_page_stride + offset * a.c.scale_token_stride);
-      k.old = 0.f;
-      if (there && !(a.causal && token >= q.pos0))
-        k.old = in[page * p.l.in_page + offset * p.l.in_token];
     };
-    auto weigh = [&](const Keys& k, int page, int t) {
+    auto fetch = [&](Own& o, int stage, int t) {
+      o.page = pages[stage * 32];
+      o.scale = 0;
+      o.old = 0.f;
+      const int token = t * S::kTile + own_of;
+      const int offset = token - p.by_page.of(token) * a.c.page_size;
+      if (o.page < 0 || o.page >= a.c.num_pages) return;
+      if (KV == kE4m3)
+        o.scale = __ldg(scales + o.page * a.c.scale_page_stride + offset * a.c.scale_token_stride);
+      if (!(a.causal && token >= q.pos0)) o.old = in[o.page * p.l.in_page + offset * p.l.in_token];
+    };
+    auto weigh = [&](const Own& o, int stage, int t) {
+      const uint8_t* keys = stages + stage * S::kStage;
       float mine = 0.f;  // of the own token
 #pragma unroll
       for (int i = 0; i < kSets; ++i) {
@@ -288,7 +324,8 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV>::kBlocks)
           for (int j = 0; j < 4; ++j) s[nr][j] = 0.f;
 #pragma unroll
         for (int x = 0; x < kPieces; ++x) {
-          const uint4 u = k.k[i][0][x], v = k.k[i][1][x];
+          const uint4 u = ld_shared_u128(keys + (i * 2 * kPieces + x) * 512);
+          const uint4 v = ld_shared_u128(keys + ((i * 2 + 1) * kPieces + x) * 512);
           if (KV != kE4m3) {
             const uint32_t a0[4] = {u.x, v.x, u.y, v.y}, a1[4] = {u.z, v.z, u.w, v.w};
 #pragma unroll
@@ -320,7 +357,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV>::kBlocks)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           if (KV == kE4m3) {
-            const uint32_t byte = __shfl_sync(0xffffffffu, k.scale, 4 * g + 2 * i + h);
+            const uint32_t byte = __shfl_sync(0xffffffffu, o.scale, 4 * g + 2 * i + h);
             const float key = byte == 255u ? __int_as_float(0x7fc00000) : __uint_as_float(byte << 23);
 #pragma unroll
             for (int nr = 0; nr < NR; ++nr) s[nr][2 * h] *= key, s[nr][2 * h + 1] *= key;
@@ -345,38 +382,42 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV>::kBlocks)
         }
       }
       const int token = t * S::kTile + own_of;
-      if ((kSets == 1 && c > 1) || page < 0 || page >= a.c.num_pages) return;
+      if ((kSets == 1 && c > 1) || o.page < 0 || o.page >= a.c.num_pages) return;
       // (in place, what no row sees stays as it is)
       if (copies || (a.causal && token >= q.pos0) || (rows > 0 && token >= lowest))
-        out[page * p.l.out_page + (token - p.by_page.of(token) * a.c.page_size) * p.l.out_token] =
-            k.old + mine;
+        out[o.page * p.l.out_page + (token - p.by_page.of(token) * a.c.page_size) * p.l.out_token] =
+            o.old + mine;
     };
-    // Two tiles in turn: one is worked on while the other is on its way, and the page
-    // numbers of the next but one.
-    Keys ka, kb;
-    int pa = look(tile), pb = look(tile + 1);
-    load(ka, pa, tile);
+    // Keys are kStages - 1 tiles ahead, page numbers one more; the rest of a token a tile.
+    int page = look(tile);
+#pragma unroll 1
+    for (int i = 0; i < kStages - 1; ++i) {
+      const int next = look(tile + i + 1);
+      copy(i, page, tile + i);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      page = next;
+    }
+    Own oa, ob;
+    fetch(oa, 0, tile);
+    int stage = 0;
+    auto turn = [&](Own& now, Own& next, int t) {
+      const int free = stage == 0 ? kStages - 1 : stage - 1;  // the tile before's
+      const int ahead = look(t + kStages);
+      copy(free, page, t + kStages - 1);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      page = ahead;
+      const int then = stage + 1 == kStages ? 0 : stage + 1;
+      fetch(next, then, t + 1);
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+      weigh(now, stage, t);
+      stage = then;
+    };
 #pragma unroll 1
     for (int t = tile; t < tile1; t += 2) {
-      load(kb, pb, t + 1);
-      int next = look(t + 2);
-      weigh(ka, pa, t);
-      pa = next;
-      load(ka, pa, t + 2);
-      next = look(t + 3);
-      if (t + 1 < tile1) weigh(kb, pb, t + 1);
-      pb = next;
+      turn(oa, ob, t);
+      if (t + 1 < tile1) turn(ob, oa, t + 1);
     }
-    at += tile1 - tile;
-    tile = 0;
-    if (tile1 == n && ++head == a.c.heads) {
-      head = 0;
-      if (at < end) {
-        do {
-          ++seq;
-        } while (tiles_of(seq_lens(a, seq)) == 0);
-      }
-    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   }
   if (__any_sync(0xffffffffu, bad) && lane == 0) {
     atomicOr(a.status.call, kDevBadPage);
@@ -386,10 +427,23 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV>::kBlocks)
 
 template <int D, int KV>
 cudaError_t launch(const RowParams& p, int rows, cudaStream_t stream) {
-  const dim3 grid((unsigned)(Shape<D, KV>::kBlocks * device_sm_count()));
-  return rows <= 8
-             ? launch_pdl(kv_scores_stream_kernel<D, KV, 1>, grid, dim3(kThreads), 0, stream, p)
-             : launch_pdl(kv_scores_stream_kernel<D, KV, 2>, grid, dim3(kThreads), 0, stream, p);
+  using S = Shape<D, KV>;
+  static_assert((S::kSmem + 4096) * S::kBlocks <= 227 * 1024, "shared memory");
+  static bool configured[64] = {};
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err != cudaSuccess) return err;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (!configured[dev]) {
+    for (auto kernel : {kv_scores_stream_kernel<D, KV, 1>, kv_scores_stream_kernel<D, KV, 2>}) {
+      err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem);
+      if (err != cudaSuccess) return err;
+    }
+    configured[dev] = true;
+  }
+  return launch_pdl(rows <= 8 ? kv_scores_stream_kernel<D, KV, 1> : kv_scores_stream_kernel<D, KV, 2>,
+                    dim3((unsigned)(S::kBlocks * device_sm_count())), dim3(kThreads), S::kSmem, stream,
+                    p);
 }
 
 template <int D>
