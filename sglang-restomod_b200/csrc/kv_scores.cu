@@ -14,8 +14,12 @@
 // and one writer for each score, so results do not depend on timing. What a lane
 // holds past the last token stays in that lane and is dropped.
 //
-// Bound: few new tokens, HBM (each key once); many, the exponentials, one per (row,
-// key) at 16 a clock and SM, which take twice as long as the products at head_dim 128.
+// For more than 16 rows a sequence (kv_scores_stream.cu takes fewer).
+//
+// Bound: the exponentials, one per (row, key) at 16 a clock and SM, which take twice
+// as long as the products at head_dim 128. (A polynomial on the fma pipe for one, two
+// or three eighths of them made it slower: 462, 475, 500, 533 us for a prompt of 8192
+// tokens.) Few rows: HBM, each key once.
 //
 // e4m3 keys go to the tensor cores as they are (kind::f8f6f4): a query is brought
 // into [128, 256) by a power of two and split into e4m3 terms, q = t1 + (t2 + t3) / 32,
@@ -23,17 +27,20 @@
 // K t1 and K (t2 + t3) are two sums, side by side in tensor memory. The key's
 // scale multiplies their sum in fp32.
 //
-// Work: items of up to `run` units of 256 tokens of a (sequence, head), given out by
-// a counter, the longest first where a prompt's units see fewer and fewer rows.
-// Warps: 0-3 and 4-7 epilogue of a unit's first and second 128 tokens, 8 the items and
-// copies of Q, 9 products and tensor memory, 10-13 the tokens, a tile of 128 in turn
-// (page, old score, scale, place of the new score; where pages are no multiple of 8
-// tokens also the copies of their keys, 16 bytes at a time), 14 tensor copies of keys.
+// Work: items of 256 tokens of a (sequence, head), given out by a counter, the
+// longest first where a prompt's tokens are seen by fewer and fewer rows. Warps: 0-7
+// and 8-15 epilogue of an item's first and second 128 tokens, four of the eight for
+// the even 32 columns of a tile and four for the odd, 16 the items and copies of Q, 17
+// and 18 products of either half, 19 tensor copies of keys, 20 and 21 the tokens of
+// either half (page, old score, scale, place of the new score; where pages are no
+// multiple of 8 tokens also the copies of their keys, 16 bytes at a time).
 //
-// The roles' code is kept short (no divisions, waits' slow path and rare cases out of
-// line, loops not unrolled that need not be): all roles run at once, and what they
-// execute for a unit of a decode step has to fit the instruction cache. At 30 KB it
-// did not, and half of the time went by without instructions.
+// While products read their operands from shared memory everything else there is
+// slow: a wait on a barrier that is long complete takes 300 clocks, and a tile of 128 x
+// 128 x 128 takes 600. So each half's products have a thread of their own, with two
+// waits a tile (one thread for both, with slices counted at run time: 750 us), and four
+// epilogue warps share a quarter of the SM to fill one another's waits (with two, 64
+// columns at a time: 462 us).
 #include <algorithm>
 
 #include "attn_maps.cuh"
@@ -48,22 +55,20 @@ namespace {
 using namespace tcg;
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kEpiWarps = 8, kQWarp = 8, kMmaWarp = 9, kTokenWarp = 10, kTokenWarps = 4;
-constexpr int kKeyWarp = kTokenWarp + kTokenWarps;
-constexpr int kPages = 4;        // K tiles whose page numbers are on their way
-constexpr int kUnit = 256;       // tokens of a unit: two tiles of 128
-constexpr int kMaxKeys = 12, kMaxQ = 3, kItems = 4;
+// A hidden column is an infinity that factors multiply, so a factor of zero becomes the
+// smallest normal number: finite products still come to e^0.
+constexpr float kMinScale = 1.1754944e-38f;
+constexpr int kEpiWarps = 16, kQWarp = 16, kMmaWarp = 17, kKeyWarp = 19, kTokenWarp = 20;
+constexpr int kThreads = 22 * 32;
+constexpr int kUnit = 256;       // tokens of an item: two tiles of 128
+constexpr int kMaxKeys = 12, kMaxQ = 3, kItems = 4, kTokens = 2;
 constexpr int kScan = 256;       // threads that share out the sequences
 constexpr uint32_t kTmemCols = 512;
 constexpr int kTerms = 3;        // e4m3 terms of an f16 query (bf16: two)
 constexpr int kFine = 32;        // t2 and t3 are in units of 1 / 32
-
-constexpr int kTables = kEpiWarps * 128 * 4 + kTokenWarps * 128 * 16;
-
-template <bool TMA>
-constexpr int threads() {
-  return (kKeyWarp + (TMA ? 1 : 0)) * 32;
-}
+// Of Q tiles' rows, [16 warps][128] floats; of tokens, [2 halves][kTokens][128]; sums of
+// the odd columns, [2 halves][2][128] floats.
+constexpr int kTables = kEpiWarps * 128 * 4 + 2 * kTokens * 128 * 16 + 2 * 2 * 128 * 4;
 
 struct ScoreParams {
   AttnLaunch a;
@@ -78,7 +83,6 @@ struct ScoreParams {
   int terms;              // e4m3
   int key_stages, q_stages, key_bytes, q_bytes;
   int row_bytes, slices;  // of a slice of a vector (128, or 64), and how many it has
-  int run;                // units of an item
   int box_rows, heads_first;
   Divisor by_page, by_tile;  // of the page size, of tile_tokens
   int* next;              // [0] items given out, [1] blocks done; zero between calls
@@ -87,8 +91,9 @@ struct ScoreParams {
 };
 
 struct Item {
-  int seq, head, unit, units;  // seq < 0: no more
+  int seq, head, key0;  // seq < 0: no more
   int q0, q_len, pos0, kv_len;
+  int first, last;      // Q tiles with a row that sees one of the tokens
 };
 
 struct Ctl {
@@ -96,10 +101,10 @@ struct Ctl {
   uint64_t q_full[kMaxQ], q_empty[kMaxQ];
   uint64_t s_full[4], s_empty[4];  // tile * 2 + buffer
   uint64_t item_full[kItems], item_empty[kItems];
-  uint64_t token_full[kTokenWarps], token_empty[kTokenWarps];
-  uint64_t drained;
+  uint64_t token_full[2 * kTokens], token_empty[2 * kTokens];  // half * kTokens + slot
+  uint64_t odd_full[4], odd_empty[4];  // half * 2 + buffer
+  uint64_t drained[2];
   Item items[kItems];
-  int pages[kPages][16];  // of the boxes of K tiles
   uint32_t tmem;
   int abort, errors;
 };
@@ -158,20 +163,19 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, Ctl* c
   return __shfl_sync(0xffffffffu, ok, 0);
 }
 
-// Q tiles [first, last) with a row that sees a token of the unit from key0 on.
-__device__ __forceinline__ void q_tiles(const ScoreParams& p, const Item& it, int key0, int& first,
-                                        int& last) {
+// Q tiles [first, last) with a row that sees a token of the item.
+__device__ __forceinline__ void q_tiles(const ScoreParams& p, Item& it) {
   // new tokens [lo, hi) see some of them
   int lo = 0, hi = it.q_len;
   if (p.a.causal) {
-    lo = max(0, key0 - it.pos0);
+    lo = max(0, it.key0 - it.pos0);
     if (p.a.window > 0) {
-      const long long end = (long long)min(key0 + kUnit, it.kv_len) - 1 + p.a.window - it.pos0;
+      const long long end = (long long)min(it.key0 + kUnit, it.kv_len) - 1 + p.a.window - it.pos0;
       hi = end < hi ? max(0, (int)end) : hi;
     }
   }
-  first = p.by_tile.of(lo);
-  last = lo < hi ? p.by_tile.of(hi - 1) + 1 : first;
+  it.first = p.by_tile.of(lo);
+  it.last = lo < hi ? p.by_tile.of(hi - 1) + 1 : it.first;
 }
 
 // The items in the order they are given out, for one role.
@@ -194,41 +198,27 @@ struct Items {
     end = it.seq < 0;
     return !end;
   }
-};
-
-// A tile of 128 tokens whose keys some row needs, for their copies.
-struct KeyTile {
-  int seq, head, key0, kv_len;
-};
-struct KeyTiles {
-  Items items;
-  Item it;
-  int key0 = 0, end = 0;  // the item's tokens that are left
-  // The next tile. Without `wait` also none where its item is not out yet: whoever
-  // holds a tile that it has not copied must not wait for an item, which may wait for
-  // that tile's products.
-  __device__ __forceinline__ bool next(const ScoreParams& p, int lane, bool wait, KeyTile& t) {
-    for (;;) {
-      if (key0 >= end) {
-        if (items.end || (!wait && !items.ready())) return false;
-        if (!items.next(it, lane)) return false;
-        key0 = it.unit * kUnit;
-        end = min(key0 + it.units * kUnit, it.kv_len);
-      }
-      t.seq = it.seq, t.head = it.head, t.key0 = key0, t.kv_len = it.kv_len;
-      int first, last;
-      q_tiles(p, it, key0 & ~(kUnit - 1), first, last);
-      key0 += 128;
-      if (first < last) return true;
-    }
+  __device__ bool next_alone(Item& it) {  // of one thread
+    if (end) return false;
+    const uint32_t slot = n % kItems, phase = n / kItems & 1u;
+    ++n;
+    end = !wait_one(&ctl->item_full[slot], phase, ctl);
+    if (end) return false;
+    it = ctl->items[slot];
+    mbar_arrive(&ctl->item_empty[slot]);
+    end = it.seq < 0;
+    return !end;
   }
 };
 
-__device__ __forceinline__ uint64_t operand_desc(uint32_t saddr, int row_bytes) {
-  // K-major, atoms of 8 rows; 128-byte swizzle is layout 2, 64-byte 4
-  return (uint64_t)((saddr >> 4) & 0x3fffu) | (uint64_t)1u << 16 |
-         (uint64_t)(8u * row_bytes >> 4) << 32 | (uint64_t)1u << 46 |
-         (uint64_t)(row_bytes == 128 ? 2u : 4u) << 61;
+// K-major operand descriptors, atoms of 8 rows of 128 bytes (128-byte swizzle, layout
+// 2) or of 64 (64-byte, 4): the low word holds the address, in 16-byte units.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr) { return (saddr >> 4 & 0x3fffu) | 1u << 16; }
+template <int ROW>
+__device__ __forceinline__ uint64_t desc_of(uint32_t lo) {
+  constexpr uint64_t kHi = (uint64_t)(8u * ROW >> 4) << 32 | (uint64_t)1u << 46 |
+                           (uint64_t)(ROW == 128 ? 2u : 4u) << 61;
+  return kHi | lo;
 }
 // fp32 accumulator, M = 128, both operands K-major: f16 (0) or bf16 (1) of
 // kind::f16, e4m3 (0) of kind::f8f6f4.
@@ -257,6 +247,32 @@ __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint3
         "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
         : "memory");
 }
+// D (+)= K Q^T over SLICES slices of ROW bytes, 32 bytes at a time; a slice of K has
+// 128 rows, Q's are q_slice (16-byte units) apart. (The thread's instructions wait on
+// one another: with slices and steps counted at run time a tile's products took 1500
+// clocks to issue.)
+template <bool Q8, int ROW, int SLICES>
+__device__ __forceinline__ void mma_slices(uint32_t d, uint32_t k, uint32_t q, uint32_t q_slice,
+                                           uint32_t idesc, uint32_t accumulate) {
+#pragma unroll
+  for (int sl = 0; sl < SLICES; ++sl)
+#pragma unroll
+    for (int kk = 0; kk < ROW / 32; ++kk)
+      mma_ss<Q8>(d, desc_of<ROW>(k + (sl * 128 * ROW >> 4) + 2 * kk), desc_of<ROW>(q + sl * q_slice + 2 * kk),
+                 idesc, sl + kk > 0 ? 1u : accumulate);
+}
+template <bool Q8>
+__device__ __forceinline__ void mma_tile(const ScoreParams& p, uint32_t d, uint32_t k, uint32_t q,
+                                         uint32_t q_slice, uint32_t idesc, uint32_t accumulate) {
+  if (Q8 && p.row_bytes == 64)
+    mma_slices<Q8, 64, 1>(d, k, q, q_slice, idesc, accumulate);
+  else if (p.slices == 1)
+    mma_slices<Q8, 128, 1>(d, k, q, q_slice, idesc, accumulate);
+  else if (p.slices == 2)
+    mma_slices<Q8, 128, 2>(d, k, q, q_slice, idesc, accumulate);
+  else
+    mma_slices<Q8, 128, 4>(d, k, q, q_slice, idesc, accumulate);
+}
 __device__ __forceinline__ void fence_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
@@ -268,118 +284,50 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
       "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
       : "memory");
 }
-__device__ __forceinline__ void tmem_ld16_nowait(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,"
-      "%15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-        "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr));
-}
-// Completes the loads into r (the operands tie their uses to the wait).
-__device__ __forceinline__ void tmem_wait16(uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.wait::ld.sync.aligned;"
-      : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]),
-        "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]),
-        "+r"(r[14]), "+r"(r[15])::"memory");
-}
-
-__device__ __forceinline__ void tmem_wait(uint32_t (&r)[16]) { tmem_wait16(r); }
-__device__ __forceinline__ void tmem_wait(uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.wait::ld.sync.aligned;"
-      : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]),
-        "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]),
-        "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]),
-        "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]),
-        "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
-}
-__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[16]) {
-  tmem_ld16_nowait(taddr, r);
-}
-__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[32]) {
-  tmem_ld32_nowait(taddr, r);
-}
-// Ties r's uses to a wait that came before.
-template <int N>
-__device__ __forceinline__ void tie(uint32_t (&r)[N]) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
-}
-
-// 2^x on the fma pipe, two at once: x = n + f with f in [-1/2, 1/2], 2^f by a
-// polynomial of degree 5 (minimax in relative error by an exchange iteration,
-// 2^-23.7; with its fp32 steps 2^-22.0, as the special function unit's), 2^n by its
-// exponent bits. Below -126.5 zero, above 127.5 infinity, NaN stays.
-__device__ __forceinline__ float clamp_exponent(float x) {
-  asm("min.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(128.f));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(-127.f));
-  return x;
-}
-__device__ __forceinline__ uint64_t both(float v) { return f32x2(v, v); }
-__device__ __forceinline__ uint64_t exp2_fma(uint64_t x) {
-  constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: its unit is 1
-  const float2 v = unpack_f32x2(x);
-  x = f32x2(clamp_exponent(v.x), clamp_exponent(v.y));
-  const uint64_t r = add_f32x2(x, both(kMagic));
-  const uint64_t f = add_f32x2(x, mul_f32x2(add_f32x2(r, both(-kMagic)), both(-1.f)));
-  uint64_t y = fma_f32x2(both(0.0013276472454890609f), f, both(0.009675540961325169f));
-  y = fma_f32x2(y, f, both(0.05550713092088699f));
-  y = fma_f32x2(y, f, both(0.24022120237350464f));
-  y = fma_f32x2(y, f, both(0.6931469440460205f));
-  y = fma_f32x2(y, f, both(1.0000001192092896f));
-  const float2 n = unpack_f32x2(r);
-  return mul_f32x2(y, f32x2(__uint_as_float((__float_as_uint(n.x) << 23) + 0x3f800000u),
-                            __uint_as_float((__float_as_uint(n.y) << 23) + 0x3f800000u)));
-}
-
-// The sum of a lane's weights over N columns: e^x in log2, x = s * factor + nl.
+// The sum of a lane's weights over 32 columns: e^x in log2, x = s * factor + nl.
 // s: fp32 products (e4m3: the coarse sum, `fine` the one in units of 1 / kFine,
-// `key` the key's scale). kFma of eight pairs are taken by exp2_fma, so that both
-// pipes work; hidden columns take the other path alone.
-constexpr int kFma = 3;
-template <bool Q8, bool MASKED, int N>
-__device__ __forceinline__ float weigh(const uint32_t (&s)[N], const uint32_t (&fine)[N], float scale,
-                                       float key, const float* nl, const float* factor, int c0,
-                                       int lo, int hi) {
-  uint64_t sum[2] = {0, 0};
+// `key` the key's scale). (One fp32 operation at a time: in pairs, the moves that join
+// and part them made it 8 instructions a column.)
+template <bool Q8>
+__device__ __forceinline__ float weigh(const uint32_t* s, const uint32_t* fine, float scale, float key,
+                                       const float* nl, const float* factor) {
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < N; i += 4) {
-    const float4 n4 = *reinterpret_cast<const float4*>(nl + c0 + i);
-    float4 f4 = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (Q8) f4 = *reinterpret_cast<const float4*>(factor + c0 + i);
+  for (int i = 0; i < 32; i += 4) {
+    const float4 n4 = *reinterpret_cast<const float4*>(nl + i);
+    const float n[4] = {n4.x, n4.y, n4.z, n4.w};
+    float f[4] = {scale, scale, scale, scale};
+    if (Q8) {
+      const float4 f4 = *reinterpret_cast<const float4*>(factor + i);
+      f[0] = f4.x, f[1] = f4.y, f[2] = f4.z, f[3] = f4.w;
+    }
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int j = i + 2 * h;
-      uint64_t x = f32x2(__uint_as_float(s[j]), __uint_as_float(s[j + 1]));
-      const uint64_t n2 = h ? f32x2(n4.z, n4.w) : f32x2(n4.x, n4.y);
-      if (Q8) {
-        x = fma_f32x2(f32x2(__uint_as_float(fine[j]), __uint_as_float(fine[j + 1])),
-                      both(1.f / kFine), x);
-        x = fma_f32x2(mul_f32x2(x, both(key)), h ? f32x2(f4.z, f4.w) : f32x2(f4.x, f4.y), n2);
-      } else {
-        x = fma_f32x2(x, both(scale), n2);
-      }
-      if (!MASKED && (j / 2 * kFma) % 8 < kFma) {
-        x = exp2_fma(x);
-      } else {
-        float2 v = unpack_f32x2(x);
-        if (MASKED) {
-          v.x = c0 + j >= lo && c0 + j < hi ? v.x : -INFINITY;
-          v.y = c0 + j + 1 >= lo && c0 + j + 1 < hi ? v.y : -INFINITY;
-        }
-        x = f32x2(ex2(v.x), ex2(v.y));
-      }
-      sum[h] = add_f32x2(sum[h], x);
+    for (int j = 0; j < 4; ++j) {
+      float x = __uint_as_float(s[i + j]);
+      if (Q8) x = fmaf(__uint_as_float(fine[i + j]), 1.f / kFine, x) * key;
+      x = fmaf(x, f[j], n[j]);
+      sum[j] += ex2(x);
     }
   }
-  const float2 t = unpack_f32x2(add_f32x2(sum[0], sum[1]));
-  return t.x + t.y;
+  return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+}
+// Columns outside [lo, hi) become `hidden`, an infinity that the factor makes -inf.
+__device__ __forceinline__ void hide(uint32_t* s, int lo, int hi, float hidden) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) s[i] = i >= lo && i < hi ? s[i] : __float_as_uint(hidden);
+}
+// Ties r's uses to a tcgen05.wait::ld that came before.
+__device__ __forceinline__ void tie32(uint32_t* r) {
+  asm volatile(""
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
+                 "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                 "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]),
+                 "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31]));
 }
 
-// A unit's token, from the token warps to the epilogue.
+// An item's token, from the token warps to the epilogue.
 struct __align__(16) Token {
   float old;        // its score so far
   float key_scale;  // e4m3
@@ -387,7 +335,7 @@ struct __align__(16) Token {
 };
 
 template <bool Q8, bool TMA>
-__global__ void __launch_bounds__(threads<TMA>(), 1)
+__global__ void __launch_bounds__(kThreads, 1)
     kv_scores_kernel(const ScoreParams p, const __grid_constant__ CUtensorMap q_map,
                      const __grid_constant__ CUtensorMap k_map) {
   extern __shared__ uint8_t smem_raw[];
@@ -395,10 +343,11 @@ __global__ void __launch_bounds__(threads<TMA>(), 1)
   const uint32_t keys_at = smem_u32(smem);
   const uint32_t q_at = keys_at + p.key_stages * p.key_bytes;
   uint8_t* after = smem + p.key_stages * p.key_bytes + p.q_stages * p.q_bytes;
-  // of the Q tile's rows: -lse in log2 (16-bit caches), or with the row's factor
-  // beside it, a warp its own: [8][128] floats
+  // Of a Q tile's rows, a warp its own: -lse in log2, and (e4m3) from 64 on the row's
+  // factor.
   float* row_sh = reinterpret_cast<float*>(after);
-  Token* token_sh = reinterpret_cast<Token*>(after + kEpiWarps * 128 * 4);  // [kTokenWarps][128]
+  Token* token_sh = reinterpret_cast<Token*>(after + kEpiWarps * 128 * 4);
+  float* odd_sh = reinterpret_cast<float*>(after + kEpiWarps * 128 * 4 + 2 * kTokens * 128 * 16);
   Ctl* ctl = reinterpret_cast<Ctl*>(after + kTables);
   const AttnLaunch& a = p.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -411,21 +360,23 @@ __global__ void __launch_bounds__(threads<TMA>(), 1)
     }
     for (int i = 0; i < kMaxQ; ++i) {
       mbar_init(&ctl->q_full[i], 1);
-      mbar_init(&ctl->q_empty[i], 1);
+      mbar_init(&ctl->q_empty[i], 2);
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(&ctl->s_full[i], 1);
-      mbar_init(&ctl->s_empty[i], 4);
+      mbar_init(&ctl->s_empty[i], 8);
+      mbar_init(&ctl->odd_full[i], 4);
+      mbar_init(&ctl->odd_empty[i], 4);
     }
     for (int i = 0; i < kItems; ++i) {
       mbar_init(&ctl->item_full[i], 1);
-      mbar_init(&ctl->item_empty[i], kEpiWarps + 1 + kTokenWarps + (TMA ? 1 : 0));
+      mbar_init(&ctl->item_empty[i], kEpiWarps + 4 + (TMA ? 1 : 0));
     }
-    for (int i = 0; i < kTokenWarps; ++i) {
+    for (int i = 0; i < 2 * kTokens; ++i) {
       mbar_init(&ctl->token_full[i], 1);
       mbar_init(&ctl->token_empty[i], kEpiWarps / 2);
     }
-    mbar_init(&ctl->drained, 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&ctl->drained[i], 1);
     ctl->abort = ctl->errors = 0;
     fence_mbar_init();
   }
@@ -437,22 +388,22 @@ __global__ void __launch_bounds__(threads<TMA>(), 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   // Rows of a Q tile that no copy fills stay zeros.
-  for (int i = tid * 16; i < p.q_stages * p.q_bytes; i += threads<TMA>() * 16)
+  for (int i = tid * 16; i < p.q_stages * p.q_bytes; i += kThreads * 16)
     *reinterpret_cast<uint4*>(smem + p.key_stages * p.key_bytes + i) = make_uint4(0u, 0u, 0u, 0u);
   fence_async_smem();
   griddep_wait();
 
-  // Items before each thread's sequences: a sequence has runs(s) for each head.
-  auto runs = [&](int s) -> long long {
+  // Items before each thread's sequences: a sequence has units(s) for each head.
+  auto units = [&](int s) -> long long {
     const SeqLens q = seq_lens(a, s);
-    return (q.kv_len + kUnit * p.run - 1) / (kUnit * p.run);
+    return (q.kv_len + kUnit - 1) / kUnit;
   };
   const int per = (a.seqs + kScan - 1) / kScan;
-  long long before = 0, mine_runs = 0;
+  long long before = 0, mine_units = 0;
   if (tid < kScan) {
     const int s0 = min(tid * per, a.seqs), s1 = min(s0 + per, a.seqs);
-    for (int s = s0; s < s1; ++s) mine_runs += runs(s) * a.c.heads;
-    before = mine_runs;
+    for (int s = s0; s < s1; ++s) mine_units += units(s) * a.c.heads;
+    before = mine_units;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const long long y = __shfl_up_sync(0xffffffffu, before, o);
@@ -466,7 +417,7 @@ __global__ void __launch_bounds__(threads<TMA>(), 1)
     if (w < warp) before += scan_sh[w];
     total += scan_sh[w];
   }
-  if (tid < kScan) base_sh[tid] = before - mine_runs;
+  if (tid < kScan) base_sh[tid] = before - mine_units;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -476,18 +427,19 @@ __global__ void __launch_bounds__(threads<TMA>(), 1)
 
   if (warp < kEpiWarps) {
     // ------------------------------------------------------------ epilogue
-    const int half = warp >> 2, row = (warp & 3) * 32 + lane;
+    const int half = warp >> 3, odd = warp >> 2 & 1, row = (warp & 3) * 32 + lane;
     const uint32_t lane_addr = tmem + ((uint32_t)(warp & 3) << 21) + half * 256;
     float* mine = row_sh + warp * 128;
     Items items{ctl};
     Item it;
-    // Rows of Q tiles: row c = lane + 32 k of a tile is token c / groups, head c %
-    // groups. Their log-sums and factors are in shared memory for one tile, a warp its
-    // own, and on their way in registers for the next.
-    int row_token[4], row_at[4];
+    // Rows of Q tiles: row c of a tile is token c / groups, head c % groups. Their
+    // log-sums and factors are in shared memory for one tile, a warp its own, and on
+    // their way in registers for the next.
+    // (this warp's 32 columns c0 = 32 odd, and 64 + c0)
+    int row_token[2], row_at[2];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int c = lane + 32 * k;
+    for (int k = 0; k < 2; ++k) {
+      const int c = lane + 32 * odd + 64 * k;
       row_token[k] = c < rows ? c / p.groups : 0x40000000;
       row_at[k] = c / p.groups * a.q_heads + c % p.groups;
     }
@@ -496,140 +448,120 @@ __global__ void __launch_bounds__(threads<TMA>(), 1)
       __device__ bool is(const Tile& o) const { return seq == o.seq && head == o.head && q == o.q; }
     };
     Tile have, coming;
-    float lse_next[4], factor_next[4];
+    float lse_next[2], factor_next = 0.f;
+    const float plus = p.scale_log2 >= 0.f ? 1.f : -1.f;
     auto load_rows = [&](const Tile& t, const Item& of) {
       coming = t;
       const int tok0 = t.q * p.tile_tokens;
       const long long at = (long long)(of.q0 + tok0) * a.q_heads + t.head * p.groups;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < 2; ++k) {
         lse_next[k] = -INFINITY;
-        factor_next[k] = 0.f;
-        if (32 * k < p.nq && row_token[k] < of.q_len - tok0) {
-          lse_next[k] = __ldg(a.lse + at + row_at[k]);
-          if (Q8) factor_next[k] = __ldg(p.q_scale + at + row_at[k]);
-        }
+        if (row_token[k] < of.q_len - tok0) lse_next[k] = __ldg(a.lse + at + row_at[k]);
       }
+      // (of the scale's sign where there is no row: hidden columns come to -inf)
+      if (Q8) factor_next = row_token[0] < of.q_len - tok0 ? __ldg(p.q_scale + at + row_at[0]) : plus;
     };
     auto publish_rows = [&]() {
       have = coming;
       __syncwarp();
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (32 * k < p.nq) {
-          mine[lane + 32 * k] = lse_next[k] == -INFINITY ? -INFINITY : -lse_next[k] * kLog2e;
-          if (Q8 && k < 2) mine[64 + lane + 32 * k] = factor_next[k];
-        }
+      for (int k = 0; k < 2; ++k)
+        mine[lane + 32 * k] = lse_next[k] == -INFINITY ? -INFINITY : -lse_next[k] * kLog2e;
+      if (Q8) mine[64 + lane] = factor_next;
       __syncwarp();
     };
-    constexpr int kCols = Q8 ? 16 : 32;  // columns on their way together
-    uint32_t count = 0, tokens = half;   // S tiles so far; place among the token tiles
+    const float hidden = plus * -INFINITY;
+    uint32_t count = 0, tokens = 0;      // S tiles and items so far
     bool ok = true;
-    auto tokens_ready = [&](uint32_t slot) {
-      return wait_warp(&ctl->token_full[slot], tokens / kTokenWarps & 1u, ctl);
-    };
-    auto key_scale = [&](uint32_t slot) {
-      if (!Q8) return 1.f;
-      ok = tokens_ready(slot);
-      return token_sh[slot * 128 + row].key_scale;
-    };
-
     while (ok && items.next(it, lane)) {
+      const int key = it.key0 + half * 128 + row;
+      if (it.key0 + half * 128 >= it.kv_len) it.last = it.first;
+      // the columns, from the sequence's first row on, that see this token
+      const int seen0 = a.causal ? max(0, key - it.pos0) * p.groups : 0;
+      int seen1 = it.q_len;
+      if (a.window > 0)
+        seen1 = (int)min((long long)seen1, max(0ll, (long long)key + a.window - it.pos0));
+      seen1 *= p.groups;
+      const uint32_t slot = half * kTokens + tokens % kTokens;
+      float sum = 0.f, key_scale = 1.f;
+      if (Q8 && it.first < it.last) {
+        ok = wait_warp(&ctl->token_full[slot], tokens / kTokens & 1u, ctl);
+        // (zero would make a hidden column NaN: the smallest number instead)
+        key_scale = token_sh[slot * 128 + row].key_scale;
+        key_scale = key_scale == 0.f ? kMinScale : key_scale;
+      }
 #pragma unroll 1
-      for (int u = 0; u < it.units && ok; ++u, tokens += 2) {
-        const int key0 = (it.unit + u) * kUnit, key = key0 + half * 128 + row;
-        int first, last;
-        q_tiles(p, it, key0, first, last);
-        if (key0 + half * 128 >= it.kv_len) last = first;
-        // the columns, from the sequence's first row on, that see this token
-        const int seen0 = a.causal ? max(0, key - it.pos0) * p.groups : 0;
-        int seen1 = it.q_len;
-        if (a.window > 0)
-          seen1 = (int)min((long long)seen1, max(0ll, (long long)key + a.window - it.pos0));
-        seen1 *= p.groups;
-        const uint32_t slot = tokens % kTokenWarps;
-        float sum = 0.f;
-#pragma unroll 1
-        for (int q = first; q < last && ok; ++q, ++count) {
-          const Tile tile{it.seq, it.head, q};
-          if (!have.is(tile)) {
-            if (!coming.is(tile)) load_rows(tile, it);
-            publish_rows();
-          }
-          // the rows of what comes after this tile
-          if (q + 1 < last) {
-            load_rows(Tile{tile.seq, tile.head, q + 1}, it);
-          } else if (u + 1 == it.units && items.ready()) {
-            const Item& then = ctl->items[items.n % kItems];
-            int q0, q1;
-            q_tiles(p, then, then.unit * kUnit, q0, q1);
-            if (then.seq >= 0 && q0 < q1) load_rows(Tile{then.seq, then.head, q0}, then);
-          }
-          const int col0 = q * rows;
-          const int buf = (int)(count & 1u);
-          ok = wait_warp(&ctl->s_full[half * 2 + buf], count >> 1 & 1u, ctl);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t ts = lane_addr + buf * 128;
-          // of the tile's columns
-          const int lo = max(0, seen0 - col0), hi = min(rows, seen1 - col0);
-          const bool masked = __any_sync(0xffffffffu, lo > 0 || hi < p.nq);
-          auto release = [&]() {  // all of the tile is in registers
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&ctl->s_empty[half * 2 + buf]);
-          };
-          float part = 0.f;
-          if (p.nq == 16) {
-            uint32_t s[16], fine[16];
-            tmem_load(ts, s);
-            if (Q8) tmem_load(ts + 16, fine);
-            tmem_wait(s);
-            tie(fine);
-            release();
-            part = weigh<Q8, true, 16>(s, fine, p.scale_log2, key_scale(slot), mine, mine + 64, 0, lo, hi);
-          } else {
-            uint32_t s[2][kCols], fine[2][Q8 ? kCols : 1];
-            auto load = [&](int c, int b) {
-              tmem_load(ts + c, s[b]);
-              if constexpr (Q8) tmem_load(ts + p.nq + c, fine[b]);
-            };
-            const float key = key_scale(slot);
-            load(0, 0);
-#pragma unroll 1
-            for (int c0 = 0; c0 < p.nq; c0 += 2 * kCols) {
-#pragma unroll
-              for (int b = 0; b < 2; ++b) {
-                const int c = c0 + b * kCols;
-                if (c >= p.nq) break;
-                tmem_wait(s[b]);
-                if constexpr (Q8) tie(fine[b]);
-                if (c + kCols < p.nq)
-                  load(c + kCols, b ^ 1);
-                else
-                  release();
-                const auto& rest = [&]() -> const uint32_t(&)[kCols] {
-                  if constexpr (Q8)
-                    return fine[b];
-                  else
-                    return s[b];
-                }();
-                part += masked ? weigh<Q8, true, kCols>(s[b], rest, p.scale_log2, key, mine, mine + 64,
-                                                        c, lo, hi)
-                               : weigh<Q8, false, kCols>(s[b], rest, p.scale_log2, key, mine, mine + 64,
-                                                         c, lo, hi);
-              }
-            }
-          }
-          sum += part;
+      for (int q = it.first; q < it.last && ok; ++q, ++count) {
+        const Tile tile{it.seq, it.head, q};
+        if (!have.is(tile)) {
+          if (!coming.is(tile)) load_rows(tile, it);
+          publish_rows();
         }
-        ok = ok && tokens_ready(slot);
+        // the rows of what comes after this tile
+        if (q + 1 < it.last) {
+          load_rows(Tile{tile.seq, tile.head, q + 1}, it);
+        } else if (items.ready()) {
+          const Item& then = ctl->items[items.n % kItems];
+          if (then.seq >= 0 && then.first < then.last)
+            load_rows(Tile{then.seq, then.head, then.first}, then);
+        }
+        const int col0 = q * rows;
+        const int buf = (int)(count & 1u);
+        ok = wait_warp(&ctl->s_full[half * 2 + buf], count >> 1 & 1u, ctl);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t ts = lane_addr + buf * 128;
+        // of the tile's columns
+        const int lo = max(0, seen0 - col0), hi = min(rows, seen1 - col0);
+        const bool masked = __any_sync(0xffffffffu, lo > 0 || hi < p.nq);
+        auto release = [&]() {  // this warp has read its columns
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&ctl->s_empty[half * 2 + buf]);
+        };
+        float part = 0.f;
+#pragma unroll 1
+        for (int c0 = 32 * odd; c0 < p.nq; c0 += 64) {
+          uint32_t s[32], fine[Q8 ? 32 : 1];
+          tmem_ld32_nowait(ts + c0, s);
+          if constexpr (Q8) tmem_ld32_nowait(ts + p.nq + c0, fine);
+          tmem_ld_wait();
+          tie32(s);
+          if constexpr (Q8) tie32(fine);
+          if (c0 + 64 >= p.nq) release();
+          if (masked) hide(s, lo - c0, hi - c0, hidden);
+          part += weigh<Q8>(s, fine, p.scale_log2, key_scale, mine + c0 / 64 * 32, mine + 64);
+        }
+        if (32 * odd >= p.nq) release();  // (no column of the tile)
+        sum += part;
+      }
+      // the odd columns' sums to the warps of the even ones
+      const uint32_t pass = half * 2 + (tokens & 1u), phase = tokens >> 1 & 1u;
+      float* mid = odd_sh + pass * 128 + row;
+      if (odd) {
+        ok = ok && wait_warp(&ctl->odd_empty[pass], phase ^ 1u, ctl);
+        if (!ok) break;
+        *mid = sum;
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&ctl->odd_full[pass]);
+          mbar_arrive(&ctl->token_empty[slot]);
+        }
+      } else {
+        ok = ok && wait_warp(&ctl->token_full[slot], tokens / kTokens & 1u, ctl) &&
+             wait_warp(&ctl->odd_full[pass], phase, ctl);
         if (!ok) break;
         const Token token = token_sh[slot * 128 + row];
+        sum += *mid;
         __syncwarp();
-        if (lane == 0) mbar_arrive(&ctl->token_empty[slot]);
+        if (lane == 0) {
+          mbar_arrive(&ctl->odd_empty[pass]);
+          mbar_arrive(&ctl->token_empty[slot]);
+        }
         if (token.out_at >= 0) p.scores_out[token.out_at] = token.old + sum;
       }
+      ++tokens;
     }
   } else if (warp == kQWarp) {
     // --------------------------------------------- the items, and their Q tiles
@@ -671,17 +603,17 @@ __global__ void __launch_bounds__(threads<TMA>(), 1)
         }
         long long x = i - base_sh[lo];
         int s = lo * per;
-        long long mine = runs(s) * a.c.heads;
+        long long mine = units(s) * a.c.heads;
         while (x >= mine) {
           x -= mine;
-          mine = runs(++s) * a.c.heads;
+          mine = units(++s) * a.c.heads;
         }
         const SeqLens q = seq_lens(a, s);
         it.seq = s;
         it.head = (int)(x % a.c.heads);
-        it.unit = (int)(x / a.c.heads) * p.run;
-        it.units = min(p.run, (q.kv_len + kUnit - 1) / kUnit - it.unit);
+        it.key0 = (int)(x / a.c.heads) * kUnit;
         it.q0 = q.q0, it.q_len = q.q_len, it.pos0 = q.pos0, it.kv_len = q.kv_len;
+        q_tiles(p, it);
       }
       const uint32_t slot = n % kItems;
       ok = wait_warp(&ctl->item_empty[slot], (n / kItems & 1u) ^ 1u, ctl);
@@ -691,246 +623,181 @@ __global__ void __launch_bounds__(threads<TMA>(), 1)
         mbar_arrive(&ctl->item_full[slot]);
       }
       if (it.seq < 0) break;
-      const int tiles = (it.q_len + p.tile_tokens - 1) / p.tile_tokens;
-      if (tiles == 1) {  // one tile serves all of the item's units
-        load(it, 0);
-      } else {
-        for (int u = 0; u < it.units && ok; ++u) {
-          int first, last;
-          q_tiles(p, it, (it.unit + u) * kUnit, first, last);
-          for (int q = first; q < last && ok; ++q) load(it, q);
-        }
-      }
-      if (lane == 0 && ok) i = gridDim.x + (long long)atomicAdd(p.next, 1);
-      i = __shfl_sync(0xffffffffu, i, 0);
+      // (an item of few tiles is over soon: its successor is asked for ahead)
+      const bool soon = it.last - it.first <= kMaxQ;
+      long long then = 0;
+      if (soon && lane == 0) then = gridDim.x + (long long)atomicAdd(p.next, 1);
+      for (int q = it.first; q < it.last && ok; ++q) load(it, q);
+      if (!soon && lane == 0 && ok) then = gridDim.x + (long long)atomicAdd(p.next, 1);
+      i = __shfl_sync(0xffffffffu, then, 0);
     }
-  } else if (warp == kMmaWarp) {
-    // -------------------------------------------------------------- products
-    Items items{ctl};
-    Item it;
-    uint32_t key_n = 0, q_n = 0, count[2] = {0, 0};
-    bool ok = true;
-    const uint32_t type = Q8 ? 0u : p.f16 ? 0u : 1u;
-    const uint32_t id_all = instr_desc(type, Q8 ? 2 * p.nq : p.nq), id_one = instr_desc(type, p.nq);
-    const int steps = p.row_bytes / 32;
-    while (ok && items.next(it, lane)) {
-      const int tiles = (it.q_len + p.tile_tokens - 1) / p.tile_tokens;
-      const bool hold = tiles == 1;
-      if (hold) ok = wait_warp(&ctl->q_full[q_n % p.q_stages], q_n / p.q_stages & 1u, ctl);
-      for (int u = 0; u < it.units && ok; ++u) {
-        const int key0 = (it.unit + u) * kUnit;
-        int first, last;
-        q_tiles(p, it, key0, first, last);
-        if (first == last) continue;
-        const int halves = key0 + 128 < it.kv_len ? 2 : 1;
-        for (int h = 0; h < halves && ok; ++h)
-          ok = wait_warp(&ctl->key_full[(key_n + h) % p.key_stages],
-                         (key_n + h) / p.key_stages & 1u, ctl);
-        if (!TMA) fence_async_smem();
-        for (int q = first; q < last && ok; ++q) {
-          const uint32_t qs = q_n % p.q_stages;
-          if (!hold) ok = wait_warp(&ctl->q_full[qs], q_n / p.q_stages & 1u, ctl);
-          for (int h = 0; h < halves && ok; ++h) {
-            const uint32_t buf = count[h] & 1u;
-            ok = wait_warp(&ctl->s_empty[h * 2 + buf], (count[h] >> 1 & 1u) ^ 1u, ctl);
-            if (!ok) break;
-            ++count[h];
-            tc_fence_after();
-            if (elect_one()) {
-              const uint32_t d = tmem + h * 256 + buf * 128;
-              const uint32_t ka = keys_at + (key_n + h) % p.key_stages * p.key_bytes;
-              const uint32_t qa = q_at + qs * p.q_bytes;
-              const int terms = Q8 ? p.terms : 1;
-#pragma unroll 1
-              for (int sl = 0; sl < p.slices; ++sl) {
-                const uint64_t kd = operand_desc(ka + sl * 128 * p.row_bytes, p.row_bytes);
-                const uint64_t qd = operand_desc(qa + sl * terms * p.nq * p.row_bytes, p.row_bytes);
-#pragma unroll 2
-                for (int kk = 0; kk < steps; ++kk)
-                  mma_ss<Q8>(d, kd + 2 * kk, qd + 2 * kk, id_all, sl + kk > 0);
-              }
-              if (Q8 && terms == 3)
-#pragma unroll 1
-                for (int sl = 0; sl < p.slices; ++sl) {
-                  const uint64_t kd = operand_desc(ka + sl * 128 * p.row_bytes, p.row_bytes);
-                  const uint64_t qd =
-                      operand_desc(qa + (sl * terms + 2) * p.nq * p.row_bytes, p.row_bytes);
-                  for (int kk = 0; kk < steps; ++kk)
-                    mma_ss<Q8>(d + p.nq, kd + 2 * kk, qd + 2 * kk, id_one, 1u);
-                }
-              mma_commit(&ctl->s_full[h * 2 + buf]);
-              if (!hold && h == halves - 1) mma_commit(&ctl->q_empty[qs]);
-              if (q == last - 1) mma_commit(&ctl->key_empty[(key_n + h) % p.key_stages]);
-            }
-            __syncwarp();
-          }
-          if (!hold) ++q_n;
-        }
-        key_n += halves;
-      }
-      if (hold) {
-        if (ok && elect_one()) mma_commit(&ctl->q_empty[q_n % p.q_stages]);
-        __syncwarp();
-        ++q_n;
-      }
-    }
-    // Everything issued has finished before the block gives its memories back.
+  } else if (warp == kMmaWarp || warp == kMmaWarp + 1) {
+    // ------------------------------------------------- products of a half, one thread
+    const int half = warp - kMmaWarp;
     if (elect_one()) {
-      mma_commit(&ctl->drained);
-      if (!mbar_wait(&ctl->drained, 0, static_cast<int*>(nullptr))) ctl->abort = 1;
+      Items items{ctl};
+      Item it;
+      uint32_t key_n = half, q_n = 0, count = 0;  // K stage, Q tiles, S tiles
+      bool ok = true;
+      const uint32_t type = Q8 ? 0u : p.f16 ? 0u : 1u;
+      const uint32_t id_all = instr_desc(type, Q8 ? 2 * p.nq : p.nq), id_one = instr_desc(type, p.nq);
+      const uint32_t k_desc = desc_lo(keys_at), q_desc = desc_lo(q_at);
+      const uint32_t q_slice = p.nq * p.row_bytes * (Q8 ? p.terms : 1) >> 4;
+      while (ok && items.next_alone(it)) {
+        if (it.first == it.last) continue;
+        const bool two = it.key0 + 128 < it.kv_len, mine = half == 0 || two;
+        const uint32_t ks = key_n % p.key_stages, ka = k_desc + (ks * p.key_bytes >> 4);
+        if (mine) {
+          ok = wait_one(&ctl->key_full[ks], key_n / p.key_stages & 1u, ctl);
+          if (!TMA) fence_async_smem();
+        }
+#pragma unroll 1
+        for (int q = it.first; q < it.last && ok; ++q, ++q_n) {
+          const uint32_t qs = q_n % p.q_stages;
+          ok = wait_one(&ctl->q_full[qs], q_n / p.q_stages & 1u, ctl);
+          if (!ok) break;
+          if (!mine) {
+            mbar_arrive(&ctl->q_empty[qs]);
+            continue;
+          }
+          const uint32_t buf = count & 1u;
+          ok = wait_one(&ctl->s_empty[half * 2 + buf], (count >> 1 & 1u) ^ 1u, ctl);
+          if (!ok) break;
+          ++count;
+          tc_fence_after();
+          const uint32_t d = tmem + half * 256 + buf * 128, qa = q_desc + (qs * p.q_bytes >> 4);
+          mma_tile<Q8>(p, d, ka, qa, q_slice, id_all, 0u);
+          if (Q8 && p.terms == 3)
+            mma_tile<Q8>(p, d + p.nq, ka, qa + (2 * p.nq * p.row_bytes >> 4), q_slice, id_one, 1u);
+          mma_commit(&ctl->s_full[half * 2 + buf]);
+          mma_commit(&ctl->q_empty[qs]);
+        }
+        if (ok && mine) mma_commit(&ctl->key_empty[ks]);
+        key_n += two ? 2 : 1;
+      }
+      // Everything issued has finished before the block gives its memories back.
+      mma_commit(&ctl->drained[half]);
+      if (!mbar_wait(&ctl->drained[half], 0, static_cast<int*>(nullptr))) ctl->abort = 1;
     }
     __syncwarp();
-  } else if (warp < kKeyWarp) {
+  } else if (warp == kTokenWarp || warp == kTokenWarp + 1) {
     // ------------------------------------------------------------- the tokens
-    // Warp w takes the tiles w, w + 4, ... of 128 tokens, two tiles a unit.
-    const uint32_t part = warp - kTokenWarp;
+    const int half = warp - kTokenWarp;
     Items items{ctl};
     Item it;
-    uint32_t tiles = 0, used = 0;  // so far, and of them with keys that some row needs
+    uint32_t tokens = 0, used = 0;  // items, and K tiles that some row needs, so far
     bool ok = true;
     constexpr int kElem = Q8 ? 1 : 2;
     while (ok && items.next(it, lane)) {
-#pragma unroll 1
-      for (int t = 0; t < 2 * it.units && ok; ++t, ++tiles) {
-        const int key0 = it.unit * kUnit + 128 * t;
-        int first, last;
-        q_tiles(p, it, key0 & ~(kUnit - 1), first, last);
-        const bool seen = first < last && key0 < it.kv_len;
-        const uint32_t stage = used % p.key_stages, stage_phase = used / p.key_stages & 1u;
-        used += seen;
-        if (tiles % kTokenWarps != part) continue;
-        int page[4], at[4];
+      const int key0 = it.key0 + 128 * half;
+      const bool seen = it.first < it.last && key0 < it.kv_len;
+      const uint32_t tile = used + half;  // (a first half always has tokens)
+      if (it.first < it.last) used += it.key0 + 128 < it.kv_len ? 2 : 1;
+      int page[4], at[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int key = key0 + lane + 32 * k, i = p.page_of(key);
-          at[k] = key - i * a.c.page_size;
-          page[k] = key < it.kv_len ? __ldg(a.table + it.seq * a.table_stride + i) : -2;
-        }
-        float old[4];
-        uint32_t scale[4];
-        long long out_at[4];
+      for (int k = 0; k < 4; ++k) {
+        const int key = key0 + lane + 32 * k, i = p.page_of(key);
+        at[k] = key - i * a.c.page_size;
+        page[k] = key < it.kv_len ? __ldg(a.table + it.seq * a.table_stride + i) : -2;
+      }
+      float old[4];
+      uint32_t scale[4];
+      long long out_at[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const bool good = page[k] >= 0 && page[k] < a.c.num_pages;
-          if (!good && page[k] != -2) atomicOr(&ctl->errors, kDevBadPage);
-          const bool fresh = a.causal && key0 + lane + 32 * k >= it.pos0;
-          old[k] = 0.f;
-          if (good && !fresh)
-            old[k] = p.scores_in[page[k] * p.in_page + at[k] * p.in_token + it.head * p.in_head];
-          scale[k] = 0;
-          if (Q8 && good && seen)
-            scale[k] = __ldg(a.c.k_scale + page[k] * a.c.scale_page_stride +
-                             at[k] * a.c.scale_token_stride + it.head * a.c.scale_head_stride);
-          // (in place, what no row sees stays as it is)
-          out_at[k] = good && (fresh || seen || p.scores_in != p.scores_out)
-                          ? page[k] * p.out_page + at[k] * p.out_token + it.head * p.out_head
-                          : -1;
-        }
-        ok = wait_warp(&ctl->token_empty[part], (tiles / kTokenWarps & 1u) ^ 1u, ctl);
+      for (int k = 0; k < 4; ++k) {
+        const bool good = page[k] >= 0 && page[k] < a.c.num_pages;
+        if (!good && page[k] != -2) atomicOr(&ctl->errors, kDevBadPage);
+        const bool fresh = a.causal && key0 + lane + 32 * k >= it.pos0;
+        old[k] = 0.f;
+        if (good && !fresh)
+          old[k] = p.scores_in[page[k] * p.in_page + at[k] * p.in_token + it.head * p.in_head];
+        scale[k] = 0;
+        if (Q8 && good && seen)
+          scale[k] = __ldg(a.c.k_scale + page[k] * a.c.scale_page_stride +
+                           at[k] * a.c.scale_token_stride + it.head * a.c.scale_head_stride);
+        // (in place, what no row sees stays as it is)
+        out_at[k] = good && (fresh || seen || p.scores_in != p.scores_out)
+                        ? page[k] * p.out_page + at[k] * p.out_token + it.head * p.out_head
+                        : -1;
+      }
+      const uint32_t slot = half * kTokens + tokens % kTokens;
+      ok = wait_warp(&ctl->token_empty[slot], (tokens / kTokens & 1u) ^ 1u, ctl);
+      if (!ok) break;
+      ++tokens;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        Token to;
+        to.old = old[k];
+        to.key_scale = scale[k] == 255u ? __int_as_float(0x7fc00000) : __uint_as_float(scale[k] << 23);
+        to.out_at = out_at[k];
+        token_sh[slot * 128 + lane + 32 * k] = to;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctl->token_full[slot]);
+      if (!TMA && seen) {
+        // the tile's keys, 16 bytes a lane, the pieces of a row by neighbouring lanes
+        const uint32_t stage = tile % p.key_stages;
+        ok = wait_warp(&ctl->key_empty[stage], (tile / p.key_stages & 1u) ^ 1u, ctl);
         if (!ok) break;
+        const int chunks = a.c.head_dim * kElem / 16, per_pass = 32 / chunks;
+        const int slice_chunks = p.row_bytes / 16, chunk = lane % chunks;
+        const int sl = chunk / slice_chunks, c = chunk % slice_chunks;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          Token to;
-          to.old = old[k];
-          to.key_scale = scale[k] == 255u ? __int_as_float(0x7fc00000) : __uint_as_float(scale[k] << 23);
-          to.out_at = out_at[k];
-          token_sh[part * 128 + lane + 32 * k] = to;
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&ctl->token_full[part]);
-        if (!TMA && seen) {
-          // the tile's keys, 16 bytes a lane, chunks of a row by neighbouring lanes
-          ok = wait_warp(&ctl->key_empty[stage], stage_phase ^ 1u, ctl);
-          if (!ok) break;
-          const int chunks = a.c.head_dim * kElem / 16, per_pass = 32 / chunks;
-          const int slice_chunks = p.row_bytes / 16, chunk = lane % chunks;
-          const int sl = chunk / slice_chunks, c = chunk % slice_chunks;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const long long off =
-                page[k] >= 0 && page[k] < a.c.num_pages
-                    ? (page[k] * a.c.page_stride + at[k] * a.c.token_stride +
-                       it.head * a.c.head_stride) * kElem
-                    : -1;
+          const long long off = page[k] >= 0 && page[k] < a.c.num_pages
+                                    ? (page[k] * a.c.page_stride + at[k] * a.c.token_stride +
+                                       it.head * a.c.head_stride) * kElem
+                                    : -1;
 #pragma unroll 4
-            for (int j = 0; j < chunks; ++j) {
-              const int r32 = j * per_pass + lane / chunks, r = 32 * k + r32;
-              const long long o = __shfl_sync(0xffffffffu, off, r32);
-              const uint32_t x = (uint32_t)c ^ (p.row_bytes == 128 ? r & 7 : r >> 1 & 3);
-              if (o >= 0)
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
-                                 keys_at + stage * p.key_bytes + (sl * 128 + r) * p.row_bytes + x * 16),
-                             "l"(static_cast<const uint8_t*>(a.c.k) + o + chunk * 16)
-                             : "memory");
-            }
+          for (int j = 0; j < chunks; ++j) {
+            const int r32 = j * per_pass + lane / chunks, r = 32 * k + r32;
+            const long long o = __shfl_sync(0xffffffffu, off, r32);
+            const uint32_t x = (uint32_t)c ^ (p.row_bytes == 128 ? r & 7 : r >> 1 & 3);
+            if (o >= 0)
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                               keys_at + stage * p.key_bytes + (sl * 128 + r) * p.row_bytes + x * 16),
+                           "l"(static_cast<const uint8_t*>(a.c.k) + o + chunk * 16)
+                           : "memory");
           }
-          cp_async_arrive_noinc(&ctl->key_full[stage]);
         }
+        cp_async_arrive_noinc(&ctl->key_full[stage]);
       }
     }
     if (!TMA) asm volatile("cp.async.wait_all;" ::: "memory");
-  } else {
+  } else if (TMA && warp == kKeyWarp) {
     // --------------------------------------------------------------- K tiles
-    // A lane per box of a page's tokens. Page numbers come to shared memory by
-    // asynchronous copies, for up to kPages tiles ahead.
-    KeyTiles tiles;
-    tiles.items.ctl = ctl;
-    KeyTile held[kPages];  // [0] is the next one to copy
-    int n = 0;             // of them
-    uint32_t slot = 0;     // of held[0]'s page numbers
+    // A lane per box of a page's tokens: lanes 0-15 of the first half, 16-31 of the
+    // second.
+    Items items{ctl};
+    Item it;
     bool ok = true;
-    const int boxes = 128 / p.box_rows;
-    auto token_of = [&](const KeyTile& t) { return t.key0 + lane * p.box_rows; };
-    while (ok) {
-      KeyTile t;
-      const bool more = n < kPages && tiles.next(p, lane, n == 0, t);
-      if (more) {
-        const int token = token_of(t);
-        if (lane < boxes && token < t.kv_len)
-          cp_async_4(&ctl->pages[(slot + n) % kPages][lane],
-                     a.table + t.seq * a.table_stride + p.page_of(token));
-#pragma unroll
-        for (int i = 0; i < kPages; ++i)
-          if (i == n) held[i] = t;
-        ++n;
-      }
-      // (a group a turn: when a tile is copied, all but the last kPages - 1 have landed)
-      asm volatile("cp.async.commit_group;" ::: "memory");
-      if (n == 0) break;
-      if (more && n < kPages) continue;
-      // (its turn came kPages - 1 turns ago, or nothing more is known)
-      if (more)
-        asm volatile("cp.async.wait_group %0;" ::"n"(kPages - 1) : "memory");
-      else
-        asm volatile("cp.async.wait_all;" ::: "memory");
-      const uint32_t s = keys_copied % p.key_stages;
-      ok = wait_warp(&ctl->key_empty[s], (keys_copied / p.key_stages & 1u) ^ 1u, ctl);
-      if (!ok) break;
-      if (lane == 0) mbar_arrive_expect_tx(&ctl->key_full[s], p.key_bytes);
-      __syncwarp();
-      ++keys_copied;
-      const int token = token_of(held[0]);
-      if (lane < boxes) {
-        int from = token < held[0].kv_len
-                       ? *reinterpret_cast<volatile int*>(&ctl->pages[slot % kPages][lane])
-                       : -1;
-        int at = token - p.page_of(token) * a.c.page_size;
-        // past the last token, or no page of the cache: from past the map's end
-        if (from < 0 || from >= a.c.num_pages) from = (int)a.c.num_pages, at = 0;
-        const int per_slice = p.row_bytes / (Q8 ? 1 : 2);
+    const int boxes = 128 / p.box_rows, half = lane >> 4, box = lane & 15;
+    while (ok && items.next(it, lane)) {
+      if (it.first == it.last) continue;
+      const int token = it.key0 + half * 128 + box * p.box_rows, i = p.page_of(token);
+      int page = box < boxes && token < it.kv_len ? __ldg(a.table + it.seq * a.table_stride + i) : -1;
+      int at = token - i * a.c.page_size;
+      // past the last token, or no page of the cache: from past the map's end
+      if (page < 0 || page >= a.c.num_pages) page = (int)a.c.num_pages, at = 0;
+      const int halves = it.key0 + 128 < it.kv_len ? 2 : 1;
+      for (int h = 0; h < halves && ok; ++h) {
+        const uint32_t s = keys_copied % p.key_stages;
+        ok = wait_warp(&ctl->key_empty[s], (keys_copied / p.key_stages & 1u) ^ 1u, ctl);
+        if (!ok) break;
+        if (lane == 0) mbar_arrive_expect_tx(&ctl->key_full[s], p.key_bytes);
+        __syncwarp();
+        ++keys_copied;
+        if (half == h && box < boxes) {
+          const int per_slice = p.row_bytes / (Q8 ? 1 : 2);
 #pragma unroll 1
-        for (int sl = 0; sl < p.slices; ++sl)
-          tma_load_4d(keys_at + s * p.key_bytes + (sl * 128 + lane * p.box_rows) * p.row_bytes, &k_map,
-                      sl * per_slice, p.heads_first ? held[0].head : at,
-                      p.heads_first ? at : held[0].head, from, &ctl->key_full[s]);
+          for (int sl = 0; sl < p.slices; ++sl)
+            tma_load_4d(keys_at + s * p.key_bytes + (sl * 128 + box * p.box_rows) * p.row_bytes, &k_map,
+                        sl * per_slice, p.heads_first ? it.head : at, p.heads_first ? at : it.head, page,
+                        &ctl->key_full[s]);
+        }
+        __syncwarp();
       }
-      __syncwarp();
-#pragma unroll
-      for (int i = 0; i + 1 < kPages; ++i) held[i] = held[i + 1];
-      --n;
-      ++slot;
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
   }
 
   tc_fence_before();
@@ -1021,7 +888,7 @@ cudaError_t launch(const ScoreParams& p, size_t smem, const CUtensorMap& q_map,
     configured[dev] = true;
   }
   return launch_pdl(kv_scores_kernel<Q8, TMA>, dim3((unsigned)device_sm_count()),
-                    dim3(threads<TMA>()), smem, stream, p, q_map, k_map);
+                    dim3(kThreads), smem, stream, p, q_map, k_map);
 }
 
 }  // namespace
@@ -1044,7 +911,7 @@ cudaError_t launch_kv_scores(const ScoresLaunch& l, cudaStream_t stream) {
   p.in_page = l.in_page, p.in_token = l.in_token, p.in_head = l.in_head;
   p.out_page = l.out_page, p.out_token = l.out_token, p.out_head = l.out_head;
   p.groups = a.q_heads / a.c.heads;
-  p.scale_log2 = a.scale * kLog2e;
+  p.scale_log2 = a.scale == 0.f ? kMinScale : a.scale * kLog2e;
   p.f16 = a.cache_dtype == 1;
   p.terms = a.q_f16 ? 3 : 2;
   p.row_bytes = q8 && d == 64 ? 64 : 128;
@@ -1055,7 +922,7 @@ cudaError_t launch_kv_scores(const ScoresLaunch& l, cudaStream_t stream) {
   // or vectors of 512 bytes).
   const int most = q8 || d == 256 ? 64 : 128;
   const long long rows = (long long)a.max_q * p.groups;
-  p.nq = 16;
+  p.nq = 32;
   while (p.nq < most && p.nq < rows) p.nq *= 2;
   p.tile_tokens = p.nq / p.groups;
   p.by_tile = divisor(p.tile_tokens);
@@ -1068,13 +935,6 @@ cudaError_t launch_kv_scores(const ScoresLaunch& l, cudaStream_t stream) {
   p.key_stages = std::min(kMaxKeys, (kRoom - p.q_stages * p.q_bytes) / p.key_bytes);
   const size_t smem = (size_t)p.key_stages * p.key_bytes + p.q_stages * p.q_bytes + kControl;
   const long long sms = device_sm_count();
-  // Where one Q tile serves a sequence an item takes several units, as long as
-  // there are eight items a block.
-  const long long cap = ((long long)a.table_width * a.c.page_size + kUnit - 1) / kUnit;
-  p.run = 1;
-  if (a.max_q <= p.tile_tokens)
-    while (p.run < 8 && cap * a.seqs * a.c.heads / (2 * p.run) >= 8 * sms) p.run *= 2;
-
   const void* q = a.q;
   long long head_stride = a.q_head_stride, token_stride = a.q_token_stride, q_rows = a.q_tokens;
   CUtensorMapDataType type = a.q_f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
