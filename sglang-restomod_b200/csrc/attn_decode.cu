@@ -271,7 +271,12 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
     }
     fence_mbar_init();
   }
-  griddep_wait();
+  // (beside another kernel of the call: that one is waited for at the end)
+  if (!a.beside) griddep_wait();
+  auto leave = [&]() {
+    if (a.beside) griddep_wait();
+    griddep_launch_dependents();
+  };
 
   // ---- this block's range of the flattened (sequence, head, cost) space: a
   // pair's first kPairCost places stand for its constant cost, the others for a
@@ -308,11 +313,11 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
       total += sm.scan[w];
       pairs += sm.scan_pairs[w];
     }
-    if (total == 0) return;
+    if (total == 0) return leave();
     long long n = (total + kMinTiles - 1) / kMinTiles;
     n = min(n, min(pairs * kMaxParts, (long long)gridDim.x));
     ctas = (int)n;
-    if (blockIdx.x >= ctas) return;
+    if (blockIdx.x >= ctas) return leave();
     const long long t0 = total * blockIdx.x / ctas;
     if (t0 >= before && t0 < before + mine) {
       int s = s0;
@@ -513,8 +518,7 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
       }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
-    griddep_launch_dependents();
-    return;
+    return leave();
   }
 
   // The scale bytes of token lane % 16 of this warp's part of tile `slot`: 0
@@ -1102,7 +1106,7 @@ __global__ void __launch_bounds__(Shape<D, KV, NR, TMA>::kThreads, Shape<D, KV, 
       mbar_arrive(&sm.q_empty[buf]);
     }
   }
-  griddep_launch_dependents();
+  leave();
 }
 
 template <int D, int KV, int NR, bool TMA>

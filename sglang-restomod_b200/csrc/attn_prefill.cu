@@ -105,6 +105,7 @@ struct PrefillParams {
   int4* units;      // sequence, first token in it, first key, key tiles
   long long* unit_at;  // place of each unit's first cost (nullptr: not wanted)
   int max_units;
+  int plan_only, planned;  // (host) launch the plan alone, or all but it
   float* parts;
   // tensor copies: rows of a page that one copy takes (a power of two that
   // divides the page size), and whether heads come before tokens in the map
@@ -410,8 +411,10 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const PrefillPa
   __shared__ long long at_sh[kPlanThreads];
   // (each step of the search below reads it: from global memory 1 us a step)
   int* seq_base = p.a.seqs <= kPlanSeqs ? base_sh : p.seq_base;
-  griddep_wait();
   const AttnLaunch& a = p.a;
+  // (see AttnLaunch::beside)
+  if (!a.beside) griddep_wait();
+  if (p.unit_at != nullptr) griddep_launch_dependents();
   const int tid = threadIdx.x;
   long long total_units, total;
   {
@@ -491,6 +494,7 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const PrefillPa
     const int h = (int)(x / cost);
     p.start[c] = make_int4(u, h, (int)(x - (long long)h * cost), 0);
   }
+  if (a.beside) griddep_wait();
   griddep_launch_dependents();
 }
 
@@ -769,10 +773,11 @@ __global__ void __launch_bounds__(128) attn_combine_kernel(const PrefillParams p
 // Where sequences share prefixes: for each row the parts of the pass over its
 // group's prefix (or the row that one block finished) and the row of the pass over
 // its sequence's own tokens, added as attn_combine_kernel adds parts. A finished row
-// is a part with m = lse and l = 1. Rows that the own pass left alone (past max_q, or
-// of no sequence) keep their mark and are left alone here. Threads as there; a block
-// goes through the (unit, head) pairs.
+// is a part with m = lse and l = 1. Rows that the own pass left alone (past max_q) are
+// left alone here. Threads as there; a block goes through the (unit, head) pairs.
 struct PrefixEnds {
+  const int* q_starts;  // of the sequences
+  int seqs, max_q;
   const float* own_out;  // fp32 [q_tokens][q_heads][d]
   const float* own_lse;
   void* out;
@@ -785,6 +790,11 @@ __global__ void __launch_bounds__(128) attn_prefix_finish_kernel(const PrefillPa
   const long long total = __ldcg(p.head), ctas = __ldcg(p.head + 1), units = __ldcg(p.head + 2);
   const int groups = d / kCombineCols, tile = blockIdx.y / groups;
   const int col = blockIdx.y % groups * kCombineCols, row = threadIdx.x;
+  constexpr int kStarts = 4096;
+  __shared__ int starts_sh[kStarts];
+  for (int i = threadIdx.x; i < min(e.seqs, kStarts); i += 128) starts_sh[i] = __ldg(e.q_starts + i);
+  __syncthreads();
+  auto start = [&](int s) { return e.seqs <= kStarts ? starts_sh[s] : __ldg(e.q_starts + s); };
   for (long long pair = blockIdx.x; pair < units * a.c.heads; pair += gridDim.x) {
     const int unit = (int)(pair / a.c.heads), head = (int)(pair % a.c.heads);
     const int4 u = __ldcg(p.units + unit);
@@ -794,8 +804,16 @@ __global__ void __launch_bounds__(128) attn_prefix_finish_kernel(const PrefillPa
     const long long token = (long long)q.q0 + tok;
     const int qh = head * p.groups + row % p.groups;
     const long long at_row = token * a.q_heads + qh;
+    int lo = 0, hi = e.seqs - 1;  // the row's sequence: the last that starts at or before it
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (start(mid) <= token)
+        lo = mid;
+      else
+        hi = mid - 1;
+    }
+    if (token - start(lo) >= e.max_q) continue;
     const float own = __ldcg(e.own_lse + at_row);
-    if (__float_as_uint(own) == kNoRow) continue;
     float m = -INFINITY, l = 0.f, acc[kCombineCols];
 #pragma unroll
     for (int i = 0; i < kCombineCols; ++i) acc[i] = 0.f;
@@ -1020,8 +1038,6 @@ __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
       const bool whole = g.tiles == g.unit_tiles;
       const long long token = (long long)q.q0 + tok;
       const int qh = g.head * p.groups + row_head;
-      if (a.mark != nullptr && valid)
-        a.mark[token * a.q_heads + qh] = __uint_as_float(kNoRow);
       // 64 bytes of the warp's 32 rows (32 columns, or 16 in fp32), through shared
       // memory so that a store covers 64 neighbouring bytes of each of 8 rows
       const bool wide = a.out32 != nullptr;
@@ -1600,9 +1616,12 @@ cudaError_t launch(const PrefillParams& p, const CUtensorMap (&maps)[3], cudaStr
   static_assert(S::kSmem <= 227 * 1024 && S::kStages >= 4, "shared memory");
   static_assert(sizeof(Ctl) <= 4096, "control block");
   const int sms = device_sm_count();
-  err = launch_pdl(attn_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, p,
-                   MT * p.tile_tokens, S::kBN, sms);
-  if (err != cudaSuccess) return err;
+  if (!p.planned) {
+    err = launch_pdl(attn_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, p,
+                     MT * p.tile_tokens, S::kBN, sms);
+    if (err != cudaSuccess) return err;
+  }
+  if (p.plan_only) return cudaSuccess;
   err = launch_pdl(attn_prefill_kernel<D, MT, KV, TMA>, dim3((unsigned)sms), dim3(S::kThreads),
                    S::kSmem, stream, p, maps[0], maps[1], maps[2]);
   if (err != cudaSuccess || p.unit_at != nullptr) return err;  // (its parts are added later)
@@ -1735,20 +1754,26 @@ cudaError_t launch_attn_prefix(AttnLaunch prefix, AttnLaunch own, cudaStream_t s
   take(attn_prefill_scratch_bytes(d, prefix.q_tokens, prefix.seqs));
   long long* unit_at = reinterpret_cast<long long*>(take(8 * max_units(prefix.q_tokens, prefix.seqs)));
   own.scratch = take(attn_scratch_bytes(d, own.q_tokens, own.seqs));
-  const PrefixEnds ends{reinterpret_cast<float*>(take(4 * rows * d)),
-                        reinterpret_cast<float*>(take(4 * rows)), own.out, own.lse};
+  float* own_out = reinterpret_cast<float*>(take(4 * rows * d));
+  float* own_lse = reinterpret_cast<float*>(take(4 * rows));
+  const PrefixEnds ends{own.q_starts, own.seqs, own.max_q, own_out, own_lse, own.out, own.lse};
   prefix.out32 = reinterpret_cast<float*>(take(4 * rows * d));
   prefix.lse = reinterpret_cast<float*>(take(4 * rows));
-  prefix.mark = const_cast<float*>(ends.own_lse);
-  own.out32 = const_cast<float*>(ends.own_out);
-  own.lse = const_cast<float*>(ends.own_lse);
+  own.out32 = own_out;
+  own.lse = own_lse;
+  own.beside = 1;
   PrefillParams p = prefill_params(prefix);
   p.unit_at = unit_at;
+  // The plan of the prefix pass, beside it the own pass, then the prefix pass.
+  p.plan_only = 1;
   cudaError_t err = launch_prefill(p, stream);
   if (err != cudaSuccess) return err;
   const bool few = (long long)own.max_q * p.groups <= attn_decode_rows(own);
   err = few ? launch_attn_decode(own, stream) : launch_attn_prefill(own, stream);
   if (err != cudaSuccess) return err;
+  p.plan_only = 0;
+  p.planned = 1;
+  if ((err = launch_prefill(p, stream)) != cudaSuccess) return err;
   const int mt = two_tiles(p) ? 2 : 1;
   const long long pairs = (long long)p.max_units * own.c.heads;
   const long long blocks = std::min<long long>(pairs, 2ll * device_sm_count());

@@ -373,7 +373,9 @@ struct AttnLaunch {
   const int* group_starts; // "sequence" g is sequences group_starts[g] ... g + 1 of q_starts
   int group_seqs;          // how many sequences q_starts has then
   long long unit_rows;     // rows of a typical sequence (0: max_q's)
-  float* mark;             // [q_tokens][q_heads]: kNoRow at every row of the pass, or nullptr
+  // The launch before is of the same call and what this pass starts with does not
+  // depend on it: its first kernel runs beside that one, and waits for it at its end.
+  int beside;
 
   __device__ int q_start(int s) const {
     if (group_starts == nullptr) return __ldg(q_starts + s);
@@ -381,8 +383,6 @@ struct AttnLaunch {
     return __ldg(q_starts + (g < 0 ? 0 : g > group_seqs ? group_seqs : g));
   }
 };
-// What no log-sum-exp is: a NaN of a bit pattern that arithmetic does not make.
-constexpr unsigned kNoRow = 0x7f800001u;
 // The decode kernel takes up to attn_decode_rows() rows (new tokens x query
 // heads per key/value head) of a sequence; the tensor-core kernel any number.
 int attn_decode_rows(const AttnLaunch& l);

@@ -61,7 +61,7 @@ constexpr float kMinScale = 1.1754944e-38f;
 constexpr int kEpiWarps = 16, kQWarp = 16, kMmaWarp = 17, kKeyWarp = 19, kTokenWarp = 20;
 constexpr int kThreads = 22 * 32;
 constexpr int kUnit = 256;       // tokens of an item: two tiles of 128
-constexpr int kMaxKeys = 12, kMaxQ = 3, kItems = 4, kTokens = 2;
+constexpr int kMaxKeys = 12, kMaxQ = 4, kItems = 4, kTokens = 2;
 constexpr int kScan = 256;       // threads that share out the sequences
 constexpr uint32_t kTmemCols = 512;
 constexpr int kTerms = 3;        // e4m3 terms of an f16 query (bf16: two)
@@ -284,16 +284,16 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
       "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
       : "memory");
 }
-// The sum of a lane's weights over 32 columns: e^x in log2, x = s * factor + nl.
+// The sum of a lane's weights over N columns: e^x in log2, x = s * factor + nl.
 // s: fp32 products (e4m3: the coarse sum, `fine` the one in units of 1 / kFine,
 // `key` the key's scale). (One fp32 operation at a time: in pairs, the moves that join
 // and part them made it 8 instructions a column.)
-template <bool Q8>
-__device__ __forceinline__ float weigh(const uint32_t* s, const uint32_t* fine, float scale, float key,
+template <bool Q8, int N>
+__device__ __forceinline__ float weigh(const uint32_t (&s)[N], const uint32_t* fine, float scale, float key,
                                        const float* nl, const float* factor) {
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < 32; i += 4) {
+  for (int i = 0; i < N; i += 4) {
     const float4 n4 = *reinterpret_cast<const float4*>(nl + i);
     const float n[4] = {n4.x, n4.y, n4.z, n4.w};
     float f[4] = {scale, scale, scale, scale};
@@ -312,19 +312,31 @@ __device__ __forceinline__ float weigh(const uint32_t* s, const uint32_t* fine, 
   return (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 // Columns outside [lo, hi) become `hidden`, an infinity that the factor makes -inf.
-__device__ __forceinline__ void hide(uint32_t* s, int lo, int hi, float hidden) {
+template <int N>
+__device__ __forceinline__ void hide(uint32_t (&s)[N], int lo, int hi, float hidden) {
 #pragma unroll
-  for (int i = 0; i < 32; ++i) s[i] = i >= lo && i < hi ? s[i] : __float_as_uint(hidden);
+  for (int i = 0; i < N; ++i) s[i] = i >= lo && i < hi ? s[i] : __float_as_uint(hidden);
 }
-// Ties r's uses to a tcgen05.wait::ld that came before.
-__device__ __forceinline__ void tie32(uint32_t* r) {
-  asm volatile(""
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
-                 "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
-                 "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]),
-                 "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
-                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
-                 "+r"(r[30]), "+r"(r[31]));
+// Loads of tensor memory, and the wait for all of them (which ties r's uses to it).
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[32]) {
+  tmem_ld32_nowait(taddr, r);
+}
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,"
+      "%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+template <int N>
+__device__ __forceinline__ void tie(uint32_t (&r)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; i += 8)
+    asm volatile(""
+                 : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]),
+                   "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]));
 }
 
 // An item's token, from the token warps to the epilogue.
@@ -521,17 +533,19 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (lane == 0) mbar_arrive(&ctl->s_empty[half * 2 + buf]);
         };
         float part = 0.f;
+        constexpr int kCols = Q8 ? 16 : 32;  // at once
 #pragma unroll 1
-        for (int c0 = 32 * odd; c0 < p.nq; c0 += 64) {
-          uint32_t s[32], fine[Q8 ? 32 : 1];
-          tmem_ld32_nowait(ts + c0, s);
-          if constexpr (Q8) tmem_ld32_nowait(ts + p.nq + c0, fine);
+        for (int c0 = 32 * odd; c0 < p.nq; c0 += c0 % 32 + kCols < 32 ? kCols : 64 - c0 % 32) {
+          uint32_t s[kCols], fine[Q8 ? kCols : 8];
+          tmem_load(ts + c0, s);
+          if constexpr (Q8) tmem_load(ts + p.nq + c0, fine);
           tmem_ld_wait();
-          tie32(s);
-          if constexpr (Q8) tie32(fine);
-          if (c0 + 64 >= p.nq) release();
+          tie(s);
+          if (Q8) tie(fine);
+          if (c0 % 32 + kCols == 32 && c0 + 64 >= p.nq) release();
           if (masked) hide(s, lo - c0, hi - c0, hidden);
-          part += weigh<Q8>(s, fine, p.scale_log2, key_scale, mine + c0 / 64 * 32, mine + 64);
+          const int at = c0 / 64 * 32 + c0 % 32;
+          part += weigh<Q8>(s, fine, p.scale_log2, key_scale, mine + at, mine + 64 + at);
         }
         if (32 * odd >= p.nq) release();  // (no column of the tile)
         sum += part;
@@ -930,8 +944,9 @@ cudaError_t launch_kv_scores(const ScoresLaunch& l, cudaStream_t stream) {
   p.q_bytes = p.nq * p.row_bytes * p.slices * (q8 ? p.terms : 1);
   constexpr int kControl = kTables + sizeof(Ctl) + 1024;
   constexpr int kRoom = 220 * 1024 - kControl;
-  p.q_stages = 3;
-  if (kRoom - 3 * p.q_bytes < 3 * p.key_bytes) p.q_stages = 2;
+  // Items of many Q tiles want them ahead, items of few the next items' keys.
+  p.q_stages = rows > 4 * p.nq ? std::min(kMaxQ, (kRoom - 2 * p.key_bytes) / p.q_bytes)
+                               : kRoom - 3 * p.q_bytes < 3 * p.key_bytes ? 2 : 3;
   p.key_stages = std::min(kMaxKeys, (kRoom - p.q_stages * p.q_bytes) / p.key_bytes);
   const size_t smem = (size_t)p.key_stages * p.key_bytes + p.q_stages * p.q_bytes + kControl;
   const long long sms = device_sm_count();
