@@ -80,6 +80,7 @@ constexpr float kLazy = 8.f;
 // A block takes at least this much work, in key tiles (2 instead: 100 tokens on
 // 16384, one head, 46 us against 45; 16 mixed chunks 62 against 56).
 constexpr int kMinTiles = 4;
+constexpr int kPrefixMinTiles = 2;
 // What a run of key tiles of one (rows, head) costs beside them, in key tiles:
 // Q in, O out and the pipeline's filling (3.7 us, a tile 2.2). With 1, 2, 3 a
 // prompt of 8192 tokens takes 570, 515, 527 us, 16 mixed chunks 61, 56, 66, 512
@@ -105,6 +106,7 @@ struct PrefillParams {
   int4* units;      // sequence, first token in it, first key, key tiles
   long long* unit_at;  // place of each unit's first cost (nullptr: not wanted)
   int max_units;
+  int min_tiles;       // work that a block takes at least
   int plan_only, planned;  // (host) launch the plan alone, or all but it
   float* parts;
   // tensor copies: rows of a page that one copy takes (a power of two that
@@ -463,7 +465,7 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const PrefillPa
   at_sh[tid] = at;  // of unit u0; `total` where the thread has none
   if (p.unit_at != nullptr)
     for (int u = u0; u < u1; ++u) p.unit_at[u] += at;
-  long long ctas = (total + kMinTiles - 1) / kMinTiles;
+  long long ctas = (total + p.min_tiles - 1) / p.min_tiles;
   if (ctas > max_ctas) ctas = max_ctas;
   if (tid == 0) {
     p.head[0] = total;
@@ -1704,6 +1706,7 @@ PrefillParams prefill_params(const AttnLaunch& l) {
   p.page_shift = (l.c.page_size & (l.c.page_size - 1)) == 0 ? __builtin_ctz(l.c.page_size) : -1;
   const long long sms = device_sm_count();
   p.max_units = (int)max_units(l.q_tokens, l.seqs);
+  p.min_tiles = kMinTiles;
   uint8_t* at = l.scratch;
   p.head = reinterpret_cast<long long*>(at);
   at += 256;
@@ -1764,6 +1767,7 @@ cudaError_t launch_attn_prefix(AttnLaunch prefix, AttnLaunch own, cudaStream_t s
   own.beside = 1;
   PrefillParams p = prefill_params(prefix);
   p.unit_at = unit_at;
+  p.min_tiles = kPrefixMinTiles;
   // The plan of the prefix pass, beside it the own pass, then the prefix pass.
   p.plan_only = 1;
   cudaError_t err = launch_prefill(p, stream);

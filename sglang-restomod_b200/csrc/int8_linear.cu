@@ -11,13 +11,15 @@
 // tokens], so that one to 16 tokens cost one N = 16 column block and all of a
 // weight row's bytes feed the same lane. Operands come by tensor copies with
 // 128-byte swizzle, 128 K a stage (rows past N, tokens past M and columns past K
-// read as zeros). Warps: 0-3 epilogue, 4 copies, 5 products and tensor memory.
+// read as zeros). Warps: 0-3 epilogue, 4 copies of weights, 5 products and tensor
+// memory, 6 copies of activations.
 //
 // Few tiles (a decode batch): a tile's K range is cut over a cluster of up to 8
 // blocks, which exchange their int32 partial sums through one another's shared
 // memory, each adding and storing a share of the tile's columns. Integer sums
 // are exact, so the result is the same for any cut.
 #include <algorithm>
+#include <atomic>
 
 #include "common.cuh"
 #include "internal.h"
@@ -29,8 +31,9 @@ namespace {
 using namespace tcg;
 using namespace tcg_host;
 
-constexpr int kThreads = 192;
-constexpr int kEpiWarps = 4, kProdWarp = 4, kMmaWarp = 5;
+constexpr int kThreads = 224;
+constexpr int kMaxSplits = 8;
+constexpr int kEpiWarps = 4, kProdWarp = 4, kMmaWarp = 5, kProdWarp2 = 6;
 constexpr uint32_t kATile = 128 * 128;  // 128 weight rows x 128 K
 
 struct Int8Params {
@@ -163,7 +166,7 @@ __global__ void __launch_bounds__(kThreads, Int8Shape<NT>::kBlocks)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int s = 0; s < S::kStages; ++s) {
-      mbar_init(&ctl->full[s], 1);
+      mbar_init(&ctl->full[s], 2);
       mbar_init(&ctl->empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -194,39 +197,30 @@ __global__ void __launch_bounds__(kThreads, Int8Shape<NT>::kBlocks)
   if (!(p.early && warp == kProdWarp)) griddep_wait();
   if (tid == 0) griddep_launch_dependents();
 
-  if (warp == kProdWarp) {
+  if (warp == kProdWarp || warp == kProdWarp2) {
+    // Each operand's copies by a thread of its own, since issuing them takes time.
     if (lane == 0) {
+      const bool weights = warp == kProdWarp;
+      const uint32_t bytes = weights ? kATile : NT * 128;
       long long t = 0;
       bool ok = true;
-      int ahead = 0;  // stages of the first item whose weights are on their way
-      auto expect = [&](int s) {
-        mbar_arrive_expect_tx(&ctl->full[s], S::kStageBytes);
-      };
-      if (p.early) {
-        // the weights of the first stages, while the kernel before still quantizes
-        const Int8Item it = int8_item(p, g0, NT);
-        for (; ahead < min(S::kStages, k1 - k0); ++ahead) {
-          expect(ahead);
-          tma_load_2d(smem + ahead * S::kStageBytes, &w_map, (k0 + ahead) * 128, it.tile * 128,
-                      &ctl->full[ahead]);
-        }
-        griddep_wait();
-      }
       for (long long g = g0; g < items && ok; g += gs) {
         const Int8Item it = int8_item(p, g, NT);
         for (int k = k0; k < k1; ++k, ++t) {
           const int s = (int)(t % S::kStages);
           uint8_t* st = smem + s * S::kStageBytes;
-          if (t >= ahead) {
-            ok = i8_wait(&ctl->empty[s], (uint32_t)((t / S::kStages) & 1) ^ 1u, ctl, p.status);
-            if (!ok) break;
-            expect(s);
+          ok = i8_wait(&ctl->empty[s], (uint32_t)((t / S::kStages) & 1) ^ 1u, ctl, p.status);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&ctl->full[s], bytes);
+          if (weights)
             tma_load_2d(st, &w_map, k * 128, it.tile * 128, &ctl->full[s]);
-          }
-          tma_load_2d(st + kATile, &x_map, k * 128, (int)it.token0, &ctl->full[s]);
+          else
+            tma_load_2d(st + kATile, &x_map, k * 128, (int)it.token0, &ctl->full[s]);
         }
       }
-      // after an abort, copies in flight land before the block exits
+      if (p.early && weights) griddep_wait();
+      // After an abort, copies in flight land before the block exits. (Where the other
+      // operand's never came a barrier does not complete: the wait gives up.)
       if (!ok)
         for (long long v = t > S::kStages ? t - S::kStages : 0; v < t; ++v)
           mbar_wait(&ctl->full[v % S::kStages], (uint32_t)((v / S::kStages) & 1), p.status);
@@ -332,14 +326,26 @@ __global__ void __launch_bounds__(kThreads, Int8Shape<NT>::kBlocks)
       if (n < p.n) {
         const float sw = __ldg(p.w_scales + n);
         const int* part = reinterpret_cast<const int*>(smem) + row;
-        for (int c = 0; c < count; ++c) {
-          int sum = 0;
-          for (int r = 0; r < p.splits; ++r) sum += part[(r * own + c) * 128];
-          const long long token = it.token0 + first + c;
-          const float y = (float)sum * __ldg(p.x_scales + token) * sw;
-          static_cast<uint16_t*>(p.out)[token * p.n + n] =
-              p.out_f16 ? __half_as_ushort(__float2half_rn(y))
-                        : __bfloat16_as_ushort(__float2bfloat16_rn(y));
+        // (sixteen columns at a time: their loads do not wait for one another)
+        for (int c0 = 0; c0 < count; c0 += 16) {
+          int sum[16];
+          float sx[16];
+#pragma unroll
+          for (int c = 0; c < 16; ++c) {
+            sum[c] = 0;
+            sx[c] = c0 + c < count ? __ldg(p.x_scales + it.token0 + first + c0 + c) : 0.f;
+          }
+          for (int r = 0; r < p.splits; ++r)
+#pragma unroll
+            for (int c = 0; c < 16; ++c) sum[c] += part[(r * own + c0 + c) * 128];
+          uint16_t* out = static_cast<uint16_t*>(p.out) + (it.token0 + first + c0) * p.n + n;
+#pragma unroll
+          for (int c = 0; c < 16; ++c) {
+            if (c0 + c >= count) break;
+            const float y = (float)sum[c] * sx[c] * sw;
+            out[c * p.n] = p.out_f16 ? __half_as_ushort(__float2half_rn(y))
+                                     : __bfloat16_as_ushort(__float2bfloat16_rn(y));
+          }
         }
       }
     }
@@ -355,9 +361,10 @@ __global__ void __launch_bounds__(kThreads, Int8Shape<NT>::kBlocks)
 }
 
 // --------------------------------------------------- activation quantization
-// A row by a warp (up to 4096 columns), or by a cluster of blocks of 256 threads;
-// the row's values stay in registers between the maximum and the codes.
-constexpr int kHeld = 16;  // vectors of 8 a thread keeps; what is beyond is read again
+// A row by a warp (many short ones), or by a cluster of blocks of 256 threads; the
+// row's values stay in registers between the maximum and the codes, HELD vectors of 8
+// a thread (2, 4 or 16: code for vectors that are not there takes time); what is
+// beyond is read again.
 
 template <bool F16>
 __device__ __forceinline__ void unpack8(const uint4& raw, float (&v)[8]) {
@@ -384,14 +391,27 @@ __device__ __forceinline__ uint32_t top2(uint32_t top, const uint4& r) {
   return __vmaxu2(top, r.w & 0x7fff7fffu);
 }
 
-template <bool F16, int TPR>
+// Eight codes by division, out of line: it is rarely needed, and sixteen copies of it
+// drove the rest out of the instruction cache (8192 rows of 4096: 42 us).
+template <bool F16>
+__device__ __noinline__ uint2 quotients(uint4 raw, float scale) {
+  float v[8];
+  unpack8<F16>(raw, v);
+  uint32_t o[2] = {0u, 0u};
+  if (scale > 0.f)
+    for (int i = 0; i < 8; ++i)
+      o[i / 4] |= (uint32_t)(min(127, max(-127, __float2int_rn(v[i] / scale))) & 255) << (8 * (i % 4));
+  return make_uint2(o[0], o[1]);
+}
+
+template <bool F16, int TPR, int HELD>
 __global__ void __launch_bounds__(256) int8_quant_kernel(const uint16_t* __restrict__ x,
                                                          long long rows, int k, int8_t* q,
                                                          float* scales) {
   __shared__ uint32_t shared_top[8];
   __shared__ uint32_t block_top;
   uint32_t blocks = 1, rank = 0;
-  if (TPR == 256) {
+  if (TPR == 256) {  // (1 and 0 in a launch without clusters)
     asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(blocks));
     rank = cluster_rank();
   }
@@ -402,19 +422,32 @@ __global__ void __launch_bounds__(256) int8_quant_kernel(const uint16_t* __restr
   const int first = TPR == 32 ? lane : (int)(rank * 256 + threadIdx.x);
   const int vecs = k / 8;
   const long long per = TPR == 32 ? (long long)gridDim.x * 8 : gridDim.x / blocks;
-  for (long long r = TPR == 32 ? (long long)blockIdx.x * 8 + warp : blockIdx.x / blocks; r < rows;
-       r += per) {
+  // (the next row is on its way while this one is worked on, where registers allow)
+  constexpr bool kAhead = HELD <= 2;
+  uint4 held[HELD], next[kAhead ? HELD : 1];
+  auto load = [&](long long r, uint4* to) {
     const uint4* src = reinterpret_cast<const uint4*>(x + r * k);
-    uint4 held[kHeld];
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
+      const int v = first + i * step;
+      to[i] = r < rows && v < vecs ? __ldg(src + v) : make_uint4(0u, 0u, 0u, 0u);
+    }
+  };
+  const long long row0 = TPR == 32 ? (long long)blockIdx.x * 8 + warp : blockIdx.x / blocks;
+  if constexpr (kAhead) load(row0, next);
+  for (long long r = row0; r < rows; r += per) {
+    const uint4* src = reinterpret_cast<const uint4*>(x + r * k);
+    if constexpr (kAhead) {
+#pragma unroll
+      for (int i = 0; i < HELD; ++i) held[i] = next[i];
+      load(r + per, next);
+    } else {
+      load(r, held);
+    }
     uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
-      const int v = first + i * step;
-      held[i] = v < vecs ? __ldg(src + v) : make_uint4(0u, 0u, 0u, 0u);
-    }
-#pragma unroll
-    for (int i = 0; i < kHeld; ++i) top = top2(top, held[i]);
-    for (int v = first + kHeld * step; v < vecs; v += step) top = top2(top, __ldg(src + v));
+    for (int i = 0; i < HELD; ++i) top = top2(top, held[i]);
+    for (int v = first + HELD * step; v < vecs; v += step) top = top2(top, __ldg(src + v));
     top = max(top & 0xffffu, top >> 16);
     top = __reduce_max_sync(0xffffffffu, top);
     if (TPR == 256) {
@@ -441,33 +474,39 @@ __global__ void __launch_bounds__(256) int8_quant_kernel(const uint16_t* __restr
     // An infinity or NaN makes the row's scale NaN, and with it its outputs.
     const bool bad = F16 ? top >= 0x7c00u : top >= 0x7f80u;
     const float scale = bad ? __int_as_float(0x7fc00000) : amax / 127.f;
+    // rint(v / scale). A product with 1 / scale is off by less than 4e-5 at 127, so it
+    // gives the same whole number unless it comes that near to a half; then, and for
+    // scales whose reciprocal is not finite, the quotient itself decides.
+    const float inv = scale > 1e-30f ? __frcp_rn(scale) : __int_as_float(0x7fc00000);
     auto codes = [&](const uint4& raw) {
-      float v[8];
+      constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: its unit is 1
+      float v[8], far = 0.f;
       unpack8<F16>(raw, v);
-      uint32_t o[2] = {0u, 0u};
-      if (scale > 0.f) {
+      uint32_t c[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int c = min(127, max(-127, __float2int_rn(v[i] / scale)));
-          o[i / 4] |= (uint32_t)(c & 255) << (8 * (i % 4));
-        }
+      for (int i = 0; i < 8; ++i) {
+        const float x = v[i] * inv, t = __fadd_rn(x, kMagic);
+        c[i] = __float_as_uint(t);
+        far = fmaxf(far, fabsf(x - __fsub_rn(t, kMagic)));
       }
-      return make_uint2(o[0], o[1]);
+      if (!(far < 0.49995f) || inv != inv) return quotients<F16>(raw, scale);
+      return make_uint2(
+          __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410),
+          __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410));
     };
     uint2* dst = reinterpret_cast<uint2*>(q + r * k);
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
+    for (int i = 0; i < HELD; ++i) {
       const int v = first + i * step;
       if (v < vecs) dst[v] = codes(held[i]);
     }
-    for (int v = first + kHeld * step; v < vecs; v += step) dst[v] = codes(__ldg(src + v));
+    for (int v = first + HELD * step; v < vecs; v += step) dst[v] = codes(__ldg(src + v));
     if (first == 0) scales[r] = scale;
   }
 }
 
 template <int NT>
-cudaError_t launch_gemm(Int8Params& p, long long ctas, const CUtensorMap& w_map,
-                        const CUtensorMap& x_map, cudaStream_t stream) {
+cudaError_t configure() {
   using S = Int8Shape<NT>;
   static_assert(S::exchange_fits(), "shared memory");
   static bool configured[64] = {};
@@ -481,6 +520,53 @@ cudaError_t launch_gemm(Int8Params& p, long long ctas, const CUtensorMap& w_map,
     if (err != cudaSuccess) return err;
     configured[dev] = true;
   }
+  return cudaSuccess;
+}
+
+// How many clusters of `splits` blocks run at once on the current device (0: the
+// query failed), asked for once.
+template <int NT>
+int clusters_of(int splits) {
+  static std::atomic<int> known[64][kMaxSplits + 1];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64 || configure<NT>() != cudaSuccess)
+    return 0;
+  int n = known[dev][splits].load(std::memory_order_relaxed);
+  if (n == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)splits);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = Int8Shape<NT>::kSmem;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)splits;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, int8_gemm_kernel<NT>, &cfg) != cudaSuccess) {
+      (void)cudaGetLastError();
+      n = -1;
+    }
+    known[dev][splits].store(n == 0 ? -1 : n, std::memory_order_relaxed);
+  }
+  return n > 0 ? n : 0;
+}
+int max_clusters(int nt, int splits) {
+  switch (nt) {
+    case 16: return clusters_of<16>(splits);
+    case 32: return clusters_of<32>(splits);
+    case 64: return clusters_of<64>(splits);
+    case 128: return clusters_of<128>(splits);
+    default: return clusters_of<256>(splits);
+  }
+}
+
+template <int NT>
+cudaError_t launch_gemm(Int8Params& p, long long ctas, const CUtensorMap& w_map,
+                        const CUtensorMap& x_map, cudaStream_t stream) {
+  using S = Int8Shape<NT>;
+  const cudaError_t err = configure<NT>();
+  if (err != cudaSuccess) return err;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)ctas);
   cfg.blockDim = dim3(kThreads);
@@ -499,35 +585,50 @@ cudaError_t launch_gemm(Int8Params& p, long long ctas, const CUtensorMap& w_map,
 
 }  // namespace
 
-cudaError_t launch_int8_quant(const void* x, bool f16, long long rows, int k, int8_t* q,
-                              float* scales, cudaStream_t stream) {
-  const uint16_t* src = static_cast<const uint16_t*>(x);
-  const long long sms = device_sm_count();
-  if (k <= 32 * 8 * kHeld) {
-    const long long blocks = std::min<long long>((rows + 7) / 8, 8 * sms);
-    return f16 ? launch_pdl(int8_quant_kernel<true, 32>, dim3((unsigned)blocks), dim3(256), 0,
-                            stream, src, rows, k, q, scales)
-               : launch_pdl(int8_quant_kernel<false, 32>, dim3((unsigned)blocks), dim3(256), 0,
-                            stream, src, rows, k, q, scales);
-  }
-  // few rows: a cluster of blocks each
-  unsigned c = 8;
-  while (c > 1 && rows * c > sms) c /= 2;
-  const long long clusters = std::min<long long>(rows, 4 * sms / c);
+namespace {
+
+template <bool F16, int TPR, int HELD>
+cudaError_t launch_quant(const uint16_t* x, long long rows, int k, int8_t* q, float* scales,
+                         long long blocks, unsigned cluster, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(clusters * c));
+  cfg.gridDim = dim3((unsigned)blocks);
   cfg.blockDim = dim3(256);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = c;
+  attr[1].val.clusterDim.x = cluster;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  return f16 ? cudaLaunchKernelEx(&cfg, int8_quant_kernel<true, 256>, src, rows, k, q, scales)
-             : cudaLaunchKernelEx(&cfg, int8_quant_kernel<false, 256>, src, rows, k, q, scales);
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, int8_quant_kernel<F16, TPR, HELD>, x, rows, k, q, scales);
+}
+
+template <bool F16>
+cudaError_t launch_quant_type(const uint16_t* x, long long rows, int k, int8_t* q, float* scales,
+                              cudaStream_t stream) {
+  const long long sms = device_sm_count();
+  if (k <= 32 * 8 * 4 && rows >= 8 * sms)  // many short rows
+    return launch_quant<F16, 32, 4>(x, rows, k, q, scales, std::min<long long>((rows + 7) / 8, 8 * sms), 1,
+                                    stream);
+  // few rows: a cluster of blocks each, as long as a block has a vector a thread
+  unsigned c = 1;
+  while (c < 8 && rows * c * 2 <= sms && k >= 256 * 8 * 2 * (int)c) c *= 2;
+  const long long blocks = std::min<long long>(rows, 8 * sms / c) * c;
+  const int held = (k / 8 + 256 * (int)c - 1) / (256 * (int)c);
+  if (held <= 2) return launch_quant<F16, 256, 2>(x, rows, k, q, scales, blocks, c, stream);
+  if (held <= 4) return launch_quant<F16, 256, 4>(x, rows, k, q, scales, blocks, c, stream);
+  return launch_quant<F16, 256, 16>(x, rows, k, q, scales, blocks, c, stream);
+}
+
+}  // namespace
+
+cudaError_t launch_int8_quant(const void* x, bool f16, long long rows, int k, int8_t* q,
+                              float* scales, cudaStream_t stream) {
+  const uint16_t* src = static_cast<const uint16_t*>(x);
+  return f16 ? launch_quant_type<true>(src, rows, k, q, scales, stream)
+             : launch_quant_type<false>(src, rows, k, q, scales, stream);
 }
 
 cudaError_t launch_int8_gemm(const Int8Launch& l, cudaStream_t stream) {
@@ -548,10 +649,15 @@ cudaError_t launch_int8_gemm(const Int8Launch& l, cudaStream_t stream) {
   p.m_chunks = (int)((l.m + nt - 1) / nt);
   const long long items = (long long)p.m_chunks * p.n_tiles;
   const long long slots = sms * (nt <= 64 ? 2 : 1);
-  // K cut over as many blocks as fill the GPU once, each with some steps of its own
+  // K cut over as many blocks as run at once, each with some steps of its own. (Clusters
+  // of 7 did not fit all at a time, though 280 blocks would have: 5120 x 25600, one
+  // token, 34 us, and 25 by 5.)
   p.splits = 1;
-  if (items < slots)
-    p.splits = (int)std::max<long long>(1, std::min<long long>({8, slots / items, p.kch / 4}));
+  for (int c = kMaxSplits; c > 1; --c)
+    if (items * c <= slots && p.kch / c >= 4 && items <= max_clusters(nt, c)) {
+      p.splits = c;
+      break;
+    }
   const long long ctas = p.splits > 1 ? items * p.splits : std::min(items, slots);
   CUtensorMap w_map, x_map;
   const unsigned long long k = (unsigned long long)l.k;
