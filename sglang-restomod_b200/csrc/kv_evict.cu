@@ -6,10 +6,11 @@
 // keep their order and become tokens 0 .. budget - 1; their keys, values, scales
 // and scores move.
 //
-// Choice: a cluster of blocks per (sequence, head). The scores are read once, as
-// whole numbers of the same order, into shared memory; three histograms of 11, 11
-// and 10 bits, added over the cluster through distributed shared memory, give the
-// smallest kept number and how many of its equals stay; a count by warps and a
+// Choice: a block per (sequence, head), or a cluster of up to 8. A warp has
+// neighbouring tokens, whose scores it reads once, as whole numbers of the same order, into
+// registers (up to 16 a thread; what is beyond is read again); three histograms of
+// 11, 11 and 10 bits, added over the cluster through distributed shared memory, give
+// the smallest kept number and how many of its equals stay; a count by warps and a
 // scan place the kept ones in order. Whole numbers throughout, so the result does
 // not depend on the order of the atomics.
 //
@@ -22,6 +23,7 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "divisor.cuh"
 #include "internal.h"
 
 namespace b200 {
@@ -32,12 +34,8 @@ constexpr int kBins = 2048;
 
 struct EvictParams {
   EvictLaunch e;
-  int page_shift;  // log2 of the page size, -1 where it is no power of two
-  int held;        // scores of a block that fit its shared memory
+  Divisor by_page;  // of the page size
 
-  __device__ int page_of(int token) const {
-    return page_shift >= 0 ? token >> page_shift : token / e.c.page_size;
-  }
   __device__ int tokens_of(int s) const {
     const long long cap = (long long)e.table_width * e.c.page_size;
     const int n = max(__ldg(e.kv_lens + s), 0);
@@ -45,7 +43,7 @@ struct EvictParams {
   }
   __device__ bool page_at(const int* table, long long stride, int s, int token, int& page,
                           int& offset) const {
-    const int i = page_of(token);
+    const int i = by_page.of(token);
     page = __ldg(table + s * stride + i);
     offset = token - i * e.c.page_size;
     return page >= 0 && page < e.c.num_pages;
@@ -71,6 +69,11 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+__device__ __forceinline__ void add_remote(void* p, uint32_t rank, uint32_t v) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("red.relaxed.cluster.shared::cluster.add.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
+}
 __device__ __forceinline__ uint32_t ld_remote(const void* p, uint32_t rank) {
   uint32_t a, v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
@@ -78,16 +81,40 @@ __device__ __forceinline__ uint32_t ld_remote(const void* p, uint32_t rank) {
   return v;
 }
 
+__device__ __forceinline__ uint4 ld_remote4(const void* p, uint32_t rank) {
+  uint32_t a;
+  uint4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(a)
+               : "memory");
+  return v;
+}
+
 struct ChoiceSmem {
   uint32_t hist[kBins];   // of this block
-  uint32_t above[kWarps]; // scan
+  alignas(16) uint32_t total[2][kBins];  // of the cluster, in its first block; steps in turn
+  uint32_t sums[kWarps];  // scan
   uint32_t bin, left;     // the step's result
   uint32_t counts[2];     // this block's kept ones above the border, and equals of it
   uint32_t warp_above[kWarps], warp_equal[kWarps];
 };
 
-__global__ void __launch_bounds__(kThreads) evict_choose_kernel(const EvictParams p, int blocks) {
-  extern __shared__ uint32_t ranks[];  // [held]
+// The sum of the values of the warps before this one, and of all; v: of lane = warp.
+__device__ __forceinline__ uint32_t sum_before(uint32_t v, int warp, uint32_t& all) {
+  uint32_t x = v;
+#pragma unroll
+  for (int o = 1; o < kWarps; o <<= 1) {
+    const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+    if ((threadIdx.x & 31) >= o) x += y;
+  }
+  all = __shfl_sync(0xffffffffu, x, kWarps - 1);
+  return __shfl_sync(0xffffffffu, x - v, warp);
+}
+
+template <int KEYS>
+__global__ void __launch_bounds__(kThreads, 2) evict_choose_kernel(const EvictParams p, int blocks) {
   __shared__ ChoiceSmem sm;
   const EvictLaunch& e = p.e;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -103,126 +130,156 @@ __global__ void __launch_bounds__(kThreads) evict_choose_kernel(const EvictParam
     for (int j = rank * kThreads + tid; j < n; j += blocks * kThreads) kept[j] = j;
     return;
   }
-  // This block's tokens [t0, t1); those in [lo, hi) are chosen from.
+  // This block's tokens [t0, t1), this warp's [w0, w1), the lane's w0 + lane, + 32, ...
   const int t0 = (int)((long long)n * rank / blocks), t1 = (int)((long long)n * (rank + 1) / blocks);
+  const int per = (t1 - t0 + kThreads - 1) / kThreads * 32;
+  const int w0 = min(t0 + warp * per, t1), w1 = min(w0 + per, t1);
+  // The first and the last tokens rank above any score.
   const int lo = e.first, hi = n - e.recent;
-  uint32_t need = (uint32_t)(e.budget - e.first - e.recent);
-  auto read = [&](int t) -> uint32_t {
-    int page, offset;
-    if (!p.page_at(e.table, e.table_stride, seq, t, page, offset)) {
-      atomicOr(e.status, kDevBadPage);
+  const float* scores = e.scores + head * e.score_head_stride;
+  const int* table = e.table + seq * e.table_stride;
+  bool bad = false;
+  auto score_of = [&](int t, int page) -> uint32_t {
+    if (t < lo || t >= hi) return 0xffffffffu;
+    if (page < 0 || page >= e.c.num_pages) {
+      bad = true;
       return 0u;
     }
-    return rank_of(e.scores[p.score_at(page, offset, head)]);
+    const int offset = t - p.by_page.of(t) * e.c.page_size;
+    return __float_as_uint(scores[page * e.score_page_stride + offset * e.score_token_stride]);
   };
-#pragma unroll 8
-  for (int i = tid; i < min(t1 - t0, p.held); i += kThreads) {
-    const int t = t0 + i;
-    ranks[i] = t >= lo && t < hi ? read(t) : 0u;
+  auto rank_at = [&](int t, uint32_t score, int page) {
+    return t < lo || t >= hi || page < 0 || page >= e.c.num_pages ? score
+                                                                   : rank_of(__uint_as_float(score));
+  };
+  auto read = [&](int t) -> uint32_t {
+    const int page = __ldg(table + p.by_page.of(t));
+    return rank_at(t, score_of(t, page), page);
+  };
+  // (all page numbers, then all scores: one after the other a token cost two latencies)
+  uint32_t keys[KEYS];
+  int pages[KEYS];
+#pragma unroll
+  for (int i = 0; i < KEYS; ++i) {
+    const int t = w0 + 32 * i + lane;
+    pages[i] = t < w1 ? __ldg(table + p.by_page.of(t)) : 0;
   }
-  __syncthreads();
-  auto value = [&](int t) { return t - t0 < p.held ? ranks[t - t0] : read(t); };
+#pragma unroll
+  for (int i = 0; i < KEYS; ++i) {
+    const int t = w0 + 32 * i + lane;
+    keys[i] = t < w1 ? score_of(t, pages[i]) : 0u;
+  }
+#pragma unroll
+  for (int i = 0; i < KEYS; ++i) keys[i] = rank_at(w0 + 32 * i + lane, keys[i], pages[i]);
+  // f(token, its rank, whether there is one) for the lane's tokens
+  auto each = [&](auto&& f) {
+#pragma unroll
+    for (int i = 0; i < KEYS; ++i)
+      if (w0 + 32 * i < w1) f(w0 + 32 * i + lane, keys[i], w0 + 32 * i + lane < w1);
+    for (int t = w0 + 32 * KEYS + lane; t - lane < w1; t += 32) f(t, t < w1 ? read(t) : 0u, t < w1);
+  };
 
+  if (blocks > 1) {
+#pragma unroll
+    for (int i = 0; i < kBins / kThreads; ++i) sm.total[0][tid + i * kThreads] = 0;
+    cluster_sync();
+  }
+  uint32_t need = (uint32_t)e.budget;
   uint32_t border = 0;  // the digits of the smallest kept rank found so far
-  const int c0 = max(t0, lo), c1 = min(t1, hi);
-  if (need > 0) {
 #pragma unroll 1
-    for (int step = 0; step < 3; ++step) {
-      const int shift = step == 0 ? 21 : step == 1 ? 10 : 0, bits = step == 2 ? 10 : 11;
-      for (int i = tid; i < kBins; i += kThreads) sm.hist[i] = 0;
-      __syncthreads();
-      for (int t = c0 + tid; t < c1; t += kThreads) {
-        const uint32_t v = value(t);
-        if (step > 0 && (v ^ border) >> (shift + bits)) continue;
+  for (int step = 0; step < 3; ++step) {
+    const int shift = step == 0 ? 21 : step == 1 ? 10 : 0, bits = step == 2 ? 10 : 11;
+#pragma unroll
+    for (int i = 0; i < kBins / kThreads; ++i) sm.hist[tid + i * kThreads] = 0;
+    __syncthreads();
+    const uint32_t high = (uint32_t)(0xffffffffull << (shift + bits));  // digits that are known
+    each([&](int, uint32_t v, bool on) {
+      if (on && ((v ^ border) & high) == 0)
         atomicAdd(&sm.hist[v >> shift & ((1u << bits) - 1u)], 1u);
-      }
-      if (blocks > 1)
-        cluster_sync();
-      else
-        __syncthreads();
-      // thread i: the cluster's counts of bins 4i .. 4i + 3 from the top
-      uint32_t count[4], sum = 0;
+    });
+    __syncthreads();
+    // thread i: the counts of bins 4i .. 4i + 3 from the top, the cluster's by way of
+    // its first block
+    uint32_t count[4], sum = 0;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int b = kBins - 1 - (4 * tid + k);
-        count[k] = blocks > 1 ? 0u : sm.hist[b];
-        if (blocks > 1)
-          for (int r = 0; r < blocks; ++r) count[k] += ld_remote(&sm.hist[b], r);
-        sum += count[k];
-      }
-      uint32_t above = sum;
+    for (int k = 0; k < 4; ++k) count[k] = sm.hist[kBins - 1 - (4 * tid + k)];
+    if (blocks > 1) {
+      uint32_t* total = &sm.total[step & 1][kBins - 1 - 4 * tid];
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t x = __shfl_up_sync(0xffffffffu, above, o);
-        if (lane >= o) above += x;
-      }
-      if (lane == 31) sm.above[warp] = above;
-      __syncthreads();
-      above -= sum;
-      for (int w = 0; w < warp; ++w) above += sm.above[w];
+      for (int k = 0; k < 4; ++k)
+        if (count[k]) add_remote(total - k, 0, count[k]);
+      cluster_sync();
+      // (16 bytes a load: every thread of the cluster reads the one block)
+      const uint4 four = ld_remote4(total - 3, 0);
+      count[0] = four.w, count[1] = four.z, count[2] = four.y, count[3] = four.x;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if (above < need && above + count[k] >= need) {
-          sm.bin = kBins - 1 - (4 * tid + k);
-          sm.left = need - above;
-        }
-        above += count[k];
-      }
-      if (blocks > 1)
-        cluster_sync();  // all have read this block's counts
-      else
-        __syncthreads();
-      border |= sm.bin << shift;
-      need = sm.left;
+      for (int k = 0; k < 4; ++k) sm.total[(step & 1) ^ 1][tid + k * kThreads] = 0;
     }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) sum += count[k];
+    uint32_t above = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t x = __shfl_up_sync(0xffffffffu, above, o);
+      if (lane >= o) above += x;
+    }
+    if (lane == 31) sm.sums[warp] = above;
+    __syncthreads();
+    uint32_t all;
+    above += sum_before(lane < kWarps ? sm.sums[lane] : 0u, warp, all) - sum;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (above < need && above + count[k] >= need) {
+        sm.bin = kBins - 1 - (4 * tid + k);
+        sm.left = need - above;
+      }
+      above += count[k];
+    }
+    if (blocks > 1)
+      cluster_sync();  // all have read the counts, and the others are cleared
+    else
+      __syncthreads();
+    border |= sm.bin << shift;
+    need = sm.left;
   }
-  // Kept: ranks above the border, and the first `need` equals of it. (None are
-  // where none are needed: the border is then above every rank.)
-  const bool none = e.budget == e.first + e.recent;
-  auto above_border = [&](int t) {
-    return t < lo || t >= hi || (!none && value(t) > border);
-  };
-  auto equals = [&](int t) { return t >= lo && t < hi && !none && value(t) == border; };
-  const int per = (t1 - t0 + kWarps * 32 - 1) / (kWarps * 32) * 32;
-  const int w0 = min(t0 + warp * per, t1), w1 = min(w0 + per, t1);
+  // Kept: ranks above the border, and the first `need` equals of it.
   uint32_t mine = 0, even = 0;
-  for (int t = w0 + lane; t - lane < w1; t += 32) {
-    mine += __popc(__ballot_sync(0xffffffffu, t < w1 && above_border(t)));
-    even += __popc(__ballot_sync(0xffffffffu, t < w1 && equals(t)));
-  }
+  each([&](int, uint32_t v, bool on) {
+    mine += on && v > border;
+    even += on && v == border;
+  });
+  mine = __reduce_add_sync(0xffffffffu, mine);
+  even = __reduce_add_sync(0xffffffffu, even);
   if (lane == 0) {
     sm.warp_above[warp] = mine;
     sm.warp_equal[warp] = even;
   }
   __syncthreads();
-  uint32_t before = 0, before_equal = 0;  // in the row, before this warp's tokens
-  {
-    uint32_t all = 0, all_equal = 0;
-    for (int w = 0; w < kWarps; ++w) {
-      if (w == warp) before = all, before_equal = all_equal;
-      all += sm.warp_above[w];
-      all_equal += sm.warp_equal[w];
+  uint32_t all, all_equal;  // before: in the row, before this warp's tokens
+  uint32_t before = sum_before(lane < kWarps ? sm.warp_above[lane] : 0u, warp, all);
+  uint32_t before_equal = sum_before(lane < kWarps ? sm.warp_equal[lane] : 0u, warp, all_equal);
+  if (blocks > 1) {
+    if (tid == 0) sm.counts[0] = all, sm.counts[1] = all_equal;
+    cluster_sync();
+    uint32_t up = 0, eq = 0;
+    if (lane < rank) {
+      up = ld_remote(&sm.counts[0], lane);
+      eq = ld_remote(&sm.counts[1], lane);
     }
-    if (blocks > 1) {
-      if (tid == 0) sm.counts[0] = all, sm.counts[1] = all_equal;
-      cluster_sync();
-      for (int r = 0; r < rank; ++r) {
-        before += ld_remote(&sm.counts[0], r);
-        before_equal += ld_remote(&sm.counts[1], r);
-      }
-      cluster_sync();  // read by all before any block ends
-    }
+    before += __reduce_add_sync(0xffffffffu, up);
+    before_equal += __reduce_add_sync(0xffffffffu, eq);
+    cluster_sync();  // read by all before any block ends
   }
-  for (int t = w0 + lane; t - lane < w1; t += 32) {
-    const bool up = t < w1 && above_border(t), eq = t < w1 && equals(t);
+  const uint32_t below = (1u << lane) - 1u;
+  each([&](int t, uint32_t v, bool on) {
+    const bool up = on && v > border, eq = on && v == border;
     const uint32_t ups = __ballot_sync(0xffffffffu, up), eqs = __ballot_sync(0xffffffffu, eq);
-    const uint32_t below = (1u << lane) - 1u;
     const uint32_t eq_rank = before_equal + __popc(eqs & below);
-    const uint32_t at = before + __popc(ups & below) + min(eq_rank, need);
-    if (up || (eq && eq_rank < need)) kept[at] = t;
+    if (up || (eq && eq_rank < need)) kept[before + __popc(ups & below) + min(eq_rank, need)] = t;
     before += __popc(ups);
     before_equal += __popc(eqs);
-  }
+  });
+  if (bad) atomicOr(e.status, kDevBadPage);
 }
 
 // Where kept token j comes from and goes to, in elements of each array; from < 0:
@@ -379,29 +436,15 @@ __global__ void __launch_bounds__(kShiftThreads) evict_shift_kernel(const EvictP
 cudaError_t launch_kv_evict(const EvictLaunch& l, cudaStream_t stream) {
   EvictParams p{};
   p.e = l;
-  p.page_shift = (l.c.page_size & (l.c.page_size - 1)) == 0 ? __builtin_ctz(l.c.page_size) : -1;
+  p.by_page = divisor(l.c.page_size);
   const long long sms = device_sm_count(), pairs = (long long)l.seqs * l.c.heads;
   const long long most = (long long)l.table_width * l.c.page_size;
-  // few rows: a cluster of blocks each, with some tokens of its own
+  // long rows: a cluster of blocks each, as long as they all run at once
   int blocks = 1;
-  while (blocks < 8 && pairs * blocks * 2 <= 2 * sms && most > 1024 * blocks) blocks *= 2;
-  constexpr int kMost = 48 * 1024;  // ranks that fit a block's shared memory
-  p.held = (int)std::min<long long>(kMost, (most + blocks - 1) / blocks);
-  static bool configured[64] = {};
-  int dev = 0;
-  cudaError_t err = cudaGetDevice(&dev);
-  if (err != cudaSuccess) return err;
-  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-  if (!configured[dev]) {
-    err = cudaFuncSetAttribute(evict_choose_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               kMost * 4);
-    if (err != cudaSuccess) return err;
-    configured[dev] = true;
-  }
+  while (blocks < 8 && pairs * blocks * 2 <= 2 * sms && most > 16ll * kThreads * blocks) blocks *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(pairs * blocks));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = (size_t)p.held * 4;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -411,7 +454,9 @@ cudaError_t launch_kv_evict(const EvictLaunch& l, cudaStream_t stream) {
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = blocks > 1 ? 2 : 1;
-  err = cudaLaunchKernelEx(&cfg, evict_choose_kernel, p, blocks);
+  const cudaError_t err = most <= 4ll * kThreads * blocks
+                              ? cudaLaunchKernelEx(&cfg, evict_choose_kernel<4>, p, blocks)
+                              : cudaLaunchKernelEx(&cfg, evict_choose_kernel<16>, p, blocks);
   if (err != cudaSuccess) return err;
   const int chunks = l.c.head_dim * (l.c.k_scale != nullptr ? 1 : 2) / 16;
   if (l.out_table != nullptr) {
