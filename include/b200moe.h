@@ -72,10 +72,11 @@ int b200_num_sms(void);
 int b200_workspace_status(void* workspace, int32_t* bits, int32_t reset, void* stream);
 
 /*
- * The same bits of all norm and attention calls on the current device since they
- * were last cleared: those without a workspace, and those whose workspace is
- * gone or lies in a captured graph. Attention records its bits in its call's
- * workspace too. Synchronizes `stream`; order it after the calls.
+ * The same bits of all norm, attention, 8-bit integer linear, score and eviction
+ * calls on the current device since they were last cleared: those without a
+ * workspace, and those whose workspace is gone or lies in a captured graph.
+ * Attention and scores record their bits in their call's workspace too.
+ * Synchronizes `stream`; order it after the calls.
  */
 int b200_device_status(int32_t* bits, int32_t reset, void* stream);
 
@@ -458,9 +459,9 @@ int b200_w8a8_moe_gemm(const void* a, int32_t a_dtype, int64_t a_rows, int64_t k
  *   s[t] = max_k |x[t, k]| / 127,  q[t, k] = rint(x[t, k] / s[t])  (0 where s is 0),
  *   y[t, n] = (sum_k q[t, k] * w[n, k]) * s[t] * w_scales[n],
  * the sum exact in int32, the rest fp32. A token with an infinity or NaN has a
- * NaN scale, codes of zero, and NaN outputs. w int8 [n, k] row-major, any values
- * (-128 included), w_scales fp32 [n]; k a multiple of 16 up to 131072, any m and
- * n. No workspace; b200_int8_linear takes q [m, k] and scales [m] to leave the
+ * NaN scale, codes of zero, and NaN outputs. A q of the caller's own holds codes
+ * of -127 .. 127. w int8 [n, k] row-major, any values (-128 included), w_scales
+ * fp32 [n]; k a multiple of 16 up to 131072, any m and n. No workspace; b200_int8_linear takes q [m, k] and scales [m] to leave the
  * quantized activations in.
  */
 int b200_int8_act_quant(const void* x, int32_t x_dtype, int64_t rows, int64_t k, int8_t* q,
@@ -579,10 +580,10 @@ int b200_paged_attention(const b200_kv_cache* cache, const void* q, int32_t dtyp
 /*
  * b200_paged_attention of a batch whose sequences share long prefixes, each
  * prefix read once for all of its sequences. Group g is the sequences
- * group_starts[g] .. group_starts[g + 1] (group_starts[0 .. groups] ascends from 0
- * to seqs); its prefix is the first prefix_lens[g] tokens (0: none) of the pages
- * prefix_table[g * prefix_table_stride ..], prefix_table_width entries. Sequence
- * s has kv_lens[s] cached tokens of its own, which come after its group's prefix:
+ * group_starts[g] .. group_starts[g + 1] - 1 (group_starts[0 .. groups] ascends
+ * from 0 to seqs: every sequence has a group); its prefix is the first prefix_lens[g]
+ * tokens (0: none) of the pages prefix_table[g * prefix_table_stride ..],
+ * prefix_table_width entries. Sequence s has kv_lens[s] cached tokens of its own, which come after its group's prefix:
  * the tables of both may name any pages, and a prefix may end within a page. Every
  * new token sees its group's whole prefix, and of its sequence's own tokens those at
  * its position and before. lse is over both. The rest as in
@@ -612,9 +613,9 @@ int b200_shared_prefix_attention(
  * and everything else as in b200_paged_attention, whose masks these are; of new
  * tokens past max_q_len none adds to the sums. lse may also be that of
  * b200_shared_prefix_attention. Scores are fp32 of (page, offset, head), at strides of
- * their own; scores_out may be scores. Each score has one writer, in a fixed order: two
- * calls give the same bits. No two sequences of a call may have a page in common. At
- * most 64 query heads per key/value head; q's vectors apart in memory. Products are
+ * their own; scores_out may be scores, or has no memory in common with them. Each
+ * score has one writer, in a fixed order: two calls give the same bits. No page may
+ * stand twice among the pages of the call's tokens. At most 64 query heads per key/value head; q's vectors apart in memory. Products are
  * exact to fp32's sums (e4m3 keys: queries to 2^-22 of their largest element);
  * a key scale byte may be any. Infinite or NaN queries or keys give NaN scores where
  * they are seen. Page numbers outside the cache set status bit 16. Workspace as
@@ -643,11 +644,12 @@ int b200_kv_cache_scores(const b200_kv_cache* cache, const void* q, int32_t dtyp
  * kept [seqs][kv_heads][budget]: their indices before, -1 past the sequence's
  * end; lens [seqs] = min(kv_lens, budget).
  * out_table NULL (or page_table): in place, in the sequence's first pages; the
- * slots after token lens[s] - 1 keep what they hold. No two sequences of the call
- * may have a page in common then. Otherwise the kept tokens, of sequences within the budget
+ * slots after token lens[s] - 1 keep what they hold. No page may stand twice among
+ * the pages of the call's tokens then. Otherwise the kept tokens, of sequences within the budget
  * too, are copied to the pages out_table[s * out_table_stride ..]
- * (out_table_width entries, enough for the budget), which hold no token of the
- * call's sequences; the source stays as it is. Page numbers outside the
+ * (out_table_width entries, enough for the budget), none of them twice, which hold
+ * no token of the call's sequences; the source stays as it is. At most 4194240 tokens
+ * of a row stay. Page numbers outside the
  * cache set status bit 16 (b200_device_status): such a token has the lowest score and is not
  * moved, nor is one whose new page is outside. Capturable; no workspace.
  */

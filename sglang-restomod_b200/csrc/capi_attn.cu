@@ -285,7 +285,9 @@ int b200_shared_prefix_attention(
   if (rc) return rc;
   if (groups < 0 || prefix_table_width < 0 || q_tokens + groups > 0x7fffffffll)
     return fail(B200_ERR_INVALID, "negative or too large count");
-  if (none || groups == 0) return B200_OK;
+  if (none) return B200_OK;
+  if (groups == 0)
+    return fail(B200_ERR_INVALID, "%d sequences in no group (a group may be without a prefix)", seqs);
   if (prefix_lens == nullptr || group_starts == nullptr ||
       (prefix_table_width > 0 && prefix_table == nullptr))
     return fail(B200_ERR_INVALID, "null pointer argument");
@@ -358,6 +360,9 @@ int b200_kv_cache_scores(const b200_kv_cache* cache, const void* q, int32_t dtyp
                                score_token_stride != out_token_stride ||
                                score_head_stride != out_head_stride))
     return fail(B200_ERR_INVALID, "scores in place need the same strides");
+  if (!apart3(out_page_stride, s.a.c.num_pages, out_token_stride, s.a.c.page_size, out_head_stride,
+              s.a.c.heads, 1))
+    return fail(B200_ERR_INVALID, "the scores overlap");
   const int64_t need = b200_kv_cache_scores_workspace_bytes(s.a.c.head_dim, q_tokens, q_heads);
   if ((rc = attention_workspace(s.a, workspace, workspace_bytes, need,
                                 "b200_kv_cache_scores_workspace_bytes")))

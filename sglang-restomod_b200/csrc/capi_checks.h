@@ -3,6 +3,7 @@
 
 #include <cstdarg>
 #include <cstdio>
+#include <utility>
 
 #include "../../include/b200moe.h"
 #include "internal.h"
@@ -35,6 +36,26 @@ namespace {
   return head_stride <= token_stride
              ? head_stride >= dim && token_stride >= (heads - 1) * head_stride + dim
              : token_stride >= dim && head_stride >= (tokens - 1) * token_stride + dim;
+}
+
+// The same of three counts (pages, tokens of a page, heads), of vectors of `dim`: from
+// the smallest stride up, each at least as long as what the smaller ones cover. A count of
+// one has no stride.
+[[maybe_unused]] bool apart3(int64_t s0, int64_t n0, int64_t s1, int64_t n1, int64_t s2, int64_t n2, int64_t dim) {
+  int64_t stride[3] = {s0, s1, s2}, count[3] = {n0, n1, n2};
+  for (int i = 0; i < 2; ++i)
+    for (int j = 0; j < 2 - i; ++j)
+      if (stride[j] > stride[j + 1]) {
+        std::swap(stride[j], stride[j + 1]);
+        std::swap(count[j], count[j + 1]);
+      }
+  int64_t covered = dim;
+  for (int i = 0; i < 3; ++i) {
+    if (count[i] <= 1) continue;
+    if (stride[i] < covered) return false;
+    covered += (count[i] - 1) * stride[i];
+  }
+  return true;
 }
 
 // The cache's description, checked and in the kernels' form.

@@ -1,6 +1,8 @@
 // C ABI of the 8-bit integer linear and of the eviction of cached tokens by their
 // accumulated weights. Host-side validation and launches; declared in
 // include/b200moe.h.
+#include <algorithm>
+
 #include "capi_checks.h"
 
 using namespace b200;
@@ -17,13 +19,16 @@ int check_int8(int64_t m, int64_t k, int64_t n) {
   return B200_OK;
 }
 
-// The scores of a cache's tokens: an array beside it, and its strides.
-int check_scores(const float* scores, int64_t page_stride, int64_t token_stride,
-                 int64_t head_stride) {
+// The scores of a cache's tokens: an array beside it, and its strides. They move, so
+// they may not share memory.
+int check_scores(const KvCacheView& c, const float* scores, int64_t page_stride,
+                 int64_t token_stride, int64_t head_stride) {
   if (scores == nullptr) return fail(B200_ERR_INVALID, "null pointer argument");
   if (!aligned(scores, 4)) return fail(B200_ERR_INVALID, "scores must be 4-byte aligned");
   if (page_stride < 0 || token_stride < 0 || head_stride < 0)
     return fail(B200_ERR_INVALID, "negative strides");
+  if (!apart3(page_stride, c.num_pages, token_stride, c.page_size, head_stride, c.heads, 1))
+    return fail(B200_ERR_INVALID, "the scores overlap");
   return B200_OK;
 }
 
@@ -125,11 +130,15 @@ int b200_kv_cache_evict(const b200_kv_cache* cache, float* scores, int64_t score
                 budget, first, recent);
   if ((int64_t)seqs * cache->kv_heads * 8 > 0x7fffffffll)
     return fail(B200_ERR_UNSUPPORTED, "more than 2^28 rows in one call");
-  // (the grid's second dimension counts the kept tokens)
-  if (budget > 65535 * 64)
-    return fail(B200_ERR_UNSUPPORTED, "the budget is at most %d tokens, got %d", 65535 * 64, budget);
   if (seqs == 0) return B200_OK;
-  if ((rc = check_scores(scores, score_page_stride, score_token_stride, score_head_stride))) return rc;
+  if ((rc = check_scores(l.c, scores, score_page_stride, score_token_stride, score_head_stride)))
+    return rc;
+  if (!apart3(l.c.page_stride, l.c.num_pages, l.c.token_stride, l.c.page_size, l.c.head_stride,
+              l.c.heads, l.c.head_dim) ||
+      (l.c.k_scale != nullptr &&
+       !apart3(l.c.scale_page_stride, l.c.num_pages, l.c.scale_token_stride, l.c.page_size,
+               l.c.scale_head_stride, l.c.heads, 1)))
+    return fail(B200_ERR_INVALID, "the cache's vectors overlap");
   if (kv_lens == nullptr || kept == nullptr || lens == nullptr ||
       (page_table_width > 0 && page_table == nullptr))
     return fail(B200_ERR_INVALID, "null pointer argument");
@@ -140,6 +149,10 @@ int b200_kv_cache_evict(const b200_kv_cache* cache, float* scores, int64_t score
     return fail(B200_ERR_INVALID, "negative strides");
   const int64_t most = (int64_t)page_table_width * cache->page_size;
   if (most > 0x7fffffffll) return fail(B200_ERR_UNSUPPORTED, "a table of more than 2^31 - 1 tokens");
+  // (the grid's second dimension counts the kept tokens that there can be)
+  if (std::min<int64_t>(budget, most) > 65535 * 64)
+    return fail(B200_ERR_UNSUPPORTED, "at most %d tokens stay, got a budget of %d of %lld", 65535 * 64,
+                budget, (long long)most);
   if (out_table == page_table && out_table_stride == page_table_stride) out_table = nullptr;
   if (out_table != nullptr &&
       (int64_t)out_table_width * cache->page_size < (budget < most ? budget : most))

@@ -460,7 +460,9 @@ cudaError_t launch_kv_evict(const EvictLaunch& l, cudaStream_t stream) {
   if (err != cudaSuccess) return err;
   const int chunks = l.c.head_dim * (l.c.k_scale != nullptr ? 1 : 2) / 16;
   if (l.out_table != nullptr) {
-    const dim3 grid((unsigned)pairs, (unsigned)((l.budget + kMoveTokens - 1) / kMoveTokens));
+    const long long stay = std::min<long long>(l.budget, most);
+    if (stay == 0) return cudaSuccess;  // a table without pages
+    const dim3 grid((unsigned)pairs, (unsigned)((stay + kMoveTokens - 1) / kMoveTokens));
     switch (chunks) {
       case 4: return launch_pdl(evict_move_kernel<4>, grid, dim3(kMoveThreads), 0, stream, p);
       case 8: return launch_pdl(evict_move_kernel<8>, grid, dim3(kMoveThreads), 0, stream, p);

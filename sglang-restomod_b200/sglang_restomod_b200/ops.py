@@ -1044,9 +1044,10 @@ def reserve_attention_workspace(head_dim: int, q_tokens: int, seqs: int,
 
 
 def attention_status(device: torch.device | None = None, reset: bool = True) -> int:
-    """Error bits of a device's norm and attention calls, those replayed from graphs
-    included (0 = none, 1 = a wait gave up, 16 = a page number outside the cache,
-    32 = a chunk met a scale byte outside 103 .. 134). Synchronizes the device."""
+    """Error bits of a device's norm, attention, integer linear, score and eviction
+    calls, those replayed from graphs included (0 = none, 1 = a wait gave up, 16 = a
+    page number outside the cache, 32 = a chunk met a scale byte outside 103 .. 134).
+    Synchronizes the device."""
     index = torch.cuda.current_device() if device is None or device.index is None else device.index
     torch.cuda.synchronize(index)
     bits = ctypes.c_int32(0)
@@ -1226,8 +1227,8 @@ def kv_cache_scores(q: torch.Tensor, cache, page_table: torch.Tensor, kv_lens: t
     Call it after the attention call, with its arguments and its log-sum-exp ``lse``.
     ``scores`` fp32 ``[pages, page_size, kv_heads]``, any strides
     (:meth:`~.kv_cache.PagedKVCache.empty_scores`); ``out``, by default ``scores``
-    itself, takes the new values. No two sequences may have a page in common. The
-    result does not depend on timing. Returns ``out``."""
+    itself, takes the new values. No page may stand twice among those of the call's
+    tokens. The result does not depend on timing. Returns ``out``."""
     index = _on_device("kv_cache_scores", q, cache.k, page_table, kv_lens, q_starts, lse, scores,
                        out, workspace)
     code, tokens, heads, dim, seqs, _ = _attention_args(q, cache, page_table, kv_lens, q_starts, q)
@@ -1268,7 +1269,7 @@ def kv_cache_evict(cache, scores: torch.Tensor, page_table: torch.Tensor, kv_len
     lowest index). Heads choose by themselves; the kept tokens stay in order.
 
     Without ``out_table`` they move to the front of the sequence's own pages, keys,
-    values, scales and scores, in place; no two sequences may have a page in common.
+    values, scales and scores, in place; no page may stand twice among those tokens' pages.
     With it (int32 ``[seqs, pages]``, pages that hold none of the sequences' tokens)
     they are copied there, and the source stays.
 

@@ -76,6 +76,18 @@ def fp8_bank(experts: int, n: int, k: int, device, seed: int, first_expert: int 
     return q, s
 
 
+def int8_bank(experts: int, n: int, k: int, device, seed: int, first_expert: int = 0):
+    """(int8 [E, N, K], fp32 scales [E, N]): each row's largest element is 127."""
+    q = torch.empty(experts, n, k, dtype=torch.int8, device=device)
+    s = torch.empty(experts, n, dtype=torch.float32, device=device)
+    for e in range(experts):
+        g = _expert_gen(device, seed, first_expert + e)
+        w = torch.randn(n, k, generator=g, device=device) * WEIGHT_STD
+        s[e] = w.abs().amax(1) / 127
+        q[e] = (w / s[e][:, None]).round().clamp(-127, 127).to(torch.int8)
+    return q, s
+
+
 def nvfp4_bank(experts: int, n: int, k: int, device, seed: int, first_expert: int = 0):
     """(packed uint8 [E, N, K/2], e4m3 [E, N, K/16], fp32 global [E])."""
     p = torch.empty(experts, n, k // 2, dtype=torch.uint8, device=device)
