@@ -96,7 +96,8 @@ struct ChoiceSmem {
   uint32_t hist[kBins];   // of this block
   alignas(16) uint32_t total[2][kBins];  // of the cluster, in its first block; steps in turn
   uint32_t sums[kWarps];  // scan
-  uint32_t bin, left;     // the step's result
+  uint32_t bin, left;     // the step's result,
+  uint32_t whole;         // and whether all of the bin stay
   uint32_t counts[2];     // this block's kept ones above the border, and equals of it
   uint32_t warp_above[kWarps], warp_equal[kWarps];
 };
@@ -139,38 +140,33 @@ __global__ void __launch_bounds__(kThreads, 2) evict_choose_kernel(const EvictPa
   const float* scores = e.scores + head * e.score_head_stride;
   const int* table = e.table + seq * e.table_stride;
   bool bad = false;
-  auto score_of = [&](int t, int page) -> uint32_t {
-    if (t < lo || t >= hi) return 0xffffffffu;
+  // (no page of the cache: the lowest score, as NaN has)
+  auto score_of = [&](int t, int page) {
     if (page < 0 || page >= e.c.num_pages) {
       bad = true;
-      return 0u;
+      return __uint_as_float(0x7fffffffu);
     }
     const int offset = t - p.by_page.of(t) * e.c.page_size;
-    return __float_as_uint(scores[page * e.score_page_stride + offset * e.score_token_stride]);
+    return scores[page * e.score_page_stride + offset * e.score_token_stride];
   };
-  auto rank_at = [&](int t, uint32_t score, int page) {
-    return t < lo || t >= hi || page < 0 || page >= e.c.num_pages ? score
-                                                                   : rank_of(__uint_as_float(score));
+  auto rank_at = [&](int t, float score) {
+    return (uint32_t)(t - lo) < (uint32_t)(hi - lo) ? rank_of(score) : 0xffffffffu;
   };
-  auto read = [&](int t) -> uint32_t {
-    const int page = __ldg(table + p.by_page.of(t));
-    return rank_at(t, score_of(t, page), page);
-  };
+  auto read = [&](int t) { return rank_at(t, score_of(t, __ldg(table + p.by_page.of(t)))); };
   // (all page numbers, then all scores: one after the other a token cost two latencies)
   uint32_t keys[KEYS];
-  int pages[KEYS];
 #pragma unroll
   for (int i = 0; i < KEYS; ++i) {
     const int t = w0 + 32 * i + lane;
-    pages[i] = t < w1 ? __ldg(table + p.by_page.of(t)) : 0;
+    keys[i] = t < w1 ? (uint32_t)__ldg(table + p.by_page.of(t)) : 0u;
   }
 #pragma unroll
   for (int i = 0; i < KEYS; ++i) {
     const int t = w0 + 32 * i + lane;
-    keys[i] = t < w1 ? score_of(t, pages[i]) : 0u;
+    keys[i] = t < w1 ? __float_as_uint(score_of(t, (int)keys[i])) : 0u;
   }
 #pragma unroll
-  for (int i = 0; i < KEYS; ++i) keys[i] = rank_at(w0 + 32 * i + lane, keys[i], pages[i]);
+  for (int i = 0; i < KEYS; ++i) keys[i] = rank_at(w0 + 32 * i + lane, __uint_as_float(keys[i]));
   // f(token, its rank, whether there is one) for the lane's tokens
   auto each = [&](auto&& f) {
 #pragma unroll
@@ -232,6 +228,7 @@ __global__ void __launch_bounds__(kThreads, 2) evict_choose_kernel(const EvictPa
       if (above < need && above + count[k] >= need) {
         sm.bin = kBins - 1 - (4 * tid + k);
         sm.left = need - above;
+        sm.whole = above + count[k] == need;
       }
       above += count[k];
     }
@@ -241,12 +238,17 @@ __global__ void __launch_bounds__(kThreads, 2) evict_choose_kernel(const EvictPa
       __syncthreads();
     border |= sm.bin << shift;
     need = sm.left;
+    if (sm.whole) {  // all from here up: no more digits (the rank below is none of these)
+      --border;
+      need = 0;
+      break;
+    }
   }
   // Kept: ranks above the border, and the first `need` equals of it.
   uint32_t mine = 0, even = 0;
   each([&](int, uint32_t v, bool on) {
     mine += on && v > border;
-    even += on && v == border;
+    even += on && need && v == border;
   });
   mine = __reduce_add_sync(0xffffffffu, mine);
   even = __reduce_add_sync(0xffffffffu, even);
@@ -272,7 +274,7 @@ __global__ void __launch_bounds__(kThreads, 2) evict_choose_kernel(const EvictPa
   }
   const uint32_t below = (1u << lane) - 1u;
   each([&](int t, uint32_t v, bool on) {
-    const bool up = on && v > border, eq = on && v == border;
+    const bool up = on && v > border, eq = on && need && v == border;
     const uint32_t ups = __ballot_sync(0xffffffffu, up), eqs = __ballot_sync(0xffffffffu, eq);
     const uint32_t eq_rank = before_equal + __popc(eqs & below);
     if (up || (eq && eq_rank < need)) kept[before + __popc(ups & below) + min(eq_rank, need)] = t;
