@@ -1288,8 +1288,9 @@ def kv_cache_evict(cache, scores: torch.Tensor, page_table: torch.Tensor, kv_len
         if out_table.dim() != 2 or out_table.shape[0] != seqs:
             raise ValueError(f"out_table must be [{seqs}, pages], got {tuple(out_table.shape)}")
         to = (out_table.data_ptr(), out_table.stride(0), out_table.shape[1])
-    if not 0 < budget < 1 << 31:
-        raise ValueError(f"the budget must be a positive int32, got {budget}")
+    if not 0 < budget < 1 << 31 or recent < 0 or first < 0 or recent + first > budget:
+        raise ValueError(f"the budget must be a positive int32 and hold the first and recent tokens, "
+                         f"got {budget}, {first}, {recent}")
     kept = torch.empty(seqs, cache.kv_heads, budget, dtype=torch.int32, device=scores.device)
     lens = torch.empty(seqs, dtype=torch.int32, device=scores.device)
     _lib.check(lib().b200_kv_cache_evict(

@@ -340,3 +340,5 @@ def test_wrappers_refuse_shapes_and_types(monkeypatch):
     refused(ValueError, "out_table must be", evict(out_table=table[:2]))
     for budget in (0, -1, 1 << 31):
         refused(ValueError, "budget", evict(budget=budget))
+    for kept in (dict(recent=-1), dict(first=-1), dict(recent=1, first=2), dict(recent=1 << 32)):
+        refused(ValueError, "budget", evict(**kept))
