@@ -108,7 +108,7 @@ struct PrefillParams {
   int4* units;      // sequence, first token in it, first key, key tiles
   long long* unit_at;  // place of each unit's first cost (nullptr: not wanted)
   int max_units;
-  int min_tiles;       // work that a block takes at least
+  int min_tiles;       // work that a block takes at least, with shared prefixes
   int plan_only, planned;  // (host) launch the plan alone, or all but it
   float* parts;
   // tensor copies: rows of a page that one copy takes (a power of two that
@@ -358,9 +358,13 @@ struct SeqLens {
   int q0, q_len, kv_len;
   int pos0;  // position of the first new token
 };
+// SHARED: a pass of a call with shared prefixes (groups for sequences, rows in fp32).
+// (Decided at run time it cost calls without: a chunk of 512 on 16384 166 us, so 158.)
+template <bool SHARED>
 __device__ __forceinline__ SeqLens seq_lens(const AttnLaunch& a, int s) {
   SeqLens r;
-  const int q0 = a.q_start(s), q1 = a.q_start(s + 1);
+  const int q0 = SHARED ? a.q_start(s) : __ldg(a.q_starts + s);
+  const int q1 = SHARED ? a.q_start(s + 1) : __ldg(a.q_starts + s + 1);
   const long long cap = (long long)a.table_width * a.c.page_size;
   int kv = max(__ldg(a.kv_lens + s), 0);
   if (kv > cap) kv = (int)cap;
@@ -406,6 +410,7 @@ __device__ long long block_scan(long long v, long long* sh, long long& total) {
 // ranges, and where in the flattened (unit, head, cost) space each block of the
 // attention kernel starts. A unit's first kUnitCost places stand for its
 // constant cost, the others for one key tile each.
+template <bool SHARED>
 __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const PrefillParams p,
                                                                  int unit_tokens, int bn,
                                                                  int max_ctas) {
@@ -417,19 +422,19 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const PrefillPa
   int* seq_base = p.a.seqs <= kPlanSeqs ? base_sh : p.seq_base;
   const AttnLaunch& a = p.a;
   // (see AttnLaunch::beside)
-  if (!a.beside) griddep_wait();
-  if (p.unit_at != nullptr) griddep_launch_dependents();
+  if (!(SHARED && a.beside)) griddep_wait();
+  if (SHARED && p.unit_at != nullptr) griddep_launch_dependents();
   const int tid = threadIdx.x;
   long long total_units, total;
   {
     const int per = (a.seqs + kPlanThreads - 1) / kPlanThreads;
     const int s0 = min(tid * per, a.seqs), s1 = min(s0 + per, a.seqs);
     long long n = 0;
-    for (int s = s0; s < s1; ++s) n += (seq_lens(a, s).q_len + unit_tokens - 1) / unit_tokens;
+    for (int s = s0; s < s1; ++s) n += (seq_lens<SHARED>(a, s).q_len + unit_tokens - 1) / unit_tokens;
     long long base = block_scan(n, sh, total_units);
     for (int s = s0; s < s1; ++s) {
       seq_base[s] = (int)base;
-      base += (seq_lens(a, s).q_len + unit_tokens - 1) / unit_tokens;
+      base += (seq_lens<SHARED>(a, s).q_len + unit_tokens - 1) / unit_tokens;
     }
     if (tid == 0) seq_base[a.seqs] = (int)total_units;
   }
@@ -449,9 +454,9 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const PrefillPa
         hi = mid - 1;
     }
     int s = lo;
-    SeqLens q = seq_lens(a, s);
+    SeqLens q = seq_lens<SHARED>(a, s);
     for (int u = u0; u < u1; ++u) {
-      while (s + 1 < a.seqs && seq_base[s + 1] <= u) q = seq_lens(a, ++s);
+      while (s + 1 < a.seqs && seq_base[s + 1] <= u) q = seq_lens<SHARED>(a, ++s);
       const int tok0 = (u - seq_base[s]) * unit_tokens;
       const int last = min(tok0 + unit_tokens, q.q_len) - 1;
       int end = a.causal ? min(q.kv_len, q.pos0 + last + 1) : q.kv_len;
@@ -459,15 +464,16 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const PrefillPa
       begin -= begin % p.box_rows;
       const int tiles = end > begin ? (end - begin + bn - 1) / bn : 1;
       p.units[u] = make_int4(s, tok0, begin, tiles);
-      if (p.unit_at != nullptr) p.unit_at[u] = mine;  // (from unit u0; see below)
+      if (SHARED && p.unit_at != nullptr) p.unit_at[u] = mine;  // (from unit u0; see below)
       mine += (long long)(tiles + kUnitCost) * a.c.heads;
     }
   }
   const long long at = block_scan(mine, sh, total);
   at_sh[tid] = at;  // of unit u0; `total` where the thread has none
-  if (p.unit_at != nullptr)
+  if (SHARED && p.unit_at != nullptr)
     for (int u = u0; u < u1; ++u) p.unit_at[u] += at;
-  long long ctas = (total + p.min_tiles - 1) / p.min_tiles;
+  const int min_tiles = SHARED ? p.min_tiles : kMinTiles;
+  long long ctas = (total + min_tiles - 1) / min_tiles;
   if (ctas > max_ctas) ctas = max_ctas;
   if (tid == 0) {
     p.head[0] = total;
@@ -498,7 +504,7 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(const PrefillPa
     const int h = (int)(x / cost);
     p.start[c] = make_int4(u, h, (int)(x - (long long)h * cost), 0);
   }
-  if (a.beside) griddep_wait();
+  if (SHARED && a.beside) griddep_wait();
   griddep_launch_dependents();
 }
 
@@ -700,6 +706,7 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
 // 40 tokens on 8192, 8 heads, 59 to 32; 512 on 16384, e4m3, 176 to 166; where
 // little is cut it costs 1 to 2 us of 55.)
 constexpr int kCombineCols = 16;
+template <bool SHARED>
 __global__ void __launch_bounds__(128) attn_combine_kernel(const PrefillParams p, int d, int mt) {
   griddep_wait();
   const AttnLaunch& a = p.a;
@@ -713,7 +720,7 @@ __global__ void __launch_bounds__(128) attn_combine_kernel(const PrefillParams p
   if (t1 - t0 < cost - s.z) return;  // the pair goes on
   const int groups = d / kCombineCols, tile = blockIdx.y / groups;
   const int col = blockIdx.y % groups * kCombineCols, row = threadIdx.x;
-  const SeqLens q = seq_lens(a, u.x);
+  const SeqLens q = seq_lens<SHARED>(a, u.x);
   const int tok = u.y + tile * p.tile_tokens + row / p.groups;
   if (row >= p.tile_tokens * p.groups || tok >= q.q_len) return;
   // the block that holds the pair's first key tile
@@ -750,7 +757,7 @@ __global__ void __launch_bounds__(128) attn_combine_kernel(const PrefillParams p
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const long long token = (long long)q.q0 + tok;
   const int qh = s.y * p.groups + row % p.groups;
-  if (a.out32 != nullptr) {
+  if (SHARED) {
     float* out = a.out32 + (token * a.q_heads + qh) * d + col;
 #pragma unroll
     for (int i = 0; i < kCombineCols; i += 4)
@@ -804,7 +811,7 @@ __global__ void __launch_bounds__(128) attn_prefix_finish_kernel(const PrefillPa
     const int unit = (int)(pair / a.c.heads), head = (int)(pair % a.c.heads);
     const int4 u = __ldcg(p.units + unit);
     const long long place = __ldcg(p.unit_at + unit);
-    const SeqLens q = seq_lens(a, u.x);
+    const SeqLens q = seq_lens<true>(a, u.x);
     const int tok = u.y + tile * p.tile_tokens + row / p.groups;
     if (row >= p.tile_tokens * p.groups || tok >= q.q_len) continue;
     const long long token = (long long)q.q0 + tok;
@@ -884,7 +891,7 @@ __global__ void __launch_bounds__(128) attn_prefix_finish_kernel(const PrefillPa
   griddep_wait();  // (the end of this kernel is the end of the call)
 }
 
-template <int D, int MT, int KV, bool TMA>
+template <int D, int MT, int KV, bool TMA, bool SHARED>
 __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
     attn_prefill_kernel(const PrefillParams p, const __grid_constant__ CUtensorMap q_map,
                         const __grid_constant__ CUtensorMap k_map,
@@ -959,7 +966,7 @@ __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
     // of all rows' scales: the passes over S are taken by whole warps
     const bool negative = p.scale_log2 < 0.f;
     while (cur.next(g)) {
-      const SeqLens q = seq_lens(a, g.seq);
+      const SeqLens q = seq_lens<SHARED>(a, g.seq);
       const int tok = g.tok0 + wg * p.tile_tokens + row_token;
       const bool valid = row < p.tile_tokens * p.groups && tok < q.q_len &&
                          tok < g.tok0 + MT * p.tile_tokens;
@@ -1047,7 +1054,6 @@ __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
       const int qh = g.head * p.groups + row_head;
       // 64 bytes of the warp's 32 rows (32 columns, or 16 in fp32), through shared
       // memory so that a store covers 64 neighbouring bytes of each of 8 rows
-      const bool wide = a.out32 != nullptr;
       long long out_at[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -1056,19 +1062,18 @@ __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
         const long long to_token = (long long)q.q0 + t;
         const int to_head = g.head * p.groups + r % p.groups;
         out_at[j] = r < p.tile_tokens * p.groups && t < q.q_len
-                        ? (wide ? (to_token * a.q_heads + to_head) * (D * 4)
-                                : (to_token * a.out_token_stride + to_head * a.out_head_stride) * 2) +
+                        ? (SHARED ? (to_token * a.q_heads + to_head) * (D * 4)
+                                  : (to_token * a.out_token_stride + to_head * a.out_head_stride) * 2) +
                               (lane & 3) * 16
                         : -1;
       }
-      uint8_t* out_base = wide ? reinterpret_cast<uint8_t*>(a.out32) : static_cast<uint8_t*>(a.out);
+      uint8_t* out_base = SHARED ? reinterpret_cast<uint8_t*>(a.out32) : static_cast<uint8_t*>(a.out);
       uint8_t* stage_out = smem + S::kOffOut + warp * 2048;
-      auto emit = [&](int c, const uint32_t (&w)[16]) {
+      auto emit = [&](int c, auto&& piece) {
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          *reinterpret_cast<uint4*>(stage_out + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) =
-              make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+          *reinterpret_cast<uint4*>(stage_out + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) = piece(i);
         __syncwarp();
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -1080,7 +1085,7 @@ __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
       };
       if (whole) {
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        if (wide) {
+        if constexpr (SHARED) {
 #pragma unroll 1
           for (int c = 0; c < D / 16; ++c) {
             uint32_t o[16];
@@ -1088,20 +1093,27 @@ __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
             tmem_wait16(o);
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * inv);
-            emit(c, o);
+            emit(c, [&](int i) {
+              return make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            });
           }
         } else {
 #pragma unroll 1
           for (int c = 0; c < D / 32; ++c) {
-            uint32_t o[32], w[16];
+            uint32_t o[32];
+            float v[32];
             tmem_ld32_nowait(to + 32 * c, o);
             tmem_wait32(o);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float x = __uint_as_float(o[2 * i]) * inv, y = __uint_as_float(o[2 * i + 1]) * inv;
-              w[i] = a.q_f16 ? pack2<true>(x, y) : pack2<false>(x, y);
-            }
-            emit(c, w);
+            for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(o[i]) * inv;
+            emit(c, [&](int i) {
+              uint32_t w[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                w[j] = a.q_f16 ? pack2<true>(v[8 * i + 2 * j], v[8 * i + 2 * j + 1])
+                               : pack2<false>(v[8 * i + 2 * j], v[8 * i + 2 * j + 1]);
+              return make_uint4(w[0], w[1], w[2], w[3]);
+            });
           }
         }
         if (valid && a.lse != nullptr)
@@ -1136,12 +1148,12 @@ __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
       return __ldg(a.table + sg.seq * a.table_stride + p.page_of(token));
     };
     bool more = cur.next(g), run = true;  // run: no wait has given up
-    SeqLens q = seq_lens(a, g.seq);
+    SeqLens q = seq_lens<SHARED>(a, g.seq);
     int page_n = page_of(g, q.kv_len, 0);
     while (more) {
       Segment gn = g;
       const bool more_n = cur.next(gn);
-      const SeqLens qn = more_n ? seq_lens(a, gn.seq) : q;
+      const SeqLens qn = more_n ? seq_lens<SHARED>(a, gn.seq) : q;
       int page = -2, page_before = -2;  // of tile t and t - 1
       auto fill_entry = [&](int t, bool is_v, int pg) {
         if (lane == 0) {
@@ -1269,7 +1281,7 @@ __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
       }
     };
     bool more = cur.next(g);
-    SeqLens q = seq_lens(a, g.seq);
+    SeqLens q = seq_lens<SHARED>(a, g.seq);
     int page2 = page_of(g, q.kv_len, 2);
     Info info0 = info_of(g, q.kv_len, 0, page_of(g, q.kv_len, 0));
     Info info1 = info_of(g, q.kv_len, 1, page_of(g, q.kv_len, 1));
@@ -1283,7 +1295,7 @@ __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
       SeqLens qn = q;
       int page0n = -1, page1n = -1;
       if (more_n) {
-        qn = seq_lens(a, gn.seq);
+        qn = seq_lens<SHARED>(a, gn.seq);
         page0n = page_of(gn, qn.kv_len, 0);
         page1n = page_of(gn, qn.kv_len, 1);
       }
@@ -1471,7 +1483,7 @@ __global__ void __launch_bounds__(Shape<D, MT, KV, TMA>::kThreads, 1)
         }
       };
       while (cur.next(g)) {
-        const SeqLens q = seq_lens(a, g.seq);
+        const SeqLens q = seq_lens<SHARED>(a, g.seq);
         // the first key that any row of the unit sees
         const int lowest = a.window > 0 ? q.pos0 + g.tok0 - a.window + 1 : 0;
         for (int n = 0; n < 2 * g.tiles; ++n) {
@@ -1600,8 +1612,8 @@ long long align256(long long v) { return (v + 255) / 256 * 256; }
 // The most units a call can have, of one token each.
 long long max_units(long long q_tokens, int seqs) { return q_tokens + seqs; }
 
-template <int D, int MT, int KV, bool TMA>
-cudaError_t launch(const PrefillParams& p, const CUtensorMap (&maps)[3], cudaStream_t stream) {
+template <int D, int MT, int KV, bool TMA, bool SHARED>
+cudaError_t launch_as(const PrefillParams& p, const CUtensorMap (&maps)[3], cudaStream_t stream) {
   using S = Shape<D, MT, KV, TMA>;
   static bool configured[64] = {};
   int dev = 0;
@@ -1609,12 +1621,12 @@ cudaError_t launch(const PrefillParams& p, const CUtensorMap (&maps)[3], cudaStr
   if (err != cudaSuccess) return err;
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   if (!configured[dev]) {
-    err = cudaFuncSetAttribute(attn_prefill_kernel<D, MT, KV, TMA>,
+    err = cudaFuncSetAttribute(attn_prefill_kernel<D, MT, KV, TMA, SHARED>,
                                cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem);
     if (err != cudaSuccess) return err;
     if (S::kDeal) {  // the kernel must not ask for more registers than it gets
       cudaFuncAttributes fa;
-      err = cudaFuncGetAttributes(&fa, attn_prefill_kernel<D, MT, KV, TMA>);
+      err = cudaFuncGetAttributes(&fa, attn_prefill_kernel<D, MT, KV, TMA, SHARED>);
       if (err != cudaSuccess) return err;
       if (fa.numRegs * S::kThreads < S::kDealtRegs) return cudaErrorLaunchOutOfResources;
     }
@@ -1624,16 +1636,21 @@ cudaError_t launch(const PrefillParams& p, const CUtensorMap (&maps)[3], cudaStr
   static_assert(sizeof(Ctl) <= 4096, "control block");
   const int sms = device_sm_count();
   if (!p.planned) {
-    err = launch_pdl(attn_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, p,
+    err = launch_pdl(attn_plan_kernel<SHARED>, dim3(1), dim3(kPlanThreads), 0, stream, p,
                      MT * p.tile_tokens, S::kBN, sms);
     if (err != cudaSuccess) return err;
   }
   if (p.plan_only) return cudaSuccess;
-  err = launch_pdl(attn_prefill_kernel<D, MT, KV, TMA>, dim3((unsigned)sms), dim3(S::kThreads),
+  err = launch_pdl(attn_prefill_kernel<D, MT, KV, TMA, SHARED>, dim3((unsigned)sms), dim3(S::kThreads),
                    S::kSmem, stream, p, maps[0], maps[1], maps[2]);
   if (err != cudaSuccess || p.unit_at != nullptr) return err;  // (its parts are added later)
-  return launch_pdl(attn_combine_kernel, dim3((unsigned)sms, MT * (D / kCombineCols)), dim3(128), 0,
-                    stream, p, D, MT);
+  return launch_pdl(attn_combine_kernel<SHARED>, dim3((unsigned)sms, MT * (D / kCombineCols)),
+                    dim3(128), 0, stream, p, D, MT);
+}
+template <int D, int MT, int KV, bool TMA>
+cudaError_t launch(const PrefillParams& p, const CUtensorMap (&maps)[3], cudaStream_t stream) {
+  return p.a.out32 != nullptr ? launch_as<D, MT, KV, TMA, true>(p, maps, stream)
+                              : launch_as<D, MT, KV, TMA, false>(p, maps, stream);
 }
 
 // Tensor maps of q [tokens][heads][D] and of the cache. False where maps cannot

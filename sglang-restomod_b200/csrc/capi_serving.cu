@@ -148,7 +148,7 @@ int b200_kv_cache_evict(const b200_kv_cache* cache, float* scores, int64_t score
   if (page_table_stride < 0 || out_table_stride < 0)
     return fail(B200_ERR_INVALID, "negative strides");
   const int64_t most = (int64_t)page_table_width * cache->page_size;
-  if (most > 0x7fffffffll) return fail(B200_ERR_UNSUPPORTED, "a table of more than 2^31 - 1 tokens");
+  if (most > 0x7fff0000ll) return fail(B200_ERR_UNSUPPORTED, "a table of more than 2^31 - 2^16 tokens");
   // (the grid's second dimension counts the kept tokens that there can be)
   if (std::min<int64_t>(budget, most) > 65535 * 64)
     return fail(B200_ERR_UNSUPPORTED, "at most %d tokens stay, got a budget of %d of %lld", 65535 * 64,
