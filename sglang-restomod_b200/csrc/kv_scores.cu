@@ -21,7 +21,7 @@
 // sixteenths of them: 442, 453, 465, 488 us against 449 for a prompt of 8192 tokens.) Few
 // rows: HBM, each key once. Measured: that prompt, 8 x 4 heads of 128, 449 us (the
 // exponentials alone 240 at 1.9 GHz, the products 165 at the measured bf16 rate); 16 chunks of up to
-// 300 f16 tokens on up to 4096 single-token pages, window 1000, 8 x 3 heads of 64, 96.
+// 300 f16 tokens on up to 4096 single-token pages, window 1000, 8 x 3 heads of 64, 66.
 //
 // e4m3 keys go to the tensor cores as they are (kind::f8f6f4): a query is brought
 // into [128, 256) by a power of two and split into e4m3 terms, q = t1 + (t2 + t3) / 32,
@@ -34,8 +34,9 @@
 // and 8-15 epilogue of an item's first and second 128 tokens, four of the eight for
 // the even 32 columns of a tile and four for the odd, 16 the items and copies of Q, 17
 // and 18 products of either half, 19 tensor copies of keys, 20 and 21 the tokens of
-// either half (page, old score, scale, place of the new score; where pages are no
-// multiple of 8 tokens also the copies of their keys, 16 bytes at a time).
+// either half (page, old score, scale, place of the new score). Where pages are no
+// multiple of 8 tokens warps 19 to 26 have the tokens, four a half, and copy their keys
+// too, 16 bytes at a time (one a half: the chunks above took 96 us, two 72).
 //
 // While products read their operands from shared memory everything else there is
 // slow: a wait on a barrier that is long complete takes 300 clocks, and a tile of 128 x
@@ -60,8 +61,15 @@ constexpr float kLog2e = 1.4426950408889634f;
 // A hidden column is an infinity that factors multiply, so a factor of zero becomes the
 // smallest normal number: finite products still come to e^0.
 constexpr float kMinScale = 1.1754944e-38f;
-constexpr int kEpiWarps = 16, kQWarp = 16, kMmaWarp = 17, kKeyWarp = 19, kTokenWarp = 20;
-constexpr int kThreads = 22 * 32;
+constexpr int kEpiWarps = 16, kQWarp = 16, kMmaWarp = 17, kKeyWarp = 19;
+// The tokens' warps of a half: one, or where these copy the keys too four, a quarter of
+// the half's tokens each.
+template <bool TMA>
+struct Roles {
+  static constexpr int kSplit = TMA ? 1 : 4;
+  static constexpr int kTokenWarp = TMA ? 20 : 19;
+  static constexpr int kThreads = (kTokenWarp + 2 * kSplit) * 32;
+};
 constexpr int kUnit = 256;       // tokens of an item: two tiles of 128
 constexpr int kMaxKeys = 12, kMaxQ = 4, kItems = 4, kTokens = 2;
 constexpr int kScan = 256;       // threads that share out the sequences
@@ -349,9 +357,11 @@ struct __align__(16) Token {
 };
 
 template <bool Q8, bool TMA>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Roles<TMA>::kThreads, 1)
     kv_scores_kernel(const ScoreParams p, const __grid_constant__ CUtensorMap q_map,
                      const __grid_constant__ CUtensorMap k_map) {
+  using R = Roles<TMA>;
+  constexpr int kSplit = R::kSplit, kTokenWarp = R::kTokenWarp, kThreads = R::kThreads;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t keys_at = smem_u32(smem);
@@ -369,7 +379,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (tid == 0) {
     for (int i = 0; i < kMaxKeys; ++i) {
-      mbar_init(&ctl->key_full[i], TMA ? 1 : 32);
+      mbar_init(&ctl->key_full[i], TMA ? 1 : 32 * kSplit);
       mbar_init(&ctl->key_empty[i], 1);
     }
     for (int i = 0; i < kMaxQ; ++i) {
@@ -384,10 +394,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < kItems; ++i) {
       mbar_init(&ctl->item_full[i], 1);
-      mbar_init(&ctl->item_empty[i], kEpiWarps + 4 + (TMA ? 1 : 0));
+      mbar_init(&ctl->item_empty[i], kEpiWarps + 2 + 2 * kSplit + (TMA ? 1 : 0));
     }
     for (int i = 0; i < 2 * kTokens; ++i) {
-      mbar_init(&ctl->token_full[i], 1);
+      mbar_init(&ctl->token_full[i], kSplit);
       mbar_init(&ctl->token_empty[i], kEpiWarps / 2);
     }
     for (int i = 0; i < 2; ++i) mbar_init(&ctl->drained[i], 1);
@@ -696,9 +706,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!mbar_wait(&ctl->drained[half], 0, static_cast<int*>(nullptr))) ctl->abort = 1;
     }
     __syncwarp();
-  } else if (warp == kTokenWarp || warp == kTokenWarp + 1) {
+  } else if (warp >= kTokenWarp) {
     // ------------------------------------------------------------- the tokens
-    const int half = warp - kTokenWarp;
+    constexpr int kPer = 4 / kSplit;  // tokens of a lane
+    const int half = (warp - kTokenWarp) / kSplit;
+    const int first = (warp - kTokenWarp) % kSplit * kPer * 32 + lane;  // of the half's tokens
     Items items{ctl};
     Item it;
     uint32_t tokens = 0, used = 0;  // items, and K tiles that some row needs, so far
@@ -709,21 +721,21 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool seen = it.first < it.last && key0 < it.kv_len;
       const uint32_t tile = used + half;  // (a first half always has tokens)
       if (it.first < it.last) used += it.key0 + 128 < it.kv_len ? 2 : 1;
-      int page[4], at[4];
+      int page[kPer], at[kPer];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int key = key0 + lane + 32 * k, i = p.page_of(key);
+      for (int k = 0; k < kPer; ++k) {
+        const int key = key0 + first + 32 * k, i = p.page_of(key);
         at[k] = key - i * a.c.page_size;
         page[k] = key < it.kv_len ? __ldg(a.table + it.seq * a.table_stride + i) : -2;
       }
-      float old[4];
-      uint32_t scale[4];
-      long long out_at[4];
+      float old[kPer];
+      uint32_t scale[kPer];
+      long long out_at[kPer];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < kPer; ++k) {
         const bool good = page[k] >= 0 && page[k] < a.c.num_pages;
         if (!good && page[k] != -2) atomicOr(&ctl->errors, kDevBadPage);
-        const bool fresh = a.causal && key0 + lane + 32 * k >= it.pos0;
+        const bool fresh = a.causal && key0 + first + 32 * k >= it.pos0;
         old[k] = 0.f;
         if (good && !fresh)
           old[k] = p.scores_in[page[k] * p.in_page + at[k] * p.in_token + it.head * p.in_head];
@@ -741,12 +753,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) break;
       ++tokens;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < kPer; ++k) {
         Token to;
         to.old = old[k];
         to.key_scale = scale[k] == 255u ? __int_as_float(0x7fc00000) : __uint_as_float(scale[k] << 23);
         to.out_at = out_at[k];
-        token_sh[slot * 128 + lane + 32 * k] = to;
+        token_sh[slot * 128 + first + 32 * k] = to;
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&ctl->token_full[slot]);
@@ -759,14 +771,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int slice_chunks = p.row_bytes / 16, chunk = lane % chunks;
         const int sl = chunk / slice_chunks, c = chunk % slice_chunks;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < kPer; ++k) {
           const long long off = page[k] >= 0 && page[k] < a.c.num_pages
                                     ? (page[k] * a.c.page_stride + at[k] * a.c.token_stride +
                                        it.head * a.c.head_stride) * kElem
                                     : -1;
 #pragma unroll 4
           for (int j = 0; j < chunks; ++j) {
-            const int r32 = j * per_pass + lane / chunks, r = 32 * k + r32;
+            const int r32 = j * per_pass + lane / chunks, r = first - lane + 32 * k + r32;
             const long long o = __shfl_sync(0xffffffffu, off, r32);
             const uint32_t x = (uint32_t)c ^ (p.row_bytes == 128 ? r & 7 : r >> 1 & 3);
             if (o >= 0)
@@ -904,7 +916,7 @@ cudaError_t launch(const ScoreParams& p, size_t smem, const CUtensorMap& q_map,
     configured[dev] = true;
   }
   return launch_pdl(kv_scores_kernel<Q8, TMA>, dim3((unsigned)device_sm_count()),
-                    dim3(kThreads), smem, stream, p, q_map, k_map);
+                    dim3(Roles<TMA>::kThreads), smem, stream, p, q_map, k_map);
 }
 
 }  // namespace
