@@ -91,7 +91,7 @@ struct ScoreParams {
   int f16;                // operand type of a 16-bit cache
   int nq, tile_tokens;    // rows of a Q tile, and the tokens that fill them
   int terms;              // e4m3
-  int key_stages, q_stages, key_bytes, q_bytes;
+  int key_stages, q_stages, key_bytes, q_bytes;  // (key stages of each half)
   int row_bytes, slices;  // of a slice of a vector (128, or 64), and how many it has
   int box_rows, heads_first;
   Divisor by_page, by_tile;  // of the page size, of tile_tokens
@@ -365,8 +365,8 @@ __global__ void __launch_bounds__(Roles<TMA>::kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t keys_at = smem_u32(smem);
-  const uint32_t q_at = keys_at + p.key_stages * p.key_bytes;
-  uint8_t* after = smem + p.key_stages * p.key_bytes + p.q_stages * p.q_bytes;
+  const uint32_t q_at = keys_at + 2 * p.key_stages * p.key_bytes;
+  uint8_t* after = smem + 2 * p.key_stages * p.key_bytes + p.q_stages * p.q_bytes;
   // Of a Q tile's rows, a warp its own: -lse in log2, and (e4m3) from 64 on the row's
   // factor.
   float* row_sh = reinterpret_cast<float*>(after);
@@ -413,7 +413,7 @@ __global__ void __launch_bounds__(Roles<TMA>::kThreads, 1)
   }
   // Rows of a Q tile that no copy fills stay zeros.
   for (int i = tid * 16; i < p.q_stages * p.q_bytes; i += kThreads * 16)
-    *reinterpret_cast<uint4*>(smem + p.key_stages * p.key_bytes + i) = make_uint4(0u, 0u, 0u, 0u);
+    *reinterpret_cast<uint4*>(smem + 2 * p.key_stages * p.key_bytes + i) = make_uint4(0u, 0u, 0u, 0u);
   fence_async_smem();
   griddep_wait();
 
@@ -447,7 +447,13 @@ __global__ void __launch_bounds__(Roles<TMA>::kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&ctl->tmem);
   const int rows = p.tile_tokens * p.groups;  // of a full Q tile
-  uint32_t keys_copied = 0, q_copied = 0;     // stages whose copies were issued
+  uint32_t keys_copied = 0, q_copied = 0;     // stages whose copies were issued; of the second
+  uint32_t keys_copied1 = 0;                  // half's keys
+  // The n-th K tile of a half. (Each half has a ring of its own: its products are taken by a
+  // thread of its own, and of a ring's barriers every phase must be waited for by whoever
+  // waits for one. In a ring for both, a half that was ahead took the phase before the
+  // one that it waited for, of the other half's keys, for its own.)
+  auto key_stage = [&](int half, uint32_t n) { return half * p.key_stages + n % p.key_stages; };
 
   if (warp < kEpiWarps) {
     // ------------------------------------------------------------ epilogue
@@ -663,7 +669,7 @@ __global__ void __launch_bounds__(Roles<TMA>::kThreads, 1)
     if (elect_one()) {
       Items items{ctl};
       Item it;
-      uint32_t key_n = half, q_n = 0, count = 0;  // K stage, Q tiles, S tiles
+      uint32_t key_n = 0, q_n = 0, count = 0;  // K tiles, Q tiles, S tiles
       bool ok = true;
       const uint32_t type = Q8 ? 0u : p.f16 ? 0u : 1u;
       const uint32_t id_all = instr_desc(type, Q8 ? 2 * p.nq : p.nq), id_one = instr_desc(type, p.nq);
@@ -672,7 +678,7 @@ __global__ void __launch_bounds__(Roles<TMA>::kThreads, 1)
       while (ok && items.next_alone(it)) {
         if (it.first == it.last) continue;
         const bool two = it.key0 + 128 < it.kv_len, mine = half == 0 || two;
-        const uint32_t ks = key_n % p.key_stages, ka = k_desc + (ks * p.key_bytes >> 4);
+        const uint32_t ks = key_stage(half, key_n), ka = k_desc + (ks * p.key_bytes >> 4);
         if (mine) {
           ok = wait_one(&ctl->key_full[ks], key_n / p.key_stages & 1u, ctl);
           if (!TMA) fence_async_smem();
@@ -699,7 +705,7 @@ __global__ void __launch_bounds__(Roles<TMA>::kThreads, 1)
           mma_commit(&ctl->q_empty[qs]);
         }
         if (ok && mine) mma_commit(&ctl->key_empty[ks]);
-        key_n += two ? 2 : 1;
+        key_n += mine;
       }
       // Everything issued has finished before the block gives its memories back.
       mma_commit(&ctl->drained[half]);
@@ -713,14 +719,14 @@ __global__ void __launch_bounds__(Roles<TMA>::kThreads, 1)
     const int first = (warp - kTokenWarp) % kSplit * kPer * 32 + lane;  // of the half's tokens
     Items items{ctl};
     Item it;
-    uint32_t tokens = 0, used = 0;  // items, and K tiles that some row needs, so far
+    uint32_t tokens = 0, used = 0;  // items, and K tiles of the half that some row needs, so far
     bool ok = true;
     constexpr int kElem = Q8 ? 1 : 2;
     while (ok && items.next(it, lane)) {
       const int key0 = it.key0 + 128 * half;
       const bool seen = it.first < it.last && key0 < it.kv_len;
-      const uint32_t tile = used + half;  // (a first half always has tokens)
-      if (it.first < it.last) used += it.key0 + 128 < it.kv_len ? 2 : 1;
+      const uint32_t tile = used;
+      used += seen;
       int page[kPer], at[kPer];
 #pragma unroll
       for (int k = 0; k < kPer; ++k) {
@@ -764,7 +770,7 @@ __global__ void __launch_bounds__(Roles<TMA>::kThreads, 1)
       if (lane == 0) mbar_arrive(&ctl->token_full[slot]);
       if (!TMA && seen) {
         // the tile's keys, 16 bytes a lane, the pieces of a row by neighbouring lanes
-        const uint32_t stage = tile % p.key_stages;
+        const uint32_t stage = key_stage(half, tile);
         ok = wait_warp(&ctl->key_empty[stage], (tile / p.key_stages & 1u) ^ 1u, ctl);
         if (!ok) break;
         const int chunks = a.c.head_dim * kElem / 16, per_pass = 32 / chunks;
@@ -809,12 +815,12 @@ __global__ void __launch_bounds__(Roles<TMA>::kThreads, 1)
       if (page < 0 || page >= a.c.num_pages) page = (int)a.c.num_pages, at = 0;
       const int halves = it.key0 + 128 < it.kv_len ? 2 : 1;
       for (int h = 0; h < halves && ok; ++h) {
-        const uint32_t s = keys_copied % p.key_stages;
-        ok = wait_warp(&ctl->key_empty[s], (keys_copied / p.key_stages & 1u) ^ 1u, ctl);
+        const uint32_t n = h ? keys_copied1 : keys_copied, s = key_stage(h, n);
+        ok = wait_warp(&ctl->key_empty[s], (n / p.key_stages & 1u) ^ 1u, ctl);
         if (!ok) break;
         if (lane == 0) mbar_arrive_expect_tx(&ctl->key_full[s], p.key_bytes);
         __syncwarp();
-        ++keys_copied;
+        ++(h ? keys_copied1 : keys_copied);
         if (half == h && box < boxes) {
           const int per_slice = p.row_bytes / (Q8 ? 1 : 2);
 #pragma unroll 1
@@ -832,8 +838,11 @@ __global__ void __launch_bounds__(Roles<TMA>::kThreads, 1)
   __syncthreads();
   if (ctl->abort) {  // copies in flight land before the block exits
     if (TMA && tid == kKeyWarp * 32)
-      for (uint32_t e = keys_copied - min(keys_copied, (uint32_t)p.key_stages); e < keys_copied; ++e)
-        mbar_wait(&ctl->key_full[e % p.key_stages], e / p.key_stages & 1u, a.status);
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t n = h ? keys_copied1 : keys_copied;
+        for (uint32_t e = n - min(n, (uint32_t)p.key_stages); e < n; ++e)
+          mbar_wait(&ctl->key_full[key_stage(h, e)], e / p.key_stages & 1u, a.status);
+      }
     if (tid == kQWarp * 32)
       for (uint32_t e = q_copied - min(q_copied, (uint32_t)p.q_stages); e < q_copied; ++e)
         mbar_wait(&ctl->q_full[e % p.q_stages], e / p.q_stages & 1u, a.status);
@@ -958,11 +967,12 @@ cudaError_t launch_kv_scores(const ScoresLaunch& l, cudaStream_t stream) {
   p.q_bytes = p.nq * p.row_bytes * p.slices * (q8 ? p.terms : 1);
   constexpr int kControl = kTables + sizeof(Ctl) + 1024;
   constexpr int kRoom = 220 * 1024 - kControl;
-  // Items of many Q tiles want them ahead, items of few the next items' keys.
+  // Items of many Q tiles want them ahead, items of few the next items' keys. (At least
+  // one stage a half: two tiles of head_dim 256 and two Q tiles are 192 KB.)
   p.q_stages = rows > 4 * p.nq ? std::min(kMaxQ, (kRoom - 2 * p.key_bytes) / p.q_bytes)
-                               : kRoom - 3 * p.q_bytes < 3 * p.key_bytes ? 2 : 3;
-  p.key_stages = std::min(kMaxKeys, (kRoom - p.q_stages * p.q_bytes) / p.key_bytes);
-  const size_t smem = (size_t)p.key_stages * p.key_bytes + p.q_stages * p.q_bytes + kControl;
+                               : kRoom - 3 * p.q_bytes < 4 * p.key_bytes ? 2 : 3;
+  p.key_stages = std::min(kMaxKeys, (kRoom - p.q_stages * p.q_bytes) / p.key_bytes) / 2;
+  const size_t smem = 2 * (size_t)p.key_stages * p.key_bytes + p.q_stages * p.q_bytes + kControl;
   const long long sms = device_sm_count();
   const void* q = a.q;
   long long head_stride = a.q_head_stride, token_stride = a.q_token_stride, q_rows = a.q_tokens;

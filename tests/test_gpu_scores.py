@@ -282,3 +282,12 @@ def test_no_new_tokens(cuda_device):
     before = s.clone()
     ops.kv_cache_scores(q[:0], cache, table, kv, torch.zeros_like(starts), 1, c.lse[:0], s)
     assert torch.equal(torch.nan_to_num(s, 3.0), torch.nan_to_num(before, 3.0))
+
+
+@pytest.mark.parametrize("store", [BF16, E4M3])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("page", [1, 16])
+def test_many_items_a_block(cuda_device, store, dim, page):
+    """Several items an SM, some of a single half: the halves' rings of keys come round."""
+    kv = [700 - 29 * (i % 7) for i in range(25)]
+    Case(dim + page, [5 - i % 3 for i in range(25)], kv, 8, 8, dim, page, BF16, store).all()
