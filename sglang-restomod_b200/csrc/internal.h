@@ -412,7 +412,9 @@ struct ScoresLaunch {
 };
 long long kv_scores_scratch_bytes(int head_dim, long long q_tokens, int q_heads);
 cudaError_t launch_kv_scores(const ScoresLaunch& l, cudaStream_t stream);
-// up to 16 rows (new tokens x query heads of a key/value head) a sequence
+// up to kv_scores_stream_rows() rows (new tokens x query heads of a key/value head) a
+// sequence
+int kv_scores_stream_rows(const ScoresLaunch& l);
 cudaError_t launch_kv_scores_stream(const ScoresLaunch& l, cudaStream_t stream);
 
 // Held, one per device, while a call that uses a workspace puts its launches on a

@@ -14,7 +14,7 @@
 // and one writer for each score, so results do not depend on timing. What a lane
 // holds past the last token stays in that lane and is dropped.
 //
-// For more than 16 rows a sequence (kv_scores_stream.cu takes fewer).
+// For more than 16 or 32 rows a sequence (kv_scores_stream.cu takes fewer).
 //
 // Bound: the exponentials, one per (row, key) at 16 a clock and SM, which take twice
 // as long as the products at head_dim 128. (A polynomial on the fma pipe for one to four
@@ -936,7 +936,7 @@ long long kv_scores_scratch_bytes(int head_dim, long long q_tokens, int q_heads)
 }
 
 cudaError_t launch_kv_scores(const ScoresLaunch& l, cudaStream_t stream) {
-  if ((long long)l.a.max_q * (l.a.q_heads / l.a.c.heads) <= 16)
+  if ((long long)l.a.max_q * (l.a.q_heads / l.a.c.heads) <= kv_scores_stream_rows(l))
     return launch_kv_scores_stream(l, stream);
   ScoreParams p{};
   p.a = l.a;

@@ -5,8 +5,8 @@
 //   score[t] = (t is new ? 0 : score[t]) + sum over rows r that see t of
 //              e^(scale * q_r . k_t - lse_r)
 //
-// rows: new tokens x query heads that share the key/value head, up to 16 (kv_scores.cu
-// takes more).
+// rows: new tokens x query heads that share the key/value head, up to 16 or 32
+// (kv_scores_stream_rows(); kv_scores.cu takes more).
 //
 // Bound: HBM, each key once; 2 * rows operations an element are far below the
 // tensor rate. A warp takes 16 tokens in M of m16n8k16 and 8 rows in N. The order of
@@ -55,6 +55,11 @@ struct RowParams {
 template <int D, int KV>
 struct Shape {
   static constexpr int kElem = KV == kE4m3 ? 1 : 2;
+  // Rows whose queries fit the registers, and up to which this kernel is ahead: against
+  // the other one, 16 sequences of up to 4096 tokens, 8 heads, 32 rows each, pages of 64
+  // and of one, head_dim 64 bf16 17 / 35 and 18 / 42 us, e4m3 20 / 39 and 21 / 41, 128
+  // bf16 31 / 36 and 34 / 57; but e4m3 44 / 40 and 46 / 49 (24 rows 43 / 34).
+  static constexpr int kMostRows = D == 64 || (D == 128 && KV != kE4m3) ? 32 : 16;
   static constexpr int kPieces = D * kElem / 64;       // of 16 bytes, a lane's of a token
   static constexpr int kRegs = 8 * kPieces;            // of 16 tokens
   // of 16 tokens, a tile: a lane of a quarter has one token of a tile as its own
@@ -195,7 +200,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D, KV>::kBlocks)
     uint32_t qf[kSteps][NR][2];
     float factor[NR][2], nl[NR][2];
     int row_token[NR][2];  // -1: no such row
-    int all_lo = 0, all_hi = 0x7fffffff;  // tokens that all eight (or 16) columns see
+    int all_lo = 0, all_hi = 0x7fffffff;  // tokens that all columns see
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr) {
       const int r = 8 * nr + g;
@@ -437,14 +442,18 @@ cudaError_t launch(const RowParams& p, int rows, cudaStream_t stream) {
   cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return err;
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  constexpr int kMost = S::kMostRows / 8;
   if (!configured[dev]) {
-    for (auto kernel : {kv_scores_stream_kernel<D, KV, 1>, kv_scores_stream_kernel<D, KV, 2>}) {
+    for (auto kernel : {kv_scores_stream_kernel<D, KV, 1>, kv_scores_stream_kernel<D, KV, 2>,
+                        kv_scores_stream_kernel<D, KV, kMost>}) {
       err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::kSmem);
       if (err != cudaSuccess) return err;
     }
     configured[dev] = true;
   }
-  return launch_pdl(rows <= 8 ? kv_scores_stream_kernel<D, KV, 1> : kv_scores_stream_kernel<D, KV, 2>,
+  return launch_pdl(rows <= 8    ? kv_scores_stream_kernel<D, KV, 1>
+                    : rows <= 16 ? kv_scores_stream_kernel<D, KV, 2>
+                                 : kv_scores_stream_kernel<D, KV, kMost>,
                     dim3((unsigned)(S::kBlocks * device_sm_count())), dim3(kThreads), S::kSmem, stream,
                     p);
 }
@@ -456,6 +465,15 @@ cudaError_t launch_type(const RowParams& p, int rows, cudaStream_t stream) {
 }
 
 }  // namespace
+
+int kv_scores_stream_rows(const ScoresLaunch& l) {
+  const bool e4m3 = l.a.cache_dtype == 3;
+  switch (l.a.c.head_dim) {
+    case 64: return e4m3 ? Shape<64, kE4m3>::kMostRows : Shape<64, kBf16>::kMostRows;
+    case 128: return e4m3 ? Shape<128, kE4m3>::kMostRows : Shape<128, kBf16>::kMostRows;
+    default: return Shape<256, kBf16>::kMostRows;
+  }
+}
 
 cudaError_t launch_kv_scores_stream(const ScoresLaunch& l, cudaStream_t stream) {
   RowParams p{};

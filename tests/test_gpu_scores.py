@@ -291,3 +291,13 @@ def test_many_items_a_block(cuda_device, store, dim, page):
     """Several items an SM, some of a single half: the halves' rings of keys come round."""
     kv = [700 - 29 * (i % 7) for i in range(25)]
     Case(dim + page, [5 - i % 3 for i in range(25)], kv, 8, 8, dim, page, BF16, store).all()
+
+
+@pytest.mark.parametrize("q_dtype,store", [(BF16, BF16), (F16, F16), (BF16, E4M3), (F16, E4M3)])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("q_len,groups,window", [(4, 8, 0), (7, 3, 0), (17, 1, 9), (2, 16, 100), (32, 1, 0)])
+def test_a_few_tokens(cuda_device, q_dtype, store, dim, q_len, groups, window):
+    """17 to 32 rows: the most that the streaming kernel takes, and one more than half of it."""
+    kv = [q_len + n for n in (0, 1, 30, 205, 999)]
+    q_lens = [q_len, q_len, 1, q_len, q_len - 1]
+    Case(dim + q_len, q_lens, kv, 2, groups, dim, 16, q_dtype, store, window=window).all()
