@@ -454,8 +454,7 @@ int b200_w8a8_moe_gemm(const void* a, int32_t a_dtype, int64_t a_rows, int64_t k
 
 /*
  * Linear with 8-bit integer weights and activations (no counterpart in the
- * reference; upstream SGLang's w8a8_int8 arithmetic): x [m, k] is quantized per
- * token,
+ * reference): x [m, k] is quantized per token,
  *   s[t] = max_k |x[t, k]| / 127,  q[t, k] = rint(x[t, k] / s[t])  (0 where s is 0),
  *   y[t, n] = (sum_k q[t, k] * w[n, k]) * s[t] * w_scales[n],
  * the sum exact in int32, the rest fp32. A token with an infinity or NaN has a
