@@ -15,7 +15,6 @@ by both scales. The quantized cache is that of ``operators.py``: e4m3 codes, and
 byte 127 + e per vector for the power of two they are multiplied by.
 """
 
-import functools
 import math
 import random
 import sys
@@ -28,7 +27,6 @@ own = False
 DTYPES = {"bf16": torch.bfloat16, "f16": torch.float16}
 
 
-@functools.cache  # a program imports it once
 def _library():
     root = str(Path(__file__).resolve().parents[1] / "sglang-restomod_b200")
     if root not in sys.path:
