@@ -58,9 +58,6 @@ namespace {
 using namespace tcg;
 
 constexpr float kLog2e = 1.4426950408889634f;
-// A hidden column is an infinity that factors multiply, so a factor of zero becomes the
-// smallest normal number: finite products still come to e^0.
-constexpr float kMinScale = 1.1754944e-38f;
 constexpr int kEpiWarps = 16, kQWarp = 16, kMmaWarp = 17, kKeyWarp = 19;
 // The tokens' warps of a half: one, or where these copy the keys too four, a quarter of
 // the half's tokens each.
@@ -296,11 +293,13 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
 }
 // The sum of a lane's weights over N columns: e^x in log2, x = s * factor + nl.
 // s: fp32 products (e4m3: the coarse sum, `fine` the one in units of 1 / kFine,
-// `key` the key's scale). (One fp32 operation at a time: in pairs, the moves that join
+// `key` the key's scale). MASKED: the columns outside [lo, hi) add nothing, which is decided
+// when x is complete: they may be rows of another sequence, whose products, factors and
+// log-sums may be anything. (One fp32 operation at a time: in pairs, the moves that join
 // and part them made it 8 instructions a column.)
-template <bool Q8, int N>
+template <bool Q8, bool MASKED, int N>
 __device__ __forceinline__ float weigh(const uint32_t (&s)[N], const uint32_t* fine, float scale, float key,
-                                       const float* nl, const float* factor) {
+                                       const float* nl, const float* factor, int lo, int hi) {
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < N; i += 4) {
@@ -316,16 +315,11 @@ __device__ __forceinline__ float weigh(const uint32_t (&s)[N], const uint32_t* f
       float x = __uint_as_float(s[i + j]);
       if (Q8) x = fmaf(__uint_as_float(fine[i + j]), 1.f / kFine, x) * key;
       x = fmaf(x, f[j], n[j]);
+      if (MASKED) x = i + j >= lo && i + j < hi ? x : -INFINITY;
       sum[j] += ex2(x);
     }
   }
   return (sum[0] + sum[1]) + (sum[2] + sum[3]);
-}
-// Columns outside [lo, hi) become `hidden`, an infinity that the factor makes -inf.
-template <int N>
-__device__ __forceinline__ void hide(uint32_t (&s)[N], int lo, int hi, float hidden) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) s[i] = i >= lo && i < hi ? s[i] : __float_as_uint(hidden);
 }
 // Loads of tensor memory, and the wait for all of them (which ties r's uses to it).
 __device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&r)[32]) {
@@ -479,7 +473,6 @@ __global__ void __launch_bounds__(Roles<TMA>::kThreads, 1)
     };
     Tile have, coming;
     float lse_next[2], factor_next = 0.f;
-    const float plus = p.scale_log2 >= 0.f ? 1.f : -1.f;
     auto load_rows = [&](const Tile& t, const Item& of) {
       coming = t;
       const int tok0 = t.q * p.tile_tokens;
@@ -489,8 +482,7 @@ __global__ void __launch_bounds__(Roles<TMA>::kThreads, 1)
         lse_next[k] = -INFINITY;
         if (row_token[k] < of.q_len - tok0) lse_next[k] = __ldg(a.lse + at + row_at[k]);
       }
-      // (of the scale's sign where there is no row: hidden columns come to -inf)
-      if (Q8) factor_next = row_token[0] < of.q_len - tok0 ? __ldg(p.q_scale + at + row_at[0]) : plus;
+      if (Q8) factor_next = row_token[0] < of.q_len - tok0 ? __ldg(p.q_scale + at + row_at[0]) : 0.f;
     };
     auto publish_rows = [&]() {
       have = coming;
@@ -501,7 +493,6 @@ __global__ void __launch_bounds__(Roles<TMA>::kThreads, 1)
       if (Q8) mine[64 + lane] = factor_next;
       __syncwarp();
     };
-    const float hidden = plus * -INFINITY;
     uint32_t count = 0, tokens = 0;      // S tiles and items so far
     bool ok = true;
     while (ok && items.next(it, lane)) {
@@ -517,9 +508,7 @@ __global__ void __launch_bounds__(Roles<TMA>::kThreads, 1)
       float sum = 0.f, key_scale = 1.f;
       if (Q8 && it.first < it.last) {
         ok = wait_warp(&ctl->token_full[slot], tokens / kTokens & 1u, ctl);
-        // (zero would make a hidden column NaN: the smallest number instead)
         key_scale = token_sh[slot * 128 + row].key_scale;
-        key_scale = key_scale == 0.f ? kMinScale : key_scale;
       }
 #pragma unroll 1
       for (int q = it.first; q < it.last && ok; ++q, ++count) {
@@ -561,9 +550,11 @@ __global__ void __launch_bounds__(Roles<TMA>::kThreads, 1)
           tie(s);
           if (Q8) tie(fine);
           if (c0 % 32 + kCols == 32 && c0 + 64 >= p.nq) release();
-          if (masked) hide(s, lo - c0, hi - c0, hidden);
           const int at = c0 / 64 * 32 + c0 % 32;
-          part += weigh<Q8>(s, fine, p.scale_log2, key_scale, mine + at, mine + 64 + at);
+          part += masked ? weigh<Q8, true>(s, fine, p.scale_log2, key_scale, mine + at, mine + 64 + at,
+                                           lo - c0, hi - c0)
+                         : weigh<Q8, false>(s, fine, p.scale_log2, key_scale, mine + at,
+                                            mine + 64 + at, 0, 0);
         }
         if (32 * odd >= p.nq) release();  // (no column of the tile)
         sum += part;
@@ -948,7 +939,7 @@ cudaError_t launch_kv_scores(const ScoresLaunch& l, cudaStream_t stream) {
   p.in_page = l.in_page, p.in_token = l.in_token, p.in_head = l.in_head;
   p.out_page = l.out_page, p.out_token = l.out_token, p.out_head = l.out_head;
   p.groups = a.q_heads / a.c.heads;
-  p.scale_log2 = a.scale == 0.f ? kMinScale : a.scale * kLog2e;
+  p.scale_log2 = a.scale * kLog2e;
   p.f16 = a.cache_dtype == 1;
   p.terms = a.q_f16 ? 3 : 2;
   p.row_bytes = q8 && d == 64 ? 64 : 128;
