@@ -641,7 +641,8 @@ int b200_kv_cache_scores(const b200_kv_cache* cache, const void* q, int32_t dtyp
  * - 1 of the sequence; keys, values, scales and scores move, bit for bit. Scores:
  * fp32 of (page, offset, head) at the score strides.
  * kept [seqs][kv_heads][budget]: their indices before, -1 past the sequence's
- * end; lens [seqs] = min(kv_lens, budget).
+ * end; lens [seqs] = min(kv_lens, budget). Neither shares memory with the other, kv_lens
+ * or a table.
  * out_table NULL (or page_table): in place, in the sequence's first pages; the
  * slots after token lens[s] - 1 keep what they hold. No page may stand twice among
  * the pages of the call's tokens then. Otherwise the kept tokens, of sequences within the budget

@@ -32,6 +32,16 @@ int check_scores(const KvCacheView& c, const float* scores, int64_t page_stride,
   return B200_OK;
 }
 
+// Whether two arrays of int32 share memory.
+struct Ints {
+  const void* at;
+  int64_t count;
+};
+bool overlap(const Ints& a, const Ints& b) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(b.at);
+  return a.count > 0 && b.count > 0 && (x < y ? (y - x) / 4 < (uintptr_t)a.count : (x - y) / 4 < (uintptr_t)b.count);
+}
+
 }  // namespace
 
 extern "C" {
@@ -158,6 +168,16 @@ int b200_kv_cache_evict(const b200_kv_cache* cache, float* scores, int64_t score
       (int64_t)out_table_width * cache->page_size < (budget < most ? budget : most))
     return fail(B200_ERR_INVALID, "out_table's %d pages of %d do not hold the budget of %d tokens",
                 out_table_width, cache->page_size, budget);
+  // Blocks read the lengths and the tables at different times: none may find a result there.
+  const Ints kept_ids{kept, (int64_t)seqs * cache->kv_heads * budget}, new_lens{lens, seqs};
+  const Ints inputs[3] = {
+      {kv_lens, seqs},
+      {page_table, page_table_width > 0 ? (seqs - 1) * page_table_stride + page_table_width : 0},
+      {out_table, out_table && out_table_width > 0 ? (seqs - 1) * out_table_stride + out_table_width : 0}};
+  bool shared = overlap(kept_ids, new_lens);
+  for (const Ints& in : inputs) shared = shared || overlap(kept_ids, in) || overlap(new_lens, in);
+  if (shared)
+    return fail(B200_ERR_INVALID, "kept and lens need memory of their own, apart from kv_lens and the tables");
   l.scores = scores;
   l.score_page_stride = score_page_stride;
   l.score_token_stride = score_token_stride;
