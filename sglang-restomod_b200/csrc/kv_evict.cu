@@ -136,7 +136,9 @@ __global__ void __launch_bounds__(kThreads, 2) evict_choose_kernel(const EvictPa
   const int n = p.tokens_of(seq), keep = min(n, e.budget);
   int* kept = e.kept + (long long)pair * e.budget;
   if (head == 0 && rank == 0 && tid == 0) e.lens[seq] = keep;
-  for (int j = keep + rank * kThreads + tid; j < e.budget; j += blocks * kThreads) kept[j] = -1;
+  // (a budget may be any int: the last step goes past it)
+  for (long long j = (long long)keep + rank * kThreads + tid; j < e.budget; j += blocks * kThreads)
+    kept[j] = -1;
   if (n <= e.budget) {
     for (int j = rank * kThreads + tid; j < n; j += blocks * kThreads) kept[j] = j;
     return;
