@@ -643,7 +643,7 @@ int b200_kv_cache_scores(const b200_kv_cache* cache, const void* q, int32_t dtyp
  * kept [seqs][kv_heads][budget]: their indices before, -1 past the sequence's
  * end; lens [seqs] = min(kv_lens, budget). Neither shares memory with the other, kv_lens
  * or a table.
- * out_table NULL (or page_table): in place, in the sequence's first pages; the
+ * out_table NULL (or page_table, with its stride): in place, in the sequence's first pages; the
  * slots after token lens[s] - 1 keep what they hold. No page may stand twice among
  * the pages of the call's tokens then. Otherwise the kept tokens, of sequences within the budget
  * too, are copied to the pages out_table[s * out_table_stride ..]

@@ -163,7 +163,12 @@ int b200_kv_cache_evict(const b200_kv_cache* cache, float* scores, int64_t score
   if (std::min<int64_t>(budget, most) > 65535 * 64)
     return fail(B200_ERR_UNSUPPORTED, "at most %d tokens stay, got a budget of %d of %lld", 65535 * 64,
                 budget, (long long)most);
-  if (out_table == page_table && out_table_stride == page_table_stride) out_table = nullptr;
+  if (out_table == page_table) {  // in place (one row has no stride)
+    if (out_table_stride != page_table_stride && seqs > 1)
+      return fail(B200_ERR_INVALID, "in place out_table needs page_table's stride, got %lld for %lld",
+                  (long long)out_table_stride, (long long)page_table_stride);
+    out_table = nullptr;
+  }
   if (out_table != nullptr &&
       (int64_t)out_table_width * cache->page_size < (budget < most ? budget : most))
     return fail(B200_ERR_INVALID, "out_table's %d pages of %d do not hold the budget of %d tokens",

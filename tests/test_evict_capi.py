@@ -38,3 +38,9 @@ def evict(cache=None, **kw):
 def test_results_with_memory_of_an_input(kw):
     kw = {name: v and at(v) for name, v in kw.items()}
     assert "memory of their own" in err(evict(**kw), _lib.ERR_INVALID)
+
+
+def test_the_same_table_with_another_stride():
+    """In place or not: rows after the first would be other pages."""
+    assert "page_table's stride" in err(evict(out_table=at(1 << 16), out_stride=3, out_width=3),
+                                        _lib.ERR_INVALID)

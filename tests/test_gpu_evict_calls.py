@@ -24,3 +24,16 @@ def test_largest_budgets(cuda_device, budget):
     for got, was in zip(c.dev, c.data):
         assert torch.equal(got.cpu(), was)
     assert ops.attention_status() == 0
+
+
+@pytest.mark.parametrize("lens", [[700], [700, 90, 333]])
+def test_out_table_is_the_page_table(cuda_device, lens):
+    """In place, also where one row's view has another stride."""
+    c = Case(2, lens, 100, 9, 3, 2, 64, 16, BF16)
+    table = c.table.cuda()
+    out = table[0, :12][None] if len(lens) == 1 else table
+    assert (out.stride(0) != table.stride(0)) == (len(lens) == 1)
+    kept, new = ops.kv_cache_evict(c.cache, c.scores, table,
+                                   torch.tensor(lens, dtype=torch.int32, device="cuda"), 100, recent=9,
+                                   first=3, out_table=out)
+    c.check(True, kept, new)
