@@ -638,7 +638,8 @@ int b200_kv_cache_scores(const b200_kv_cache* cache, const void* q, int32_t dtyp
  * last `recent`, and of those between the budget - first - recent with the largest
  * scores (ties: the lowest index; NaN counts as the lowest score, -0 as 0). Heads
  * choose by themselves. The kept tokens stay in order and become tokens 0 .. budget
- * - 1 of the sequence; keys, values, scales and scores move, bit for bit. Scores:
+ * - 1 of the sequence; keys, values, scales and scores move, bit for bit; keys and
+ * values are not the same memory. Scores:
  * fp32 of (page, offset, head) at the score strides.
  * kept [seqs][kv_heads][budget]: their indices before, -1 past the sequence's
  * end; lens [seqs] = min(kv_lens, budget). Neither shares memory with the other, kv_lens

@@ -149,6 +149,8 @@ int b200_kv_cache_evict(const b200_kv_cache* cache, float* scores, int64_t score
        !apart3(l.c.scale_page_stride, l.c.num_pages, l.c.scale_token_stride, l.c.page_size,
                l.c.scale_head_stride, l.c.heads, 1)))
     return fail(B200_ERR_INVALID, "the cache's vectors overlap");
+  // (they move independently of one another)
+  if (l.c.k == l.c.v) return fail(B200_ERR_INVALID, "keys and values are the same memory");
   if (kv_lens == nullptr || kept == nullptr || lens == nullptr ||
       (page_table_width > 0 && page_table == nullptr))
     return fail(B200_ERR_INVALID, "null pointer argument");

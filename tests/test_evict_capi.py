@@ -44,3 +44,9 @@ def test_the_same_table_with_another_stride():
     """In place or not: rows after the first would be other pages."""
     assert "page_table's stride" in err(evict(out_table=at(1 << 16), out_stride=3, out_width=3),
                                         _lib.ERR_INVALID)
+
+
+def test_keys_that_are_the_values():
+    """Each moves without waiting for the other."""
+    for out_table in (None, at(3 << 16)):
+        assert "same memory" in err(evict(desc(v=4096), out_table=out_table), _lib.ERR_INVALID)
