@@ -84,6 +84,8 @@ int b200_int8_linear_quantized(const int8_t* q, const float* scales, int64_t m, 
   l.out = y;
   l.out_f16 = y_dtype == B200_DTYPE_F16;
   if ((rc = device_status_word(&l.status))) return rc;
+  // (a kernel's first launch on a device configures it, which is not for two threads at once)
+  const std::lock_guard<std::mutex> alone(launch_mutex());
   return check_cuda(launch_int8_gemm(l, reinterpret_cast<cudaStream_t>(stream)), "int8 GEMM launch");
 }
 
