@@ -608,17 +608,18 @@ int b200_shared_prefix_attention(
  *                + sum over the new tokens and the query heads that share the head,
  *                  of those that see t, of e^(scale * q . k_t - lse)
  * (not causal: the queries' tokens are not among the cached ones, none starts from 0)
- * with lse [q_tokens, q_heads] from the attention call (a row of -inf adds nothing),
- * and everything else as in b200_paged_attention, whose masks these are; of new
- * tokens past max_q_len none adds to the sums. lse may also be that of
- * b200_shared_prefix_attention. Scores are fp32 of (page, offset, head), at strides of
- * their own; scores_out may be scores, or has no memory in common with them. Each
- * score has one writer, in a fixed order: two calls give the same bits. No page may
- * stand twice among the pages of the call's tokens. At most 64 query heads per key/value head; q's vectors apart in memory. Products are
- * exact to fp32's sums (e4m3 keys: queries to 2^-22 of their largest element);
- * a key scale byte may be any. Infinite or NaN queries or keys give NaN scores where
- * they are seen. Page numbers outside the cache set status bit 16. Workspace as
- * for b200_paged_attention, and it may be the same one.
+ * with lse [q_tokens, q_heads] from the attention call (a row of -inf adds nothing, if
+ * its query is finite), and everything else as in b200_paged_attention, whose masks
+ * these are; of new tokens past max_q_len none adds to the sums. lse may also be that
+ * of b200_shared_prefix_attention. Scores are fp32 of (page, offset, head), at strides
+ * of their own; scores_out may be scores, or has no memory in common with them (such a
+ * call needs new tokens). Each score has one writer, in a fixed order: two calls give
+ * the same bits. No page may stand twice among the pages of the call's tokens. At most
+ * 64 query heads per key/value head; q's vectors apart in memory. Products are exact to
+ * fp32's sums (e4m3 keys: queries to 2^-22 of their largest element); a key scale byte
+ * may be any. Infinite or NaN queries, log-sums or keys give NaN scores where they are
+ * seen, and nowhere else. Page numbers outside the cache set status bit 16. Workspace
+ * as for b200_paged_attention, and it may be the same one.
  */
 int64_t b200_kv_cache_scores_workspace_bytes(int32_t head_dim, int64_t q_tokens, int32_t q_heads);
 int b200_kv_cache_scores(const b200_kv_cache* cache, const void* q, int32_t dtype, int64_t q_tokens,
@@ -639,8 +640,8 @@ int b200_kv_cache_scores(const b200_kv_cache* cache, const void* q, int32_t dtyp
  * scores (ties: the lowest index; NaN counts as the lowest score, -0 as 0). Heads
  * choose by themselves. The kept tokens stay in order and become tokens 0 .. budget
  * - 1 of the sequence; keys, values, scales and scores move, bit for bit; keys and
- * values are not the same memory. Scores:
- * fp32 of (page, offset, head) at the score strides.
+ * values are not the same memory. Scores: fp32 of (page, offset, head) at the score
+ * strides.
  * kept [seqs][kv_heads][budget]: their indices before, -1 past the sequence's
  * end; lens [seqs] = min(kv_lens, budget). Neither shares memory with the other, kv_lens
  * or a table.

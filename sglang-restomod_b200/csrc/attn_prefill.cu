@@ -1712,7 +1712,10 @@ namespace {
 // head_dim 128, by rows of a sequence: 256 (16 x 4096 keys) bf16 55 / 62, e4m3
 // 93 / 115, single-token pages 71 / 73; 512 (4 x 4096) 35 / 38, 45 / 55, 42 /
 // 46; 1024 (16384) 87 / 78, 124 / 104, 95 / 85; 2048 (16384) e4m3 221 / 165;
-// 32768 (a prompt of 8192) bf16 613 / 506.
+// 32768 (a prompt of 8192) bf16 613 / 506. The same for passes over a prefix of 8192,
+// single tokens of 16 to 256 sequences on it, 8 x 8 heads, the whole call: 128 rows
+// bf16 31 / 35, e4m3 36 / 44; 256 39 / 41, 45 / 47; 512 55 / 55, 64 / 63; 768 70 / 68,
+// 82 / 78; 1024 84 / 82, 101 / 94; 2048 147 / 136, 179 / 149.
 bool two_tiles(const PrefillParams& p) {
   const long long rows = p.a.unit_rows ? p.a.unit_rows : (long long)p.a.max_q * p.groups;
   return p.a.c.head_dim != 256 && rows > 512;

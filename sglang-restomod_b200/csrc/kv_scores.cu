@@ -19,9 +19,10 @@
 // Bound: the exponentials, one per (row, key) at 16 a clock and SM, which take twice
 // as long as the products at head_dim 128. (A polynomial on the fma pipe for one to four
 // sixteenths of them: 442, 453, 465, 488 us against 449 for a prompt of 8192 tokens.) Few
-// rows: HBM, each key once. Measured: that prompt, 8 x 4 heads of 128, 449 us (the
+// rows: HBM, each key once. Measured: that prompt, 8 x 4 heads of 128, 447 us (the
 // exponentials alone 240 at 1.9 GHz, the products 165 at the measured bf16 rate); 16 chunks of up to
-// 300 f16 tokens on up to 4096 single-token pages, window 1000, 8 x 3 heads of 64, 66.
+// 300 f16 tokens on up to 4096 single-token pages, window 1000, 8 x 3 heads of 64, 64; the
+// prompt over e4m3 keys 803.
 //
 // e4m3 keys go to the tensor cores as they are (kind::f8f6f4): a query is brought
 // into [128, 256) by a power of two and split into e4m3 terms, q = t1 + (t2 + t3) / 32,

@@ -978,8 +978,10 @@ _PREFIX_BYTES: dict[tuple[int, int, int, int, int], int] = {}
 _SCORES_BYTES: dict[tuple[int, int, int], int] = {}
 # Workspaces that a larger one has replaced, kept because a captured graph may still
 # use them. Each is at most half of the one after it, so a stream's together are
-# below its present one. (Nearly all of a workspace is its partial results, a
-# constant: 20 to 40 MB by head_dim, and 16 bytes a token.)
+# below its present one. (Without shared prefixes nearly all of a workspace is its
+# partial results, a constant: 20 to 40 MB by head_dim, and 16 bytes a token. Shared
+# prefixes add 8 bytes a query element, scores over an e4m3 cache 3: a chunk of 16384
+# tokens with 64 heads of 128 takes 1.1 GB and 0.4 GB, which stay.)
 _ATTN_OUTGROWN: list[torch.Tensor] = []
 _ATTN_MIN_TOKENS, _ATTN_MIN_SEQS = 16384, 4096
 
@@ -1169,7 +1171,10 @@ def shared_prefix_attention(q: torch.Tensor, cache, prefix_table: torch.Tensor,
     ``[groups, pages]``). ``page_table``, ``kv_lens``, ``q_starts`` and ``max_q_len``
     describe each sequence's own tokens, which come after the prefix and begin on a
     page of their own; its new tokens are the last of them. Every new token sees its
-    group's whole prefix and its own tokens causally; the log-sum-exp is over both."""
+    group's whole prefix and its own tokens causally; the log-sum-exp is over both.
+
+    The workspace holds both passes' rows in fp32, 8 bytes a query element, and stays
+    with its stream: with many new tokens, call for a part of the sequences at a time."""
     index = _on_device("shared_prefix_attention", q, cache.k, prefix_table, prefix_lens,
                        group_starts, page_table, kv_lens, q_starts, out, workspace)
     code, tokens, heads, dim, seqs, out = _attention_args(q, cache, page_table, kv_lens, q_starts,
