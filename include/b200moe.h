@@ -617,9 +617,9 @@ int b200_shared_prefix_attention(
  * the same bits. No page may stand twice among the pages of the call's tokens. At most
  * 64 query heads per key/value head; q's vectors apart in memory. Products are exact to
  * fp32's sums (e4m3 keys: queries to 2^-22 of their largest element); a key scale byte
- * may be any. Infinite or NaN queries, log-sums or keys give NaN scores where they are
- * seen, and nowhere else. Page numbers outside the cache set status bit 16. Workspace
- * as for b200_paged_attention, and it may be the same one.
+ * may be any. Infinite or NaN queries or keys and NaN log-sums give NaN scores where
+ * they are seen, and nowhere else. Page numbers outside the cache set status bit 16.
+ * Workspace as for b200_paged_attention, and it may be the same one.
  */
 int64_t b200_kv_cache_scores_workspace_bytes(int32_t head_dim, int64_t q_tokens, int32_t q_heads);
 int b200_kv_cache_scores(const b200_kv_cache* cache, const void* q, int32_t dtype, int64_t q_tokens,
